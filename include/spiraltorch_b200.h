@@ -307,6 +307,13 @@ int st_norm_fwd_f32_rounded(int rms, const float* x, const float* residual, cons
 int st_norm_gelu_bwd(const void* dy, const void* x, const void* gamma, const void* beta, const float* mean, const float* rstd, void* dx, float* dgamma, float* dbeta, int accumulate, float* scratch, int rows, int d, void* stream_v);   /* csrc/norm/norm.cu */
 int st_norm_gelu_fwd(const void* x, const void* gamma, const void* beta, void* y, float* mean, float* rstd, int rows, int d, float eps, void* stream_v);   /* csrc/norm/norm.cu */
 int st_norm_gelu_max_features();   /* csrc/norm/norm.cu */
+int st_paged_attention(const void* q, const void* k_codes, const void* v_codes, const float* k_scale, const float* v_scale, const int* table, const int* starts, const int* lengths, void* out, float* lse, float* workspace, long long q_row, long long q_head, long long o_row, long long o_head, long long table_row, long long pages, long long rows, int width, int page_size, int B, int heads, int kv_heads, int dim, int max_queries, float scale, int causal, int zero_tail, int type, void* stream_v);   /* csrc/serving/paged_attn.cu */
+long long st_paged_attention_workspace(int max_queries, int heads, int kv_heads, int dim);   /* csrc/serving/paged_attn.cu */
+int st_paged_max_sequences();   /* csrc/serving/paged_cache.cu */
+int st_paged_plan(const int* lengths, const int* added, int* table, long long table_row, int width, const int* free_list, const int* free_count, int free_size, int page_size, int B, long long rows, int* starts, int* positions, long long* slots, int* lengths_after, int* free_after, void* stream_v);   /* csrc/serving/paged_cache.cu */
+int st_paged_read(const void* k_codes, const void* v_codes, const float* k_scale, const float* v_scale, const int* table, const int* lengths, long long table_row, int width, int B, int room, int kv_heads, int dim, int page_size, long long pages, void* k_out, void* v_out, int wide_out, void* stream_v);   /* csrc/serving/paged_cache.cu */
+int st_paged_release(int* lengths, const void* done, int* table, long long table_row, int width, int* free_list, int* free_count, int free_size, int page_size, int B, void* stream_v);   /* csrc/serving/paged_cache.cu */
+int st_paged_store(const void* k, const void* v, void* k_codes, void* v_codes, float* k_scale, float* v_scale, const long long* slots, long long rows, int kv_heads, int dim, int page_size, long long pages, long long k_row, long long k_head, long long v_row, long long v_head, int type, void* stream_v);   /* csrc/serving/paged_cache.cu */
 int st_poincare_project(const float* x, float* y, int rows, int cols, float curvature, void* stream_v);   /* csrc/optim/optim.cu */
 int st_preprocess(const float* in, float* out, const StPreprocessArgs* a, void* stream_v);   /* csrc/vision/vision.cu */
 int st_preprocess_own_means(const float* in, float* out, const StPreprocessArgs* a, float* workspace, void* stream_v);   /* csrc/vision/vision.cu */
@@ -319,6 +326,7 @@ int st_reduce_partials(const float* partial, float* out, int parts, int n, int a
 int st_rnn_scan(const StRnnScanArgs* a, void* stream_v);   /* csrc/recurrent/scan.cu */
 int st_rnn_scan_supported(int H, int cell);   /* csrc/recurrent/scan.cu */
 int st_rope(void* x, const float* cos_t, const float* sin_t, long long T, int heads, int D, long long ld, int seq_len, int pos_offset, int backward, void* stream_v);   /* csrc/elementwise/elementwise.cu */
+int st_rotary(const void* q, const void* k, void* qo, void* ko, const void* positions, int pos64, const double* freq, long long tokens, int heads, int kv_heads, int dim, int half, long long q_row, long long q_head, long long k_row, long long k_head, long long qo_row, long long qo_head, long long ko_row, long long ko_head, int interleaved, float magnitude, int backward, int type, void* stream_v);   /* csrc/serving/rotary.cu */
 int st_row_normalize(const void* z, float* y, float* norm, int rows, int d, void* stream_v);   /* csrc/elementwise/embed.cu */
 int st_row_normalize_bwd(const float* g, const float* y, const float* norm, void* dz, int rows, int d, void* stream_v);   /* csrc/elementwise/embed.cu */
 int st_row_softmax_f32(const float* x, float* y, float* hard, int rows, int cols, void* stream_v);   /* csrc/elementwise/elementwise.cu */

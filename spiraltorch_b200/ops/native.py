@@ -6,6 +6,7 @@ be built, every CUDA op raises instead of silently running a PyTorch fallback.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -189,6 +190,14 @@ def address(t: Optional[torch.Tensor]) -> int:
 def raw_stream(index: int) -> int:
     """Handle of the current stream of device ``index``."""
     return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def on_device(index: int):
+    """Context in which device ``index`` is the current one, as a launch needs that; it costs nothing where it is already."""
+    return _HERE if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def deterministic_reduction() -> bool:
