@@ -38,6 +38,7 @@ from ..ops import gemm as gemm_ops
 from ..ops import loss as loss_ops
 from ..ops import native
 from ..ops import norm as norm_ops
+from ..ops import rotary as rotary_ops
 from ..parallel.tp import TPContext
 
 
@@ -55,6 +56,10 @@ class GPTConfig:
     norm: str = "rms"            # "rms" | "layer"
     positional: str = "rope"     # "rope" | "learned"
     bias: bool = False
+    # rotary positions other than the whole head in halves at base frequencies
+    rope_dim: Optional[int] = None           # rotated elements of a head
+    rope_interleaved: bool = False
+    rope_scaling: Optional[rotary_ops.Scaling] = None
 
     @property
     def head_dim(self) -> int:
@@ -167,6 +172,11 @@ class GPTModel(nn.Module):
             self.register_parameter(name.replace(".", "_"), p)
         self.p = params
         self.last_loss: Optional[torch.Tensor] = None
+        self._rope_plain = cfg.rope_dim is None and not cfg.rope_interleaved and cfg.rope_scaling is None
+        self.rope_freq = None if cfg.positional != "rope" else rotary_ops.frequencies(
+            cfg.head_dim if cfg.rope_dim is None else cfg.rope_dim, cfg.rope_base, cfg.rope_scaling, self.flat_w.device)
+        if self.rope_freq is not None and 2 * self.rope_freq.numel() > cfg.head_dim:
+            raise ValueError(f"rope_dim {cfg.rope_dim} is larger than head_dim {cfg.head_dim}")
 
     # ------------------------------------------------------------------------------------------
     def named_flat_views(self):
@@ -190,6 +200,16 @@ class GPTModel(nn.Module):
         return norm_ops.norm_backward(dy, x, self.p[name + ".gamma"], mean, rstd, rms,
                                       self.p[name + ".gamma"].main_grad, beta_g, True, dres, out=out)
 
+    def _rotate_(self, qkv, B: int, S: int, backward: bool = False) -> None:
+        """Rotary positions of the queries and keys of ``[B * S, 3 * heads * D]`` training rows, in place."""
+        hl, D = self.heads_local, self.cfg.head_dim
+        if self._rope_plain:
+            ew.rope_(qkv, 2 * hl, D, S, self.cfg.rope_base, backward=backward)
+            return
+        qk = qkv.view(B * S, 3, hl, D)
+        pos = torch.arange(S, dtype=torch.int32, device=qkv.device).repeat(B)
+        rotary_ops.rotary_(qk[:, 0], qk[:, 1], pos, self.rope_freq, interleaved=self.cfg.rope_interleaved, backward=backward)
+
     # ------------------------------------------------------------------------------------------
     def _layer_forward(self, l: int, resid, x, B: int, S: int, keep: bool):
         cfg, tp, hl, D = self.cfg, self.tp, self.heads_local, self.cfg.head_dim
@@ -202,7 +222,7 @@ class GPTModel(nn.Module):
             y1, h1, m1, r1 = self._norm_fwd(x, f"h{l}.norm1", residual=resid, gather_key=(l, "y1"))
         qkv, y1_full = tp.ag_gemm(y1, P[f"h{l}.qkv.weight"], key=(l, "y1"))
         if cfg.positional == "rope":
-            ew.rope_(qkv, 2 * hl, D, S, cfg.rope_base)
+            self._rotate_(qkv, B, S)
         qkv5 = qkv.view(B, S, 3, hl, D)
         o, lse = attn_ops.attention_forward(qkv5[:, :, 0], qkv5[:, :, 1], qkv5[:, :, 2], True)
         attn_out = tp.gemm_rs(o.view(B * S, hl * D), P[f"h{l}.proj.weight"])
@@ -272,7 +292,7 @@ class GPTModel(nn.Module):
                                     do.view(B, S, hl, D), True, None,
                                     dq=dqkv5[:, :, 0], dk=dqkv5[:, :, 1], dv=dqkv5[:, :, 2])
         if cfg.positional == "rope":
-            ew.rope_(dqkv, 2 * hl, D, S, cfg.rope_base, backward=True)
+            self._rotate_(dqkv, B, S, backward=True)
         self._wgrads([(dqkv, act.y1_full, wqkv.main_grad)])
         dy1 = tp.gemm_rs(dqkv, wqkv, b_mn=True)
         # the result is the next layer's `d_out`, which its first all-gather pushes
@@ -372,6 +392,19 @@ class GPTModel(nn.Module):
                 out, _ = self._forward(tokens, targets, loss_scale, keep=False)
             return out
         return _GPTLossFn.apply(self, tokens, targets, loss_scale, self.p["norm_f.gamma"])
+
+    # ------------------------------------------------------------------------------------------
+    def decoder(self, sequences: int, max_length: int, *, pages: Optional[int] = None, page_size: int = 64):
+        """A :class:`~spiraltorch_b200.models.gpt_decoder.GPTDecoder` of this model: an 8-bit paged cache for ``sequences``
+        sequences of up to ``max_length`` tokens."""
+        from .gpt_decoder import GPTDecoder
+        return GPTDecoder(self, sequences, max_length, pages=pages, page_size=page_size)
+
+    def generate(self, prompts, max_new_tokens: int, *, stop: Optional[int] = None, page_size: int = 64) -> list:
+        """The likeliest continuation of each prompt (a list of token ids), token by token, up to ``max_new_tokens`` or the token ``stop``.
+        Returns the new tokens of each."""
+        longest = max((len(p) for p in prompts), default=0)
+        return self.decoder(len(prompts), longest + max_new_tokens, page_size=page_size).generate(prompts, max_new_tokens, stop=stop)
 
     # ------------------------------------------------------------------------------------------
     def sync_replicated_grads(self) -> None:

@@ -1,0 +1,171 @@
+"""Answering token by token with a :class:`~spiraltorch_b200.models.gpt.GPTModel`: keys and values in an 8-bit paged cache.
+
+Every call is one pass of the model over the new tokens of all sequences, one after another in the rows of one matrix:
+:func:`ops.paged.plan` takes pages and maps the rows, then per layer the fused projection, rotary positions, :func:`ops.paged.store` and
+attention over the cache.  Parts of prompts that are long enough to fill the tiles of dense attention (``DENSE_FROM`` tokens) read the
+cache back instead (:func:`ops.paged.read`) and run ``ops.attention`` over it, so that a prompt sees the same keys and values that later tokens do.
+
+The reference has no counterpart (its language models do not decode with a cache)."""
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import torch
+
+from ..ops import attention as attn_ops
+from ..ops import elementwise as ew
+from ..ops import gemm as gemm_ops
+from ..ops import paged
+from ..ops import rotary as rotary_ops
+
+DENSE_FROM = 64      # new tokens of one sequence
+
+
+class GPTDecoder:
+    """``sequences`` places for sequences of up to ``max_length`` tokens over ``pages`` pages (default: enough for all of them).
+
+    The lengths are kept on the host as well, so that a call that does not fit is refused before anything is launched."""
+
+    def __init__(self, model, sequences: int, max_length: int, *, pages: Optional[int] = None, page_size: int = 64):
+        cfg = model.cfg
+        if model.tp.world != 1:
+            raise ValueError("GPTDecoder: tensor-parallel models are not supported")
+        if sequences < 1 or max_length < 1:
+            raise ValueError(f"GPTDecoder: {sequences} sequences of up to {max_length} tokens")
+        if cfg.positional == "learned" and max_length > cfg.seq_len:
+            raise ValueError(f"GPTDecoder: learned positions end at {cfg.seq_len}, not at {max_length}")
+        self.model, self.sequences, self.max_length, self.page_size = model, sequences, max_length, page_size
+        dev = model.flat_w.device
+        width = -(-max_length // page_size)
+        self.pages = sequences * width if pages is None else pages
+        self.cache = [paged.Pages.allocate(self.pages, cfg.n_heads, page_size, cfg.head_dim, dev) for _ in range(cfg.n_layers)]
+        i32 = dict(dtype=torch.int32, device=dev)
+        self.table = torch.full((sequences, width), -1, **i32)
+        self.free = torch.arange(self.pages, **i32)
+        self.free_count = torch.full((1,), self.pages, **i32)
+        self.lengths = torch.zeros(sequences, **i32)
+        self.held = [0] * sequences
+
+    # ---- host side ------------------------------------------------------------------------------------------------------------
+    def _blocks(self, tokens: int) -> int:
+        return -(-tokens // self.page_size)
+
+    @property
+    def pages_left(self) -> int:
+        return self.pages - sum(self._blocks(n) for n in self.held)
+
+    def _admit(self, added: Sequence[int]) -> None:
+        need = sum(self._blocks(h + n) - self._blocks(h) for h, n in zip(self.held, added))
+        for b, (h, n) in enumerate(zip(self.held, added)):
+            if h + n > self.max_length:
+                raise ValueError(f"GPTDecoder: sequence {b} would have {h + n} tokens, at most {self.max_length}")
+        if need > self.pages_left:
+            raise ValueError(f"GPTDecoder: {need} pages are needed and {self.pages_left} are left")
+        self.held = [h + n for h, n in zip(self.held, added)]
+
+    # ---- device side ----------------------------------------------------------------------------------------------------------
+    def _pass(self, tokens: torch.Tensor, added: torch.Tensor, last: Optional[torch.Tensor], counts: Sequence[int]) -> torch.Tensor:
+        """Logits of the rows ``last`` (None: all) of ``tokens`` ``[rows]``, of which sequence ``b`` has ``counts[b]``."""
+        m, cfg = self.model, self.model.cfg
+        H, D, rows, most = cfg.n_heads, cfg.head_dim, tokens.shape[0], max(counts)
+        step = paged.plan(self.lengths, added, self.table, self.free, self.free_count, page_size=self.page_size, rows=rows)
+        self.lengths.copy_(step.lengths)
+        self.free_count.copy_(step.free_count)
+        resid, x = ew.embedding_forward(tokens, m.p["embed.weight"]), None
+        if cfg.positional == "learned":
+            resid = resid + m.p["pos.weight"][step.positions.long()]
+        for l in range(cfg.n_layers):
+            y, h, _, _ = m._norm_fwd(resid if x is None else x, f"h{l}.norm1", residual=None if x is None else resid)
+            if x is not None:
+                resid = h
+            qkv = gemm_ops.gemm(y, m.p[f"h{l}.qkv.weight"]).view(rows, 3, H, D)
+            q, k, v = qkv[:, 0], qkv[:, 1], qkv[:, 2]
+            if m.rope_freq is not None:
+                rotary_ops.rotary_(q, k, step.positions, m.rope_freq, interleaved=cfg.rope_interleaved)
+            paged.store(k, v, self.cache[l], step.slots)
+            o = self._dense(q, l, counts) if most >= DENSE_FROM else paged.attention(
+                q, self.cache[l], self.table, step.starts, step.lengths, max_queries=most)
+            a = gemm_ops.gemm(o.view(rows, H * D), m.p[f"h{l}.proj.weight"])
+            y, resid, _, _ = m._norm_fwd(a, f"h{l}.norm2", residual=resid)
+            u = gemm_ops.gemm(y, m.p[f"h{l}.fc1.weight"], act="gelu")
+            x = gemm_ops.gemm(u, m.p[f"h{l}.fc2.weight"])
+        if last is not None:
+            x, resid = x.index_select(0, last), resid.index_select(0, last)
+        y, _, _, _ = m._norm_fwd(x, "norm_f", residual=resid)
+        return gemm_ops.gemm(y, m.p["embed.weight"])
+
+    def _dense(self, q: torch.Tensor, l: int, counts: Sequence[int]) -> torch.Tensor:
+        o, r = torch.empty(q.shape, dtype=q.dtype, device=q.device), 0
+        for b, n in enumerate(counts):
+            if n:
+                k, v = paged.read(self.cache[l], self.table[b:b + 1], self.lengths[b:b + 1], self.held[b],
+                                  torch.bfloat16 if q.is_cuda else torch.float32)
+                o[r:r + n] = attn_ops.attention_forward(q[None, r:r + n], k, v, True)[0][0]
+                r += n
+        return o
+
+    @torch.no_grad()
+    def extend(self, tokens: Sequence) -> torch.Tensor:
+        """``tokens``: for every sequence the ids to append (a list or a 1-D host tensor; empty: the sequence waits).  Returns the logits behind the last
+        token of each sequence that got some, ``[such sequences, vocab]``."""
+        if len(tokens) != self.sequences:
+            raise ValueError(f"GPTDecoder: tokens for {len(tokens)} of {self.sequences} sequences")
+        ids = [torch.as_tensor(t, dtype=torch.int64).reshape(-1) for t in tokens]
+        counts = [t.numel() for t in ids]
+        flat = torch.cat(ids)
+        vocab = self.model.cfg.vocab_size
+        if flat.numel() and (int(flat.min()) < 0 or int(flat.max()) >= vocab):
+            raise ValueError(f"GPTDecoder: a token id is outside the vocabulary of {vocab}")
+        if not flat.numel():
+            raise ValueError("GPTDecoder: no tokens")
+        self._admit(counts)
+        dev = self.lengths.device
+        last = torch.tensor([sum(counts[:b + 1]) - 1 for b, n in enumerate(counts) if n])
+        return self._pass(flat.to(dev), torch.tensor(counts, dtype=torch.int32, device=dev), last.to(dev), counts)
+
+    @torch.no_grad()
+    def step(self, tokens: torch.Tensor) -> torch.Tensor:
+        """One token for every sequence: ``tokens`` int64 ``[sequences]`` on the model's device, ids inside the vocabulary (not looked at).
+        Returns the logits behind them.  It looks at nothing on the device, so it can be captured into a CUDA graph; replays do not pass
+        through the host's count, and what they append beyond ``max_length`` or the pages is not stored."""
+        if tokens.shape != (self.sequences,) or tokens.dtype != torch.int64 or tokens.device != self.lengths.device:
+            raise ValueError(f"GPTDecoder: step takes int64 [{self.sequences}] on {self.lengths.device}, got {tokens.dtype} {tuple(tokens.shape)} on {tokens.device}")
+        counts = [1] * self.sequences
+        self._admit(counts)
+        return self._pass(tokens, torch.ones(self.sequences, dtype=torch.int32, device=tokens.device), None, counts)
+
+    def release(self, which: Sequence[int]) -> None:
+        """Ends the sequences of these places and frees their pages; the places can take new ones."""
+        done = [False] * self.sequences
+        for b in which:
+            if not 0 <= b < self.sequences:
+                raise ValueError(f"GPTDecoder: no place {b}")
+            done[b] = True
+        paged.release(self.lengths, torch.tensor(done, device=self.lengths.device), self.table, self.free, self.free_count, page_size=self.page_size)
+        self.held = [0 if d else h for h, d in zip(self.held, done)]
+
+    def generate(self, prompts: Sequence, max_new_tokens: int, *, stop: Optional[int] = None) -> list:
+        """The likeliest continuation of a prompt in every place, up to ``max_new_tokens`` or the token ``stop`` (which is not returned).
+        A place that met ``stop`` waits.  Starts from empty places."""
+        if any(self.held):
+            raise ValueError("GPTDecoder: generate starts from empty places; release them first")
+        if max_new_tokens < 0 or any(len(p) == 0 for p in prompts):
+            raise ValueError("GPTDecoder: prompts need a token at least")
+        out = [[] for _ in prompts]
+        if max_new_tokens == 0:
+            return out
+        active = list(range(self.sequences))
+        logits = self.extend(prompts)
+        while True:
+            best = logits.argmax(-1)
+            going, feed = [], [[] for _ in prompts]
+            for b, t in zip(active, best.tolist()):
+                if t != stop:
+                    out[b].append(t)
+                    if len(out[b]) < max_new_tokens:
+                        going.append(b)
+                        feed[b] = [t]
+            if not going:
+                return out
+            active = going
+            logits = self.step(best) if len(going) == self.sequences else self.extend(feed)

@@ -316,8 +316,8 @@ def attention(q: torch.Tensor, pages: Pages, table: torch.Tensor, starts: torch.
     P, Hk, page, D = _check_pages(pages)
     if q.dim() != 3 or q.shape[2] != D or q.shape[1] < Hk or q.shape[1] % Hk:
         raise ValueError(f"paged.attention: q {tuple(q.shape)} does not fit pages of {Hk} heads of {D}")
-    if q.dtype not in (torch.bfloat16, torch.float16) or q.stride(2) != 1:
-        raise ValueError("paged.attention: q must be bf16 or fp16 with contiguous head elements")
+    if not (q.dtype in (torch.bfloat16, torch.float16) or q.dtype == torch.float32 and not q.is_cuda) or q.stride(2) != 1:
+        raise ValueError("paged.attention: q must be bf16 or fp16 (on the CPU also fp32) with contiguous head elements")
     _ints("table", table, 2)
     _ints("starts", starts, 1)
     _ints("lengths", lengths, 1)

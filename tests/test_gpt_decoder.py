@@ -1,0 +1,175 @@
+"""Decoding with the cache: logits against the plain network whose keys and values pass the cache's rounding, prompts in parts, places that
+wait, end and start again, refusals; on the GPU against the same decoder on the CPU."""
+import pytest
+import torch
+
+from spiraltorch_b200.models.gpt import GPTConfig, GPTModel
+from spiraltorch_b200.ops import paged as P
+from spiraltorch_b200.ops import rotary as R
+
+CONFIGS = [dict(), dict(norm="layer", positional="learned"), dict(rope_dim=32, rope_interleaved=True),
+           dict(rope_scaling=R.Scaling("bands", 4.0, original=64))]
+
+
+def _model(device="cpu", dtype=torch.float32, **kw):
+    cfg = GPTConfig(vocab_size=96, d_model=128, n_layers=2, n_heads=2, ffn=256, seq_len=256, init_std=0.08, **kw)
+    return GPTModel(cfg, device=device, dtype=dtype)
+
+
+def _rounded(x, page):
+    """fp64 keys or values [S, H, D] as the cache holds them when a sequence is stored at once."""
+    y = x.clone()
+    for i in range(0, x.shape[0], page):
+        unit = torch.exp2(P.page_exponent(x[i:i + page].abs().amax((0, 2))).double())[None, :, None]
+        y[i:i + page] = P.to_codes((x[i:i + page] / unit).float()).double() * unit
+    return y
+
+
+def _plain(model, tokens, page):
+    """Logits of every position."""
+    cfg, w = model.cfg, {k: v.detach().double() for k, v in model.p.items()}
+    S, H, D = len(tokens), cfg.n_heads, cfg.head_dim
+
+    def norm(x, name):
+        if cfg.norm == "rms":
+            return x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + cfg.norm_eps) * w[name + ".gamma"]
+        return torch.nn.functional.layer_norm(x, (cfg.d_model,), w[name + ".gamma"], w[name + ".beta"], cfg.norm_eps)
+
+    h = w["embed.weight"][tokens]
+    if cfg.positional == "learned":
+        h = h + w["pos.weight"][:S]
+    for l in range(cfg.n_layers):
+        q, k, v = (norm(h, f"h{l}.norm1") @ w[f"h{l}.qkv.weight"].T).view(S, 3, H, D).unbind(1)
+        if cfg.positional == "rope":
+            q, k = (R.rotary_reference(t, torch.arange(S), model.rope_freq, cfg.rope_interleaved) for t in (q, k))
+        k, v = _rounded(k, page), _rounded(v, page)
+        s = torch.einsum("ihd,jhd->hij", q, k) * D ** -0.5 + torch.full((S, S), float("-inf"), dtype=torch.float64).triu(1)
+        h = h + torch.einsum("hij,jhd->ihd", torch.softmax(s, -1), v).reshape(S, H * D) @ w[f"h{l}.proj.weight"].T
+        h = h + torch.nn.functional.gelu(norm(h, f"h{l}.norm2") @ w[f"h{l}.fc1.weight"].T, approximate="tanh") @ w[f"h{l}.fc2.weight"].T
+    return norm(h, "norm_f") @ w["embed.weight"].T
+
+
+@pytest.mark.parametrize("kw", CONFIGS)
+def test_prompt_logits_against_the_plain_network(kw):
+    """The decoder computes in fp32, the plain network in fp64.  A key or value that stands within fp32's error of a border between two codes may
+    fall to the other one, 2^-4 of it away at most: seeds are as they are, such elements are few, and one moves a logit by its share of one head
+    element in one key.  Allowed: 2 % of the logits' spread, which one code in 16 and a key in 5 would reach only if all of a head's 64 elements moved."""
+    model = _model(**kw)
+    g = torch.Generator().manual_seed(4)
+    prompts = [torch.randint(0, 96, (n,), generator=g) for n in (5, 33, 70)]
+    for page in (16, 64):
+        got = model.decoder(3, 128, page_size=page).extend(prompts)
+        for p, row in zip(prompts, got):
+            want = _plain(model, p, page)[-1]
+            assert (row.double() - want).abs().max() <= 0.02 * want.std()
+
+
+def test_parts_waiting_and_places_that_start_again():
+    model = _model()
+    g = torch.Generator().manual_seed(5)
+    a, b, c = (torch.randint(0, 96, (n,), generator=g).tolist() for n in (40, 23, 9))
+    d = model.decoder(2, 64, pages=5, page_size=16)
+    whole = model.decoder(1, 64, page_size=64).extend([a])[0]
+    assert d.extend([a[:17], []]).shape == (1, 96) and d.held == [17, 0]
+    assert d.extend([a[17:39], b[:20]]).shape == (2, 96) and d.pages_left == 0
+    last = d.step(torch.tensor([a[39], b[20]]))
+    # the same tokens in parts: scales grow as tokens come, which re-rounds what becomes subnormal, and pages have other sizes
+    assert torch.nn.functional.cosine_similarity(last[0], whole, dim=0) > 0.99
+    with pytest.raises(ValueError, match="pages"):
+        d.extend([c * 2, []])
+    with pytest.raises(ValueError, match="tokens, at most"):
+        d.extend([[], [1] * 60])
+    assert d.held == [40, 21]
+    d.release([1])
+    assert d.pages_left == 2 and d.lengths.tolist() == [40, 0] and int(d.free_count) == 2
+    again = d.extend([[], c])[0]
+    fresh = model.decoder(1, 64, page_size=16).extend([c])[0]
+    assert torch.equal(again, fresh)
+
+
+def test_generate():
+    model = _model()
+    prompts = [[1, 2, 3], [7], list(range(30))]
+    got = model.generate(prompts, 6, page_size=16)
+    assert [len(t) for t in got] == [6, 6, 6]
+    for p, t in zip(prompts, got):                        # alone, as in company
+        d = model.decoder(1, 40, page_size=16)
+        row = d.extend([p])
+        for want in t:
+            assert int(row.argmax()) == want
+            row = d.step(torch.tensor([want]))
+    stop = got[0][2]
+    cut = model.generate(prompts, 6, stop=stop, page_size=16)
+    for full, t in zip(got, cut):
+        assert t == (full[:full.index(stop)] if stop in full else full)
+    assert model.generate(prompts, 0) == [[], [], []]
+
+
+def test_training_with_other_rotary_forms_matches_autograd():
+    for kw in CONFIGS[2:]:
+        cfg = GPTConfig(vocab_size=64, d_model=128, n_layers=1, n_heads=2, ffn=128, seq_len=8, init_std=0.05, **kw)
+        model = GPTModel(cfg, device="cpu", dtype=torch.float32)
+        tokens, targets = torch.randint(0, 64, (2, 8)), torch.randint(0, 64, (2, 8))
+        w = model.p["h0.qkv.weight"]
+        model.forward_backward(tokens, targets)
+        grad = w.main_grad.clone()
+        for at in ((3, 5), (70, 1), (130, 100), (300, 7)):      # q, q, k and v rows against differences
+            with torch.no_grad():
+                keep, loss = float(w[at]), []
+                for step in (1e-2, -1e-2):
+                    w[at] = keep + step
+                    loss.append(float(model(tokens, targets)))
+                w[at] = keep
+            # fp32 losses near 4.2: 2^-22 each over 2e-2, and the third derivative's 1e-4 of a gradient
+            assert abs((loss[0] - loss[1]) / 2e-2 - float(grad[at])) <= 2 * 4.2 * 2 ** -22 / 2e-2 + 0.01 * float(grad.abs().max())
+
+
+def test_refusals():
+    model = _model(norm="layer", positional="learned")
+    for bad in (lambda: model.decoder(0, 8), lambda: model.decoder(1, 0), lambda: model.decoder(1, 257), lambda: model.decoder(1, 8, page_size=24),
+                lambda: model.decoder(2, 8).extend([[1]]), lambda: model.decoder(1, 8).extend([[96]]), lambda: model.decoder(1, 8).extend([[]]),
+                lambda: model.decoder(1, 8).extend([[-1]]), lambda: model.decoder(2, 8).step(torch.zeros(1, dtype=torch.int64)),
+                lambda: model.decoder(2, 8).step(torch.zeros(2)), lambda: model.decoder(1, 8).release([1]), lambda: model.generate([[]], 2),
+                lambda: GPTModel(GPTConfig(vocab_size=64, d_model=128, n_layers=1, n_heads=2, ffn=128, rope_dim=66), device="cpu")):
+        with pytest.raises(ValueError):
+            bad()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", CONFIGS)
+def test_gpu_decoder_follows_the_cpu_one(kw):
+    gpu = _model("cuda", torch.bfloat16, **kw)
+    cpu = _model(**kw)
+    cpu.flat_w.copy_(gpu.flat_w.float().cpu())
+    g = torch.Generator().manual_seed(6)
+    prompts = [torch.randint(0, 96, (n,), generator=g) for n in (3, 100, 17)]
+    a, b = gpu.decoder(3, 256, page_size=32), cpu.decoder(3, 256, page_size=32)
+    rows = [(a.extend(prompts), b.extend(prompts))]              # 100 tokens: the dense path
+    rows.append((a.extend([p[:9] for p in prompts]), b.extend([p[:9] for p in prompts])))
+    for _ in range(3):
+        t = torch.randint(0, 96, (3,), generator=g)
+        rows.append((a.step(t.cuda()), b.step(t)))
+    for x, y in rows:
+        # bf16 activations through two layers: 2^-8 a rounding, about ten of them in a row, and codes that fall to their neighbours (2^-4)
+        assert torch.nn.functional.cosine_similarity(x.float().cpu(), y, dim=-1).min() > 0.99
+
+
+@pytest.mark.gpu
+def test_gpu_step_captured():
+    model = _model("cuda", torch.bfloat16)
+    d, e = model.decoder(2, 200, page_size=16), model.decoder(2, 200, page_size=16)
+    tokens = torch.tensor([3, 5], device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for x in (d, e):
+            x.extend([[1, 2, 3], [4]])
+            x.step(tokens)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = d.step(tokens)
+    for i in range(60):
+        tokens.copy_(torch.tensor([i, 95 - i]))
+        graph.replay()
+        assert torch.equal(out, e.step(tokens))

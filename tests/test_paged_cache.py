@@ -431,7 +431,7 @@ def test_refusals():
             lambda: P.store(k.transpose(1, 2).contiguous().transpose(1, 2), k, pages, slots), lambda: P.store(k, k, pages, torch.tensor([0, 5, 1, 2])),
             lambda: P.store(k, k, pages._replace(k=pages.k.half()), slots), lambda: P.store(k, k, pages._replace(k_scale=pages.k_scale[:2]), slots),
             lambda: P.read(pages, i32(2, 3), i32(3), 4), lambda: P.read(pages, i32(2, 3), i32(2), 4, torch.float16), lambda: P.read(pages, i32(1, 1) + 3, i32(1) + 1, 4),
-            lambda: P.attention(q.float(), pages, i32(2, 3), i32(3), i32(2), **ok), lambda: P.attention(q[:, :3], pages, i32(2, 3), i32(3), i32(2), **ok),
+            lambda: P.attention(q.double(), pages, i32(2, 3), i32(3), i32(2), **ok), lambda: P.attention(q[:, :3], pages, i32(2, 3), i32(3), i32(2), **ok),
             lambda: P.attention(q[..., :32], pages, i32(2, 3), i32(3), i32(2), **ok), lambda: P.attention(q, pages, i32(2, 3), i32(2), i32(2), **ok),
             lambda: P.attention(q, pages, i32(2, 3), i32(3), i32(2), max_queries=0), lambda: P.attention(q, pages, i32(2, 3), i32(3), i32(2), scale=float("nan"), **ok),
             lambda: P.attention(q, pages, i32(2, 3), i32(3), i32(2), out=q.half(), **ok), lambda: P.attention(q.requires_grad_(True), pages, i32(2, 3), i32(3), i32(2), **ok)):
