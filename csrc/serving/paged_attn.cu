@@ -364,8 +364,9 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
     }
   }
   const long long all = units_in_all<N>(p, sh.sums);
-  const long long u0 = all * blockIdx.x / gridDim.x, u1 = all * (blockIdx.x + 1) / gridDim.x;
-  if (u0 >= u1) return;
+  const int runs = static_cast<int>(min(static_cast<long long>(gridDim.x), all));      // none of them empty
+  if (static_cast<int>(blockIdx.x) >= runs) return;
+  const long long u0 = all * blockIdx.x / runs, u1 = all * (blockIdx.x + 1) / runs;
   Found f = find_unit<N>(p, u0, sh.sums, &sh.found);
   Seq sq = sequence<N>(p, f.b);
 
@@ -492,49 +493,84 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
   }
 }
 
-// Joins the parts of an item that several blocks worked on.  Block c looks at the border between the runs of blocks c and c + 1: if it is
-// the first one inside an item, the item is this block's.
+// Joins the parts of an item that several blocks worked on, a block (border, row): border c is the one between the runs of blocks c and
+// c + 1, and the first border inside an item stands for the item.  All parts' maxima and sums are read at once; then each warp adds up its
+// share of the parts, D / 32 elements a thread, with as many loads in flight as it has parts.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads) paged_join_kernel(AttnParams p, int runs) {
-  constexpr int N = 8 * NT;
+__global__ void __launch_bounds__(kThreads) paged_join_kernel(AttnParams p, int most_runs) {
+  constexpr int N = 8 * NT, E = D / 32;
+  extern __shared__ float weight[];      // [parts]
   __shared__ long long sums[kWarps];
   __shared__ Found found;
+  __shared__ float red[2][kWarps], rows[kWarps][D];
   chain_begin(p.table, p.starts, p.lengths);
   const long long all = units_in_all<N>(p, sums);
-  const int c = blockIdx.x;
+  const int runs = static_cast<int>(min(static_cast<long long>(most_runs), all)), c = blockIdx.x;
+  if (c + 1 >= runs) return;
   const long long u0 = all * c / runs, u1 = all * (c + 1) / runs;
-  if (u0 >= u1 || u1 >= all) return;
   const Found f = find_unit<N>(p, u1, sums, &found);
   const Seq sq = sequence<N>(p, f.b);
   const long long in = u1 - f.first;
-  const int t = static_cast<int>(in % sq.tiles);
+  const int t = static_cast<int>(in % sq.tiles), r = blockIdx.y;
   if (t == 0 || u1 - t < u0) return;
   const long long end = u1 - t + sq.tiles, item = in / sq.tiles;
   const int rb = static_cast<int>(item % sq.row_blocks), h = static_cast<int>(item / sq.row_blocks);
   const int row0 = rb * N, row_end = min(sq.n * p.group, row0 + N);
-  T* out = static_cast<T*>(p.out);
-  constexpr int PER = D / 4, AT_ONCE = kThreads / PER;      // threads of a row: four elements each
-  for (int r = blockIdx.y * AT_ONCE + threadIdx.x / PER; r < row_end - row0; r += gridDim.y * AT_ONCE) {
-    const int d = threadIdx.x % PER * 4;
-    float m = -INFINITY, l = 0.0f;
-    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int b = c; b < runs && all * b / runs < end; ++b) {
-      if (all * b / runs >= all * (b + 1) / runs) continue;
-      const float* part = part_of<D, NT>(p, 2LL * b + (b == c ? 1 : 0));
-      const float pm = part[N * D + r], pl = part[N * D + N + r];
-      const float4 y = *reinterpret_cast<const float4*>(part + r * D + d);
-      if (pl == 0.0f) continue;      // saw nothing
-      const float mx = fmaxf(m, pm), a = l == 0.0f ? 0.0f : exp2f(m - mx), e = exp2f(pm - mx);
-      m = mx, l = l * a + pl * e;
-      x.x = x.x * a + y.x * e, x.y = x.y * a + y.y * e, x.z = x.z * a + y.z * e, x.w = x.w * a + y.w * e;
-    }
-    const int fr = row0 + r;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T* o = out + (sq.start + fr / p.group) * p.o_row + (h * p.group + fr % p.group) * p.o_head + d;
-    o[0] = from_f<T>(x.x * inv), o[1] = from_f<T>(x.y * inv), o[2] = from_f<T>(x.z * inv), o[3] = from_f<T>(x.w * inv);
-    if (d == 0 && p.lse != nullptr)
-      p.lse[(sq.start + fr / p.group) * static_cast<long long>(p.heads) + h * p.group + fr % p.group] = l == 0.0f ? -INFINITY : (m + log2f(l)) / kLog2e;
+  if (r >= row_end - row0) return;
+  // block b holds a part if its run begins before the end: all * b / runs < end, which is all * b < end * runs
+  const int parts = static_cast<int>((end * runs - 1) / all) - c + 1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr long long kSlot = N * (D + 2);
+  const float* base = p.parts + (2LL * c) * kSlot;      // part 0 lies in the block's second slot, the others in the first slots of their blocks
+
+  float m = -INFINITY;
+  for (int i = threadIdx.x; i < parts; i += kThreads) {
+    const float* part = base + (2LL * i + (i == 0 ? 1 : 0)) * kSlot + N * D;
+    if (part[N + r] != 0.0f) m = fmaxf(m, part[r]);      // a sum of 0: saw nothing
   }
+  m = st::warp_max(m);
+  if (lane == 0) red[0][warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) m = fmaxf(m, red[0][w]);
+  float l = 0.0f;
+  for (int i = threadIdx.x; i < parts; i += kThreads) {
+    const float* part = base + (2LL * i + (i == 0 ? 1 : 0)) * kSlot + N * D;
+    const float pl = part[N + r], e = pl == 0.0f ? 0.0f : exp2f(part[r] - m);
+    weight[i] = e;
+    l += pl * e;
+  }
+  l = st::warp_sum(l);
+  if (lane == 0) red[1][warp] = l;
+  __syncthreads();
+  l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+
+  float x[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = 0.0f;
+#pragma unroll 8
+  for (int i = warp; i < parts; i += kWarps) {
+    const float w = weight[i];
+    const float* part = base + (2LL * i + (i == 0 ? 1 : 0)) * kSlot + r * D + lane * E;
+    if constexpr (E == 4) {
+      const float4 y = *reinterpret_cast<const float4*>(part);
+      x[0] = fmaf(y.x, w, x[0]), x[1] = fmaf(y.y, w, x[1]), x[2] = fmaf(y.z, w, x[2]), x[3] = fmaf(y.w, w, x[3]);
+    } else {
+      const float2 y = *reinterpret_cast<const float2*>(part);
+      x[0] = fmaf(y.x, w, x[0]), x[1] = fmaf(y.y, w, x[1]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) rows[warp][lane * E + e] = x[e];
+  __syncthreads();
+  const int d = threadIdx.x, fr = row0 + r;
+  const long long row = sq.start + fr / p.group;
+  const int head = h * p.group + fr % p.group;
+  if (d < D) {
+    const float sum = (rows[0][d] + rows[1][d]) + (rows[2][d] + rows[3][d]);
+    static_cast<T*>(p.out)[row * p.o_row + head * p.o_head + d] = from_f<T>(l == 0.0f ? 0.0f : sum / l);
+  }
+  if (d == 0 && p.lse != nullptr) p.lse[row * p.heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) / kLog2e;
 }
 
 // Row tiles of 8 by the rows that the longest step of a sequence has.
@@ -552,7 +588,7 @@ int launch(const AttnParams& p, cudaStream_t stream) {
   if (smem > 48 * 1024) ST_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaError_t e = st::chained(kernel, dim3(runs), dim3(kThreads), smem, stream)(p);
   if (e != cudaSuccess) return st::fail_cuda(e, "paged attention");
-  e = st::chained(paged_join_kernel<T, D, NT>, dim3(runs - 1, NT * 2), dim3(kThreads), 0, stream)(p, runs);
+  e = st::chained(paged_join_kernel<T, D, NT>, dim3(runs - 1, 8 * NT), dim3(kThreads), runs * sizeof(float), stream)(p, runs);
   if (e != cudaSuccess) return st::fail_cuda(e, "paged attention: join");
   return ST_OK;
 }

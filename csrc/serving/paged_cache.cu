@@ -174,65 +174,72 @@ __global__ void __launch_bounds__(kPlanThreads) release_kernel(int* lengths, con
 // ---- storing --------------------------------------------------------------------------------------------------------------------
 // Bound by memory: 2 (4 for fp32) bytes read and 1 written per element.  Rows that follow one another in a page are a group, found by
 // its first row; the largest magnitude of the group and of each head decides the scale, so every element is looked at twice: the
-// second time from the registers of the team that works on the group, or from L1 where the group is larger.
-constexpr int kStoreThreads = 256;
+// second time from registers, which hold 16 rows of 128 elements of 16 bits per warp, or from L1 where there are more rows.
+// A warp works on one group, head and tensor; where a page holds more rows than its registers, two or four warps share a group.
+constexpr int kStoreThreads = 256, kStoreWarps = kStoreThreads / 32;
+constexpr int kHeld = 8;      // 16-byte loads that a thread keeps
 
 struct PutParams {
   long long k_row, k_head, v_row, v_head;
-  long long rows;
-  int kv_heads, shift, segment;
-  long long pages;
+  long long rows, pages;
+  int kv_heads, shift;
+  int segment, team, heads_per_block;      // set at launch
 };
 
-template <typename T> __device__ __forceinline__ void load8f(const T* p, bool wide, float (&f)[8]);
-template <> __device__ __forceinline__ void load8f(const float* p, bool wide, float (&f)[8]) {
-  if (wide) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = p[i];
+// What differs between the types: 16 bytes to magnitudes (as integers, which order as they do), and to codes.
+template <typename T> struct Raw;
+template <typename T> struct Raw16 {
+  static constexpr int kCodes = 8;
+  static __device__ __forceinline__ uint4 load(const T* p, bool wide) {
+    if (wide) return *reinterpret_cast<const uint4*>(p);
+    const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+    return make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
   }
-}
-template <> __device__ __forceinline__ void load8f(const __half* p, bool wide, float (&f)[8]) {
-  if (wide) {
-    uint4 u = *reinterpret_cast<const uint4*>(p);
-    const __half2* h = reinterpret_cast<const __half2*>(&u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { const float2 x = __half22float2(h[i]); f[2 * i] = x.x, f[2 * i + 1] = x.y; }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = __half2float(p[i]);
+  static __device__ __forceinline__ uint32_t top(uint32_t m, uint4 x) {      // two magnitudes side by side
+    m = __vmaxu2(m, __vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu));
+    return __vmaxu2(m, __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
   }
-}
-template <> __device__ __forceinline__ void load8f(const __nv_bfloat16* p, bool wide, float (&f)[8]) {
-  if (wide) {
-    uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { const float2 x = st::unpack_bf16x2(w[i]); f[2 * i] = x.x, f[2 * i + 1] = x.y; }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = __bfloat162float(p[i]);
+  static __device__ __forceinline__ uint32_t one(uint32_t m) { return max(m & 0xffffu, m >> 16); }
+  static __device__ __forceinline__ uint32_t finite(uint32_t x) {
+    const uint32_t lo = x & 0x7fffu, hi = x >> 16 & 0x7fffu;
+    return (lo < Raw<T>::kInf ? lo : 0u) | (hi < Raw<T>::kInf ? hi << 16 : 0u);
   }
-}
-
-__device__ __forceinline__ float finite_max(float m, const float (&f)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = fabsf(f[i]);
-    m = a < INFINITY ? fmaxf(m, a) : m;      // false for NaN too
+  static __device__ __forceinline__ uint32_t pair(float2 x, float inv) { return __nv_cvt_float2_to_fp8x2(make_float2(x.x * inv, x.y * inv), __NV_SATFINITE, __NV_E4M3); }
+  static __device__ __forceinline__ void put(unsigned char* p, uint4 x, float inv) {
+    const uint32_t a = pair(Raw<T>::two(x.x), inv) | pair(Raw<T>::two(x.y), inv) << 16, b = pair(Raw<T>::two(x.z), inv) | pair(Raw<T>::two(x.w), inv) << 16;
+    *reinterpret_cast<uint2*>(p) = make_uint2(a, b);
   }
-  return m;
-}
-
-// Eight codes of values times a power of two; the conversion saturates and keeps NaN.
-__device__ __forceinline__ uint2 codes8(const float (&f)[8], float inv) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * i] * inv, f[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-  return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
-}
+};
+template <> struct Raw<__nv_bfloat16> : Raw16<__nv_bfloat16> {
+  static constexpr uint32_t kInf = 0x7f80;
+  static __device__ __forceinline__ float value(uint32_t m) { return __uint_as_float(m << 16); }
+  static __device__ __forceinline__ float2 two(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+};
+template <> struct Raw<__half> : Raw16<__half> {
+  static constexpr uint32_t kInf = 0x7c00;
+  static __device__ __forceinline__ float value(uint32_t m) { return __half2float(__ushort_as_half(static_cast<unsigned short>(m))); }
+  static __device__ __forceinline__ float2 two(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+};
+template <> struct Raw<float> {
+  static constexpr int kCodes = 4;
+  static constexpr uint32_t kInf = 0x7f800000u;
+  static __device__ __forceinline__ uint4 load(const float* p, bool wide) {
+    if (wide) return *reinterpret_cast<const uint4*>(p);
+    const unsigned* u = reinterpret_cast<const unsigned*>(p);
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  static __device__ __forceinline__ uint32_t top(uint32_t m, uint4 x) {
+    return max(max(m, max(x.x & 0x7fffffffu, x.y & 0x7fffffffu)), max(x.z & 0x7fffffffu, x.w & 0x7fffffffu));
+  }
+  static __device__ __forceinline__ uint32_t one(uint32_t m) { return m; }
+  static __device__ __forceinline__ uint32_t finite(uint32_t x) { return (x & 0x7fffffffu) < kInf ? x & 0x7fffffffu : 0u; }
+  static __device__ __forceinline__ float value(uint32_t m) { return __uint_as_float(m); }
+  static __device__ __forceinline__ void put(unsigned char* p, uint4 x, float inv) {
+    *reinterpret_cast<uint32_t*>(p) =
+        __nv_cvt_float2_to_fp8x2(make_float2(__uint_as_float(x.x) * inv, __uint_as_float(x.y) * inv), __NV_SATFINITE, __NV_E4M3) |
+        static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(__uint_as_float(x.z) * inv, __uint_as_float(x.w) * inv), __NV_SATFINITE, __NV_E4M3)) << 16;
+  }
+};
 
 // The page's older codes re-rounded to a larger scale: code * 2^(old - new).
 __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
@@ -246,108 +253,118 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
   return out;
 }
 
-// One tensor's part of a group: rows [r0, r0 + n) of one head go to page offsets [off, off + n).  A team of TEAM threads (a warp or the
-// block); L = D / 8 lanes hold a row.
-template <typename T, int D, int TEAM>
-__device__ void store_group(const T* src, long long row_stride, bool wide, unsigned char* dst, float* scale, int off, int n, float* shared_max, unsigned* err) {
-  constexpr int L = D / 8, RPT = TEAM / L, HELD = 4;      // rows a pass, passes held in registers
-  const int me = TEAM == 32 ? threadIdx.x & 31 : threadIdx.x, lane = me % L, row = me / L;
-  float held[HELD][8];
-  float m = 0.0f;
+// One tensor's part of a group: rows [0, n) of one head from src go to page offsets [off, off + n).  The team is `warps` warps, this one
+// its `me`-th; with several, all teams of the block come here together (n = 0: only for the barriers).
+template <typename T, int D>
+__device__ void store_group(const T* src, long long row_stride, bool wide, unsigned char* dst, float* scale, int off, int n, int me, int warps, uint32_t* shared_top) {
+  using R = Raw<T>;
+  constexpr int L = D / R::kCodes, RP = 32 / L;      // lanes of a row, rows of a load
+  const int lane = threadIdx.x & 31, first = me * RP + lane / L, step = warps * RP, at = lane % L * R::kCodes;
+  uint4 held[kHeld];
 #pragma unroll
-  for (int i = 0; i < HELD; ++i) {
-    const int r = row + i * RPT;
-    if (r < n) load8f(src + r * row_stride + lane * 8, wide, held[i]);
-    else
-#pragma unroll
-      for (int e = 0; e < 8; ++e) held[i][e] = 0.0f;
+  for (int i = 0; i < kHeld; ++i) {
+    const int r = first + i * step;
+    held[i] = r < n ? R::load(src + r * row_stride + at, wide) : make_uint4(0, 0, 0, 0);
   }
-  const float before = off > 0 ? *scale : 0.0f;
+  const float before = n > 0 && off > 0 ? *scale : 0.0f;
+  uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < HELD; ++i) m = finite_max(m, held[i]);
-  for (int r = row + HELD * RPT; r < n; r += RPT) {
-    float f[8];
-    load8f(src + r * row_stride + lane * 8, wide, f);
-    m = finite_max(m, f);
+  for (int i = 0; i < kHeld; ++i) m = R::top(m, held[i]);
+  for (int r = first + kHeld * step; r < n; r += step) m = R::top(m, R::load(src + r * row_stride + at, wide));
+  m = R::one(m);
+  if (__any_sync(0xffffffffu, m >= R::kInf)) {      // once more without what is not finite
+    m = 0;
+    for (int r = first; r < n; r += step) {
+      const uint4 x = R::load(src + r * row_stride + at, wide);
+      m = R::top(m, make_uint4(R::finite(x.x), R::finite(x.y), R::finite(x.z), R::finite(x.w)));
+    }
+    m = R::one(m);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if constexpr (TEAM > 32) {
-    __syncthreads();                                    // the one before may still be read
-    if ((threadIdx.x & 31) == 0) shared_max[threadIdx.x >> 5] = m;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < TEAM / 32; ++w) m = fmaxf(m, shared_max[w]);
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (warps > 1) {
+    const int warp = threadIdx.x >> 5;
+    __syncthreads();      // the group before may still be read
+    if (lane == 0) shared_top[warp] = m;
+    __syncthreads();      // and every warp has read the old scale
+    for (int w = 0; w < warps; ++w) m = max(m, shared_top[warp - me + w]);
   }
-  if constexpr (TEAM == 32) __syncwarp();               // every thread has read the old scale; one writes the new one
-  int e = st::page_exponent(m);
+  if (n == 0) return;
+  __syncwarp();
+  int e = st::page_exponent(R::value(m));
   const int old = off > 0 ? st::scale_exponent(before) : st::kMinExponent;
   e = max(e, old);
   const float inv = st::exp2_int(-e);
   if (e > old && off > 0) {
-    const float ratio = st::exp2_int(max(old - e, -126));
-    for (int i = me; i < off * (D / 4); i += TEAM) {
+    const float ratio = st::exp2_int(old - e);      // 2^-120 at least
+    for (int i = me * 32 + lane; i < off * (D / 4); i += warps * 32) {
       uint32_t* p = reinterpret_cast<uint32_t*>(dst) + i;
       *p = rescale4(*p, ratio);
     }
   }
-  if (me == 0) *scale = st::exp2_int(e);
-  unsigned char* out = dst + static_cast<long long>(off) * D + lane * 8;
+  if (me == 0 && lane == 0) *scale = st::exp2_int(e);
+  unsigned char* out = dst + static_cast<long long>(off) * D + at;
 #pragma unroll
-  for (int i = 0; i < HELD; ++i) {
-    const int r = row + i * RPT;
-    if (r < n) *reinterpret_cast<uint2*>(out + r * D) = codes8(held[i], inv);
+  for (int i = 0; i < kHeld; ++i) {
+    const int r = first + i * step;
+    if (r < n) R::put(out + r * D, held[i], inv);
   }
-  for (int r = row + HELD * RPT; r < n; r += RPT) {
-    float f[8];
-    load8f(src + r * row_stride + lane * 8, wide, f);
-    *reinterpret_cast<uint2*>(out + r * D) = codes8(f, inv);
-  }
-  if constexpr (TEAM == 32) __syncwarp();
+  for (int r = first + kHeld * step; r < n; r += step) R::put(out + r * D, R::load(src + r * row_stride + at, wide), inv);
+  __syncwarp();
 }
 
-// Block (segment of rows, head).  Few groups in the segment: the block takes them one after another; many (decoding: a group is a row):
-// a warp each.
+// Block (segment of at most a page's rows, heads_per_block heads).
 template <typename T, int D>
 __global__ void __launch_bounds__(kStoreThreads) store_kernel(const T* __restrict__ k, const T* __restrict__ v, unsigned char* kc, unsigned char* vc, float* ks, float* vs,
                                                               const long long* __restrict__ slots, const PutParams p, bool wide, unsigned* err) {
   chain_begin(k, v, slots);
+  __shared__ uint32_t goes_on[2 * kStoreThreads / 32];      // a bit per row of the segment and of the page's length behind it: it follows the row before in its page
   __shared__ int first_row[kStoreThreads], group_rows[kStoreThreads];
+  __shared__ long long first_slot[kStoreThreads];
   __shared__ int groups;
-  __shared__ float shared_max[kStoreThreads / 32];
+  __shared__ uint32_t shared_top[kStoreWarps];
   const long long r0 = static_cast<long long>(blockIdx.x) * p.segment;
-  const int h = blockIdx.y, P = 1 << p.shift;
+  const int P = 1 << p.shift, warp = threadIdx.x >> 5;
   const long long limit = p.pages << p.shift;
   if (threadIdx.x == 0) groups = 0;
-  __syncthreads();
-  const long long r = r0 + threadIdx.x;
-  if (threadIdx.x < p.segment && r < p.rows) {
-    const long long s = slots[r];
-    if (s >= limit) {
-      if (h == 0) st::report_error(err, st::ERR_BOUNDS, 0x7002);
-    } else if (s >= 0 && ((s & (P - 1)) == 0 || r == 0 || slots[r - 1] != s - 1)) {
-      const int off = static_cast<int>(s & (P - 1));
-      int n = 1;
-      while (n < P - off && r + n < p.rows && slots[r + n] == s + n) ++n;
-      const int at = atomicAdd(&groups, 1);      // which team takes which group does not change results
-      first_row[at] = threadIdx.x, group_rows[at] = n;
+  bool leads = false;
+  long long mine = -1;
+  for (int j = threadIdx.x, part = 0; part < (p.segment + P + kStoreThreads - 1) / kStoreThreads; j += kStoreThreads, ++part) {
+    const long long r = r0 + j, s = r < p.rows ? slots[r] : -1;
+    const bool goes = s >= 0 && (s & (P - 1)) != 0 && r > 0 && slots[r - 1] == s - 1;
+    const uint32_t bits = __ballot_sync(0xffffffffu, goes);
+    if ((threadIdx.x & 31) == 0) goes_on[j >> 5] = bits;
+    if (part == 0) {
+      leads = j < p.segment && s >= 0 && s < limit && !goes;
+      mine = s;
+      if (j < p.segment && s >= limit && blockIdx.y == 0) st::report_error(err, st::ERR_BOUNDS, 0x7002);
     }
   }
   __syncthreads();
-  const int n_groups = groups, warp = threadIdx.x >> 5;
-  const bool by_warp = n_groups > 2;
-  for (int i = by_warp ? warp : 0; i < n_groups; i += by_warp ? kStoreThreads / 32 : 1) {
-    const long long row = r0 + first_row[i], s = slots[row], page = s >> p.shift, at = page * gridDim.y + h;
-    const int off = static_cast<int>(s & (P - 1)), n = group_rows[i];
-    const T *sk = k + row * p.k_row + h * p.k_head, *sv = v + row * p.v_row + h * p.v_head;
-    unsigned char *dk = kc + at * P * D, *dv = vc + at * P * D;
-    if (by_warp) {
-      store_group<T, D, 32>(sk, p.k_row, wide, dk, ks + at, off, n, shared_max, err);
-      store_group<T, D, 32>(sv, p.v_row, wide, dv, vs + at, off, n, shared_max, err);
-    } else {
-      store_group<T, D, kStoreThreads>(sk, p.k_row, wide, dk, ks + at, off, n, shared_max, err);
-      store_group<T, D, kStoreThreads>(sv, p.v_row, wide, dv, vs + at, off, n, shared_max, err);
+  if (leads) {
+    int j = threadIdx.x + 1, w = j >> 5;
+    uint32_t ends = ~goes_on[w] >> (j & 31);
+    if (ends) j += __ffs(ends) - 1;
+    else {
+      const int last = (p.segment + P - 1) >> 5;
+      for (++w; w <= last && goes_on[w] == 0xffffffffu; ++w) {}
+      j = w > last ? 32 * w : 32 * w + __ffs(~goes_on[w]) - 1;
     }
+    const int at = atomicAdd(&groups, 1);      // which warp takes which group does not change results
+    first_row[at] = threadIdx.x, group_rows[at] = min(j - static_cast<int>(threadIdx.x), P - static_cast<int>(mine & (P - 1))), first_slot[at] = mine;
+  }
+  __syncthreads();
+  const int n_groups = groups, h0 = blockIdx.y * p.heads_per_block, heads = min(p.heads_per_block, p.kv_heads - h0);
+  auto work = [&](int group, int unit, int me, int warps) {
+    const bool any = unit < 2 * heads;
+    const int h = h0 + (any ? unit >> 1 : 0), second = unit & 1;
+    const long long row = r0 + first_row[group], s = first_slot[group], at = (s >> p.shift) * p.kv_heads + h;
+    store_group<T, D>(second ? v + row * p.v_row + h * p.v_head : k + row * p.k_row + h * p.k_head, second ? p.v_row : p.k_row, wide, (second ? vc : kc) + at * P * D,
+                      (second ? vs : ks) + at, static_cast<int>(s & (P - 1)), any ? group_rows[group] : 0, me, warps, shared_top);
+  };
+  if (p.team > 1 && n_groups <= 2) {
+    for (int g = 0; g < n_groups; ++g) work(g, warp / p.team, warp % p.team, p.team);
+  } else {
+    for (int i = warp; i < n_groups * 2 * heads; i += kStoreWarps) work(i / (2 * heads), i % (2 * heads), 0, 1);
   }
 }
 
@@ -355,13 +372,17 @@ template <typename T>
 int launch_store(const void* k, const void* v, void* kc, void* vc, float* ks, float* vs, const long long* slots, PutParams p, int dim, cudaStream_t stream) {
   const long long strides = p.k_row | p.k_head | p.v_row | p.v_head;
   const bool wide = (strides * static_cast<long long>(sizeof(T))) % 16 == 0 && ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
-  // a page's rows to a block, fewer while that leaves the chip short of blocks
+  // four warps to a page's rows of a head, two where its rows are few; 8 warps work on the keys and values of 1, 2 or 4 heads
+  p.team = p.shift >= 6 ? 4 : p.shift == 5 ? 2 : 1;
+  p.heads_per_block = 4 / p.team;
+  const int y = (p.kv_heads + p.heads_per_block - 1) / p.heads_per_block;
+  // a page's rows to a block, fewer while that leaves the chip short of blocks: down to a warp per row, head and tensor
   int segment = 1 << p.shift;
-  while (segment > 8 && (p.rows + segment - 1) / segment * p.kv_heads < 2 * st::sm_count()) segment /= 2;
+  while (segment * p.heads_per_block > 4 && (p.rows + segment - 1) / segment * y < 2 * st::sm_count()) segment /= 2;
   p.segment = segment;
   const long long blocks = (p.rows + segment - 1) / segment;
   if (blocks > 2147483647LL) return st::fail(ST_ERR_TOO_LARGE, "paged store: too many rows");
-  const dim3 grid(static_cast<unsigned>(blocks), p.kv_heads);
+  const dim3 grid(static_cast<unsigned>(blocks), y);
   const cudaError_t e = st::chained(dim == 64 ? store_kernel<T, 64> : store_kernel<T, 128>, grid, dim3(kStoreThreads), 0, stream)(
       static_cast<const T*>(k), static_cast<const T*>(v), static_cast<unsigned char*>(kc), static_cast<unsigned char*>(vc), ks, vs, slots, p, wide, st::error_word());
   if (e != cudaSuccess) return st::fail_cuda(e, "paged store");
@@ -458,7 +479,7 @@ ST_API int st_paged_store(const void* k, const void* v, void* k_codes, void* v_c
     return st::fail(ST_ERR_INVALID, "paged store: sizes out of range (page 16 to 256, dim 64 or 128)");
   if ((reinterpret_cast<uintptr_t>(k_codes) | reinterpret_cast<uintptr_t>(v_codes)) & 15) return st::fail(ST_ERR_INVALID, "paged store: codes must be 16-byte aligned");
   if (rows == 0) return ST_OK;
-  const PutParams p{k_row, k_head, v_row, v_head, rows, kv_heads, shift, 0, pages};
+  const PutParams p{k_row, k_head, v_row, v_head, rows, pages, kv_heads, shift, 0, 0, 0};
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
   switch (type) {
     case 0: return launch_store<__nv_bfloat16>(k, v, k_codes, v_codes, k_scale, v_scale, slots, p, dim, stream);

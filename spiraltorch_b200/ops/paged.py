@@ -65,21 +65,22 @@ class Step(NamedTuple):
 
 
 def _ints(name: str, t: torch.Tensor, dim: int, dtype=torch.int32) -> None:
-    if t.dtype != dtype or t.dim() != dim or (t.numel() and t.stride(-1) != 1):
+    if t.dtype is not dtype or t.dim() != dim or (t.stride()[-1] != 1 and t.numel() > 0):
         raise ValueError(f"paged: {name} must be {dtype} with {dim} dimension{'s' if dim > 1 else ''} and contiguous, got {t.dtype} {tuple(t.shape)}")
 
 
 def _check_pages(p: Pages) -> tuple:
     k, v, ks, vs = p
-    if k.dim() != 4 or k.shape != v.shape or ks.shape != k.shape[:2] or vs.shape != k.shape[:2]:
-        raise ValueError(f"paged: codes {tuple(k.shape)}, {tuple(v.shape)} and scales {tuple(ks.shape)}, {tuple(vs.shape)} do not belong together")
-    if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn or ks.dtype != torch.float32 or vs.dtype != torch.float32:
+    shape = k.shape
+    if len(shape) != 4 or shape != v.shape or ks.shape != shape[:2] or vs.shape != shape[:2]:
+        raise ValueError(f"paged: codes {tuple(shape)}, {tuple(v.shape)} and scales {tuple(ks.shape)}, {tuple(vs.shape)} do not belong together")
+    if k.dtype is not torch.float8_e4m3fn or v.dtype is not torch.float8_e4m3fn or ks.dtype is not torch.float32 or vs.dtype is not torch.float32:
         raise ValueError("paged: codes must be float8_e4m3fn and scales float32")
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError("paged: codes and scales must be contiguous")
-    if k.shape[2] not in PAGE_SIZES or k.shape[3] not in (64, 128) or k.shape[1] < 1:
-        raise ValueError(f"paged: pages of {k.shape[2]} tokens and heads of {k.shape[3]} are not supported (sizes {PAGE_SIZES}, 64 or 128)")
-    return k.shape
+    if shape[2] not in PAGE_SIZES or shape[3] not in (64, 128) or shape[1] < 1:
+        raise ValueError(f"paged: pages of {shape[2]} tokens and heads of {shape[3]} are not supported (sizes {PAGE_SIZES}, 64 or 128)")
+    return shape
 
 
 @functools.cache
@@ -99,27 +100,26 @@ def plan(lengths: torch.Tensor, added: torch.Tensor, table: torch.Tensor, free: 
     global launch_count
     if page_size not in PAGE_SIZES:
         raise ValueError(f"paged: page size must be one of {PAGE_SIZES}, got {page_size}")
-    for n, t, d in (("lengths", lengths, 1), ("added", added, 1), ("table", table, 2), ("free", free, 1), ("free_count", free_count, 1)):
-        _ints(n, t, d)
+    _ints("lengths", lengths, 1)
+    _ints("added", added, 1)
+    _ints("table", table, 2)
+    _ints("free", free, 1)
+    _ints("free_count", free_count, 1)
     B, width = table.shape
     if lengths.shape[0] != B or added.shape[0] != B or free_count.shape[0] != 1 or rows < 0:
         raise ValueError(f"paged: lengths {tuple(lengths.shape)}, added {tuple(added.shape)}, table {tuple(table.shape)}, "
                          f"free_count {tuple(free_count.shape)} and {rows} rows do not belong together")
-    dev = lengths.device
     if not native.use_native(lengths):
         return _plan_reference(lengths, added, table, free, free_count, page_size, rows)
     index = native.require_cuda("paged.plan", lengths, added, table, free, free_count)
     if B > _max_sequences():
         raise ValueError(f"paged.plan: {B} sequences, at most {_max_sequences()}")
-    small = torch.empty(2 * B + 2, dtype=torch.int32, device=dev)
-    positions = torch.empty(rows, dtype=torch.int32, device=dev)
-    slots = torch.empty(rows, dtype=torch.int64, device=dev)
-    step = Step(small[:B + 1], positions, slots, small[B + 1:2 * B + 1], small[2 * B + 1:])
-    base = small.data_ptr()
+    step = Step(free_count.new_empty(B + 1), free_count.new_empty(rows), free_count.new_empty(rows, dtype=torch.int64), free_count.new_empty(B),
+                torch.empty_like(free_count))
     with native.on_device(index):
-        st = native.entry("st_paged_plan", "pppqippiiiqppppp" + "p")(
+        st = native.entry("st_paged_plan", "pppqippiiiqpppppp")(
             lengths.data_ptr(), added.data_ptr(), table.data_ptr(), table.stride(0), width, free.data_ptr(), free_count.data_ptr(), free.shape[0],
-            page_size, B, rows, base, positions.data_ptr(), slots.data_ptr(), base + 4 * (B + 1), base + 4 * (2 * B + 1), native.raw_stream(index))
+            page_size, B, rows, *(t.data_ptr() for t in step), native.raw_stream(index))
     native.check(st, "st_paged_plan")
     launch_count += 1
     return step
@@ -194,7 +194,7 @@ def store(k: torch.Tensor, v: torch.Tensor, pages: Pages, slots: torch.Tensor) -
         raise ValueError(f"paged.store: k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} do not match pages of {H} heads of {D}")
     if k.dtype not in _TYPES:
         raise ValueError(f"paged.store: bf16, fp16 and fp32 rows, got {k.dtype}")
-    if k.stride(2) != 1 or v.stride(2) != 1:
+    if k.stride()[2] != 1 or v.stride()[2] != 1:
         raise ValueError("paged.store: head elements must be contiguous")
     _ints("slots", slots, 1, torch.int64)
     if slots.shape[0] != k.shape[0]:
@@ -205,7 +205,7 @@ def store(k: torch.Tensor, v: torch.Tensor, pages: Pages, slots: torch.Tensor) -
     with native.on_device(index):
         st = native.entry("st_paged_store", "pppppppqiiiqqqqqip")(
             k.data_ptr(), v.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), slots.data_ptr(),
-            k.shape[0], H, D, page, P, k.stride(0), k.stride(1), v.stride(0), v.stride(1), _TYPES[k.dtype], native.raw_stream(index))
+            k.shape[0], H, D, page, P, *k.stride()[:2], *v.stride()[:2], _TYPES[k.dtype], native.raw_stream(index))
     native.check(st, "st_paged_store")
     launch_count += 1
 
@@ -268,7 +268,8 @@ def read(pages: Pages, table: torch.Tensor, lengths: torch.Tensor, max_length: i
     if not native.use_native(pages.k):
         return tuple(_dense_reference(c, s, table, lengths, max_length).to(dtype) for c, s in ((pages.k, pages.k_scale), (pages.v, pages.v_scale)))
     index = native.require_cuda("paged.read", *pages, table, lengths)
-    k, v = (torch.empty((B, max_length, H, D), dtype=dtype, device=pages.k.device) for _ in range(2))
+    k = pages.k_scale.new_empty((B, max_length, H, D), dtype=dtype)
+    v = torch.empty_like(k)
     with native.on_device(index):
         st = native.entry("st_paged_read", "ppppppqiiiiiiqppip")(
             pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), table.data_ptr(), lengths.data_ptr(),
@@ -316,7 +317,7 @@ def attention(q: torch.Tensor, pages: Pages, table: torch.Tensor, starts: torch.
     P, Hk, page, D = _check_pages(pages)
     if q.dim() != 3 or q.shape[2] != D or q.shape[1] < Hk or q.shape[1] % Hk:
         raise ValueError(f"paged.attention: q {tuple(q.shape)} does not fit pages of {Hk} heads of {D}")
-    if not (q.dtype in (torch.bfloat16, torch.float16) or q.dtype == torch.float32 and not q.is_cuda) or q.stride(2) != 1:
+    if not (q.dtype in (torch.bfloat16, torch.float16) or q.dtype == torch.float32 and not q.is_cuda) or q.stride()[2] != 1:
         raise ValueError("paged.attention: q must be bf16 or fp16 (on the CPU also fp32) with contiguous head elements")
     _ints("table", table, 2)
     _ints("starts", starts, 1)
@@ -343,13 +344,13 @@ def attention(q: torch.Tensor, pages: Pages, table: torch.Tensor, starts: torch.
             o = out
         return (o, lse.float()) if return_lse else o
     index = native.require_cuda("paged.attention", q, *pages, table, starts, lengths, out)
-    o = torch.empty((rows, H, D), dtype=q.dtype, device=q.device) if out is None else out
-    lse = torch.empty((rows, H), dtype=torch.float32, device=q.device) if return_lse else None
+    o = (torch.empty_like(q) if q.is_contiguous() else q.new_empty((rows, H, D))) if out is None else out
+    lse = pages.k_scale.new_empty((rows, H)) if return_lse else None
     with native.on_device(index):
-        work = torch.empty(_workspace(max_queries, H, Hk, D, index), dtype=torch.float32, device=q.device)
-        st = native.entry("st_paged_attention", "ppppppppppp" + "qqqqqqq" + "iiiiiii" + "f" + "iiip")(
+        work = pages.k_scale.new_empty(_workspace(max_queries, H, Hk, D, index))
+        st = native.entry("st_paged_attention", "pppppppppppqqqqqqqiiiiiiifiiip")(
             q.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), table.data_ptr(), starts.data_ptr(),
-            lengths.data_ptr(), o.data_ptr(), native.address(lse), work.data_ptr(), q.stride(0), q.stride(1), o.stride(0), o.stride(1), table.stride(0), P, rows,
+            lengths.data_ptr(), o.data_ptr(), native.address(lse), work.data_ptr(), *q.stride()[:2], *o.stride()[:2], table.stride(0), P, rows,
             width, page, B, H, Hk, D, max_queries, scale, int(causal), int(out is None), int(q.dtype == torch.float16), native.raw_stream(index))
     native.check(st, "st_paged_attention")
     launch_count += 2

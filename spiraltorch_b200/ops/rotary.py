@@ -75,7 +75,7 @@ def rotary_reference(x: torch.Tensor, positions: torch.Tensor, freq: torch.Tenso
 
 def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
     """``x`` as ``[tokens, heads, dim]`` without a copy of a strided view that has such a form."""
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
+    if x.stride()[-1] != 1 and x.shape[-1] > 1:
         raise ValueError(f"rotary: {name} must have contiguous head elements")
     return x if x.dim() == 3 else x.flatten(0, -3) if x.dim() > 3 else x.unsqueeze(0)
 
@@ -87,7 +87,7 @@ def _check(q, k, positions, freq) -> None:
         raise ValueError(f"rotary: positions {tuple(positions.shape)} do not match q {tuple(q.shape)} without heads and head elements")
     if positions.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"rotary: positions must be int32 or int64, got {positions.dtype}")
-    if k is not None and (k.dtype != q.dtype or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]):
+    if k is not None and (k.dtype != q.dtype or k.shape[:-2] != positions.shape or k.shape[-1] != q.shape[-1]):
         raise ValueError(f"rotary: k {tuple(k.shape)} {k.dtype} does not match q {tuple(q.shape)} {q.dtype}")
     if freq.dtype != torch.float64 or freq.dim() != 1 or not freq.is_contiguous():
         raise ValueError("rotary: freq must be a contiguous fp64 vector, as frequencies() gives")
@@ -108,20 +108,23 @@ def _launch(q, k, qo, ko, positions, freq, interleaved, magnitude, backward) -> 
     with native.on_device(index):
         st = native.entry("st_rotary", "pppppipqiiiiqqqqqqqqifiip")(
             q.data_ptr(), kk.data_ptr(), qo.data_ptr(), kko.data_ptr(), positions.data_ptr(), int(positions.dtype == torch.int64),
-            freq.data_ptr(), q.shape[0], h, hk, q.shape[2], freq.numel(), q.stride(0), q.stride(1), kk.stride(0), kk.stride(1),
-            qo.stride(0), qo.stride(1), kko.stride(0), kko.stride(1), int(interleaved), magnitude, int(backward), _TYPES[q.dtype],
-            native.raw_stream(index))
+            freq.data_ptr(), q.shape[0], h, hk, q.shape[2], freq.numel(), *q.stride()[:2], *kk.stride()[:2], *qo.stride()[:2], *kko.stride()[:2],
+            int(interleaved), magnitude, int(backward), _TYPES[q.dtype], native.raw_stream(index))
     native.check(st, "st_rotary")
     launch_count += 1
+
+
+def _like(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
 
 
 def _apply(q, k, positions, freq, interleaved, magnitude, backward):
     if not native.use_native(q):
         return tuple(None if x is None else rotary_reference(x, positions, freq, interleaved, magnitude, backward) for x in (q, k))
-    out = [None if x is None else torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k)]
-    views = [None if x is None else _rows(x, n) for x, n in ((q, "q"), (k, "k"), (out[0], "q"), (out[1], "k"))]
-    _launch(*views, positions.contiguous(), freq, interleaved, magnitude, backward)
-    return tuple(out)
+    qo, ko = _like(q), None if k is None else _like(k)
+    _launch(_rows(q, "q"), None if k is None else _rows(k, "k"), _rows(qo, "q"), None if k is None else _rows(ko, "k"), positions.contiguous(), freq,
+            interleaved, magnitude, backward)
+    return qo, ko
 
 
 class _RotaryFn(torch.autograd.Function):
