@@ -6,19 +6,21 @@
 // heads of one key head) it is bound by reading the cache once.
 //
 // Work.  The rows of a sequence that share a key head are its n tokens times the G query heads of the group; N = 8, 16 or 32 of them
-// are an item together with one (sequence, key head), and 64 keys of an item are a unit.  All units of the call are numbered through and
+// are an item together with one (sequence, key head), and 128 keys of an item are a unit.  All units of the call are numbered through and
 // every block takes an equal run of them, whatever the lengths are: the split needs nothing from the host but the shapes, so a captured
 // launch stays right while the sequences grow, and one long sequence fills the chip as well as many short ones.  Each block finds its run
 // by a prefix sum over the sequences.  Where a run ends inside an item, the block leaves (maximum, sum, output) in the workspace,
 // and a second kernel joins the parts of such items in their order, so results do not depend on timing.
 //
-// Inner loop.  A warp takes 16 keys of a unit at a time straight from global memory to registers: each thread loads 16 bytes of
-// contiguous codes, and the order of the head elements inside the matrix instructions is chosen so that those bytes are its own
-// fragments (keys as the rows of A, S^T = K Q^T; values transposed by byte permutes, O^T = V^T P^T), converted to fp16, which holds e4m3
-// exactly.  So nothing passes through shared memory, and the queries are the N side of m16n8k16, which wastes nothing from 8 rows on.
-// Queries are scaled by a power of two per row so that fp16 holds bf16's bits too.  The softmax runs over x + b instead of x
-// (b: the page's value exponent): the weights exp2(x + b - max) are those that multiply the codes, at most 1, and fp16 keeps 11 bits
-// of them; the sum takes exp2(-b) back out.
+// Inner loop.  A warp takes 32 keys of a unit at a time through a ring of its own in shared memory, two slots of 8 KB (for heads of 128) that
+// one lane fills by tiled copies while the warp works on the other: nothing but a barrier per slot, no registers, and 96 KB in flight per SM.
+// The order of the head elements inside the matrix instructions is chosen so that 16 contiguous bytes of a key are a thread's
+// fragments (keys as the rows of A, S^T = K Q^T; values transposed by byte permutes, O^T = V^T P^T), the order of the keys so that no two
+// lanes' loads from the swizzled rows meet in a bank (key_of below).  Codes become fp16, which holds e4m3 exactly, and the queries are the
+// N side of m16n8k16, which wastes nothing from 8 rows on.  (m16n8k32 on the codes themselves, with a query as the sum of two e4m3 values, is
+// no gain: it takes more instructions than the conversion, 78 us against 75 on the case of 64 sequences.)  Queries are scaled by a power of two
+// per row so that fp16 holds bf16's bits too.  The softmax runs over x + b instead of x (b: the page's value exponent): the weights exp2(x + b - max) are those that
+// multiply the codes, at most 1, and fp16 keeps 11 bits of them; the sum takes exp2(-b) back out.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "../common/host.h"
@@ -28,7 +30,7 @@
 namespace {
 using st::chain_begin;
 
-constexpr int kWarps = 4, kThreads = 32 * kWarps, kTile = 16 * kWarps;      // keys of a unit
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kTile = 32 * kWarps;      // keys of a unit
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnParams {
@@ -42,7 +44,7 @@ struct AttnParams {
   long long rows;      // of q and out
   int width, shift, B, heads, kv_heads, group;
   float scale;
-  int causal, zero_tail;
+  int causal, zero_tail, wide;      // wide: a page holds 32 keys or more
   unsigned* err;
 };
 
@@ -66,50 +68,70 @@ __device__ __forceinline__ Seq sequence(const AttnParams& p, int b) {
   return s;
 }
 
-// Units of all sequences, and of those before `want`: the sequence that holds unit `want` and the number of its first one.
+// Where the block's share begins: the sequence that holds a unit, and the number of the sequence's first one.
 struct Found {
   int b;
   long long first;
 };
-template <int N>
-__device__ long long units_in_all(const AttnParams& p, long long* shared) {
-  long long sum = 0;
-  for (int b = threadIdx.x; b < p.B; b += kThreads) sum += sequence<N>(p, b).units;
+__device__ __forceinline__ long long scan_block(long long mine, long long* shared, long long& total) {      // sum of the threads before, and of all
+  long long s = mine;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = sum;
-  __syncthreads();
-  sum = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) sum += shared[w];
-  __syncthreads();
-  return sum;
-}
-template <int N>
-__device__ Found find_unit(const AttnParams& p, long long want, long long* shared, Found* found) {
-  long long before = 0;
-  for (int base = 0; base < p.B; base += kThreads) {
-    const int b = base + threadIdx.x;
-    const long long mine = b < p.B ? sequence<N>(p, b).units : 0;
-    long long s = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, s, o);
-      if ((threadIdx.x & 31) >= o) s += u;
-    }
-    if ((threadIdx.x & 31) == 31) shared[threadIdx.x >> 5] = s;
-    __syncthreads();
-    long long first = before + s - mine;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < (threadIdx.x >> 5)) first += shared[w];
-      before += shared[w];
-    }
-    if (want >= first && want < first + mine) *found = Found{b, first};      // one thread at most
-    __syncthreads();
-    if (want < before) break;
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, s, o);
+    if ((threadIdx.x & 31) >= o) s += u;
   }
-  return *found;
+  __syncthreads();
+  if ((threadIdx.x & 31) == 31) shared[threadIdx.x >> 5] = s;
+  __syncthreads();
+  long long before = s - mine;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < static_cast<int>(threadIdx.x >> 5)) before += shared[w];
+    total += shared[w];
+  }
+  return before;
+}
+// The block's share [u0, u1) of the units, if it has one, and where unit `at_end ? u1 : u0` lies.  Up to a block's threads of sequences are looked at once.
+template <int N>
+__device__ bool find_share(const AttnParams& p, int block, int most_runs, bool at_end, long long* shared, Found* found, long long& all, int& runs, long long& u0, long long& u1,
+                           Found& f) {
+  const bool once = p.B <= kThreads;
+  long long mine = 0, total = 0, before = 0;
+  for (int b = threadIdx.x; b < p.B; b += kThreads) mine += sequence<N>(p, b).units;
+  before = scan_block(mine, shared, total);
+  all = total;
+  runs = static_cast<int>(min(static_cast<long long>(most_runs), all));      // none of them empty
+  if (block >= runs) return false;
+  u0 = all * block / runs, u1 = all * (block + 1) / runs;
+  const long long want = at_end ? u1 : u0;
+  if (want >= all) return false;
+  if (once) {
+    if (want >= before && want < before + mine) *found = Found{static_cast<int>(threadIdx.x), before};      // one thread
+  } else {
+    long long base = 0;
+    for (int b0 = 0; b0 < p.B && want >= base; b0 += kThreads) {
+      const int b = b0 + threadIdx.x;
+      mine = b < p.B ? sequence<N>(p, b).units : 0;
+      before = base + scan_block(mine, shared, total);
+      if (want >= before && want < before + mine) *found = Found{b, before};
+      base += total;
+    }
+  }
+  __syncthreads();
+  f = *found;
+  return true;
+}
+// a / b and a % b, by 32-bit arithmetic where both fit.
+__device__ __forceinline__ long long divide(long long a, int b, int& rest) {
+  if (a >> 32 == 0) {
+    const unsigned q = static_cast<unsigned>(a) / static_cast<unsigned>(b);
+    rest = static_cast<int>(static_cast<unsigned>(a) - q * b);
+    return q;
+  }
+  const long long q = a / b;
+  rest = static_cast<int>(a - q * b);
+  return q;
 }
 
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t pair) {      // of the low 16 bits
@@ -132,16 +154,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint4 load_stream(const unsigned char* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 load_stream8(const unsigned char* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
 // Bytes of e4m3 that are no number, as 0x80 in their places.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
@@ -161,64 +173,112 @@ template <typename T> __device__ __forceinline__ T from_f(float x);
 template <> __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
 
-// 16 keys of one head: codes of keys and values as this thread's fragments take them, and the page's exponents.
-template <int D>
-struct Chunk {
-  static constexpr int W = D / 16;      // words per key row part / value row part
-  uint32_t k[2][W], v[4][D / 32];
-  float ks;
-  int ve;
+// A piece: 16 keys of one head.  What its page says of it:
+struct Piece {
+  float ks;      // the keys' scale
+  int ve;        // the values' exponent
   bool valid;
 };
+// One lane's share of the page numbers and scales of the warp's next 32 pieces.
+struct PieceList {
+  int page;      // -1: nothing there
+  float ks;
+  int ve;
+};
+
+// A slot of a warp's ring: 32 keys and their values, as the copies leave them: lines of 128 bytes (a token, or two of 64 elements) whose 16-byte
+// parts are swizzled by the line's number.
+template <int D>
+struct Slot {
+  unsigned char k[2][16 * D], v[2][16 * D];
+};
+// The key of a piece that stands at row g (0..7) of a matrix fragment, and how far behind it that of row g + 8 is.  A quarter warp's 16-byte loads of
+// keys are rows (2i, 2i + 1) with parts 0..3 or 4..7; its loads of values rows 0, 2, 4, 6 (or 1, 3, 5, 7) with two neighbouring parts: both touch
+// all eight parts of the swizzled lines once.
+template <int D>
+__device__ __forceinline__ int key_of(int g) {
+  return D == 128 ? (g & 1 ? g ^ 4 : g) : 4 * (g >> 1) + (g & 1);
+}
+template <int D>
+constexpr int kSecond = D == 128 ? 8 : 2;
+// Byte of element 16 * part of token `key` of a piece.
+template <int D>
+__device__ __forceinline__ int at_part(int key, int part) {
+  if constexpr (D == 128) return key * 128 + ((part ^ (key & 7)) << 4);
+  return (key >> 1) * 128 + (((4 * (key & 1) + part) ^ (key >> 1 & 7)) << 4);
+}
 
 template <int D, int NT>
 struct Shared {
   static constexpr int N = 8 * NT;
   static constexpr int OUT_ROW = D + 8;
+  union {      // a warp's ring, then its outputs; a multiple of 1024 bytes, as the swizzle counts lines from there
+    Slot<D> ring[2];
+    float out[N][OUT_ROW];
+  } w[kWarps];
   uint2 q[NT][D / 16][32];
-  float out[kWarps][N][OUT_ROW];
+  unsigned long long full[kWarps][2];      // barrier of each slot
   float m[kWarps][N], l[kWarps][N], mx[N], inv[N];
   float factor[N];
   int limit[N];
   long long sums[kWarps];
   Found found;
+  int abort;
+  static_assert(sizeof(w[0]) % 1024 == 0, "slots must start on 1024 bytes");
 };
 
-template <int D>
-__device__ __forceinline__ void load_chunk(Chunk<D>& c, const AttnParams& p, const int* table, int key0, int keys, int h, int g, int q4) {
-  c.valid = key0 < keys;
-  c.ks = 0.0f;
-  c.ve = 0;
-  if (!c.valid) return;
-  const long long page = table[key0 >> p.shift];
-  if (page < 0 || page >= p.pages) {
-    if ((threadIdx.x & 31) == 0) st::report_error(p.err, st::ERR_BOUNDS, 0x7004);
-    c.valid = false;
-    return;
-  }
-  const long long at = page * p.kv_heads + h;
-  const long long base = ((at << p.shift) + (key0 & ((1 << p.shift) - 1))) * D;
-  const unsigned char *kp = p.kc + base, *vp = p.vc + base;
-#pragma unroll
-  for (int r = 0; r < 2; ++r)
-#pragma unroll
-    for (int j = 0; j < D / 64; ++j) {
-      const uint4 x = load_stream(kp + (g + 8 * r) * D + 64 * j + 16 * q4);
-      c.k[r][4 * j] = x.x, c.k[r][4 * j + 1] = x.y, c.k[r][4 * j + 2] = x.z, c.k[r][4 * j + 3] = x.w;
-    }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const unsigned char* row = vp + (2 * q4 + (i & 1) + 8 * (i >> 1)) * D + g * (D / 8);
-    if constexpr (D == 128) {
-      const uint4 x = load_stream(row);
-      c.v[i][0] = x.x, c.v[i][1] = x.y, c.v[i][2] = x.z, c.v[i][3] = x.w;
+// Lane i: piece 2 * (first + i / 2) + i % 2 of the warp, whose key is key0 + (first + i / 2) * kTile + 16 * (i % 2).
+__device__ __forceinline__ PieceList list_pieces(const AttnParams& p, const int* table, int key0, int first, int keys, int h) {
+  const int lane = threadIdx.x & 31;
+  const long long key = key0 + static_cast<long long>(first + lane / 2) * kTile + 16 * (lane & 1);
+  PieceList l{-1, 0.0f, 0};
+  if (key < keys) {
+    const int page = table[key >> p.shift];
+    if (page < 0 || page >= p.pages) {
+      st::report_error(p.err, st::ERR_BOUNDS, 0x7004);
     } else {
-      const uint2 x = load_stream8(row);
-      c.v[i][0] = x.x, c.v[i][1] = x.y;
+      const long long at = static_cast<long long>(page) * p.kv_heads + h;
+      l.page = page;
+      l.ks = p.ks[at];
+      l.ve = st::scale_exponent(p.vs[at]);
     }
   }
-  c.ks = p.ks[at];
-  c.ve = st::scale_exponent(p.vs[at]);
+  return l;
+}
+
+// Starts the copies of the 32 keys from key0 on, whose pieces `from` holds at lanes index and index + 1, into a slot.
+template <int D>
+__device__ __forceinline__ void copy_keys(Slot<D>& slot, uint32_t bar, Piece (&c)[2], const AttnParams& p, const CUtensorMap* km, const CUtensorMap* vm, const PieceList& from,
+                                          int index, int key0, int h) {
+  const int page = __shfl_sync(0xffffffffu, from.page, index), lane = threadIdx.x & 31;
+  c[0] = Piece{__shfl_sync(0xffffffffu, from.ks, index), __shfl_sync(0xffffffffu, from.ve, index), page >= 0};
+  const int mask = (1 << p.shift) - 1;
+  if (p.wide) {      // one page, one copy of each; what lies behind the last key is masked
+    c[1] = c[0];
+    if (lane == 0) {
+      st::mbar_arrive_expect_tx(bar, page >= 0 ? sizeof(Slot<D>) : 0);
+      if (page >= 0) {
+        const int line = static_cast<int>((((static_cast<long long>(page) * p.kv_heads + h) << p.shift) + (key0 & mask)) * D / 128);
+        st::tma_load_2d(st::smem_u32(slot.k), km, bar, 0, line);
+        st::tma_load_2d(st::smem_u32(slot.v), vm, bar, 0, line);
+      }
+    }
+  } else {           // pages of 16
+    const int page2 = __shfl_sync(0xffffffffu, from.page, index + 1);
+    c[1] = Piece{__shfl_sync(0xffffffffu, from.ks, index + 1), __shfl_sync(0xffffffffu, from.ve, index + 1), page2 >= 0};
+    if (lane == 0) {
+      st::mbar_arrive_expect_tx(bar, ((page >= 0) + (page2 >= 0)) * static_cast<int>(sizeof(Slot<D>) / 2));
+      const int lines = 16 * D / 128;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int pg = j == 0 ? page : page2;
+        if (pg < 0) continue;
+        const int line = static_cast<int>((static_cast<long long>(pg) * p.kv_heads + h) * lines);
+        st::tma_load_2d(st::smem_u32(slot.k[j]), km, bar, 0, line);
+        st::tma_load_2d(st::smem_u32(slot.v[j]), vm, bar, 0, line);
+      }
+    }
+  }
 }
 
 template <int D, int NT>
@@ -227,109 +287,151 @@ struct Running {
   float m[NT][2], l[NT][2];
 };
 
-// One chunk of 16 keys: scores, running maximum and sum, weights times values.
-template <int D, int NT>
-__device__ __forceinline__ void process(Chunk<D>& c, Running<D, NT>& st_, const Shared<D, NT>& sh, const uint2 (&qreg)[D / 16], int key0, int keys, int limit_min, int g, int q4) {
-  float s[NT][4];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+// KS pieces of 16 keys: scores, running maximum and sum, weights times values.
+template <int D, int NT, int KS>
+__device__ __forceinline__ void process(const Slot<D>& slot, int piece0, const Piece (&piece)[KS], Running<D, NT>& run, const Shared<D, NT>& sh, const uint2 (&qreg)[D / 16],
+                                        const float (&freg)[2], int key0, int keys, int limit_min, int g, int q4) {
+  constexpr int KW = D / 16, VW = D / 32;      // words of a key row's and a value row's part
   const int lane = threadIdx.x & 31;
+  float s[KS][NT][4];
 #pragma unroll
-  for (int k = 0; k < D / 16; ++k) {
-    const uint32_t a0 = e4m3x2_to_f16x2(c.k[0][k]), a1 = e4m3x2_to_f16x2(c.k[1][k]), a2 = e4m3x2_hi_to_f16x2(c.k[0][k]), a3 = e4m3x2_hi_to_f16x2(c.k[1][k]);
+  for (int j = 0; j < KS; ++j) {
+    uint32_t k0[KW], k1[KW];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const uint2 b = NT == 1 ? qreg[k] : sh.q[n][k][lane];
-      mma(s[n], a0, a1, a2, a3, b.x, b.y);
+    for (int i = 0; i < D / 64; ++i) {
+      const uint4 x = *reinterpret_cast<const uint4*>(slot.k[piece0 + j] + at_part<D>(key_of<D>(g), 4 * i + q4));
+      const uint4 y = *reinterpret_cast<const uint4*>(slot.k[piece0 + j] + at_part<D>(key_of<D>(g) + kSecond<D>, 4 * i + q4));
+      k0[4 * i] = x.x, k0[4 * i + 1] = x.y, k0[4 * i + 2] = x.z, k0[4 * i + 3] = x.w;
+      k1[4 * i] = y.x, k1[4 * i + 1] = y.y, k1[4 * i + 2] = y.z, k1[4 * i + 3] = y.w;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[j][n][0] = s[j][n][1] = s[j][n][2] = s[j][n][3] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KW; ++k) {
+      const uint32_t a0 = e4m3x2_to_f16x2(k0[k]), a1 = e4m3x2_to_f16x2(k1[k]), a2 = e4m3x2_hi_to_f16x2(k0[k]), a3 = e4m3x2_hi_to_f16x2(k1[k]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const uint2 b = NT == 1 ? qreg[k] : sh.q[n][k][lane];
+        mma(s[j][n], a0, a1, a2, a3, b.x, b.y);
+      }
     }
   }
-  const bool edge = key0 + 16 > limit_min;      // some row does not see some of these keys
-  const float ve = static_cast<float>(c.ve), take = st::exp2_int(-c.ve);
-  uint32_t pw[NT][2];
+  bool edge = key0 + 16 * KS > limit_min;      // some row does not see some of these keys
+#pragma unroll
+  for (int j = 0; j < KS; ++j) edge = edge || !piece[j].valid;
+  uint32_t pw[KS][NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int r0 = 8 * n + 2 * q4;
-    const float f0 = sh.factor[r0] * c.ks, f1 = sh.factor[r0 + 1] * c.ks;
-    float x0 = fmaf(s[n][0], f0, ve), x1 = fmaf(s[n][1], f1, ve), x2 = fmaf(s[n][2], f0, ve), x3 = fmaf(s[n][3], f1, ve);
-    if (edge) {
-      const int l0 = sh.limit[r0], l1 = sh.limit[r0 + 1];
-      if (key0 + g >= l0) x0 = -INFINITY;
-      if (key0 + g >= l1) x1 = -INFINITY;
-      if (key0 + g + 8 >= l0) x2 = -INFINITY;
-      if (key0 + g + 8 >= l1) x3 = -INFINITY;
+    const float f0 = NT == 1 ? freg[0] : sh.factor[r0], f1 = NT == 1 ? freg[1] : sh.factor[r0 + 1];
+    float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < KS; ++j) {
+      const float a0 = f0 * piece[j].ks, a1 = f1 * piece[j].ks, ve = static_cast<float>(piece[j].ve);
+      float (&x)[4] = s[j][n];
+      x[0] = fmaf(x[0], a0, ve), x[1] = fmaf(x[1], a1, ve), x[2] = fmaf(x[2], a0, ve), x[3] = fmaf(x[3], a1, ve);
+      if (edge) {
+        const int key = key0 + 16 * j + key_of<D>(g), l0 = piece[j].valid ? sh.limit[r0] : 0, l1 = piece[j].valid ? sh.limit[r0 + 1] : 0;
+        if (key >= l0) x[0] = -INFINITY;
+        if (key >= l1) x[1] = -INFINITY;
+        if (key + kSecond<D> >= l0) x[2] = -INFINITY;
+        if (key + kSecond<D> >= l1) x[3] = -INFINITY;
+      }
+      m0 = st::max3(m0, x[0], x[2]), m1 = st::max3(m1, x[1], x[3]);
     }
-    float m0 = fmaxf(x0, x2), m1 = fmaxf(x1, x3);
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) {
       m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
       m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
     }
-    m0 = fmaxf(m0, st_.m[n][0]), m1 = fmaxf(m1, st_.m[n][1]);
-    if (__any_sync(0xffffffffu, m0 > st_.m[n][0] || m1 > st_.m[n][1])) {
-      const float a0 = m0 > st_.m[n][0] ? exp2f(st_.m[n][0] - m0) : 1.0f, a1 = m1 > st_.m[n][1] ? exp2f(st_.m[n][1] - m1) : 1.0f;
-      st_.m[n][0] = m0, st_.m[n][1] = m1;
-      st_.l[n][0] *= a0, st_.l[n][1] *= a1;
+    m0 = fmaxf(m0, run.m[n][0]), m1 = fmaxf(m1, run.m[n][1]);
+    if (__any_sync(0xffffffffu, m0 > run.m[n][0] || m1 > run.m[n][1])) {
+      const float a0 = m0 > run.m[n][0] ? st::exp2_ftz(run.m[n][0] - m0) : 1.0f, a1 = m1 > run.m[n][1] ? st::exp2_ftz(run.m[n][1] - m1) : 1.0f;
+      run.m[n][0] = m0, run.m[n][1] = m1;
+      run.l[n][0] *= a0, run.l[n][1] *= a1;
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) st_.o[i][n][0] *= a0, st_.o[i][n][1] *= a1, st_.o[i][n][2] *= a0, st_.o[i][n][3] *= a1;
+      for (int i = 0; i < D / 16; ++i) run.o[i][n][0] *= a0, run.o[i][n][1] *= a1, run.o[i][n][2] *= a0, run.o[i][n][3] *= a1;
     }
     const float z0 = m0 == -INFINITY ? 0.0f : m0, z1 = m1 == -INFINITY ? 0.0f : m1;      // nothing seen so far: weights 0, not NaN
-    const float w0 = exp2f(x0 - z0), w1 = exp2f(x1 - z1), w2 = exp2f(x2 - z0), w3 = exp2f(x3 - z1);
-    st_.l[n][0] = fmaf(w0 + w2, take, st_.l[n][0]);
-    st_.l[n][1] = fmaf(w1 + w3, take, st_.l[n][1]);
-    pw[n][0] = transpose8x8(pack_f16x2(w0, w1));
-    pw[n][1] = transpose8x8(pack_f16x2(w2, w3));
+#pragma unroll
+    for (int j = 0; j < KS; ++j) {
+      const float (&x)[4] = s[j][n];
+      // fp16 ends at 2^-24, so exp2's subnormal results, from 2^-126 on, are 0 anyway
+      const float w0 = st::exp2_ftz(x[0] - z0), w1 = st::exp2_ftz(x[1] - z1), w2 = st::exp2_ftz(x[2] - z0), w3 = st::exp2_ftz(x[3] - z1);
+      const float take = st::exp2_int(-piece[j].ve);
+      run.l[n][0] = fmaf(w0 + w2, take, run.l[n][0]);
+      run.l[n][1] = fmaf(w1 + w3, take, run.l[n][1]);
+      pw[j][n][0] = transpose8x8(pack_f16x2(w0, w1));
+      pw[j][n][1] = transpose8x8(pack_f16x2(w2, w3));
+    }
   }
-  if (edge) {
-    // what lies behind the end is no value; a value that is no number counts only for the rows that see it
-    uint32_t some = 0;
+#pragma unroll
+  for (int j = 0; j < KS; ++j) {
+    uint32_t v[4][VW];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const bool behind = key0 + 2 * q4 + (i & 1) + 8 * (i >> 1) >= keys;
-#pragma unroll
-      for (int w = 0; w < D / 32; ++w) {
-        if (behind) c.v[i][w] = 0;
-        some |= nan_bytes(c.v[i][w]);
+      const int key = key_of<D>(2 * q4 + (i & 1)) + kSecond<D> * (i >> 1);
+      if constexpr (D == 128) {
+        const uint4 x = *reinterpret_cast<const uint4*>(slot.v[piece0 + j] + at_part<D>(key, g));
+        v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(slot.v[piece0 + j] + at_part<D>(key, g >> 1) + 8 * (g & 1));
+        v[i][0] = x.x, v[i][1] = x.y;
       }
     }
-    if (__any_sync(0xffffffffu, some != 0)) {
-      uint32_t bad[4];      // a bit per element of the thread's part of a key's row
+    if (edge) {
+      // what lies behind the end is no value; a value that is no number counts only for the rows that see it
+      const int first = key0 + 16 * j;
+      uint32_t some = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        bad[i] = 0;
+        const bool behind = !piece[j].valid || first + key_of<D>(2 * q4 + (i & 1)) + kSecond<D> * (i >> 1) >= keys;
 #pragma unroll
-        for (int w = 0; w < D / 32; ++w) {
-          const uint32_t nb = nan_bytes(c.v[i][w]);
-          bad[i] |= ((nb >> 7 & 1) | (nb >> 14 & 2) | (nb >> 21 & 4) | (nb >> 28 & 8)) << (4 * w);
-          c.v[i][w] &= ~((nb >> 7) * 255u);
+        for (int w = 0; w < VW; ++w) {
+          if (behind) v[i][w] = 0;
+          some |= nan_bytes(v[i][w]);
         }
       }
-#pragma unroll
-      for (int src = 0; src < 4; ++src)
+      if (__any_sync(0xffffffffu, some != 0)) {
+        uint32_t bad[4];      // a bit per element of the thread's part of a key's row
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t bits = __shfl_sync(0xffffffffu, bad[i], (lane & ~3) | src);
-          const int key = key0 + 2 * src + (i & 1) + 8 * (i >> 1);
+          bad[i] = 0;
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-              if (bits && key < sh.limit[8 * n + 2 * q4 + r])
-#pragma unroll
-                for (int d = 0; d < D / 16; ++d) {
-                  if (bits >> (2 * d) & 1) st_.o[d][n][r] = NAN;
-                  if (bits >> (2 * d + 1) & 1) st_.o[d][n][2 + r] = NAN;
-                }
+          for (int w = 0; w < VW; ++w) {
+            const uint32_t nb = nan_bytes(v[i][w]);
+            bad[i] |= ((nb >> 7 & 1) | (nb >> 14 & 2) | (nb >> 21 & 4) | (nb >> 28 & 8)) << (4 * w);
+            v[i][w] &= ~((nb >> 7) * 255u);
+          }
         }
+#pragma unroll 1
+        for (int src = 0; src < 4; ++src)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t bits = __shfl_sync(0xffffffffu, bad[i], (lane & ~3) | src);
+            const int key = first + key_of<D>(2 * src + (i & 1)) + kSecond<D> * (i >> 1);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int r = 0; r < 2; ++r)
+                if (bits && key < sh.limit[8 * n + 2 * q4 + r])
+#pragma unroll
+                  for (int d = 0; d < D / 16; ++d) {
+                    if (bits >> (2 * d) & 1) run.o[d][n][r] = NAN;
+                    if (bits >> (2 * d + 1) & 1) run.o[d][n][2 + r] = NAN;
+                  }
+          }
+      }
     }
-  }
 #pragma unroll
-  for (int d = 0; d < D / 16; ++d) {
-    const int w = d / 2;
-    const uint32_t sel = d & 1 ? 0x7362 : 0x5140;
-    const uint32_t lo = __byte_perm(c.v[0][w], c.v[1][w], sel), hi = __byte_perm(c.v[2][w], c.v[3][w], sel);
-    const uint32_t a0 = e4m3x2_to_f16x2(lo), a1 = e4m3x2_hi_to_f16x2(lo), a2 = e4m3x2_to_f16x2(hi), a3 = e4m3x2_hi_to_f16x2(hi);
+    for (int d = 0; d < D / 16; ++d) {
+      const int w = d / 2;
+      const uint32_t sel = d & 1 ? 0x7362 : 0x5140;
+      const uint32_t lo = __byte_perm(v[0][w], v[1][w], sel), hi = __byte_perm(v[2][w], v[3][w], sel);
+      const uint32_t a0 = e4m3x2_to_f16x2(lo), a1 = e4m3x2_hi_to_f16x2(lo), a2 = e4m3x2_to_f16x2(hi), a3 = e4m3x2_hi_to_f16x2(hi);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) mma(st_.o[d][n], a0, a1, a2, a3, pw[n][0], pw[n][1]);
+      for (int n = 0; n < NT; ++n) mma(run.o[d][n], a0, a1, a2, a3, pw[j][n][0], pw[j][n][1]);
+    }
   }
 }
 
@@ -345,11 +447,21 @@ __device__ __forceinline__ int out_at(int d) {
   return (d % PER / 2) * 16 + (d / PER) * 2 + (d & 1);
 }
 
+// Blocks of an SM: by registers (128 to 255 a thread) and 64 KB of rings for heads of 128.
+template <int D, int NT> constexpr int kBlocks = NT == 4 ? 2 : (D == 64 ? 5 : 4) - NT;
+
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
+__global__ void __launch_bounds__(kThreads, kBlocks<D, NT>) paged_attn_kernel(AttnParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   constexpr int N = 8 * NT;
-  extern __shared__ __align__(16) unsigned char raw[];
+  extern __shared__ __align__(1024) unsigned char raw[];
   Shared<D, NT>& sh = *reinterpret_cast<Shared<D, NT>*>(raw);
+  if (threadIdx.x == 0) {
+    st::tma_prefetch_desc(&k_map);
+    st::tma_prefetch_desc(&v_map);
+    for (int i = 0; i < 2 * kWarps; ++i) st::mbar_init(st::smem_u32(&sh.full[0][0] + i), 1);
+    st::fence_barrier_init();
+    sh.abort = 0;
+  }
   chain_begin(p.kc, p.vc, p.ks, p.vs, p.table, p.starts, p.lengths);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q4 = lane & 3;
   const T* q = static_cast<const T*>(p.q);
@@ -363,12 +475,14 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
       if (p.lse != nullptr && e % D == 0) p.lse[row * p.heads + e / D] = -INFINITY;
     }
   }
-  const long long all = units_in_all<N>(p, sh.sums);
-  const int runs = static_cast<int>(min(static_cast<long long>(gridDim.x), all));      // none of them empty
-  if (static_cast<int>(blockIdx.x) >= runs) return;
-  const long long u0 = all * blockIdx.x / runs, u1 = all * (blockIdx.x + 1) / runs;
-  Found f = find_unit<N>(p, u0, sh.sums, &sh.found);
+  long long all, u0, u1;
+  int runs;
+  Found f;
+  if (!find_share<N>(p, blockIdx.x, gridDim.x, false, sh.sums, &sh.found, all, runs, u0, u1, f)) return;
   Seq sq = sequence<N>(p, f.b);
+  const uint32_t bar = st::smem_u32(&sh.full[warp][0]);
+  Slot<D>* ring = sh.w[warp].ring;
+  uint32_t turn = 0;      // of the warp's ring: slot turn % 2, for the (turn / 2)-th time
 
   for (long long u = u0; u < u1;) {
     while (u >= f.first + sq.units) {
@@ -376,10 +490,8 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
       sq = sequence<N>(p, ++f.b);
     }
     // unit -> (key head, row block, tile): row blocks of one head next to each other, as they read the same pages
-    const long long in = u - f.first;
-    const int t0 = static_cast<int>(in % sq.tiles);
-    const long long item = in / sq.tiles;
-    const int rb = static_cast<int>(item % sq.row_blocks), h = static_cast<int>(item / sq.row_blocks);
+    int t0, rb;
+    const int h = static_cast<int>(divide(divide(u - f.first, sq.tiles, t0), sq.row_blocks, rb));
     const int t1 = static_cast<int>(min(static_cast<long long>(sq.tiles), t0 + (u1 - u)));
     const int row0 = rb * N, row_end = min(sq.n * p.group, row0 + N);
     const int* table = p.table + f.b * p.table_row;
@@ -387,10 +499,13 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
     const int hidden = p.causal ? sq.n - 1 - row0 / p.group : 0, hidden_last = p.causal ? sq.n - 1 - (row_end - 1) / p.group : 0;
     const int limit_min = max(sq.len - hidden, 0), keys = max(sq.len - hidden_last, 0);
 
-    Chunk<D> next;
-    int key0 = t0 * kTile + warp * 16;
-    load_chunk(next, p, table, key0, min(keys, t1 * kTile), h, g, q4);
-    __syncthreads();      // the item before is done with the shared memory
+    // the warp's pieces: iteration i has the keys from key0 + i * kTile on
+    const int key0 = t0 * kTile + warp * 32, iterations = t1 - t0;
+    PieceList list = list_pieces(p, table, key0, 0, min(keys, t1 * kTile), h), list_next{-1, 0.0f, 0};
+    st::fence_proxy_async_smem();      // outputs of the item before lie where copies go now
+    __syncthreads();
+    Piece coming[2];
+    copy_keys<D>(ring[turn & 1], bar + 8 * (turn & 1), coming, p, &k_map, &v_map, list, 0, key0, h);
     for (int r = warp; r < N; r += kWarps) {
       float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       const int fr = row0 + r;
@@ -423,13 +538,30 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) s.o[d][n][0] = s.o[d][n][1] = s.o[d][n][2] = s.o[d][n][3] = 0.0f;
     }
-    for (int t = t0; t < t1; ++t) {
-      Chunk<D> c = next;
-      const int at = key0;
-      key0 += kTile;
-      load_chunk(next, p, table, key0, min(keys, t1 * kTile), h, g, q4);
-      if (c.valid) process<D, NT>(c, s, sh, qreg, at, keys, limit_min, g, q4);
+    const float freg[2] = {sh.factor[2 * q4], sh.factor[2 * q4 + 1]};
+    for (int i = 0; i < iterations; ++i) {
+      const Piece piece[2] = {coming[0], coming[1]};
+      const int next = i + 1, at = key0 + i * kTile;
+      if ((next & 15) == 8) list_next = list_pieces(p, table, key0, (next & ~15) + 16, min(keys, t1 * kTile), h);
+      if ((next & 15) == 0) list = list_next;
+      __syncwarp();      // every lane is done with the other slot
+      if (next < iterations) copy_keys<D>(ring[(turn + 1) & 1], bar + 8 * ((turn + 1) & 1), coming, p, &k_map, &v_map, list, 2 * next % 32, at + kTile, h);
+      const bool here = st::mbar_wait_warp(bar + 8 * (turn & 1), turn >> 1 & 1, &sh.abort);
+      const Slot<D>& slot = ring[turn & 1];
+      ++turn;
+      if (!here) {
+        if (lane == 0) st::report_error(p.err, st::ERR_MBAR_TIMEOUT, 0x7005);
+      } else if (piece[0].valid || piece[1].valid) {
+        if constexpr (NT <= 2) {
+          process<D, NT, 2>(slot, 0, piece, s, sh, qreg, freg, at, keys, limit_min, g, q4);
+        } else {      // one piece at a time: two do not fit the registers
+          const Piece first[1] = {piece[0]}, second[1] = {piece[1]};
+          if (piece[0].valid) process<D, NT, 1>(slot, 0, first, s, sh, qreg, freg, at, keys, limit_min, g, q4);
+          if (piece[1].valid) process<D, NT, 1>(slot, 1, second, s, sh, qreg, freg, at + 16, keys, limit_min, g, q4);
+        }
+      }
     }
+    __syncwarp();      // the ring becomes room for the outputs
 
     // join the warps
 #pragma unroll
@@ -448,20 +580,20 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
       for (int r = 0; r < 2; ++r) {
         const int row = 8 * n + 2 * q4 + r;
         const float mx = fmaxf(fmaxf(sh.m[0][row], sh.m[1][row]), fmaxf(sh.m[2][row], sh.m[3][row]));
-        a[r] = s.l[n][r] == 0.0f ? 0.0f : exp2f(s.m[n][r] - mx);      // 0: saw nothing; a score that is no number leaves a sum that is none
+        a[r] = s.l[n][r] == 0.0f ? 0.0f : st::exp2_ftz(s.m[n][r] - mx);      // 0: saw nothing; a score that is no number leaves a sum that is none
       }
 #pragma unroll
       for (int d = 0; d < D / 16; ++d)
 #pragma unroll
         for (int r = 0; r < 2; ++r)
-          *reinterpret_cast<float2*>(&sh.out[warp][8 * n + 2 * q4 + r][16 * d + 2 * g]) = make_float2(s.o[d][n][r] * a[r], s.o[d][n][2 + r] * a[r]);
+          *reinterpret_cast<float2*>(&sh.w[warp].out[8 * n + 2 * q4 + r][16 * d + 2 * g]) = make_float2(s.o[d][n][r] * a[r], s.o[d][n][2 + r] * a[r]);
     }
     if (threadIdx.x < N) {
       const int row = threadIdx.x;
       const float mx = fmaxf(fmaxf(sh.m[0][row], sh.m[1][row]), fmaxf(sh.m[2][row], sh.m[3][row]));
       float l = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) l += sh.l[w][row] == 0.0f ? 0.0f : sh.l[w][row] * exp2f(sh.m[w][row] - mx);
+      for (int w = 0; w < kWarps; ++w) l += sh.l[w][row] == 0.0f ? 0.0f : sh.l[w][row] * st::exp2_ftz(sh.m[w][row] - mx);
       sh.mx[row] = mx, sh.inv[row] = l;
     }
     __syncthreads();
@@ -473,7 +605,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(AttnParams p) {
       float2 x = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float2 y = *reinterpret_cast<const float2*>(&sh.out[w][row][at]);
+        const float2 y = *reinterpret_cast<const float2*>(&sh.w[w].out[row][at]);
         x.x += y.x, x.y += y.y;
       }
       const float l = sh.inv[row];
@@ -504,17 +636,15 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(AttnParams p, int 
   __shared__ Found found;
   __shared__ float red[2][kWarps], rows[kWarps][D];
   chain_begin(p.table, p.starts, p.lengths);
-  const long long all = units_in_all<N>(p, sums);
-  const int runs = static_cast<int>(min(static_cast<long long>(most_runs), all)), c = blockIdx.x;
-  if (c + 1 >= runs) return;
-  const long long u0 = all * c / runs, u1 = all * (c + 1) / runs;
-  const Found f = find_unit<N>(p, u1, sums, &found);
+  long long all, u0, u1;
+  int runs, t, rb;
+  const int c = blockIdx.x, r = blockIdx.y;
+  Found f;
+  if (!find_share<N>(p, c, most_runs, true, sums, &found, all, runs, u0, u1, f)) return;
   const Seq sq = sequence<N>(p, f.b);
-  const long long in = u1 - f.first;
-  const int t = static_cast<int>(in % sq.tiles), r = blockIdx.y;
+  const int h = static_cast<int>(divide(divide(u1 - f.first, sq.tiles, t), sq.row_blocks, rb));
   if (t == 0 || u1 - t < u0) return;
-  const long long end = u1 - t + sq.tiles, item = in / sq.tiles;
-  const int rb = static_cast<int>(item % sq.row_blocks), h = static_cast<int>(item / sq.row_blocks);
+  const long long end = u1 - t + sq.tiles;
   const int row0 = rb * N, row_end = min(sq.n * p.group, row0 + N);
   if (r >= row_end - row0) return;
   // block b holds a part if its run begins before the end: all * b / runs < end, which is all * b < end * runs
@@ -536,7 +666,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(AttnParams p, int 
   float l = 0.0f;
   for (int i = threadIdx.x; i < parts; i += kThreads) {
     const float* part = base + (2LL * i + (i == 0 ? 1 : 0)) * kSlot + N * D;
-    const float pl = part[N + r], e = pl == 0.0f ? 0.0f : exp2f(part[r] - m);
+    const float pl = part[N + r], e = pl == 0.0f ? 0.0f : st::exp2_ftz(part[r] - m);
     weight[i] = e;
     l += pl * e;
   }
@@ -578,15 +708,22 @@ int row_tiles(long long max_queries, int group) {
   const long long rows = max_queries * group;
   return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
 }
-int runs_of(int nt) { return st::sm_count() * (nt == 4 ? 2 : 3); }
+int runs_of(int nt, int dim) {
+  return st::sm_count() * (dim == 64 ? nt == 1 ? kBlocks<64, 1> : nt == 2 ? kBlocks<64, 2> : kBlocks<64, 4> : nt == 1 ? kBlocks<128, 1> : nt == 2 ? kBlocks<128, 2> : kBlocks<128, 4>);
+}
 
 template <typename T, int D, int NT>
 int launch(const AttnParams& p, cudaStream_t stream) {
-  const int runs = runs_of(NT);
+  const int runs = runs_of(NT, D);
   constexpr int smem = sizeof(Shared<D, NT>);
+  CUtensorMap maps[2];
+  const uint64_t dims[2] = {128, (static_cast<uint64_t>(p.pages) * p.kv_heads << p.shift) * D / 128}, strides[1] = {128};
+  const uint32_t box[2] = {128, (p.wide ? 32u : 16u) * D / 128};
+  for (int i = 0; i < 2; ++i)
+    if (!st::encode_tmap(&maps[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, i == 0 ? p.kc : p.vc, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return ST_ERR_CUDA;
   auto kernel = paged_attn_kernel<T, D, NT>;
   if (smem > 48 * 1024) ST_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  cudaError_t e = st::chained(kernel, dim3(runs), dim3(kThreads), smem, stream)(p);
+  cudaError_t e = st::chained(kernel, dim3(runs), dim3(kThreads), smem, stream)(p, maps[0], maps[1]);
   if (e != cudaSuccess) return st::fail_cuda(e, "paged attention");
   e = st::chained(paged_join_kernel<T, D, NT>, dim3(runs - 1, 8 * NT), dim3(kThreads), runs * sizeof(float), stream)(p, runs);
   if (e != cudaSuccess) return st::fail_cuda(e, "paged attention: join");
@@ -603,7 +740,7 @@ int dispatch(const AttnParams& p, int dim, int nt, cudaStream_t stream) {
 ST_API long long st_paged_attention_workspace(int max_queries, int heads, int kv_heads, int dim) {
   if (kv_heads < 1 || heads < kv_heads) return 0;
   const int nt = row_tiles(max_queries, heads / kv_heads);
-  return 2LL * runs_of(nt) * 8 * nt * (dim + 2);
+  return 2LL * runs_of(nt, dim) * 8 * nt * (dim + 2);
 }
 
 // q, out [rows, heads, dim] (dim contiguous, strides in elements): row starts[b] + i is the i-th of the newest tokens of sequence b, whose keys and values,
@@ -614,14 +751,14 @@ ST_API int st_paged_attention(const void* q, const void* k_codes, const void* v_
                               long long table_row, long long pages, long long rows, int width, int page_size, int B, int heads, int kv_heads, int dim, int max_queries, float scale,
                               int causal, int zero_tail, int type, void* stream_v) {
   const int shift = st::page_shift(page_size);
-  if (shift < 0 || B < 0 || rows < 0 || rows > 2147483647LL || width < 0 || (static_cast<long long>(width) << shift) > 2147483647LL || kv_heads < 1 || heads < kv_heads ||
-      heads % kv_heads || (dim != 64 && dim != 128) || pages < 0 || max_queries < 1 || (type != 0 && type != 1) || rows * (heads / kv_heads) > 2147483647LL)
-    return st::fail(ST_ERR_INVALID, "paged attention: sizes out of range (page 16 to 256, dim 64 or 128, heads a multiple of kv_heads)");
+  if (shift < 0 || B < 0 || rows < 0 || rows > 2147483647LL || width < 0 || (static_cast<long long>(width) << shift) > 2147480000LL || kv_heads < 1 || heads < kv_heads ||
+      heads % kv_heads || (dim != 64 && dim != 128) || pages < 1 || (pages * kv_heads << shift) > 2147483647LL || max_queries < 1 || (type != 0 && type != 1) || rows * (heads / kv_heads) > 2147483647LL)
+    return st::fail(ST_ERR_INVALID, "paged attention: sizes out of range (page 16 to 256, dim 64 or 128, heads a multiple of kv_heads, 1 to 2^31 - 1 tokens times kv_heads)");
   if ((reinterpret_cast<uintptr_t>(k_codes) | reinterpret_cast<uintptr_t>(v_codes) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return st::fail(ST_ERR_INVALID, "paged attention: codes must be 16-byte aligned");
   if (rows == 0) return ST_OK;
   const AttnParams p{q, static_cast<const unsigned char*>(k_codes), static_cast<const unsigned char*>(v_codes), k_scale, v_scale, table, starts, lengths, out, lse, workspace,
-                     q_row, q_head, o_row, o_head, table_row, pages, rows, width, shift, B, heads, kv_heads, heads / kv_heads, scale, causal, zero_tail, st::error_word()};
+                     q_row, q_head, o_row, o_head, table_row, pages, rows, width, shift, B, heads, kv_heads, heads / kv_heads, scale, causal, zero_tail, shift >= 5, st::error_word()};
   const int nt = row_tiles(max_queries, heads / kv_heads);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
   return type == 0 ? dispatch<__nv_bfloat16>(p, dim, nt, stream) : dispatch<__half>(p, dim, nt, stream);

@@ -328,6 +328,8 @@ def attention(q: torch.Tensor, pages: Pages, table: torch.Tensor, starts: torch.
         raise ValueError(f"paged.attention: table {tuple(table.shape)}, starts {tuple(starts.shape)} and lengths {tuple(lengths.shape)} do not belong together")
     if max_queries < 1 or max_queries * H >= 1 << 31:
         raise ValueError(f"paged.attention: max_queries {max_queries}")
+    if not 0 < P * Hk * page < 1 << 31:
+        raise ValueError(f"paged.attention: {P} pages of {page} tokens and {Hk} heads")
     if torch.is_grad_enabled() and q.requires_grad:
         raise ValueError("paged.attention: not differentiable; use ops.attention for training")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1):
