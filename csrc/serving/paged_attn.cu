@@ -5,24 +5,29 @@
 // What bounds it: a key is 2 * D bytes and 4 * D operations per query row, so for the rows of one decoding step (the query
 // heads of one key head) it is bound by reading the cache once.
 //
-// Work.  The rows of a sequence that share a key head are its n tokens times the G query heads of the group; N = 8, 16 or 32 of them
+// Work.  The rows of a sequence that share a key head are its n tokens times the G query heads of the group; R = 8, 16 or 32 of them
 // are an item together with one (sequence, key head), and 128 keys of an item are a unit.  All units of the call are numbered through and
 // every block takes an equal run of them, whatever the lengths are: the split needs nothing from the host but the shapes, so a captured
 // launch stays right while the sequences grow, and one long sequence fills the chip as well as many short ones.  Each block finds its run
-// by a prefix sum over the sequences.  Where a run ends inside an item, the block leaves (maximum, sum, output) in the workspace,
+// by a prefix sum over the sequences.  An item counts some units more than it has, for what its beginning and end cost a block: without
+// them blocks in short sequences took up to a third longer than those in long ones.  Where a run ends inside an item, the block leaves (maximum, sum, output) in the workspace,
 // and a second kernel joins the parts of such items in their order, so results do not depend on timing.  It finds them by the notes
 // that the blocks leave about the border between their run and the next.
 //
-// Inner loop.  A warp takes 32 keys of a unit at a time through rings of its own in shared memory, two slots of 4 KB (for heads of 128) for keys
-// and two for values, which one lane fills by tiled copies: the keys two steps ahead are asked for as soon as the scores of this step are
-// formed, the values when its products are, and the run's next item follows the last one without a pause.
-// The order of the head elements inside the matrix instructions is chosen so that 16 contiguous bytes of a key are a thread's
-// fragments (keys as the rows of A, S^T = K Q^T; values transposed by byte permutes, O^T = V^T P^T), the order of the keys so that no two
-// lanes' loads from the swizzled rows meet in a bank (key_of below).  Codes become fp16, which holds e4m3 exactly, and the queries are the
-// N side of m16n8k16, which wastes nothing from 8 rows on.  (m16n8k32 on the codes themselves, with a query as the sum of two e4m3 values, is
-// no gain: it takes more instructions than the conversion, 78 us against 75 on the case of 64 sequences.)  Queries are scaled by a power of two
-// per row so that fp16 holds bf16's bits too.  The softmax runs over x + b instead of x (b: the page's value exponent): the weights exp2(x + b - max) are those that
-// multiply the codes, at most 1, and fp16 keeps 11 bits of them; the sum takes exp2(-b) back out.
+// Products.  Both run on tcgen05 with the codes as they lie in the cache: no code is ever converted or passes through a register.  A unit's keys
+// are the 128 rows of S^T = K Q^T (keys in lanes, so a thread has all rows' scores of its key), its values, read along the tokens,
+// those of O^T = V^T P^T.  The other operands, queries and weights, are fp16 numbers written as sums of e5m2 numbers, whose three
+// significant bits are those of fp16's upper byte: the byte, the byte of what it leaves, and so on; three hold bf16's 8 bits, four fp16's
+// 11.  Queries' parts follow one another in the sum over K, weights' parts side by side in N, added when the item is done.  So the products are exact
+// and a unit costs a warp about 150 instructions instead of the 650 of mma.sync on converted codes (64 sequences: 78 us alone).
+// Queries are scaled by a power of two per row to use fp16's range.  The softmax runs over x + b instead of x (b: the page's value
+// exponent): the weights exp2(x + b - M) are those that multiply the codes, and the sum takes exp2(-b) back out.  M is not the running
+// maximum but some number that no x + b exceeds by more than 6: it moves, and the outputs with it, in the first unit and rarely after, and the
+// weights, times 2^9, stay below 2^15.
+//
+// Blocks: four warps for the softmax, one that copies (a tiled copy per page and unit), one that issues products, one that prepares the queries
+// of the next item, so that a run's items follow one another without a pause: with that in the softmax warps' way an item cost them 4500 cycles more.  Heads of 64: the copies lay two tokens
+// side by side, 64 rows of 128, and the weights of even and odd tokens have columns of their own; half of each product is not used.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "../common/host.h"
@@ -32,8 +37,12 @@
 namespace {
 using st::chain_begin;
 
-constexpr int kWarps = 4, kThreads = 32 * kWarps, kTile = 32 * kWarps;      // keys of a unit
+constexpr int kSoftThreads = 128, kThreads = 256, kTile = 128;      // threads of the softmax, of a block; keys of a unit
+constexpr int kScanWarps = kThreads / 32;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoMax = -1e30f;      // before a row has seen a key
+constexpr float kLag = 6.0f, kLift = 9.0f;
+constexpr int kParts = 4;             // e5m2 numbers of a weight
 
 struct AttnParams {
   const void* q;
@@ -51,45 +60,43 @@ struct AttnParams {
   unsigned* err;
 };
 
+// What the beginning and the end of an item cost, in units: 5000 cycles of about 2300, with 32 rows 20000 of 4500.
+template <int N> constexpr int kItemCost = N == 32 ? 4 : 2;
+
 struct Seq {
-  int start, n, len, row_blocks, tiles;
-  long long units;
+  int start, n, len, row_blocks, tiles, units;
 };
 template <int N>
 __device__ __forceinline__ Seq sequence(const AttnParams& p, int b) {
   Seq s;
-  const long long a = p.starts[b], e = p.starts[b + 1];
-  s.start = static_cast<int>(a < 0 ? 0 : a);
-  const long long end = e < p.rows ? e : p.rows;
-  s.n = end > s.start ? static_cast<int>(end - s.start) : 0;
-  const long long room = static_cast<long long>(p.width) << p.shift;
-  const int len = max(p.lengths[b], 0);
-  s.len = len < room ? len : static_cast<int>(room);
-  s.row_blocks = (static_cast<long long>(s.n) * p.group + N - 1) / N;
+  const int rows = static_cast<int>(p.rows), a = p.starts[b], e = p.starts[b + 1], len = max(p.lengths[b], 0);
+  s.start = max(a, 0);
+  s.n = max(min(e, rows) - s.start, 0);
+  s.len = min(len, p.width << p.shift);
+  s.row_blocks = (s.n * p.group + N - 1) / N;
   s.tiles = max((s.len + kTile - 1) / kTile, 1);      // a sequence without keys still gets its zero rows
-  s.units = static_cast<long long>(s.row_blocks) * s.tiles * p.kv_heads;
+  s.units = s.row_blocks * (s.tiles + kItemCost<N>) * p.kv_heads;
   return s;
 }
 
 // Where the block's share begins: the sequence that holds a unit, and the number of the sequence's first one.
 struct Found {
-  int b;
-  long long first;
+  int b, first;
 };
-__device__ __forceinline__ long long scan_block(long long mine, long long* shared, long long& total) {      // sum of the threads before, and of all
-  long long s = mine;
+__device__ __forceinline__ int scan_block(int mine, int* shared, int& total) {      // sum of the threads before, and of all
+  int s = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, s, o);
+    const int u = __shfl_up_sync(0xffffffffu, s, o);
     if ((threadIdx.x & 31) >= o) s += u;
   }
   __syncthreads();
   if ((threadIdx.x & 31) == 31) shared[threadIdx.x >> 5] = s;
   __syncthreads();
-  long long before = s - mine;
+  int before = s - mine;
   total = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < kScanWarps; ++w) {
     if (w < static_cast<int>(threadIdx.x >> 5)) before += shared[w];
     total += shared[w];
   }
@@ -97,18 +104,23 @@ __device__ __forceinline__ long long scan_block(long long mine, long long* share
 }
 // The block's share [u0, u1) of the units, if it has one, and where unit u0 lies.  Up to a block's threads of sequences are looked at once.
 template <int N>
-__device__ bool find_share(const AttnParams& p, long long* shared, Found* found, long long& all, int& runs, long long& u0, long long& u1, Found& f) {
-  long long mine = 0, total = 0, before = 0;
+__device__ bool find_share(const AttnParams& p, int* shared, Found* found, int& all, int& runs, int& u0, int& u1, Found& f) {
+  int mine = 0, total = 0, before = 0;
+#pragma unroll 1
   for (int b = threadIdx.x; b < p.B; b += kThreads) mine += sequence<N>(p, b).units;
   before = scan_block(mine, shared, total);
   all = total;
-  runs = static_cast<int>(min(static_cast<long long>(gridDim.x), all));      // none of them empty
-  if (static_cast<int>(blockIdx.x) >= runs) return false;
-  u0 = all * blockIdx.x / runs, u1 = all * (blockIdx.x + 1) / runs;
+  runs = min(static_cast<int>(gridDim.x), all);      // none of them empty
+  const int me = blockIdx.x;
+  if (me >= runs) return false;
+  // floor(all * block / runs) without the product
+  const unsigned each = static_cast<unsigned>(all) / static_cast<unsigned>(runs), rest = all - each * runs;
+  u0 = me * each + me * rest / runs, u1 = (me + 1) * each + (me + 1) * rest / runs;
   if (p.B <= kThreads) {
     if (u0 >= before && u0 < before + mine) *found = Found{static_cast<int>(threadIdx.x), before};      // one thread
   } else {
-    long long base = 0;
+    int base = 0;
+#pragma unroll 1
     for (int b0 = 0; b0 < p.B && u0 >= base; b0 += kThreads) {
       const int b = b0 + threadIdx.x;
       mine = b < p.B ? sequence<N>(p, b).units : 0;
@@ -121,365 +133,178 @@ __device__ bool find_share(const AttnParams& p, long long* shared, Found* found,
   f = *found;
   return true;
 }
-// a / b and a % b, by 32-bit arithmetic where both fit.
-__device__ __forceinline__ long long divide(long long a, int b, int& rest) {
-  if (a >> 32 == 0) {
-    const unsigned q = static_cast<unsigned>(a) / static_cast<unsigned>(b);
-    rest = static_cast<int>(static_cast<unsigned>(a) - q * b);
-    return q;
-  }
-  const long long q = a / b;
-  rest = static_cast<int>(a - q * b);
-  return q;
-}
 
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t pair) {      // of the low 16 bits
-  uint32_t d;
-  asm("{ .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %1;\n cvt.rn.f16x2.e4m3x2 %0, lo; }" : "=r"(d) : "r"(pair));
-  return d;
+// Eight 16-bit elements, wherever they begin.
+template <typename T> __device__ __forceinline__ uint4 load8(const T* p, bool wide) {
+  if (wide) return *reinterpret_cast<const uint4*>(p);
+  const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+  return make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
 }
-__device__ __forceinline__ uint32_t e4m3x2_hi_to_f16x2(uint32_t pair) {   // of the high 16 bits
-  uint32_t d;
-  asm("{ .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %1;\n cvt.rn.f16x2.e4m3x2 %0, hi; }" : "=r"(d) : "r"(pair));
-  return d;
-}
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
-  uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-// Bytes of e4m3 that are no number, as 0x80 in their places.
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <typename T> __device__ __forceinline__ void load4f(const T* p, float (&f)[4]);
-template <> __device__ __forceinline__ void load4f(const __nv_bfloat16* p, float (&f)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = __bfloat162float(p[i]);
-}
-template <> __device__ __forceinline__ void load4f(const __half* p, float (&f)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = __half2float(p[i]);
-}
+template <typename T> __device__ __forceinline__ float2 two_floats(uint32_t u);
+template <> __device__ __forceinline__ float2 two_floats<__nv_bfloat16>(uint32_t u) { return st::unpack_bf16x2(u); }
+template <> __device__ __forceinline__ float2 two_floats<__half>(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 template <typename T> __device__ __forceinline__ T from_f(float x);
 template <> __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
-
-// What the page (WIDE: pages of 32 tokens and more) or the two pages of 32 keys say of them.
-template <bool WIDE>
-struct Info {
-  static constexpr int PAGES = WIDE ? 1 : 2;
-  int page[PAGES];      // -1: nothing there
-  float ks[PAGES];      // the keys' scale
-  int ve[PAGES];        // the values' exponent
-  __device__ __forceinline__ bool valid(int piece) const { return page[WIDE ? 0 : piece] >= 0; }
-  __device__ __forceinline__ bool any() const { return WIDE ? page[0] >= 0 : page[0] >= 0 || page[PAGES - 1] >= 0; }
-  __device__ __forceinline__ float key_scale(int piece) const { return ks[WIDE ? 0 : piece]; }
-  __device__ __forceinline__ int value_exponent(int piece) const { return ve[WIDE ? 0 : piece]; }
-};
-// One lane's share of the page numbers and scales of the warp's next 16 steps: piece lane % 2 of step lane / 2.
-struct PieceList {
-  int page;
-  float ks;
-  int ve;
-};
-
-// A slot of a warp's ring: 32 keys (or values), as the copies leave them: lines of 128 bytes (a token, or two of 64 elements) whose 16-byte
-// parts are swizzled by the line's number.
-template <int D>
-struct Slot {
-  unsigned char piece[2][16 * D];
-};
-// The key of a piece that stands at row g (0..7) of a matrix fragment, and how far behind it that of row g + 8 is.  A quarter warp's 16-byte loads of
-// keys are rows (2i, 2i + 1) with parts 0..3 or 4..7; its loads of values rows 0, 2, 4, 6 (or 1, 3, 5, 7) with two neighbouring parts: both touch
-// all eight parts of the swizzled lines once.
-template <int D>
-__device__ __forceinline__ int key_of(int g) {
-  return D == 128 ? (g & 1 ? g ^ 4 : g) : 4 * (g >> 1) + (g & 1);
-}
-template <int D>
-constexpr int kSecond = D == 128 ? 8 : 2;
-// Byte of element 16 * part of token `key` of a piece.
-template <int D>
-__device__ __forceinline__ int at_part(int key, int part) {
-  if constexpr (D == 128) return key * 128 + ((part ^ (key & 7)) << 4);
-  return (key >> 1) * 128 + (((4 * (key & 1) + part) ^ (key >> 1 & 7)) << 4);
-}
-
-template <int D, int NT>
-struct Shared {
-  static constexpr int N = 8 * NT;
-  static constexpr int OUT_ROW = D + 4;      // lanes' stores of outputs in 32 banks
-  Slot<D> ring[kWarps][2][2];                // keys, values
-  float out[2][N][OUT_ROW];
-  uint2 q[NT][D / 16][32];
-  unsigned long long full[kWarps][2][2];     // barriers of the slots
-  float m[kWarps][N], l[kWarps][N], mx[N], sum[N];
-  float factor[N];
-  int limit[N];
-  long long place[N];                        // of a row in the output
-  long long sums[kWarps];
-  Found found;
-  int abort;
-};
 
 // An item, or the part of it that the block's run covers: units [t0, t1) of one head's rows [row0, row_end) of a sequence.
 struct Item {
   const int* table;
   int start, n, len, h, row0, row_end, t0, t1, tiles;
-  __device__ __forceinline__ int steps() const { return t1 - t0; }
+  int keys;      // that the last row sees
+  int next;      // number of the unit behind it
+  // Units to work on: those behind the last key are left out, one stays.
+  __device__ __forceinline__ int steps() const { return max(min(t1, (keys + kTile - 1) / kTile) - t0, 1); }
 };
+// The first item with work at or behind unit u of the run that ends at u1; false: there is none.
 template <int N>
-__device__ __forceinline__ Item item_at(const AttnParams& p, long long u, long long u1, Found& f, Seq& sq) {
-  while (u >= f.first + sq.units) {
-    f.first += sq.units;
-    sq = sequence<N>(p, ++f.b);
-  }
-  // unit -> (key head, row block, tile): row blocks of one head next to each other, as they read the same pages
-  Item it;
-  int rb;
-  it.h = static_cast<int>(divide(divide(u - f.first, sq.tiles, it.t0), sq.row_blocks, rb));
-  it.t1 = static_cast<int>(min(static_cast<long long>(sq.tiles), it.t0 + (u1 - u)));
-  it.tiles = sq.tiles, it.start = sq.start, it.n = sq.n, it.len = sq.len;
-  it.row0 = rb * N, it.row_end = min(sq.n * p.group, it.row0 + N);
-  it.table = p.table + f.b * p.table_row;
-  return it;
-}
-// Keys that a row sees: all of the sequence, or those up to its own place.
-__device__ __forceinline__ int keys_of(const AttnParams& p, const Item& it, int row) { return max(it.len - (p.causal ? it.n - 1 - row / p.group : 0), 0); }
-
-// Lane i: piece i % 2 of the warp's step first + i / 2.
-__device__ __forceinline__ PieceList list_pieces(const AttnParams& p, const Item& it, int first, int keys) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long key = (it.t0 + first + lane / 2) * static_cast<long long>(kTile) + warp * 32 + 16 * (lane & 1);
-  PieceList l{-1, 0.0f, 0};
-  if (key < keys && first + lane / 2 < it.steps()) {
-    const int page = it.table[key >> p.shift];
-    if (page < 0 || page >= p.pages) {
-      st::report_error(p.err, st::ERR_BOUNDS, 0x7004);
-    } else {
-      const long long at = static_cast<long long>(page) * p.kv_heads + it.h;
-      l.page = page;
-      l.ks = p.ks[at];
-      l.ve = st::scale_exponent(p.vs[at]);
+__device__ __forceinline__ bool item_at(Item& it, const AttnParams& p, int u, int u1, Found& f, Seq& sq) {
+#pragma unroll 1
+  while (u < u1) {
+    while (u >= f.first + sq.units) {
+      f.first += sq.units;
+      sq = sequence<N>(p, ++f.b);
     }
+    // unit -> (key head, row block, tile): row blocks of one head next to each other, as they read the same pages
+    const unsigned size = sq.tiles + kItemCost<N>, in = u - f.first, item = in / size;
+    const int at = in - item * size, end = min(static_cast<int>(size), at + (u1 - u));
+    u += end - at;
+    it.t0 = max(at - kItemCost<N>, 0), it.t1 = end - kItemCost<N>;
+    if (it.t1 <= it.t0) continue;      // nothing but the count for its beginning
+    it.next = u;
+    it.h = item / static_cast<unsigned>(sq.row_blocks);
+    const int rb = item - it.h * sq.row_blocks;
+    it.tiles = sq.tiles, it.start = sq.start, it.n = sq.n, it.len = sq.len;
+    it.row0 = rb * N, it.row_end = min(sq.n * p.group, it.row0 + N);
+    it.table = p.table + f.b * p.table_row;
+    it.keys = max(it.len - (p.causal ? it.n - 1 - (it.row_end - 1) / p.group : 0), 0);
+    return true;
   }
-  return l;
-}
-template <bool WIDE>
-__device__ __forceinline__ Info<WIDE> info_of(const PieceList& list, int step) {
-  Info<WIDE> c;
-#pragma unroll
-  for (int j = 0; j < Info<WIDE>::PAGES; ++j) {
-    const int lane = 2 * (step & 15) + j;
-    c.page[j] = __shfl_sync(0xffffffffu, list.page, lane);
-    c.ks[j] = __shfl_sync(0xffffffffu, list.ks, lane);
-    c.ve[j] = __shfl_sync(0xffffffffu, list.ve, lane);
-  }
-  return c;
-}
-// Starts the copies of 32 keys (or values) into a slot: one page, or two of 16 tokens.  What lies behind the last key is masked.
-template <int D, bool WIDE>
-__device__ __forceinline__ void copy_keys(Slot<D>& slot, uint32_t bar, const CUtensorMap* map, const AttnParams& p, const Info<WIDE>& c, int h, int key0) {
-  if ((threadIdx.x & 31) != 0) return;
-  if constexpr (WIDE) {
-    st::mbar_arrive_expect_tx(bar, c.page[0] >= 0 ? sizeof(Slot<D>) : 0);
-    if (c.page[0] < 0) return;
-    const long long row = ((static_cast<long long>(c.page[0]) * p.kv_heads + h) << p.shift) + (key0 & ((1 << p.shift) - 1));
-    st::tma_load_2d(st::smem_u32(slot.piece), map, bar, 0, static_cast<int>(row * D / 128));
-  } else {
-    st::mbar_arrive_expect_tx(bar, ((c.page[0] >= 0) + (c.page[1] >= 0)) * static_cast<int>(sizeof(Slot<D>) / 2));
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      if (c.page[j] >= 0)
-        st::tma_load_2d(st::smem_u32(slot.piece[j]), map, bar, 0, static_cast<int>((static_cast<long long>(c.page[j]) * p.kv_heads + h) * (16 * D / 128)));
-  }
+  return false;
 }
 
-template <int D, int NT>
-struct Running {
-  float o[D / 16][NT][4];
-  float m[NT][2], l[NT][2];
+__device__ __forceinline__ void umma_codes(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+      "}\n"
+      ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// A is e4m3 (0), B e5m2 (1), the sums fp32.
+constexpr uint32_t codes_idesc(int M, int N, bool mn_major) {
+  return (1u << 4) | (0u << 7) | (1u << 10) | (static_cast<uint32_t>(mn_major) << 15) | (static_cast<uint32_t>(mn_major) << 16) | (static_cast<uint32_t>(N >> 3) << 17) |
+         (static_cast<uint32_t>(M >> 4) << 24);
+}
+// Descriptor of a tile whose rows are WIDTH bytes, swizzled over that width: rows of K-major operands, or the K of MN-major ones; 8 rows are a group.
+// `block`: distance of the next WIDTH bytes along M or N; `group`: of the next 8 rows.
+template <int WIDTH>
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t block = 16, uint32_t group = 8 * WIDTH) {
+  static_assert(WIDTH == 32 || WIDTH == 64 || WIDTH == 128);
+  constexpr uint64_t kind = WIDTH == 128 ? 2 : WIDTH == 64 ? 4 : 6;
+  return ((addr & 0x3FFFF) >> 4) | static_cast<uint64_t>(block >> 4) << 16 | static_cast<uint64_t>(group >> 4) << 32 | 1ull << 46 | kind << 61;
+}
+// Byte of 16-byte part `part` of row `row` in such a tile.
+template <int WIDTH>
+__device__ __forceinline__ uint32_t swizzled(uint32_t row, uint32_t part) {
+  constexpr uint32_t mask = WIDTH / 16 - 1;
+  return row * WIDTH + ((part ^ (row * WIDTH >> 7 & mask)) << 4);
+}
+__device__ __forceinline__ void tmem_ld_8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool soft_any(bool x) {      // of the softmax threads; a barrier too
+  uint32_t y;
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.u32 p, %1, 0;\n"
+      "barrier.cta.red.or.pred q, 1, 128, p;\n"
+      "selp.u32 %0, 1, 0, q;\n"
+      "}\n"
+      : "=r"(y)
+      : "r"(static_cast<uint32_t>(x))
+      : "memory");
+  return y != 0;
+}
+// Bytes of e4m3 that are no number, as 0x80 in their places.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+// Splits off the upper bytes, e5m2 numbers, of eight fp16 numbers: returns them side by side, and leaves the rest (exactly).
+__device__ __forceinline__ uint2 split_off(__half2 (&x)[4]) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    u[i] = *reinterpret_cast<const uint32_t*>(&x[i]);
+    const uint32_t high = u[i] & 0xff00ff00u;
+    x[i] = __hsub2(x[i], *reinterpret_cast<const __half2*>(&high));
+  }
+  return make_uint2(__byte_perm(u[0], u[1], 0x7531), __byte_perm(u[2], u[3], 0x7531));
+}
+
+// e5m2 numbers of a query element: bf16 has 8 bits, fp16 11.
+template <typename T> constexpr int kQueryParts = 3;
+template <> constexpr int kQueryParts<__half> = 4;
+
+template <int D, int R, int QP>
+struct Layout {
+  static constexpr int S_N = R < 16 ? 16 : R;                          // columns of the scores
+  static constexpr int SIDES = D == 64 ? 2 : 1;                        // tokens side by side
+  static constexpr int P_N = SIDES * kParts * R;                       // columns of the products with values
+  static constexpr int P_WIDTH = P_N < 128 ? P_N : 128;                // bytes of a swizzled row of weights
+  static constexpr int P_ROWS = kTile / SIDES;
+  static constexpr int P_BYTES = P_ROWS * P_N;
+  static constexpr int COLUMNS = 2 * S_N + P_N <= 64 ? 64 : 2 * S_N + P_N <= 128 ? 128 : 2 * S_N + P_N <= 256 ? 256 : 512;
+  static constexpr int BLOCKS = COLUMNS == 512 ? 1 : 2;                // of an SM
+  static constexpr int Q_BYTES = QP * R * D;                           // 8 rows stand for 16 columns, see product_warp
+  // What fits the shared memory of two blocks (111 KB each, 2 KB of them for the small things): queries twice before a third stage of values, that
+  // before weights twice, and a third one of keys last.
+  static constexpr int ROOM = (BLOCKS == 2 ? 113 * 1024 : 226 * 1024) - 3072, ONE = kTile * D;
+  static constexpr int Q_BUFS = (D == 64 ? 4 : 2) * 2 * ONE + P_BYTES + 2 * Q_BYTES <= ROOM ? 2 : 1;
+  static constexpr int P_BUFS = (D == 64 ? 4 : 2) * 2 * ONE + 2 * P_BYTES + Q_BUFS * Q_BYTES <= ROOM ? 2 : 1;
+  static constexpr int V_STAGES = D == 64 ? 4 : 5 * ONE + P_BUFS * P_BYTES + Q_BUFS * Q_BYTES <= ROOM ? 3 : 2;
+  static constexpr int K_STAGES = D == 64 ? 4 : (3 + V_STAGES) * ONE + P_BUFS * P_BYTES + Q_BUFS * Q_BYTES <= ROOM ? 3 : 2;
 };
 
-// Scores of KS pieces of 16 keys.
-template <int D, int NT, int KS>
-__device__ __forceinline__ void scores(float (&s)[KS][NT][4], const Slot<D>& slot, int piece0, const Shared<D, NT>& sh, const uint2 (&qreg)[D / 16], int g, int q4) {
-  constexpr int KW = D / 16;      // words of a key row's part
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int j = 0; j < KS; ++j) {
-    uint32_t k0[KW], k1[KW];
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-      const uint4 x = *reinterpret_cast<const uint4*>(slot.piece[piece0 + j] + at_part<D>(key_of<D>(g), 4 * i + q4));
-      const uint4 y = *reinterpret_cast<const uint4*>(slot.piece[piece0 + j] + at_part<D>(key_of<D>(g) + kSecond<D>, 4 * i + q4));
-      k0[4 * i] = x.x, k0[4 * i + 1] = x.y, k0[4 * i + 2] = x.z, k0[4 * i + 3] = x.w;
-      k1[4 * i] = y.x, k1[4 * i + 1] = y.y, k1[4 * i + 2] = y.z, k1[4 * i + 3] = y.w;
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) s[j][n][0] = s[j][n][1] = s[j][n][2] = s[j][n][3] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < KW; ++k) {
-      const uint32_t a0 = e4m3x2_to_f16x2(k0[k]), a1 = e4m3x2_to_f16x2(k1[k]), a2 = e4m3x2_hi_to_f16x2(k0[k]), a3 = e4m3x2_hi_to_f16x2(k1[k]);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const uint2 b = NT == 1 ? qreg[k] : sh.q[n][k][lane];
-        mma(s[j][n], a0, a1, a2, a3, b.x, b.y);
-      }
-    }
-  }
-}
+// An item as the query warp hands it over.
+template <int D, int R>
+struct Rows {
+  Item item;
+  float factor[R];
+  int limit[R];
+  long long place[R];
+};
 
-// Running maximum and sum, and the weights in fp16, transposed to fragments.  edge: some row does not see some of these keys.
-template <int D, int NT, int KS, bool WIDE>
-__device__ __forceinline__ void weights(uint32_t (&pw)[KS][NT][2], float (&s)[KS][NT][4], Running<D, NT>& run, const Info<WIDE>& info, int piece0, const Shared<D, NT>& sh,
-                                        const float (&freg)[2], int key0, bool edge, int g, int q4) {
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int r0 = 8 * n + 2 * q4;
-    const float f0 = NT == 1 ? freg[0] : sh.factor[r0], f1 = NT == 1 ? freg[1] : sh.factor[r0 + 1];
-    float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < KS; ++j) {
-      const float ks = info.key_scale(piece0 + j), a0 = f0 * ks, a1 = f1 * ks, ve = static_cast<float>(info.value_exponent(piece0 + j));
-      float (&x)[4] = s[j][n];
-      x[0] = fmaf(x[0], a0, ve), x[1] = fmaf(x[1], a1, ve), x[2] = fmaf(x[2], a0, ve), x[3] = fmaf(x[3], a1, ve);
-      if (edge) {
-        const bool valid = info.valid(piece0 + j);
-        const int key = key0 + 16 * j + key_of<D>(g), l0 = valid ? sh.limit[r0] : 0, l1 = valid ? sh.limit[r0 + 1] : 0;
-        if (key >= l0) x[0] = -INFINITY;
-        if (key >= l1) x[1] = -INFINITY;
-        if (key + kSecond<D> >= l0) x[2] = -INFINITY;
-        if (key + kSecond<D> >= l1) x[3] = -INFINITY;
-      }
-      m0 = st::max3(m0, x[0], x[2]), m1 = st::max3(m1, x[1], x[3]);
-    }
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) {
-      m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-      m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-    }
-    m0 = fmaxf(m0, run.m[n][0]), m1 = fmaxf(m1, run.m[n][1]);
-    if (__any_sync(0xffffffffu, m0 > run.m[n][0] || m1 > run.m[n][1])) {
-      const float a0 = m0 > run.m[n][0] ? st::exp2_ftz(run.m[n][0] - m0) : 1.0f, a1 = m1 > run.m[n][1] ? st::exp2_ftz(run.m[n][1] - m1) : 1.0f;
-      run.m[n][0] = m0, run.m[n][1] = m1;
-      run.l[n][0] *= a0, run.l[n][1] *= a1;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) run.o[i][n][0] *= a0, run.o[i][n][1] *= a1, run.o[i][n][2] *= a0, run.o[i][n][3] *= a1;
-    }
-    const float z0 = m0 == -INFINITY ? 0.0f : m0, z1 = m1 == -INFINITY ? 0.0f : m1;      // nothing seen so far: weights 0, not NaN
-#pragma unroll
-    for (int j = 0; j < KS; ++j) {
-      const float (&x)[4] = s[j][n];
-      // fp16 ends at 2^-24, so exp2's subnormal results, from 2^-126 on, are 0 anyway
-      const float w0 = st::exp2_ftz(x[0] - z0), w1 = st::exp2_ftz(x[1] - z1), w2 = st::exp2_ftz(x[2] - z0), w3 = st::exp2_ftz(x[3] - z1);
-      const float take = st::exp2_int(-info.value_exponent(piece0 + j));
-      run.l[n][0] = fmaf(w0 + w2, take, run.l[n][0]);
-      run.l[n][1] = fmaf(w1 + w3, take, run.l[n][1]);
-      pw[j][n][0] = transpose8x8(pack_f16x2(w0, w1));
-      pw[j][n][1] = transpose8x8(pack_f16x2(w2, w3));
-    }
-  }
-}
-
-// Weights times values.
-template <int D, int NT, int KS, bool WIDE>
-__device__ __forceinline__ void values(Running<D, NT>& run, const uint32_t (&pw)[KS][NT][2], const Slot<D>& slot, const Info<WIDE>& info, int piece0, const Shared<D, NT>& sh,
-                                       int key0, int keys, bool edge, int g, int q4) {
-  constexpr int VW = D / 32;      // words of a value row's part
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int j = 0; j < KS; ++j) {
-    uint32_t v[4][VW];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int key = key_of<D>(2 * q4 + (i & 1)) + kSecond<D> * (i >> 1);
-      if constexpr (D == 128) {
-        const uint4 x = *reinterpret_cast<const uint4*>(slot.piece[piece0 + j] + at_part<D>(key, g));
-        v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
-      } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(slot.piece[piece0 + j] + at_part<D>(key, g >> 1) + 8 * (g & 1));
-        v[i][0] = x.x, v[i][1] = x.y;
-      }
-    }
-    if (edge) {
-      // what lies behind the end is no value; a value that is no number counts only for the rows that see it
-      const int first = key0 + 16 * j;
-      uint32_t some = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool behind = !info.valid(piece0 + j) || first + key_of<D>(2 * q4 + (i & 1)) + kSecond<D> * (i >> 1) >= keys;
-#pragma unroll
-        for (int w = 0; w < VW; ++w) {
-          if (behind) v[i][w] = 0;
-          some |= nan_bytes(v[i][w]);
-        }
-      }
-      if (__any_sync(0xffffffffu, some != 0)) {
-        uint32_t bad[4];      // a bit per element of the thread's part of a key's row
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          bad[i] = 0;
-#pragma unroll
-          for (int w = 0; w < VW; ++w) {
-            const uint32_t nb = nan_bytes(v[i][w]);
-            bad[i] |= ((nb >> 7 & 1) | (nb >> 14 & 2) | (nb >> 21 & 4) | (nb >> 28 & 8)) << (4 * w);
-            v[i][w] &= ~((nb >> 7) * 255u);
-          }
-        }
-#pragma unroll 1
-        for (int src = 0; src < 4; ++src)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t bits = __shfl_sync(0xffffffffu, bad[i], (lane & ~3) | src);
-            const int key = first + key_of<D>(2 * src + (i & 1)) + kSecond<D> * (i >> 1);
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int r = 0; r < 2; ++r)
-                if (bits && key < sh.limit[8 * n + 2 * q4 + r])
-#pragma unroll
-                  for (int d = 0; d < D / 16; ++d) {
-                    if (bits >> (2 * d) & 1) run.o[d][n][r] = NAN;
-                    if (bits >> (2 * d + 1) & 1) run.o[d][n][2 + r] = NAN;
-                  }
-          }
-      }
-    }
-#pragma unroll
-    for (int d = 0; d < D / 16; ++d) {
-      const int w = d / 2;
-      const uint32_t sel = d & 1 ? 0x7362 : 0x5140;
-      const uint32_t lo = __byte_perm(v[0][w], v[1][w], sel), hi = __byte_perm(v[2][w], v[3][w], sel);
-      const uint32_t a0 = e4m3x2_to_f16x2(lo), a1 = e4m3x2_hi_to_f16x2(lo), a2 = e4m3x2_to_f16x2(hi), a3 = e4m3x2_hi_to_f16x2(hi);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) mma(run.o[d][n], a0, a1, a2, a3, pw[j][n][0], pw[j][n][1]);
-    }
-  }
-}
-
-template <int D, int NT>
-__device__ __forceinline__ float* part_of(const AttnParams& p, long long slot) {      // [N][D] output, [N] maximum, [N] sum
-  return p.parts + slot * (8 * NT * (D + 2));
-}
-
-// Where an output element stands in a row of Shared::out: element 16 g + 2 i + e (D = 128) at 16 i + 2 g + e.
-template <int D>
-__device__ __forceinline__ int out_at(int d) {
-  constexpr int PER = D / 8;
-  return (d % PER / 2) * 16 + (d / PER) * 2 + (d & 1);
-}
-
-// Blocks of an SM: by registers (128 to 255 a thread) and 32 or 64 KB of rings.
-template <int D, int NT> constexpr int kBlocks = NT == 4 ? 2 : (D == 64 ? 5 : 4) - NT;
+template <int D, int R, int QP>
+struct Shared {
+  using L = Layout<D, R, QP>;
+  unsigned char k[L::K_STAGES][kTile * D], v[L::V_STAGES][kTile * D];
+  unsigned char p[L::P_BUFS][L::P_BYTES];
+  unsigned char q[L::Q_BUFS][QP][R * D];
+  unsigned long long k_full[L::K_STAGES], k_empty[L::K_STAGES], v_full[L::V_STAGES], v_empty[L::V_STAGES], s_full[2], p_full[2], pv_done[2], q_full[L::Q_BUFS], q_empty[L::Q_BUFS];
+  float ks[L::V_STAGES][8];      // of the unit's pages
+  int ve[L::V_STAGES][8];        // kInvalid: no such page
+  Rows<D, R> rows[L::Q_BUFS];
+  float m[4][R], sum[R];
+  uint32_t bad[R][D / 32];     // outputs that a value which is no number reaches though not all rows see it
+  int sums[kScanWarps];
+  Found found;
+  uint32_t tmem;
+  int abort;
+};
+static_assert(sizeof(Shared<128, 8, 3>) <= 113 * 1024 && sizeof(Shared<128, 16, 3>) <= 113 * 1024 && sizeof(Shared<128, 32, 3>) <= 113 * 1024 && sizeof(Shared<128, 8, 4>) <= 113 * 1024 &&
+              sizeof(Shared<128, 16, 4>) <= 113 * 1024 && sizeof(Shared<128, 32, 4>) <= 113 * 1024 && sizeof(Shared<64, 16, 4>) <= 113 * 1024 && sizeof(Shared<64, 32, 4>) <= 226 * 1024);
+constexpr int kInvalid = -1000;
 
 // What a block notes about the border behind its run: the item that it is inside of (parts 0: none).
 struct Note {
@@ -488,245 +313,521 @@ struct Note {
   int unused;
 };
 
-template <typename T, int D, int NT, bool WIDE>
-__global__ void __launch_bounds__(kThreads, kBlocks<D, NT>) paged_attn_kernel(AttnParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
-  constexpr int N = 8 * NT;
-  extern __shared__ __align__(1024) unsigned char raw[];      // the swizzle counts lines from multiples of 1024
-  Shared<D, NT>& sh = *reinterpret_cast<Shared<D, NT>*>(raw);
+
+template <int R>
+__device__ __forceinline__ float* part_of(const AttnParams& p, int D, long long slot) {      // [R][D] output, [R] maximum, [R] sum
+  return p.parts + slot * (R * (D + 2));
+}
+
+// ---- the copying warp -------------------------------------------------------------------------------------------------------------
+template <typename L, int D, int R, typename S>
+__device__ __forceinline__ void copy_warp(S& sh, const AttnParams& p, const CUtensorMap* km, const CUtensorMap* vm, int u0, int u1, Found f, Seq sq) {
+  const int lane = threadIdx.x & 31, rows = min(1 << p.shift, kTile), pages = kTile / rows;
+  struct Next {
+    int page, ve;
+    float ks;
+  };
+  auto look = [&](const Item& it, int t) {      // lane j: page j of the unit
+    const int key = t * kTile + lane * rows;
+    Next n{-1, kInvalid, 0.0f};
+    if (lane < pages && key < it.keys) {
+      const int page = it.table[key >> p.shift];
+      if (page < 0 || page >= p.pages) {
+        st::report_error(p.err, st::ERR_BOUNDS, 0x7004);
+      } else {
+        const long long at = static_cast<long long>(page) * p.kv_heads + it.h;
+        n.page = page, n.ks = p.ks[at], n.ve = st::scale_exponent(p.vs[at]);
+      }
+    }
+    return n;
+  };
+  uint32_t turn = 0;
+  Item it;
+  for (int u = u0; item_at<R>(it, p, u, u1, f, sq); u = it.next) {
+    const int steps = it.steps();
+    Next next = look(it, it.t0);
+    for (int i = 0; i < steps; ++i, ++turn) {
+      const Next n = next;
+      const int t = it.t0 + i;
+      if (i + 1 < steps) next = look(it, t + 1);
+      const int ks = turn % L::K_STAGES, vs = turn % L::V_STAGES;
+      const uint32_t live = __ballot_sync(0xffffffffu, n.page >= 0);
+      const uint32_t bytes = __popc(live) * rows * D;
+      const long long token = ((static_cast<long long>(n.page) * p.kv_heads + it.h) << p.shift) + ((t * kTile + lane * rows) & ((1 << p.shift) - 1));
+      if (!st::mbar_wait_warp(st::smem_u32(&sh.k_empty[ks]), (turn / L::K_STAGES & 1) ^ 1, &sh.abort)) return;
+      if (lane == 0) st::mbar_arrive_expect_tx(st::smem_u32(&sh.k_full[ks]), bytes);
+      __syncwarp();
+      if (n.page >= 0) st::tma_load_2d(st::smem_u32(sh.k[ks]) + lane * rows * D, km, st::smem_u32(&sh.k_full[ks]), 0, static_cast<int>(token));
+      if (!st::mbar_wait_warp(st::smem_u32(&sh.v_empty[vs]), (turn / L::V_STAGES & 1) ^ 1, &sh.abort)) return;
+      if (lane < pages) sh.ks[vs][lane] = n.ks, sh.ve[vs][lane] = n.ve;
+      __syncwarp();
+      if (lane == 0) st::mbar_arrive_expect_tx(st::smem_u32(&sh.v_full[vs]), bytes);
+      __syncwarp();
+      if (n.page >= 0) st::tma_load_2d(st::smem_u32(sh.v[vs]) + lane * rows * D, vm, st::smem_u32(&sh.v_full[vs]), 0, static_cast<int>(token * D / 128));
+    }
+  }
+}
+
+// ---- the warp that issues products (one lane) -------------------------------------------------------------------------------------
+// Scores take 16 columns at least: with 8 rows the second group of eight is the first one again (a distance of 0), and nobody reads it.
+template <typename L, int D, int R, int QP, typename S>
+__device__ __forceinline__ void product_warp(S& sh, uint32_t tmem, int u1) {
+  constexpr uint32_t s_idesc = codes_idesc(128, L::S_N, false), p_idesc = codes_idesc(128, L::P_N, true);
+  uint32_t turn = 0, item = 0;
+  auto ask_scores = [&](uint32_t t, uint32_t of) {
+    const int slot = t % L::K_STAGES;
+    if (!st::mbar_wait(st::smem_u32(&sh.k_full[slot]), t / L::K_STAGES & 1, &sh.abort)) return false;
+    st::tc_fence_after();
+#pragma unroll
+    for (int i = 0; i < QP; ++i)
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k)
+        umma_codes(tmem + (t & 1) * L::S_N, tile_desc<D>(st::smem_u32(sh.k[slot])) + 2 * k,
+                   tile_desc<D>(st::smem_u32(sh.q[of % L::Q_BUFS][i]), 16, R == 8 ? 0 : 8 * D) + 2 * k, s_idesc, i + k > 0);
+    st::umma_commit(st::smem_u32(&sh.s_full[t & 1]));
+    st::umma_commit(st::smem_u32(&sh.k_empty[slot]));
+    return true;
+  };
+  // the item's number of units, 0 behind the last one, once its queries are there
+  auto next_item = [&](uint32_t of, int& steps, int& next) {
+    if (!st::mbar_wait(st::smem_u32(&sh.q_full[of % L::Q_BUFS]), of / L::Q_BUFS & 1, &sh.abort)) return false;
+    const Item& it = sh.rows[of % L::Q_BUFS].item;
+    steps = it.t1 > it.t0 ? it.steps() : 0, next = it.next;
+    return true;
+  };
+  int steps = 0, next = 0, steps_next = 0, next_next = 0;
+  if (!next_item(0, steps, next) || steps == 0 || !ask_scores(0, 0)) return;
+  for (;; ++item) {
+    const bool more = next < u1;
+    for (int i = 0; i < steps; ++i, ++turn) {
+      // the scores of the next unit, be it the next item's: not with one buffer of queries, which waits for this item's end
+      if (i + 1 < steps) {
+        if (!ask_scores(turn + 1, item)) return;
+      } else if (more && L::Q_BUFS == 2) {
+        if (!next_item(item + 1, steps_next, next_next) || (steps_next > 0 && !ask_scores(turn + 1, item + 1))) return;
+      }
+      const int slot = turn % L::V_STAGES;
+      if (!st::mbar_wait(st::smem_u32(&sh.p_full[turn & 1]), turn >> 1 & 1, &sh.abort)) return;
+      if (!st::mbar_wait(st::smem_u32(&sh.v_full[slot]), turn / L::V_STAGES & 1, &sh.abort)) return;
+      st::tc_fence_after();
+      // 32 rows of K (tokens, or pairs of them) at a time: 4 groups of 8
+#pragma unroll
+      for (int k = 0; k < L::P_ROWS / 32; ++k)
+        umma_codes(tmem + 2 * L::S_N, tile_desc<128>(st::smem_u32(sh.v[slot])) + k * (32 * 128 >> 4),
+                   tile_desc<L::P_WIDTH>(st::smem_u32(sh.p[turn % L::P_BUFS]), L::P_ROWS * L::P_WIDTH) + k * (32 * L::P_WIDTH >> 4), p_idesc, i + k > 0);
+      st::umma_commit(st::smem_u32(&sh.pv_done[turn & 1]));
+      st::umma_commit(st::smem_u32(&sh.v_empty[slot]));
+    }
+    if (!more) return;
+    if (L::Q_BUFS == 1 && (!next_item(item + 1, steps_next, next_next) || (steps_next > 0 && !ask_scores(turn, item + 1)))) return;
+    if (steps_next == 0) return;
+    steps = steps_next, next = next_next;
+  }
+}
+
+// ---- the warp that prepares queries -------------------------------------------------------------------------------------------------
+template <typename T, typename L, int D, int R, int QP, typename S>
+__device__ __forceinline__ void query_warp(S& sh, const AttnParams& p, int u0, int u1, Found f, Seq sq) {
+  const int lane = threadIdx.x & 31;
+  const T* q = static_cast<const T*>(p.q);
+  const bool wide = ((p.q_row | p.q_head) & 7) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+  uint32_t item = 0;
+  Item it;
+  for (int u = u0; u < u1; ++item) {
+    if (!item_at<R>(it, p, u, u1, f, sq)) {      // the last word: no more items; no rows either, so nothing is read
+      it = Item{};
+      it.next = u1;
+    }
+    u = it.next;
+    const int buf = item % L::Q_BUFS;
+    if (!st::mbar_wait_warp(st::smem_u32(&sh.q_empty[buf]), (item / L::Q_BUFS & 1) ^ 1, &sh.abort)) return;
+    Rows<D, R>& to = sh.rows[buf];
+    if (lane == 0) to.item = it;
+    // four lanes to a row, a quarter of it each; loops as they are, as code that runs once per item costs its way into the instruction cache
+#pragma unroll 1
+    for (int r = lane / 4; r < R; r += 8) {
+      constexpr int VECS = D / 32;      // 8 elements each
+      const int fr = it.row0 + r, i = fr / p.group, head = it.h * p.group + fr - i * p.group;
+      const bool live = fr < it.row_end;
+      const T* from = q + (it.start + i) * p.q_row + head * p.q_head + (lane & 3) * (D / 4);
+      uint4 raw[VECS];
+#pragma unroll
+      for (int k = 0; k < VECS; ++k) raw[k] = live ? load8(from + 8 * k, wide) : make_uint4(0, 0, 0, 0);
+      float top = 0.0f;
+#pragma unroll
+      for (int k = 0; k < VECS; ++k) {
+        const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 x = two_floats<T>(w[j]);
+          top = st::max3(top, fabsf(x.x), fabsf(x.y));
+        }
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // the largest to [2^14, 2^15): exact down to 2^-14 of e5m2, 2^-28 of the largest; a row with infinities gives NaN
+      int e = static_cast<int>((__float_as_uint(top) >> 23) & 255) - 127 - 14;
+      e = top < INFINITY ? max(e, -100) : 0;
+      const float mul = top < INFINITY ? st::exp2_int(-e) : NAN;
+#pragma unroll
+      for (int k = 0; k < VECS; ++k) {
+        const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+        __half2 h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 x = two_floats<T>(w[j]);
+          h[j] = __floats2half2_rn(x.x * mul, x.y * mul);
+        }
+        const int d = (lane & 3) * (D / 4) + 8 * k;
+#pragma unroll
+        for (int j = 0; j < QP; ++j) *reinterpret_cast<uint2*>(sh.q[buf][j] + swizzled<D>(r, d / 16) + d % 16) = split_off(h);
+      }
+      if ((lane & 3) == 0) {
+        to.factor[r] = p.scale * kLog2e * st::exp2_int(e);
+        to.limit[r] = live ? max(it.len - (p.causal ? it.n - 1 - i : 0), 0) : 0x7fffffff;      // rows that are none are not written
+        to.place[r] = (it.start + i) * p.o_row + head * p.o_head;
+      }
+    }
+    st::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) st::mbar_arrive(st::smem_u32(&sh.q_full[buf]));
+  }
+}
+
+// ---- the softmax -------------------------------------------------------------------------------------------------------------------
+// The largest over a warp; NaN counts only where all are.
+__device__ __forceinline__ float warp_top(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+// COLUMNS of this warp's lanes.
+template <int COLUMNS>
+__device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&r)[COLUMNS]) {
+  if constexpr (COLUMNS == 8) tmem_ld_8(taddr, r);
+  else if constexpr (COLUMNS == 16) st::tmem_ld_32x16(taddr, r);
+  else st::tmem_ld_32x32(taddr, r);
+}
+
+// Keys that not all rows see, in a unit's values: what lies behind the end becomes 0; a value that is no number becomes 0 too, and the
+// outputs of the rows that see it are noted.  One key a thread.
+template <int D, int R, typename S>
+__device__ __forceinline__ void clean_values(S& sh, const Rows<D, R>& of, int slot, int key, bool there, int limit_min) {
+  constexpr int SIDES = D == 64 ? 2 : 1, PARTS = D / 16;
+  const int t = threadIdx.x, line = t / SIDES, side = t % SIDES * PARTS;
+#pragma unroll 1
+  for (int c = 0; c < PARTS; ++c) {
+    uint4* at = reinterpret_cast<uint4*>(sh.v[slot] + swizzled<128>(line, side + c));
+    if (!there) {
+      *at = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    uint4 x = *at;
+    uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t nb = nan_bytes(w[i]);
+      bits |= ((nb >> 7 & 1) | (nb >> 14 & 2) | (nb >> 21 & 4) | (nb >> 28 & 8)) << (4 * i);
+      w[i] &= ~((nb >> 7) * 255u);
+    }
+    if (bits == 0 || key < limit_min) continue;
+    for (int r = 0; r < R; ++r)
+      if (key < of.limit[r]) atomicOr(&sh.bad[r][c / 2], bits << (16 * (c & 1)));
+    *at = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+template <typename T, typename L, int D, int R, typename S>
+__device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t tmem_all, Note* note, int u1, int runs, int all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = threadIdx.x;
+  const uint32_t tmem = tmem_all + (warp << 21);                                                          // the warp's 32 lanes
+  const uint32_t o_cols = tmem + 2 * L::S_N + (D == 64 && warp >= 2 ? kParts * R : 0);                      // lanes 64..127 of heads of 64: the odd tokens'
+  const int page_at = t >> min(p.shift, 7);
+  T* out = static_cast<T*>(p.out);
+  // A wait that runs out sets the abort flag, and all later ones return at once: the warps finish the item together and stop at the next one.
+  uint32_t turn = 0, item = 0;
+  for (int i = t; i < R * (D / 32); i += kSoftThreads) sh.bad[i / (D / 32)][i % (D / 32)] = 0;
+  for (;; ++item) {
+    const Rows<D, R>& of = sh.rows[item % L::Q_BUFS];
+    if (soft_any(!st::mbar_wait_warp(st::smem_u32(&sh.q_full[item % L::Q_BUFS]), item / L::Q_BUFS & 1, &sh.abort))) return;
+    if (of.item.t1 <= of.item.t0) return;      // no more items
+    const int steps = of.item.steps(), t0 = of.item.t0, keys = of.item.keys, next = of.item.next;
+    const int limit_min = of.limit[0];      // rows come in order
+    float m[R], l[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) m[r] = kNoMax, l[r] = 0.0f;
+
+    for (int i = 0; i < steps; ++i, ++turn) {
+      const int slot = turn % L::V_STAGES, key = (t0 + i) * kTile + t;
+      st::mbar_wait_warp(st::smem_u32(&sh.v_full[slot]), turn / L::V_STAGES & 1, &sh.abort);
+      const float ks = sh.ks[slot][page_at];
+      const int ve_or_not = sh.ve[slot][page_at];
+      const bool there = ve_or_not != kInvalid && key < keys;
+      const int ve = there ? ve_or_not : 0;
+      const bool gone = (t0 + i + 1) * kTile > limit_min || !there;      // of this unit's keys some row may not see this one
+      float a[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) a[r] = of.factor[r] * ks;
+      st::mbar_wait_warp(st::smem_u32(&sh.s_full[turn & 1]), turn >> 1 & 1, &sh.abort);
+      st::tc_fence_after();
+      uint32_t raw[R];
+      tmem_ld_columns<R>(tmem + (turn & 1) * L::S_N, raw);
+      st::tmem_ld_wait();
+      float x[R];
+      const float lift = static_cast<float>(ve);
+#pragma unroll
+      for (int r = 0; r < R; ++r) x[r] = fmaf(__uint_as_float(raw[r]), a[r], lift);
+      if (gone) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (!there || key >= of.limit[r]) x[r] = -INFINITY;
+      }
+      float over = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < R; r += 2) over = st::max3(over, x[r] - m[r], x[r + 1] - m[r + 1]);
+      // the reference moves where a weight would be too large; the first unit always sets it
+      if (soft_any(over > kLag)) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float top = warp_top(x[r]);
+          if (lane == 0) sh.m[warp][r] = top;
+        }
+        soft_sync();
+        if (i > 0) {
+          st::mbar_wait_warp(st::smem_u32(&sh.pv_done[(turn - 1) & 1]), (turn - 1) >> 1 & 1, &sh.abort);
+          st::tc_fence_after();
+        }
+#pragma unroll
+        for (int c = 0; c < R / 8; ++c) {
+          float b[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            const int row = 8 * c + r;
+            const float to = fmaxf(m[row], fmaxf(fmaxf(sh.m[0][row], sh.m[1][row]), fmaxf(sh.m[2][row], sh.m[3][row])));
+            b[r] = st::exp2_ftz(m[row] - to);
+            m[row] = to;
+            l[row] *= b[r];
+          }
+          if (i > 0)
+#pragma unroll
+            for (int j = 0; j < kParts; ++j) {
+              uint32_t o[8];
+              tmem_ld_8(o_cols + j * R + 8 * c, o);
+              st::tmem_ld_wait();
+#pragma unroll
+              for (int r = 0; r < 8; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * b[r]);
+              tmem_st_8(o_cols + j * R + 8 * c, o);
+            }
+        }
+        if (i > 0) st::tmem_st_wait();
+        soft_sync();      // the maxima are read
+      }
+      if (gone) clean_values<D, R>(sh, of, slot, key, there, limit_min);
+      // the buffer's last products are done
+      if constexpr (L::P_BUFS == 2) st::mbar_wait_warp(st::smem_u32(&sh.pv_done[turn & 1]), (turn >> 1 & 1) ^ 1, &sh.abort);
+      else if (turn > 0) st::mbar_wait_warp(st::smem_u32(&sh.pv_done[(turn - 1) & 1]), (turn - 1) >> 1 & 1, &sh.abort);
+      const float take = st::exp2_int(-ve - static_cast<int>(kLift));
+      unsigned char* to = sh.p[turn % L::P_BUFS];
+      const uint32_t row = t / L::SIDES, first = t % L::SIDES * kParts * R;
+#pragma unroll
+      for (int c = 0; c < R / 8; ++c) {
+        __half2 w[4];
+#pragma unroll
+        for (int r = 0; r < 8; r += 2) {
+          const float y = st::exp2_ftz(x[8 * c + r] - m[8 * c + r] + kLift), z = st::exp2_ftz(x[8 * c + r + 1] - m[8 * c + r + 1] + kLift);
+          l[8 * c + r] = fmaf(y, take, l[8 * c + r]), l[8 * c + r + 1] = fmaf(z, take, l[8 * c + r + 1]);
+          w[r / 2] = __floats2half2_rn(y, z);
+        }
+#pragma unroll
+        for (int j = 0; j < kParts; ++j) {
+          const uint32_t byte = first + j * R + 8 * c;
+          *reinterpret_cast<uint2*>(to + byte / 128 * (L::P_ROWS * 128) + swizzled<L::P_WIDTH>(row, byte % 128 / 16) + byte % 16) = split_off(w);
+        }
+      }
+      st::fence_proxy_async_smem();
+      st::tc_fence_before();
+      st::mbar_arrive(st::smem_u32(&sh.p_full[turn & 1]));
+    }
+
+    // the item's outputs, and the sums over all keys, through the room of the weights, which no product reads now
+    st::mbar_wait_warp(st::smem_u32(&sh.pv_done[(turn - 1) & 1]), (turn - 1) >> 1 & 1, &sh.abort);
+    st::tc_fence_after();
+    const Item& it = of.item;
+    const int rows = it.row_end - it.row0;
+    const bool whole = it.t0 == 0 && it.t1 == it.tiles;
+    float* part = whole ? nullptr : part_of<R>(p, D, 2LL * blockIdx.x + (it.t0 == 0 ? 1 : 0));
+    float* room = reinterpret_cast<float*>(sh.p[0]);      // [R][128]
+#pragma unroll
+    for (int r = 0; r < R; ++r) room[r * 128 + t] = l[r];
+    soft_sync();
+    {      // 128 / R threads to a row, R keys each; where they begin keeps them out of one another's banks
+      const int r = t / (128 / R), first = t % (128 / R) * R;
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < R / 4; ++i) {
+        const float4 y = *reinterpret_cast<const float4*>(room + r * 128 + first + 4 * ((i + t) % (R / 4)));
+        sum += (y.x + y.y) + (y.z + y.w);
+      }
+#pragma unroll
+      for (int o = 64 / R; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (t % (128 / R) == 0) sh.sum[r] = sum;
+    }
+    soft_sync();
+#pragma unroll
+    for (int c = 0; c < R / 8; ++c) {
+      float o[8];
+      if constexpr (R == 8) {      // the parts of 8 rows are 32 neighbouring columns
+        uint32_t raw[32];
+        st::tmem_ld_32x32(o_cols, raw);
+        st::tmem_ld_wait();
+#pragma unroll
+        for (int r = 0; r < 8; ++r) o[r] = (__uint_as_float(raw[r]) + __uint_as_float(raw[8 + r])) + (__uint_as_float(raw[16 + r]) + __uint_as_float(raw[24 + r]));
+      } else {
+        uint32_t raw[kParts][8];
+#pragma unroll
+        for (int j = 0; j < kParts; ++j) tmem_ld_8(o_cols + j * R + 8 * c, raw[j]);
+        st::tmem_ld_wait();
+#pragma unroll
+        for (int r = 0; r < 8; ++r) o[r] = (__uint_as_float(raw[0][r]) + __uint_as_float(raw[1][r])) + (__uint_as_float(raw[2][r]) + __uint_as_float(raw[3][r]));
+      }
+      if constexpr (D == 64) {
+        if (warp >= 2)
+#pragma unroll
+          for (int r = 0; r < 8; ++r) room[r * 64 + t - 64] = o[r];
+        soft_sync();
+        if (warp < 2)
+#pragma unroll
+          for (int r = 0; r < 8; ++r) o[r] += room[r * 64 + t];
+        if (c + 1 < R / 8) soft_sync();
+      }
+      if (D == 128 || warp < 2) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const int row = 8 * c + r;
+          if (row >= rows) continue;
+          const float sum = sh.sum[row];
+          float y = o[r] * (1.0f / 512.0f);      // 2^-kLift
+          if (sh.bad[row][t / 32] >> (t & 31) & 1) y = NAN;
+          if (whole) out[of.place[row] + t] = from_f<T>(sum == 0.0f ? 0.0f : __fdividef(y, sum));
+          else part[row * D + t] = y;
+          if (t == 0) {
+            if (!whole) part[R * D + row] = m[row], part[R * D + R + row] = sum;
+            else if (p.lse != nullptr) {
+              const int fr = it.row0 + row;
+              p.lse[(it.start + fr / p.group) * static_cast<long long>(p.heads) + it.h * p.group + fr % p.group] = sum == 0.0f ? -INFINITY : (m[row] + log2f(sum)) / kLog2e;
+            }
+          }
+        }
+      }
+    }
+    if (t == 0 && it.t1 < it.tiles) {      // the run ends inside the item
+      // Block b holds a part if its run begins before the item's end, all * b / runs < end, which is all * b < end * runs, and ends behind its first unit.
+      const long long first_unit = u1 - it.t1, end = first_unit + it.tiles;
+      Note n{};
+      n.first = static_cast<int>(((first_unit + 1) * runs - 1) / all);
+      n.parts = static_cast<int>((end * runs - 1) / all) - n.first + 1;
+      n.border = static_cast<int>(blockIdx.x) - n.first;
+      n.rows = rows, n.start = it.start, n.row0 = it.row0, n.h = it.h;
+      *note = n;
+    }
+    st::tc_fence_before();
+    soft_sync();      // everything of the item is read
+    if (next >= u1) return;
+    for (int i = t; i < R * (D / 32); i += kSoftThreads) sh.bad[i / (D / 32)][i % (D / 32)] = 0;
+    if (t == 0) st::mbar_arrive(st::smem_u32(&sh.q_empty[item % L::Q_BUFS]));
+  }
+}
+
+// Rows behind the last sequence: 0, by one warp of every block.
+template <typename T, int D>
+__device__ __forceinline__ void zero_rows(const AttnParams& p) {
+  const int lane = threadIdx.x & 31, vectors = p.heads * (D / 2);
+  const long long from = p.B > 0 ? max(p.starts[p.B], 0) : 0;
+#pragma unroll 1
+  for (long long row = from + blockIdx.x; row < p.rows; row += gridDim.x) {
+    T* o = static_cast<T*>(p.out) + row * p.o_row;
+#pragma unroll 1
+    for (int i = lane; i < vectors; i += 32) {
+      T* at = o + i / (D / 2) * p.o_head + i % (D / 2) * 2;
+      at[0] = at[1] = from_f<T>(0.0f);
+    }
+    if (p.lse != nullptr)
+      for (int i = lane; i < p.heads; i += 32) p.lse[row * p.heads + i] = -INFINITY;
+  }
+}
+
+template <typename T, int D, int R>
+__global__ void __launch_bounds__(kThreads, Layout<D, R, kQueryParts<T>>::BLOCKS) paged_attn_kernel(AttnParams p, const __grid_constant__ CUtensorMap k_map,
+                                                                                                     const __grid_constant__ CUtensorMap v_map) {
+  constexpr int QP = kQueryParts<T>;
+  using L = Layout<D, R, QP>;
+  extern __shared__ __align__(1024) unsigned char raw[];      // swizzles count rows from multiples of 1024
+  using S = Shared<D, R, QP>;
+  S& sh = *reinterpret_cast<S*>(raw);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     st::tma_prefetch_desc(&k_map);
     st::tma_prefetch_desc(&v_map);
-    for (int i = 0; i < 4 * kWarps; ++i) st::mbar_init(st::smem_u32(&sh.full[0][0][0] + i), 1);
+    for (int i = 0; i < L::K_STAGES; ++i) st::mbar_init(st::smem_u32(&sh.k_full[i]), 1), st::mbar_init(st::smem_u32(&sh.k_empty[i]), 1);
+    for (int i = 0; i < L::V_STAGES; ++i) st::mbar_init(st::smem_u32(&sh.v_full[i]), 1), st::mbar_init(st::smem_u32(&sh.v_empty[i]), 1);
+    for (int i = 0; i < 2; ++i) {
+      st::mbar_init(st::smem_u32(&sh.s_full[i]), 1);
+      st::mbar_init(st::smem_u32(&sh.p_full[i]), kSoftThreads);
+      st::mbar_init(st::smem_u32(&sh.pv_done[i]), 1);
+    }
+    for (int i = 0; i < L::Q_BUFS; ++i) st::mbar_init(st::smem_u32(&sh.q_full[i]), 1), st::mbar_init(st::smem_u32(&sh.q_empty[i]), 1);
     st::fence_barrier_init();
     sh.abort = 0;
   }
   chain_begin(p.ks, p.vs, p.table, p.starts, p.lengths);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q4 = lane & 3;
-  const T* q = static_cast<const T*>(p.q);
-  T* out = static_cast<T*>(p.out);
 
-  if (p.zero_tail) {      // rows behind the last sequence
-    const long long from = p.B > 0 ? max(p.starts[p.B], 0) : 0, per = static_cast<long long>(p.heads) * D;
-    for (long long i = from * per + blockIdx.x * kThreads + threadIdx.x; i < p.rows * per; i += static_cast<long long>(gridDim.x) * kThreads) {
-      const long long row = i / per, e = i - row * per;
-      out[row * p.o_row + e / D * p.o_head + e % D] = from_f<T>(0.0f);
-      if (p.lse != nullptr && e % D == 0) p.lse[row * p.heads + e / D] = -INFINITY;
-    }
+  if (warp == 5) {
+    st::tmem_alloc(st::smem_u32(&sh.tmem), L::COLUMNS);
+    st::tmem_relinquish();
   }
-  long long all, u0, u1;
-  int runs;
+  st::tc_fence_before();      // before the barriers of the scan
+  int all, u0, u1, runs;
   Found f;
   Note* note = reinterpret_cast<Note*>(p.notes) + blockIdx.x;
-  if (!find_share<N>(p, sh.sums, &sh.found, all, runs, u0, u1, f)) {
-    if (threadIdx.x == 0) note->parts = 0;
+  const bool share = find_share<R>(p, sh.sums, &sh.found, all, runs, u0, u1, f);
+  st::tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  if (p.zero_tail && warp == 7) zero_rows<T, D>(p);
+  if (threadIdx.x == 0) note->parts = 0;
+  if (!share) {
+    if (warp == 5) st::tmem_dealloc(tmem, L::COLUMNS);
     return;
   }
-  Seq sq = sequence<N>(p, f.b);
-  const uint32_t k_bar = st::smem_u32(&sh.full[warp][0][0]), v_bar = k_bar + 16;
-  Slot<D>(&k_ring)[2] = sh.ring[warp][0];
-  Slot<D>(&v_ring)[2] = sh.ring[warp][1];
-  uint32_t turn = 0;      // steps that the warp has worked on: slot turn % 2 of the rings, for the (turn / 2)-th time
-
-  long long u = u0;
-  Item it = item_at<N>(p, u, u1, f, sq), after;
-  int keys = min(keys_of(p, it, it.row_end - 1), it.t1 * kTile);      // what the run's part of the item is about, of what its last row sees
-  PieceList list = list_pieces(p, it, 0, keys), list_more{-1, 0.0f, 0}, list_after{-1, 0.0f, 0};
-  Info<WIDE> info[2];      // of this step and the next one
-  int asked = 0, keys_after = 0;
-  for (;;) {
-    const int steps = it.steps(), key0 = it.t0 * kTile + warp * 32;
-    for (; asked < 2 && asked < steps; ++asked) {
-      const Info<WIDE> c = info_of<WIDE>(list, asked);
-      const uint32_t to = (turn + asked) & 1;
-      if (asked == 0) info[0] = c; else info[1] = c;
-      copy_keys<D, WIDE>(k_ring[to], k_bar + 8 * to, &k_map, p, c, it.h, key0 + asked * kTile);
-      copy_keys<D, WIDE>(v_ring[to], v_bar + 8 * to, &v_map, p, c, it.h, key0 + asked * kTile);
+  const Seq sq = sequence<R>(p, f.b);
+  // With 16 rows and more the softmax takes registers from the other warps: 176 and 80 of the 128 of the launch (one warp does nothing else).
+  constexpr bool kShift = R >= 16 && L::BLOCKS == 2;
+  if (warp >= 4) {
+    if constexpr (kShift) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == 4) {
+      copy_warp<L, D, R>(sh, p, &k_map, &v_map, u0, u1, f, sq);
+    } else if (warp == 5) {
+      if (lane == 0) product_warp<L, D, R, QP>(sh, tmem, u1);
+      __syncwarp();
+    } else if (warp == 6) {
+      query_warp<T, L, D, R, QP>(sh, p, u0, u1, f, sq);
     }
-    const bool more = u + steps < u1;
-    __syncthreads();      // the item before is done with the queries and the rows' places
-    for (int r = warp; r < N; r += kWarps) {
-      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      const int fr = it.row0 + r, i = fr / p.group, head = it.h * p.group + fr - i * p.group;
-      const bool live = fr < it.row_end;
-      if (live && 4 * lane < D) load4f(q + (it.start + i) * p.q_row + head * p.q_head + 4 * lane, x);
-      const float top = st::warp_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
-      // the largest to [2^13, 2^14): exact for bf16 and fp16 down to 2^-27 of it; a row with infinities stays as it is
-      int e = static_cast<int>((__float_as_uint(top) >> 23) & 255) - 127 - 13;
-      e = top < INFINITY ? max(e, -100) : 0;
-      const float mul = st::exp2_int(-e);
-      if (4 * lane < D) {
-        const int d = 4 * lane, k = d / 64 * 4 + d % 16 / 4, c = d % 64 / 16;
-        sh.q[r / 8][k][(r % 8) * 4 + c] = make_uint2(pack_f16x2(x[0] * mul, x[1] * mul), pack_f16x2(x[2] * mul, x[3] * mul));
-      }
-      if (lane == 0) {
-        sh.factor[r] = p.scale * kLog2e * st::exp2_int(e);
-        sh.limit[r] = live ? max(it.len - (p.causal ? it.n - 1 - i : 0), 0) : 0x7fffffff;      // rows that are none are not written
-        sh.place[r] = (it.start + i) * p.o_row + head * p.o_head;
-      }
-    }
-    if (more) {      // the loads are in flight while this item is worked on
-      after = item_at<N>(p, u + steps, u1, f, sq);
-      keys_after = min(keys_of(p, after, after.row_end - 1), after.t1 * kTile);
-      list_after = list_pieces(p, after, 0, keys_after);
-    }
-    __syncthreads();
-    const int limit_min = sh.limit[0];      // rows come in order
-    uint2 qreg[D / 16];
-    if constexpr (NT == 1)
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) qreg[k] = sh.q[0][k][lane];
-    const float freg[2] = {sh.factor[2 * q4], sh.factor[2 * q4 + 1]};
-    Running<D, NT> s;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      s.m[n][0] = s.m[n][1] = -INFINITY;
-      s.l[n][0] = s.l[n][1] = 0.0f;
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) s.o[d][n][0] = s.o[d][n][1] = s.o[d][n][2] = s.o[d][n][3] = 0.0f;
-    }
-    asked = 0;      // of the next item's steps
-    if (steps == 1 && more) {
-      info[1] = info_of<WIDE>(list_after, 0);
-      const uint32_t to = (turn + 1) & 1;
-      copy_keys<D, WIDE>(k_ring[to], k_bar + 8 * to, &k_map, p, info[1], after.h, after.t0 * kTile + warp * 32);
-      copy_keys<D, WIDE>(v_ring[to], v_bar + 8 * to, &v_map, p, info[1], after.h, after.t0 * kTile + warp * 32);
-      asked = 1;
-    }
-    for (int i = 0; i < steps; ++i) {
-      // the step after the next, of this item or of the next one
-      const int ahead = i + 2, over = ahead - steps, at = key0 + i * kTile;
-      if ((ahead & 15) == 8) list_more = list_pieces(p, it, (ahead & ~15) + 16, keys);
-      if ((ahead & 15) == 0) list = list_more;
-      Info<WIDE> coming = info[1];
-      const bool ask = over < 0 || (more && over < after.steps());
-      if (ask) coming = over < 0 ? info_of<WIDE>(list, ahead) : info_of<WIDE>(list_after, over);
-      const int ask_h = over < 0 ? it.h : after.h, ask_key = over < 0 ? at + 2 * kTile : after.t0 * kTile + warp * 32 + over * kTile;
-
-      const uint32_t now = turn & 1, phase = turn >> 1 & 1;
-      const bool edge = at + 32 > limit_min || !info[0].valid(0) || !info[0].valid(1);
-      bool here = st::mbar_wait_warp(k_bar + 8 * now, phase, &sh.abort);
-      if constexpr (NT <= 2) {
-        float sc[2][NT][4];
-        uint32_t pw[2][NT][2];
-        const bool any = here && info[0].any();
-        if (any) scores<D, NT, 2>(sc, k_ring[now], 0, sh, qreg, g, q4);
-        __syncwarp();      // every lane is done with the keys
-        if (ask) copy_keys<D, WIDE>(k_ring[now], k_bar + 8 * now, &k_map, p, coming, ask_h, ask_key);
-        if (any) weights<D, NT, 2, WIDE>(pw, sc, s, info[0], 0, sh, freg, at, edge, g, q4);
-        here = st::mbar_wait_warp(v_bar + 8 * now, phase, &sh.abort) && here;
-        if (any && here) values<D, NT, 2, WIDE>(s, pw, v_ring[now], info[0], 0, sh, at, keys, edge, g, q4);
-      } else {      // a piece at a time: two do not fit the registers
-        here = st::mbar_wait_warp(v_bar + 8 * now, phase, &sh.abort) && here;
-#pragma unroll 1
-        for (int j = 0; j < 2; ++j) {
-          if (!here || !info[0].valid(j)) continue;
-          float sc[1][NT][4];
-          uint32_t pw[1][NT][2];
-          scores<D, NT, 1>(sc, k_ring[now], j, sh, qreg, g, q4);
-          weights<D, NT, 1, WIDE>(pw, sc, s, info[0], j, sh, freg, at + 16 * j, edge, g, q4);
-          values<D, NT, 1, WIDE>(s, pw, v_ring[now], info[0], j, sh, at + 16 * j, keys, edge, g, q4);
-        }
-        __syncwarp();
-        if (ask) copy_keys<D, WIDE>(k_ring[now], k_bar + 8 * now, &k_map, p, coming, ask_h, ask_key);
-      }
-      __syncwarp();      // and with the values
-      if (ask) {
-        copy_keys<D, WIDE>(v_ring[now], v_bar + 8 * now, &v_map, p, coming, ask_h, ask_key);
-        if (over >= 0) ++asked;
-      }
-      if (!here && lane == 0) st::report_error(p.err, st::ERR_MBAR_TIMEOUT, 0x7005);
-      ++turn;
-      info[0] = info[1];
-      info[1] = coming;
-    }
-
-    // join the warps: two write their outputs, the others add theirs
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) s.l[n][r] += __shfl_xor_sync(0xffffffffu, s.l[n][r], o);
-        if (g == 0) sh.m[warp][8 * n + 2 * q4 + r] = s.m[n][r], sh.l[warp][8 * n + 2 * q4 + r] = s.l[n][r];
-      }
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = 8 * n + 2 * q4 + r;
-        const float mx = fmaxf(fmaxf(sh.m[0][row], sh.m[1][row]), fmaxf(sh.m[2][row], sh.m[3][row]));
-        const float a = s.l[n][r] == 0.0f ? 0.0f : st::exp2_ftz(s.m[n][r] - mx);      // 0: saw nothing; a score that is no number leaves a sum that is none
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d) s.o[d][n][r] *= a, s.o[d][n][2 + r] *= a;
-      }
-    if (threadIdx.x < N) {
-      const int row = threadIdx.x;
-      const float mx = fmaxf(fmaxf(sh.m[0][row], sh.m[1][row]), fmaxf(sh.m[2][row], sh.m[3][row]));
-      float l = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) l += sh.l[w][row] == 0.0f ? 0.0f : sh.l[w][row] * st::exp2_ftz(sh.m[w][row] - mx);
-      sh.mx[row] = mx, sh.sum[row] = l;
-    }
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if (warp / 2 == half)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              float2* to = reinterpret_cast<float2*>(&sh.out[warp & 1][8 * n + 2 * q4 + r][16 * d + 2 * g]);
-              float2 x = make_float2(s.o[d][n][r], s.o[d][n][2 + r]);
-              if (half == 1) x.x += to->x, x.y += to->y;
-              *to = x;
-            }
-      __syncthreads();
-    }
-    const int rows = it.row_end - it.row0;
-    const bool whole = it.t0 == 0 && it.t1 == it.tiles;
-    float* part = whole ? nullptr : part_of<D, NT>(p, 2LL * blockIdx.x + (it.t0 == 0 ? 1 : 0));
-    for (int i = threadIdx.x; i < rows * (D / 2); i += kThreads) {
-      const int row = i / (D / 2), d = i % (D / 2) * 2, from = out_at<D>(d);
-      const float2 x = *reinterpret_cast<const float2*>(&sh.out[0][row][from]), y = *reinterpret_cast<const float2*>(&sh.out[1][row][from]);
-      const float l = sh.sum[row];
-      if (whole) {
-        T* o = out + sh.place[row] + d;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        o[0] = from_f<T>((x.x + y.x) * inv), o[1] = from_f<T>((x.y + y.y) * inv);
-        if (d == 0 && p.lse != nullptr) {
-          const int fr = it.row0 + row;
-          p.lse[(it.start + fr / p.group) * static_cast<long long>(p.heads) + it.h * p.group + fr % p.group] = l == 0.0f ? -INFINITY : (sh.mx[row] + log2f(l)) / kLog2e;
-        }
-      } else {
-        *reinterpret_cast<float2*>(part + row * D + d) = make_float2(x.x + y.x, x.y + y.y);
-        if (d == 0) part[N * D + row] = sh.mx[row], part[N * D + N + row] = l;
-      }
-    }
-    u += steps;
-    if (!more) break;
-    it = after, keys = keys_after, list = list_after;
+  } else {
+    if constexpr (kShift) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    soft_warps<T, L, D, R>(sh, p, tmem, note, u1, runs, all);
+    if (threadIdx.x == 0 && sh.abort) st::report_error(p.err, st::ERR_MBAR_TIMEOUT, 0x7005);
   }
-  if (threadIdx.x == 0) {
-    Note n{};
-    if (it.t1 < it.tiles) {
-      // block b holds a part if its run begins before the item's end, all * b / runs < end, which is all * b < end * runs, and ends behind its first unit
-      const long long first_unit = u1 - it.t1, end = first_unit + it.tiles;
-      n.first = static_cast<int>(((first_unit + 1) * runs - 1) / all);
-      n.parts = static_cast<int>((end * runs - 1) / all) - n.first + 1;
-      n.border = static_cast<int>(blockIdx.x) - n.first;
-      n.rows = it.row_end - it.row0, n.start = it.start, n.row0 = it.row0, n.h = it.h;
-    }
-    *note = n;
-  }
+  st::tc_fence_before();
+  __syncthreads();
+  if (warp == 5) st::tmem_dealloc(tmem, L::COLUMNS);
 }
 
 // Joins the parts of the items that several blocks worked on.  A block per border; an item of P parts has P - 1 of them, which share its rows.
 // With few parts a warp does a row; with many, the block's warps share the parts of a row.
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads) paged_join_kernel(AttnParams p) {
-  constexpr int N = 8 * NT, E = D / 32;
+constexpr int kJoinThreads = 128, kWarps = kJoinThreads / 32;
+template <typename T, int D, int N>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(AttnParams p) {
+  constexpr int E = D / 32;
   extern __shared__ float weight[];      // [kWarps][few] or [parts]
   __shared__ float red[2][kWarps], rows[kWarps][D];
   const float* parts = p.parts;
@@ -739,7 +840,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(AttnParams p) {
   constexpr int kFew = 8;
   const float* base = parts + 2LL * n.first * kSlot;      // part 0 lies in its block's second slot, the others in the first slots of their blocks
   const bool few = n.parts <= kFew;
-  const int members = few ? kWarps : 1, me = few ? warp : 0, width = few ? 32 : kThreads, at = few ? lane : threadIdx.x;
+  const int members = few ? kWarps : 1, me = few ? warp : 0, width = few ? 32 : kJoinThreads, at = few ? lane : threadIdx.x;
   for (int r = n.border * members + me; r < n.rows; r += (n.parts - 1) * members) {      // few: warps go their own ways, without barriers
     float m = -INFINITY;
     for (int i = at; i < n.parts; i += width) {
@@ -803,49 +904,53 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(AttnParams p) {
   }
 }
 
-// Row tiles of 8 by the rows that the longest step of a sequence has.
-int row_tiles(long long max_queries, int group) {
+// Rows of an item, by those that the longest step of a sequence has for a key head.
+int item_rows(long long max_queries, int group) {
   const long long rows = max_queries * group;
-  return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  return rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
 }
-int runs_of(int nt, int dim) {
-  return st::sm_count() * (dim == 64 ? nt == 1 ? kBlocks<64, 1> : nt == 2 ? kBlocks<64, 2> : kBlocks<64, 4> : nt == 1 ? kBlocks<128, 1> : nt == 2 ? kBlocks<128, 2> : kBlocks<128, 4>);
-}
+// Blocks that run at once: two to an SM, one where the products take all columns of tensor memory.
+int runs_of(int rows, int dim) { return st::sm_count() * (dim == 64 && rows == 32 ? Layout<64, 32, 4>::BLOCKS : Layout<128, 32, 4>::BLOCKS); }
 
-template <typename T, int D, int NT, bool WIDE>
+template <typename T, int D, int R>
 int launch(const AttnParams& p, cudaStream_t stream) {
-  const int runs = runs_of(NT, D);
-  constexpr int smem = sizeof(Shared<D, NT>);
+  const int runs = runs_of(R, D);
+  constexpr int smem = sizeof(Shared<D, R, kQueryParts<T>>);
+  // keys: rows of one token, swizzled over its D bytes; values: lines of 128 bytes; a copy takes a page's tokens, or a unit's
   CUtensorMap maps[2];
-  const uint64_t dims[2] = {128, (static_cast<uint64_t>(p.pages) * p.kv_heads << p.shift) * D / 128}, strides[1] = {128};
-  const uint32_t box[2] = {128, (WIDE ? 32u : 16u) * D / 128};
-  for (int i = 0; i < 2; ++i)
-    if (!st::encode_tmap(&maps[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, i == 0 ? p.kc : p.vc, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return ST_ERR_CUDA;
-  auto kernel = paged_attn_kernel<T, D, NT, WIDE>;
+  const uint64_t tokens = static_cast<uint64_t>(p.pages) * p.kv_heads << p.shift;
+  const uint32_t rows = p.shift < 7 ? 1u << p.shift : kTile;
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t width = i == 0 ? D : 128, dims[2] = {width, tokens * D / width}, strides[1] = {width};
+    const uint32_t box[2] = {static_cast<uint32_t>(width), static_cast<uint32_t>(rows * D / width)};
+    if (!st::encode_tmap(&maps[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, i == 0 ? p.kc : p.vc, dims, strides, box,
+                         width == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B))
+      return ST_ERR_CUDA;
+  }
+  auto kernel = paged_attn_kernel<T, D, R>;
   static bool opted[st::kMaxDevices];
   if (bool& done = opted[st::current_device()]; !done) {
     ST_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     done = true;
   }
-  // in order: blocks that come early pile up on the SMs that fall free first (64 sequences: 98 us a pass against 80)
+  // in order: blocks that come early pile up on the SMs that fall free first
   cudaError_t e = st::in_order(kernel, dim3(runs), dim3(kThreads), smem, stream)(p, maps[0], maps[1]);
   if (e != cudaSuccess) return st::fail_cuda(e, "paged attention");
-  e = st::chained(paged_join_kernel<T, D, NT>, dim3(runs - 1), dim3(kThreads), runs * sizeof(float), stream)(p);
+  e = st::chained(paged_join_kernel<T, D, R>, dim3(runs - 1), dim3(kJoinThreads), runs * sizeof(float), stream)(p);
   if (e != cudaSuccess) return st::fail_cuda(e, "paged attention: join");
   return ST_OK;
 }
 template <typename T, int D>
-int dispatch(const AttnParams& p, int nt, cudaStream_t stream) {
-  if (p.shift >= 5) return nt == 1 ? launch<T, D, 1, true>(p, stream) : nt == 2 ? launch<T, D, 2, true>(p, stream) : launch<T, D, 4, true>(p, stream);
-  return nt == 1 ? launch<T, D, 1, false>(p, stream) : nt == 2 ? launch<T, D, 2, false>(p, stream) : launch<T, D, 4, false>(p, stream);
+int dispatch(const AttnParams& p, int rows, cudaStream_t stream) {
+  return rows == 8 ? launch<T, D, 8>(p, stream) : rows == 16 ? launch<T, D, 16>(p, stream) : launch<T, D, 32>(p, stream);
 }
 }  // namespace
 
 // Floats of workspace that st_paged_attention takes.
 ST_API long long st_paged_attention_workspace(int max_queries, int heads, int kv_heads, int dim) {
   if (kv_heads < 1 || heads < kv_heads) return 0;
-  const int nt = row_tiles(max_queries, heads / kv_heads);
-  return (2LL * 8 * nt * (dim + 2) + sizeof(Note) / sizeof(float)) * runs_of(nt, dim);
+  const int r = item_rows(max_queries, heads / kv_heads);
+  return (2LL * r * (dim + 2) + sizeof(Note) / sizeof(float)) * runs_of(r, dim);
 }
 
 // q, out [rows, heads, dim] (dim contiguous, strides in elements): row starts[b] + i is the i-th of the newest tokens of sequence b, whose keys and values,
@@ -862,11 +967,14 @@ ST_API int st_paged_attention(const void* q, const void* k_codes, const void* v_
   if ((reinterpret_cast<uintptr_t>(k_codes) | reinterpret_cast<uintptr_t>(v_codes) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return st::fail(ST_ERR_INVALID, "paged attention: codes must be 16-byte aligned");
   if (rows == 0) return ST_OK;
-  const int nt = row_tiles(max_queries, heads / kv_heads);
-  int* notes = reinterpret_cast<int*>(workspace + 2LL * 8 * nt * (dim + 2) * runs_of(nt, dim));      // behind the parts
+  const int r = item_rows(max_queries, heads / kv_heads);
+  // units are counted in 32 bits
+  if ((rows * (heads / kv_heads) / r + B) * (((static_cast<long long>(width) << shift) + kTile - 1) / kTile + 1 + kItemCost<32>) * kv_heads > 2147483647LL)
+    return st::fail(ST_ERR_TOO_LARGE, "paged attention: rows times the table's width is too large for one call");
+  int* notes = reinterpret_cast<int*>(workspace + 2LL * r * (dim + 2) * runs_of(r, dim));      // behind the parts
   const AttnParams p{q, static_cast<const unsigned char*>(k_codes), static_cast<const unsigned char*>(v_codes), k_scale, v_scale, table, starts, lengths, out, lse, workspace, notes,
                      q_row, q_head, o_row, o_head, table_row, pages, rows, width, shift, B, heads, kv_heads, heads / kv_heads, scale, causal, zero_tail, st::error_word()};
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
-  if (type == 0) return dim == 64 ? dispatch<__nv_bfloat16, 64>(p, nt, stream) : dispatch<__nv_bfloat16, 128>(p, nt, stream);
-  return dim == 64 ? dispatch<__half, 64>(p, nt, stream) : dispatch<__half, 128>(p, nt, stream);
+  if (type == 0) return dim == 64 ? dispatch<__nv_bfloat16, 64>(p, r, stream) : dispatch<__nv_bfloat16, 128>(p, r, stream);
+  return dim == 64 ? dispatch<__half, 64>(p, r, stream) : dispatch<__half, 128>(p, r, stream);
 }
