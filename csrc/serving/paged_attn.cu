@@ -37,8 +37,12 @@
 namespace {
 using st::chain_begin;
 
-constexpr int kSoftThreads = 128, kThreads = 256, kTile = 128;      // threads of the softmax, of a block; keys of a unit
-constexpr int kScanWarps = kThreads / 32;
+constexpr int kTile = 128;            // keys of a unit
+// Warps of the softmax: with 32 rows twice as many, each of which has half of the rows (118 us against 4 on the case of parts of prompts);
+// then come the copying one, the product's, the queries', and one for the rows behind the last sequence.
+template <int R> constexpr int kSoftWarps = R == 32 ? 8 : 4;
+template <int R> constexpr int kThreadsOf = 32 * (kSoftWarps<R> + 4);
+constexpr int kMaxWarps = 12;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -1e30f;      // before a row has seen a key
 constexpr float kLag = 6.0f, kLift = 9.0f;
@@ -83,6 +87,7 @@ __device__ __forceinline__ Seq sequence(const AttnParams& p, int b) {
 struct Found {
   int b, first;
 };
+template <int WARPS>
 __device__ __forceinline__ int scan_block(int mine, int* shared, int& total) {      // sum of the threads before, and of all
   int s = mine;
 #pragma unroll
@@ -96,7 +101,7 @@ __device__ __forceinline__ int scan_block(int mine, int* shared, int& total) {  
   int before = s - mine;
   total = 0;
 #pragma unroll
-  for (int w = 0; w < kScanWarps; ++w) {
+  for (int w = 0; w < WARPS; ++w) {
     if (w < static_cast<int>(threadIdx.x >> 5)) before += shared[w];
     total += shared[w];
   }
@@ -105,10 +110,11 @@ __device__ __forceinline__ int scan_block(int mine, int* shared, int& total) {  
 // The block's share [u0, u1) of the units, if it has one, and where unit u0 lies.  Up to a block's threads of sequences are looked at once.
 template <int N>
 __device__ bool find_share(const AttnParams& p, int* shared, Found* found, int& all, int& runs, int& u0, int& u1, Found& f) {
+  constexpr int kThreads = kThreadsOf<N>, kWarps = kThreads / 32;
   int mine = 0, total = 0, before = 0;
 #pragma unroll 1
   for (int b = threadIdx.x; b < p.B; b += kThreads) mine += sequence<N>(p, b).units;
-  before = scan_block(mine, shared, total);
+  before = scan_block<kWarps>(mine, shared, total);
   all = total;
   runs = min(static_cast<int>(gridDim.x), all);      // none of them empty
   const int me = blockIdx.x;
@@ -124,7 +130,7 @@ __device__ bool find_share(const AttnParams& p, int* shared, Found* found, int& 
     for (int b0 = 0; b0 < p.B && u0 >= base; b0 += kThreads) {
       const int b = b0 + threadIdx.x;
       mine = b < p.B ? sequence<N>(p, b).units : 0;
-      before = base + scan_block(mine, shared, total);
+      before = base + scan_block<kWarps>(mine, shared, total);
       if (u0 >= before && u0 < before + mine) *found = Found{b, before};
       base += total;
     }
@@ -223,18 +229,20 @@ __device__ __forceinline__ void tmem_st_8(uint32_t taddr, const uint32_t (&r)[8]
                ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
-__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+template <int THREADS>
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
+template <int THREADS>
 __device__ __forceinline__ bool soft_any(bool x) {      // of the softmax threads; a barrier too
   uint32_t y;
   asm volatile(
       "{\n"
       ".reg .pred p, q;\n"
       "setp.ne.u32 p, %1, 0;\n"
-      "barrier.cta.red.or.pred q, 1, 128, p;\n"
+      "barrier.cta.red.or.pred q, 1, %2, p;\n"
       "selp.u32 %0, 1, 0, q;\n"
       "}\n"
       : "=r"(y)
-      : "r"(static_cast<uint32_t>(x))
+      : "r"(static_cast<uint32_t>(x)), "n"(THREADS)
       : "memory");
   return y != 0;
 }
@@ -297,7 +305,7 @@ struct Shared {
   Rows<D, R> rows[L::Q_BUFS];
   float m[4][R], sum[R];
   uint32_t bad[R][D / 32];     // outputs that a value which is no number reaches though not all rows see it
-  int sums[kScanWarps];
+  int sums[kMaxWarps];
   Found found;
   uint32_t tmem;
   int abort;
@@ -514,7 +522,7 @@ __device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&r)[CO
 template <int D, int R, typename S>
 __device__ __forceinline__ void clean_values(S& sh, const Rows<D, R>& of, int slot, int key, bool there, int limit_min) {
   constexpr int SIDES = D == 64 ? 2 : 1, PARTS = D / 16;
-  const int t = threadIdx.x, line = t / SIDES, side = t % SIDES * PARTS;
+  const int t = threadIdx.x & 127, line = t / SIDES, side = t % SIDES * PARTS;
 #pragma unroll 1
   for (int c = 0; c < PARTS; ++c) {
     uint4* at = reinterpret_cast<uint4*>(sh.v[slot] + swizzled<128>(line, side + c));
@@ -540,23 +548,25 @@ __device__ __forceinline__ void clean_values(S& sh, const Rows<D, R>& of, int sl
 
 template <typename T, typename L, int D, int R, typename S>
 __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t tmem_all, Note* note, int u1, int runs, int all) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = threadIdx.x;
+  // a thread has RT rows from `low` on of one key
+  constexpr int SOFT = 32 * kSoftWarps<R>, RT = R * 128 / SOFT;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5 & 3, t = threadIdx.x & 127, half = threadIdx.x >> 7, low = half * RT;
   const uint32_t tmem = tmem_all + (warp << 21);                                                          // the warp's 32 lanes
   const uint32_t o_cols = tmem + 2 * L::S_N + (D == 64 && warp >= 2 ? kParts * R : 0);                      // lanes 64..127 of heads of 64: the odd tokens'
   const int page_at = t >> min(p.shift, 7);
   T* out = static_cast<T*>(p.out);
   // A wait that runs out sets the abort flag, and all later ones return at once: the warps finish the item together and stop at the next one.
   uint32_t turn = 0, item = 0;
-  for (int i = t; i < R * (D / 32); i += kSoftThreads) sh.bad[i / (D / 32)][i % (D / 32)] = 0;
+  for (int i = threadIdx.x; i < R * (D / 32); i += SOFT) sh.bad[i / (D / 32)][i % (D / 32)] = 0;
   for (;; ++item) {
     const Rows<D, R>& of = sh.rows[item % L::Q_BUFS];
-    if (soft_any(!st::mbar_wait_warp(st::smem_u32(&sh.q_full[item % L::Q_BUFS]), item / L::Q_BUFS & 1, &sh.abort))) return;
+    if (soft_any<SOFT>(!st::mbar_wait_warp(st::smem_u32(&sh.q_full[item % L::Q_BUFS]), item / L::Q_BUFS & 1, &sh.abort))) return;
     if (of.item.t1 <= of.item.t0) return;      // no more items
     const int steps = of.item.steps(), t0 = of.item.t0, keys = of.item.keys, next = of.item.next;
     const int limit_min = of.limit[0];      // rows come in order
-    float m[R], l[R];
+    float m[RT], l[RT];
 #pragma unroll
-    for (int r = 0; r < R; ++r) m[r] = kNoMax, l[r] = 0.0f;
+    for (int r = 0; r < RT; ++r) m[r] = kNoMax, l[r] = 0.0f;
 
     for (int i = 0; i < steps; ++i, ++turn) {
       const int slot = turn % L::V_STAGES, key = (t0 + i) * kTile + t;
@@ -566,45 +576,42 @@ __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t 
       const bool there = ve_or_not != kInvalid && key < keys;
       const int ve = there ? ve_or_not : 0;
       const bool gone = (t0 + i + 1) * kTile > limit_min || !there;      // of this unit's keys some row may not see this one
-      float a[R];
-#pragma unroll
-      for (int r = 0; r < R; ++r) a[r] = of.factor[r] * ks;
       st::mbar_wait_warp(st::smem_u32(&sh.s_full[turn & 1]), turn >> 1 & 1, &sh.abort);
       st::tc_fence_after();
-      uint32_t raw[R];
-      tmem_ld_columns<R>(tmem + (turn & 1) * L::S_N, raw);
+      uint32_t raw[RT];
+      tmem_ld_columns<RT>(tmem + (turn & 1) * L::S_N + low, raw);
       st::tmem_ld_wait();
-      float x[R];
+      float x[RT];
       const float lift = static_cast<float>(ve);
 #pragma unroll
-      for (int r = 0; r < R; ++r) x[r] = fmaf(__uint_as_float(raw[r]), a[r], lift);
+      for (int r = 0; r < RT; ++r) x[r] = fmaf(__uint_as_float(raw[r]), of.factor[low + r] * ks, lift);
       if (gone) {
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-          if (!there || key >= of.limit[r]) x[r] = -INFINITY;
+        for (int r = 0; r < RT; ++r)
+          if (!there || key >= of.limit[low + r]) x[r] = -INFINITY;
       }
       float over = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < R; r += 2) over = st::max3(over, x[r] - m[r], x[r + 1] - m[r + 1]);
+      for (int r = 0; r < RT; r += 2) over = st::max3(over, x[r] - m[r], x[r + 1] - m[r + 1]);
       // the reference moves where a weight would be too large; the first unit always sets it
-      if (soft_any(over > kLag)) {
+      if (soft_any<SOFT>(over > kLag)) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
+        for (int r = 0; r < RT; ++r) {
           const float top = warp_top(x[r]);
-          if (lane == 0) sh.m[warp][r] = top;
+          if (lane == 0) sh.m[warp][low + r] = top;
         }
-        soft_sync();
+        soft_sync<SOFT>();
         if (i > 0) {
           st::mbar_wait_warp(st::smem_u32(&sh.pv_done[(turn - 1) & 1]), (turn - 1) >> 1 & 1, &sh.abort);
           st::tc_fence_after();
         }
 #pragma unroll
-        for (int c = 0; c < R / 8; ++c) {
+        for (int c = 0; c < RT / 8; ++c) {
           float b[8];
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
             const int row = 8 * c + r;
-            const float to = fmaxf(m[row], fmaxf(fmaxf(sh.m[0][row], sh.m[1][row]), fmaxf(sh.m[2][row], sh.m[3][row])));
+            const float to = fmaxf(m[row], fmaxf(fmaxf(sh.m[0][low + row], sh.m[1][low + row]), fmaxf(sh.m[2][low + row], sh.m[3][low + row])));
             b[r] = st::exp2_ftz(m[row] - to);
             m[row] = to;
             l[row] *= b[r];
@@ -613,25 +620,25 @@ __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t 
 #pragma unroll
             for (int j = 0; j < kParts; ++j) {
               uint32_t o[8];
-              tmem_ld_8(o_cols + j * R + 8 * c, o);
+              tmem_ld_8(o_cols + j * R + low + 8 * c, o);
               st::tmem_ld_wait();
 #pragma unroll
               for (int r = 0; r < 8; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * b[r]);
-              tmem_st_8(o_cols + j * R + 8 * c, o);
+              tmem_st_8(o_cols + j * R + low + 8 * c, o);
             }
         }
         if (i > 0) st::tmem_st_wait();
-        soft_sync();      // the maxima are read
+        soft_sync<SOFT>();      // the maxima are read
       }
-      if (gone) clean_values<D, R>(sh, of, slot, key, there, limit_min);
+      if (gone && half == 0) clean_values<D, R>(sh, of, slot, key, there, limit_min);
       // the buffer's last products are done
       if constexpr (L::P_BUFS == 2) st::mbar_wait_warp(st::smem_u32(&sh.pv_done[turn & 1]), (turn >> 1 & 1) ^ 1, &sh.abort);
       else if (turn > 0) st::mbar_wait_warp(st::smem_u32(&sh.pv_done[(turn - 1) & 1]), (turn - 1) >> 1 & 1, &sh.abort);
       const float take = st::exp2_int(-ve - static_cast<int>(kLift));
       unsigned char* to = sh.p[turn % L::P_BUFS];
-      const uint32_t row = t / L::SIDES, first = t % L::SIDES * kParts * R;
+      const uint32_t row = t / L::SIDES, first = t % L::SIDES * kParts * R + low;
 #pragma unroll
-      for (int c = 0; c < R / 8; ++c) {
+      for (int c = 0; c < RT / 8; ++c) {
         __half2 w[4];
 #pragma unroll
         for (int r = 0; r < 8; r += 2) {
@@ -659,23 +666,25 @@ __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t 
     float* part = whole ? nullptr : part_of<R>(p, D, 2LL * blockIdx.x + (it.t0 == 0 ? 1 : 0));
     float* room = reinterpret_cast<float*>(sh.p[0]);      // [R][128]
 #pragma unroll
-    for (int r = 0; r < R; ++r) room[r * 128 + t] = l[r];
-    soft_sync();
-    {      // 128 / R threads to a row, R keys each; where they begin keeps them out of one another's banks
-      const int r = t / (128 / R), first = t % (128 / R) * R;
+    for (int r = 0; r < RT; ++r) room[(low + r) * 128 + t] = l[r];
+    soft_sync<SOFT>();
+    {      // SOFT / R threads to a row; where they begin keeps them out of one another's banks
+      constexpr int TPR = SOFT / R, KEYS = 128 / TPR;
+      const int r = threadIdx.x / TPR, first = threadIdx.x % TPR * KEYS;
       float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < R / 4; ++i) {
-        const float4 y = *reinterpret_cast<const float4*>(room + r * 128 + first + 4 * ((i + t) % (R / 4)));
+      for (int i = 0; i < KEYS / 4; ++i) {
+        const float4 y = *reinterpret_cast<const float4*>(room + r * 128 + first + 4 * ((i + t) % (KEYS / 4)));
         sum += (y.x + y.y) + (y.z + y.w);
       }
 #pragma unroll
-      for (int o = 64 / R; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (t % (128 / R) == 0) sh.sum[r] = sum;
+      for (int o = TPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (threadIdx.x % TPR == 0) sh.sum[r] = sum;
     }
-    soft_sync();
+    soft_sync<SOFT>();
+    room += half * 512;
 #pragma unroll
-    for (int c = 0; c < R / 8; ++c) {
+    for (int c = 0; c < RT / 8; ++c) {
       float o[8];
       if constexpr (R == 8) {      // the parts of 8 rows are 32 neighbouring columns
         uint32_t raw[32];
@@ -686,7 +695,7 @@ __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t 
       } else {
         uint32_t raw[kParts][8];
 #pragma unroll
-        for (int j = 0; j < kParts; ++j) tmem_ld_8(o_cols + j * R + 8 * c, raw[j]);
+        for (int j = 0; j < kParts; ++j) tmem_ld_8(o_cols + j * R + low + 8 * c, raw[j]);
         st::tmem_ld_wait();
 #pragma unroll
         for (int r = 0; r < 8; ++r) o[r] = (__uint_as_float(raw[0][r]) + __uint_as_float(raw[1][r])) + (__uint_as_float(raw[2][r]) + __uint_as_float(raw[3][r]));
@@ -695,16 +704,16 @@ __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t 
         if (warp >= 2)
 #pragma unroll
           for (int r = 0; r < 8; ++r) room[r * 64 + t - 64] = o[r];
-        soft_sync();
+        soft_sync<SOFT>();
         if (warp < 2)
 #pragma unroll
           for (int r = 0; r < 8; ++r) o[r] += room[r * 64 + t];
-        if (c + 1 < R / 8) soft_sync();
+        if (c + 1 < RT / 8) soft_sync<SOFT>();
       }
       if (D == 128 || warp < 2) {
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-          const int row = 8 * c + r;
+          const int row = low + 8 * c + r;
           if (row >= rows) continue;
           const float sum = sh.sum[row];
           float y = o[r] * (1.0f / 512.0f);      // 2^-kLift
@@ -712,16 +721,16 @@ __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t 
           if (whole) out[of.place[row] + t] = from_f<T>(sum == 0.0f ? 0.0f : __fdividef(y, sum));
           else part[row * D + t] = y;
           if (t == 0) {
-            if (!whole) part[R * D + row] = m[row], part[R * D + R + row] = sum;
+            if (!whole) part[R * D + row] = m[8 * c + r], part[R * D + R + row] = sum;
             else if (p.lse != nullptr) {
               const int fr = it.row0 + row;
-              p.lse[(it.start + fr / p.group) * static_cast<long long>(p.heads) + it.h * p.group + fr % p.group] = sum == 0.0f ? -INFINITY : (m[row] + log2f(sum)) / kLog2e;
+              p.lse[(it.start + fr / p.group) * static_cast<long long>(p.heads) + it.h * p.group + fr % p.group] = sum == 0.0f ? -INFINITY : (m[8 * c + r] + log2f(sum)) / kLog2e;
             }
           }
         }
       }
     }
-    if (t == 0 && it.t1 < it.tiles) {      // the run ends inside the item
+    if (threadIdx.x == 0 && it.t1 < it.tiles) {      // the run ends inside the item
       // Block b holds a part if its run begins before the item's end, all * b / runs < end, which is all * b < end * runs, and ends behind its first unit.
       const long long first_unit = u1 - it.t1, end = first_unit + it.tiles;
       Note n{};
@@ -732,10 +741,10 @@ __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t 
       *note = n;
     }
     st::tc_fence_before();
-    soft_sync();      // everything of the item is read
+    soft_sync<SOFT>();      // everything of the item is read
     if (next >= u1) return;
-    for (int i = t; i < R * (D / 32); i += kSoftThreads) sh.bad[i / (D / 32)][i % (D / 32)] = 0;
-    if (t == 0) st::mbar_arrive(st::smem_u32(&sh.q_empty[item % L::Q_BUFS]));
+    for (int i = threadIdx.x; i < R * (D / 32); i += SOFT) sh.bad[i / (D / 32)][i % (D / 32)] = 0;
+    if (threadIdx.x == 0) st::mbar_arrive(st::smem_u32(&sh.q_empty[item % L::Q_BUFS]));
   }
 }
 
@@ -758,9 +767,9 @@ __device__ __forceinline__ void zero_rows(const AttnParams& p) {
 }
 
 template <typename T, int D, int R>
-__global__ void __launch_bounds__(kThreads, Layout<D, R, kQueryParts<T>>::BLOCKS) paged_attn_kernel(AttnParams p, const __grid_constant__ CUtensorMap k_map,
+__global__ void __launch_bounds__(kThreadsOf<R>, Layout<D, R, kQueryParts<T>>::BLOCKS) paged_attn_kernel(AttnParams p, const __grid_constant__ CUtensorMap k_map,
                                                                                                      const __grid_constant__ CUtensorMap v_map) {
-  constexpr int QP = kQueryParts<T>;
+  constexpr int QP = kQueryParts<T>, SW = kSoftWarps<R>;
   using L = Layout<D, R, QP>;
   extern __shared__ __align__(1024) unsigned char raw[];      // swizzles count rows from multiples of 1024
   using S = Shared<D, R, QP>;
@@ -773,7 +782,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, R, kQueryParts<T>>::BLOCKS
     for (int i = 0; i < L::V_STAGES; ++i) st::mbar_init(st::smem_u32(&sh.v_full[i]), 1), st::mbar_init(st::smem_u32(&sh.v_empty[i]), 1);
     for (int i = 0; i < 2; ++i) {
       st::mbar_init(st::smem_u32(&sh.s_full[i]), 1);
-      st::mbar_init(st::smem_u32(&sh.p_full[i]), kSoftThreads);
+      st::mbar_init(st::smem_u32(&sh.p_full[i]), 32 * SW);
       st::mbar_init(st::smem_u32(&sh.pv_done[i]), 1);
     }
     for (int i = 0; i < L::Q_BUFS; ++i) st::mbar_init(st::smem_u32(&sh.q_full[i]), 1), st::mbar_init(st::smem_u32(&sh.q_empty[i]), 1);
@@ -782,7 +791,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, R, kQueryParts<T>>::BLOCKS
   }
   chain_begin(p.ks, p.vs, p.table, p.starts, p.lengths);
 
-  if (warp == 5) {
+  if (warp == SW + 1) {
     st::tmem_alloc(st::smem_u32(&sh.tmem), L::COLUMNS);
     st::tmem_relinquish();
   }
@@ -793,33 +802,34 @@ __global__ void __launch_bounds__(kThreads, Layout<D, R, kQueryParts<T>>::BLOCKS
   const bool share = find_share<R>(p, sh.sums, &sh.found, all, runs, u0, u1, f);
   st::tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  if (p.zero_tail && warp == 7) zero_rows<T, D>(p);
+  if (p.zero_tail && warp == SW + 3) zero_rows<T, D>(p);
   if (threadIdx.x == 0) note->parts = 0;
   if (!share) {
-    if (warp == 5) st::tmem_dealloc(tmem, L::COLUMNS);
+    if (warp == SW + 1) st::tmem_dealloc(tmem, L::COLUMNS);
     return;
   }
   const Seq sq = sequence<R>(p, f.b);
-  // With 16 rows and more the softmax takes registers from the other warps: 176 and 80 of the 128 of the launch (one warp does nothing else).
+  // With 16 rows and more the softmax takes registers from the other warps: 176 and 80 of the 128 of the launch, with 32 rows 88
+  // (of two warpgroups) and 64 of 80.
   constexpr bool kShift = R >= 16 && L::BLOCKS == 2;
-  if (warp >= 4) {
-    if constexpr (kShift) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == 4) {
+  if (warp >= SW) {
+    if constexpr (kShift) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R == 32 ? 64 : 80));
+    if (warp == SW) {
       copy_warp<L, D, R>(sh, p, &k_map, &v_map, u0, u1, f, sq);
-    } else if (warp == 5) {
+    } else if (warp == SW + 1) {
       if (lane == 0) product_warp<L, D, R, QP>(sh, tmem, u1);
       __syncwarp();
-    } else if (warp == 6) {
+    } else if (warp == SW + 2) {
       query_warp<T, L, D, R, QP>(sh, p, u0, u1, f, sq);
     }
   } else {
-    if constexpr (kShift) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    if constexpr (kShift) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R == 32 ? 88 : 176));
     soft_warps<T, L, D, R>(sh, p, tmem, note, u1, runs, all);
     if (threadIdx.x == 0 && sh.abort) st::report_error(p.err, st::ERR_MBAR_TIMEOUT, 0x7005);
   }
   st::tc_fence_before();
   __syncthreads();
-  if (warp == 5) st::tmem_dealloc(tmem, L::COLUMNS);
+  if (warp == SW + 1) st::tmem_dealloc(tmem, L::COLUMNS);
 }
 
 // Joins the parts of the items that several blocks worked on.  A block per border; an item of P parts has P - 1 of them, which share its rows.
@@ -934,7 +944,7 @@ int launch(const AttnParams& p, cudaStream_t stream) {
     done = true;
   }
   // in order: blocks that come early pile up on the SMs that fall free first
-  cudaError_t e = st::in_order(kernel, dim3(runs), dim3(kThreads), smem, stream)(p, maps[0], maps[1]);
+  cudaError_t e = st::in_order(kernel, dim3(runs), dim3(kThreadsOf<R>), smem, stream)(p, maps[0], maps[1]);
   if (e != cudaSuccess) return st::fail_cuda(e, "paged attention");
   e = st::chained(paged_join_kernel<T, D, R>, dim3(runs - 1), dim3(kJoinThreads), runs * sizeof(float), stream)(p);
   if (e != cudaSuccess) return st::fail_cuda(e, "paged attention: join");
