@@ -114,8 +114,9 @@ def plan(lengths: torch.Tensor, added: torch.Tensor, table: torch.Tensor, free: 
     index = native.require_cuda("paged.plan", lengths, added, table, free, free_count)
     if B > _max_sequences():
         raise ValueError(f"paged.plan: {B} sequences, at most {_max_sequences()}")
-    step = Step(free_count.new_empty(B + 1), free_count.new_empty(rows), free_count.new_empty(rows, dtype=torch.int64), free_count.new_empty(B),
-                torch.empty_like(free_count))
+    # one allocation for the 32-bit results: five of them take as long as the launch twice
+    positions, starts, after, left = free_count.new_empty(rows + 2 * B + 2).split_with_sizes((rows, B + 1, B, 1))
+    step = Step(starts, positions, free_count.new_empty(rows, dtype=torch.int64), after, left)
     with native.on_device(index):
         st = native.entry("st_paged_plan", "pppqippiiiqpppppp")(
             lengths.data_ptr(), added.data_ptr(), table.data_ptr(), table.stride(0), width, free.data_ptr(), free_count.data_ptr(), free.shape[0],

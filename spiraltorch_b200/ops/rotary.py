@@ -122,33 +122,36 @@ def _apply(q, k, positions, freq, interleaved, magnitude, backward):
     if not native.use_native(q):
         return tuple(None if x is None else rotary_reference(x, positions, freq, interleaved, magnitude, backward) for x in (q, k))
     qo, ko = _like(q), None if k is None else _like(k)
-    _launch(_rows(q, "q"), None if k is None else _rows(k, "k"), _rows(qo, "q"), None if k is None else _rows(ko, "k"), positions.contiguous(), freq,
-            interleaved, magnitude, backward)
+    _launch(_rows(q, "q"), None if k is None else _rows(k, "k"), qo if qo.dim() == 3 else _rows(qo, "q"), ko if ko is None or ko.dim() == 3 else _rows(ko, "k"),
+            positions.contiguous(), freq, interleaved, magnitude, backward)
     return qo, ko
 
 
 class _RotaryFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, positions, freq, interleaved, magnitude, backward):
+    def forward(ctx, q, k, positions, freq, form):
         ctx.save_for_backward(positions, freq)
-        ctx.form = (interleaved, magnitude, not backward)
+        ctx.form = form
         ctx.set_materialize_grads(False)
-        return _apply(q, k, positions, freq, interleaved, magnitude, backward)
+        return _apply(q, k, positions, freq, *form)
 
     @staticmethod
     def backward(ctx, dq, dk):
-        given = [g if g is None or g.stride(-1) == 1 else g.contiguous()
-                 for g in (dq if ctx.needs_input_grad[0] else None, dk if ctx.needs_input_grad[1] else None)]
-        first, second = given if given[0] is not None else (given[1], None)
-        if first is None:
-            return (None,) * 7
-        out = _rotate(first, second, *ctx.saved_tensors, *ctx.form)
-        return (out if given[0] is not None else (None, out[0])) + (None,) * 5
+        need_q, need_k, *_ = ctx.needs_input_grad
+        dq, dk = (g if need and (g is None or g.stride()[-1] == 1) else g.contiguous() if need and g is not None else None
+                  for g, need in ((dq, need_q), (dk, need_k)))
+        if dq is None and dk is None:
+            return None, None, None, None, None
+        interleaved, magnitude, back = ctx.form
+        positions, freq = ctx.saved_tensors
+        if dq is None:
+            return None, _rotate(dk, None, positions, freq, interleaved, magnitude, not back)[0], None, None, None
+        return *_rotate(dq, dk, positions, freq, interleaved, magnitude, not back), None, None, None
 
 
 def _rotate(q, k, positions, freq, interleaved, magnitude, backward):
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _RotaryFn.apply(q, k, positions, freq, interleaved, magnitude, backward)
+        return _RotaryFn.apply(q, k, positions, freq, (interleaved, magnitude, backward))
     return _apply(q, k, positions, freq, interleaved, magnitude, backward)
 
 
