@@ -14,6 +14,9 @@
 // and a second kernel joins the parts of such items in their order, so results do not depend on timing.  It finds them by the notes
 // that the blocks leave about the border between their run and the next.
 //
+// Where the table holds few units for a sequence, an item is not split: nothing has to be joined then, and a block is through with it in the time
+// that the second kernel takes.
+//
 // Products.  Both run on tcgen05 with the codes as they lie in the cache: no code is ever converted or passes through a register.  A unit's keys
 // are the 128 rows of S^T = K Q^T (keys in lanes, so a thread has all rows' scores of its key), its values, read along the tokens,
 // those of O^T = V^T P^T.  The other operands, queries and weights, are fp16 numbers written as sums of e5m2 numbers, whose three
@@ -60,7 +63,7 @@ struct AttnParams {
   long long rows;      // of q and out
   int width, shift, B, heads, kv_heads, group;
   float scale;
-  int causal, zero_tail;
+  int causal, zero_tail, whole;      // whole: items are not split
   unsigned* err;
 };
 
@@ -68,7 +71,7 @@ struct AttnParams {
 template <int N> constexpr int kItemCost = N == 32 ? 4 : 2;
 
 struct Seq {
-  int start, n, len, row_blocks, tiles, units;
+  int start, n, len, row_blocks, tiles, size, units;      // size: what an item counts
 };
 template <int N>
 __device__ __forceinline__ Seq sequence(const AttnParams& p, int b) {
@@ -79,7 +82,8 @@ __device__ __forceinline__ Seq sequence(const AttnParams& p, int b) {
   s.len = min(len, p.width << p.shift);
   s.row_blocks = (s.n * p.group + N - 1) / N;
   s.tiles = max((s.len + kTile - 1) / kTile, 1);      // a sequence without keys still gets its zero rows
-  s.units = s.row_blocks * (s.tiles + kItemCost<N>) * p.kv_heads;
+  s.size = p.whole ? 1 : s.tiles + kItemCost<N>;
+  s.units = s.row_blocks * s.size * p.kv_heads;
   return s;
 }
 
@@ -172,10 +176,10 @@ __device__ __forceinline__ bool item_at(Item& it, const AttnParams& p, int u, in
       sq = sequence<N>(p, ++f.b);
     }
     // unit -> (key head, row block, tile): row blocks of one head next to each other, as they read the same pages
-    const unsigned size = sq.tiles + kItemCost<N>, in = u - f.first, item = in / size;
+    const unsigned size = sq.size, in = u - f.first, item = in / size;
     const int at = in - item * size, end = min(static_cast<int>(size), at + (u1 - u));
     u += end - at;
-    it.t0 = max(at - kItemCost<N>, 0), it.t1 = end - kItemCost<N>;
+    it.t0 = p.whole ? 0 : max(at - kItemCost<N>, 0), it.t1 = p.whole ? sq.tiles : end - kItemCost<N>;
     if (it.t1 <= it.t0) continue;      // nothing but the count for its beginning
     it.next = u;
     it.h = item / static_cast<unsigned>(sq.row_blocks);
@@ -312,7 +316,7 @@ struct Shared {
 };
 static_assert(sizeof(Shared<128, 8, 3>) <= 113 * 1024 && sizeof(Shared<128, 16, 3>) <= 113 * 1024 && sizeof(Shared<128, 32, 3>) <= 113 * 1024 && sizeof(Shared<128, 8, 4>) <= 113 * 1024 &&
               sizeof(Shared<128, 16, 4>) <= 113 * 1024 && sizeof(Shared<128, 32, 4>) <= 113 * 1024 && sizeof(Shared<64, 16, 4>) <= 113 * 1024 && sizeof(Shared<64, 32, 4>) <= 226 * 1024);
-constexpr int kInvalid = -1000;
+constexpr int kInvalid = -1000, kBehind = -2147483647 - 1;      // of a page: none by that number; none, as the keys end before it
 
 // What a block notes about the border behind its run: the item that it is inside of (parts 0: none).
 struct Note {
@@ -328,51 +332,67 @@ __device__ __forceinline__ float* part_of(const AttnParams& p, int D, long long 
 }
 
 // ---- the copying warp -------------------------------------------------------------------------------------------------------------
+// Page numbers and scales are looked up for 32 pages at a time (4 units of 8 pages of 16 tokens to 32 units of one page), a batch ahead of the
+// copies: two loads that wait for one another, 1400 cycles, at every unit set the pace before.
 template <typename L, int D, int R, typename S>
 __device__ __forceinline__ void copy_warp(S& sh, const AttnParams& p, const CUtensorMap* km, const CUtensorMap* vm, int u0, int u1, Found f, Seq sq) {
-  const int lane = threadIdx.x & 31, rows = min(1 << p.shift, kTile), pages = kTile / rows;
-  struct Next {
-    int page, ve;
-    float ks;
+  const int lane = threadIdx.x & 31, rows = min(1 << p.shift, kTile), pages = kTile / rows, units = 32 / pages, mine = lane / pages, at_page = lane % pages;
+  struct Batch {
+    int t, n, h;      // units [t, t + n) of an item (n 0: the end), its key head
+    int page;         // the lane's: page lane % pages of unit lane / pages; -1: none
   };
-  auto look = [&](const Item& it, int t) {      // lane j: page j of the unit
-    const int key = t * kTile + lane * rows;
-    Next n{-1, kInvalid, 0.0f};
-    if (lane < pages && key < it.keys) {
-      const int page = it.table[key >> p.shift];
-      if (page < 0 || page >= p.pages) {
-        st::report_error(p.err, st::ERR_BOUNDS, 0x7004);
-      } else {
-        const long long at = static_cast<long long>(page) * p.kv_heads + it.h;
-        n.page = page, n.ks = p.ks[at], n.ve = st::scale_exponent(p.vs[at]);
-      }
+  Item it;
+  int t = 0, end = 0;      // the next batch's place in `it`
+  int u = u0;
+  auto look_pages = [&]() {
+    Batch b{0, 0, 0, -1};
+    if (t >= end) {
+      if (!item_at<R>(it, p, u, u1, f, sq)) return b;
+      u = it.next, t = it.t0, end = it.t0 + it.steps();
     }
-    return n;
+    b.t = t, b.n = min(units, end - t), b.h = it.h;
+    const int key = (t + mine) * kTile + at_page * rows;
+    if (mine < b.n && key < it.keys) b.page = it.table[key >> p.shift];
+    else b.page = kBehind;
+    t += b.n;
+    return b;
+  };
+  auto look_scales = [&](Batch& b, float& ks, int& ve) {
+    ks = 0.0f, ve = kInvalid;
+    if (b.page < 0 || b.page >= p.pages) {
+      if (b.n > 0 && b.page != kBehind) st::report_error(p.err, st::ERR_BOUNDS, 0x7004);
+      b.page = -1;
+      return;
+    }
+    const long long at = static_cast<long long>(b.page) * p.kv_heads + b.h;
+    ks = p.ks[at], ve = st::scale_exponent(p.vs[at]);
   };
   uint32_t turn = 0;
-  Item it;
-  for (int u = u0; item_at<R>(it, p, u, u1, f, sq); u = it.next) {
-    const int steps = it.steps();
-    Next next = look(it, it.t0);
-    for (int i = 0; i < steps; ++i, ++turn) {
-      const Next n = next;
-      const int t = it.t0 + i;
-      if (i + 1 < steps) next = look(it, t + 1);
-      const int ks = turn % L::K_STAGES, vs = turn % L::V_STAGES;
-      const uint32_t live = __ballot_sync(0xffffffffu, n.page >= 0);
-      const uint32_t bytes = __popc(live) * rows * D;
-      const long long token = ((static_cast<long long>(n.page) * p.kv_heads + it.h) << p.shift) + ((t * kTile + lane * rows) & ((1 << p.shift) - 1));
-      if (!st::mbar_wait_warp(st::smem_u32(&sh.k_empty[ks]), (turn / L::K_STAGES & 1) ^ 1, &sh.abort)) return;
-      if (lane == 0) st::mbar_arrive_expect_tx(st::smem_u32(&sh.k_full[ks]), bytes);
+  Batch now = look_pages();
+  float ks, ks_next = 0.0f;
+  int ve, ve_next = kInvalid;
+  look_scales(now, ks, ve);
+  while (now.n > 0) {
+    Batch next = look_pages();
+    const long long first = (static_cast<long long>(now.page) * p.kv_heads + now.h) << p.shift;
+    for (int i = 0; i < now.n; ++i, ++turn) {
+      const int kslot = turn % L::K_STAGES, vslot = turn % L::V_STAGES;
+      const bool live = mine == i && now.page >= 0;
+      const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, live)) * rows * D;
+      const long long token = first + (((now.t + i) * kTile + at_page * rows) & ((1 << p.shift) - 1));
+      if (!st::mbar_wait_warp(st::smem_u32(&sh.k_empty[kslot]), (turn / L::K_STAGES & 1) ^ 1, &sh.abort)) return;
+      if (lane == 0) st::mbar_arrive_expect_tx(st::smem_u32(&sh.k_full[kslot]), bytes);
       __syncwarp();
-      if (n.page >= 0) st::tma_load_2d(st::smem_u32(sh.k[ks]) + lane * rows * D, km, st::smem_u32(&sh.k_full[ks]), 0, static_cast<int>(token));
-      if (!st::mbar_wait_warp(st::smem_u32(&sh.v_empty[vs]), (turn / L::V_STAGES & 1) ^ 1, &sh.abort)) return;
-      if (lane < pages) sh.ks[vs][lane] = n.ks, sh.ve[vs][lane] = n.ve;
+      if (live) st::tma_load_2d(st::smem_u32(sh.k[kslot]) + at_page * rows * D, km, st::smem_u32(&sh.k_full[kslot]), 0, static_cast<int>(token));
+      if (!st::mbar_wait_warp(st::smem_u32(&sh.v_empty[vslot]), (turn / L::V_STAGES & 1) ^ 1, &sh.abort)) return;
+      if (mine == i) sh.ks[vslot][at_page] = ks, sh.ve[vslot][at_page] = ve;
       __syncwarp();
-      if (lane == 0) st::mbar_arrive_expect_tx(st::smem_u32(&sh.v_full[vs]), bytes);
+      if (lane == 0) st::mbar_arrive_expect_tx(st::smem_u32(&sh.v_full[vslot]), bytes);
       __syncwarp();
-      if (n.page >= 0) st::tma_load_2d(st::smem_u32(sh.v[vs]) + lane * rows * D, vm, st::smem_u32(&sh.v_full[vs]), 0, static_cast<int>(token * D / 128));
+      if (live) st::tma_load_2d(st::smem_u32(sh.v[vslot]) + at_page * rows * D, vm, st::smem_u32(&sh.v_full[vslot]), 0, static_cast<int>(token * D / 128));
+      if (i == 0) look_scales(next, ks_next, ve_next);      // the page numbers have come by now
     }
+    now = next, ks = ks_next, ve = ve_next;
   }
 }
 
@@ -730,7 +750,7 @@ __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t 
         }
       }
     }
-    if (threadIdx.x == 0 && it.t1 < it.tiles) {      // the run ends inside the item
+    if (threadIdx.x == 0 && it.t1 < it.tiles) {      // the run ends inside the item; never where items are whole, which have no notes
       // Block b holds a part if its run begins before the item's end, all * b / runs < end, which is all * b < end * runs, and ends behind its first unit.
       const long long first_unit = u1 - it.t1, end = first_unit + it.tiles;
       Note n{};
@@ -803,7 +823,7 @@ __global__ void __launch_bounds__(kThreadsOf<R>, Layout<D, R, kQueryParts<T>>::B
   st::tc_fence_after();
   const uint32_t tmem = sh.tmem;
   if (p.zero_tail && warp == SW + 3) zero_rows<T, D>(p);
-  if (threadIdx.x == 0) note->parts = 0;
+  if (threadIdx.x == 0 && !p.whole) note->parts = 0;
   if (!share) {
     if (warp == SW + 1) st::tmem_dealloc(tmem, L::COLUMNS);
     return;
@@ -922,6 +942,10 @@ int item_rows(long long max_queries, int group) {
 // Blocks that run at once: two to an SM, one where the products take all columns of tensor memory.
 int runs_of(int rows, int dim) { return st::sm_count() * (dim == 64 && rows == 32 ? Layout<64, 32, 4>::BLOCKS : Layout<128, 32, 4>::BLOCKS); }
 
+// Whether items of sequences of up to `tokens` tokens are whole: a unit takes a block 1000 cycles, of 32 rows 2500, the second kernel and what it waits for
+// 6 us of the GPU and 4 of the host.
+bool not_split(int rows, long long tokens) { return tokens <= (rows == 32 ? 18 : 7) * kTile; }
+
 template <typename T, int D, int R>
 int launch(const AttnParams& p, cudaStream_t stream) {
   const int runs = runs_of(R, D);
@@ -946,6 +970,7 @@ int launch(const AttnParams& p, cudaStream_t stream) {
   // in order: blocks that come early pile up on the SMs that fall free first
   cudaError_t e = st::in_order(kernel, dim3(runs), dim3(kThreadsOf<R>), smem, stream)(p, maps[0], maps[1]);
   if (e != cudaSuccess) return st::fail_cuda(e, "paged attention");
+  if (p.whole) return ST_OK;
   e = st::chained(paged_join_kernel<T, D, R>, dim3(runs - 1), dim3(kJoinThreads), runs * sizeof(float), stream)(p);
   if (e != cudaSuccess) return st::fail_cuda(e, "paged attention: join");
   return ST_OK;
@@ -957,8 +982,8 @@ int dispatch(const AttnParams& p, int rows, cudaStream_t stream) {
 }  // namespace
 
 // Floats of workspace that st_paged_attention takes.
-ST_API long long st_paged_attention_workspace(int max_queries, int heads, int kv_heads, int dim) {
-  if (kv_heads < 1 || heads < kv_heads) return 0;
+ST_API long long st_paged_attention_workspace(int max_queries, int heads, int kv_heads, int dim, int width, int page_size) {
+  if (kv_heads < 1 || heads < kv_heads || not_split(item_rows(max_queries, heads / kv_heads), static_cast<long long>(width) * page_size)) return 0;
   const int r = item_rows(max_queries, heads / kv_heads);
   return (2LL * r * (dim + 2) + sizeof(Note) / sizeof(float)) * runs_of(r, dim);
 }
@@ -983,7 +1008,7 @@ ST_API int st_paged_attention(const void* q, const void* k_codes, const void* v_
     return st::fail(ST_ERR_TOO_LARGE, "paged attention: rows times the table's width is too large for one call");
   int* notes = reinterpret_cast<int*>(workspace + 2LL * r * (dim + 2) * runs_of(r, dim));      // behind the parts
   const AttnParams p{q, static_cast<const unsigned char*>(k_codes), static_cast<const unsigned char*>(v_codes), k_scale, v_scale, table, starts, lengths, out, lse, workspace, notes,
-                     q_row, q_head, o_row, o_head, table_row, pages, rows, width, shift, B, heads, kv_heads, heads / kv_heads, scale, causal, zero_tail, st::error_word()};
+                     q_row, q_head, o_row, o_head, table_row, pages, rows, width, shift, B, heads, kv_heads, heads / kv_heads, scale, causal, zero_tail, not_split(r, static_cast<long long>(width) << shift), st::error_word()};
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
   if (type == 0) return dim == 64 ? dispatch<__nv_bfloat16, 64>(p, r, stream) : dispatch<__nv_bfloat16, 128>(p, r, stream);
   return dim == 64 ? dispatch<__half, 64>(p, r, stream) : dispatch<__half, 128>(p, r, stream);

@@ -308,7 +308,7 @@ int st_norm_gelu_bwd(const void* dy, const void* x, const void* gamma, const voi
 int st_norm_gelu_fwd(const void* x, const void* gamma, const void* beta, void* y, float* mean, float* rstd, int rows, int d, float eps, void* stream_v);   /* csrc/norm/norm.cu */
 int st_norm_gelu_max_features();   /* csrc/norm/norm.cu */
 int st_paged_attention(const void* q, const void* k_codes, const void* v_codes, const float* k_scale, const float* v_scale, const int* table, const int* starts, const int* lengths, void* out, float* lse, float* workspace, long long q_row, long long q_head, long long o_row, long long o_head, long long table_row, long long pages, long long rows, int width, int page_size, int B, int heads, int kv_heads, int dim, int max_queries, float scale, int causal, int zero_tail, int type, void* stream_v);   /* csrc/serving/paged_attn.cu */
-long long st_paged_attention_workspace(int max_queries, int heads, int kv_heads, int dim);   /* csrc/serving/paged_attn.cu */
+long long st_paged_attention_workspace(int max_queries, int heads, int kv_heads, int dim, int width, int page_size);   /* csrc/serving/paged_attn.cu */
 int st_paged_max_sequences();   /* csrc/serving/paged_cache.cu */
 int st_paged_plan(const int* lengths, const int* added, int* table, long long table_row, int width, const int* free_list, const int* free_count, int free_size, int page_size, int B, long long rows, int* starts, int* positions, long long* slots, int* lengths_after, int* free_after, void* stream_v);   /* csrc/serving/paged_cache.cu */
 int st_paged_read(const void* k_codes, const void* v_codes, const float* k_scale, const float* v_scale, const int* table, const int* lengths, long long table_row, int width, int B, int room, int kv_heads, int dim, int page_size, long long pages, void* k_out, void* v_out, int wide_out, void* stream_v);   /* csrc/serving/paged_cache.cu */

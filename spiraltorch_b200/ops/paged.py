@@ -295,11 +295,11 @@ def _dense_reference(codes, scale, table, lengths, max_length, dtype=torch.float
 
 
 # ---- attention ------------------------------------------------------------------------------------------------------------------
-@functools.cache
-def _workspace(max_queries: int, heads: int, kv_heads: int, dim: int, index: int) -> int:
-    size = native.entry("st_paged_attention_workspace", "iiii")
+@functools.lru_cache(maxsize=1024)
+def _workspace(max_queries: int, heads: int, kv_heads: int, dim: int, width: int, page: int, index: int) -> int:
+    size = native.entry("st_paged_attention_workspace", "iiiiii")
     size.restype = ctypes.c_longlong
-    return size(max_queries, heads, kv_heads, dim)
+    return size(max_queries, heads, kv_heads, dim, width, page)
 
 
 def attention(q: torch.Tensor, pages: Pages, table: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, *, max_queries: int, causal: bool = True,
@@ -350,13 +350,14 @@ def attention(q: torch.Tensor, pages: Pages, table: torch.Tensor, starts: torch.
     o = (torch.empty_like(q) if q.is_contiguous() else q.new_empty((rows, H, D))) if out is None else out
     lse = pages.k_scale.new_empty((rows, H)) if return_lse else None
     with native.on_device(index):
-        work = pages.k_scale.new_empty(_workspace(max_queries, H, Hk, D, index))
+        room = _workspace(max_queries, H, Hk, D, width, page, index)
+        work = pages.k_scale.new_empty(room) if room else None
         st = native.entry("st_paged_attention", "pppppppppppqqqqqqqiiiiiiifiiip")(
             q.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), table.data_ptr(), starts.data_ptr(),
-            lengths.data_ptr(), o.data_ptr(), native.address(lse), work.data_ptr(), *q.stride()[:2], *o.stride()[:2], table.stride(0), P, rows,
+            lengths.data_ptr(), o.data_ptr(), native.address(lse), native.address(work), *q.stride()[:2], *o.stride()[:2], table.stride(0), P, rows,
             width, page, B, H, Hk, D, max_queries, scale, int(causal), int(out is None), int(q.dtype == torch.float16), native.raw_stream(index))
     native.check(st, "st_paged_attention")
-    launch_count += 2
+    launch_count += 2 if room else 1
     return (o, lse) if return_lse else o
 
 
