@@ -21,7 +21,7 @@
 // are the 128 rows of S^T = K Q^T (keys in lanes, so a thread has all rows' scores of its key), its values, read along the tokens,
 // those of O^T = V^T P^T.  The other operands, queries and weights, are fp16 numbers written as sums of e5m2 numbers, whose three
 // significant bits are those of fp16's upper byte: the byte, the byte of what it leaves, and so on; three hold bf16's 8 bits, four fp16's
-// 11.  Queries' parts follow one another in the sum over K, weights' parts side by side in N, added when the item is done.  So the products are exact
+// 11.  The parts stand side by side in N; those of a score are added by its thread, those of an output when the item is done.  So the products are exact
 // and a unit costs a warp about 150 instructions instead of the 650 of mma.sync on converted codes (64 sequences: 78 us alone).
 // Queries are scaled by a power of two per row to use fp16's range.  The softmax runs over x + b instead of x (b: the page's value
 // exponent): the weights exp2(x + b - M) are those that multiply the codes, and the sum takes exp2(-b) back out.  M is not the running
@@ -209,12 +209,12 @@ constexpr uint32_t codes_idesc(int M, int N, bool mn_major) {
          (static_cast<uint32_t>(M >> 4) << 24);
 }
 // Descriptor of a tile whose rows are WIDTH bytes, swizzled over that width: rows of K-major operands, or the K of MN-major ones; 8 rows are a group.
-// `block`: distance of the next WIDTH bytes along M or N; `group`: of the next 8 rows.
+// `block`: distance of the next WIDTH bytes along M or N.
 template <int WIDTH>
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t block = 16, uint32_t group = 8 * WIDTH) {
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t block = 16) {
   static_assert(WIDTH == 32 || WIDTH == 64 || WIDTH == 128);
   constexpr uint64_t kind = WIDTH == 128 ? 2 : WIDTH == 64 ? 4 : 6;
-  return ((addr & 0x3FFFF) >> 4) | static_cast<uint64_t>(block >> 4) << 16 | static_cast<uint64_t>(group >> 4) << 32 | 1ull << 46 | kind << 61;
+  return ((addr & 0x3FFFF) >> 4) | static_cast<uint64_t>(block >> 4) << 16 | static_cast<uint64_t>(8 * WIDTH >> 4) << 32 | 1ull << 46 | kind << 61;
 }
 // Byte of 16-byte part `part` of row `row` in such a tile.
 template <int WIDTH>
@@ -270,7 +270,10 @@ template <> constexpr int kQueryParts<__half> = 4;
 
 template <int D, int R, int QP>
 struct Layout {
-  static constexpr int S_N = R < 16 ? 16 : R;                          // columns of the scores
+  // Parts of the queries that stand side by side in N; with 32 rows two, as tensor memory has no room for more, and the others follow in the sum.
+  // (One product of N = 16 takes 90 cycles before the next can add to it: with all 12 of a unit in a row it took a block 1900 cycles.)
+  static constexpr int WAYS = R == 32 ? 2 : QP, SETS = (QP + WAYS - 1) / WAYS;
+  static constexpr int S_N = (WAYS * R + 15) / 16 * 16;                // columns of the scores
   static constexpr int SIDES = D == 64 ? 2 : 1;                        // tokens side by side
   static constexpr int P_N = SIDES * kParts * R;                       // columns of the products with values
   static constexpr int P_WIDTH = P_N < 128 ? P_N : 128;                // bytes of a swizzled row of weights
@@ -278,7 +281,7 @@ struct Layout {
   static constexpr int P_BYTES = P_ROWS * P_N;
   static constexpr int COLUMNS = 2 * S_N + P_N <= 64 ? 64 : 2 * S_N + P_N <= 128 ? 128 : 2 * S_N + P_N <= 256 ? 256 : 512;
   static constexpr int BLOCKS = COLUMNS == 512 ? 1 : 2;                // of an SM
-  static constexpr int Q_BYTES = QP * R * D;                           // 8 rows stand for 16 columns, see product_warp
+  static constexpr int Q_BYTES = QP * R * D;
   // What fits the shared memory of two blocks (111 KB each, 2 KB of them for the small things): queries twice before a third stage of values, that
   // before weights twice, and a third one of keys last.
   static constexpr int ROOM = (BLOCKS == 2 ? 113 * 1024 : 226 * 1024) - 3072, ONE = kTile * D;
@@ -397,21 +400,23 @@ __device__ __forceinline__ void copy_warp(S& sh, const AttnParams& p, const CUte
 }
 
 // ---- the warp that issues products (one lane) -------------------------------------------------------------------------------------
-// Scores take 16 columns at least: with 8 rows the second group of eight is the first one again (a distance of 0), and nobody reads it.
+// N is a multiple of 16: three parts of 8 rows are followed by 8 columns that nobody reads, from whatever lies behind them.
 template <typename L, int D, int R, int QP, typename S>
 __device__ __forceinline__ void product_warp(S& sh, uint32_t tmem, int u1) {
-  constexpr uint32_t s_idesc = codes_idesc(128, L::S_N, false), p_idesc = codes_idesc(128, L::P_N, true);
+  constexpr uint32_t p_idesc = codes_idesc(128, L::P_N, true);
   uint32_t turn = 0, item = 0;
   auto ask_scores = [&](uint32_t t, uint32_t of) {
     const int slot = t % L::K_STAGES;
     if (!st::mbar_wait(st::smem_u32(&sh.k_full[slot]), t / L::K_STAGES & 1, &sh.abort)) return false;
     st::tc_fence_after();
 #pragma unroll
-    for (int i = 0; i < QP; ++i)
+    for (int i = 0; i < L::SETS; ++i) {
+      const int ways = min(L::WAYS, QP - i * L::WAYS);
 #pragma unroll
       for (int k = 0; k < D / 32; ++k)
-        umma_codes(tmem + (t & 1) * L::S_N, tile_desc<D>(st::smem_u32(sh.k[slot])) + 2 * k,
-                   tile_desc<D>(st::smem_u32(sh.q[of % L::Q_BUFS][i]), 16, R == 8 ? 0 : 8 * D) + 2 * k, s_idesc, i + k > 0);
+        umma_codes(tmem + (t & 1) * L::S_N, tile_desc<D>(st::smem_u32(sh.k[slot])) + 2 * k, tile_desc<D>(st::smem_u32(sh.q[of % L::Q_BUFS][i * L::WAYS])) + 2 * k,
+                   codes_idesc(128, (ways * R + 15) / 16 * 16, false), i + k > 0);
+    }
     st::umma_commit(st::smem_u32(&sh.s_full[t & 1]));
     st::umma_commit(st::smem_u32(&sh.k_empty[slot]));
     return true;
@@ -598,13 +603,19 @@ __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t 
       const bool gone = (t0 + i + 1) * kTile > limit_min || !there;      // of this unit's keys some row may not see this one
       st::mbar_wait_warp(st::smem_u32(&sh.s_full[turn & 1]), turn >> 1 & 1, &sh.abort);
       st::tc_fence_after();
-      uint32_t raw[RT];
-      tmem_ld_columns<RT>(tmem + (turn & 1) * L::S_N + low, raw);
+      uint32_t raw[L::WAYS][RT];
+#pragma unroll
+      for (int w = 0; w < L::WAYS; ++w) tmem_ld_columns<RT>(tmem + (turn & 1) * L::S_N + w * R + low, raw[w]);
       st::tmem_ld_wait();
       float x[RT];
       const float lift = static_cast<float>(ve);
 #pragma unroll
-      for (int r = 0; r < RT; ++r) x[r] = fmaf(__uint_as_float(raw[r]), of.factor[low + r] * ks, lift);
+      for (int r = 0; r < RT; ++r) {
+        float sum = __uint_as_float(raw[L::WAYS - 1][r]);      // the smallest first
+#pragma unroll
+        for (int w = L::WAYS - 2; w >= 0; --w) sum += __uint_as_float(raw[w][r]);
+        x[r] = fmaf(sum, of.factor[low + r] * ks, lift);
+      }
       if (gone) {
 #pragma unroll
         for (int r = 0; r < RT; ++r)
