@@ -28,8 +28,8 @@
 // maximum but some number that no x + b exceeds by more than 6: it moves, and the outputs with it, in the first unit and rarely after, and the
 // weights, times 2^9, stay below 2^15.
 //
-// Blocks: four warps for the softmax, one that copies (a tiled copy per page and unit), one that issues products, one that prepares the queries
-// of the next item, so that a run's items follow one another without a pause: with that in the softmax warps' way an item cost them 4500 cycles more.  Heads of 64: the copies lay two tokens
+// Blocks: four warps for the softmax, one that copies keys (a tiled copy per page and unit) and issues scores, one that copies values, one that
+// issues the products with them, one that prepares the queries of the next item, so that a run's items follow one another without a pause: with that in the softmax warps' way an item cost them 4500 cycles more.  Heads of 64: the copies lay two tokens
 // side by side, 64 rows of 128, and the weights of even and odd tokens have columns of their own; half of each product is not used.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -42,7 +42,7 @@ using st::chain_begin;
 
 constexpr int kTile = 128;            // keys of a unit
 // Warps of the softmax: with 32 rows twice as many, each of which has half of the rows (118 us against 4 on the case of parts of prompts);
-// then come the copying one, the product's, the queries', and one for the rows behind the last sequence.
+// then come one that copies keys and issues scores, one that issues the products with values, one that prepares queries, one that copies values.
 template <int R> constexpr int kSoftWarps = R == 32 ? 8 : 4;
 template <int R> constexpr int kThreadsOf = 32 * (kSoftWarps<R> + 4);
 constexpr int kMaxWarps = 12;
@@ -293,10 +293,10 @@ struct Layout {
 
 // An item as the query warp hands it over.
 template <int D, int R>
-struct Rows {
+struct alignas(16) Rows {
   Item item;
-  float factor[R];
-  int limit[R];
+  alignas(16) float factor[R];
+  alignas(16) int limit[R];
   long long place[R];
 };
 
@@ -306,11 +306,13 @@ struct Shared {
   unsigned char k[L::K_STAGES][kTile * D], v[L::V_STAGES][kTile * D];
   unsigned char p[L::P_BUFS][L::P_BYTES];
   unsigned char q[L::Q_BUFS][QP][R * D];
-  unsigned long long k_full[L::K_STAGES], k_empty[L::K_STAGES], v_full[L::V_STAGES], v_empty[L::V_STAGES], s_full[2], p_full[2], pv_done[2], q_full[L::Q_BUFS], q_empty[L::Q_BUFS];
+  // s_full: the scores of a stage's keys are there, which are not read any more; pv_done: the same for values
+  unsigned long long k_full[L::K_STAGES], s_full[L::K_STAGES], v_full[L::V_STAGES], pv_done[L::V_STAGES], p_full[2], q_full[L::Q_BUFS], q_empty[L::Q_BUFS];
   float ks[L::V_STAGES][8];      // of the unit's pages
   int ve[L::V_STAGES][8];        // kInvalid: no such page
   Rows<D, R> rows[L::Q_BUFS];
-  float m[4][R], sum[R];
+  float m[4][R], sum[R];       // largest x of each warp's keys, less 9
+  alignas(16) float ref[2][R == 32 ? R : 1];
   uint32_t bad[R][D / 32];     // outputs that a value which is no number reaches though not all rows see it
   int sums[kMaxWarps];
   Found found;
@@ -330,131 +332,170 @@ struct Note {
 
 
 template <int R>
-__device__ __forceinline__ float* part_of(const AttnParams& p, int D, long long slot) {      // [R][D] output, [R] maximum, [R] sum
+__device__ __forceinline__ float* part_of(const AttnParams& p, int D, long long slot) {      // [R][D] output, [R] reference, [R] sum
   return p.parts + slot * (R * (D + 2));
 }
 
-// ---- the copying warp -------------------------------------------------------------------------------------------------------------
-// Page numbers and scales are looked up for 32 pages at a time (4 units of 8 pages of 16 tokens to 32 units of one page), a batch ahead of the
-// copies: two loads that wait for one another, 1400 cycles, at every unit set the pace before.
-template <typename L, int D, int R, typename S>
-__device__ __forceinline__ void copy_warp(S& sh, const AttnParams& p, const CUtensorMap* km, const CUtensorMap* vm, int u0, int u1, Found f, Seq sq) {
-  const int lane = threadIdx.x & 31, rows = min(1 << p.shift, kTile), pages = kTile / rows, units = 32 / pages, mine = lane / pages, at_page = lane % pages;
+// After a wait ran out: what the block's last `turns` turns set going, a ring of barriers long, gets a millisecond to come to its end.
+template <int STAGES>
+__device__ __forceinline__ void settle(unsigned long long (&bars)[STAGES], uint32_t turns) {
+  const uint64_t t0 = st::globaltimer_ns();
+#pragma unroll 1
+  for (uint32_t i = turns > STAGES ? turns - STAGES : 0; i < turns; ++i)
+    while (!st::mbar_try_wait(st::smem_u32(&bars[i % STAGES]), i / STAGES & 1) && st::globaltimer_ns() - t0 < 1000000) {}
+}
+
+// ---- copies -------------------------------------------------------------------------------------------------------------------------
+// The run's units one after another, for keys or for values.  Page numbers and scales are looked up for 32 pages at a time (4 units of 8 pages
+// of 16 tokens to 32 units of one page), a batch ahead of the copies: two loads that wait for one another, 1400 cycles, at every unit set the
+// pace before.  A copy takes its warp about 110 cycles, so keys and values have warps of their own.
+template <typename L, int D, int R, bool VALUES, typename S>
+struct Copier {
+  static constexpr int ST = VALUES ? L::V_STAGES : L::K_STAGES;
   struct Batch {
     int t, n, h;      // units [t, t + n) of an item (n 0: the end), its key head
     int page;         // the lane's: page lane % pages of unit lane / pages; -1: none
+    float ks;
+    int ve;
   };
+  S& sh;
+  const AttnParams& p;
+  const CUtensorMap* map;
+  int u, u1, t = 0, end = 0;      // behind the next batch
+  Found f;
+  Seq sq;
   Item it;
-  int t = 0, end = 0;      // the next batch's place in `it`
-  int u = u0;
-  auto look_pages = [&]() {
-    Batch b{0, 0, 0, -1};
+  int lane, rows, pages, mine, at_page, i = 0;
+  uint32_t turn = 0;
+  Batch now, next;
+
+  __device__ __forceinline__ Copier(S& sh_, const AttnParams& p_, const CUtensorMap* map_, int u0, int u1_, Found f_, const Seq& sq_)
+      : sh(sh_), p(p_), map(map_), u(u0), u1(u1_), f(f_), sq(sq_), lane(threadIdx.x & 31), rows(min(1 << p.shift, kTile)), pages(kTile / rows), mine(lane / pages), at_page(lane % pages) {
+    now = look_pages();
+    look_scales(now);
+    next = look_pages();
+  }
+  __device__ __forceinline__ Batch look_pages() {
+    Batch b{0, 0, 0, -1, 0.0f, kInvalid};
     if (t >= end) {
       if (!item_at<R>(it, p, u, u1, f, sq)) return b;
       u = it.next, t = it.t0, end = it.t0 + it.steps();
     }
-    b.t = t, b.n = min(units, end - t), b.h = it.h;
+    b.t = t, b.n = min(32 / pages, end - t), b.h = it.h;
     const int key = (t + mine) * kTile + at_page * rows;
     if (mine < b.n && key < it.keys) b.page = it.table[key >> p.shift];
     else b.page = kBehind;
     t += b.n;
     return b;
-  };
-  auto look_scales = [&](Batch& b, float& ks, int& ve) {
-    ks = 0.0f, ve = kInvalid;
+  }
+  __device__ __forceinline__ void look_scales(Batch& b) {
     if (b.page < 0 || b.page >= p.pages) {
-      if (b.n > 0 && b.page != kBehind) st::report_error(p.err, st::ERR_BOUNDS, 0x7004);
+      if (VALUES && b.n > 0 && b.page != kBehind) st::report_error(p.err, st::ERR_BOUNDS, 0x7004);
       b.page = -1;
       return;
     }
+    if (!VALUES) return;
     const long long at = static_cast<long long>(b.page) * p.kv_heads + b.h;
-    ks = p.ks[at], ve = st::scale_exponent(p.vs[at]);
-  };
-  uint32_t turn = 0;
-  Batch now = look_pages();
-  float ks, ks_next = 0.0f;
-  int ve, ve_next = kInvalid;
-  look_scales(now, ks, ve);
-  while (now.n > 0) {
-    Batch next = look_pages();
-    const long long first = (static_cast<long long>(now.page) * p.kv_heads + now.h) << p.shift;
-    for (int i = 0; i < now.n; ++i, ++turn) {
-      const int kslot = turn % L::K_STAGES, vslot = turn % L::V_STAGES;
-      const bool live = mine == i && now.page >= 0;
-      const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, live)) * rows * D;
-      const long long token = first + (((now.t + i) * kTile + at_page * rows) & ((1 << p.shift) - 1));
-      if (!st::mbar_wait_warp(st::smem_u32(&sh.k_empty[kslot]), (turn / L::K_STAGES & 1) ^ 1, &sh.abort)) return;
-      if (lane == 0) st::mbar_arrive_expect_tx(st::smem_u32(&sh.k_full[kslot]), bytes);
-      __syncwarp();
-      if (live) st::tma_load_2d(st::smem_u32(sh.k[kslot]) + at_page * rows * D, km, st::smem_u32(&sh.k_full[kslot]), 0, static_cast<int>(token));
-      if (!st::mbar_wait_warp(st::smem_u32(&sh.v_empty[vslot]), (turn / L::V_STAGES & 1) ^ 1, &sh.abort)) return;
-      if (mine == i) sh.ks[vslot][at_page] = ks, sh.ve[vslot][at_page] = ve;
-      __syncwarp();
-      if (lane == 0) st::mbar_arrive_expect_tx(st::smem_u32(&sh.v_full[vslot]), bytes);
-      __syncwarp();
-      if (live) st::tma_load_2d(st::smem_u32(sh.v[vslot]) + at_page * rows * D, vm, st::smem_u32(&sh.v_full[vslot]), 0, static_cast<int>(token * D / 128));
-      if (i == 0) look_scales(next, ks_next, ve_next);      // the page numbers have come by now
+    b.ks = p.ks[at], b.ve = st::scale_exponent(p.vs[at]);
+  }
+  // The next unit into its stage, once that is free; false: there is none, or a wait ran out.
+  __device__ __forceinline__ bool copy() {
+    if (now.n == 0) return false;
+    const int slot = turn % ST;
+    const bool live = mine == i && now.page >= 0;
+    const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, live)) * rows * D;
+    const long long token = (((static_cast<long long>(now.page) * p.kv_heads + now.h) << p.shift)) + (((now.t + i) * kTile + at_page * rows) & ((1 << p.shift) - 1));
+    const uint32_t full = st::smem_u32(VALUES ? &sh.v_full[slot] : &sh.k_full[slot]);
+    if (!st::mbar_wait_warp(st::smem_u32(VALUES ? &sh.pv_done[slot] : &sh.s_full[slot]), (turn / ST & 1) ^ 1, &sh.abort)) return false;
+    if (live) st::tma_load_2d(st::smem_u32(VALUES ? sh.v[slot] : sh.k[slot]) + at_page * rows * D, map, full, 0, static_cast<int>(VALUES ? token * D / 128 : token));
+    if (VALUES && mine == i) sh.ks[slot][at_page] = now.ks, sh.ve[slot][at_page] = now.ve;      // the scales may still be on their way
+    __syncwarp();
+    if (lane == 0) st::mbar_arrive_expect_tx(full, bytes);      // what has come before counts
+    ++turn;
+    if (++i == 1) look_scales(next);      // the page numbers have come by now
+    if (i == now.n) {
+      now = next, i = 0;
+      next = look_pages();
     }
-    now = next, ks = ks_next, ve = ve_next;
+    return true;
+  }
+};
+
+// ---- products -----------------------------------------------------------------------------------------------------------------------
+// N is a multiple of 16: three parts of 8 rows are followed by 8 columns that nobody reads, from whatever lies behind them.  Each of the two products has
+// a warp of its own: an instruction or a wait takes the issuing lane 70 to 130 cycles, a unit's scores 600, its outputs 700.
+
+// The number of an item's units, 0 behind the last one, once its queries are there; -1: a wait ran out.
+template <typename L, typename S>
+__device__ __forceinline__ int steps_of(S& sh, uint32_t item) {
+  if (!st::mbar_wait_warp(st::smem_u32(&sh.q_full[item % L::Q_BUFS]), item / L::Q_BUFS & 1, &sh.abort)) return -1;
+  const Item& it = sh.rows[item % L::Q_BUFS].item;
+  return it.t1 > it.t0 ? it.steps() : 0;
+}
+
+// Copies keys and issues scores, two units ahead of the softmax at most.  Returns the units that it copied and those whose scores it issued.
+template <typename L, int D, int R, int QP, typename S>
+__device__ __forceinline__ uint2 score_warp(S& sh, const AttnParams& p, const CUtensorMap* map, uint32_t tmem, int u0, int u1, Found f, const Seq& sq) {
+  Copier<L, D, R, false, S> keys(sh, p, map, u0, u1, f, sq);
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int i = 0; i < L::K_STAGES; ++i) keys.copy();
+  uint32_t turn = 0;
+  for (uint32_t item = 0;; ++item) {
+    const int steps = steps_of<L>(sh, item);
+    if (steps <= 0) return make_uint2(keys.turn, turn);
+    const bool more = sh.rows[item % L::Q_BUFS].item.next < u1;
+#pragma unroll 1
+    for (int i = 0; i < steps; ++i, ++turn) {
+      const int slot = turn % L::K_STAGES;
+      if (!st::mbar_wait_warp(st::smem_u32(&sh.k_full[slot]), turn / L::K_STAGES & 1, &sh.abort)) return make_uint2(keys.turn, turn);
+      // the columns are free again once the softmax has written the weights of the unit before last
+      if (turn > 1 && !st::mbar_wait_warp(st::smem_u32(&sh.p_full[turn & 1]), (turn - 2) >> 1 & 1, &sh.abort)) return make_uint2(keys.turn, turn);
+      st::tc_fence_after();
+      if (lane == 0) {
+        const uint64_t a = tile_desc<D>(st::smem_u32(sh.k[slot]));
+#pragma unroll
+        for (int j = 0; j < L::SETS; ++j) {
+          const int ways = min(L::WAYS, QP - j * L::WAYS);
+          const uint64_t b = tile_desc<D>(st::smem_u32(sh.q[item % L::Q_BUFS][j * L::WAYS]));
+#pragma unroll
+          for (int k = 0; k < D / 32; ++k) umma_codes(tmem + (turn & 1) * L::S_N, a + 2 * k, b + 2 * k, codes_idesc(128, (ways * R + 15) / 16 * 16, false), j + k > 0);
+        }
+        st::umma_commit(st::smem_u32(&sh.s_full[slot]));
+      }
+      __syncwarp();
+      if (turn > 0) keys.copy();      // into the stage of the unit before, whose scores are there by now
+    }
+    if (!more) return make_uint2(keys.turn, turn);
   }
 }
 
-// ---- the warp that issues products (one lane) -------------------------------------------------------------------------------------
-// N is a multiple of 16: three parts of 8 rows are followed by 8 columns that nobody reads, from whatever lies behind them.
-template <typename L, int D, int R, int QP, typename S>
-__device__ __forceinline__ void product_warp(S& sh, uint32_t tmem, int u1) {
-  constexpr uint32_t p_idesc = codes_idesc(128, L::P_N, true);
-  uint32_t turn = 0, item = 0;
-  auto ask_scores = [&](uint32_t t, uint32_t of) {
-    const int slot = t % L::K_STAGES;
-    if (!st::mbar_wait(st::smem_u32(&sh.k_full[slot]), t / L::K_STAGES & 1, &sh.abort)) return false;
-    st::tc_fence_after();
-#pragma unroll
-    for (int i = 0; i < L::SETS; ++i) {
-      const int ways = min(L::WAYS, QP - i * L::WAYS);
-#pragma unroll
-      for (int k = 0; k < D / 32; ++k)
-        umma_codes(tmem + (t & 1) * L::S_N, tile_desc<D>(st::smem_u32(sh.k[slot])) + 2 * k, tile_desc<D>(st::smem_u32(sh.q[of % L::Q_BUFS][i * L::WAYS])) + 2 * k,
-                   codes_idesc(128, (ways * R + 15) / 16 * 16, false), i + k > 0);
-    }
-    st::umma_commit(st::smem_u32(&sh.s_full[t & 1]));
-    st::umma_commit(st::smem_u32(&sh.k_empty[slot]));
-    return true;
-  };
-  // the item's number of units, 0 behind the last one, once its queries are there
-  auto next_item = [&](uint32_t of, int& steps, int& next) {
-    if (!st::mbar_wait(st::smem_u32(&sh.q_full[of % L::Q_BUFS]), of / L::Q_BUFS & 1, &sh.abort)) return false;
-    const Item& it = sh.rows[of % L::Q_BUFS].item;
-    steps = it.t1 > it.t0 ? it.steps() : 0, next = it.next;
-    return true;
-  };
-  int steps = 0, next = 0, steps_next = 0, next_next = 0;
-  if (!next_item(0, steps, next) || steps == 0 || !ask_scores(0, 0)) return;
-  for (;; ++item) {
-    const bool more = next < u1;
+// Issues the products with values; returns of how many units.
+template <typename L, int D, int R, typename S>
+__device__ __forceinline__ uint32_t value_warp(S& sh, uint32_t tmem, int u1) {
+  constexpr uint32_t idesc = codes_idesc(128, L::P_N, true);
+  const int lane = threadIdx.x & 31;
+  uint32_t turn = 0;
+  for (uint32_t item = 0;; ++item) {
+    const int steps = steps_of<L>(sh, item);
+    if (steps <= 0) return turn;
+    const bool more = sh.rows[item % L::Q_BUFS].item.next < u1;
+#pragma unroll 1
     for (int i = 0; i < steps; ++i, ++turn) {
-      // the scores of the next unit, be it the next item's: not with one buffer of queries, which waits for this item's end
-      if (i + 1 < steps) {
-        if (!ask_scores(turn + 1, item)) return;
-      } else if (more && L::Q_BUFS == 2) {
-        if (!next_item(item + 1, steps_next, next_next) || (steps_next > 0 && !ask_scores(turn + 1, item + 1))) return;
-      }
       const int slot = turn % L::V_STAGES;
-      if (!st::mbar_wait(st::smem_u32(&sh.p_full[turn & 1]), turn >> 1 & 1, &sh.abort)) return;
-      if (!st::mbar_wait(st::smem_u32(&sh.v_full[slot]), turn / L::V_STAGES & 1, &sh.abort)) return;
+      if (!st::mbar_wait_warp(st::smem_u32(&sh.v_full[slot]), turn / L::V_STAGES & 1, &sh.abort)) return turn;
+      if (!st::mbar_wait_warp(st::smem_u32(&sh.p_full[turn & 1]), turn >> 1 & 1, &sh.abort)) return turn;
       st::tc_fence_after();
-      // 32 rows of K (tokens, or pairs of them) at a time: 4 groups of 8
+      if (lane == 0) {
+        // 32 rows of K (tokens, or pairs of them) at a time: 4 groups of 8
+        const uint64_t a = tile_desc<128>(st::smem_u32(sh.v[slot])), b = tile_desc<L::P_WIDTH>(st::smem_u32(sh.p[turn % L::P_BUFS]), L::P_ROWS * L::P_WIDTH);
 #pragma unroll
-      for (int k = 0; k < L::P_ROWS / 32; ++k)
-        umma_codes(tmem + 2 * L::S_N, tile_desc<128>(st::smem_u32(sh.v[slot])) + k * (32 * 128 >> 4),
-                   tile_desc<L::P_WIDTH>(st::smem_u32(sh.p[turn % L::P_BUFS]), L::P_ROWS * L::P_WIDTH) + k * (32 * L::P_WIDTH >> 4), p_idesc, i + k > 0);
-      st::umma_commit(st::smem_u32(&sh.pv_done[turn & 1]));
-      st::umma_commit(st::smem_u32(&sh.v_empty[slot]));
+        for (int k = 0; k < L::P_ROWS / 32; ++k) umma_codes(tmem + 2 * L::S_N, a + k * (32 * 128 >> 4), b + k * (32 * L::P_WIDTH >> 4), idesc, i + k > 0);
+        st::umma_commit(st::smem_u32(&sh.pv_done[slot]));
+      }
+      __syncwarp();
     }
-    if (!more) return;
-    if (L::Q_BUFS == 1 && (!next_item(item + 1, steps_next, next_next) || (steps_next > 0 && !ask_scores(turn, item + 1)))) return;
-    if (steps_next == 0) return;
-    steps = steps_next, next = next_next;
+    if (!more) return turn;
   }
 }
 
@@ -548,14 +589,16 @@ template <int D, int R, typename S>
 __device__ __forceinline__ void clean_values(S& sh, const Rows<D, R>& of, int slot, int key, bool there, int limit_min) {
   constexpr int SIDES = D == 64 ? 2 : 1, PARTS = D / 16;
   const int t = threadIdx.x & 127, line = t / SIDES, side = t % SIDES * PARTS;
+  if (!there) {
+#pragma unroll
+    for (int c = 0; c < PARTS; ++c) *reinterpret_cast<uint4*>(sh.v[slot] + swizzled<128>(line, side + c)) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  if (key < limit_min) return;      // all rows see it
 #pragma unroll 1
   for (int c = 0; c < PARTS; ++c) {
     uint4* at = reinterpret_cast<uint4*>(sh.v[slot] + swizzled<128>(line, side + c));
-    if (!there) {
-      *at = make_uint4(0, 0, 0, 0);
-      continue;
-    }
-    uint4 x = *at;
+    const uint4 x = *at;
     uint32_t w[4] = {x.x, x.y, x.z, x.w};
     uint32_t bits = 0;
 #pragma unroll
@@ -564,7 +607,7 @@ __device__ __forceinline__ void clean_values(S& sh, const Rows<D, R>& of, int sl
       bits |= ((nb >> 7 & 1) | (nb >> 14 & 2) | (nb >> 21 & 4) | (nb >> 28 & 8)) << (4 * i);
       w[i] &= ~((nb >> 7) * 255u);
     }
-    if (bits == 0 || key < limit_min) continue;
+    if (bits == 0) continue;
     for (int r = 0; r < R; ++r)
       if (key < of.limit[r]) atomicOr(&sh.bad[r][c / 2], bits << (16 * (c & 1)));
     *at = make_uint4(w[0], w[1], w[2], w[3]);
@@ -582,16 +625,25 @@ __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t 
   T* out = static_cast<T*>(p.out);
   // A wait that runs out sets the abort flag, and all later ones return at once: the warps finish the item together and stop at the next one.
   uint32_t turn = 0, item = 0;
+  // The rows' references are the same for all keys: registers, or with 32 rows, which leave none, shared memory, the old ones and the new ones.
+  constexpr bool kShared = R == 32;
+  int flip = 0;
   for (int i = threadIdx.x; i < R * (D / 32); i += SOFT) sh.bad[i / (D / 32)][i % (D / 32)] = 0;
   for (;; ++item) {
     const Rows<D, R>& of = sh.rows[item % L::Q_BUFS];
+    if (kShared && threadIdx.x < R) sh.ref[flip][threadIdx.x] = kNoMax;
     if (soft_any<SOFT>(!st::mbar_wait_warp(st::smem_u32(&sh.q_full[item % L::Q_BUFS]), item / L::Q_BUFS & 1, &sh.abort))) return;
     if (of.item.t1 <= of.item.t0) return;      // no more items
     const int steps = of.item.steps(), t0 = of.item.t0, keys = of.item.keys, next = of.item.next;
     const int limit_min = of.limit[0];      // rows come in order
-    float m[RT], l[RT];
+    float own_ref[kShared ? 1 : RT]{}, l[RT];
+    auto ref = [&](int r) { return kShared ? sh.ref[flip][low + r] : own_ref[kShared ? 0 : r]; };      // M - 9
+    bool unseen = false;
 #pragma unroll
-    for (int r = 0; r < RT; ++r) m[r] = kNoMax, l[r] = 0.0f;
+    for (int r = 0; r < RT; ++r) {
+      if (!kShared) own_ref[kShared ? 0 : r] = kNoMax;
+      l[r] = 0.0f;
+    }
 
     for (int i = 0; i < steps; ++i, ++turn) {
       const int slot = turn % L::V_STAGES, key = (t0 + i) * kTile + t;
@@ -601,7 +653,7 @@ __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t 
       const bool there = ve_or_not != kInvalid && key < keys;
       const int ve = there ? ve_or_not : 0;
       const bool gone = (t0 + i + 1) * kTile > limit_min || !there;      // of this unit's keys some row may not see this one
-      st::mbar_wait_warp(st::smem_u32(&sh.s_full[turn & 1]), turn >> 1 & 1, &sh.abort);
+      st::mbar_wait_warp(st::smem_u32(&sh.s_full[turn % L::K_STAGES]), turn / L::K_STAGES & 1, &sh.abort);
       st::tc_fence_after();
       uint32_t raw[L::WAYS][RT];
 #pragma unroll
@@ -621,31 +673,46 @@ __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t 
         for (int r = 0; r < RT; ++r)
           if (!there || key >= of.limit[low + r]) x[r] = -INFINITY;
       }
-      float over = -INFINITY;
+      // the reference moves where a weight would be too large; the first unit sets it, or a later one for a row that saw nothing before
+      const bool fresh = i == 0 || unseen;
+      bool move = fresh;
+      if (!fresh) {
+        float over = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < RT; r += 2) over = st::max3(over, x[r] - m[r], x[r + 1] - m[r + 1]);
-      // the reference moves where a weight would be too large; the first unit always sets it
-      if (soft_any<SOFT>(over > kLag)) {
+        for (int r = 0; r < RT; ++r) x[r] -= ref(r);
+#pragma unroll
+        for (int r = 0; r < RT; r += 2) over = st::max3(over, x[r], x[r + 1]);
+        move = soft_any<SOFT>(over > kLag + kLift);
+      }
+      if (move) {
+        if (!fresh) {
+#pragma unroll
+          for (int r = 0; r < RT; ++r) x[r] += ref(r);
+        }
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
           const float top = warp_top(x[r]);
-          if (lane == 0) sh.m[warp][low + r] = top;
+          if (lane == 0) sh.m[warp][low + r] = top - kLift;
         }
         soft_sync<SOFT>();
         if (i > 0) {
-          st::mbar_wait_warp(st::smem_u32(&sh.pv_done[(turn - 1) & 1]), (turn - 1) >> 1 & 1, &sh.abort);
+          st::mbar_wait_warp(st::smem_u32(&sh.pv_done[(turn - 1) % L::V_STAGES]), (turn - 1) / L::V_STAGES & 1, &sh.abort);
           st::tc_fence_after();
         }
+        bool none = false;
 #pragma unroll
         for (int c = 0; c < RT / 8; ++c) {
           float b[8];
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
             const int row = 8 * c + r;
-            const float to = fmaxf(m[row], fmaxf(fmaxf(sh.m[0][low + row], sh.m[1][low + row]), fmaxf(sh.m[2][low + row], sh.m[3][low + row])));
-            b[r] = st::exp2_ftz(m[row] - to);
-            m[row] = to;
+            const float from = ref(row), to = fmaxf(from, fmaxf(fmaxf(sh.m[0][low + row], sh.m[1][low + row]), fmaxf(sh.m[2][low + row], sh.m[3][low + row])));
+            b[r] = st::exp2_ftz(from - to);
+            none = none || to == kNoMax;
+            if (!kShared) own_ref[kShared ? 0 : row] = to;
+            else if (t == 0) sh.ref[flip ^ 1][low + row] = to;
             l[row] *= b[r];
+            x[row] -= to;
           }
           if (i > 0)
 #pragma unroll
@@ -659,12 +726,13 @@ __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t 
             }
         }
         if (i > 0) st::tmem_st_wait();
-        soft_sync<SOFT>();      // the maxima are read
+        unseen = soft_any<SOFT>(none);      // and the maxima are read
+        flip ^= 1;
       }
       if (gone && half == 0) clean_values<D, R>(sh, of, slot, key, there, limit_min);
       // the buffer's last products are done
-      if constexpr (L::P_BUFS == 2) st::mbar_wait_warp(st::smem_u32(&sh.pv_done[turn & 1]), (turn >> 1 & 1) ^ 1, &sh.abort);
-      else if (turn > 0) st::mbar_wait_warp(st::smem_u32(&sh.pv_done[(turn - 1) & 1]), (turn - 1) >> 1 & 1, &sh.abort);
+      if (L::P_BUFS == 2 && turn > 1) st::mbar_wait_warp(st::smem_u32(&sh.pv_done[(turn - 2) % L::V_STAGES]), (turn - 2) / L::V_STAGES & 1, &sh.abort);
+      if (L::P_BUFS == 1 && turn > 0) st::mbar_wait_warp(st::smem_u32(&sh.pv_done[(turn - 1) % L::V_STAGES]), (turn - 1) / L::V_STAGES & 1, &sh.abort);
       const float take = st::exp2_int(-ve - static_cast<int>(kLift));
       unsigned char* to = sh.p[turn % L::P_BUFS];
       const uint32_t row = t / L::SIDES, first = t % L::SIDES * kParts * R + low;
@@ -673,7 +741,7 @@ __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t 
         __half2 w[4];
 #pragma unroll
         for (int r = 0; r < 8; r += 2) {
-          const float y = st::exp2_ftz(x[8 * c + r] - m[8 * c + r] + kLift), z = st::exp2_ftz(x[8 * c + r + 1] - m[8 * c + r + 1] + kLift);
+          const float y = st::exp2_ftz(x[8 * c + r]), z = st::exp2_ftz(x[8 * c + r + 1]);
           l[8 * c + r] = fmaf(y, take, l[8 * c + r]), l[8 * c + r + 1] = fmaf(z, take, l[8 * c + r + 1]);
           w[r / 2] = __floats2half2_rn(y, z);
         }
@@ -689,7 +757,7 @@ __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t 
     }
 
     // the item's outputs, and the sums over all keys, through the room of the weights, which no product reads now
-    st::mbar_wait_warp(st::smem_u32(&sh.pv_done[(turn - 1) & 1]), (turn - 1) >> 1 & 1, &sh.abort);
+    st::mbar_wait_warp(st::smem_u32(&sh.pv_done[(turn - 1) % L::V_STAGES]), (turn - 1) / L::V_STAGES & 1, &sh.abort);
     st::tc_fence_after();
     const Item& it = of.item;
     const int rows = it.row_end - it.row0;
@@ -747,15 +815,15 @@ __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t 
           const int row = low + 8 * c + r;
           if (row >= rows) continue;
           const float sum = sh.sum[row];
-          float y = o[r] * (1.0f / 512.0f);      // 2^-kLift
+          float y = o[r] * (1.0f / 512.0f);      // 2^-9
           if (sh.bad[row][t / 32] >> (t & 31) & 1) y = NAN;
           if (whole) out[of.place[row] + t] = from_f<T>(sum == 0.0f ? 0.0f : __fdividef(y, sum));
           else part[row * D + t] = y;
           if (t == 0) {
-            if (!whole) part[R * D + row] = m[8 * c + r], part[R * D + R + row] = sum;
+            if (!whole) part[R * D + row] = ref(8 * c + r), part[R * D + R + row] = sum;
             else if (p.lse != nullptr) {
               const int fr = it.row0 + row;
-              p.lse[(it.start + fr / p.group) * static_cast<long long>(p.heads) + it.h * p.group + fr % p.group] = sum == 0.0f ? -INFINITY : (m[8 * c + r] + log2f(sum)) / kLog2e;
+              p.lse[(it.start + fr / p.group) * static_cast<long long>(p.heads) + it.h * p.group + fr % p.group] = sum == 0.0f ? -INFINITY : (ref(8 * c + r) + kLift + log2f(sum)) / kLog2e;
             }
           }
         }
@@ -805,17 +873,13 @@ __global__ void __launch_bounds__(kThreadsOf<R>, Layout<D, R, kQueryParts<T>>::B
   extern __shared__ __align__(1024) unsigned char raw[];      // swizzles count rows from multiples of 1024
   using S = Shared<D, R, QP>;
   S& sh = *reinterpret_cast<S*>(raw);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     st::tma_prefetch_desc(&k_map);
     st::tma_prefetch_desc(&v_map);
-    for (int i = 0; i < L::K_STAGES; ++i) st::mbar_init(st::smem_u32(&sh.k_full[i]), 1), st::mbar_init(st::smem_u32(&sh.k_empty[i]), 1);
-    for (int i = 0; i < L::V_STAGES; ++i) st::mbar_init(st::smem_u32(&sh.v_full[i]), 1), st::mbar_init(st::smem_u32(&sh.v_empty[i]), 1);
-    for (int i = 0; i < 2; ++i) {
-      st::mbar_init(st::smem_u32(&sh.s_full[i]), 1);
-      st::mbar_init(st::smem_u32(&sh.p_full[i]), 32 * SW);
-      st::mbar_init(st::smem_u32(&sh.pv_done[i]), 1);
-    }
+    for (int i = 0; i < L::K_STAGES; ++i) st::mbar_init(st::smem_u32(&sh.k_full[i]), 1), st::mbar_init(st::smem_u32(&sh.s_full[i]), 1);
+    for (int i = 0; i < L::V_STAGES; ++i) st::mbar_init(st::smem_u32(&sh.v_full[i]), 1), st::mbar_init(st::smem_u32(&sh.pv_done[i]), 1);
+    for (int i = 0; i < 2; ++i) st::mbar_init(st::smem_u32(&sh.p_full[i]), 32 * SW);
     for (int i = 0; i < L::Q_BUFS; ++i) st::mbar_init(st::smem_u32(&sh.q_full[i]), 1), st::mbar_init(st::smem_u32(&sh.q_empty[i]), 1);
     st::fence_barrier_init();
     sh.abort = 0;
@@ -833,9 +897,9 @@ __global__ void __launch_bounds__(kThreadsOf<R>, Layout<D, R, kQueryParts<T>>::B
   const bool share = find_share<R>(p, sh.sums, &sh.found, all, runs, u0, u1, f);
   st::tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  if (p.zero_tail && warp == SW + 3) zero_rows<T, D>(p);
   if (threadIdx.x == 0 && !p.whole) note->parts = 0;
   if (!share) {
+    if (p.zero_tail && warp == SW + 3) zero_rows<T, D>(p);
     if (warp == SW + 1) st::tmem_dealloc(tmem, L::COLUMNS);
     return;
   }
@@ -843,15 +907,20 @@ __global__ void __launch_bounds__(kThreadsOf<R>, Layout<D, R, kQueryParts<T>>::B
   // With 16 rows and more the softmax takes registers from the other warps: 176 and 80 of the 128 of the launch, with 32 rows 88
   // (of two warpgroups) and 64 of 80.
   constexpr bool kShift = R >= 16 && L::BLOCKS == 2;
+  uint2 under_way = make_uint2(0, 0);
   if (warp >= SW) {
     if constexpr (kShift) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R == 32 ? 64 : 80));
     if (warp == SW) {
-      copy_warp<L, D, R>(sh, p, &k_map, &v_map, u0, u1, f, sq);
+      under_way = score_warp<L, D, R, QP>(sh, p, &k_map, tmem, u0, u1, f, sq);
     } else if (warp == SW + 1) {
-      if (lane == 0) product_warp<L, D, R, QP>(sh, tmem, u1);
-      __syncwarp();
+      under_way.y = value_warp<L, D, R>(sh, tmem, u1);
     } else if (warp == SW + 2) {
       query_warp<T, L, D, R, QP>(sh, p, u0, u1, f, sq);
+    } else {
+      Copier<L, D, R, true, S> values(sh, p, &v_map, u0, u1, f, sq);
+      while (values.copy()) {}
+      under_way.x = values.turn;
+      if (p.zero_tail) zero_rows<T, D>(p);
     }
   } else {
     if constexpr (kShift) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R == 32 ? 88 : 176));
@@ -860,6 +929,12 @@ __global__ void __launch_bounds__(kThreadsOf<R>, Layout<D, R, kQueryParts<T>>::B
   }
   st::tc_fence_before();
   __syncthreads();
+  if (sh.abort) {
+    if (warp == SW) settle(sh.k_full, under_way.x), settle(sh.s_full, under_way.y);
+    if (warp == SW + 1) settle(sh.pv_done, under_way.y);
+    if (warp == SW + 3) settle(sh.v_full, under_way.x);
+    __syncthreads();
+  }
   if (warp == SW + 1) st::tmem_dealloc(tmem, L::COLUMNS);
 }
 
@@ -941,7 +1016,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(AttnParams p) 
       const int d = threadIdx.x;
       if (d < D) o[d] = from_f<T>(((rows[0][d] + rows[1][d]) + (rows[2][d] + rows[3][d])) * inv);
     }
-    if (at == 0 && p.lse != nullptr) p.lse[row * p.heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) / kLog2e;
+    if (at == 0 && p.lse != nullptr) p.lse[row * p.heads + head] = l == 0.0f ? -INFINITY : (m + kLift + log2f(l)) / kLog2e;
   }
 }
 

@@ -289,6 +289,79 @@ def test_attention_over_many_blocks_of_one_sequence():
 
 
 @GPU
+@pytest.mark.parametrize("D,H,G,page,dtype,lengths,added,causal", [
+    (64, 2, 4, 256, torch.float16, [2500, 1, 900], [1, 1, 1], True), (128, 1, 4, 32, torch.bfloat16, [3000, 130], [4, 1], True),
+    (64, 1, 16, 16, torch.bfloat16, [5000], [1], True), (128, 2, 4, 64, torch.float16, [4100, 3000], [20, 9], True),
+    (64, 1, 3, 128, torch.bfloat16, [3000, 2400, 0, 700], [33, 3, 1, 17], False), (128, 1, 8, 16, torch.bfloat16, [2600, 2599], [64, 65], True),
+    (64, 2, 2, 16, torch.float16, [2305, 2600], [40, 5], True)])
+def test_attention_of_items_that_several_blocks_share(D, H, G, page, dtype, lengths, added, causal):
+    _check_attention(lengths, added, H, G, page, D, dtype, causal, seed=D + G)
+
+
+@GPU
+@pytest.mark.parametrize("D,n,G,page", [(64, 1, 8, 16), (128, 2, 8, 64), (64, 9, 4, 16), (128, 9, 4, 256)])
+def test_attention_of_long_sequences_whose_pages_are_none_or_hold_no_numbers(D, n, G, page):
+    from spiraltorch_b200.ops import native
+    lengths, added = [2600, 3000], [n, n]
+    pages, table = _cache(lengths, 1, page, D, 4)
+    starts, ln = torch.tensor([0, n, 2 * n], dtype=torch.int32), torch.tensor(lengths, dtype=torch.int32)
+    q = torch.randn(2 * n, G, D, generator=torch.Generator().manual_seed(4)).bfloat16()
+    pages.v.view(torch.uint8)[table[1, 2999 // page], 0, 2999 % page, 7] = 0xFF       # seen by the last token's rows alone
+    sees = torch.zeros(2 * n, dtype=torch.bool)
+    sees[-1] = True
+    want = P.attention_reference(q, pages, table, starts, ln, True, None, torch.float64)[0]
+    dev = P.Pages(*(t.cuda() for t in pages))
+    call = lambda table: P.attention(q.cuda(), dev, table.cuda(), starts.cuda(), ln.cuda(), max_queries=n)                      # noqa: E731
+    good = call(table)
+    assert torch.equal(good.isnan().any(-1).any(-1).cpu(), sees) and torch.allclose(good.cpu().double(), want, atol=0.1, rtol=0.01, equal_nan=True)
+    holes = table.clone()                   # sequence 0: the first 256 keys, and some in the middle; they count as keys that no row sees
+    holes[0, :256 // page] = -1
+    holes[0, 1024 // page:1280 // page] = pages.k.shape[0]
+    got = call(holes)
+    torch.cuda.synchronize()
+    assert native.read_error_word()[0] == 3
+    assert torch.equal(got[n:].nan_to_num(5), good[n:].nan_to_num(5))
+    seen = torch.cat([torch.arange(256, 1024), torch.arange(1280, 2600)])
+    at = table[0, seen // page].long(), seen % page
+    k, v = (c[at[0], 0, at[1]].double() * s[at[0], 0, None].double() for c, s in ((pages.k.float(), pages.k_scale), (pages.v.float(), pages.v_scale)))
+    s = torch.einsum("ihd,kd->ihk", q[:n].double(), k) * D ** -0.5
+    s.masked_fill_(seen[None, None] >= (2600 - n + 1 + torch.arange(n))[:, None, None], float("-inf"))
+    assert torch.allclose(got[:n].cpu().double(), s.softmax(-1) @ v, atol=0.1, rtol=0.01)
+
+
+@GPU
+def test_attention_of_long_tables_captured_twice():
+    """Items are split; two graphs and an eager call in turn have workspaces of their own."""
+    lengths, H, G, D, page = [1, 40], 2, 4, 64, 16
+    pages, table = _cache([3000, 1500], H, page, D, 6)
+    pages.k.view(torch.uint8).bitwise_and_(0x77)                # numbers everywhere
+    pages.v.view(torch.uint8).bitwise_and_(0x77)
+    dev, table_gpu, starts = P.Pages(*(t.cuda() for t in pages)), table.cuda(), torch.arange(3, dtype=torch.int32, device="cuda")
+    ln, q = torch.tensor(lengths, dtype=torch.int32, device="cuda"), torch.randn(2, H * G, D, device="cuda").bfloat16()
+    call = lambda: P.attention(q, dev, table_gpu, starts, ln, max_queries=1)                     # noqa: E731
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(call())
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for now in ([1, 40], [129, 1], [0, 1500], [3000, 1111], [2047, 1025]):
+        ln.copy_(torch.tensor(now))
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = call()
+        torch.cuda.synchronize()
+        want = P.attention_reference(q.cpu(), pages, table, starts.cpu(), ln.cpu(), True, None, torch.float64)[0]
+        assert torch.equal(outs[0], eager) and torch.equal(outs[1], eager)
+        assert torch.allclose(eager.cpu().double(), want, atol=0.1, rtol=0.01)
+
+
+@GPU
 def test_attention_scales_far_apart_and_large_scores():
     _check_attention(LENGTHS, [1] * 9, 2, 2, 16, 64, torch.bfloat16, spread=7)
     # value scales 2^40 apart: the codes of the small ones must not be lost in front of the large ones' masked or light keys
