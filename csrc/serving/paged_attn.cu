@@ -31,167 +31,14 @@
 // Blocks: four warps for the softmax, one that copies keys (a tiled copy per page and unit) and issues scores, one that copies values, one that
 // issues the products with them, one that prepares the queries of the next item, so that a run's items follow one another without a pause: with that in the softmax warps' way an item cost them 4500 cycles more.  Heads of 64: the copies lay two tokens
 // side by side, 64 rows of 128, and the weights of even and odd tokens have columns of their own; half of each product is not used.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include "../common/host.h"
-#include "../common/ptx.cuh"
-#include "paged.cuh"
+#include "paged_prompt.cuh"
 
 namespace {
-using st::chain_begin;
-
-constexpr int kTile = 128;            // keys of a unit
 // Warps of the softmax: with 32 rows twice as many, each of which has half of the rows (118 us against 4 on the case of parts of prompts);
 // then come one that copies keys and issues scores, one that issues the products with values, one that prepares queries, one that copies values.
 template <int R> constexpr int kSoftWarps = R == 32 ? 8 : 4;
-template <int R> constexpr int kThreadsOf = 32 * (kSoftWarps<R> + 4);
-constexpr int kMaxWarps = 12;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNoMax = -1e30f;      // before a row has seen a key
-constexpr float kLag = 6.0f, kLift = 9.0f;
+static_assert(kThreadsOf<8> == 32 * (kSoftWarps<8> + 4) && kThreadsOf<32> == 32 * (kSoftWarps<32> + 4));
 constexpr int kParts = 4;             // e5m2 numbers of a weight
-
-struct AttnParams {
-  const void* q;
-  const unsigned char *kc, *vc;
-  const float *ks, *vs;
-  const int *table, *starts, *lengths;
-  void* out;
-  float *lse, *parts;
-  int* notes;
-  long long q_row, q_head, o_row, o_head, table_row, pages;
-  long long rows;      // of q and out
-  int width, shift, B, heads, kv_heads, group;
-  float scale;
-  int causal, zero_tail, whole;      // whole: items are not split
-  unsigned* err;
-};
-
-// What the beginning and the end of an item cost, in units: 5000 cycles of about 2300, with 32 rows 20000 of 4500.
-template <int N> constexpr int kItemCost = N == 32 ? 4 : 2;
-
-struct Seq {
-  int start, n, len, row_blocks, tiles, size, units;      // size: what an item counts
-};
-template <int N>
-__device__ __forceinline__ Seq sequence(const AttnParams& p, int b) {
-  Seq s;
-  const int rows = static_cast<int>(p.rows), a = p.starts[b], e = p.starts[b + 1], len = max(p.lengths[b], 0);
-  s.start = max(a, 0);
-  s.n = max(min(e, rows) - s.start, 0);
-  s.len = min(len, p.width << p.shift);
-  s.row_blocks = (s.n * p.group + N - 1) / N;
-  s.tiles = max((s.len + kTile - 1) / kTile, 1);      // a sequence without keys still gets its zero rows
-  s.size = p.whole ? 1 : s.tiles + kItemCost<N>;
-  s.units = s.row_blocks * s.size * p.kv_heads;
-  return s;
-}
-
-// Where the block's share begins: the sequence that holds a unit, and the number of the sequence's first one.
-struct Found {
-  int b, first;
-};
-template <int WARPS>
-__device__ __forceinline__ int scan_block(int mine, int* shared, int& total) {      // sum of the threads before, and of all
-  int s = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, s, o);
-    if ((threadIdx.x & 31) >= o) s += u;
-  }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 31) shared[threadIdx.x >> 5] = s;
-  __syncthreads();
-  int before = s - mine;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    if (w < static_cast<int>(threadIdx.x >> 5)) before += shared[w];
-    total += shared[w];
-  }
-  return before;
-}
-// The block's share [u0, u1) of the units, if it has one, and where unit u0 lies.  Up to a block's threads of sequences are looked at once.
-template <int N>
-__device__ bool find_share(const AttnParams& p, int* shared, Found* found, int& all, int& runs, int& u0, int& u1, Found& f) {
-  constexpr int kThreads = kThreadsOf<N>, kWarps = kThreads / 32;
-  int mine = 0, total = 0, before = 0;
-#pragma unroll 1
-  for (int b = threadIdx.x; b < p.B; b += kThreads) mine += sequence<N>(p, b).units;
-  before = scan_block<kWarps>(mine, shared, total);
-  all = total;
-  runs = min(static_cast<int>(gridDim.x), all);      // none of them empty
-  const int me = blockIdx.x;
-  if (me >= runs) return false;
-  // floor(all * block / runs) without the product
-  const unsigned each = static_cast<unsigned>(all) / static_cast<unsigned>(runs), rest = all - each * runs;
-  u0 = me * each + me * rest / runs, u1 = (me + 1) * each + (me + 1) * rest / runs;
-  if (p.B <= kThreads) {
-    if (u0 >= before && u0 < before + mine) *found = Found{static_cast<int>(threadIdx.x), before};      // one thread
-  } else {
-    int base = 0;
-#pragma unroll 1
-    for (int b0 = 0; b0 < p.B && u0 >= base; b0 += kThreads) {
-      const int b = b0 + threadIdx.x;
-      mine = b < p.B ? sequence<N>(p, b).units : 0;
-      before = base + scan_block<kWarps>(mine, shared, total);
-      if (u0 >= before && u0 < before + mine) *found = Found{b, before};
-      base += total;
-    }
-  }
-  __syncthreads();
-  f = *found;
-  return true;
-}
-
-// Eight 16-bit elements, wherever they begin.
-template <typename T> __device__ __forceinline__ uint4 load8(const T* p, bool wide) {
-  if (wide) return *reinterpret_cast<const uint4*>(p);
-  const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
-  return make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-}
-template <typename T> __device__ __forceinline__ float2 two_floats(uint32_t u);
-template <> __device__ __forceinline__ float2 two_floats<__nv_bfloat16>(uint32_t u) { return st::unpack_bf16x2(u); }
-template <> __device__ __forceinline__ float2 two_floats<__half>(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
-template <typename T> __device__ __forceinline__ T from_f(float x);
-template <> __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
-template <> __device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
-
-// An item, or the part of it that the block's run covers: units [t0, t1) of one head's rows [row0, row_end) of a sequence.
-struct Item {
-  const int* table;
-  int start, n, len, h, row0, row_end, t0, t1, tiles;
-  int keys;      // that the last row sees
-  int next;      // number of the unit behind it
-  // Units to work on: those behind the last key are left out, one stays.
-  __device__ __forceinline__ int steps() const { return max(min(t1, (keys + kTile - 1) / kTile) - t0, 1); }
-};
-// The first item with work at or behind unit u of the run that ends at u1; false: there is none.
-template <int N>
-__device__ __forceinline__ bool item_at(Item& it, const AttnParams& p, int u, int u1, Found& f, Seq& sq) {
-#pragma unroll 1
-  while (u < u1) {
-    while (u >= f.first + sq.units) {
-      f.first += sq.units;
-      sq = sequence<N>(p, ++f.b);
-    }
-    // unit -> (key head, row block, tile): row blocks of one head next to each other, as they read the same pages
-    const unsigned size = sq.size, in = u - f.first, item = in / size;
-    const int at = in - item * size, end = min(static_cast<int>(size), at + (u1 - u));
-    u += end - at;
-    it.t0 = p.whole ? 0 : max(at - kItemCost<N>, 0), it.t1 = p.whole ? sq.tiles : end - kItemCost<N>;
-    if (it.t1 <= it.t0) continue;      // nothing but the count for its beginning
-    it.next = u;
-    it.h = item / static_cast<unsigned>(sq.row_blocks);
-    const int rb = item - it.h * sq.row_blocks;
-    it.tiles = sq.tiles, it.start = sq.start, it.n = sq.n, it.len = sq.len;
-    it.row0 = rb * N, it.row_end = min(sq.n * p.group, it.row0 + N);
-    it.table = p.table + f.b * p.table_row;
-    it.keys = max(it.len - (p.causal ? it.n - 1 - (it.row_end - 1) / p.group : 0), 0);
-    return true;
-  }
-  return false;
-}
 
 __device__ __forceinline__ void umma_codes(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -233,25 +80,6 @@ __device__ __forceinline__ void tmem_st_8(uint32_t taddr, const uint32_t (&r)[8]
                ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
-template <int THREADS>
-__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
-template <int THREADS>
-__device__ __forceinline__ bool soft_any(bool x) {      // of the softmax threads; a barrier too
-  uint32_t y;
-  asm volatile(
-      "{\n"
-      ".reg .pred p, q;\n"
-      "setp.ne.u32 p, %1, 0;\n"
-      "barrier.cta.red.or.pred q, 1, %2, p;\n"
-      "selp.u32 %0, 1, 0, q;\n"
-      "}\n"
-      : "=r"(y)
-      : "r"(static_cast<uint32_t>(x)), "n"(THREADS)
-      : "memory");
-  return y != 0;
-}
-// Bytes of e4m3 that are no number, as 0x80 in their places.
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 // Splits off the upper bytes, e5m2 numbers, of eight fp16 numbers: returns them side by side, and leaves the rest (exactly).
 __device__ __forceinline__ uint2 split_off(__half2 (&x)[4]) {
   uint32_t u[4];
@@ -321,29 +149,6 @@ struct Shared {
 };
 static_assert(sizeof(Shared<128, 8, 3>) <= 113 * 1024 && sizeof(Shared<128, 16, 3>) <= 113 * 1024 && sizeof(Shared<128, 32, 3>) <= 113 * 1024 && sizeof(Shared<128, 8, 4>) <= 113 * 1024 &&
               sizeof(Shared<128, 16, 4>) <= 113 * 1024 && sizeof(Shared<128, 32, 4>) <= 113 * 1024 && sizeof(Shared<64, 16, 4>) <= 113 * 1024 && sizeof(Shared<64, 32, 4>) <= 226 * 1024);
-constexpr int kInvalid = -1000, kBehind = -2147483647 - 1;      // of a page: none by that number; none, as the keys end before it
-
-// What a block notes about the border behind its run: the item that it is inside of (parts 0: none).
-struct Note {
-  int parts, first, border;      // parts of the item, block of the first one, place of this border among the item's
-  int rows, start, row0, h;      // live rows, and where they belong
-  int unused;
-};
-
-
-template <int R>
-__device__ __forceinline__ float* part_of(const AttnParams& p, int D, long long slot) {      // [R][D] output, [R] reference, [R] sum
-  return p.parts + slot * (R * (D + 2));
-}
-
-// After a wait ran out: what the block's last `turns` turns set going, a ring of barriers long, gets a millisecond to come to its end.
-template <int STAGES>
-__device__ __forceinline__ void settle(unsigned long long (&bars)[STAGES], uint32_t turns) {
-  const uint64_t t0 = st::globaltimer_ns();
-#pragma unroll 1
-  for (uint32_t i = turns > STAGES ? turns - STAGES : 0; i < turns; ++i)
-    while (!st::mbar_try_wait(st::smem_u32(&bars[i % STAGES]), i / STAGES & 1) && st::globaltimer_ns() - t0 < 1000000) {}
-}
 
 // ---- copies -------------------------------------------------------------------------------------------------------------------------
 // The run's units one after another, for keys or for values.  Page numbers and scales are looked up for 32 pages at a time (4 units of 8 pages
@@ -829,39 +634,12 @@ __device__ __forceinline__ void soft_warps(S& sh, const AttnParams& p, uint32_t 
         }
       }
     }
-    if (threadIdx.x == 0 && it.t1 < it.tiles) {      // the run ends inside the item; never where items are whole, which have no notes
-      // Block b holds a part if its run begins before the item's end, all * b / runs < end, which is all * b < end * runs, and ends behind its first unit.
-      const long long first_unit = u1 - it.t1, end = first_unit + it.tiles;
-      Note n{};
-      n.first = static_cast<int>(((first_unit + 1) * runs - 1) / all);
-      n.parts = static_cast<int>((end * runs - 1) / all) - n.first + 1;
-      n.border = static_cast<int>(blockIdx.x) - n.first;
-      n.rows = rows, n.start = it.start, n.row0 = it.row0, n.h = it.h;
-      *note = n;
-    }
+    if (threadIdx.x == 0 && it.t1 < it.tiles) *note = note_of(it, u1, runs, all);      // the run ends inside the item; never where items are whole, which have no notes
     st::tc_fence_before();
     soft_sync<SOFT>();      // everything of the item is read
     if (next >= u1) return;
     for (int i = threadIdx.x; i < R * (D / 32); i += SOFT) sh.bad[i / (D / 32)][i % (D / 32)] = 0;
     if (threadIdx.x == 0) st::mbar_arrive(st::smem_u32(&sh.q_empty[item % L::Q_BUFS]));
-  }
-}
-
-// Rows behind the last sequence: 0, by one warp of every block.
-template <typename T, int D>
-__device__ __forceinline__ void zero_rows(const AttnParams& p) {
-  const int lane = threadIdx.x & 31, vectors = p.heads * (D / 2);
-  const long long from = p.B > 0 ? max(p.starts[p.B], 0) : 0;
-#pragma unroll 1
-  for (long long row = from + blockIdx.x; row < p.rows; row += gridDim.x) {
-    T* o = static_cast<T*>(p.out) + row * p.o_row;
-#pragma unroll 1
-    for (int i = lane; i < vectors; i += 32) {
-      T* at = o + i / (D / 2) * p.o_head + i % (D / 2) * 2;
-      at[0] = at[1] = from_f<T>(0.0f);
-    }
-    if (p.lse != nullptr)
-      for (int i = lane; i < p.heads; i += 32) p.lse[row * p.heads + i] = -INFINITY;
   }
 }
 
@@ -938,100 +716,38 @@ __global__ void __launch_bounds__(kThreadsOf<R>, Layout<D, R, kQueryParts<T>>::B
   if (warp == SW + 1) st::tmem_dealloc(tmem, L::COLUMNS);
 }
 
-// Joins the parts of the items that several blocks worked on.  A block per border; an item of P parts has P - 1 of them, which share its rows.
-// With few parts a warp does a row; with many, the block's warps share the parts of a row.
-constexpr int kJoinThreads = 128, kWarps = kJoinThreads / 32;
-template <typename T, int D, int N>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(AttnParams p) {
-  constexpr int E = D / 32;
-  extern __shared__ float weight[];      // [kWarps][few] or [parts]
-  __shared__ float red[2][kWarps], rows[kWarps][D];
-  const float* parts = p.parts;
-  const Note* notes = reinterpret_cast<const Note*>(p.notes);
-  chain_begin(parts, notes);
-  const Note n = notes[blockIdx.x];
-  if (n.parts < 2) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  constexpr long long kSlot = N * (D + 2);
-  constexpr int kFew = 8;
-  const float* base = parts + 2LL * n.first * kSlot;      // part 0 lies in its block's second slot, the others in the first slots of their blocks
-  const bool few = n.parts <= kFew;
-  const int members = few ? kWarps : 1, me = few ? warp : 0, width = few ? 32 : kJoinThreads, at = few ? lane : threadIdx.x;
-  for (int r = n.border * members + me; r < n.rows; r += (n.parts - 1) * members) {      // few: warps go their own ways, without barriers
-    float m = -INFINITY;
-    for (int i = at; i < n.parts; i += width) {
-      const float* part = base + (2LL * i + (i == 0 ? 1 : 0)) * kSlot + N * D;
-      if (part[N + r] != 0.0f) m = fmaxf(m, part[r]);      // a sum of 0: saw nothing
-    }
-    m = st::warp_max(m);
-    if (!few) {
-      __syncthreads();
-      if (lane == 0) red[0][warp] = m;
-      __syncthreads();
-      m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    }
-    float l = 0.0f, *w = weight + (few ? warp * kFew : 0);
-    for (int i = at; i < n.parts; i += width) {
-      const float* part = base + (2LL * i + (i == 0 ? 1 : 0)) * kSlot + N * D;
-      const float pl = part[N + r], e = pl == 0.0f ? 0.0f : st::exp2_ftz(part[r] - m);
-      w[i] = e;
-      l += pl * e;
-    }
-    l = st::warp_sum(l);
-    if (few) {
-      __syncwarp();
-    } else {
-      if (lane == 0) red[1][warp] = l;
-      __syncthreads();
-      l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-    }
-    float x[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = 0.0f;
-#pragma unroll 8
-    for (int i = few ? 0 : warp; i < n.parts; i += few ? 1 : kWarps) {
-      const float e = w[i];
-      const float* part = base + (2LL * i + (i == 0 ? 1 : 0)) * kSlot + r * D + lane * E;
-      if constexpr (E == 4) {
-        const float4 y = *reinterpret_cast<const float4*>(part);
-        x[0] = fmaf(y.x, e, x[0]), x[1] = fmaf(y.y, e, x[1]), x[2] = fmaf(y.z, e, x[2]), x[3] = fmaf(y.w, e, x[3]);
-      } else {
-        const float2 y = *reinterpret_cast<const float2*>(part);
-        x[0] = fmaf(y.x, e, x[0]), x[1] = fmaf(y.y, e, x[1]);
-      }
-    }
-    const int fr = n.row0 + r;
-    const long long row = n.start + fr / p.group;
-    const int head = n.h * p.group + fr % p.group;
-    T* o = static_cast<T*>(p.out) + row * p.o_row + head * p.o_head;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (few) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[lane * E + e] = from_f<T>(x[e] * inv);
-      __syncwarp();
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) rows[warp][lane * E + e] = x[e];
-      __syncthreads();
-      const int d = threadIdx.x;
-      if (d < D) o[d] = from_f<T>(((rows[0][d] + rows[1][d]) + (rows[2][d] + rows[3][d])) * inv);
-    }
-    if (at == 0 && p.lse != nullptr) p.lse[row * p.heads + head] = l == 0.0f ? -INFINITY : (m + kLift + log2f(l)) / kLog2e;
-  }
-}
-
 // Rows of an item, by those that the longest step of a sequence has for a key head.
 int item_rows(long long max_queries, int group) {
   const long long rows = max_queries * group;
-  return rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+  return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : kPromptRows;
 }
 // Blocks that run at once: two to an SM, one where the products take all columns of tensor memory.
-int runs_of(int rows, int dim) { return st::sm_count() * (dim == 64 && rows == 32 ? Layout<64, 32, 4>::BLOCKS : Layout<128, 32, 4>::BLOCKS); }
+int runs_of(int rows, int dim) { return st::sm_count() * (rows == kPromptRows ? 1 : dim == 64 && rows == 32 ? Layout<64, 32, 4>::BLOCKS : Layout<128, 32, 4>::BLOCKS); }
 
 // Whether items of sequences of up to `tokens` tokens are whole: a unit takes a block 1000 cycles, of 32 rows 2500, the second kernel and what it waits for
 // 6 us of the GPU and 4 of the host.
 bool not_split(int rows, long long tokens) { return tokens <= (rows == 32 ? 18 : 7) * kTile; }
 
+template <typename T, int D, int R>
+int launch_join(const AttnParams& p, cudaStream_t stream) {
+  if (p.whole) return ST_OK;
+  const int runs = runs_of(R, D);
+  const cudaError_t e = st::chained(paged_join_kernel<T, D, R>, dim3(runs - 1, R == kPromptRows ? 16 : 1), dim3(kJoinThreads), runs * sizeof(float), stream)(p);
+  return e == cudaSuccess ? ST_OK : st::fail_cuda(e, "paged attention: join");
+}
+template <typename T, int D>
+int launch_prompt(const AttnParams& p, cudaStream_t stream) {
+  constexpr int smem = sizeof(PromptShared<D>);
+  auto kernel = paged_prompt_kernel<T, D>;
+  static bool opted[st::kMaxDevices];
+  if (bool& done = opted[st::current_device()]; !done) {
+    ST_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    done = true;
+  }
+  const cudaError_t e = st::in_order(kernel, dim3(runs_of(kPromptRows, D)), dim3(kThreadsOf<kPromptRows>), smem, stream)(p);
+  if (e != cudaSuccess) return st::fail_cuda(e, "paged attention");
+  return launch_join<T, D, kPromptRows>(p, stream);
+}
 template <typename T, int D, int R>
 int launch(const AttnParams& p, cudaStream_t stream) {
   const int runs = runs_of(R, D);
@@ -1054,16 +770,13 @@ int launch(const AttnParams& p, cudaStream_t stream) {
     done = true;
   }
   // in order: blocks that come early pile up on the SMs that fall free first
-  cudaError_t e = st::in_order(kernel, dim3(runs), dim3(kThreadsOf<R>), smem, stream)(p, maps[0], maps[1]);
+  const cudaError_t e = st::in_order(kernel, dim3(runs), dim3(kThreadsOf<R>), smem, stream)(p, maps[0], maps[1]);
   if (e != cudaSuccess) return st::fail_cuda(e, "paged attention");
-  if (p.whole) return ST_OK;
-  e = st::chained(paged_join_kernel<T, D, R>, dim3(runs - 1), dim3(kJoinThreads), runs * sizeof(float), stream)(p);
-  if (e != cudaSuccess) return st::fail_cuda(e, "paged attention: join");
-  return ST_OK;
+  return launch_join<T, D, R>(p, stream);
 }
 template <typename T, int D>
 int dispatch(const AttnParams& p, int rows, cudaStream_t stream) {
-  return rows == 8 ? launch<T, D, 8>(p, stream) : rows == 16 ? launch<T, D, 16>(p, stream) : launch<T, D, 32>(p, stream);
+  return rows == 8 ? launch<T, D, 8>(p, stream) : rows == 16 ? launch<T, D, 16>(p, stream) : rows == 32 ? launch<T, D, 32>(p, stream) : launch_prompt<T, D>(p, stream);
 }
 }  // namespace
 

@@ -362,6 +362,31 @@ def test_attention_of_long_tables_captured_twice():
 
 
 @GPU
+@pytest.mark.parametrize("D,H,G,page,dtype,causal", [(128, 2, 1, 16, torch.bfloat16, True), (64, 1, 2, 64, torch.float16, True), (128, 1, 3, 256, torch.float16, False), (64, 2, 1, 128, torch.bfloat16, False)])
+def test_attention_of_parts_of_prompts(D, H, G, page, dtype, causal):
+    """Items of 128 rows: of one unit, two, an odd number; whole prompts and their ends; rows that fill no item."""
+    _check_attention([1, 127, 128, 129, 256, 257, 385, 500], [1, 127, 128, 129, 100, 257, 385, 33], H, G, page, D, dtype, causal, seed=G, max_queries=400)
+    _check_attention([3000, 40, 2500, 0], [200, 40, 129, 3], H, G, page, D, dtype, causal, seed=G)
+    _check_attention([200, 130], [130, 130], H, G, page, D, dtype, causal, scale=-0.3)
+    _check_attention([200, 130], [130, 130], H, G, page, D, dtype, causal, scale=0.0, spread=7)
+
+
+@GPU
+def test_attention_of_parts_of_prompts_with_numbers_that_are_none():
+    def values(pages, table, fused):       # hidden from the rows before them
+        pages.v.view(torch.uint8)[table[0, 20], 0, 1, 5] = 0xFF
+        pages.v.view(torch.uint8)[table[0, 3], 0, 13, 63] = 0x7F
+        pages.k.view(torch.uint8)[table[0, 30], 0, 2, 9] = 0x7F
+    got = _check_attention([500, 70], [460, 60], 1, 1, 16, 64, torch.bfloat16, edit=values)
+    assert not got[:21, 0, 63].isnan().any() and got[21:460, 0, 63].isnan().all() and not got[:281, 0, 5].isnan().any() and got[281:460, 0, 5].isnan().all()
+    assert got[442:460].isnan().all() and not got[460:].isnan().any() and not got[:442, 0, 6].isnan().any()
+    def queries(pages, table, fused):      # one row's
+        fused[7, 3] = float("nan")
+    got = _check_attention([300], [200], 1, 1, 64, 128, torch.float16, edit=queries)
+    assert got[7].isnan().all() and got.isnan().any(-1).sum() == 1
+
+
+@GPU
 def test_attention_scales_far_apart_and_large_scores():
     _check_attention(LENGTHS, [1] * 9, 2, 2, 16, 64, torch.bfloat16, spread=7)
     # value scales 2^40 apart: the codes of the small ones must not be lost in front of the large ones' masked or light keys
