@@ -28,7 +28,7 @@ struct PromptShared {
   Item item[2];
   float factor[2][kPromptRows];
   float2 stat[2][kPromptRows];      // a group's references and sums
-  int bad[4][D];                    // first row that a value reaches which is no number though not all rows see it
+  int bad[4][D], some_bad[4];       // first row that a value reaches which is no number though not all rows see it; whether there are such
   int sums[kMaxWarps];
   Found found;
   uint32_t tmem;
@@ -47,94 +47,110 @@ __device__ __forceinline__ uint32_t two_halves(uint32_t codes) {
 }
 
 // ---- keys or values: pages -> registers -> fp16 in shared memory ---------------------------------------------------------------------
-// Four warps; each has 32 keys of a unit, at most two pages, and loads a unit's codes while it converts those of the unit before.
+// Four warps; each has 32 keys of a unit, at most two pages.
 template <int D, bool VALUES, typename S>
 __device__ __forceinline__ void convert_warp(S& sh, const AttnParams& p, int u, int u1, Found f, Seq sq) {
   constexpr int VECS = D / 16, PER = 32 / VECS, LOADS = 32 / PER;      // 16-byte vectors of a key, keys of a load
   const int lane = threadIdx.x & 31, first = (threadIdx.x >> 5 & 3) * 32, at = lane / VECS, vec = lane % VECS;
   const unsigned char* codes = (VALUES ? p.vc : p.kc) + at * D + vec * 16;
   const int mask = (1 << p.shift) - 1;
-  // The unit whose codes are loaded: t of it, -1 behind the last; its pages, one to 16 lanes.
+  // A unit ahead of the one that is converted its codes and scales are on their way, two ahead its page numbers.
+  struct Unit {
+    int key, h, keys;          // its first key (-1: no more), key head, keys that the item sees
+    int all, sees, item;       // keys of it that all rows see, first row that sees its first key
+    int page;                  // one to 16 lanes
+  };
   Item it;
-  int t = 0, end = 0, items = -1, page = -1;
-  auto advance = [&] {
+  int t = 0, end = 0, items = -1;
+  auto advance = [&](Unit& x) {
     if (++t >= end) {
       if (!item_at<kPromptRows>(it, p, u, u1, f, sq)) {
-        t = -1;
+        u = u1, t = end - 1, x = Unit{-1, 0, 0, kTile, 0, 0, kBehind};
         return;
       }
       u = it.next, t = it.t0, end = it.t0 + it.steps(), ++items;
     }
-    const int key = t * kTile + first + (lane & 16);
-    page = key < it.keys ? it.table[key >> p.shift] : kBehind;
+    x.key = t * kTile, x.h = it.h, x.keys = it.keys, x.item = items & 3;
+    x.all = max(it.len - (p.causal ? it.n - 1 - it.row0 / p.group : 0), 0) - x.key, x.sees = (x.key + it.n - it.len) * p.group - it.row0;
+    const int key = x.key + first + (lane & 16);
+    x.page = key < it.keys ? it.table[key >> p.shift] : kBehind;
   };
   uint4 raw[LOADS];
+  float ks = 0.0f, vs = 0.0f;
   const unsigned char* from[2];
   int live[2];      // keys of 16 that there are
-  auto look = [&] {      // the page numbers have come
-    if (page < 0 || page >= p.pages) {
-      if (VALUES && page != kBehind && (lane & 15) == 0) st::report_error(p.err, st::ERR_BOUNDS, 0x7004);
-      page = -1;
+  auto look = [&](Unit& x) {
+    if (x.page < 0 || x.page >= p.pages) {
+      if (VALUES && x.page != kBehind && (lane & 15) == 0) st::report_error(p.err, st::ERR_BOUNDS, 0x7004);
+      x.page = -1;
+    } else if (VALUES) {
+      const long long scale = static_cast<long long>(x.page) * p.kv_heads + x.h;
+      ks = p.ks[scale], vs = p.vs[scale];
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int pg = __shfl_sync(0xffffffffu, page, 16 * h), key = t * kTile + first + 16 * h;
-      from[h] = codes + (((static_cast<long long>(pg) * p.kv_heads + it.h) << p.shift) + (key & mask)) * D;
-      live[h] = pg >= 0 ? it.keys - key : 0;
+      const int pg = __shfl_sync(0xffffffffu, x.page, 16 * h), key = x.key + first + 16 * h;
+      from[h] = codes + (((static_cast<long long>(pg) * p.kv_heads + x.h) << p.shift) + (key & mask)) * D;
+      live[h] = pg >= 0 ? x.keys - key : 0;
     }
   };
   auto load = [&](int j) {
     const int h = j * PER / 16, in = j * PER % 16;
-    raw[j] = in + at < live[h] ? *reinterpret_cast<const uint4*>(from[h] + in * D) : make_uint4(0, 0, 0, 0);
+    raw[j] = make_uint4(0, 0, 0, 0);
+    if (in + at < live[h]) raw[j] = *reinterpret_cast<const uint4*>(from[h] + in * D);
   };
-  advance();
-  if (t < 0) return;
-  look();
+  Unit now, next;
+  advance(now);
+  if (now.key < 0) return;
+  advance(next);
+  look(now);
 #pragma unroll
   for (int j = 0; j < LOADS; ++j) load(j);
   uint32_t turn = 0;
 #pragma unroll 1
   for (;; ++turn) {
-    const int g = turn & 1, now_item = items & 3;
+    const int g = turn & 1;
     const uint32_t before = (turn >> 1 & 1) ^ 1;
-    const int limit_min = max(it.len - (p.causal ? it.n - 1 - it.row0 / p.group : 0), 0) - t * kTile;      // keys that all rows see
-    const int sees = (t * kTile + it.n - it.len) * p.group - it.row0;                                      // first row that sees key 0 of the unit
     if (VALUES) {
-      const bool there = page >= 0;
-      const long long scale = static_cast<long long>(page) * p.kv_heads + it.h;
-      const float ks = there ? p.ks[scale] : 0.0f;
-      const int b = there ? st::scale_exponent(p.vs[scale]) : 0;
       if (!st::mbar_wait_warp(st::smem_u32(&sh.p_full[g]), before, &sh.abort)) return;      // the scales of the turn before last are read
       if ((lane & 15) == 0) {
-        const int group = (first + lane) / 16;
-        sh.ks[g][group] = ks;
+        const int group = (first + lane) / 16, b = st::scale_exponent(vs);
+        const bool there = now.page >= 0;
+        sh.ks[g][group] = there ? ks : 0.0f;
         sh.lift[g][group] = there ? static_cast<float>(b) : -INFINITY;
         sh.take[g][group] = there ? st::exp2_int(-b - static_cast<int>(kLift)) : 0.0f;
         st::mbar_arrive(st::smem_u32(&sh.scales[g]));
       }
       __syncwarp();
     }
-    advance();
-    if (!st::mbar_wait_warp(st::smem_u32(VALUES ? &sh.pv_done[g] : &sh.s_full[g]), before, &sh.abort)) return;
-    if (t >= 0) look();
-    else live[0] = live[1] = 0;
-    unsigned char* to = (VALUES ? sh.v[g] : sh.k[g]) + vec / 4 * (128 * 128);
+    if (VALUES && now.all < kTile) {      // values that are no numbers and not for all rows: 0, and a note of the first row that sees them
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      const int row = first + j * PER + at;
-      uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
-      load(j);
-      if (VALUES && limit_min < kTile && (nan_bytes(w[0]) | nan_bytes(w[1]) | nan_bytes(w[2]) | nan_bytes(w[3])) != 0 && row >= limit_min) {
-        // no numbers, and not for all rows: those from this one on see the key
+      for (int j = 0; j < LOADS; ++j) {
+        uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+        const int row = first + j * PER + at;
+        if ((nan_bytes(w[0]) | nan_bytes(w[1]) | nan_bytes(w[2]) | nan_bytes(w[3])) == 0 || row < now.all) continue;
+        sh.some_bad[now.item] = 1;
 #pragma unroll 1
         for (int c = 0; c < 16; ++c) {
           const uint32_t x = c < 4 ? w[0] : c < 8 ? w[1] : c < 12 ? w[2] : w[3];
-          if (nan_bytes(x) >> (8 * (c & 3) + 7) & 1) atomicMin(&sh.bad[now_item][vec * 16 + c], max(sees + row * p.group, 0));
+          if (nan_bytes(x) >> (8 * (c & 3) + 7) & 1) atomicMin(&sh.bad[now.item][vec * 16 + c], max(now.sees + row * p.group, 0));
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] &= ~((nan_bytes(w[i]) >> 7) * 255u);
+        raw[j] = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      const int chunk = vec % 4 * 2, odd = D == 128 ? vec / 4 : 0;      // the second half's odd part first: other banks than the first half's even one
+    }
+    if (!st::mbar_wait_warp(st::smem_u32(VALUES ? &sh.pv_done[g] : &sh.s_full[g]), before, &sh.abort)) return;
+    const bool more = next.key >= 0;
+    now = next;
+    look(now);
+    unsigned char* to = (VALUES ? sh.v[g] : sh.k[g]) + vec / 4 * (128 * 128);
+    const int chunk = vec % 4 * 2, odd = D == 128 ? vec / 4 : 0;      // the second half's odd part first: other banks than the first half's even one
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      const int row = first + j * PER + at;
+      const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+      load(j);
       uint4 h[2];
       h[0] = make_uint4(two_halves(w[0]), two_halves(w[0] >> 16), two_halves(w[1]), two_halves(w[1] >> 16));
       h[1] = make_uint4(two_halves(w[2]), two_halves(w[2] >> 16), two_halves(w[3]), two_halves(w[3] >> 16));
@@ -143,7 +159,8 @@ __device__ __forceinline__ void convert_warp(S& sh, const AttnParams& p, int u, 
     }
     st::fence_proxy_async_smem();
     st::mbar_arrive(st::smem_u32(VALUES ? &sh.v_full[g] : &sh.k_full[g]));
-    if (t < 0) return;
+    if (!more) return;
+    advance(next);
   }
 }
 
@@ -235,7 +252,7 @@ __device__ __forceinline__ void prompt_query_warp(S& sh, const AttnParams& p, in
     const int buf = item & 1;
     if (!st::mbar_wait_warp(st::smem_u32(&sh.q_empty[buf]), (item >> 1 & 1) ^ 1, &sh.abort)) return;
     if (w == 0 && lane == 0) sh.item[buf] = it;
-#pragma unroll 1
+#pragma unroll 3
     for (int r = 8 * w + lane / 4; r < kPromptRows; r += 24) {
       const int fr = it.row0 + r, i = fr / p.group, head = it.h * p.group + fr - i * p.group;
       const bool live = fr < it.row_end;
@@ -281,12 +298,68 @@ __device__ __forceinline__ void prompt_query_warp(S& sh, const AttnParams& p, in
 }
 
 // ---- the softmax ---------------------------------------------------------------------------------------------------------------------
+// The largest x of a row's scores.  MASKED: keys from `end` on do not count, nor those of pages that are none.
+template <bool MASKED>
+__device__ __forceinline__ float prompt_top(uint32_t s_cols, float factor, const float* ks, const float* lift, int end) {
+  float top = -INFINITY;
+#pragma unroll 2
+  for (int c = 0; c < 4; ++c) {
+    uint32_t raw[32];
+    st::tmem_ld_32x32(s_cols + 32 * c, raw);
+    const float2 k = *reinterpret_cast<const float2*>(ks + 2 * c), b = *reinterpret_cast<const float2*>(lift + 2 * c);
+    st::tmem_ld_wait();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float x[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = MASKED && 32 * c + 16 * h + j >= end ? -INFINITY : __uint_as_float(raw[16 * h + j]);
+      float m = st::max3(x[0], x[1], x[2]), n = st::max3(x[3], x[4], x[5]);
+      m = st::max3(m, x[6], x[7]), n = st::max3(n, x[8], x[9]);
+      m = st::max3(m, x[10], x[11]), n = st::max3(n, x[12], x[13]);
+      m = st::max3(m, x[14], x[15]);
+      top = fmaxf(top, fmaf(fmaxf(m, n), factor * (h ? k.y : k.x), h ? b.y : b.x));
+    }
+  }
+  return top;
+}
+// Weights over the scores that they are made from; returns the sum with them.
+template <bool MASKED>
+__device__ __forceinline__ float prompt_weights(uint32_t s_cols, float factor, float ref, float sum, const float* ks, const float* lift, const float* take, int end) {
+#pragma unroll 2
+  for (int c = 0; c < 4; ++c) {
+    uint32_t raw[32], w[16];
+    st::tmem_ld_32x32(s_cols + 32 * c, raw);
+    const float2 k = *reinterpret_cast<const float2*>(ks + 2 * c), b = *reinterpret_cast<const float2*>(lift + 2 * c), t = *reinterpret_cast<const float2*>(take + 2 * c);
+    st::tmem_ld_wait();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float lifted = h ? b.y : b.x;
+      const float2 fs = st::splat2(factor * (h ? k.y : k.x)), bs = st::splat2(lifted - ref);
+      const bool none = MASKED && lifted == -INFINITY;
+      float2 part = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) {
+        float2 x = st::fma2(make_float2(__uint_as_float(raw[16 * h + j]), __uint_as_float(raw[16 * h + j + 1])), fs, bs);
+        x.x = st::exp2_ftz(x.x), x.y = st::exp2_ftz(x.y);
+        if (MASKED && (none || 32 * c + 16 * h + j >= end)) x.x = 0.0f;
+        if (MASKED && (none || 32 * c + 16 * h + j + 1 >= end)) x.y = 0.0f;
+        part = st::add2(part, x);
+        const __half2 y = __floats2half2_rn(x.x, x.y);
+        w[8 * h + j / 2] = *reinterpret_cast<const uint32_t*>(&y);
+      }
+      sum = fmaf(part.x + part.y, h ? t.y : t.x, sum);
+    }
+    st::tmem_st_32x16(s_cols + 16 * c, w);
+  }
+  return sum;
+}
+
 template <typename T, int D, typename S>
 __device__ __forceinline__ void prompt_soft_warps(S& sh, const AttnParams& p, uint32_t tmem_all, Note* note, int u1, int runs, int all) {
   const int row = threadIdx.x & 127, g = threadIdx.x >> 7;
   const uint32_t lanes = tmem_all + ((threadIdx.x >> 5 & 3) << 21), s_cols = lanes + g * 128, o_cols = lanes + 256 + g * D;
   T* out = static_cast<T*>(p.out);
-  const bool wide = ((p.o_row | p.o_head) & 7) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  const bool wide = ((p.o_row | p.o_head) & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0;
   uint32_t first = 0;      // turn of the item's first unit
 #pragma unroll 1
   for (uint32_t item = 0;; ++item) {
@@ -305,36 +378,14 @@ __device__ __forceinline__ void prompt_soft_warps(S& sh, const AttnParams& p, ui
     for (int i = mine; i < steps; i += 2) {
       const uint32_t turn = first + i, phase = turn >> 1 & 1;
       st::mbar_wait_warp(st::smem_u32(&sh.scales[g]), phase, &sh.abort);
-      float f[8], b[8];
-      bool gone = (t0 + i + 1) * kTile > limit_min;      // some row may not see some key
+      bool none = false;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        f[c] = factor * sh.ks[g][c], b[c] = sh.lift[g][c];
-        gone = gone || b[c] == -INFINITY;
-      }
+      for (int c = 0; c < 8; ++c) none = none || sh.lift[g][c] == -INFINITY;
+      const bool gone = none || (t0 + i + 1) * kTile > limit_min;      // some row may not see some key
       const int end = limit - (t0 + i) * kTile;      // keys of the unit that the row sees
       st::mbar_wait_warp(st::smem_u32(&sh.s_full[g]), phase, &sh.abort);
       st::tc_fence_after();
-      float top = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t raw[32];
-        st::tmem_ld_32x32(s_cols + 32 * c, raw);
-        st::tmem_ld_wait();
-        if (gone) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (32 * c + j >= end) raw[j] = __float_as_uint(-INFINITY);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float m = __uint_as_float(raw[16 * h]);
-#pragma unroll
-          for (int j = 1; j < 15; j += 2) m = st::max3(m, __uint_as_float(raw[16 * h + j]), __uint_as_float(raw[16 * h + j + 1]));
-          m = fmaxf(m, __uint_as_float(raw[16 * h + 15]));
-          top = fmaxf(top, fmaf(m, f[2 * c + h], b[2 * c + h]));
-        }
-      }
+      const float top = gone ? prompt_top<true>(s_cols, factor, sh.ks[g], sh.lift[g], end) : prompt_top<false>(s_cols, factor, sh.ks[g], sh.lift[g], end);
       if (__any_sync(0xffffffffu, top - ref > kLag + kLift)) {
         const float to = fmaxf(ref, top - kLift), shrink = st::exp2_ftz(ref - to);
         ref = to, sum *= shrink;
@@ -353,32 +404,7 @@ __device__ __forceinline__ void prompt_soft_warps(S& sh, const AttnParams& p, ui
           st::tmem_st_wait();
         }
       }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t raw[32], w[16];
-        st::tmem_ld_32x32(s_cols + 32 * c, raw);
-        st::tmem_ld_wait();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float2 fs = st::splat2(f[2 * c + h]), bs = st::splat2(b[2 * c + h] - ref);
-          float2 part = make_float2(0.0f, 0.0f);
-#pragma unroll
-          for (int j = 0; j < 16; j += 2) {
-            float2 x = st::fma2(make_float2(__uint_as_float(raw[16 * h + j]), __uint_as_float(raw[16 * h + j + 1])), fs, bs);
-            x.x = st::exp2_ftz(x.x), x.y = st::exp2_ftz(x.y);
-            if (gone) {
-              const bool none = b[2 * c + h] == -INFINITY;
-              if (none || 32 * c + 16 * h + j >= end) x.x = 0.0f;
-              if (none || 32 * c + 16 * h + j + 1 >= end) x.y = 0.0f;
-            }
-            part = st::add2(part, x);
-            const __half2 y = __floats2half2_rn(x.x, x.y);
-            w[8 * h + j / 2] = *reinterpret_cast<const uint32_t*>(&y);
-          }
-          sum = fmaf(part.x + part.y, sh.take[g][2 * c + h], sum);
-        }
-        st::tmem_st_32x16(s_cols + 16 * c, w);      // over scores that are read
-      }
+      sum = gone ? prompt_weights<true>(s_cols, factor, ref, sum, sh.ks[g], sh.lift[g], sh.take[g], end) : prompt_weights<false>(s_cols, factor, ref, sum, sh.ks[g], sh.lift[g], sh.take[g], end);
       st::tmem_st_wait();
       st::tc_fence_before();
       st::mbar_arrive(st::smem_u32(&sh.p_full[g]));
@@ -402,38 +428,52 @@ __device__ __forceinline__ void prompt_soft_warps(S& sh, const AttnParams& p, ui
     const float scale[2] = {(g == 0 ? w_own : w_other) * by, (g == 0 ? w_other : w_own) * by};
     const bool has[2] = {steps > 1 || (first & 1) == 0, steps > 1 || (first & 1) == 1};
     float* part = whole ? nullptr : part_of<kPromptRows>(p, D, 2LL * blockIdx.x + (it.t0 == 0 ? 1 : 0));
-    const int head = it.h * p.group + fr - query * p.group;
+    const int head = it.h * p.group + fr - query * p.group, lane = threadIdx.x & 31;
     const long long place = (it.start + query) * p.o_row + head * p.o_head;
+    const bool check = sh.some_bad[item & 3] != 0;
+    // 32 columns at a time through the room of the item's queries, which no product reads now: a warp's own 4 KB of it, four rows to a store
+    float* room = reinterpret_cast<float*>(sh.q[item & 1]) + (threadIdx.x >> 5) * 1024;
 #pragma unroll 1
-    for (int c = 0; c < D / 32; ++c) {
-      const int d = g * (D / 2) + 16 * c;
-      uint32_t o[2][16];
+    for (int c = 0; c < D / 64; ++c) {
+      const int d0 = g * (D / 2) + 32 * c;
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (has[k]) st::tmem_ld_32x16(lanes + 256 + k * D + d, o[k]);
-      st::tmem_ld_wait();
-      float y[16];
+      for (int half = 0; half < 2; ++half) {
+        const int d = d0 + 16 * half;
+        uint32_t o[2][16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float a = has[0] ? __uint_as_float(o[0][j]) * scale[0] : 0.0f;
-        y[j] = has[1] ? fmaf(__uint_as_float(o[1][j]), scale[1], a) : a;
-        if (whole && all_sum == 0.0f) y[j] = 0.0f;
-        if (row >= sh.bad[item & 3][d + j]) y[j] = NAN;
+        for (int k = 0; k < 2; ++k)
+          if (has[k]) st::tmem_ld_32x16(lanes + 256 + k * D + d, o[k]);
+        st::tmem_ld_wait();
+        float y[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float a = has[0] ? __uint_as_float(o[0][j]) * scale[0] : 0.0f;
+          y[j] = has[1] ? fmaf(__uint_as_float(o[1][j]), scale[1], a) : a;
+          if (whole && all_sum == 0.0f) y[j] = 0.0f;
+        }
+        if (check)
+          for (int j = 0; j < 16; ++j)
+            if (row >= sh.bad[item & 3][d + j]) y[j] = NAN;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(room + 32 * lane + 4 * ((4 * half + j) ^ (lane & 7))) = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
       }
-      if (row >= rows) continue;
-      if (!whole) {
-#pragma unroll
-        for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(part + row * D + d + j) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
-      } else if (wide) {
-        T h[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) h[j] = from_f<T>(y[j]);
-        reinterpret_cast<uint4*>(out + place + d)[0] = reinterpret_cast<const uint4*>(h)[0];
-        reinterpret_cast<uint4*>(out + place + d)[1] = reinterpret_cast<const uint4*>(h)[1];
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) out[place + d + j] = from_f<T>(y[j]);
+      __syncwarp();
+#pragma unroll 2
+      for (int k = 0; k < 8; ++k) {
+        const int r = 4 * k + lane / 8, in = (threadIdx.x >> 5 & 3) * 32 + r, d = d0 + 4 * (lane & 7);
+        const float4 y = *reinterpret_cast<const float4*>(room + 32 * r + 4 * ((lane & 7) ^ (r & 7)));
+        const long long to = __shfl_sync(0xffffffffu, place, r);
+        if (in >= rows) continue;
+        if (!whole) {
+          *reinterpret_cast<float4*>(part + in * D + d) = y;
+        } else {
+          const T h[4] = {from_f<T>(y.x), from_f<T>(y.y), from_f<T>(y.z), from_f<T>(y.w)};
+          if (wide) *reinterpret_cast<uint2*>(out + to + d) = *reinterpret_cast<const uint2*>(h);
+          else
+            for (int j = 0; j < 4; ++j) out[to + d + j] = h[j];
+        }
       }
+      __syncwarp();
     }
     if (g == 0 && row < rows) {
       if (!whole) part[kPromptRows * D + row] = m, part[kPromptRows * D + kPromptRows + row] = all_sum;
@@ -443,7 +483,10 @@ __device__ __forceinline__ void prompt_soft_warps(S& sh, const AttnParams& p, ui
     st::tc_fence_before();
     soft_sync<256>();      // everything of the item is read
     if (next >= u1) return;
-    if (threadIdx.x < D) sh.bad[item & 3][threadIdx.x] = kNoRow;
+    if (check) {
+      if (threadIdx.x < D) sh.bad[item & 3][threadIdx.x] = kNoRow;
+      if (threadIdx.x == 0) sh.some_bad[item & 3] = 0;
+    }
     if (threadIdx.x == 0) st::mbar_arrive(st::smem_u32(&sh.q_empty[item & 1]));
     first += steps;
   }
@@ -464,6 +507,7 @@ __global__ void __launch_bounds__(kThreadsOf<kPromptRows>, 1) paged_prompt_kerne
     st::fence_barrier_init();
     sh.abort = 0;
   }
+  if (threadIdx.x < 4) sh.some_bad[threadIdx.x] = 0;
   if (threadIdx.x < 4 * D) sh.bad[threadIdx.x / D][threadIdx.x % D] = kNoRow;
   chain_begin(p.ks, p.vs, p.table, p.starts, p.lengths);
   if (warp == 16) {
@@ -485,18 +529,14 @@ __global__ void __launch_bounds__(kThreadsOf<kPromptRows>, 1) paged_prompt_kerne
   }
   const Seq sq = sequence<kPromptRows>(p, f.b);
   uint2 under_way = make_uint2(0, 0);
-  // Registers of the launch: 96 of 640 threads.  Two groups of softmax get 128, two that convert 80, the others 64: 128 * (2 * 128 + 2 * 80 + 64) = 640 * 96.
   if (warp >= 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == 16) under_way = product_warp<D>(sh, tmem, u1);
     else prompt_query_warp<T, D>(sh, p, warp - 17, u0, u1, f, sq);
     if (p.zero_tail && warp == 19) zero_rows<T, D>(p);
   } else if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp < 12) convert_warp<D, false>(sh, p, u0, u1, f, sq);
     else convert_warp<D, true>(sh, p, u0, u1, f, sq);
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
     prompt_soft_warps<T, D>(sh, p, tmem, note, u1, runs, all);
     if (threadIdx.x == 0 && sh.abort) st::report_error(p.err, st::ERR_MBAR_TIMEOUT, 0x7006);
   }
