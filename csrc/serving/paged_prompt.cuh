@@ -47,12 +47,13 @@ __device__ __forceinline__ uint32_t two_halves(uint32_t codes) {
 }
 
 // ---- keys or values: pages -> registers -> fp16 in shared memory ---------------------------------------------------------------------
-// Four warps; each has 32 keys of a unit, at most two pages.
-template <int D, bool VALUES, typename S>
-__device__ __forceinline__ void convert_warp(S& sh, const AttnParams& p, int u, int u1, Found f, Seq sq) {
+// Four warps for keys and four for values, in the same code: with code for each, and with more of the rest unrolled, a quarter of the time went to waiting for
+// instructions.  Each warp has 32 keys of a unit, at most two pages.
+template <int D, typename S>
+__device__ __forceinline__ void convert_warp(S& sh, const AttnParams& p, bool values, int u, int u1, Found f, Seq sq) {
   constexpr int VECS = D / 16, PER = 32 / VECS, LOADS = 32 / PER;      // 16-byte vectors of a key, keys of a load
   const int lane = threadIdx.x & 31, first = (threadIdx.x >> 5 & 3) * 32, at = lane / VECS, vec = lane % VECS;
-  const unsigned char* codes = (VALUES ? p.vc : p.kc) + at * D + vec * 16;
+  const unsigned char* codes = (values ? p.vc : p.kc) + at * D + vec * 16;
   const int mask = (1 << p.shift) - 1;
   // A unit ahead of the one that is converted its codes and scales are on their way, two ahead its page numbers.
   struct Unit {
@@ -81,9 +82,9 @@ __device__ __forceinline__ void convert_warp(S& sh, const AttnParams& p, int u, 
   int live[2];      // keys of 16 that there are
   auto look = [&](Unit& x) {
     if (x.page < 0 || x.page >= p.pages) {
-      if (VALUES && x.page != kBehind && (lane & 15) == 0) st::report_error(p.err, st::ERR_BOUNDS, 0x7004);
+      if (values && x.page != kBehind && (lane & 15) == 0) st::report_error(p.err, st::ERR_BOUNDS, 0x7004);
       x.page = -1;
-    } else if (VALUES) {
+    } else if (values) {
       const long long scale = static_cast<long long>(x.page) * p.kv_heads + x.h;
       ks = p.ks[scale], vs = p.vs[scale];
     }
@@ -111,7 +112,7 @@ __device__ __forceinline__ void convert_warp(S& sh, const AttnParams& p, int u, 
   for (;; ++turn) {
     const int g = turn & 1;
     const uint32_t before = (turn >> 1 & 1) ^ 1;
-    if (VALUES) {
+    if (values) {
       if (!st::mbar_wait_warp(st::smem_u32(&sh.p_full[g]), before, &sh.abort)) return;      // the scales of the turn before last are read
       if ((lane & 15) == 0) {
         const int group = (first + lane) / 16, b = st::scale_exponent(vs);
@@ -123,7 +124,7 @@ __device__ __forceinline__ void convert_warp(S& sh, const AttnParams& p, int u, 
       }
       __syncwarp();
     }
-    if (VALUES && now.all < kTile) {      // values that are no numbers and not for all rows: 0, and a note of the first row that sees them
+    if (values && now.all < kTile) {      // values that are no numbers and not for all rows: 0, and a note of the first row that sees them
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) {
         uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
@@ -140,11 +141,11 @@ __device__ __forceinline__ void convert_warp(S& sh, const AttnParams& p, int u, 
         raw[j] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    if (!st::mbar_wait_warp(st::smem_u32(VALUES ? &sh.pv_done[g] : &sh.s_full[g]), before, &sh.abort)) return;
+    if (!st::mbar_wait_warp(st::smem_u32(values ? &sh.pv_done[g] : &sh.s_full[g]), before, &sh.abort)) return;
     const bool more = next.key >= 0;
     now = next;
     look(now);
-    unsigned char* to = (VALUES ? sh.v[g] : sh.k[g]) + vec / 4 * (128 * 128);
+    unsigned char* to = (values ? sh.v[g] : sh.k[g]) + vec / 4 * (128 * 128);
     const int chunk = vec % 4 * 2, odd = D == 128 ? vec / 4 : 0;      // the second half's odd part first: other banks than the first half's even one
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
@@ -158,7 +159,7 @@ __device__ __forceinline__ void convert_warp(S& sh, const AttnParams& p, int u, 
       *reinterpret_cast<uint4*>(to + st::sw128_offset(row, chunk + (odd ^ 1))) = odd ? h[0] : h[1];
     }
     st::fence_proxy_async_smem();
-    st::mbar_arrive(st::smem_u32(VALUES ? &sh.v_full[g] : &sh.k_full[g]));
+    st::mbar_arrive(st::smem_u32(values ? &sh.v_full[g] : &sh.k_full[g]));
     if (!more) return;
     advance(next);
   }
@@ -252,7 +253,7 @@ __device__ __forceinline__ void prompt_query_warp(S& sh, const AttnParams& p, in
     const int buf = item & 1;
     if (!st::mbar_wait_warp(st::smem_u32(&sh.q_empty[buf]), (item >> 1 & 1) ^ 1, &sh.abort)) return;
     if (w == 0 && lane == 0) sh.item[buf] = it;
-#pragma unroll 3
+#pragma unroll 1
     for (int r = 8 * w + lane / 4; r < kPromptRows; r += 24) {
       const int fr = it.row0 + r, i = fr / p.group, head = it.h * p.group + fr - i * p.group;
       const bool live = fr < it.row_end;
@@ -302,7 +303,7 @@ __device__ __forceinline__ void prompt_query_warp(S& sh, const AttnParams& p, in
 template <bool MASKED>
 __device__ __forceinline__ float prompt_top(uint32_t s_cols, float factor, const float* ks, const float* lift, int end) {
   float top = -INFINITY;
-#pragma unroll 2
+#pragma unroll 1
   for (int c = 0; c < 4; ++c) {
     uint32_t raw[32];
     st::tmem_ld_32x32(s_cols + 32 * c, raw);
@@ -325,7 +326,7 @@ __device__ __forceinline__ float prompt_top(uint32_t s_cols, float factor, const
 // Weights over the scores that they are made from; returns the sum with them.
 template <bool MASKED>
 __device__ __forceinline__ float prompt_weights(uint32_t s_cols, float factor, float ref, float sum, const float* ks, const float* lift, const float* take, int end) {
-#pragma unroll 2
+#pragma unroll 1
   for (int c = 0; c < 4; ++c) {
     uint32_t raw[32], w[16];
     st::tmem_ld_32x32(s_cols + 32 * c, raw);
@@ -436,7 +437,7 @@ __device__ __forceinline__ void prompt_soft_warps(S& sh, const AttnParams& p, ui
 #pragma unroll 1
     for (int c = 0; c < D / 64; ++c) {
       const int d0 = g * (D / 2) + 32 * c;
-#pragma unroll
+#pragma unroll 1
       for (int half = 0; half < 2; ++half) {
         const int d = d0 + 16 * half;
         uint32_t o[2][16];
@@ -458,7 +459,7 @@ __device__ __forceinline__ void prompt_soft_warps(S& sh, const AttnParams& p, ui
         for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(room + 32 * lane + 4 * ((4 * half + j) ^ (lane & 7))) = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
       }
       __syncwarp();
-#pragma unroll 2
+#pragma unroll 1
       for (int k = 0; k < 8; ++k) {
         const int r = 4 * k + lane / 8, in = (threadIdx.x >> 5 & 3) * 32 + r, d = d0 + 4 * (lane & 7);
         const float4 y = *reinterpret_cast<const float4*>(room + 32 * r + 4 * ((lane & 7) ^ (r & 7)));
@@ -534,8 +535,7 @@ __global__ void __launch_bounds__(kThreadsOf<kPromptRows>, 1) paged_prompt_kerne
     else prompt_query_warp<T, D>(sh, p, warp - 17, u0, u1, f, sq);
     if (p.zero_tail && warp == 19) zero_rows<T, D>(p);
   } else if (warp >= 8) {
-    if (warp < 12) convert_warp<D, false>(sh, p, u0, u1, f, sq);
-    else convert_warp<D, true>(sh, p, u0, u1, f, sq);
+    convert_warp<D>(sh, p, warp >= 12, u0, u1, f, sq);
   } else {
     prompt_soft_warps<T, D>(sh, p, tmem, note, u1, runs, all);
     if (threadIdx.x == 0 && sh.abort) st::report_error(p.err, st::ERR_MBAR_TIMEOUT, 0x7006);
