@@ -240,9 +240,10 @@ __device__ __forceinline__ int steps_of(S& sh, uint32_t item) {
 
 // Copies keys and issues scores, two units ahead of the softmax at most.  Returns the units that it copied and those whose scores it issued.
 template <typename L, int D, int R, int QP, typename S>
-__device__ __forceinline__ uint2 score_warp(S& sh, const AttnParams& p, const CUtensorMap* map, uint32_t tmem, int u0, int u1, Found f, const Seq& sq) {
+__device__ __forceinline__ uint2 score_warp(S& sh, const AttnParams& p, const CUtensorMap* map, uint32_t tmem_, int u0, int u1, Found f, const Seq& sq) {
   Copier<L, D, R, false, S> keys(sh, p, map, u0, u1, f, sq);
-  const int lane = threadIdx.x & 31;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_, 0);
+  const bool leader = st::elect_one();
 #pragma unroll 1
   for (int i = 0; i < L::K_STAGES; ++i) keys.copy();
   uint32_t turn = 0;
@@ -257,7 +258,7 @@ __device__ __forceinline__ uint2 score_warp(S& sh, const AttnParams& p, const CU
       // the columns are free again once the softmax has written the weights of the unit before last
       if (turn > 1 && !st::mbar_wait_warp(st::smem_u32(&sh.p_full[turn & 1]), (turn - 2) >> 1 & 1, &sh.abort)) return make_uint2(keys.turn, turn);
       st::tc_fence_after();
-      if (lane == 0) {
+      if (leader) {
         const uint64_t a = tile_desc<D>(st::smem_u32(sh.k[slot]));
 #pragma unroll
         for (int j = 0; j < L::SETS; ++j) {
@@ -277,9 +278,10 @@ __device__ __forceinline__ uint2 score_warp(S& sh, const AttnParams& p, const CU
 
 // Issues the products with values; returns of how many units.
 template <typename L, int D, int R, typename S>
-__device__ __forceinline__ uint32_t value_warp(S& sh, uint32_t tmem, int u1) {
+__device__ __forceinline__ uint32_t value_warp(S& sh, uint32_t tmem_, int u1) {
   constexpr uint32_t idesc = codes_idesc(128, L::P_N, true);
-  const int lane = threadIdx.x & 31;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_, 0);
+  const bool leader = st::elect_one();
   uint32_t turn = 0;
   for (uint32_t item = 0;; ++item) {
     const int steps = steps_of<L>(sh, item);
@@ -291,7 +293,7 @@ __device__ __forceinline__ uint32_t value_warp(S& sh, uint32_t tmem, int u1) {
       if (!st::mbar_wait_warp(st::smem_u32(&sh.v_full[slot]), turn / L::V_STAGES & 1, &sh.abort)) return turn;
       if (!st::mbar_wait_warp(st::smem_u32(&sh.p_full[turn & 1]), turn >> 1 & 1, &sh.abort)) return turn;
       st::tc_fence_after();
-      if (lane == 0) {
+      if (leader) {
         // 32 rows of K (tokens, or pairs of them) at a time: 4 groups of 8
         const uint64_t a = tile_desc<128>(st::smem_u32(sh.v[slot])), b = tile_desc<L::P_WIDTH>(st::smem_u32(sh.p[turn % L::P_BUFS]), L::P_ROWS * L::P_WIDTH);
 #pragma unroll

@@ -52,7 +52,9 @@ __device__ __forceinline__ uint32_t two_halves(uint32_t codes) {
 template <int D, typename S>
 __device__ __forceinline__ void convert_warp(S& sh, const AttnParams& p, bool values, int u, int u1, Found f, Seq sq) {
   constexpr int VECS = D / 16, PER = 32 / VECS, LOADS = 32 / PER;      // 16-byte vectors of a key, keys of a load
-  const int lane = threadIdx.x & 31, first = (threadIdx.x >> 5 & 3) * 32, at = lane / VECS, vec = lane % VECS;
+  const int lane = threadIdx.x & 31, first = (threadIdx.x >> 5 & 3) * 32;
+  // eight lanes write parts of two neighbouring rows, whose swizzles keep them in different banks
+  const int vec = D == 64 ? lane & 3 : (lane & 3) | (lane >> 1 & 4), at = D == 64 ? lane >> 2 : (lane >> 2 & 1) | (lane >> 3 & 2);
   const unsigned char* codes = (values ? p.vc : p.kc) + at * D + vec * 16;
   const int mask = (1 << p.shift) - 1;
   // A unit ahead of the one that is converted its codes and scales are on their way, two ahead its page numbers.
@@ -145,18 +147,14 @@ __device__ __forceinline__ void convert_warp(S& sh, const AttnParams& p, bool va
     const bool more = next.key >= 0;
     now = next;
     look(now);
-    unsigned char* to = (values ? sh.v[g] : sh.k[g]) + vec / 4 * (128 * 128);
-    const int chunk = vec % 4 * 2, odd = D == 128 ? vec / 4 : 0;      // the second half's odd part first: other banks than the first half's even one
+    unsigned char* to = (values ? sh.v[g] : sh.k[g]) + vec / 4 * (128 * 128) + (first + at) * 128;
+    const uint32_t part = (vec % 4 * 2 ^ at) * 16;      // swizzled; at < 8
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
-      const int row = first + j * PER + at;
-      const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+      const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w}, swizzle = j * PER % 8 * 16;
       load(j);
-      uint4 h[2];
-      h[0] = make_uint4(two_halves(w[0]), two_halves(w[0] >> 16), two_halves(w[1]), two_halves(w[1] >> 16));
-      h[1] = make_uint4(two_halves(w[2]), two_halves(w[2] >> 16), two_halves(w[3]), two_halves(w[3] >> 16));
-      *reinterpret_cast<uint4*>(to + st::sw128_offset(row, chunk + odd)) = odd ? h[1] : h[0];
-      *reinterpret_cast<uint4*>(to + st::sw128_offset(row, chunk + (odd ^ 1))) = odd ? h[0] : h[1];
+      *reinterpret_cast<uint4*>(to + j * PER * 128 + (part ^ swizzle)) = make_uint4(two_halves(w[0]), two_halves(w[0] >> 16), two_halves(w[1]), two_halves(w[1] >> 16));
+      *reinterpret_cast<uint4*>(to + j * PER * 128 + (part ^ swizzle ^ 16)) = make_uint4(two_halves(w[2]), two_halves(w[2] >> 16), two_halves(w[3]), two_halves(w[3] >> 16));
     }
     st::fence_proxy_async_smem();
     st::mbar_arrive(st::smem_u32(values ? &sh.v_full[g] : &sh.k_full[g]));
@@ -169,9 +167,10 @@ __device__ __forceinline__ void convert_warp(S& sh, const AttnParams& p, bool va
 // Returns the turns whose scores and whose outputs it issued.  Scores go two turns ahead; they overwrite the weights of the turn before last, whose
 // product was issued before by the same thread.
 template <int D, typename S>
-__device__ __forceinline__ uint2 product_warp(S& sh, uint32_t tmem, int u1) {
+__device__ __forceinline__ uint2 product_warp(S& sh, uint32_t tmem_, int u1) {
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_, 0);
   constexpr uint32_t hi = st::smem_desc_hi(1024), score = half_idesc(128, false), value = half_idesc(D, true);
-  const int lane = threadIdx.x & 31;
+  const bool leader = st::elect_one();
   struct Cursor {
     uint32_t turn, item;
     int left, at;
@@ -202,7 +201,7 @@ __device__ __forceinline__ uint2 product_warp(S& sh, uint32_t tmem, int u1) {
       return;
     }
     st::tc_fence_after();
-    if (lane == 0) {
+    if (leader) {
       const uint32_t a = st::smem_desc_lo(st::smem_u32(sh.q[(s.item - 1) & 1]), 16), b = st::smem_desc_lo(st::smem_u32(sh.k[g]), 16);
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
@@ -220,7 +219,7 @@ __device__ __forceinline__ uint2 product_warp(S& sh, uint32_t tmem, int u1) {
     const int g = v.turn & 1;
     if (!st::mbar_wait_warp(st::smem_u32(&sh.v_full[g]), v.turn >> 1 & 1, &sh.abort) || !st::mbar_wait_warp(st::smem_u32(&sh.p_full[g]), v.turn >> 1 & 1, &sh.abort)) break;
     st::tc_fence_after();
-    if (lane == 0) {
+    if (leader) {
       const uint32_t b = st::smem_desc_lo(st::smem_u32(sh.v[g]), 128 * 128);
 #pragma unroll
       for (int k = 0; k < 8; ++k) st::umma_bf16_ts_split(tmem + 256 + g * D, tmem + g * 128 + k * 8, b + (k * (16 * 128) >> 4), hi, value, v.at > 1 || k > 0);
