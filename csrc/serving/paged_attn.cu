@@ -728,7 +728,7 @@ int runs_of(int rows, int dim) { return st::sm_count() * (rows == kPromptRows ? 
 
 // Whether items of sequences of up to `tokens` tokens are whole: a unit takes a block 1000 cycles, of 32 rows 2500, the second kernel and what it waits for
 // 6 us of the GPU and 4 of the host.
-bool not_split(int rows, long long tokens) { return tokens <= (rows == 32 ? 18 : 7) * kTile; }
+bool not_split(int rows, long long tokens) { return tokens <= (rows == 32 ? 18 : rows == kPromptRows ? 12 : 7) * kTile; }
 
 template <typename T, int D, int R>
 int launch_join(const AttnParams& p, cudaStream_t stream) {
