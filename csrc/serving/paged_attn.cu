@@ -22,19 +22,25 @@
 // those of O^T = V^T P^T.  The other operands, queries and weights, are fp16 numbers written as sums of e5m2 numbers, whose three
 // significant bits are those of fp16's upper byte: the byte, the byte of what it leaves, and so on; three hold bf16's 8 bits, four fp16's
 // 11.  The parts stand side by side in N; those of a score are added by its thread, those of an output when the item is done.  So the products are exact
-// and a unit costs a warp about 150 instructions instead of the 650 of mma.sync on converted codes (64 sequences: 78 us alone).
+// and a unit costs a warp about 150 instructions; with mma.sync on codes converted in registers it was 650 (64 sequences: 87 us against 71).
 // Queries are scaled by a power of two per row to use fp16's range.  The softmax runs over x + b instead of x (b: the page's value
 // exponent): the weights exp2(x + b - M) are those that multiply the codes, and the sum takes exp2(-b) back out.  M is not the running
 // maximum but some number that no x + b exceeds by more than 6: it moves, and the outputs with it, in the first unit and rarely after, and the
 // weights, times 2^9, stay below 2^15.
 //
 // Blocks: four warps for the softmax, one that copies keys (a tiled copy per page and unit) and issues scores, one that copies values, one that
-// issues the products with them, one that prepares the queries of the next item, so that a run's items follow one another without a pause: with that in the softmax warps' way an item cost them 4500 cycles more.  Heads of 64: the copies lay two tokens
-// side by side, 64 rows of 128, and the weights of even and odd tokens have columns of their own; half of each product is not used.
+// issues the products with them, one that prepares the queries of the next item, so that a run's items follow one another without a pause: with that in the
+// softmax warps' way an item cost them 4500 cycles more.  Heads of 64: the copies lay two tokens side by side, 64 rows of 128, and the weights of
+// even and odd tokens have columns of their own; half of each product is not used.
+//
+// Measured (device time in a graph, 128-wide heads if not said): 64 sequences of up to 8192 tokens, 32 heads over 8, 67 us, 5.5 TB/s of the 6.5 that a copy
+// reaches; two of up to 131001, 32 over 4, 39 us, 4.4 TB/s, of which the parts' way through the workspace and the joining take about 8; one of 777, 16 heads, 12 us: seven
+// units one after the other behind a beginning of 5000 cycles, most of it spent on instructions that have to be fetched; 12 sequences of 5 drafted tokens
+// behind up to 2049, 12 heads of 64, fp16, 19 us.
 #include "paged_prompt.cuh"
 
 namespace {
-// Warps of the softmax: with 32 rows twice as many, each of which has half of the rows (118 us against 4 on the case of parts of prompts);
+// Warps of the softmax: with 32 rows twice as many, each of which has half of the rows (4 sequences of 256 tokens: 118 us with four warps, 86 with eight);
 // then come one that copies keys and issues scores, one that issues the products with values, one that prepares queries, one that copies values.
 template <int R> constexpr int kSoftWarps = R == 32 ? 8 : 4;
 static_assert(kThreadsOf<8> == 32 * (kSoftWarps<8> + 4) && kThreadsOf<32> == 32 * (kSoftWarps<32> + 4));
@@ -718,7 +724,8 @@ __global__ void __launch_bounds__(kThreadsOf<R>, Layout<D, R, kQueryParts<T>>::B
   if (warp == SW + 1) st::tmem_dealloc(tmem, L::COLUMNS);
 }
 
-// Rows of an item, by those that the longest step of a sequence has for a key head.
+// Rows of an item, by those that the longest step of a sequence has for a key head.  Two items of 32 rows against one of 128 at 40 rows: 16 sequences at 6000
+// 118 us and 91, 64 at 1000 with heads of 64 107 and 67.
 int item_rows(long long max_queries, int group) {
   const long long rows = max_queries * group;
   return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : kPromptRows;
@@ -726,8 +733,9 @@ int item_rows(long long max_queries, int group) {
 // Blocks that run at once: two to an SM, one where the products take all columns of tensor memory.
 int runs_of(int rows, int dim) { return st::sm_count() * (rows == kPromptRows ? 1 : dim == 64 && rows == 32 ? Layout<64, 32, 4>::BLOCKS : Layout<128, 32, 4>::BLOCKS); }
 
-// Whether items of sequences of up to `tokens` tokens are whole: a unit takes a block 1000 cycles, of 32 rows 2500, the second kernel and what it waits for
-// 6 us of the GPU and 4 of the host.
+// Whether items of sequences of up to `tokens` tokens are whole: a unit takes a block 1000 cycles, of 32 rows 2500, of 128 rows 3200, the second kernel and what it
+// waits for 6 us of the GPU and 4 of the host.  One prompt of 777 tokens: 22 us split, 18 whole; 8 sequences of 128 tokens at 1024: 28 and 21; the limits are
+// where a single sequence loses no more by it than that.
 bool not_split(int rows, long long tokens) { return tokens <= (rows == 32 ? 18 : rows == kPromptRows ? 12 : 7) * kTile; }
 
 template <typename T, int D, int R>

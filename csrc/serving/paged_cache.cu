@@ -176,6 +176,8 @@ __global__ void __launch_bounds__(kPlanThreads) release_kernel(int* lengths, con
 // its first row; the largest magnitude of the group and of each head decides the scale, so every element is looked at twice: the
 // second time from registers, which hold 16 rows of 128 elements of 16 bits per warp, or from L1 where there are more rows.
 // A warp works on one group, head and tensor; where a page holds more rows than its registers, two or four warps share a group.
+// Measured: 7 prompts of up to 4096 tokens, 16 heads of 128, pages of 16, stored and read back, 94 us (the bytes: 77); a block that went through a
+// group's heads one after the other took 324.  One token of each of 96 sequences: two launches, host time.
 constexpr int kStoreThreads = 256, kStoreWarps = kStoreThreads / 32;
 constexpr int kHeld = 8;      // 16-byte loads that a thread keeps
 

@@ -3,7 +3,8 @@ and, for attention, against the formula in 64 bits.
 
 Tolerance of attention.  With p the softmax weights of a row, A = sum p |v|, S = the largest sum_d |q_d k_d| * scale and n keys:
 - scores are fp32 sums of D exact products: D 2^-24 S off at most, so a weight is that much off relatively, numerator and sum alike: 2 D 2^-24 S A;
-- weights are rounded to fp16, 2^-11 relatively, or 2^-25 of the largest below 2^-14: 2^-11 A + n 2^-25 max |v|;
+- weights are rounded to fp16 relative to a reference that is 9 below one of the row's scores and never above the largest less 9, 2^-11 relatively, and what is
+  below 2^-16 of that, 2^-25 of the largest, may be dropped: 2^-11 A + n 2^-25 max |v|;
 - exp2 and the fp32 sums of weights and of products: 2^-20 A is more than their few units in the last place per step of 16 keys, for n up to 4096;
 - the result is rounded once: half a step of the type times |o|."""
 import pytest
@@ -286,6 +287,7 @@ def test_attention_over_many_blocks_of_one_sequence():
     _check_attention([3001, 7, 4095], [3, 2, 1], 2, 3, 16, 64, torch.float16)
     _check_attention([1024] * 150, [1] * 150, 1, 1, 64, 64, torch.float16)
     _check_attention([9] * 700, [1] * 700, 1, 2, 16, 64, torch.bfloat16)                # more sequences than a block scans at once
+    _check_attention([9] * 700, [1] * 700, 1, 2, 16, 64, torch.bfloat16, max_queries=40)
 
 
 @GPU
