@@ -73,7 +73,7 @@ class GPTDecoder:
         self.free_count.copy_(step.free_count)
         resid, x = ew.embedding_forward(tokens, m.p["embed.weight"]), None
         if cfg.positional == "learned":
-            resid = resid + m.p["pos.weight"][step.positions.long()]
+            resid = resid + m.p["pos.weight"][step.positions.long().clamp_(max=cfg.seq_len - 1)]      # replays may go on behind the end
         for l in range(cfg.n_layers):
             y, h, _, _ = m._norm_fwd(resid if x is None else x, f"h{l}.norm1", residual=None if x is None else resid)
             if x is not None:

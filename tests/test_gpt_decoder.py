@@ -124,6 +124,17 @@ def test_training_with_other_rotary_forms_matches_autograd():
             assert abs((loss[0] - loss[1]) / 2e-2 - float(grad[at])) <= 2 * 4.2 * 2 ** -22 / 2e-2 + 0.01 * float(grad.abs().max())
 
 
+def test_steps_past_the_end_as_replays_do_them():
+    """Replays do not pass through the host's count: what lies beyond the last position is computed at it, not read from behind the table."""
+    model = _model(norm="layer", positional="learned")
+    d = model.decoder(1, 256)
+    d.extend([[3] * 255])
+    for _ in range(3):
+        d._admit = lambda counts: None
+        assert torch.isfinite(d.step(torch.tensor([5]))).all()
+    assert d.lengths.tolist() == [258]
+
+
 def test_refusals():
     model = _model(norm="layer", positional="learned")
     for bad in (lambda: model.decoder(0, 8), lambda: model.decoder(1, 0), lambda: model.decoder(1, 257), lambda: model.decoder(1, 8, page_size=24),
