@@ -2,8 +2,8 @@
 
 Every call is one pass of the model over the new tokens of all sequences, one after another in the rows of one matrix:
 :func:`ops.paged.plan` takes pages and maps the rows, then per layer the fused projection, rotary positions, :func:`ops.paged.store` and
-attention over the cache.  Parts of prompts that are long enough to fill the tiles of dense attention (``DENSE_FROM`` tokens) read the
-cache back instead (:func:`ops.paged.read`) and run ``ops.attention`` over it, so that a prompt sees the same keys and values that later tokens do.
+attention over the cache.  Whole prompts of ``DENSE_FROM`` tokens and more read the cache back instead (:func:`ops.paged.read`) and run ``ops.attention``
+over it, which knows that a causal prompt's first tokens see few keys; so a prompt sees the same keys and values that later tokens do.
 
 The reference has no counterpart (its language models do not decode with a cache)."""
 from __future__ import annotations
@@ -18,7 +18,8 @@ from ..ops import gemm as gemm_ops
 from ..ops import paged
 from ..ops import rotary as rotary_ops
 
-DENSE_FROM = 64      # new tokens of one sequence
+# Tokens of a whole prompt.  16 heads of 128, one prompt, us over the cache and read back: 512 tokens 29 and 52, 1024 44 and 52, 2048 80 and 57, 4096 216 and 87.
+DENSE_FROM = 1536
 
 
 class GPTDecoder:
@@ -68,6 +69,7 @@ class GPTDecoder:
         """Logits of the rows ``last`` (None: all) of ``tokens`` ``[rows]``, of which sequence ``b`` has ``counts[b]``."""
         m, cfg = self.model, self.model.cfg
         H, D, rows, most = cfg.n_heads, cfg.head_dim, tokens.shape[0], max(counts)
+        dense = all(n == 0 or DENSE_FROM <= n == held for n, held in zip(counts, self.held))      # as many queries as keys
         step = paged.plan(self.lengths, added, self.table, self.free, self.free_count, page_size=self.page_size, rows=rows)
         self.lengths.copy_(step.lengths)
         self.free_count.copy_(step.free_count)
@@ -83,8 +85,7 @@ class GPTDecoder:
             if m.rope_freq is not None:
                 rotary_ops.rotary_(q, k, step.positions, m.rope_freq, interleaved=cfg.rope_interleaved)
             paged.store(k, v, self.cache[l], step.slots)
-            o = self._dense(q, l, counts) if most >= DENSE_FROM else paged.attention(
-                q, self.cache[l], self.table, step.starts, step.lengths, max_queries=most)
+            o = self._dense(q, l, counts) if dense else paged.attention(q, self.cache[l], self.table, step.starts, step.lengths, max_queries=most)
             a = gemm_ops.gemm(o.view(rows, H * D), m.p[f"h{l}.proj.weight"])
             y, resid, _, _ = m._norm_fwd(a, f"h{l}.norm2", residual=resid)
             u = gemm_ops.gemm(y, m.p[f"h{l}.fc1.weight"], act="gelu")

@@ -312,8 +312,8 @@ def attention(q: torch.Tensor, pages: Pages, table: torch.Tensor, starts: torch.
     ``max_queries``: the most rows of one sequence; it decides the kernel's tile, not the result.  ``scale``: ``1 / sqrt(dim)`` if not given.
 
     Returns ``o`` like ``q`` (contiguous, or ``out``), with ``return_lse`` also the log-sum-exp of every row's scores, fp32 ``[rows, heads]``.  Rows behind the
-    last sequence are 0 (lse -inf); in a given ``out`` they stay as they were.  Not differentiable.  Parts of prompts of hundreds of
-    tokens run faster over :func:`read` and ``ops.attention``, which has the rows for larger tiles."""
+    last sequence are 0 (lse -inf); in a given ``out`` they stay as they were.  Not differentiable.  Whole causal
+    prompts of 1500 tokens and more run faster over :func:`read` and ``ops.attention``."""
     global launch_count
     P, Hk, page, D = _check_pages(pages)
     if q.dim() != 3 or q.shape[2] != D or q.shape[1] < Hk or q.shape[1] % Hk:

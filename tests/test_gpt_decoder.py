@@ -155,7 +155,7 @@ def test_gpu_decoder_follows_the_cpu_one(kw):
     g = torch.Generator().manual_seed(6)
     prompts = [torch.randint(0, 96, (n,), generator=g) for n in (3, 100, 17)]
     a, b = gpu.decoder(3, 256, page_size=32), cpu.decoder(3, 256, page_size=32)
-    rows = [(a.extend(prompts), b.extend(prompts))]              # 100 tokens: the dense path
+    rows = [(a.extend(prompts), b.extend(prompts))]
     rows.append((a.extend([p[:9] for p in prompts]), b.extend([p[:9] for p in prompts])))
     for _ in range(3):
         t = torch.randint(0, 96, (3,), generator=g)
@@ -163,6 +163,24 @@ def test_gpu_decoder_follows_the_cpu_one(kw):
     for x, y in rows:
         # bf16 activations through two layers: 2^-8 a rounding, about ten of them in a row, and codes that fall to their neighbours (2^-4)
         assert torch.nn.functional.cosine_similarity(x.float().cpu(), y, dim=-1).min() > 0.99
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dense_from", [1, 80, 1536])
+def test_gpu_parts_of_prompts_and_whole_ones(dense_from, monkeypatch):
+    """Prompts read back and not, and long parts behind what the cache holds, which never are."""
+    from spiraltorch_b200.models import gpt_decoder
+    gpu = _model("cuda", torch.bfloat16)
+    cpu = _model()
+    cpu.flat_w.copy_(gpu.flat_w.float().cpu())
+    g = torch.Generator().manual_seed(7)
+    a, b = gpu.decoder(2, 256, page_size=16), cpu.decoder(2, 256, page_size=16)
+    for parts in ((80, 90), (100, 70), (1, 65), (70, 0)):
+        ids = [torch.randint(0, 96, (n,), generator=g) for n in parts]
+        monkeypatch.setattr(gpt_decoder, "DENSE_FROM", dense_from)
+        x = a.extend(ids)
+        monkeypatch.setattr(gpt_decoder, "DENSE_FROM", 1 << 30)
+        assert torch.nn.functional.cosine_similarity(x.float().cpu(), b.extend(ids), dim=-1).min() > 0.99
 
 
 @pytest.mark.gpu
