@@ -437,14 +437,16 @@ __device__ __forceinline__ void prompt_soft_warps(S& sh, const AttnParams& p, ui
     const int head = it.h * p.group + fr - query * p.group, lane = threadIdx.x & 31;
     const long long place = (it.start + query) * p.o_row + head * p.o_head;
     const bool check = sh.some_bad[item & 3] != 0;
-    // 32 columns at a time through the room of the item's queries, which no product reads now: a warp's own 4 KB of it, four rows to a store
-    float* room = reinterpret_cast<float*>(sh.q[item & 1]) + (threadIdx.x >> 5) * 1024;
+    // a quarter of the columns at a time through the room of the item's queries, which no product reads now: a warp's own eighth of it, whole rows to a store
+    constexpr int WIDE = D / 4, LANES = WIDE / 4;      // columns, lanes of a row
+    static_assert(8 * 32 * WIDE * sizeof(float) == S::TILE);
+    float* room = reinterpret_cast<float*>(sh.q[item & 1]) + (threadIdx.x >> 5) * (32 * WIDE);
 #pragma unroll 1
-    for (int c = 0; c < D / 64; ++c) {
-      const int d0 = g * (D / 2) + 32 * c;
+    for (int c = 0; c < 2; ++c) {
+      const int d0 = g * (D / 2) + WIDE * c;
 #pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
-        const int d = d0 + 16 * half;
+      for (int part16 = 0; part16 < WIDE / 16; ++part16) {
+        const int d = d0 + 16 * part16;
         uint32_t o[2][16];
 #pragma unroll
         for (int k = 0; k < 2; ++k)
@@ -461,13 +463,14 @@ __device__ __forceinline__ void prompt_soft_warps(S& sh, const AttnParams& p, ui
           for (int j = 0; j < 16; ++j)
             if (row >= sh.bad[item & 3][d + j]) y[j] = NAN;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(room + 32 * lane + 4 * ((4 * half + j) ^ (lane & 7))) = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<float4*>(room + WIDE * lane + 4 * ((4 * part16 + j) ^ (lane & (LANES - 1)))) = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
       }
       __syncwarp();
 #pragma unroll 1
-      for (int k = 0; k < 8; ++k) {
-        const int r = 4 * k + lane / 8, in = (threadIdx.x >> 5 & 3) * 32 + r, d = d0 + 4 * (lane & 7);
-        const float4 y = *reinterpret_cast<const float4*>(room + 32 * r + 4 * ((lane & 7) ^ (r & 7)));
+      for (int k = 0; k < LANES; ++k) {
+        const int r = 32 / LANES * k + lane / LANES, at = lane & (LANES - 1), in = (threadIdx.x >> 5 & 3) * 32 + r, d = d0 + 4 * at;
+        const float4 y = *reinterpret_cast<const float4*>(room + WIDE * r + 4 * (at ^ (r & (LANES - 1))));
         const long long to = __shfl_sync(0xffffffffu, place, r);
         if (in >= rows) continue;
         if (!whole) {

@@ -374,6 +374,15 @@ def test_attention_of_parts_of_prompts(D, H, G, page, dtype, causal):
 
 
 @GPU
+@pytest.mark.parametrize("D,dtype,page", [(64, torch.bfloat16, 16), (128, torch.bfloat16, 64), (64, torch.float16, 64), (128, torch.float16, 16)])
+def test_attention_of_many_items_to_a_block(D, dtype, page):
+    """Hundreds of items of one unit, two, three, four, in whole and shared ones."""
+    lengths, added = [20 + 37 * (b % 13) for b in range(200)], [18 + b % 3 for b in range(200)]
+    _check_attention(lengths, added, 2, 2, page, D, dtype, seed=D)
+    _check_attention(lengths[:60] + [1700], added[:60] + [150], 4, 3, page, D, dtype, seed=D)
+
+
+@GPU
 def test_attention_of_parts_of_prompts_with_numbers_that_are_none():
     def values(pages, table, fused):       # hidden from the rows before them
         pages.v.view(torch.uint8)[table[0, 20], 0, 1, 5] = 0xFF
