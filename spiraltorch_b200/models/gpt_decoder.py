@@ -18,8 +18,8 @@ from ..ops import gemm as gemm_ops
 from ..ops import paged
 from ..ops import rotary as rotary_ops
 
-# Tokens of a whole prompt.  16 heads of 128, one prompt, us over the cache and read back: 512 tokens 29 and 52, 1024 44 and 52, 2048 80 and 57, 4096 216 and 87.
-DENSE_FROM = 1536
+# Tokens of a whole prompt.  16 heads of 128, one prompt, us over the cache and read back: 512 tokens 28 and 52, 1024 44 and 52, 2048 71 and 57 to 70, 4096 165 and 87.
+DENSE_FROM = 2048
 
 
 class GPTDecoder:

@@ -313,7 +313,7 @@ def attention(q: torch.Tensor, pages: Pages, table: torch.Tensor, starts: torch.
 
     Returns ``o`` like ``q`` (contiguous, or ``out``), with ``return_lse`` also the log-sum-exp of every row's scores, fp32 ``[rows, heads]``.  Rows behind the
     last sequence are 0 (lse -inf); in a given ``out`` they stay as they were.  Not differentiable.  Whole causal
-    prompts of 1500 tokens and more run faster over :func:`read` and ``ops.attention``."""
+    prompts of 2000 tokens and more run faster over :func:`read` and ``ops.attention``."""
     global launch_count
     P, Hk, page, D = _check_pages(pages)
     if q.dim() != 3 or q.shape[2] != D or q.shape[1] < Hk or q.shape[1] % Hk:

@@ -166,7 +166,7 @@ def test_gpu_decoder_follows_the_cpu_one(kw):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dense_from", [1, 80, 1536])
+@pytest.mark.parametrize("dense_from", [1, 80, 2048])
 def test_gpu_parts_of_prompts_and_whole_ones(dense_from, monkeypatch):
     """Prompts read back and not, and long parts behind what the cache holds, which never are."""
     from spiraltorch_b200.models import gpt_decoder
