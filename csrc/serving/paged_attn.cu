@@ -118,7 +118,7 @@ struct Layout {
   static constexpr int Q_BYTES = QP * R * D;
   // What fits the shared memory of two blocks (111 KB each, 2 KB of them for the small things): queries twice before a third stage of values, that
   // before weights twice, and a third one of keys last.
-  static constexpr int ROOM = (BLOCKS == 2 ? 113 * 1024 : 226 * 1024) - 3072, ONE = kTile * D;
+  static constexpr int ROOM = (BLOCKS == 2 ? 113 * 1024 : 226 * 1024) - 3 * 1024, ONE = kTile * D;
   static constexpr int Q_BUFS = (D == 64 ? 4 : 2) * 2 * ONE + P_BYTES + 2 * Q_BYTES <= ROOM ? 2 : 1;
   static constexpr int P_BUFS = (D == 64 ? 4 : 2) * 2 * ONE + 2 * P_BYTES + Q_BUFS * Q_BYTES <= ROOM ? 2 : 1;
   static constexpr int V_STAGES = D == 64 ? 4 : 5 * ONE + P_BUFS * P_BYTES + Q_BUFS * Q_BYTES <= ROOM ? 3 : 2;

@@ -12,11 +12,11 @@
 // by the scale's sign, so f >= 0 and a page's largest x comes from its largest score), weights exp2(x - reference) below 2^15, the reference behind the
 // maximum by 9 at first and 15 at most, and the sum takes exp2(-b) back out per 16 keys.
 //
-// Measured: 4 sequences of 256 tokens behind up to 4000, 16 heads over 4 of 128: 40 us, where two products' operations take 6.  A unit takes a block 3200 cycles:
+// Measured: 4 sequences of 256 tokens behind up to 4000, 16 heads over 4 of 128: 41 us, where two products' operations take 6.  A unit takes a block 3200 cycles:
 // a group's scores, weights and outputs follow one another (1000 for the maximum, 2500 for the weights, 400 until the last warp is there, 1900 for the two
 // products), and two groups are what tensor memory has room for.  Before: items of 32 rows on codes 87, this with masks in the same code as the rest 77.  Tried without
 // gain: maximum and weights in one pass with corrections behind it (46), halves of 64 keys, which need half as many product instructions more (48), more of the
-// loops unrolled (48 to 58): instructions come from a cache that the block's kinds of warps share.  A beginning takes 11000 cycles for the same reason.
+// loops unrolled (48 to 58): instructions come from a cache that the block's kinds of warps share (waiting for them took 4.2 of 17 cycles an instruction at 58 us, 1.0 of 13 now).  A beginning takes 11000 cycles for the same reason.
 #pragma once
 #include "paged_work.cuh"
 
@@ -418,13 +418,12 @@ __device__ __forceinline__ void prompt_soft_warps(S& sh, const AttnParams& p, ui
 
     // both groups' outputs, half of the columns each
     sh.stat[g][row] = make_float2(ref, sum);
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int last = steps - 1 - ((first + steps - 1 ^ c) & 1);      // the last unit of group c
-      if (last >= 0) st::mbar_wait_warp(st::smem_u32(&sh.pv_done[c]), (first + last) >> 1 & 1, &sh.abort);
-    }
-    st::tc_fence_after();
+    // A group waits for its own last unit and the barrier does the rest: another's parity may stand two turns back, where a wait would not hold.
+    const int last = steps - 1 - ((first + steps - 1 ^ g) & 1);
+    if (last >= 0) st::mbar_wait_warp(st::smem_u32(&sh.pv_done[g]), (first + last) >> 1 & 1, &sh.abort);
+    st::tc_fence_before();
     soft_sync<256>();
+    st::tc_fence_after();
     const float2 other = sh.stat[g ^ 1][row];
     const float m = fmaxf(ref, other.x);
     const float w_own = st::exp2_ftz(ref - m), w_other = st::exp2_ftz(other.x - m);

@@ -312,7 +312,7 @@ def attention(q: torch.Tensor, pages: Pages, table: torch.Tensor, starts: torch.
     ``max_queries``: the most rows of one sequence; it decides the kernel's tile, not the result.  ``scale``: ``1 / sqrt(dim)`` if not given.
 
     Returns ``o`` like ``q`` (contiguous, or ``out``), with ``return_lse`` also the log-sum-exp of every row's scores, fp32 ``[rows, heads]``.  Rows behind the
-    last sequence are 0 (lse -inf); in a given ``out`` they stay as they were.  Not differentiable.  Whole causal
+    last sequence are 0 (lse -inf); in a given ``out``, which may be ``q`` itself, they stay as they were.  Not differentiable.  Whole causal
     prompts of 2000 tokens and more run faster over :func:`read` and ``ops.attention``."""
     global launch_count
     P, Hk, page, D = _check_pages(pages)

@@ -492,6 +492,52 @@ def test_attention_repeats_its_bits_and_keeps_streams_apart():
 
 
 @GPU
+@pytest.mark.parametrize("D,G,n", [(128, 4, 1), (64, 3, 5), (128, 4, 8), (64, 8, 20), (128, 2, 70)])
+def test_attention_of_rows_at_odd_places_and_in_place(D, G, n):
+    """Rows, heads and results off a 16-byte boundary, and results over the queries: the same bits."""
+    lengths, H, page = [1700, 3000], 2, 64
+    pages, table = _cache(lengths, H, page, D, 8)
+    dev, table = P.Pages(*(t.cuda() for t in pages)), table.cuda()
+    starts, ln = torch.tensor([0, n, 2 * n], dtype=torch.int32, device="cuda"), torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    q = torch.randn(2 * n + 1, H * G, D, device="cuda").half()
+    want = P.attention(q, dev, table, starts, ln, max_queries=n)
+    room = torch.zeros(2, 2 * n + 1, H * G, D + 1, device="cuda").half()
+    odd, out = room[0, ..., 1:], room[1, ..., 1:]
+    odd.copy_(q)
+    assert torch.equal(P.attention(odd, dev, table, starts, ln, max_queries=n), want)
+    P.attention(q, dev, table, starts, ln, max_queries=n, out=out)
+    assert torch.equal(out[:2 * n], want[:2 * n]) and (room[1, ..., 0] == 0).all() and (out[2 * n:] == 0).all()
+    P.attention(odd, dev, table, starts, ln, max_queries=n, out=odd)
+    assert torch.equal(odd[:2 * n], want[:2 * n]) and torch.equal(odd[2 * n:], q[2 * n:])
+
+
+@GPU
+@pytest.mark.parametrize("lengths", [[700, 90, 1100], [700, 2500, 4000]])
+def test_attention_of_parts_of_prompts_on_two_streams_and_captured(lengths):
+    n, H, G, D, page = 60, 2, 2, 128, 64
+    pages, table = _cache(lengths, H, page, D, 9)
+    dev, table = P.Pages(*(t.cuda() for t in pages)), table.cuda()
+    starts, ln = torch.arange(4, dtype=torch.int32, device="cuda") * n, torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    qs = [torch.randn(3 * n, H * G, D, device="cuda").bfloat16() for _ in range(2)]
+    call = lambda i: P.attention(qs[i], dev, table, starts, ln, max_queries=n)                   # noqa: E731
+    want = [call(0), call(1)]
+    torch.cuda.synchronize()
+    streams, graphs, got, outs = [torch.cuda.Stream(), torch.cuda.Stream()], [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], [[], []], []
+    for i, graph in enumerate(graphs):
+        with torch.cuda.graph(graph):
+            outs.append(call(i))
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call(i))
+                graphs[i].replay()
+                got[i].append(outs[i].clone())
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+@GPU
 def test_pages_that_are_none_are_refused_by_the_kernels():
     from spiraltorch_b200.ops import native
     pages = P.Pages(*(t.zero_() for t in P.Pages.allocate(3, 1, 16, 64)))
