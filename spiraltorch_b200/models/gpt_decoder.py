@@ -25,7 +25,8 @@ DENSE_FROM = 2048
 class GPTDecoder:
     """``sequences`` places for sequences of up to ``max_length`` tokens over ``pages`` pages (default: enough for all of them).
 
-    The lengths are kept on the host as well, so that a call that does not fit is refused before anything is launched."""
+    The lengths are kept on the host as well (``held``), so that a call that does not fit is refused before anything is launched.  Replays of a captured
+    :meth:`step` do not pass through them: once a step has been captured, every other call first takes them from the device (:meth:`sync`)."""
 
     def __init__(self, model, sequences: int, max_length: int, *, pages: Optional[int] = None, page_size: int = 64):
         cfg = model.cfg
@@ -46,6 +47,12 @@ class GPTDecoder:
         self.free_count = torch.full((1,), self.pages, **i32)
         self.lengths = torch.zeros(sequences, **i32)
         self.held = [0] * sequences
+        self._left = self.pages
+        self._lost = [False] * sequences        # replays found no page for some of its tokens
+        self._waiting = [False] * sequences     # released, and not extended since: steps pass it over
+        self._taking = torch.ones(sequences, **i32)      # the same on the device: tokens that a step adds
+        self._places = torch.arange(sequences + 1, **i32)
+        self._captured = False
 
     # ---- host side ------------------------------------------------------------------------------------------------------------
     def _blocks(self, tokens: int) -> int:
@@ -53,26 +60,61 @@ class GPTDecoder:
 
     @property
     def pages_left(self) -> int:
-        return self.pages - sum(self._blocks(n) for n in self.held)
+        self._settle()
+        return self._left
+
+    def sync(self) -> None:
+        """Takes ``held`` and the free pages from the device, which replays have moved on (waits for it)."""
+        block = torch.arange(self.table.shape[1], dtype=torch.int32, device=self.table.device)
+        lost = ((self.table < 0) & (block < ((self.lengths + (self.page_size - 1)) // self.page_size)[:, None])).any(1)
+        state = torch.cat([self.lengths, lost.int(), self.free_count]).tolist()
+        n = self.sequences
+        self.held, self._lost, self._left = state[:n], [x > 0 for x in state[n:2 * n]], max(state[-1], 0)
+
+    def _capturing(self) -> bool:
+        return self.lengths.is_cuda and torch.cuda.is_current_stream_capturing()
+
+    def _settle(self) -> None:
+        if self._captured and not self._capturing():
+            self.sync()
+
+    def _need(self, added: Sequence[int]) -> int:
+        return sum(self._blocks(h + n) - self._blocks(h) for h, n in zip(self.held, added))
 
     def _admit(self, added: Sequence[int]) -> None:
-        need = sum(self._blocks(h + n) - self._blocks(h) for h, n in zip(self.held, added))
+        """Refuses what does not fit."""
         for b, (h, n) in enumerate(zip(self.held, added)):
+            if n and self._lost[b]:
+                raise ValueError(f"GPTDecoder: place {b} lost tokens to replays that found no page; it must be released")
             if h + n > self.max_length:
                 raise ValueError(f"GPTDecoder: sequence {b} would have {h + n} tokens, at most {self.max_length}")
-        if need > self.pages_left:
-            raise ValueError(f"GPTDecoder: {need} pages are needed and {self.pages_left} are left")
+        if (need := self._need(added)) > self._left:
+            raise ValueError(f"GPTDecoder: {need} pages are needed and {self._left} are left")
+
+    def _commit(self, added: Sequence[int]) -> None:
+        self._left -= self._need(added)
         self.held = [h + n for h, n in zip(self.held, added)]
 
+    def _wait(self, waiting: list) -> None:
+        if waiting != self._waiting:
+            self._taking.copy_(torch.tensor([int(not w) for w in waiting], dtype=torch.int32))
+            self._waiting = waiting
+
     # ---- device side ----------------------------------------------------------------------------------------------------------
-    def _pass(self, tokens: torch.Tensor, added: torch.Tensor, last: Optional[torch.Tensor], counts: Sequence[int]) -> torch.Tensor:
-        """Logits of the rows ``last`` (None: all) of ``tokens`` ``[rows]``, of which sequence ``b`` has ``counts[b]``."""
+    def _pass(self, tokens: torch.Tensor, added: torch.Tensor, last: Optional[torch.Tensor], counts: Sequence[int], by_place: bool = False) -> torch.Tensor:
+        """Logits of the rows ``last`` (None: all) of ``tokens`` ``[rows]``, of which sequence ``b`` has ``counts[b]``.  ``by_place``: row ``b`` is that of
+        place ``b``, whether it takes its token (``added``) or waits; the logits of those that wait are 0."""
         m, cfg = self.model, self.model.cfg
         H, D, rows, most = cfg.n_heads, cfg.head_dim, tokens.shape[0], max(counts)
-        dense = all(n == 0 or DENSE_FROM <= n == held for n, held in zip(counts, self.held))      # as many queries as keys
+        dense = last is not None and all(n == 0 or DENSE_FROM <= n == held for n, held in zip(counts, self.held))      # as many queries as keys
         step = paged.plan(self.lengths, added, self.table, self.free, self.free_count, page_size=self.page_size, rows=rows)
         self.lengths.copy_(step.lengths)
         self.free_count.copy_(step.free_count)
+        waits = None
+        if by_place:      # the plan maps the tokens that are added, one after another; a place that waits has no keys, so its row of attention is 0
+            at, waits = step.starts[:-1], (added == 0)[:, None]
+            step = step._replace(starts=self._places, positions=step.positions.index_select(0, at),
+                                 slots=step.slots.index_select(0, at).masked_fill_(waits[:, 0], -1))
         resid, x = ew.embedding_forward(tokens, m.p["embed.weight"]), None
         if cfg.positional == "learned":
             resid = resid + m.p["pos.weight"][step.positions.long().clamp_(max=cfg.seq_len - 1)]      # replays may go on behind the end
@@ -93,13 +135,15 @@ class GPTDecoder:
         if last is not None:
             x, resid = x.index_select(0, last), resid.index_select(0, last)
         y, _, _, _ = m._norm_fwd(x, "norm_f", residual=resid)
+        if waits is not None:
+            y = y.masked_fill(waits, 0.0)
         return gemm_ops.gemm(y, m.p["embed.weight"])
 
     def _dense(self, q: torch.Tensor, l: int, counts: Sequence[int]) -> torch.Tensor:
         o, r = torch.empty(q.shape, dtype=q.dtype, device=q.device), 0
         for b, n in enumerate(counts):
             if n:
-                k, v = paged.read(self.cache[l], self.table[b:b + 1], self.lengths[b:b + 1], self.held[b],
+                k, v = paged.read(self.cache[l], self.table[b:b + 1], self.lengths[b:b + 1], n,
                                   torch.bfloat16 if q.is_cuda else torch.float32)
                 o[r:r + n] = attn_ops.attention_forward(q[None, r:r + n], k, v, True)[0][0]
                 r += n
@@ -119,35 +163,58 @@ class GPTDecoder:
             raise ValueError(f"GPTDecoder: a token id is outside the vocabulary of {vocab}")
         if not flat.numel():
             raise ValueError("GPTDecoder: no tokens")
+        if self._capturing():
+            raise ValueError("GPTDecoder: extend takes tokens from the host and cannot be captured; step can")
+        self._settle()
         self._admit(counts)
         dev = self.lengths.device
         last = torch.tensor([sum(counts[:b + 1]) - 1 for b, n in enumerate(counts) if n])
-        return self._pass(flat.to(dev), torch.tensor(counts, dtype=torch.int32, device=dev), last.to(dev), counts)
+        self._commit(counts)
+        logits = self._pass(flat.to(dev), torch.tensor(counts, dtype=torch.int32, device=dev), last.to(dev), counts)
+        self._wait([w and not n for w, n in zip(self._waiting, counts)])
+        return logits
 
     @torch.no_grad()
     def step(self, tokens: torch.Tensor) -> torch.Tensor:
-        """One token for every sequence: ``tokens`` int64 ``[sequences]`` on the model's device, ids inside the vocabulary (not looked at).
-        Returns the logits behind them.  It looks at nothing on the device, so it can be captured into a CUDA graph; replays do not pass
-        through the host's count, and what they append beyond ``max_length`` or the pages is not stored."""
+        """One token for every place: ``tokens`` int64 ``[sequences]`` on the model's device, ids inside the vocabulary (not looked at).
+        Returns the logits behind them.  A place that was released waits until :meth:`extend` gives it a new sequence: it takes neither its token nor a
+        page, and its logits are 0.
+
+        The call looks at nothing on the device, so it can be captured into a CUDA graph (which appends nothing by itself).  Replays
+        follow what :meth:`extend` and :meth:`release` do between them, but no host stands before them: what they append behind a place's last page, or
+        when no page is left, is not stored.  Other calls refuse such a place until it is released."""
         if tokens.shape != (self.sequences,) or tokens.dtype != torch.int64 or tokens.device != self.lengths.device:
             raise ValueError(f"GPTDecoder: step takes int64 [{self.sequences}] on {self.lengths.device}, got {tokens.dtype} {tuple(tokens.shape)} on {tokens.device}")
-        counts = [1] * self.sequences
+        if self._capturing():
+            self._captured = True
+            return self._pass(tokens, self._taking, None, [1] * self.sequences, True)
+        self._settle()
+        counts = [int(not w) for w in self._waiting]
+        if not any(counts):
+            raise ValueError("GPTDecoder: every place was released; extend begins a sequence")
         self._admit(counts)
-        return self._pass(tokens, torch.ones(self.sequences, dtype=torch.int32, device=tokens.device), None, counts)
+        self._commit(counts)
+        return self._pass(tokens, self._taking, None, counts, any(self._waiting))
 
     def release(self, which: Sequence[int]) -> None:
-        """Ends the sequences of these places and frees their pages; the places can take new ones."""
+        """Ends the sequences of these places and frees their pages; the places wait until :meth:`extend` gives them new ones."""
+        if self._capturing():
+            raise ValueError("GPTDecoder: release takes places from the host and cannot be captured")
         done = [False] * self.sequences
         for b in which:
             if not 0 <= b < self.sequences:
                 raise ValueError(f"GPTDecoder: no place {b}")
             done[b] = True
         paged.release(self.lengths, torch.tensor(done, device=self.lengths.device), self.table, self.free, self.free_count, page_size=self.page_size)
+        self._left += sum(self._blocks(h) for h, d in zip(self.held, done) if d)
         self.held = [0 if d else h for h, d in zip(self.held, done)]
+        self._lost = [x and not d for x, d in zip(self._lost, done)]
+        self._wait([w or d for w, d in zip(self._waiting, done)])
 
     def generate(self, prompts: Sequence, max_new_tokens: int, *, stop: Optional[int] = None) -> list:
         """The likeliest continuation of a prompt in every place, up to ``max_new_tokens`` or the token ``stop`` (which is not returned).
         A place that met ``stop`` waits.  Starts from empty places."""
+        self._settle()
         if any(self.held):
             raise ValueError("GPTDecoder: generate starts from empty places; release them first")
         if max_new_tokens < 0 or any(len(p) == 0 for p in prompts):

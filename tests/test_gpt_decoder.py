@@ -135,6 +135,73 @@ def test_steps_past_the_end_as_replays_do_them():
     assert d.lengths.tolist() == [258]
 
 
+def _replay(d, tokens):
+    """What the replay of a captured step does: the device's part of it, past the host's count."""
+    held, admit = list(d.held), d._admit
+    d._admit, d._capturing = lambda counts: None, lambda: True
+    row = d.step(tokens)
+    d._admit, d.held = admit, held
+    del d._capturing
+    return row
+
+
+def test_calls_behind_replays_go_by_what_the_device_holds():
+    model = _model()
+    d, e = model.decoder(2, 64, pages=6, page_size=16), model.decoder(2, 64, pages=6, page_size=16)
+    for x in (d, e):
+        x.extend([[7] * 10, [8] * 10])
+    for t in range(20):
+        tokens = torch.tensor([t, 90 - t])
+        assert torch.equal(_replay(d, tokens), e.step(tokens))
+    assert d.pages_left == e.pages_left == 2 and d.held == e.held == [30, 30]
+    with pytest.raises(ValueError, match="2 are left"):
+        d.extend([[3] * 20, [1] * 20])
+    for x in (d, e):
+        x.release([1])
+    assert d.pages_left == e.pages_left == 4
+    for t in range(4):            # a released place waits: it takes neither tokens nor pages
+        row, tokens = _replay(d, torch.tensor([t, 5])), torch.tensor([t, 6])
+        assert torch.equal(row, e.step(tokens)) and (row[1] == 0).all() and (row[0] != 0).any()
+    assert d.lengths.tolist() == [34, 0] and d.pages_left == 3 == int(d.free_count)
+    with pytest.raises(ValueError, match="pages"):
+        d.extend([[], [2] * 49])
+    again = d.extend([[], list(range(40))])[0]
+    assert torch.equal(again, model.decoder(1, 64, page_size=16).extend([list(range(40))])[0])
+    assert d.held == [34, 40] and d.pages_left == 0 == int(d.free_count)
+    e.extend([[], list(range(40))])
+    row = d.step(torch.tensor([3, 4]))
+    assert torch.equal(row, e.step(torch.tensor([3, 4]))) and (row[1] != 0).any() and d.held == [35, 41] == d.lengths.tolist()
+
+
+def test_released_places_wait_in_steps():
+    model = _model()
+    d, e = model.decoder(3, 64, page_size=16), model.decoder(3, 64, page_size=16)
+    for x in (d, e):
+        x.extend([[1, 2], [3], [4, 5, 6]])
+    d.release([1])
+    for t in range(3):
+        a, b = d.step(torch.tensor([t, 9, t + 1])), e.step(torch.tensor([t, 9, t + 1]))
+        assert torch.equal(a[[0, 2]], b[[0, 2]]) and (a[1] == 0).all()
+    assert d.held == [5, 0, 6] == d.lengths.tolist() and d.pages_left == 10
+    d.release([0, 2])
+    with pytest.raises(ValueError, match="released"):
+        d.step(torch.tensor([1, 1, 1]))
+    assert torch.equal(d.extend([[], [3], []])[0], model.decoder(1, 64, page_size=16).extend([[3]])[0])
+
+
+def test_a_prompt_behind_a_replayed_token_sees_its_own_keys(monkeypatch):
+    from spiraltorch_b200.models import gpt_decoder
+    model = _model()
+    prompt, rows = list(range(50, 80)), []
+    for dense_from in (20, 1 << 30):
+        monkeypatch.setattr(gpt_decoder, "DENSE_FROM", dense_from)
+        d = model.decoder(1, 64, page_size=16)
+        _replay(d, torch.tensor([3]))
+        rows.append(d.extend([prompt])[0])
+    # the same keys, values and products in another order at most
+    assert torch.allclose(*rows, atol=1e-5)
+
+
 def test_refusals():
     model = _model(norm="layer", positional="learned")
     for bad in (lambda: model.decoder(0, 8), lambda: model.decoder(1, 0), lambda: model.decoder(1, 257), lambda: model.decoder(1, 8, page_size=24),
@@ -202,3 +269,64 @@ def test_gpu_step_captured():
         tokens.copy_(torch.tensor([i, 95 - i]))
         graph.replay()
         assert torch.equal(out, e.step(tokens))
+
+
+@pytest.mark.gpu
+def test_gpu_calls_behind_replays():
+    """Replays, a release between them and prompts behind them, against the same in eager calls: the same bits."""
+    model = _model("cuda", torch.bfloat16)
+    d, e = (model.decoder(3, 200, pages=30, page_size=16) for _ in range(2))
+    tokens = torch.tensor([3, 5, 7], device="cuda")
+    for x in (d, e):
+        x.extend([[1, 2, 3], [4], [5] * 20])
+        x.step(tokens)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = d.step(tokens)
+    assert d.held == [4, 2, 21]              # the capture itself appends nothing
+
+    def turns(n):
+        for i in range(n):
+            tokens.copy_(torch.tensor([i, 95 - i, 2 * i]))
+            graph.replay()
+            assert torch.equal(out, e.step(tokens))
+    turns(20)
+    for x in (d, e):
+        x.release([1])
+    turns(17)
+    assert (out[1] == 0).all() and d.pages_left == e.pages_left == int(d.free_count) and d.held == e.held == [41, 0, 58]
+    prompt = list(range(40))
+    assert torch.equal(d.extend([[9], prompt, []]), e.extend([[9], prompt, []]))
+    turns(5)
+    assert torch.equal(d.step(tokens), e.step(tokens)) and d.held == e.held == [48, 46, 64] == d.lengths.tolist()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()), pytest.raises(ValueError, match="captured"):
+        d.extend([[9], [], []])
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_gpu_replays_without_pages():
+    """A place whose tokens found no page is refused until it is released; the others go on."""
+    from spiraltorch_b200.ops import native
+    model = _model("cuda", torch.bfloat16)
+    d, e = model.decoder(2, 64, pages=3, page_size=16), model.decoder(2, 64, page_size=16)
+    tokens = torch.tensor([3, 5], device="cuda")
+    for x in (d, e):
+        x.extend([[1] * 15, [2] * 15])
+        x.step(tokens)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        d.step(tokens)
+    graph.replay()                           # one page, two places that need one: the first gets it
+    e.step(tokens)
+    torch.cuda.synchronize()
+    assert native.read_error_word()[0] == 3 and d.pages_left == 0
+    with pytest.raises(ValueError, match="place 1 .* released"):
+        d.step(tokens)
+    for x in (d, e):
+        x.release([1])
+    assert d.pages_left == 1
+    assert torch.equal(d.step(tokens), e.step(tokens)) and d.held == [18, 0]
+    assert torch.equal(d.extend([[], [7] * 9])[0], model.decoder(1, 64, page_size=16).extend([[7] * 9])[0])
