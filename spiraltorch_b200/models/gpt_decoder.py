@@ -106,10 +106,8 @@ class GPTDecoder:
         place ``b``, whether it takes its token (``added``) or waits; the logits of those that wait are 0."""
         m, cfg = self.model, self.model.cfg
         H, D, rows, most = cfg.n_heads, cfg.head_dim, tokens.shape[0], max(counts)
-        dense = last is not None and all(n == 0 or DENSE_FROM <= n == held for n, held in zip(counts, self.held))      # as many queries as keys
+        dense = last is not None and all(n == 0 or DENSE_FROM <= n and held == 0 for n, held in zip(counts, self.held))      # as many queries as keys
         step = paged.plan(self.lengths, added, self.table, self.free, self.free_count, page_size=self.page_size, rows=rows)
-        self.lengths.copy_(step.lengths)
-        self.free_count.copy_(step.free_count)
         waits = None
         if by_place:      # the plan maps the tokens that are added, one after another; a place that waits has no keys, so its row of attention is 0
             at, waits = step.starts[:-1], (added == 0)[:, None]
@@ -127,7 +125,7 @@ class GPTDecoder:
             if m.rope_freq is not None:
                 rotary_ops.rotary_(q, k, step.positions, m.rope_freq, interleaved=cfg.rope_interleaved)
             paged.store(k, v, self.cache[l], step.slots)
-            o = self._dense(q, l, counts) if dense else paged.attention(q, self.cache[l], self.table, step.starts, step.lengths, max_queries=most)
+            o = self._dense(q, l, counts, step.lengths) if dense else paged.attention(q, self.cache[l], self.table, step.starts, step.lengths, max_queries=most)
             a = gemm_ops.gemm(o.view(rows, H * D), m.p[f"h{l}.proj.weight"])
             y, resid, _, _ = m._norm_fwd(a, f"h{l}.norm2", residual=resid)
             u = gemm_ops.gemm(y, m.p[f"h{l}.fc1.weight"], act="gelu")
@@ -137,13 +135,17 @@ class GPTDecoder:
         y, _, _, _ = m._norm_fwd(x, "norm_f", residual=resid)
         if waits is not None:
             y = y.masked_fill(waits, 0.0)
-        return gemm_ops.gemm(y, m.p["embed.weight"])
+        logits = gemm_ops.gemm(y, m.p["embed.weight"])
+        # only now does the step take effect: a call that failed before appended nothing, and what it wrote to the table and the pages is written anew
+        self.lengths.copy_(step.lengths)
+        self.free_count.copy_(step.free_count)
+        return logits
 
-    def _dense(self, q: torch.Tensor, l: int, counts: Sequence[int]) -> torch.Tensor:
+    def _dense(self, q: torch.Tensor, l: int, counts: Sequence[int], lengths: torch.Tensor) -> torch.Tensor:
         o, r = torch.empty(q.shape, dtype=q.dtype, device=q.device), 0
         for b, n in enumerate(counts):
             if n:
-                k, v = paged.read(self.cache[l], self.table[b:b + 1], self.lengths[b:b + 1], n,
+                k, v = paged.read(self.cache[l], self.table[b:b + 1], lengths[b:b + 1], n,
                                   torch.bfloat16 if q.is_cuda else torch.float32)
                 o[r:r + n] = attn_ops.attention_forward(q[None, r:r + n], k, v, True)[0][0]
                 r += n
@@ -169,8 +171,8 @@ class GPTDecoder:
         self._admit(counts)
         dev = self.lengths.device
         last = torch.tensor([sum(counts[:b + 1]) - 1 for b, n in enumerate(counts) if n])
-        self._commit(counts)
         logits = self._pass(flat.to(dev), torch.tensor(counts, dtype=torch.int32, device=dev), last.to(dev), counts)
+        self._commit(counts)
         self._wait([w and not n for w, n in zip(self._waiting, counts)])
         return logits
 
@@ -193,8 +195,9 @@ class GPTDecoder:
         if not any(counts):
             raise ValueError("GPTDecoder: every place was released; extend begins a sequence")
         self._admit(counts)
+        logits = self._pass(tokens, self._taking, None, counts, any(self._waiting))
         self._commit(counts)
-        return self._pass(tokens, self._taking, None, counts, any(self._waiting))
+        return logits
 
     def release(self, which: Sequence[int]) -> None:
         """Ends the sequences of these places and frees their pages; the places wait until :meth:`extend` gives them new ones."""

@@ -202,6 +202,28 @@ def test_a_prompt_behind_a_replayed_token_sees_its_own_keys(monkeypatch):
     assert torch.allclose(*rows, atol=1e-5)
 
 
+def test_a_pass_that_fails_appends_nothing(monkeypatch):
+    model = _model()
+    d, e = (model.decoder(2, 64, pages=4, page_size=16) for _ in range(2))
+    for x in (d, e):
+        x.extend([[1, 2, 3], [4]])
+    store, calls = P.store, []
+
+    def failing(*args):
+        calls.append(args)
+        if len(calls) % 2 == 0:                  # the second layer's
+            raise RuntimeError("no memory")
+        store(*args)
+    for call in (lambda x: x.extend([[5] * 20, []]), lambda x: x.step(torch.tensor([6, 7])), lambda x: x.extend([[], list(range(30))])):
+        state = list(d.held), d.pages_left, d.lengths.tolist(), int(d.free_count)
+        monkeypatch.setattr(P, "store", failing)
+        with pytest.raises(RuntimeError, match="no memory"):
+            call(d)
+        monkeypatch.setattr(P, "store", store)
+        assert (d.held, d.pages_left, d.lengths.tolist(), int(d.free_count)) == state
+        assert torch.equal(call(d), call(e))
+
+
 def test_refusals():
     model = _model(norm="layer", positional="learned")
     for bad in (lambda: model.decoder(0, 8), lambda: model.decoder(1, 0), lambda: model.decoder(1, 257), lambda: model.decoder(1, 8, page_size=24),
