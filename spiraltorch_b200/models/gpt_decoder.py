@@ -15,6 +15,7 @@ import torch
 from ..ops import attention as attn_ops
 from ..ops import elementwise as ew
 from ..ops import gemm as gemm_ops
+from ..ops import native
 from ..ops import paged
 from ..ops import rotary as rotary_ops
 
@@ -26,7 +27,10 @@ class GPTDecoder:
     """``sequences`` places for sequences of up to ``max_length`` tokens over ``pages`` pages (default: enough for all of them).
 
     The lengths are kept on the host as well (``held``), so that a call that does not fit is refused before anything is launched.  Replays of a captured
-    :meth:`step` do not pass through them: once a step has been captured, every other call first takes them from the device (:meth:`sync`)."""
+    :meth:`step` do not pass through them: once a step has been captured, every other call first takes them from the device (:meth:`sync`).
+
+    A kernel that gives up (a page that is none, a wait that runs out) leaves an error record; :meth:`extend` and :meth:`step` raise what calls and replays before
+    them left, :meth:`generate` what its own passes leave."""
 
     def __init__(self, model, sequences: int, max_length: int, *, pages: Optional[int] = None, page_size: int = 64):
         cfg = model.cfg
@@ -168,6 +172,7 @@ class GPTDecoder:
         if self._capturing():
             raise ValueError("GPTDecoder: extend takes tokens from the host and cannot be captured; step can")
         self._settle()
+        native.poll()
         self._admit(counts)
         dev = self.lengths.device
         last = torch.tensor([sum(counts[:b + 1]) - 1 for b, n in enumerate(counts) if n])
@@ -191,6 +196,7 @@ class GPTDecoder:
             self._captured = True
             return self._pass(tokens, self._taking, None, [1] * self.sequences, True)
         self._settle()
+        native.poll()
         counts = [int(not w) for w in self._waiting]
         if not any(counts):
             raise ValueError("GPTDecoder: every place was released; extend begins a sequence")
@@ -229,8 +235,9 @@ class GPTDecoder:
         logits = self.extend(prompts)
         while True:
             best = logits.argmax(-1)
-            going, feed = [], [[] for _ in prompts]
-            for b, t in zip(active, best.tolist()):
+            going, feed, chosen = [], [[] for _ in prompts], best.tolist()
+            native.poll()      # the pass is done
+            for b, t in zip(active, chosen):
                 if t != stop:
                     out[b].append(t)
                     if len(out[b]) < max_new_tokens:

@@ -224,6 +224,28 @@ def test_a_pass_that_fails_appends_nothing(monkeypatch):
         assert torch.equal(call(d), call(e))
 
 
+def test_an_error_record_of_the_kernels_ends_a_call(monkeypatch):
+    from spiraltorch_b200.ops import native
+    model, polls = _model(), []
+
+    def poll(limit):
+        polls.append(1)
+        if len(polls) == limit:
+            raise native.NativeError("device error")
+    for limit in (1, 2, 3, 5):                  # while tokens are generated: at a call's beginning and where the host has read its tokens
+        polls.clear()
+        monkeypatch.setattr(native, "poll", lambda: poll(limit))
+        with pytest.raises(native.NativeError):
+            model.generate([[1, 2], [3]], 4)
+    d = model.decoder(1, 64)
+    for call in (lambda: d.extend([[1]]), lambda: d.step(torch.tensor([2]))):
+        polls.clear()
+        monkeypatch.setattr(native, "poll", lambda: poll(1))
+        with pytest.raises(native.NativeError):
+            call()
+        assert d.held == [0] == d.lengths.tolist()
+
+
 def test_refusals():
     model = _model(norm="layer", positional="learned")
     for bad in (lambda: model.decoder(0, 8), lambda: model.decoder(1, 0), lambda: model.decoder(1, 257), lambda: model.decoder(1, 8, page_size=24),
@@ -352,3 +374,22 @@ def test_gpu_replays_without_pages():
     assert d.pages_left == 1
     assert torch.equal(d.step(tokens), e.step(tokens)) and d.held == [18, 0]
     assert torch.equal(d.extend([[], [7] * 9])[0], model.decoder(1, 64, page_size=16).extend([[7] * 9])[0])
+
+
+@pytest.mark.gpu
+def test_gpu_error_records_surface_in_the_decoder():
+    from spiraltorch_b200.ops import native
+    d = _model("cuda", torch.bfloat16).decoder(1, 64, page_size=16)
+    tokens = torch.tensor([3], device="cuda")
+    d.extend([[1] * 20])
+    page = int(d.table[0, 0])
+    d.table[0, 0] = -1                       # the kernel's own check finds it
+    d.step(tokens)
+    torch.cuda.synchronize()
+    with pytest.raises(native.NativeError, match="0x7004"):
+        d.step(tokens)
+    assert d.held == [21] and native.read_error_word()[0] == 0
+    d.table[0, 0] = page
+    d.step(tokens)
+    torch.cuda.synchronize()
+    assert native.read_error_word()[0] == 0
