@@ -685,7 +685,7 @@ __global__ void __launch_bounds__(kThreadsOf<R>, Layout<D, R, kQueryParts<T>>::B
   const uint32_t tmem = sh.tmem;
   if (threadIdx.x == 0 && !p.whole) note->parts = 0;
   if (!share) {
-    if (p.zero_tail && warp == SW + 3) zero_rows<T, D>(p);
+    if (warp == SW + 3) blank_rows<T, D>(p);
     if (warp == SW + 1) st::tmem_dealloc(tmem, L::COLUMNS);
     return;
   }
@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(kThreadsOf<R>, Layout<D, R, kQueryParts<T>>::B
       Copier<L, D, R, true, S> values(sh, p, &v_map, u0, u1, f, sq);
       while (values.copy()) {}
       under_way.x = values.turn;
-      if (p.zero_tail) zero_rows<T, D>(p);
+      blank_rows<T, D>(p);
     }
   } else {
     if constexpr (kShift) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R == 32 ? 88 : 176));
@@ -799,7 +799,7 @@ ST_API long long st_paged_attention_workspace(int max_queries, int heads, int kv
 
 // q, out [rows, heads, dim] (dim contiguous, strides in elements): row starts[b] + i is the i-th of the newest tokens of sequence b, whose keys and values,
 // these tokens' included, are the first lengths[b] of the pages in table[b].  lse [rows, heads] or null.  max_queries: the most rows of a sequence, by which
-// the row tile is chosen; more are computed too.  zero_tail: rows behind the last sequence become 0 (else they stay as they were).  type: 0 bf16, 1 fp16.
+// the row tile is chosen; more are computed too.  zero_tail: rows behind the last sequence become 0 (else they stay as they were); their lse is -inf.  type: 0 bf16, 1 fp16.
 ST_API int st_paged_attention(const void* q, const void* k_codes, const void* v_codes, const float* k_scale, const float* v_scale, const int* table, const int* starts,
                               const int* lengths, void* out, float* lse, float* workspace, long long q_row, long long q_head, long long o_row, long long o_head,
                               long long table_row, long long pages, long long rows, int width, int page_size, int B, int heads, int kv_heads, int dim, int max_queries, float scale,

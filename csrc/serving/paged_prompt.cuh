@@ -531,7 +531,7 @@ __global__ void __launch_bounds__(kThreadsOf<kPromptRows>, 1) paged_prompt_kerne
   const uint32_t tmem = sh.tmem;
   if (threadIdx.x == 0 && !p.whole) note->parts = 0;
   if (!share) {
-    if (p.zero_tail && warp == 19) zero_rows<T, D>(p);
+    if (warp == 19) blank_rows<T, D>(p);
     if (warp == 16) st::tmem_dealloc(tmem, 512);
     return;
   }
@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(kThreadsOf<kPromptRows>, 1) paged_prompt_kerne
   if (warp >= 16) {
     if (warp == 16) under_way = product_warp<D>(sh, tmem, u1);
     else prompt_query_warp<T, D>(sh, p, warp - 17, u0, u1, f, sq);
-    if (p.zero_tail && warp == 19) zero_rows<T, D>(p);
+    if (warp == 19) blank_rows<T, D>(p);
   } else if (warp >= 8) {
     convert_warp<D>(sh, p, warp >= 12, u0, u1, f, sq);
   } else {

@@ -215,10 +215,11 @@ __device__ __forceinline__ void settle(unsigned long long (&bars)[STAGES], uint3
     while (!st::mbar_try_wait(st::smem_u32(&bars[i % STAGES]), i / STAGES & 1) && st::globaltimer_ns() - t0 < 1000000) {}
 }
 
-// Rows behind the last sequence: 0, by one warp of every block.
+// Rows behind the last sequence, by one warp of every block: 0, unless the output is one that the caller gave, and a log-sum-exp of no keys.
 template <typename T, int D>
-__device__ __forceinline__ void zero_rows(const AttnParams& p) {
-  const int lane = threadIdx.x & 31, vectors = p.heads * (D / 2);
+__device__ __forceinline__ void blank_rows(const AttnParams& p) {
+  if (!p.zero_tail && p.lse == nullptr) return;
+  const int lane = threadIdx.x & 31, vectors = p.zero_tail ? p.heads * (D / 2) : 0;
   const long long from = p.B > 0 ? max(p.starts[p.B], 0) : 0;
 #pragma unroll 1
   for (long long row = from + blockIdx.x; row < p.rows; row += gridDim.x) {

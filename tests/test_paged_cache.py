@@ -555,6 +555,23 @@ def test_pages_that_are_none_are_refused_by_the_kernels():
     assert native.read_error_word()[0] == 3 and all((t.view(torch.uint8) == 0).all() for t in pages)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_attention_log_sums_of_rows_of_no_sequence(device, n):
+    """In a given output such rows stay as they were; their log-sum-exp, which the call makes, is that of no keys."""
+    pages, table = _cache([50, 64], 2, 16, 64, 3)
+    pages, table = P.Pages(*(t.to(device) for t in pages)), table.to(device)
+    starts, ln = (torch.tensor(v, dtype=torch.int32, device=device) for v in ([0, n, 2 * n], [50, 64]))
+    rows = 2 * n + 6
+    q, out = torch.randn(rows, 4, 64).bfloat16().to(device), torch.full((rows, 4, 64), 7.0, device=device).bfloat16()
+    want = P.attention(q, pages, table, starts, ln, max_queries=n, return_lse=True)
+    junk = [torch.full((rows, 4), 3.0, device=device) for _ in range(4)]        # what the call's own memory may have held
+    del junk
+    got = P.attention(q, pages, table, starts, ln, max_queries=n, return_lse=True, out=out)
+    assert torch.equal(got[1], want[1]) and (got[1][2 * n:] == float("-inf")).all()
+    assert got[0] is out and (out[2 * n:] == 7).all() and torch.equal(out[:2 * n], want[0][:2 * n])
+
+
 def test_attention_reference_against_softmax():
     pages, table = _cache([20, 33], 2, 16, 64, 1)
     q, starts, ln = torch.randn(6, 4, 64).bfloat16(), torch.tensor([0, 2, 5], dtype=torch.int32), torch.tensor([20, 33], dtype=torch.int32)
