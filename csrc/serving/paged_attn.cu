@@ -799,7 +799,8 @@ ST_API long long st_paged_attention_workspace(int max_queries, int heads, int kv
 
 // q, out [rows, heads, dim] (dim contiguous, strides in elements): row starts[b] + i is the i-th of the newest tokens of sequence b, whose keys and values,
 // these tokens' included, are the first lengths[b] of the pages in table[b].  lse [rows, heads] or null.  max_queries: the most rows of a sequence, by which
-// the row tile is chosen; more are computed too.  zero_tail: rows behind the last sequence become 0 (else they stay as they were); their lse is -inf.  type: 0 bf16, 1 fp16.
+// the row tile is chosen; more are computed too.  zero_tail: rows before the first
+// sequence and behind the last one become 0 (else they stay as they were); their lse is -inf.  type: 0 bf16, 1 fp16.
 ST_API int st_paged_attention(const void* q, const void* k_codes, const void* v_codes, const float* k_scale, const float* v_scale, const int* table, const int* starts,
                               const int* lengths, void* out, float* lse, float* workspace, long long q_row, long long q_head, long long o_row, long long o_head,
                               long long table_row, long long pages, long long rows, int width, int page_size, int B, int heads, int kv_heads, int dim, int max_queries, float scale,

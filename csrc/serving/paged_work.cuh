@@ -215,22 +215,25 @@ __device__ __forceinline__ void settle(unsigned long long (&bars)[STAGES], uint3
     while (!st::mbar_try_wait(st::smem_u32(&bars[i % STAGES]), i / STAGES & 1) && st::globaltimer_ns() - t0 < 1000000) {}
 }
 
-// Rows behind the last sequence, by one warp of every block: 0, unless the output is one that the caller gave, and a log-sum-exp of no keys.
+// Rows before the first sequence and behind the last one, by one warp of every block: 0, unless the output is one that the caller gave, and a
+// log-sum-exp of no keys.
 template <typename T, int D>
 __device__ __forceinline__ void blank_rows(const AttnParams& p) {
   if (!p.zero_tail && p.lse == nullptr) return;
   const int lane = threadIdx.x & 31, vectors = p.zero_tail ? p.heads * (D / 2) : 0;
-  const long long from = p.B > 0 ? max(p.starts[p.B], 0) : 0;
+  const long long before = p.B > 0 ? min(static_cast<long long>(max(p.starts[0], 0)), p.rows) : 0, behind = p.B > 0 ? max(p.starts[p.B], 0) : 0;
 #pragma unroll 1
-  for (long long row = from + blockIdx.x; row < p.rows; row += gridDim.x) {
+  for (long long i = blockIdx.x;; i += gridDim.x) {
+    const long long row = i < before ? i : behind + i - before;
+    if (row >= p.rows) break;
     T* o = static_cast<T*>(p.out) + row * p.o_row;
 #pragma unroll 1
-    for (int i = lane; i < vectors; i += 32) {
-      T* at = o + i / (D / 2) * p.o_head + i % (D / 2) * 2;
+    for (int j = lane; j < vectors; j += 32) {
+      T* at = o + j / (D / 2) * p.o_head + j % (D / 2) * 2;
       at[0] = at[1] = from_f<T>(0.0f);
     }
     if (p.lse != nullptr)
-      for (int i = lane; i < p.heads; i += 32) p.lse[row * p.heads + i] = -INFINITY;
+      for (int j = lane; j < p.heads; j += 32) p.lse[row * p.heads + j] = -INFINITY;
   }
 }
 

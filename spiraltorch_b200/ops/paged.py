@@ -311,8 +311,8 @@ def attention(q: torch.Tensor, pages: Pages, table: torch.Tensor, starts: torch.
     row is its newest token, and a row sees the keys up to its own place, or all where not ``causal``.  A row that sees none is 0.
     ``max_queries``: the most rows of one sequence; it decides the kernel's tile, not the result.  ``scale``: ``1 / sqrt(dim)`` if not given.
 
-    Returns ``o`` like ``q`` (contiguous, or ``out``), with ``return_lse`` also the log-sum-exp of every row's scores, fp32 ``[rows, heads]``.  Rows behind the
-    last sequence are 0 (lse -inf); in a given ``out``, which may be ``q`` itself, they stay as they were.  Not differentiable.  Whole causal
+    Returns ``o`` like ``q`` (contiguous, or ``out``), with ``return_lse`` also the log-sum-exp of every row's scores, fp32 ``[rows, heads]``.  Rows of no
+    sequence, before ``starts[0]`` and behind the last one, are 0 (lse -inf); in a given ``out``, which may be ``q`` itself, they stay as they were.  Not differentiable.  Whole causal
     prompts of 2000 tokens and more run faster over :func:`read` and ``ops.attention``."""
     global launch_count
     P, Hk, page, D = _check_pages(pages)
@@ -342,8 +342,8 @@ def attention(q: torch.Tensor, pages: Pages, table: torch.Tensor, starts: torch.
         o, lse = attention_reference(q, pages, table, starts, lengths, causal, scale)
         o = o.to(q.dtype)
         if out is not None:
-            end = min(int(starts[-1]), rows)
-            out[:end] = o[:end]
+            first, end = max(int(starts[0]), 0), min(int(starts[-1]), rows)
+            out[first:end] = o[first:end]
             o = out
         return (o, lse.float()) if return_lse else o
     index = native.require_cuda("paged.attention", q, *pages, table, starts, lengths, out)

@@ -572,6 +572,31 @@ def test_attention_log_sums_of_rows_of_no_sequence(device, n):
     assert got[0] is out and (out[2 * n:] == 7).all() and torch.equal(out[:2 * n], want[0][:2 * n])
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_attention_of_some_of_the_sequences(device, n):
+    """A part of starts, table and lengths: rows before the first sequence are no sequence's either, and are 0."""
+    pages, table = _cache([70, 50, 64, 90], 2, 16, 64, 3)
+    pages, table = P.Pages(*(t.to(device) for t in pages)), table.to(device)
+    starts, ln = (torch.tensor(v, dtype=torch.int32, device=device) for v in ([0, n, 2 * n, 3 * n, 4 * n], [70, 50, 64, 90]))
+    q = torch.randn(4 * n + 3, 4, 64).bfloat16().to(device)
+    o, lse = P.attention(q, pages, table, starts, ln, max_queries=n, return_lse=True)
+    for first, last in ((1, 3), (2, 4), (3, 3), (4, 4), (0, 4)):
+        junk = [torch.full_like(q, 3.0) for _ in range(4)], [torch.full_like(lse, 3.0) for _ in range(4)]
+        del junk
+        part = table[first:last], starts[first:last + 1], ln[first:last]
+        got, got_lse = P.attention(q, pages, *part, max_queries=n, return_lse=True)
+        mine = slice(first * n, last * n)
+        assert torch.equal(got[mine], o[mine]) and torch.equal(got_lse[mine], lse[mine])
+        for rest in (slice(0, first * n), slice(last * n, None)):
+            assert (got[rest] == 0).all() and (got_lse[rest] == float("-inf")).all()
+        out = torch.full_like(q, 7.0)
+        got_lse = P.attention(q, pages, *part, max_queries=n, return_lse=True, out=out)[1]
+        assert torch.equal(out[mine], o[mine]) and torch.equal(got_lse[mine], lse[mine])
+        for rest in (slice(0, first * n), slice(last * n, None)):
+            assert (out[rest] == 7).all() and (got_lse[rest] == float("-inf")).all()
+
+
 def test_attention_reference_against_softmax():
     pages, table = _cache([20, 33], 2, 16, 64, 1)
     q, starts, ln = torch.randn(6, 4, 64).bfloat16(), torch.tensor([0, 2, 5], dtype=torch.int32), torch.tensor([20, 33], dtype=torch.int32)
