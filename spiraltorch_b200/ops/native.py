@@ -14,6 +14,7 @@ import threading
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from ..utils import build as _build
 
@@ -207,6 +208,13 @@ def deterministic_reduction() -> bool:
     def on(name: str) -> bool:
         return os.environ.get(name, "0").strip().lower() not in ("0", "", "false", "off", "no")
     return on("SPIRAL_DETERMINISTIC_REDUCTION") or on("SPIRAL_DETERMINISTIC")
+
+
+def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a tensor carries a tangent of forward-mode differentiation, which a launch on its address would drop.  Function transforms do not
+    count: their tensors have no address to launch on."""
+    return forward_ad._current_level >= 0 and torch._C._functorch.peek_interpreter_stack() is None and \
+        any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def use_native(t: torch.Tensor) -> bool:

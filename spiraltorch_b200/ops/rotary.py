@@ -131,9 +131,19 @@ class _RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, freq, form):
         ctx.save_for_backward(positions, freq)
-        ctx.form = form
+        ctx.save_for_forward(positions, freq)
+        ctx.form, ctx.shapes = form, (q.shape, None if k is None else k.shape)
         ctx.set_materialize_grads(False)
         return _apply(q, k, positions, freq, *form)
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):      # linear in q and k; None: no tangent, or no k
+        tq, tk = (t if t is None or t.stride()[-1] == 1 else t.contiguous() for t in (tq, tk))
+        if tq is None:
+            return tk.new_zeros(ctx.shapes[0]), _rotate(tk, None, *ctx.saved_tensors, *ctx.form)[0]
+        if tk is None and ctx.shapes[1] is not None:
+            return _rotate(tq, None, *ctx.saved_tensors, *ctx.form)[0], tq.new_zeros(ctx.shapes[1])
+        return _rotate(tq, tk, *ctx.saved_tensors, *ctx.form)
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -150,14 +160,14 @@ class _RotaryFn(torch.autograd.Function):
 
 
 def _rotate(q, k, positions, freq, interleaved, magnitude, backward):
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or native.has_tangent(q, k):
         return _RotaryFn.apply(q, k, positions, freq, (interleaved, magnitude, backward))
     return _apply(q, k, positions, freq, interleaved, magnitude, backward)
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freq: torch.Tensor, *, interleaved: bool = False,
            magnitude: float = 1.0):
-    """``(q, k)`` rotated, in new contiguous tensors; differentiable in both.
+    """``(q, k)`` rotated, in new contiguous tensors; differentiable in both, in reverse and in forward mode.
 
     ``q`` ``[..., heads, dim]`` and ``k`` ``[..., kv_heads, dim]`` or None: bf16, fp16 or fp32 with contiguous head elements and any other strides;
     ``positions`` ``[...]`` int32 or int64; ``freq`` from :func:`frequencies`, on the same device: the first ``2 * len(freq)`` elements of a head are
@@ -172,6 +182,8 @@ def rotary_(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
     _check(q, k, positions, freq)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         raise ValueError("rotary_: in-place form of tensors that require gradients; use rotary()")
+    if native.has_tangent(q, k):
+        raise ValueError("rotary_: in-place form of tensors with tangents; use rotary()")
     if not native.use_native(q):
         for x in (q, k):
             if x is not None:

@@ -79,6 +79,40 @@ def test_gradients_against_differences():
     assert torch.autograd.grad(R.rotary(q.detach(), k, pos, f)[1].sum(), k)[0].shape == k.shape
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=GPU)])
+@pytest.mark.parametrize("inter", [False, True])
+def test_tangents(device, inter):
+    """The map is linear: a tangent is rotated as its tensor is."""
+    import torch.autograd.forward_ad as fw
+    g = torch.Generator().manual_seed(3)
+    q, k, tq, tk = (torch.randn(5, h, 64, generator=g).to(device) for h in (4, 2, 4, 2))
+    pos, f = torch.tensor([0, 3, 900, 5, 7], device=device), R.frequencies(32).to(device)
+    call = lambda a, b: R.rotary(a, b, pos, f, interleaved=inter, magnitude=1.25)                # noqa: E731
+    value, want = call(q, k), call(tq, tk)
+    with fw.dual_level():
+        for grad in (False, True):
+            a, b = (fw.make_dual(x.clone().requires_grad_(grad), t) for x, t in ((q, tq), (k, tk)))
+            for got, v, w in zip(call(a, b), value, want):
+                assert torch.equal(fw.unpack_dual(got).tangent, w) and torch.equal(fw.unpack_dual(got).primal, v)
+            only = call(q, b)
+            assert torch.equal(fw.unpack_dual(only[1]).tangent, want[1])
+            assert (t := fw.unpack_dual(only[0]).tangent) is None or (t == 0).all()
+            assert torch.equal(fw.unpack_dual(call(a, None)[0]).tangent, want[0])
+            wide = tq[..., :1].expand_as(tq)
+            assert torch.equal(fw.unpack_dual(call(fw.make_dual(q.clone(), wide), k)[0]).tangent, call(wide.contiguous(), None)[0])
+            plain = call(q, k)
+            assert torch.equal(plain[0], value[0]) and fw.unpack_dual(plain[0]).tangent is None
+        with pytest.raises(ValueError, match="tangent"):
+            R.rotary_(fw.make_dual(q.clone(), tq), None, pos, f)
+        with pytest.raises(ValueError, match="tangent"):
+            R.rotary_(q.clone(), fw.make_dual(k.clone(), tk), pos, f)
+        R.rotary_(q.clone(), k.clone(), pos, f)
+        # over a gradient: of sum(rotated * w) along a tangent of w
+        a = q.clone().requires_grad_(True)
+        got = torch.autograd.grad((R.rotary(a, None, pos, f, interleaved=inter)[0] * fw.make_dual(q, tq)).sum(), a)[0]
+        assert torch.equal(fw.unpack_dual(got).tangent, R.rotary_(tq.clone(), None, pos, f, interleaved=inter, backward=True)[0])
+
+
 def test_refusals():
     q, k, pos, f = torch.randn(4, 2, 16), torch.randn(4, 1, 16), torch.arange(4), R.frequencies(16)
     for bad in (lambda: R.rotary(q.to(torch.int32), k, pos, f), lambda: R.rotary(q, k, pos[:3], f), lambda: R.rotary(q, k, pos.float(), f),
