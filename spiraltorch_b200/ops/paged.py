@@ -331,7 +331,7 @@ def attention(q: torch.Tensor, pages: Pages, table: torch.Tensor, starts: torch.
         raise ValueError(f"paged.attention: max_queries {max_queries}")
     if not 0 < P * Hk * page < 1 << 31:
         raise ValueError(f"paged.attention: {P} pages of {page} tokens and {Hk} heads")
-    if torch.is_grad_enabled() and q.requires_grad:
+    if torch.is_grad_enabled() and q.requires_grad or native.has_tangent(q):
         raise ValueError("paged.attention: not differentiable; use ops.attention for training")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1):
         raise ValueError(f"paged.attention: out {tuple(out.shape)} {out.dtype} is not like q")

@@ -597,6 +597,19 @@ def test_attention_of_some_of_the_sequences(device, n):
             assert (out[rest] == 7).all() and (got_lse[rest] == float("-inf")).all()
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_attention_refuses_tangents(device):
+    import torch.autograd.forward_ad as fw
+    pages = P.Pages(*(t.zero_() for t in P.Pages.allocate(2, 1, 16, 64, device=device)))
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=device)                           # noqa: E731
+    q = torch.randn(1, 2, 64, device=device).bfloat16()
+    call = lambda q: P.attention(q, pages, i32(0).view(1, 1), i32(0, 1), i32(3), max_queries=1)  # noqa: E731
+    with fw.dual_level():
+        with pytest.raises(ValueError, match="not differentiable"):
+            call(fw.make_dual(q, torch.ones_like(q)))
+        assert (call(q) == 0).all()
+
+
 def test_attention_reference_against_softmax():
     pages, table = _cache([20, 33], 2, 16, 64, 1)
     q, starts, ln = torch.randn(6, 4, 64).bfloat16(), torch.tensor([0, 2, 5], dtype=torch.int32), torch.tensor([20, 33], dtype=torch.int32)
