@@ -453,7 +453,12 @@ ST_API int st_paged_plan(const int* lengths, const int* added, int* table, long 
   const long long want = (rows + 4 * kPlanThreads - 1) / (4 * kPlanThreads);
   const int blocks = static_cast<int>(want < 1 ? 1 : want > 4 * st::sm_count() ? 4 * st::sm_count() : want);
   const size_t smem = 2 * (static_cast<size_t>(B) + 1) * sizeof(int);
-  if (smem > 48 * 1024) ST_CUDA_CHECK(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  // once, for the most sequences: the 48 KB that need no opting in are for the sums and what the kernel declares itself together
+  static bool opted[st::kMaxDevices];
+  if (bool& done = opted[st::current_device()]; !done) {
+    ST_CUDA_CHECK(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(2 * (kMaxSequences + 1) * sizeof(int))));
+    done = true;
+  }
   const cudaError_t e = st::chained(plan_kernel, dim3(blocks), dim3(kPlanThreads), smem, reinterpret_cast<cudaStream_t>(stream_v))(
       lengths, added, table, table_row, width, free_list, free_count, free_size, shift, B, rows, starts, positions, slots, lengths_after, free_after);
   if (e != cudaSuccess) return st::fail_cuda(e, "paged plan");

@@ -7,6 +7,10 @@ Tolerance of attention.  With p the softmax weights of a row, A = sum p |v|, S =
   below 2^-16 of that, 2^-25 of the largest, may be dropped: 2^-11 A + n 2^-25 max |v|;
 - exp2 and the fp32 sums of weights and of products: 2^-20 A is more than their few units in the last place per step of 16 keys, for n up to 4096;
 - the result is rounded once: half a step of the type times |o|."""
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -97,6 +101,22 @@ def test_plan_of_many_sequences_and_strided_table():
     assert torch.equal(wide[:, :11].cpu(), table) and (wide[:, 11:] == -9).all()
     with pytest.raises(ValueError, match="8193"):
         P.plan(*(t.cuda() for t in (torch.zeros(8193).int(), torch.zeros(8193).int(), torch.zeros(8193, 1).int(), free, count)), page_size=32, rows=4)
+
+
+@GPU
+def test_plan_of_many_sequences_in_a_process_of_its_own():
+    """The prefix sums pass 48 KB of shared memory: launches that no larger one went before."""
+    code = """
+import torch
+from spiraltorch_b200.ops import paged as P
+i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")
+for B in (6100, 6126, 6127, 6143, 6144, 8192, 3):
+    free = torch.arange(B, dtype=torch.int32, device="cuda")
+    step = P.plan(i32(B), i32(B) + 1, i32(B, 1), free, i32(1) + B, page_size=16, rows=B)
+    assert torch.equal(step.slots, 16 * free.flip(0).long()) and int(step.free_count) == 0, B
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=Path(__file__).resolve().parents[1])
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 # ---- storing and reading ----------------------------------------------------------------------------------------------------------
