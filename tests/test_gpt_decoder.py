@@ -344,9 +344,13 @@ def test_gpu_calls_behind_replays():
     assert torch.equal(d.extend([[9], prompt, []]), e.extend([[9], prompt, []]))
     turns(5)
     assert torch.equal(d.step(tokens), e.step(tokens)) and d.held == e.held == [48, 46, 64] == d.lengths.tolist()
-    with torch.cuda.graph(torch.cuda.CUDAGraph()), pytest.raises(ValueError, match="captured"):
-        d.extend([[9], [], []])
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        tokens + 1
+        for call in (lambda: d.extend([[9], [], []]), lambda: d.release([0])):
+            with pytest.raises(ValueError, match="captured"):
+                call()
     torch.cuda.synchronize()
+    assert d.held == [48, 46, 64]
 
 
 @pytest.mark.gpu
