@@ -18,6 +18,7 @@ using st::chain_begin;
 
 constexpr int kThreads = 256;
 constexpr int kMaxTokens = 8;      // of a block
+constexpr int kMaxAngles = 48 * 1024 / sizeof(float2);      // of a block
 
 struct RotaryParams {
   long long q_row, q_head, k_row, k_head, qo_row, qo_head, ko_row, ko_head;
@@ -102,10 +103,10 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const T* q, const T* k
 template <typename T, int F, bool INTER, typename POS>
 int launch(const void* q, const void* k, void* qo, void* ko, const void* positions, const double* freq, RotaryParams p, bool in_place, cudaStream_t stream) {
   p.units = p.half / F + (in_place ? 0 : (p.dim - 2 * p.half + 2 * F - 1) / (2 * F));
-  // enough tokens to a block for two units per thread, while that leaves two blocks per SM
+  // enough tokens to a block for two units per thread, while that leaves two blocks per SM and their angles need no opting in
   const int per_token = (p.heads + p.kv_heads) * p.units;
   int n = 1;
-  while (n < kMaxTokens && n * per_token < 2 * kThreads && p.tokens / (2 * n) >= 2 * st::sm_count()) n *= 2;
+  while (n < kMaxTokens && n * per_token < 2 * kThreads && 2 * n * p.half <= kMaxAngles && p.tokens / (2 * n) >= 2 * st::sm_count()) n *= 2;
   p.tokens_per_block = n;
   const long long blocks = (p.tokens + n - 1) / n;
   if (blocks > 2147483647LL) return st::fail(ST_ERR_TOO_LARGE, "rotary: too many tokens");

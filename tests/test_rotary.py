@@ -147,6 +147,20 @@ def test_kernel(dtype, rows, h, hk, dim, rot, inter):
 
 
 @GPU
+@pytest.mark.parametrize("half", [776, 1016, 1544, 2040, 2048])
+@pytest.mark.parametrize("inter", [False, True])
+def test_kernel_of_one_wide_head(half, inter):
+    """Several tokens' angles of a block pass 48 KB of shared memory; and the widest head."""
+    g = torch.Generator().manual_seed(half)
+    rows, f = 2500, R.frequencies(2 * half)
+    x, pos = torch.randn(rows, 1, 2 * half + 16, generator=g).bfloat16(), torch.randint(0, 1 << 20, (rows,), generator=g)
+    want = _complex(x, pos, f, inter)
+    got = R.rotary(x.cuda(), None, pos.cuda(), f.cuda(), interleaved=inter)[0].cpu()
+    assert ((got.double() - want).abs() <= _allowed(x, want, half, inter, x.dtype)).all()
+    assert torch.equal(R.rotary_(x.cuda(), None, pos.cuda(), f.cuda(), interleaved=inter)[0].cpu(), got)
+
+
+@GPU
 def test_views_in_place_and_without_keys():
     rows, h, hk, D = 37, 6, 2, 128
     fused = torch.randn(rows, (h + 2 * hk) * D + 8, device="cuda").bfloat16()
