@@ -403,8 +403,8 @@ class GPTModel(nn.Module):
     def generate(self, prompts, max_new_tokens: int, *, stop: Optional[int] = None, page_size: int = 64) -> list:
         """The likeliest continuation of each prompt (a list of token ids), token by token, up to ``max_new_tokens`` or the token ``stop``.
         Returns the new tokens of each."""
-        longest = max((len(p) for p in prompts), default=0)
-        return self.decoder(len(prompts), longest + max_new_tokens, page_size=page_size).generate(prompts, max_new_tokens, stop=stop)
+        longest = max((len(p) for p in prompts), default=0) + max(max_new_tokens - 1, 0)      # the last new token is not appended
+        return self.decoder(len(prompts), longest, page_size=page_size).generate(prompts, max_new_tokens, stop=stop)
 
     # ------------------------------------------------------------------------------------------
     def sync_replicated_grads(self) -> None:

@@ -105,6 +105,17 @@ def test_generate():
     assert model.generate(prompts, 0) == [[], [], []]
 
 
+def test_generate_up_to_the_last_learned_position():
+    """The last new token is never appended."""
+    model = _model(norm="layer", positional="learned")
+    prompt = [i % 96 for i in range(250)]
+    got = model.generate([prompt], 7)
+    assert len(got[0]) == 7 and got == model.decoder(1, 256).generate([prompt], 7)
+    assert [len(t) for t in model.generate([prompt + [1] * 6, [5]], 1)] == [1, 1] and model.generate([prompt + [1] * 6], 0) == [[]]
+    with pytest.raises(ValueError, match="learned positions"):
+        model.generate([prompt], 8)
+
+
 def test_training_with_other_rotary_forms_matches_autograd():
     for kw in CONFIGS[2:]:
         cfg = GPTConfig(vocab_size=64, d_model=128, n_layers=1, n_heads=2, ffn=128, seq_len=8, init_std=0.05, **kw)
