@@ -188,7 +188,7 @@ def store(k: torch.Tensor, v: torch.Tensor, pages: Pages, slots: torch.Tensor) -
     ``slots`` int64 ``[rows]``, from :func:`plan`; below 0: not stored.  Tokens of one page follow one another in the rows, each slot once; a
     page belongs to one sequence.  A group of rows that starts at offset 0 begins its page anew, one behind that keeps the tokens before
     it: where the scale has to grow, their codes are rounded again.  Finite magnitudes above ``448 * 2^60`` and infinities are
-    stored as the largest value of the page, NaN as NaN."""
+    stored as the largest value of the page, NaN as NaN.  Not differentiable: the values alone are stored."""
     global launch_count
     P, H, page, D = _check_pages(pages)
     if k.shape != v.shape or k.dim() != 3 or k.shape[1:] != (H, D) or k.dtype != v.dtype:
@@ -223,6 +223,7 @@ def to_codes(x: torch.Tensor) -> torch.Tensor:
     return x.clamp(-LARGEST, LARGEST).to(torch.float8_e4m3fn)
 
 
+@torch.no_grad()
 def _store_reference(k, v, pages, slots) -> None:
     P, H, page, D = pages.k.shape
     at, rows = slots.tolist(), len(slots)

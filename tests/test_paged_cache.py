@@ -170,6 +170,16 @@ def test_store_of_what_is_not_finite(device):
     assert pages.k_scale[0, 0] == 2.0 ** 60 and P.read(pages, table, n, 17, torch.float32)[0][0, 5, 0, 0] == 448 * 2.0 ** 60
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_store_holds_values_alone(device):
+    """Rows that require gradients: the cache takes their values and no part in the graph."""
+    pages, k = P.Pages.allocate(2, 1, 16, 64, device=device), torch.randn(3, 1, 64, device=device, requires_grad=True)
+    P.store(k * 2, k * 3, pages, torch.arange(3, device=device))
+    assert not any(t.requires_grad for t in pages)
+    table, n = torch.tensor([[0]], dtype=torch.int32, device=device), torch.tensor([3], dtype=torch.int32, device=device)
+    assert not any(t.requires_grad for t in P.read(pages, table, n, 3))
+
+
 @GPU
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("D,H,page", [(64, 1, 16), (128, 3, 16), (128, 8, 64), (64, 12, 128), (128, 2, 256)])
