@@ -640,6 +640,83 @@ def test_attention_refuses_tangents(device):
         assert (call(q) == 0).all()
 
 
+def _rows_and_limits(q, pages, table, lengths, added, causal=True, weight=2.0 ** -11):
+    """Per row, in 64 bits: results, log-sum-exp, whether it sees a key, and how far off results and log-sum-exp may be by the keys that it sees itself (the module's
+    terms; ``weight``: half a step of the type that weights are rounded to).  n keys: sums in steps of 32 products, each step off by a unit of fp32, 2^-23 (n / 32 + 16) A
+    with exp2's and the last sums' own; x + b in fp32 with b up to 60: 2^-22 (64 + S) A; of the weights times 2^b, which are what is rounded, 2^-25 of the largest
+    may be dropped for each key: 2^-25 max(p 2^b) sum |code|.  Below the type's smallest normal number N its steps are eps N apart, so half a step is eps / 2 max(|o|, N);
+    a result that may lie half a step above its largest number may be infinite (both in fp16 only: N = 2^-14, 65504 + 16).  The log-sum-exp is formed from the logarithm of the sum and a reference that both hold b."""
+    rows, heads, D = q.shape
+    H, page = pages.k.shape[1:3]
+    G, at = heads // H, 0
+    want, limit = torch.zeros(rows, heads, D, dtype=torch.float64), torch.zeros(rows, heads, D, dtype=torch.float64)
+    lse, sees = torch.full((rows, heads), float("-inf"), dtype=torch.float64), torch.zeros(rows, dtype=torch.bool)
+    lse_limit = torch.zeros(rows, heads, dtype=torch.float64)
+    for b, (length, n) in enumerate(zip(lengths, added)):
+        of, off = table[b, torch.arange(length) // page].long(), torch.arange(length) % page
+        seen = torch.arange(length) < (length - n + 1 + torch.arange(n) if causal else torch.full((n,), length))[:, None]        # [n, length]
+        some = seen.any(1)
+        sees[at:at + n] = some
+        for h in range(H):
+            k, v = pages.k[of, h, off].double() * pages.k_scale[of, h, None], pages.v[of, h, off].double() * pages.v_scale[of, h, None]
+            unit = pages.v_scale[of, h].double()
+            x = q[at:at + n, h * G:(h + 1) * G].double() * D ** -0.5
+            s = (x @ k.T).masked_fill(~seen[:, None], float("-inf"))
+            size = (x.abs() @ k.abs().T).masked_fill(~seen[:, None], 0.0).amax(-1, keepdim=True) if length else torch.zeros(n, G, 1)
+            p = torch.softmax(s, -1).nan_to_num(0.0)
+            cols, A = slice(h * G, (h + 1) * G), p @ v.abs()
+            want[at:at + n, cols], lse[at:at + n, cols] = p @ v, torch.logsumexp(s, -1) if length else float("-inf")
+            drop = 2.0 ** -25 * (p * unit).amax(-1, keepdim=True) * (seen.double() @ (v.abs() / unit[:, None]))[:, None] if length else 0.0
+            sums = 2.0 ** -23 * (length / 32 + 16) + 2.0 ** -22 * (64 + size)
+            limit[at:at + n, cols] = torch.finfo(q.dtype).eps / 2 * (p @ v).abs().clamp(min=torch.finfo(q.dtype).smallest_normal) + (weight + sums + 2 * D * 2.0 ** -24 * size) * A + drop
+            lse_limit[at:at + n, cols] = (sums + D * 2.0 ** -24 * size)[..., 0] + 2.0 ** -22 * (64 + lse[at:at + n, cols].abs())
+        at += n
+    return want, lse, sees, limit, lse_limit
+
+
+def _check_rows(pages, table, lengths, added, H, G, D, dtype, causal=True, max_queries=None, seed=0):
+    q = torch.randn(sum(added), H * G, D, generator=torch.Generator().manual_seed(seed)).to(dtype)
+    want, lse, sees, limit, lse_limit = _rows_and_limits(q, pages, table, lengths, added, causal)
+    starts = torch.tensor([sum(added[:b]) for b in range(len(added) + 1)], dtype=torch.int32)
+    got, got_lse = P.attention(q.cuda(), P.Pages(*(t.cuda() for t in pages)), table.cuda(), starts.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda(),
+                               max_queries=max_queries or max(added), causal=causal, return_lse=True)
+    got, off = got.cpu(), (got.cpu().double() - want).abs()
+    beyond = got.isinf() & (got.sign() * want + limit >= torch.finfo(dtype).max * (1 + torch.finfo(dtype).eps / 4))
+    bad = ~beyond & ~(off <= limit)
+    assert not bad.any(), (bad.nonzero()[:4].tolist(), got[bad][:4], want[bad][:4], limit[bad][:4])
+    assert ((got_lse.cpu().double() - lse)[sees].abs() <= lse_limit[sees]).all() and (got_lse.cpu()[~sees] == float("-inf")).all()
+    held = want.abs().amax(-1) >= torch.finfo(dtype).smallest_normal * 16
+    assert (limit < want.abs()).any(-1)[sees[:, None] & held].all() and (got[~sees] == 0).all()        # zeros would not pass for a row that sees a key and whose results the type holds
+    assert dtype != torch.bfloat16 or held[sees].all()
+
+
+@GPU
+@pytest.mark.parametrize("D,G,n,page,lengths,causal", [
+    (64, 1, 8, 16, [50, 34, 8], True), (128, 2, 8, 16, [50, 35, 16], True), (64, 4, 8, 32, [66, 36, 9], True), (128, 2, 64, 16, [100, 80, 64], True), (64, 1, 150, 16, [200, 160, 150], True),
+    (128, 1, 8, 64, [2565, 70, 1000], True), (64, 2, 8, 16, [2597, 1700, 9], True), (128, 4, 8, 64, [2690, 70, 2400], True), (64, 2, 80, 32, [2600, 1700, 100], True), (128, 1, 130, 64, [2600, 133, 1800], False)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_with_large_values_that_first_rows_do_not_see(D, G, n, page, lengths, causal, dtype):
+    """Values 2^20 to 2^40 times as large in a sequence's last pages, hidden from its first rows, whose results come from the small ones; and in the
+    pages of another sequence.  Tolerances are each row's own."""
+    pages, table = _cache(lengths, 2, page, D, n + D)
+    for length, entries, by in zip(lengths[:2], table, (2.0 ** 40, 2.0 ** 20)):
+        hidden = range(-(-(length - n + 1) // page), -(-length // page))        # begin behind the keys of the first row
+        assert len(hidden) > 0
+        pages.v_scale[entries[list(hidden)].long()] *= by
+    pages.v_scale[table[2, :-(-lengths[2] // page)].long()] *= 2.0 ** -30
+    _check_rows(pages, table, lengths, [n] * 3, 2, G, D, dtype, causal)
+    if n == 8:
+        _check_rows(pages, table, lengths, [n] * 3, 2, G, D, dtype, causal, max_queries=200)
+        _check_rows(pages, table, lengths, [1] * 3, 2, G, D, dtype, causal)
+
+
+@GPU
+@pytest.mark.parametrize("G,n,dtype,lengths", [(8, 1, torch.bfloat16, [131001, 70000]), (2, 2, torch.float16, [131001, 5, 40000]), (2, 20, torch.bfloat16, [100003]), (1, 130, torch.float16, [60000, 131])])
+def test_attention_of_very_long_contexts(G, n, dtype, lengths):
+    pages, table = _cache(lengths, 1, 128, 128, n)
+    _check_rows(pages, table, lengths, [min(n, length) for length in lengths], 1, G, 128, dtype)
+
+
 def test_attention_reference_against_softmax():
     pages, table = _cache([20, 33], 2, 16, 64, 1)
     q, starts, ln = torch.randn(6, 4, 64).bfloat16(), torch.tensor([0, 2, 5], dtype=torch.int32), torch.tensor([20, 33], dtype=torch.int32)
