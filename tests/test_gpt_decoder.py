@@ -408,3 +408,28 @@ def test_gpu_error_records_surface_in_the_decoder():
     d.step(tokens)
     torch.cuda.synchronize()
     assert native.read_error_word()[0] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts", [[300, 0, 129], [64, 1, 500]])
+def test_gpu_whole_prompts_read_back_see_their_own_keys(counts):
+    """Attention over what the cache gives back, by its own tolerance: scores are fp32 sums of D exact products, weights are rounded to bf16 (2^-9) and
+    come from an exp2 of no more error than that, sums stay below 2^-16, and the result is rounded (2^-9): (2^-8 + 2^-16 + 2 D 2^-24 S) sum p |v| + 2^-9 |o|, S
+    the largest sum |q_d k_d| / 8.  A mask that is one key off would take a row's own key from it."""
+    d = _model("cuda", torch.bfloat16).decoder(3, 512, page_size=64)
+    g = torch.Generator().manual_seed(9)
+    rows, H, D = sum(counts), 2, 64
+    q, k, v = (torch.randn(rows, H, D, generator=g).bfloat16() for _ in range(3))
+    added = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    step = P.plan(d.lengths, added, d.table, d.free, d.free_count, page_size=64, rows=rows)
+    P.store(k.cuda(), v.cuda(), d.cache[1], step.slots)
+    got, r = d._dense(q.cuda(), 1, counts, step.lengths).cpu().double(), 0
+    k, v = (t.cpu().double() for t in P.read(d.cache[1], d.table, step.lengths, max(counts), torch.float32))
+    for b, n in enumerate(counts):
+        s = torch.einsum("ihd,jhd->hij", q[r:r + n].double(), k[b, :n]) / 8 + torch.full((n, n), float("-inf"), dtype=torch.float64).triu(1)
+        size = torch.einsum("ihd,jhd->hij", q[r:r + n].double().abs(), k[b, :n].abs()).tril().amax(-1) if n else torch.zeros(H, 0)
+        p = torch.softmax(s, -1)
+        want, A = torch.einsum("hij,jhd->ihd", p, v[b, :n]), torch.einsum("hij,jhd->ihd", p, v[b, :n].abs())
+        off = (got[r:r + n] - want).abs()
+        assert (off <= (2.0 ** -8 + 2.0 ** -16 + 2 * D * 2.0 ** -24 * size.T[..., None] / 8) * A + 2.0 ** -9 * want.abs()).all()
+        r += n
