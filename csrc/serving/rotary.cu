@@ -5,8 +5,8 @@
 // for the pairs (a, b) = (j, R/2 + j) or, interleaved, (2j, 2j + 1), j < R/2; elements from R on are copied.
 // Bound by memory: every element is read and written once, 3 operations on it.  The angles are no table, which would cap the
 // positions and be read from far away: a block forms those of its tokens once, in turns and fp64 (position * freq / 2 pi keeps 2^-35 of a
-// turn at position 2^17, where fp32 keeps 2^-7), takes the fraction of a turn and the sine and cosine of that in fp32, and keeps
-// them in shared memory for all heads of the token.
+// turn at position 2^17, where fp32 keeps 2^-7), takes the sine and cosine of the fraction of a turn in fp32, adds what fp32 does not hold of the fraction
+// to first order (its square is below 2^-46), and keeps them in shared memory for all heads of the token.
 // Measured: 16384 rows of 16 + 16 heads of 128 in bf16, forward and backward, 92 us, 5.8 TB/s of the 6.5 that a copy reaches.  A step of 64 rows is a launch.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -52,9 +52,11 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const T* q, const T* k
   for (int i = threadIdx.x; i < nt * p.half; i += kThreads) {
     const int t = i / p.half, j = i - t * p.half;
     const double turns = static_cast<double>(positions[t0 + t]) * freq[j] * 0.15915494309189533577;      // 1 / 2 pi
+    const double halves = 2.0 * (turns - rint(turns));
+    const float main = static_cast<float>(halves), rest = static_cast<float>(halves - main) * 3.14159265f;      // |rest| <= pi 2^-25
     float s, c;
-    sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
-    turn[i] = make_float2(c * p.magnitude, s * p.magnitude * p.sign);
+    sincospif(main, &s, &c);
+    turn[i] = make_float2(fmaf(-s, rest, c) * p.magnitude, fmaf(c, rest, s) * p.magnitude * p.sign);
   }
   __syncthreads();
   const int heads = p.heads + p.kv_heads, per_token = heads * p.units, rotated = p.half / F;

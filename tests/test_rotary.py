@@ -147,6 +147,19 @@ def test_kernel(dtype, rows, h, hk, dim, rot, inter):
 
 
 @GPU
+def test_kernel_angles_in_fp32():
+    """Heads of (1, 0) give cosine and sine themselves: sincospif is within a unit in the last place of its argument's, 2^-24 at most, what its argument
+    lacks of the angle is added with one more rounding, 2^-25, and angles are exact to 2^-30."""
+    f, pos = R.frequencies(128), torch.randint(0, 1 << 20, (20000,), generator=torch.Generator().manual_seed(2))
+    x = torch.zeros(20000, 1, 128)
+    x[..., :64] = 1.0
+    got = R.rotary(x.cuda(), None, pos.cuda(), f.cuda())[0].cpu().double()[:, 0]
+    angle = pos.double()[:, None] * f
+    off = (got - torch.cat([angle.cos(), angle.sin()], -1)).abs().max()
+    assert off <= 1.5 * 2.0 ** -24 + 2.0 ** -30, off * 2.0 ** 24
+
+
+@GPU
 @pytest.mark.parametrize("half", [776, 1016, 1544, 2040, 2048])
 @pytest.mark.parametrize("inter", [False, True])
 def test_kernel_of_one_wide_head(half, inter):
