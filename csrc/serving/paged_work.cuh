@@ -13,7 +13,7 @@ constexpr int kTile = 128;            // keys of a unit
 template <int R> constexpr int kThreadsOf = R == 128 ? 640 : R == 32 ? 384 : 256;      // of a block
 constexpr int kMaxWarps = 20;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNoMax = -1e30f;      // before a row has seen a key
+constexpr float kNoMax = -3e38f;      // before a row has seen a key: below all scores but fp32's very last
 constexpr float kLag = 6.0f, kLift = 9.0f;
 
 struct AttnParams {

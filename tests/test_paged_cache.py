@@ -711,6 +711,31 @@ def test_attention_with_large_values_that_first_rows_do_not_see(D, G, n, page, l
 
 
 @GPU
+@pytest.mark.parametrize("D,G,n", [(64, 1, 1), (128, 8, 1), (64, 2, 7), (128, 4, 8)])
+def test_attention_of_scores_far_below_zero(D, G, n):
+    """Scores near -10^36, within fp32's range: no less a row's keys than others.  The keys are equal and their scores with them, so weights are exactly alike and
+    results are means, rounded to bf16 (2^-8); a log-sum-exp is off by its fp32 sum of D products of one sign, D 2^-24 of it, and a few roundings."""
+    lengths = [n, 150, 1, 2600]
+    added = [n, n, 1, n]
+    pages, table = _cache(lengths, 1, 16, D, D + n)
+    pages.k.copy_(torch.full((D,), 96.0)), pages.k_scale.fill_(2.0 ** 60), pages.v_scale.fill_(2.0 ** -5)
+    pages.v.view(torch.uint8).masked_fill_(pages.v.isnan(), 0)
+    starts = torch.tensor([0, n, 2 * n, 2 * n + 1, 3 * n + 1], dtype=torch.int32)
+    q = torch.full((3 * n + 1, G, D), -2.0 ** 50).bfloat16()
+    got, lse = (t.cpu().double() for t in P.attention(q.cuda(), P.Pages(*(t.cuda() for t in pages)), table.cuda(), starts.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda(),
+                                                      max_queries=n, return_lse=True))
+    score = -2.0 ** 50 * 96 * 2.0 ** 60 * D ** 0.5
+    for b, (length, m) in enumerate(zip(lengths, added)):
+        of = table[b, torch.arange(length) // 16].long(), torch.arange(length) % 16
+        v = pages.v[of[0], 0, of[1]].double() * 2.0 ** -5
+        for i in range(m):
+            seen, r = length - m + 1 + i, int(starts[b]) + i
+            want, size = v[:seen].mean(0), v[:seen].abs().mean(0)
+            assert ((got[r] - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -23 * (length / 32 + 16)) * size + 2.0 ** -25 * v.abs().amax()).all()
+            assert ((lse[r] - score).abs() <= -score * (D + 8) * 2.0 ** -24).all()
+
+
+@GPU
 @pytest.mark.parametrize("G,n,dtype,lengths", [(8, 1, torch.bfloat16, [131001, 70000]), (2, 2, torch.float16, [131001, 5, 40000]), (2, 20, torch.bfloat16, [100003]), (1, 130, torch.float16, [60000, 131])])
 def test_attention_of_very_long_contexts(G, n, dtype, lengths):
     pages, table = _cache(lengths, 1, 128, 128, n)
