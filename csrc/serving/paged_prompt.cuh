@@ -328,7 +328,9 @@ __device__ __forceinline__ float prompt_top(uint32_t s_cols, float factor, const
   }
   return top;
 }
-// Weights over the scores that they are made from; returns the sum with them.
+// Weights over the scores that they are made from; returns the sum with them.  x - reference is one multiplication and addition, which holds the product
+// whole where the reference is rounded: of scores beyond kLarge, MASKED rounds x as the reference's was.
+constexpr float kLarge = 4194304.0f;      // 2^22: half a unit in the last place is 2^-2, and weights below 2^15 stay below fp16's 2^16 by it
 template <bool MASKED>
 __device__ __forceinline__ float prompt_weights(uint32_t s_cols, float factor, float ref, float sum, const float* ks, const float* lift, const float* take, int end) {
 #pragma unroll 1
@@ -340,12 +342,13 @@ __device__ __forceinline__ float prompt_weights(uint32_t s_cols, float factor, f
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float lifted = h ? b.y : b.x;
-      const float2 fs = st::splat2(factor * (h ? k.y : k.x)), bs = st::splat2(lifted - ref);
+      const float2 fs = st::splat2(factor * (h ? k.y : k.x)), bs = st::splat2(MASKED ? lifted : lifted - ref);
       const bool none = MASKED && lifted == -INFINITY;
       float2 part = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int j = 0; j < 16; j += 2) {
         float2 x = st::fma2(make_float2(__uint_as_float(raw[16 * h + j]), __uint_as_float(raw[16 * h + j + 1])), fs, bs);
+        if (MASKED) x = st::add2(x, st::splat2(-ref));
         x.x = st::exp2_ftz(x.x), x.y = st::exp2_ftz(x.y);
         if (MASKED && (none || 32 * c + 16 * h + j >= end)) x.x = 0.0f;
         if (MASKED && (none || 32 * c + 16 * h + j + 1 >= end)) x.y = 0.0f;
@@ -410,7 +413,7 @@ __device__ __forceinline__ void prompt_soft_warps(S& sh, const AttnParams& p, ui
           st::tmem_st_wait();
         }
       }
-      sum = gone ? prompt_weights<true>(s_cols, factor, ref, sum, sh.ks[g], sh.lift[g], sh.take[g], end) : prompt_weights<false>(s_cols, factor, ref, sum, sh.ks[g], sh.lift[g], sh.take[g], end);
+      sum = gone || __any_sync(0xffffffffu, fabsf(top) > kLarge) ? prompt_weights<true>(s_cols, factor, ref, sum, sh.ks[g], sh.lift[g], sh.take[g], end) : prompt_weights<false>(s_cols, factor, ref, sum, sh.ks[g], sh.lift[g], sh.take[g], end);
       st::tmem_st_wait();
       st::tc_fence_before();
       st::mbar_arrive(st::smem_u32(&sh.p_full[g]));

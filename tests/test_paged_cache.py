@@ -711,7 +711,7 @@ def test_attention_with_large_values_that_first_rows_do_not_see(D, G, n, page, l
 
 
 @GPU
-@pytest.mark.parametrize("D,G,n", [(64, 1, 1), (128, 8, 1), (64, 2, 7), (128, 4, 8)])
+@pytest.mark.parametrize("D,G,n", [(64, 1, 1), (128, 8, 1), (64, 2, 7), (128, 4, 8), (64, 3, 50), (128, 1, 140)])
 def test_attention_of_scores_far_below_zero(D, G, n):
     """Scores near -10^36, within fp32's range: no less a row's keys than others.  The keys are equal and their scores with them, so weights are exactly alike and
     results are means, rounded to bf16 (2^-8); a log-sum-exp is off by its fp32 sum of D products of one sign, D 2^-24 of it, and a few roundings."""
