@@ -221,11 +221,12 @@ template <typename T, int D>
 __device__ __forceinline__ void blank_rows(const AttnParams& p) {
   if (!p.zero_tail && p.lse == nullptr) return;
   const int lane = threadIdx.x & 31, vectors = p.zero_tail ? p.heads * (D / 2) : 0;
-  const long long before = p.B > 0 ? min(static_cast<long long>(max(p.starts[0], 0)), p.rows) : 0, behind = p.B > 0 ? max(p.starts[p.B], 0) : 0;
+  const int rows = static_cast<int>(p.rows), before = p.B > 0 ? min(max(p.starts[0], 0), rows) : 0, skip = (p.B > 0 ? max(p.starts[p.B], 0) : 0) - before;
 #pragma unroll 1
-  for (long long i = blockIdx.x;; i += gridDim.x) {
-    const long long row = i < before ? i : behind + i - before;
-    if (row >= p.rows) break;
+  for (unsigned i = blockIdx.x;; i += gridDim.x) {
+    const unsigned at = i < before ? i : i + skip;
+    if (at >= rows) break;
+    const long long row = at;
     T* o = static_cast<T*>(p.out) + row * p.o_row;
 #pragma unroll 1
     for (int j = lane; j < vectors; j += 32) {
