@@ -54,8 +54,9 @@ class GPTDecoder:
         self._left = self.pages
         self._lost = [False] * sequences        # replays found no page for some of its tokens
         self._waiting = [False] * sequences     # released, and not extended since: steps pass it over
-        self._taking = torch.ones(sequences, **i32)      # the same on the device: tokens that a step adds
-        self._places = torch.arange(sequences + 1, **i32)
+        # the same on the device, for steps: tokens that each place adds; the place of each row and the row of each place, -1 for those that wait
+        self._taking = torch.ones(sequences, **i32)
+        self._place_of_row, self._row_of_place = torch.arange(sequences, device=dev), torch.arange(sequences, device=dev)
         self._captured = False
 
     # ---- host side ------------------------------------------------------------------------------------------------------------
@@ -101,23 +102,23 @@ class GPTDecoder:
 
     def _wait(self, waiting: list) -> None:
         if waiting != self._waiting:
-            self._taking.copy_(torch.tensor([int(not w) for w in waiting], dtype=torch.int32))
+            take = ~torch.tensor(waiting)
+            self._taking.copy_(take)
+            self._row_of_place.copy_(torch.where(take, take.cumsum(0) - 1, -1))
+            self._place_of_row.copy_(torch.cat([take.nonzero()[:, 0], torch.full((sum(waiting),), -1)]))
             self._waiting = waiting
 
     # ---- device side ----------------------------------------------------------------------------------------------------------
     def _pass(self, tokens: torch.Tensor, added: torch.Tensor, last: Optional[torch.Tensor], counts: Sequence[int], by_place: bool = False) -> torch.Tensor:
-        """Logits of the rows ``last`` (None: all) of ``tokens`` ``[rows]``, of which sequence ``b`` has ``counts[b]``.  ``by_place``: row ``b`` is that of
-        place ``b``, whether it takes its token (``added``) or waits; the logits of those that wait are 0."""
+        """Logits of the rows ``last`` (None: all) of ``tokens`` ``[rows]``, of which sequence ``b`` has ``counts[b]``.  ``by_place``: a token
+        and logits for every place; those that wait have rows behind the last sequence, and logits of 0."""
         m, cfg = self.model, self.model.cfg
         H, D, rows, most = cfg.n_heads, cfg.head_dim, tokens.shape[0], max(counts)
         dense = last is not None and all(n == 0 or DENSE_FROM <= n and held == 0 for n, held in zip(counts, self.held))      # as many queries as keys
         step = paged.plan(self.lengths, added, self.table, self.free, self.free_count, page_size=self.page_size, rows=rows)
-        waits = None
-        if by_place:      # the plan maps the tokens that are added, one after another; a place that waits has no keys, so its row of attention is 0
-            at, waits = step.starts[:-1], (added == 0)[:, None]
-            step = step._replace(starts=self._places, positions=step.positions.index_select(0, at),
-                                 slots=step.slots.index_select(0, at).masked_fill_(waits[:, 0], -1))
         resid, x = ew.embedding_forward(tokens, m.p["embed.weight"]), None
+        if by_place:      # rows in the order of the plan; a lookup of -1 gives zeros
+            resid = ew.embedding_forward(self._place_of_row, resid)
         if cfg.positional == "learned":
             resid = resid + m.p["pos.weight"][step.positions.long().clamp_(max=cfg.seq_len - 1)]      # replays may go on behind the end
         for l in range(cfg.n_layers):
@@ -137,8 +138,8 @@ class GPTDecoder:
         if last is not None:
             x, resid = x.index_select(0, last), resid.index_select(0, last)
         y, _, _, _ = m._norm_fwd(x, "norm_f", residual=resid)
-        if waits is not None:
-            y = y.masked_fill(waits, 0.0)
+        if by_place:
+            y = ew.embedding_forward(self._row_of_place, y)
         logits = gemm_ops.gemm(y, m.p["embed.weight"])
         # only now does the step take effect: a call that failed before appended nothing, and what it wrote to the table and the pages is written anew
         self.lengths.copy_(step.lengths)
