@@ -26,7 +26,8 @@
 // Queries are scaled by a power of two per row to use fp16's range.  The softmax runs over x + b instead of x (b: the page's value
 // exponent): the weights exp2(x + b - M) are those that multiply the codes, and the sum takes exp2(-b) back out.  M is not the running
 // maximum but some number that no x + b exceeds by more than 6: it moves, and the outputs with it, in the first unit and rarely after, and the
-// weights, times 2^9, stay below 2^15.
+// weights, times 2^9, stay below 2^15.  What lies 2^126 below is flushed: with value scales of one sequence up to 2^98 apart that takes no weight
+// above 2^-28 of the largest (scales further apart: values of 10^14 next to pages of zeros).
 //
 // Blocks: four warps for the softmax, one that copies keys (a tiled copy per page and unit) and issues scores, one that copies values, one that
 // issues the products with them, one that prepares the queries of the next item, so that a run's items follow one another without a pause: with that in the
@@ -733,9 +734,20 @@ int item_rows(long long max_queries, int group) {
 // Blocks that run at once: two to an SM, one where the products take all columns of tensor memory.
 int runs_of(int rows, int dim) { return st::sm_count() * (rows == kPromptRows ? 1 : dim == 64 && rows == 32 ? Layout<64, 32, 4>::BLOCKS : Layout<128, 32, 4>::BLOCKS); }
 
-// Whether items of sequences of up to `tokens` tokens are whole: a unit takes a block 1000 cycles, of 32 rows 2500, of 128 rows 3200, the second kernel and what it
-// waits for 6 us of the GPU and 4 of the host.  One prompt of 777 tokens: 22 us split, 18 whole; 8 sequences of 128 tokens at 1024: 28 and 21; the limits are
-// where a single sequence loses no more by it than that.
+// Whether items of sequences of up to `tokens` tokens are whole: then no second kernel is launched (4 us of the host) and no parts pass through the
+// workspace.  Split ones share the chip evenly.  Device us, whole and split, 8 key heads of 128, every sequence as long as the table:
+//                          1 sequence       16             64 sequences
+//     8 rows,  7 units    13.2   13.1    15.3   18.0    30.6   36.5
+//             14          19.6   12.8    21.1   21.0    47.0   51.9
+//    16 rows,  7          21.4   16.3    23.5   26.7    45.9   66.0
+//             14          30.9   18.2    33.3   32.1    67.4   87.8
+//    32 rows,  7          29.9   21.3    31.2   43.6    77.3   95.8
+//             18          53.5   23.1    56.8   61.1   153.6  159.6
+//   128 rows, 12          31.9   19.8    33.0   45.8   127.3  130.6
+//             18          41.8   21.3    44.2   58.1   175.3  172.9
+// The limits are for the 16, which fill part of the chip: there whole items gain up to them.  A single sequence loses by them, 30 us at 18 units of 32 rows (with
+// the host's part 55 and 26 us), and so do lengths that differ (64 sequences of 300 to 2304 tokens, 32 rows: 137 and 115); the shapes that the host knows
+// tell neither the lengths nor, where the workspace is sized, how many sequences there are.
 bool not_split(int rows, long long tokens) { return tokens <= (rows == 32 ? 18 : rows == kPromptRows ? 12 : 7) * kTile; }
 
 template <typename T, int D, int R>

@@ -32,8 +32,10 @@ struct AttnParams {
   unsigned* err;
 };
 
-// What the beginning and the end of an item cost, in units: 5000 cycles of about 2300, with 32 rows 20000 of 4500; with 128 rows of those tried (4 sequences of 256
-// tokens: 3 units 40.0 us, 5 40.9, 8 43.7, 12 46.4).
+// What the beginning and the end of an item count, in units.  Of a block alone on its SM (one sequence, one key head of 128, whole; from 4 to 20 units, less
+// 2.5 us of a launch) they take 8000 cycles with 8 rows, 20000 with 16, 23000 with 32 and 18000 with 128, and a unit 1600, 2300, 4000 and 3300; where two
+// blocks share an SM a unit takes 2100, 3300 and 6800.  That is a run's first item; later ones begin beside the end of the one before.  With 128 rows
+// of those tried: 4 sequences of 256 tokens behind up to 4000, 3 units 40.0 us, 5 40.9, 8 43.7, 12 46.4.  16 rows count as 8 do.
 template <int N> constexpr int kItemCost = N == 128 ? 3 : N == 32 ? 4 : 2;
 
 struct Seq {

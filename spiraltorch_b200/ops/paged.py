@@ -257,7 +257,7 @@ def _store_reference(k, v, pages, slots) -> None:
 
 def read(pages: Pages, table: torch.Tensor, lengths: torch.Tensor, max_length: int, dtype: torch.dtype = torch.bfloat16):
     """``(k, v)`` ``[B, max_length, kv_heads, dim]``: what the cache holds of the first ``max_length`` tokens of every sequence (exact, in bf16
-    or fp32), zeros at and behind its length; the dense form that ``ops.attention`` takes."""
+    or fp32), zeros at and behind its length; the dense form that ``ops.attention`` takes.  A page number that is none: as in :func:`attention`, and zeros."""
     global launch_count
     P, H, page, D = _check_pages(pages)
     _ints("table", table, 2)
@@ -307,14 +307,17 @@ def attention(q: torch.Tensor, pages: Pages, table: torch.Tensor, starts: torch.
               scale: Optional[float] = None, out: Optional[torch.Tensor] = None, return_lse: bool = False):
     """Attention of the newest tokens of every sequence over what the cache holds of it (these tokens included).
 
-    ``q`` ``[rows, heads, dim]`` (bf16 or fp16, dim contiguous, any other strides), ``heads`` a multiple of the cache's key heads: query head ``h`` reads key head
+    ``q`` ``[rows, heads, dim]`` (bf16 or fp16, on the CPU also fp32; dim contiguous, any other strides), ``heads`` a multiple of the cache's key heads: query head ``h`` reads key head
     ``h // (heads / kv_heads)``.  Rows ``starts[b]`` to ``starts[b + 1]`` belong to sequence ``b``, whose ``lengths[b]`` tokens lie in the pages of ``table[b]``; the last
     row is its newest token, and a row sees the keys up to its own place, or all where not ``causal``.  A row that sees none is 0.
-    ``max_queries``: the most rows of one sequence; it decides the kernel's tile, not the result.  ``scale``: ``1 / sqrt(dim)`` if not given.
+    ``max_queries``: the most rows of one sequence; it decides the kernel's tile, not the result.  With more than 32 rows to a key head (tokens times the heads
+    that share it) all sequences get tiles of 128, which a single token leaves empty but for its own: 64 sequences of one token at 4096, 16 heads of 128, 172 us, with a
+    part of 256 tokens among them 497, in two calls (parts of ``starts``, ``table``, ``lengths``) 209.  ``scale``: ``1 / sqrt(dim)`` if not given.
 
     Returns ``o`` like ``q`` (contiguous, or ``out``), with ``return_lse`` also the log-sum-exp of every row's scores, fp32 ``[rows, heads]``.  Rows of no
-    sequence, before ``starts[0]`` and behind the last one, are 0 (lse -inf); in a given ``out``, which may be ``q`` itself, they stay as they were.  Not differentiable.  Whole causal
-    prompts of 2000 tokens and more run faster over :func:`read` and ``ops.attention``."""
+    sequence, before ``starts[0]`` and behind the last one, are 0 (lse -inf); in a given ``out``, which may be ``q`` itself, they stay as they were.  Softmax
+    weights are rounded to fp16, sums and products are fp32.  A page number that is none raises on the CPU; the kernels pass its keys over and leave an error record
+    (:func:`native.poll`).  Not differentiable.  Whole causal prompts of 2000 tokens and more run faster over :func:`read` and ``ops.attention``."""
     global launch_count
     P, Hk, page, D = _check_pages(pages)
     if q.dim() != 3 or q.shape[2] != D or q.shape[1] < Hk or q.shape[1] % Hk:
