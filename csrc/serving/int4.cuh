@@ -1,0 +1,47 @@
+// Weights of four bits: the layout that the kernels share.
+//
+// A matrix [rows, cols] is cut into tiles of 16 rows by 64 columns.  Tile (u, c) takes 512 bytes, 16 for each lane of a warp: word s (columns 16 s to
+// 16 s + 15) of lane 4 g + t holds, in its nibbles e and e + 4, the codes of columns k and k + 1 of row g (e = 0: k = 2 t; e = 2: k = 2 t + 8) and of row
+// g + 8 (e = 1, 3).  That is the order in which a warp's matrix instruction takes a 16 x 16 operand, and in which tensor memory is written from
+// registers, so one 16-byte load per lane is an operand of four steps and nothing is exchanged between lanes.  Tiles of one u follow one another.
+// Scales: [u][group][16] bf16, those of rows g and g + 8 next to one another.  What lies behind the last row or column is code 8 (zero).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+namespace st4 {
+
+constexpr int kTileRows = 16, kTileCols = 64, kTileBytes = 512;
+
+template <typename T> __device__ __forceinline__ float to_float(T x);
+template <> __device__ __forceinline__ float to_float(float x) { return x; }
+template <> __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float(float x) { return x; }
+template <> __device__ __forceinline__ __half from_float(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float(float x) { return __float2bfloat16_rn(x); }
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Vec {
+  T v[N];
+};
+
+__device__ __forceinline__ float bf16_bits(uint32_t low16) { return __uint_as_float(low16 << 16); }
+
+// Nibbles e and e + 4 of a word as two numbers -8..7, exactly: the nibble is put into the low bits of 128 (bf16) or 1024 (fp16), where a unit is 1, and
+// 136 or 1032 is subtracted.
+template <typename T> __device__ __forceinline__ uint32_t codes_to_pair(uint32_t word, int e);
+template <> __device__ __forceinline__ uint32_t codes_to_pair<__nv_bfloat16>(uint32_t word, int e) {
+  const uint32_t v = ((word >> (4 * e)) & 0x000F000Fu) | 0x43004300u;
+  const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __nv_bfloat162(__float2bfloat16_rn(136.0f), __float2bfloat16_rn(136.0f)));
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
+template <> __device__ __forceinline__ uint32_t codes_to_pair<__half>(uint32_t word, int e) {
+  const uint32_t v = ((word >> (4 * e)) & 0x000F000Fu) | 0x64006400u;
+  const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v), __half2(__float2half_rn(1032.0f), __float2half_rn(1032.0f)));
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
+
+}  // namespace st4

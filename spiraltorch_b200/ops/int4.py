@@ -1,0 +1,257 @@
+"""Weights of four bits and products with them (``csrc/serving/int4_weights.cu``, ``csrc/serving/int4_linear.cu``).
+
+A matrix ``[out, in]`` is held as ``q * s``: a code ``-8 <= q <= 7`` per weight and a scale per row and group of 32, 64 or 128 inputs.
+
+    held = quantize(weight, group=64)              # once, and again after an update
+    y = linear(x, held, bias, act="gelu")          # any number of rows, from one token's to a prompt's
+    weight = dequantize(held, torch.bfloat16)
+
+The scale is minus an eighth of the group's element of largest magnitude (the negative one of two), rounded to 4 significant bits (ties to even), its
+magnitude within ``2^-20`` and ``1.875 * 2^12``; the code is the weight over the scale, rounded to the nearest (ties to even) and clamped.  Every ``q * s`` is a
+bf16 and an fp16 number, so all kernels, and ``dequantize`` in any type, work with the same weights.  A group with a NaN or an infinity is NaN.
+
+CPU tensors use a plain PyTorch statement of the same (also the test oracle).  The reference has no weights of fewer than 8 bits.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import native
+from .gemm import gelu_tanh
+
+launch_count = 0
+GROUPS = (32, 64, 128)
+LEAST_SCALE, LARGEST_SCALE = 2.0 ** -20, 1.875 * 2.0 ** 12
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_ACTS = {None: 0, "relu": 1, "gelu": 2}
+
+
+class Weights(NamedTuple):
+    """``codes`` uint8 ``[tiles down, tiles across, 512]`` (16 rows by 64 columns each, in the order of the kernels), ``scales`` bf16 ``[tiles down, groups, 16]``;
+    the matrix's ``out_features`` and ``in_features``, and the inputs to a scale."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    out_features: int
+    in_features: int
+    group: int
+
+    @classmethod
+    def allocate(cls, out_features: int, in_features: int, group: int = 64, device="cuda") -> "Weights":
+        """Room for :func:`quantize` to write to."""
+        if group not in GROUPS:
+            raise ValueError(f"int4: groups of {GROUPS} inputs, got {group}")
+        if not (0 < out_features <= 1 << 30 and 0 < in_features <= 1 << 30):
+            raise ValueError(f"int4: a matrix of {out_features} x {in_features} is not supported")
+        down = -(-out_features // 16)
+        return cls(torch.empty((down, -(-in_features // 64), 512), dtype=torch.uint8, device=device),
+                   torch.empty((down, -(-in_features // group), 16), dtype=torch.bfloat16, device=device), out_features, in_features, group)
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.nbytes + self.scales.nbytes
+
+    def to(self, device) -> "Weights":
+        return self._replace(codes=self.codes.to(device), scales=self.scales.to(device))
+
+
+def _check(w: Weights, what: str) -> None:
+    codes, scales, n, k, group = w
+    if group not in GROUPS or codes.dtype is not torch.uint8 or scales.dtype is not torch.bfloat16 or not codes.is_contiguous() or not scales.is_contiguous() \
+            or codes.shape != (-(-n // 16), -(-k // 64), 512) or scales.shape != (-(-n // 16), -(-k // group), 16):
+        raise ValueError(f"{what}: codes {codes.dtype} {tuple(codes.shape)} and scales {scales.dtype} {tuple(scales.shape)} are no weights of {n} x {k} in groups of {group}")
+
+
+# ---- plain statement ------------------------------------------------------------------------------------------------------------
+def quantize_reference(weight: torch.Tensor, group: int):
+    """Codes ``[out, in]`` int8 and scales ``[out, groups]`` fp32."""
+    n, k = weight.shape
+    g = torch.nn.functional.pad(weight.double(), (0, -k % group)).unflatten(1, (-1, group))
+    low, high = g.amin(-1), g.amax(-1)
+    m, e = torch.frexp(torch.where(high > -low, high, low) * -0.125)
+    s = torch.ldexp(torch.round(m * 16), e - 4)
+    s = torch.where(s < 0, -1.0, 1.0) * s.abs().clamp(LEAST_SCALE, LARGEST_SCALE)
+    s = torch.where(g.isfinite().all(-1), s, float("nan"))
+    q = torch.round(g / s[..., None]).clamp(-8, 7).nan_to_num(nan=-8.0)
+    return q.flatten(1)[:, :k].to(torch.int8), s.float()
+
+
+def _tiles(q: torch.Tensor) -> torch.Tensor:
+    """Codes ``[out, in]`` in the order of the kernels: see ``csrc/serving/int4.cuh``."""
+    n, k = q.shape
+    v = torch.nn.functional.pad(q.to(torch.int16) + 8, (0, -k % 64, 0, -n % 16), value=8)
+    # [down, half of the rows, g, across, word, half of the columns, t, parity]
+    v = v.view(-(-n // 16), 2, 8, -(-k // 64), 4, 2, 4, 2)
+    v = v.permute(0, 3, 2, 6, 4, 7, 5, 1)      # [down, across, g, t, word, parity (nibbles 0-3, 4-7), column half, row half]
+    v = v.flatten(-2)                          # nibble e = 2 * column half + row half
+    v = v.flatten(-2).unflatten(-1, (4, 2))    # bytes of two nibbles, the lower first
+    return (v[..., 0] | v[..., 1] << 4).to(torch.uint8).reshape(v.shape[0], v.shape[1], 512)
+
+
+def _untile(codes: torch.Tensor, n: int, k: int) -> torch.Tensor:
+    b = codes.to(torch.int16)
+    v = torch.stack([b & 15, b >> 4], -1).view(codes.shape[0], codes.shape[1], 8, 4, 4, 2, 2, 2)
+    v = v.permute(0, 7, 2, 1, 4, 6, 3, 5)
+    return (v.reshape(codes.shape[0] * 16, codes.shape[1] * 64) - 8)[:n, :k].to(torch.int8)
+
+
+def _row_scales(w: Weights) -> torch.Tensor:
+    """``[out, groups]`` fp32."""
+    s = w.scales.unflatten(-1, (8, 2)).permute(0, 3, 2, 1)
+    return s.reshape(-1, w.scales.shape[1])[:w.out_features].float()
+
+
+def dequantize_reference(w: Weights, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    s = _row_scales(w).to(torch.float64 if dtype == torch.float64 else torch.float32).repeat_interleave(w.group, 1)[:, :w.in_features]
+    return (_untile(w.codes, w.out_features, w.in_features).to(s.dtype) * s).to(dtype)
+
+
+def linear_reference(x, weight, bias=None, act=None, residual=None):
+    """``weight`` ``[out, in]``: sums in fp32 (fp64 for fp64 ``x``), rounded once."""
+    t = torch.float64 if x.dtype == torch.float64 else torch.float32
+    y = x.to(t) @ weight.to(t).T
+    if bias is not None:
+        y = y + bias.to(t)
+    y = torch.relu(y) if act == "relu" else gelu_tanh(y) if act == "gelu" else y
+    return (y if residual is None else y + residual.to(t)).to(x.dtype)
+
+
+# ---- quantising -----------------------------------------------------------------------------------------------------------------
+def quantize(weight: torch.Tensor, group: int = 64, *, out: Optional[Weights] = None) -> Weights:
+    """``weight`` ``[out, in]`` in bf16, fp16 or fp32 (rows may be strided) in four bits; ``out``: written to instead of new memory, as after
+    an update of weights that a captured step holds."""
+    global launch_count
+    if weight.dim() != 2 or weight.dtype not in _TYPES and not (weight.dtype == torch.float64 and not weight.is_cuda):
+        raise ValueError(f"int4.quantize: a bf16, fp16 or fp32 matrix, got {weight.dtype} {tuple(weight.shape)}")
+    if group not in GROUPS:
+        raise ValueError(f"int4.quantize: groups of {GROUPS} inputs, got {group}")
+    n, k = weight.shape
+    if out is None:
+        out = Weights.allocate(n, k, group, weight.device)
+    else:
+        _check(out, "int4.quantize")
+        if out[2:] != (n, k, group):
+            raise ValueError(f"int4.quantize: a {n} x {k} matrix in groups of {group} into weights of {out.out_features} x {out.in_features} in groups of {out.group}")
+        native.same_device("int4.quantize", weight, out.codes, out.scales)
+    weight = weight.detach()
+    if not native.use_native(weight):
+        q, s = quantize_reference(weight, group)
+        out.codes.copy_(_tiles(q))
+        s = torch.nn.functional.pad(s, (0, 0, 0, -n % 16), value=LEAST_SCALE)
+        out.scales.copy_(s.view(-1, 2, 8, s.shape[1]).permute(0, 3, 2, 1).flatten(-2))
+        return out
+    if weight.stride(1) != 1 and k > 1:
+        weight = weight.contiguous()
+    index = native.require_cuda("int4.quantize", weight, out.codes, out.scales)
+    with native.on_device(index):
+        st = native.entry("st_int4_quantize", "pppiiqiip")(weight.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), n, k, weight.stride(0), group,
+                                                         _TYPES[weight.dtype], native.raw_stream(index))
+    native.check(st, "st_int4_quantize")
+    launch_count += 1
+    return out
+
+
+def dequantize(w: Weights, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``[out, in]`` in bf16, fp16 or fp32: the same numbers in each."""
+    global launch_count
+    _check(w, "int4.dequantize")
+    if not native.use_native(w.codes):
+        return dequantize_reference(w, dtype)
+    if dtype not in _TYPES:
+        raise ValueError(f"int4.dequantize: bf16, fp16 or fp32, got {dtype}")
+    index = native.require_cuda("int4.dequantize", w.codes, w.scales)
+    y = torch.empty((w.out_features, w.in_features), dtype=dtype, device=w.codes.device)
+    with native.on_device(index):
+        st = native.entry("st_int4_dequantize", "pppiiqiip")(w.codes.data_ptr(), w.scales.data_ptr(), y.data_ptr(), w.out_features, w.in_features, w.in_features,
+                                                           w.group, _TYPES[dtype], native.raw_stream(index))
+    native.check(st, "st_int4_dequantize")
+    launch_count += 1
+    return y
+
+
+# ---- products -------------------------------------------------------------------------------------------------------------------
+def _product(x2, w, bias, act, residual2):
+    """``[rows, in]`` to ``[rows, out]``."""
+    global launch_count
+    if not native.use_native(x2):
+        return linear_reference(x2, dequantize_reference(w, x2.dtype if x2.dtype == torch.float64 else torch.float32), bias, act, residual2)
+    if x2.stride(1) != 1 and x2.shape[1] > 1:
+        x2 = x2.contiguous()
+    if residual2 is not None and residual2.stride(1) != 1 and residual2.shape[1] > 1:
+        residual2 = residual2.contiguous()
+    if bias is not None and bias.stride(0) != 1 and bias.shape[0] > 1:
+        bias = bias.contiguous()
+    index = native.require_cuda("int4.linear", x2, w.codes, w.scales, bias, residual2)
+    rows = x2.shape[0]
+    y = x2.new_empty((rows, w.out_features))
+    if rows == 0:
+        return y
+    with native.on_device(index):
+        st = native.entry("st_int4_linear", "ppppppiiiqqqiiip")(
+            x2.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), native.address(bias), native.address(residual2), y.data_ptr(), rows, w.out_features,
+            w.in_features, x2.stride(0), 0 if residual2 is None else residual2.stride(0), w.out_features, w.group, _ACTS[act], _TYPES[x2.dtype], native.raw_stream(index))
+    native.check(st, "st_int4_linear")
+    launch_count += 1
+    return y
+
+
+def _input_gradient(dy2, w):
+    """``[rows, out]`` to ``[rows, in]``: ``dy W``."""
+    if not native.use_native(dy2):
+        t = torch.float64 if dy2.dtype == torch.float64 else torch.float32
+        return (dy2.to(t) @ dequantize_reference(w, t)).to(dy2.dtype)
+    from .gemm import gemm
+    dense = dequantize(w, torch.bfloat16)
+    if dy2.dtype == torch.bfloat16:
+        return gemm(dy2, dense, b_mn=True)
+    # an fp16 number is the sum of two bf16 numbers where the second is no smaller than they get
+    high = dy2.to(torch.bfloat16)
+    low = (dy2.float() - high.float()).to(torch.bfloat16)
+    out = gemm(high, dense, b_mn=True, out_dtype=torch.float32)
+    return gemm(low, dense, b_mn=True, out=out, accumulate=True).to(dy2.dtype)
+
+
+class _LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, bias, residual, w):
+        ctx.w, ctx.x_shape = w, x.shape
+        y = _product(x.reshape(-1, x.shape[-1]), w, bias, None, None if residual is None else residual.reshape(-1, w.out_features))
+        return y.view(*x.shape[:-1], w.out_features)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        need_x, need_bias, need_residual, _ = ctx.needs_input_grad
+        dy2 = dy.reshape(-1, ctx.w.out_features)
+        dx = _input_gradient(dy2.contiguous(), ctx.w).view(ctx.x_shape) if need_x else None
+        db = dy2.sum(0, dtype=torch.float64 if dy.dtype == torch.float64 else torch.float32).to(dy.dtype) if need_bias else None
+        return dx, db, dy if need_residual else None, None
+
+
+def linear(x: torch.Tensor, w: Weights, bias: Optional[torch.Tensor] = None, *, act: Optional[str] = None,
+           residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``act(x W^T + bias) + residual``: ``x`` ``[..., in]`` in bf16 or fp16, ``bias`` ``[out]`` and ``residual`` ``[..., out]`` of the same type, ``act`` None, ``"relu"``
+    or ``"gelu"`` (tanh form).  Sums are in fp32; the result, in ``x``'s type, is rounded once.
+
+    Differentiable in ``x``, ``bias`` and ``residual`` (the weights are constants) without ``act``: apply an activation to the result where gradients are needed."""
+    _check(w, "int4.linear")
+    if act not in _ACTS:
+        raise ValueError(f"int4.linear: act must be None, 'relu' or 'gelu', got {act!r}")
+    if x.dtype not in (torch.bfloat16, torch.float16) and (x.is_cuda or x.dtype not in (torch.float32, torch.float64)):
+        raise ValueError(f"int4.linear: bf16 and fp16 tensors, got {x.dtype}")
+    shape = (*x.shape[:-1], w.out_features)
+    if x.dim() == 0 or x.shape[-1] != w.in_features:
+        raise ValueError(f"int4.linear: x {tuple(x.shape)} does not end in the weights' {w.in_features} inputs")
+    for name, t, want in (("bias", bias, (w.out_features,)), ("residual", residual, shape)):
+        if t is not None and (t.shape != want or t.dtype != x.dtype):
+            raise ValueError(f"int4.linear: {name} must be {x.dtype} {tuple(want)}, got {t.dtype} {tuple(t.shape)}")
+    native.same_device("int4.linear", x, w.codes, w.scales, bias, residual)
+    if native.has_tangent(x, bias, residual):
+        raise ValueError("int4.linear: forward-mode differentiation is not supported")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, bias, residual)):
+        if act is not None:
+            raise ValueError("int4.linear: act with tensors that require gradients; apply it to the result")
+        return _LinearFn.apply(x, bias, residual, w)
+    y = _product(x.reshape(-1, w.in_features), w, bias, act, None if residual is None else residual.reshape(-1, w.out_features))
+    return y.view(shape)

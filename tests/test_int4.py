@@ -1,0 +1,303 @@
+"""Weights of four bits: quantising against the definition element by element in 64 bits, products against 64 bits at odd sizes, strides and types, gradients
+against the formula and against differences, refusals.
+
+Quantising is exact: codes, scales and what they stand for are compared for equality.  Tolerance of a product: the numbers that enter are exact, each of at
+most in/16 + 40 additions that follow one another in fp32 (a matrix instruction's of 16 columns as one) is off by at most 2^-22 of the sum of magnitudes A = |x| |W|^T
+(an instruction may cut off instead of rounding, and adds up 16 columns inside), and the result is rounded once, half a step.  An activation is 1-Lipschitz but for gelu's 1.13
+and computes within 2^-20 of its argument."""
+import math
+
+import pytest
+import torch
+
+from spiraltorch_b200.ops import int4
+
+GPU = pytest.mark.gpu
+cuda = torch.device("cuda")
+
+
+def _by_hand(w, group):
+    """Codes and scales of a matrix by Python's own arithmetic."""
+    from fractions import Fraction
+    n, k = w.shape
+    codes, scales = [], []
+    for r in range(n):
+        row, crow, srow = [Fraction(float(v)) for v in w[r]], [], []
+        for i in range(0, k, group):
+            part = row[i:i + group]
+            far = max(part, key=lambda v: (abs(v), -v))      # the negative one of two
+            size = abs(far) / 8
+            if size:
+                e = math.floor(math.log2(float(size)))
+                unit = Fraction(2) ** (e - 3)
+                while size / unit >= 16:
+                    unit *= 2
+                while size / unit < 8:
+                    unit /= 2
+                size = round(size / unit) * unit             # Python rounds ties to even
+            size = min(max(size, Fraction(2) ** -20), Fraction(7680))
+            s = -size if far > 0 else size
+            srow.append(float(s))
+            crow += [min(max(round(v / s), -8), 7) for v in part]
+        codes.append(crow)
+        scales.append(srow)
+    return torch.tensor(codes, dtype=torch.int8), torch.tensor(scales, dtype=torch.float32)
+
+
+def _matrix(n, k, dtype, seed=0, device="cpu"):
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randn(n, k, generator=g) * torch.exp(torch.randn(n, 1, generator=g))
+    return w.to(dtype).to(device)
+
+
+def _hard(group):
+    """Rows of borders: all zero, ties of codes and scales, equal extrema of both signs, tiny, huge and subnormal elements."""
+    rows = []
+    for s in (0.5, 9 * 2.0 ** -7, 15 * 2.0 ** -6, -11 * 2.0 ** -5):
+        rows.append(torch.tensor([s * (i % 17 - 8) / 1.0 * 0.5 for i in range(group)] + [s * (i % 16 - 8 + 0.5) for i in range(group)]))
+    rows += [torch.zeros(2 * group), torch.cat([torch.full((group,), 3.0), torch.full((group,), -3.0)]),
+             torch.tensor([3.0, -3.0] * group), torch.full((2 * group,), 2.0 ** -24), torch.tensor([1e5, -1.0] * group), torch.tensor([-7e4, 5e4] * group)]
+    for m in (8.5, 9.5, 15.5, 15.75, 8.0, 17.0):      # scales on and beside a tie of 4 bits
+        rows.append(torch.tensor([m, -m / 2] * group) * 2.0 ** -3)
+        rows.append(torch.tensor([-m * (1 + 2.0 ** -23), m / 3] * group))
+    return torch.stack(rows)
+
+
+@pytest.mark.parametrize("group", int4.GROUPS)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 31), (17, 65), (16, 128), (5, 200)])
+def test_quantize_statement_is_the_definition(shape, group):
+    w = _matrix(*shape, torch.float32)
+    codes, scales = _by_hand(w, group)
+    q, s = int4.quantize_reference(w, group)
+    assert torch.equal(q, codes) and torch.equal(s, scales)
+    held = int4.quantize(w, group)
+    want = codes.double() * scales.double().repeat_interleave(group, 1)[:, :shape[1]]
+    for t in (torch.float64, torch.float32, torch.bfloat16, torch.float16):
+        assert torch.equal(int4.dequantize(held, t).double(), want)
+
+
+@pytest.mark.parametrize("group", int4.GROUPS)
+def test_quantize_statement_at_borders(group):
+    w = _hard(group)
+    codes, scales = _by_hand(w, group)
+    q, s = int4.quantize_reference(w, group)
+    assert torch.equal(q, codes) and torch.equal(s, scales)
+
+
+def test_quantize_error_bound_and_non_finite():
+    w = _matrix(64, 256, torch.float32, 3)
+    held = int4.quantize(w, 64)
+    s = int4._row_scales(held).abs().repeat_interleave(64, 1)
+    assert ((int4.dequantize(held, torch.float32) - w).abs() <= 1.5 * s).all()      # half a step, and a step where the side of the extremum's opposite ends at 7
+    for bad in (math.nan, math.inf, -math.inf):
+        v = w.clone()
+        v[5, 70] = bad
+        d = int4.dequantize(int4.quantize(v, 64), torch.float32)
+        assert d[5, 64:128].isnan().all() and d.isnan().sum() == 64
+
+
+def test_tiles_are_in_the_order_of_the_matrix_instruction():
+    q = torch.randint(-8, 8, (33, 130), generator=torch.Generator().manual_seed(1), dtype=torch.int8)
+    tiles = int4._tiles(q)
+    assert tiles.shape == (3, 3, 512) and torch.equal(int4._untile(tiles, 33, 130), q)
+    word = tiles.view(torch.int32)[1, 1].view(32, 4)
+    for lane in range(32):
+        for s in range(4):
+            for e in range(4):
+                r, k = 16 + lane // 4 + 8 * (e & 1), 64 + 16 * s + 2 * (lane % 4) + 8 * (e >> 1)
+                assert (int(word[lane, s]) >> (4 * e) & 15) - 8 == q[r, k] and (int(word[lane, s]) >> (4 * e + 16) & 15) - 8 == q[r, k + 1]
+
+
+def test_linear_statement_and_gradients():
+    g = torch.Generator().manual_seed(2)
+    held = int4.quantize(_matrix(7, 45, torch.float32), 32)
+    w = int4.dequantize(held, torch.float64)
+    x, b, r = (torch.randn(s, generator=g, dtype=torch.float64, requires_grad=True) for s in ((2, 3, 45), (7,), (2, 3, 7)))
+    y = int4.linear(x, held, b, residual=r)
+    assert torch.allclose(y, x @ w.T + b + r, atol=1e-12)
+    dy = torch.randn(y.shape, generator=g, dtype=torch.float64)
+    dx, db, dr = torch.autograd.grad(y, (x, b, r), dy)
+    assert torch.allclose(dx, dy @ w, atol=1e-12) and torch.allclose(db, dy.sum((0, 1)), atol=1e-12) and torch.equal(dr, dy)
+    assert torch.autograd.gradcheck(lambda x, b, r: int4.linear(x, held, b, residual=r), (x, b, r))
+    with torch.no_grad():
+        assert torch.equal(int4.linear(x, held, act="relu"), torch.relu(x @ w.T))
+        assert torch.allclose(int4.linear(x, held, b, act="gelu", residual=r), torch.nn.functional.gelu(x @ w.T + b, approximate="tanh") + r, atol=1e-12)
+        assert int4.linear(x[0, 0], held).shape == (7,) and int4.linear(x[:0], held).shape == (0, 3, 7)
+
+
+def test_refusals():
+    w = _matrix(20, 70, torch.float32)
+    held = int4.quantize(w, 32)
+    x = torch.randn(3, 70)
+    for call in (lambda: int4.quantize(w, 48), lambda: int4.quantize(w[0]), lambda: int4.quantize(w.int()), lambda: int4.quantize(w, 64, out=held),
+                 lambda: int4.quantize(w[:, :64], 32, out=held), lambda: int4.Weights.allocate(0, 4), lambda: int4.Weights.allocate(4, 4, 16),
+                 lambda: int4.linear(x[:, :69], held), lambda: int4.linear(x, held, torch.zeros(21)), lambda: int4.linear(x, held, torch.zeros(20).half()),
+                 lambda: int4.linear(x, held, residual=torch.zeros(2, 20)), lambda: int4.linear(x, held, act="tanh"), lambda: int4.linear(x.int(), held),
+                 lambda: int4.linear(x, held._replace(in_features=140)), lambda: int4.dequantize(held._replace(group=64)),
+                 lambda: int4.linear(x.clone().requires_grad_(), held, act="gelu"), lambda: int4.linear(torch.tensor(1.0), held)):
+        with pytest.raises(ValueError):
+            call()
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(ValueError):
+            int4.linear(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)), held)
+
+
+# ---- kernels --------------------------------------------------------------------------------------------------------------------
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+@GPU
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group", int4.GROUPS)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 31), (16, 128), (17, 65), (37, 200), (130, 777), (64, 2048)])
+def test_quantize_kernel(shape, group, dtype):
+    w = _matrix(*shape, dtype)
+    want = int4.quantize(w, group)
+    got = int4.quantize(w.to(cuda), group)
+    assert torch.equal(got.codes.cpu(), want.codes) and torch.equal(got.scales.cpu(), want.scales)
+    for t in DTYPES:
+        d = int4.dequantize(got, t)
+        assert d.dtype == t and torch.equal(d.float().cpu(), int4.dequantize_reference(want))
+
+
+@GPU
+@pytest.mark.parametrize("group", int4.GROUPS)
+def test_quantize_kernel_at_borders_and_strides(group):
+    w = _hard(group)
+    w[2, 3], w[4, 0], w[5, 1] = math.nan, math.inf, -math.inf
+    codes, scales = int4.quantize_reference(w, group)
+    got = int4.quantize(w.to(cuda), group)
+    fine = torch.isfinite(scales)
+    keep = fine.repeat_interleave(group, 1)
+    assert torch.equal(int4._untile(got.codes.cpu(), *w.shape)[keep], codes[keep])
+    s = int4._row_scales(got).cpu()
+    assert torch.equal(s[fine], scales[fine]) and s[~fine].isnan().all()
+    # a view at an odd place of a wider matrix, a transposed one, and memory that is written to again
+    wide = torch.randn(50, 201, generator=torch.Generator().manual_seed(4)).to(cuda)
+    for view in (wide[3:40, 5:190], wide[:, :200], wide.T, wide[:, ::2]):
+        want = int4.quantize(view.cpu().contiguous(), group)
+        got = int4.quantize(view, group)
+        assert torch.equal(got.codes.cpu(), want.codes) and torch.equal(got.scales.cpu(), want.scales)
+        again = int4.quantize(view * 2, group, out=got)
+        assert again is got and torch.equal(int4.dequantize(got, torch.float32).cpu(), 2 * int4.dequantize(want, torch.float32))
+
+
+def _allowed(x, w, y, dtype, act=None):
+    a = x.abs() @ w.abs().T
+    return torch.finfo(dtype).eps / 2 * (y.abs() + torch.finfo(dtype).smallest_normal) + 1.13 * (x.shape[1] / 16 + 40) * 2.0 ** -22 * (a + 1.0)
+
+
+def _product_case(rows, n, k, group, dtype, bias, act, residual, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    held = int4.quantize(_matrix(n, k, torch.float32, seed).to(cuda) * 0.1, group)
+    x = torch.randn(rows, k, generator=g).to(dtype).to(cuda)
+    b = torch.randn(n, generator=g).to(dtype).to(cuda) if bias else None
+    r = torch.randn(rows, n, generator=g).to(dtype).to(cuda) if residual else None
+    w = int4.dequantize(held, torch.float32).double()
+    y = x.double() @ w.T
+    if bias:
+        y = y + b.double()
+    y = torch.relu(y) if act == "relu" else torch.nn.functional.gelu(y, approximate="tanh") if act == "gelu" else y
+    if residual:
+        y = y + r.double()
+    return held, x, b, r, w, y
+
+
+ROWS = [1, 2, 7, 8, 9, 16, 17, 33, 64, 100, 129, 300]
+
+
+@GPU
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("n,k,group", [(1, 1, 32), (16, 64, 64), (37, 100, 32), (130, 129, 128), (300, 777, 64), (257, 2048, 128), (64, 4160, 32)])
+def test_linear_kernel(rows, n, k, group):
+    for dtype, bias, act, residual in ((torch.bfloat16, False, None, False), (torch.float16, True, "relu", True), (torch.bfloat16, True, "gelu", True)):
+        held, x, b, r, w, y = _product_case(rows, n, k, group, dtype, bias, act, residual, rows + n)
+        got = int4.linear(x, held, b, act=act, residual=r)
+        assert got.dtype == dtype and got.shape == y.shape
+        assert ((got.double() - y).abs() <= _allowed(x.double(), w, y, dtype)).all()
+
+
+@GPU
+@pytest.mark.parametrize("rows", [1, 5, 16, 40, 200])
+def test_linear_views_and_places(rows):
+    held, x, b, r, w, _ = _product_case(rows, 150, 328, 64, torch.bfloat16, True, None, True)
+    for pad, at in ((0, 0), (8, 8), (3, 1), (2, 2), (7, 0)):
+        wide = torch.full((rows, 328 + pad), math.nan, dtype=x.dtype, device=cuda)
+        xv = wide[:, at:at + 328] if at + 328 <= wide.shape[1] else wide[:, :328]
+        xv.copy_(x)
+        rv = torch.zeros(rows, 150 + pad, dtype=x.dtype, device=cuda)[:, :150]
+        rv.copy_(r)
+        assert torch.equal(int4.linear(xv, held, b, residual=rv), int4.linear(x, held, b, residual=r))
+    assert torch.equal(int4.linear(x.T.contiguous().T, held), int4.linear(x, held))
+    assert torch.equal(int4.linear(x.view(rows, 1, 328), held), int4.linear(x, held).view(rows, 1, 150))
+    one = x[:1].expand(rows, 328)
+    assert torch.equal(int4.linear(one, held), int4.linear(one.contiguous(), held))
+    assert torch.equal(int4.linear(x, held, b[:1].expand(150)), int4.linear(x, held, b[:1].expand(150).contiguous()))
+    # memory around the result stays as it was, rows of zero tokens launch nothing
+    assert int4.linear(x[:0], held).shape == (0, 150)
+
+
+@GPU
+@pytest.mark.parametrize("rows", [1, 12, 50, 200])
+def test_linear_non_finite_values_stay_in_their_rows(rows):
+    held, x, _, _, w, _ = _product_case(rows, 70, 200, 32, torch.bfloat16, False, None, False)
+    base = int4.linear(x, held)
+    x2 = x.clone()
+    x2[0, 150] = math.nan
+    got = int4.linear(x2, held)
+    assert got[0].isnan().all() and torch.equal(got[1:], base[1:])
+    v = w.float().clone()
+    v[33, 40] = math.inf
+    got = int4.linear(x, int4.quantize(v, 32))
+    assert got[:, 33].isnan().all() and not got[:, :33].isnan().any() and not got[:, 34:].isnan().any()
+
+
+@GPU
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,n,k,group", [(1, 16, 64, 64), (5, 37, 100, 32), (33, 300, 129, 128), (200, 130, 777, 64), (300, 520, 264, 32)])
+def test_linear_gradients(rows, n, k, group, dtype):
+    held, x, b, r, w, _ = _product_case(rows, n, k, group, dtype, True, None, True)
+    for t in (x, b, r):
+        t.requires_grad_(True)
+    y = int4.linear(x, held, b, residual=r)
+    dy = torch.randn(y.shape, generator=torch.Generator().manual_seed(5)).to(dtype).to(cuda)
+    dx, db, dr = torch.autograd.grad(y, (x, b, r), dy)
+    want = dy.double() @ w
+    assert ((dx.double() - want).abs() <= _allowed(dy.double(), w.T, want, dtype)).all()
+    assert torch.equal(dr, dy)
+    want = dy.double().sum(0)
+    assert ((db.double() - want).abs() <= torch.finfo(dtype).eps / 2 * want.abs() + rows * 2.0 ** -24 * dy.double().abs().sum(0)).all()
+    # a gradient that is one number for all, and the input alone
+    got = torch.autograd.grad(int4.linear(x, held).sum(), x)[0]
+    want = torch.ones_like(dy).double() @ w
+    assert ((got.double() - want).abs() <= _allowed(torch.ones_like(dy).double(), w.T, want, dtype)).all()
+
+
+@GPU
+def test_linear_streams_graphs_and_updates():
+    held, x, b, r, w, _ = _product_case(9, 130, 512, 64, torch.bfloat16, True, None, True)
+    want = int4.linear(x, held, b, residual=r)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = int4.linear(x, held, b, residual=r)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = int4.linear(x, held, b, act="gelu", residual=r)
+    new = _matrix(130, 512, torch.bfloat16, 8, cuda)
+    int4.quantize(new, 64, out=held)      # the replay multiplies by what the weights are now
+    x.copy_(torch.randn_like(x))
+    graph.replay()
+    assert torch.equal(y, int4.linear(x, held, b, act="gelu", residual=r))
+
+
+@GPU
+def test_kernel_refusals():
+    held = int4.quantize(torch.randn(20, 70, device=cuda), 32)
+    x = torch.randn(3, 70, device=cuda)
+    for call in (lambda: int4.linear(x, held), lambda: int4.linear(x.bfloat16().cpu(), held), lambda: int4.linear(x.bfloat16(), held, torch.zeros(20).bfloat16()),
+                 lambda: int4.dequantize(held, torch.float64), lambda: int4.quantize(torch.randn(20, 70), 32, out=held), lambda: int4.linear(x.bfloat16(), held.to("cpu"))):
+        with pytest.raises(ValueError):
+            call()
