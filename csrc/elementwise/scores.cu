@@ -1,0 +1,543 @@
+// Scores of given tokens: log probability, entropy of the distribution and the likeliest tokens, from logits in one pass, and the gradient.
+//
+//   m = max x,  S = sum e^(x - m),  T = sum e^(x - m) (x - m),  log p_j = x_j - m - log S,  entropy = log S - T / S
+//   dx_j = sum_i g_i [j = id_i] - p_j (sum_i g_i + g_entropy (log p_j + entropy)),  i over the given token and the likeliest ones
+//
+// Bound by memory: a row is read once (forward; the gradient reads it again and writes as much).  Every thread keeps m, S and T of what it has seen and
+// joins them at the end.  The likeliest tokens come from the same pass: the largest elements of the threads' first vectors give a bound that `top` elements
+// reach, and only what reaches it (a hundredth of a row) is set aside in shared memory.
+#include "../common/host.h"
+#include "../common/ptx.cuh"
+#include "../common/chain.cuh"
+#include <cuda_fp16.h>
+
+namespace {
+using st::chain_begin;
+
+constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kMostTop = 32;
+constexpr float kLog2e = 1.4426950408889634f, kLowest = -3.402823466e38f;
+constexpr float kMargin = 4.0f;       // how far an element may lie above a thread's m before that follows it: e^4 rows of S are far from overflow
+constexpr float kFar = -1.0e4f;       // of e^d d where d is -inf: the product is 0, not 0 times infinity
+
+struct ScoreParams {
+  long long row, rows;      // elements between rows
+  int vocab, top, parts;
+};
+
+template <typename T> __device__ __forceinline__ float to_float(T x);
+template <> __device__ __forceinline__ float to_float(float x) { return x; }
+template <> __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float(float x) { return x; }
+template <> __device__ __forceinline__ __half from_float(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float(float x) { return __float2bfloat16_rn(x); }
+
+// 16 bytes of a row.
+template <typename T>
+struct alignas(16) Vec {
+  static constexpr int N = 16 / sizeof(T);
+  T v[N];
+};
+
+// ---- running sums -------------------------------------------------------------------------------------------------------------------
+struct Sums {
+  float m = kLowest, S = 0.0f, T = 0.0f;
+  __device__ __forceinline__ void move(float to) {      // to a larger m
+    const float f = st::exp2_ftz((m - to) * kLog2e);
+    T = f > 0.0f ? f * fmaf(S, m - to, T) : f * S;      // f = 0: what was seen counts for nothing, and S (m - to) may be infinite
+    S *= f;
+    m = to;
+  }
+  template <int N>
+  __device__ __forceinline__ void add(const float (&x)[N], float largest) {
+    if (largest > m + kMargin) move(largest);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float d = x[i] - m, e = st::exp2_ftz(d * kLog2e);      // NaN, and infinity less infinity, make S NaN
+      S += e;
+      T = fmaf(e, fmaxf(d, kFar), T);
+    }
+  }
+  __device__ __forceinline__ void join(float m2, float S2, float T2) {
+    Sums o;
+    o.m = m2, o.S = S2, o.T = T2;
+    if (m2 > m) move(m2);
+    else o.move(m);
+    S += o.S;
+    T += o.T;
+  }
+};
+__device__ __forceinline__ void join_warp(Sums& s) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m = __shfl_xor_sync(0xffffffffu, s.m, o), S = __shfl_xor_sync(0xffffffffu, s.S, o), T = __shfl_xor_sync(0xffffffffu, s.T, o);
+    s.join(m, S, T);
+  }
+}
+
+// ---- the likeliest tokens -----------------------------------------------------------------------------------------------------------
+// A key orders elements by value, equal ones by the lower index, and NaN before all: no two are equal, and none is 0.
+__device__ __forceinline__ unsigned long long key_of(float x, int index) {
+  const uint32_t b = __float_as_uint(x + 0.0f);      // -0 counts as 0
+  const uint32_t o = x != x ? 0xFFFFFFFFu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+  return static_cast<unsigned long long>(o) << 32 | ~static_cast<uint32_t>(index);
+}
+__device__ __forceinline__ float value_of(unsigned long long key) {
+  const uint32_t o = static_cast<uint32_t>(key >> 32);
+  return o == 0xFFFFFFFFu ? __uint_as_float(0x7FC00000u) : __uint_as_float((o & 0x80000000u) ? o & 0x7FFFFFFFu : ~o);
+}
+__device__ __forceinline__ unsigned long long warp_largest(unsigned long long key) {
+  const uint32_t high = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(key >> 32));
+  const uint32_t low = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(key >> 32) == high ? static_cast<uint32_t>(key) : 0u);
+  return static_cast<unsigned long long>(high) << 32 | low;
+}
+
+// W warps on one row; kRoom keys, of which a round of the careful pass fills half.
+template <int W>
+struct Candidates {
+  static constexpr int kRound = W * 32 * 8, kRoom = 2 * kRound;
+  unsigned long long key[kRoom];
+  unsigned long long best[kMostTop];
+  unsigned long long bound[W];
+  float sums[W][3];
+  int count;
+};
+
+template <int W> __device__ __forceinline__ void sync() {
+  if (W == 1) __syncwarp();
+  else __syncthreads();
+}
+
+// A key that at least `top` of the threads' keys reach: in every warp the ceil(top / W)-th largest, of these the least.
+template <int W>
+__device__ __forceinline__ unsigned long long bound_of(Candidates<W>& c, unsigned long long key, int top, int warp, int lane) {
+  unsigned long long at = 0;
+  for (int i = 0; i < (top + W - 1) / W; ++i) {
+    at = warp_largest(key);
+    if (key == at) key = 0;
+  }
+  if (W == 1) return at;
+  if (lane == 0) c.bound[warp] = at;
+  sync<W>();
+#pragma unroll
+  for (int i = 0; i < W; ++i) at = min(at, c.bound[i]);
+  sync<W>();
+  return at;
+}
+
+// The `top` largest of the first c.count keys to c.best, in order.  All threads; the keys are in place.
+template <int W>
+__device__ void select(Candidates<W>& c, int top, int tid) {
+  constexpr int kOwn = Candidates<W>::kRoom / (W * 32);
+  const int warp = tid >> 5, lane = tid & 31;
+  int n = c.count;
+  if (n > 2 * kMostTop) {      // those that reach a bound: a few more than `top`
+    unsigned long long own[kOwn], largest = 0;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const int at = i * W * 32 + tid;
+      own[i] = at < n ? c.key[at] : 0;
+      largest = max(largest, own[i]);
+    }
+    sync<W>();
+    if (tid == 0) c.count = 0;
+    const unsigned long long bound = max(bound_of(c, largest, top, warp, lane), 1ull);
+    sync<W>();
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i)
+      if (own[i] >= bound) c.key[atomicAdd(&c.count, 1)] = own[i];
+    sync<W>();
+    n = c.count;
+  }
+  for (int i = tid; i < n; i += W * 32) {
+    const unsigned long long key = c.key[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += c.key[j] > key;
+    if (rank < top) c.best[rank] = key;
+  }
+  sync<W>();
+}
+
+// Any row, whatever its order: every round's elements that are larger than the `top` best so far, then the best again.
+template <typename T, int W>
+__device__ __noinline__ void select_carefully(Candidates<W>& c, const T* x, int from, int to, int top, int tid) {
+  unsigned long long bound = 0;
+  if (tid == 0) c.count = 0;
+  sync<W>();
+  for (int at = from; at < to; at += Candidates<W>::kRound) {
+    for (int i = 0; i < 8; ++i) {
+      const int j = at + i * W * 32 + tid;
+      if (j < to) {
+        const unsigned long long key = key_of(to_float(x[j]), j);
+        if (key > bound) c.key[atomicAdd(&c.count, 1)] = key;
+      }
+    }
+    sync<W>();
+    if (c.count > Candidates<W>::kRound) {
+      select(c, top, tid);
+      if (tid < top) c.key[tid] = c.best[tid];
+      if (tid == 0) c.count = top;
+      bound = c.best[top - 1];
+    }
+    sync<W>();
+  }
+}
+
+// One row (or, in a cluster, one part of it) per W warps.
+template <typename T, int W, bool TOP>
+__global__ void __launch_bounds__(kThreads) scores_kernel(const T* logits, const long long* targets, float* logprob, float* entropy, float2* stats, long long* top_ids,
+                                                          float* top_logprobs, const ScoreParams p) {
+  extern __shared__ __align__(16) uint8_t room[];
+  chain_begin(logits, targets, logprob, entropy, stats, top_ids, top_logprobs);
+  constexpr int N = Vec<T>::N, kGroup = W * 32, kSample = 2;
+  Candidates<W>& c = reinterpret_cast<Candidates<W>*>(room)[W == 1 ? threadIdx.x >> 5 : 0];
+  const int tid = threadIdx.x % kGroup, warp = tid >> 5, lane = tid & 31;
+  const int part = W == 1 ? 0 : blockIdx.x % p.parts;
+  const long long row = W == 1 ? static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5) : blockIdx.x / p.parts;
+  if (row >= p.rows) return;
+  const T* x = logits + row * p.row;
+  // elements before the first 16-byte boundary and behind the last one go one by one, to the first threads of the first part
+  const int head = min(p.vocab, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)));
+  const int vectors = (p.vocab - head) / N, rest = head + vectors * N, singles = head + p.vocab - rest;
+  const int share = (vectors + p.parts - 1) / p.parts, v0 = part * share, v1 = min(vectors, v0 + share);
+  const Vec<T>* xv = reinterpret_cast<const Vec<T>*>(x + head);
+  Sums s;
+  if (TOP && tid == 0) c.count = 0;
+
+  unsigned long long bound = 0;
+  float limit = kLowest;      // value of the bound
+  const auto keep = [&](float v, int index) {
+    const unsigned long long key = key_of(v, index);
+    if (key >= bound) {
+      const int at = atomicAdd(&c.count, 1);
+      if (at < Candidates<W>::kRoom) c.key[at] = key;
+    }
+  };
+  const auto unpack = [](const Vec<T>& v, float (&f)[N], float& largest) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = to_float(v.v[i]);
+    largest = f[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) largest = fmaxf(largest, f[i]);
+  };
+
+  int v = v0 + tid;
+  {
+    Vec<T> first[kSample];
+    float single = 0.0f, f[N], largest;
+    const int one = tid < head ? tid : rest + tid - head;
+    const bool has_single = part == 0 && tid < singles;
+#pragma unroll
+    for (int i = 0; i < kSample; ++i)
+      if (v + i * kGroup < v1) first[i] = xv[v + i * kGroup];
+    if (has_single) single = to_float(x[one]);
+    unsigned long long best = 0;
+    if (has_single) {
+      const float own[1] = {single};
+      s.add(own, single);
+      if (TOP) best = key_of(single, one);
+    }
+#pragma unroll
+    for (int i = 0; i < kSample; ++i)
+      if (v + i * kGroup < v1) {
+        unpack(first[i], f, largest);
+        s.add(f, largest);
+        if (TOP) {
+          int at = 0;
+#pragma unroll
+          for (int k = N - 1; k >= 0; --k) at = f[k] == largest ? k : at;
+          best = max(best, key_of(largest, head + (v + i * kGroup) * N + at));
+        }
+      }
+    if (TOP) {
+      sync<W>();      // the count
+      bound = max(bound_of(c, best, p.top, warp, lane), 1ull);
+      limit = bound > 1 ? value_of(bound) : -INFINITY;
+      if (has_single) keep(single, one);
+#pragma unroll
+      for (int i = 0; i < kSample; ++i)
+        if (v + i * kGroup < v1) {
+          unpack(first[i], f, largest);
+          if (largest >= limit)
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+              if (f[k] >= limit) keep(f[k], head + (v + i * kGroup) * N + k);
+        }
+    }
+    v += kSample * kGroup;
+  }
+  constexpr int kAhead = 4;
+  for (; v < v1; v += kAhead * kGroup) {
+    Vec<T> next[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (v + i * kGroup < v1) next[i] = xv[v + i * kGroup];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (v + i * kGroup < v1) {
+        float f[N], largest;
+        unpack(next[i], f, largest);
+        s.add(f, largest);
+        if (TOP && largest >= limit)
+#pragma unroll
+          for (int k = 0; k < N; ++k)
+            if (f[k] >= limit) keep(f[k], head + (v + i * kGroup) * N + k);
+      }
+  }
+
+  // sums of the row (part): in every thread
+  join_warp(s);
+  if (W == 1) {      // lanes joined in orders of their own
+    s.m = __shfl_sync(0xffffffffu, s.m, 0), s.S = __shfl_sync(0xffffffffu, s.S, 0), s.T = __shfl_sync(0xffffffffu, s.T, 0);
+  } else {
+    if (lane == 0) c.sums[warp][0] = s.m, c.sums[warp][1] = s.S, c.sums[warp][2] = s.T;
+    sync<W>();
+    s = Sums();
+#pragma unroll
+    for (int i = 0; i < W; ++i) s.join(c.sums[i][0], c.sums[i][1], c.sums[i][2]);
+  }
+  if (TOP) {
+    sync<W>();
+    // a NaN hides from comparisons (and an infinity makes S one); keys that found no room are lost
+    if (c.count > Candidates<W>::kRoom || s.S != s.S) {
+      if (part == 0) {      // its single elements too: with one part these are the row
+        if (p.parts == 1) {
+          select_carefully<T, W>(c, x, 0, p.vocab, p.top, tid);
+        } else {
+          select_carefully<T, W>(c, x, 0, head + v1 * N, p.top, tid);
+          if (tid < p.vocab - rest) c.key[atomicAdd(&c.count, 1)] = key_of(to_float(x[rest + tid]), rest + tid);
+        }
+      } else {
+        select_carefully<T, W>(c, x, head + v0 * N, head + v1 * N, p.top, tid);
+      }
+      sync<W>();
+    }
+    select(c, p.top, tid);
+  }
+  if (W > 1 && p.parts > 1) {      // the parts of a row: blocks of a cluster, read by the first
+    const int n = c.count < p.top ? c.count : p.top;
+    sync<W>();
+    if (tid == 0) c.sums[0][0] = s.m, c.sums[0][1] = s.S, c.sums[0][2] = s.T, c.count = n;
+    st::cluster_sync();
+    if (part == 0) {
+      s = Sums();
+      for (int r = 0; r < p.parts; ++r) {
+        float f[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f[i]) : "r"(st::cluster_map(st::smem_u32(&c.sums[0][i]), r)));
+        s.join(f[0], f[1], f[2]);
+      }
+      if (TOP) {
+        // up to 8 parts of up to 32 keys: one for every thread
+        const int r = tid >> 5, i = tid & 31;
+        unsigned long long key = 0;
+        if (r < p.parts) {
+          int have;
+          asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(have) : "r"(st::cluster_map(st::smem_u32(&c.count), r)));
+          if (i < have) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key) : "r"(st::cluster_map(st::smem_u32(&c.best[i]), r)));
+        }
+        sync<W>();
+        if (tid == 0) c.count = 0;
+        sync<W>();
+        if (key) c.key[atomicAdd(&c.count, 1)] = key;
+        sync<W>();
+        select(c, p.top, tid);
+      }
+    }
+    st::cluster_sync();
+    if (part != 0) return;
+  }
+
+  // an empty row, all -inf: no probability anywhere
+  const bool empty = s.S == 0.0f;
+  const float log_S = empty ? INFINITY : logf(s.S), m = empty ? 0.0f : s.m;
+  if (tid == 0) {
+    const long long t = targets[row];
+    logprob[row] = t >= 0 && t < p.vocab ? to_float(x[t]) - m - log_S : 0.0f;
+    entropy[row] = empty ? 0.0f : log_S - s.T / s.S;
+    if (stats) stats[row] = make_float2(m, log_S);
+  }
+  if (TOP && tid < p.top) {
+    const unsigned long long key = c.best[tid];
+    top_ids[row * p.top + tid] = static_cast<long long>(~static_cast<uint32_t>(key));
+    top_logprobs[row * p.top + tid] = value_of(key) - m - log_S;
+  }
+}
+
+// ---- gradient -----------------------------------------------------------------------------------------------------------------------
+struct GradParams {
+  long long row, out_row, rows;
+  int vocab, top, parts;
+};
+
+// Blocks share a row in `parts` pieces of whole vectors; WIDE: rows of logits and gradient are at the same place between 16-byte boundaries.
+template <typename T, int W, bool WIDE>
+__global__ void __launch_bounds__(kThreads) scores_grad_kernel(const T* logits, const long long* targets, const float2* stats, const float* entropy,
+                                                               const long long* top_ids, const float* g_logprob, const float* g_entropy, const float* g_top, T* out,
+                                                               const GradParams p) {
+  __shared__ float weight[kWarps][kMostTop + 1];
+  __shared__ int id[kWarps][kMostTop + 1];
+  chain_begin(logits, targets, stats, entropy, top_ids, g_logprob, g_entropy, g_top, out);
+  constexpr int N = Vec<T>::N, kGroup = W * 32;
+  const int slot = W == 1 ? threadIdx.x >> 5 : 0, tid = threadIdx.x % kGroup;
+  const int part = W == 1 ? 0 : blockIdx.x % p.parts;
+  const long long row = W == 1 ? static_cast<long long>(blockIdx.x) * kWarps + slot : blockIdx.x / p.parts;
+  if (row >= p.rows) return;
+  const T* x = logits + row * p.row;
+  T* y = out + row * p.out_row;
+  const float2 ms = stats[row];
+  const bool empty = ms.y == INFINITY;
+  const float m = ms.x, log_S = ms.y, H = entropy[row], gH = g_entropy ? g_entropy[row] : 0.0f;
+  const int n = 1 + (g_top ? p.top : 0);
+  // the tokens with a gradient of their own
+  for (int i = tid; i < n; i += kGroup) {
+    long long t = i == 0 ? targets[row] : top_ids[row * p.top + i - 1];
+    const bool given = t >= 0 && t < p.vocab && (i > 0 || g_logprob);
+    id[slot][i] = given ? static_cast<int>(t) : -1;
+    weight[slot][i] = !given ? 0.0f : i == 0 ? g_logprob[row] : g_top[row * p.top + i - 1];
+  }
+  sync<W>();
+  float all = 0.0f;
+  for (int i = 0; i < n; ++i) all += weight[slot][i];
+  const auto shared = [&](float v) {      // what the distribution contributes
+    const float lp = v - m - log_S, e = st::exp2_ftz(lp * kLog2e);
+    return -e * fmaf(gH, fmaxf(lp, kFar) + H, all);
+  };
+  if (WIDE) {
+    const int head = min(p.vocab, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)));
+    const int vectors = (p.vocab - head) / N, rest = head + vectors * N, singles = head + p.vocab - rest;
+    const int share_v = (vectors + p.parts - 1) / p.parts, v0 = part * share_v, v1 = min(vectors, v0 + share_v);
+    const Vec<T>* xv = reinterpret_cast<const Vec<T>*>(x + head);
+    Vec<T>* yv = reinterpret_cast<Vec<T>*>(y + head);
+    if (part == 0 && tid < singles) {
+      const int at = tid < head ? tid : rest + tid - head;
+      y[at] = from_float<T>(empty ? 0.0f : shared(to_float(x[at])));
+    }
+    constexpr int kAhead = 4;
+    for (int v = v0 + tid; v < v1; v += kAhead * kGroup) {
+      Vec<T> next[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (v + i * kGroup < v1) next[i] = xv[v + i * kGroup];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (v + i * kGroup < v1) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) next[i].v[k] = from_float<T>(empty ? 0.0f : shared(to_float(next[i].v[k])));
+          yv[v + i * kGroup] = next[i];
+        }
+    }
+  } else {
+    const int share_e = (p.vocab + p.parts - 1) / p.parts;
+    for (int j = part * share_e + tid; j < min(p.vocab, (part + 1) * share_e); j += kGroup) y[j] = from_float<T>(empty ? 0.0f : shared(to_float(x[j])));
+  }
+  if (empty) return;
+  // elements of those tokens, as a whole and rounded once, by the block that wrote them
+  sync<W>();
+  for (int i = tid; i < n; i += kGroup) {
+    const int at = id[slot][i];
+    if (at < 0) continue;
+    if (p.parts > 1) {
+      const int head = min(p.vocab, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T))), vectors = (p.vocab - head) / N;
+      const int share_v = (vectors + p.parts - 1) / p.parts, share_e = (p.vocab + p.parts - 1) / p.parts;
+      const int owner = !WIDE ? at / share_e : at < head || at >= head + vectors * N ? 0 : (at - head) / N / share_v;
+      if (owner != part) continue;
+    }
+    float own = 0.0f;
+    for (int k = 0; k < n; ++k) own += id[slot][k] == at ? weight[slot][k] : 0.0f;
+    y[at] = from_float<T>(own + shared(to_float(x[at])));
+  }
+}
+
+// How many blocks share a row: rows that leave SMs without a block are split, to no less than 4096 elements a block.
+int parts_of(long long rows, int vocab) {
+  int parts = 1;
+  while (parts < 8 && rows * parts * 2 <= 2 * st::sm_count() && vocab / (2 * parts) >= 4096) parts *= 2;
+  return parts;
+}
+
+constexpr int kWarpRow = 2048;      // rows of up to as many elements go to a warp each
+
+template <typename T, int W, bool TOP>
+int forward(const void* logits, const long long* targets, float* logprob, float* entropy, float2* stats, long long* top_ids, float* top_logprobs, ScoreParams p,
+            cudaStream_t stream) {
+  p.parts = W == 1 ? 1 : parts_of(p.rows, p.vocab);
+  const long long blocks = W == 1 ? (p.rows + kWarps - 1) / kWarps : p.rows * p.parts;
+  if (blocks > 2147483647LL) return st::fail(ST_ERR_TOO_LARGE, "scores: too many rows");
+  const size_t smem = sizeof(Candidates<W>) * (W == 1 ? kWarps : 1);
+  static_assert(sizeof(Candidates<W>) * (W == 1 ? kWarps : 1) <= 48 * 1024, "candidates need no opting in");
+  const cudaError_t e = st::chained(scores_kernel<T, W, TOP>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), smem, stream, p.parts)(
+      static_cast<const T*>(logits), targets, logprob, entropy, stats, top_ids, top_logprobs, p);
+  return e == cudaSuccess ? ST_OK : st::fail_cuda(e, "token scores");
+}
+
+template <typename T>
+int forward(const void* logits, const long long* targets, float* logprob, float* entropy, float2* stats, long long* top_ids, float* top_logprobs, const ScoreParams& p,
+            cudaStream_t stream) {
+  if (p.vocab <= kWarpRow)
+    return p.top ? forward<T, 1, true>(logits, targets, logprob, entropy, stats, top_ids, top_logprobs, p, stream)
+                 : forward<T, 1, false>(logits, targets, logprob, entropy, stats, top_ids, top_logprobs, p, stream);
+  return p.top ? forward<T, kWarps, true>(logits, targets, logprob, entropy, stats, top_ids, top_logprobs, p, stream)
+               : forward<T, kWarps, false>(logits, targets, logprob, entropy, stats, top_ids, top_logprobs, p, stream);
+}
+
+template <typename T, int W, bool WIDE>
+int backward(const void* logits, const long long* targets, const float2* stats, const float* entropy, const long long* top_ids, const float* g_logprob,
+             const float* g_entropy, const float* g_top, void* out, GradParams p, cudaStream_t stream) {
+  p.parts = W == 1 ? 1 : parts_of(p.rows, p.vocab);
+  const long long blocks = W == 1 ? (p.rows + kWarps - 1) / kWarps : p.rows * p.parts;
+  if (blocks > 2147483647LL) return st::fail(ST_ERR_TOO_LARGE, "scores: too many rows");
+  const cudaError_t e = st::chained(scores_grad_kernel<T, W, WIDE>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream)(
+      static_cast<const T*>(logits), targets, stats, entropy, top_ids, g_logprob, g_entropy, g_top, static_cast<T*>(out), p);
+  return e == cudaSuccess ? ST_OK : st::fail_cuda(e, "token scores gradient");
+}
+
+template <typename T>
+int backward(const void* logits, const long long* targets, const float2* stats, const float* entropy, const long long* top_ids, const float* g_logprob,
+             const float* g_entropy, const float* g_top, void* out, const GradParams& p, cudaStream_t stream) {
+  const bool wide = (reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(out)) % 16 == 0 && (p.row - p.out_row) * static_cast<long long>(sizeof(T)) % 16 == 0;
+#define ST_GRAD(WW, FF) backward<T, WW, FF>(logits, targets, stats, entropy, top_ids, g_logprob, g_entropy, g_top, out, p, stream)
+  if (p.vocab <= kWarpRow) return wide ? ST_GRAD(1, true) : ST_GRAD(1, false);
+  return wide ? ST_GRAD(kWarps, true) : ST_GRAD(kWarps, false);
+#undef ST_GRAD
+}
+}  // namespace
+
+// Scores of rows of `vocab` logits (type 0 bf16, 1 fp16, 2 fp32; `row` elements apart): log probability of targets[row] (0 where that is no token), entropy, and the
+// `top` (0 to 32) likeliest tokens with their log probabilities.  stats (may be null; on an 8-byte boundary): 2 floats a row for the gradient.
+ST_API int st_token_scores(const void* logits, const long long* targets, float* logprob, float* entropy, void* stats, long long* top_ids, float* top_logprobs, long long rows,
+                           long long row, int vocab, int top, int type, void* stream_v) {
+  if (rows < 0 || vocab < 1 || vocab > 1 << 30 || top < 0 || top > kMostTop || top > vocab) return st::fail(ST_ERR_INVALID, "scores: sizes out of range");
+  if (reinterpret_cast<uintptr_t>(stats) & 7) return st::fail(ST_ERR_INVALID, "scores: stats must lie on an 8-byte boundary");
+  if (rows == 0) return ST_OK;
+  const ScoreParams p{row, rows, vocab, top, 1};
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
+  float2* ms = static_cast<float2*>(stats);
+  switch (type) {
+    case 0: return forward<__nv_bfloat16>(logits, targets, logprob, entropy, ms, top_ids, top_logprobs, p, stream);
+    case 1: return forward<__half>(logits, targets, logprob, entropy, ms, top_ids, top_logprobs, p, stream);
+    case 2: return forward<float>(logits, targets, logprob, entropy, ms, top_ids, top_logprobs, p, stream);
+  }
+  return st::fail(ST_ERR_INVALID, "scores: unknown type");
+}
+
+// Gradient of the logits from those of log probability, entropy and the likeliest tokens' log probabilities (each may be null: 0).
+ST_API int st_token_scores_grad(const void* logits, const long long* targets, const void* stats, const float* entropy, const long long* top_ids, const float* g_logprob,
+                                const float* g_entropy, const float* g_top, void* out, long long rows, long long row, long long out_row, int vocab, int top, int type,
+                                void* stream_v) {
+  if (rows < 0 || vocab < 1 || vocab > 1 << 30 || top < 0 || top > kMostTop || top > vocab) return st::fail(ST_ERR_INVALID, "scores: sizes out of range");
+  if (reinterpret_cast<uintptr_t>(stats) & 7) return st::fail(ST_ERR_INVALID, "scores: stats must lie on an 8-byte boundary");
+  if (rows == 0) return ST_OK;
+  const GradParams p{row, out_row, rows, vocab, top, 1};
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
+  const float2* ms = static_cast<const float2*>(stats);
+  switch (type) {
+    case 0: return backward<__nv_bfloat16>(logits, targets, ms, entropy, top_ids, g_logprob, g_entropy, g_top, out, p, stream);
+    case 1: return backward<__half>(logits, targets, ms, entropy, top_ids, g_logprob, g_entropy, g_top, out, p, stream);
+    case 2: return backward<float>(logits, targets, ms, entropy, top_ids, g_logprob, g_entropy, g_top, out, p, stream);
+  }
+  return st::fail(ST_ERR_INVALID, "scores: unknown type");
+}

@@ -153,6 +153,7 @@ ST_API int st_int4_linear(const void* x, const void* codes, const void* scales, 
                           long long x_row, long long residual_row, long long y_row, int group, int act, int type, void* stream_v) {
   if (tokens < 0 || rows < 1 || cols < 1 || rows > 1 << 30 || cols > 1 << 30 || (group != 32 && group != 64 && group != 128) || act < 0 || act > 2)
     return st::fail(ST_ERR_INVALID, "int4: sizes out of range");
+  if ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15) return st::fail(ST_ERR_INVALID, "int4: codes and scales must lie on 16-byte boundaries");
   if (tokens == 0) return ST_OK;
   const LinearParams p{x, static_cast<const uint8_t*>(codes), static_cast<const __nv_bfloat16*>(scales), bias, residual, y, x_row, residual_row, y_row,
                        tokens, rows, cols, (cols + group - 1) / group, (cols + kTileCols - 1) / kTileCols, (rows + kTileRows - 1) / kTileRows, group, act};

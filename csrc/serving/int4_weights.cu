@@ -166,7 +166,8 @@ __global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* 
   }
 }
 
-int plan(WeightsParams& p, unsigned& grid, int group) {
+int plan(WeightsParams& p, unsigned& grid, int group, const void* codes, const void* scales) {
+  if ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15) return st::fail(ST_ERR_INVALID, "int4: codes and scales must lie on 16-byte boundaries");
   if (p.rows < 1 || p.cols < 1 || p.rows > 1 << 30 || p.cols > 1 << 30 || (group != 32 && group != 64 && group != 128)) return st::fail(ST_ERR_INVALID, "int4: sizes out of range");
   p.groups = (p.cols + group - 1) / group;
   p.chunks = (p.cols + kTileCols - 1) / kTileCols;
@@ -198,7 +199,7 @@ int dequantize(const uint8_t* codes, const __nv_bfloat16* scales, void* w, const
 ST_API int st_int4_quantize(const void* w, void* codes, void* scales, int rows, int cols, long long stride, int group, int type, void* stream_v) {
   WeightsParams p{stride, rows, cols, 0, 0, 0};
   unsigned grid;
-  if (const int e = plan(p, grid, group)) return e;
+  if (const int e = plan(p, grid, group, codes, scales)) return e;
   uint8_t* c = static_cast<uint8_t*>(codes);
   __nv_bfloat16* s = static_cast<__nv_bfloat16*>(scales);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
@@ -214,7 +215,7 @@ ST_API int st_int4_quantize(const void* w, void* codes, void* scales, int rows, 
 ST_API int st_int4_dequantize(const void* codes, const void* scales, void* w, int rows, int cols, long long stride, int group, int type, void* stream_v) {
   WeightsParams p{stride, rows, cols, 0, 0, 0};
   unsigned grid;
-  if (const int e = plan(p, grid, group)) return e;
+  if (const int e = plan(p, grid, group, codes, scales)) return e;
   const uint8_t* c = static_cast<const uint8_t*>(codes);
   const __nv_bfloat16* s = static_cast<const __nv_bfloat16*>(scales);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);

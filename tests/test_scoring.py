@@ -1,0 +1,289 @@
+"""Scores of given tokens: the CPU statement against torch's log_softmax and differences, the kernels against 64 bits where a row can go wrong (masked,
+empty, equal, ordered, non-finite), refusals.
+
+Tolerances.  x - m is off by half a step of fp32, 2^-24 |x - m|; a term of S is off by 2^-22 (exp2 and its argument) plus 2^-24 |x - m| of itself where it counts
+(e^d d is below 0.37 at any d, so that part stays below 2^-24 of S / e^d), and up to vocab / 256 + 60 additions (8 per vector of a thread, then the joins) each by 2^-24: S is within
+delta = 2^-21 + (vocab / 256 + 60) 2^-24 of itself, log S within delta.  m lies up to 4 below the largest element.  log p = x - m - log S: delta + 2^-23 (|x - m| + |log S| + 4), where |x - m| <= |log p| + log vocab + 4.
+Entropy: the same for log S and delta (|T| / S + 4) for the quotient.  A gradient p (a + g (log p + H)): p and the bracket within twice the same, relative
+to the sum of magnitudes, then half a step of the type."""
+import math
+
+import pytest
+import torch
+
+from spiraltorch_b200.ops import scoring
+
+GPU = pytest.mark.gpu
+cuda = torch.device("cuda")
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+INF = math.inf
+
+
+def _logits(rows, vocab, dtype, seed=0, scale=3.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(rows, vocab, generator=g) * scale).to(dtype), torch.randint(0, vocab, (rows,), generator=g)
+
+
+def _hard(vocab, dtype, top):
+    """Rows that are masked, empty, equal, ordered, far from zero, with one token, with values behind any bound that the first elements give."""
+    low, big = torch.finfo(dtype).min, min(torch.finfo(dtype).max / 4, 1e30)
+    base = _logits(1, vocab, dtype, 5)[0][0].float()
+    ramp = torch.linspace(-20, 20, vocab)
+    one = torch.full((vocab,), -INF)
+    one[vocab // 2] = -7.0
+    some = torch.full((vocab,), -INF)
+    some[:: max(1, vocab // (top + 2))] = base[:: max(1, vocab // (top + 2))]
+    holes = base.clone()
+    holes[1::3] = -INF
+    lows = base.clone()
+    lows[::2] = low
+    rows = [base, torch.full((vocab,), -INF), torch.zeros(vocab), torch.full((vocab,), low), ramp, ramp.flip(0), one, some, holes, lows, base + 1000.0, base - 1000.0,
+            torch.where(torch.arange(vocab) % 2 == 0, 0.0, -0.0), torch.full((vocab,), big), base.round(), torch.where(torch.arange(vocab) == vocab - 1, 50.0, low)]
+    x = torch.stack(rows).to(dtype)
+    t = torch.randint(0, vocab, (len(rows),), generator=torch.Generator().manual_seed(9))
+    t[6], t[0] = vocab // 2, -100
+    t[15], t[10] = vocab - 1, vocab
+    return x, t
+
+
+def _exact(x, t, top):
+    return scoring.token_scores_reference(x.double(), t, top)
+
+
+def _check(got, x, t, top):
+    """Scores against 64 bits."""
+    vocab = x.shape[1]
+    want = _exact(x, t, top)
+    delta = 2.0 ** -21 + (vocab / 256 + 60) * 2.0 ** -24
+    span = math.log(vocab) + 4
+
+    def near(a, b, allowed):
+        a = a.double().cpu()
+        same = (a == b) | (a.isnan() & b.isnan())
+        assert ((a - b).abs() <= allowed)[~same].all(), float(((a - b).abs() / allowed)[~same].max())
+
+    assert got.logprob.dtype == got.entropy.dtype == got.top_logprobs.dtype == torch.float32
+    near(got.logprob, want.logprob, delta + 2.0 ** -23 * (want.logprob.abs().nan_to_num(0, 0, 0) + 3 * span))
+    near(got.entropy, want.entropy, delta * (2 * span + 5) + 2.0 ** -23 * 3 * span)
+    assert got.top_ids.dtype == torch.int64 and torch.equal(got.top_ids.cpu(), want.top_ids)
+    near(got.top_logprobs, want.top_logprobs, delta + 2.0 ** -23 * (want.top_logprobs.abs().nan_to_num(0, 0, 0) + 3 * span))
+
+
+@pytest.mark.parametrize("vocab,top", [(1, 1), (2, 0), (33, 5), (257, 32)])
+def test_statement(vocab, top):
+    x, t = _logits(6, vocab, torch.float64)
+    s = scoring.token_scores(x, t, top=top)
+    lp = torch.log_softmax(x, 1)
+    assert torch.allclose(s.logprob, lp.gather(1, t[:, None])[:, 0], atol=1e-12)
+    assert torch.allclose(s.entropy, -(lp.exp() * lp).sum(1), atol=1e-12)
+    assert torch.equal(s.top_ids, lp.topk(top, 1).indices) and torch.allclose(s.top_logprobs, lp.topk(top, 1).values, atol=1e-12)
+
+
+def test_statement_of_rows_that_are_masked():
+    x, t = _hard(64, torch.float32, 5)
+    s = scoring.token_scores(x, t, top=5)
+    assert s.logprob[0] == 0 and s.logprob[10] == 0                                       # no such token
+    assert s.logprob[1] == -INF and s.entropy[1] == 0 and s.top_ids[1].tolist() == [0, 1, 2, 3, 4] and (s.top_logprobs[1] == -INF).all()
+    for r in (2, 3, 12, 13):                                                              # all equal
+        assert torch.allclose(s.entropy[r], torch.tensor(math.log(64))) and s.top_ids[r].tolist() == [0, 1, 2, 3, 4]
+    assert s.entropy[6] == 0 and s.logprob[6] == 0 and s.top_ids[6, 0] == 32
+    x[0, 7] = math.nan
+    x[1, 9] = INF
+    s = scoring.token_scores(x[:2], t[:2].clamp(min=0), top=3)
+    assert s.logprob.isnan().all() and s.entropy.isnan().all() and s.top_logprobs.isnan().all()
+    assert s.top_ids[0, 0] == 7 and s.top_ids[1].tolist() == [9, 0, 1]
+
+
+def test_statement_gradients():
+    x, t = _logits(4, 9, torch.float64)
+    t[2] = -100
+    x[1, 3] = -INF
+    x.requires_grad_(True)
+    ref = x.detach().clone().requires_grad_(True)
+    lp = torch.log_softmax(ref, 1)
+    s = scoring.token_scores(x, t, top=3)
+    gl, ge, gt = torch.randn(4, dtype=torch.float64), torch.randn(4, dtype=torch.float64), torch.randn(4, 3, dtype=torch.float64)
+    ent = -torch.where(lp.isinf(), 0.0, lp.exp() * lp.masked_fill(lp.isinf(), 0.0)).sum(1)
+    given = torch.where(t >= 0, lp.gather(1, t.clamp(min=0)[:, None])[:, 0], 0.0)
+    want = torch.autograd.grad((given * gl).sum() + (ent * ge).sum() + (lp.gather(1, s.top_ids) * gt).sum(), ref)[0]
+    got = torch.autograd.grad((s.logprob, s.entropy, s.top_logprobs), x, (gl, ge, gt))[0]
+    assert torch.allclose(got, want, atol=1e-12)
+    y = torch.randn(3, 7, dtype=torch.float64, requires_grad=True)
+    u = torch.tensor([1, 6, -100])
+    assert torch.autograd.gradcheck(lambda y: (lambda s: (s.logprob, s.entropy, s.top_logprobs))(scoring.token_scores(y, u, top=2)), (y,))
+    # one output's gradient alone, none at all, and an empty row
+    only = torch.autograd.grad(scoring.token_scores(x, t).entropy.sum(), x)[0]
+    assert torch.isfinite(only).all()
+    e = torch.full((1, 5), -INF, requires_grad=True)
+    s = scoring.token_scores(e, torch.tensor([2]), top=2)
+    assert (torch.autograd.grad((s.logprob, s.entropy, s.top_logprobs), e, (torch.ones(1), torch.ones(1), torch.ones(1, 2)))[0] == 0).all()
+
+
+def test_shapes_and_refusals():
+    x, t = _logits(6, 11, torch.float32)
+    s = scoring.token_scores(x.view(2, 3, 11), t.view(2, 3), top=4)
+    assert s.logprob.shape == s.entropy.shape == (2, 3) and s.top_ids.shape == s.top_logprobs.shape == (2, 3, 4)
+    s = scoring.token_scores(x[0], t[0])
+    assert s.logprob.shape == () and s.top_ids.shape == (0,)
+    assert scoring.token_scores(x[:0], t[:0], top=2).top_ids.shape == (0, 2)
+    for call in (lambda: scoring.token_scores(x, t[:5]), lambda: scoring.token_scores(x, t.int()), lambda: scoring.token_scores(x, t, top=12),
+                 lambda: scoring.token_scores(x, t, top=-1), lambda: scoring.token_scores(x.int(), t), lambda: scoring.token_scores(x[:, :0], t),
+                 lambda: scoring.token_scores(torch.randn(2, 100), t[:2], top=33), lambda: scoring.token_scores(torch.tensor(1.0), torch.tensor(0))):
+        with pytest.raises(ValueError):
+            call()
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(ValueError):
+            scoring.token_scores(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)), t)
+
+
+# ---- kernels --------------------------------------------------------------------------------------------------------------------
+VOCABS = [1, 2, 7, 31, 64, 257, 1000, 2048, 2049, 4099, 8192, 20011, 50304, 140001]
+
+
+@GPU
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", VOCABS)
+def test_kernel(vocab, dtype):
+    for rows, top in ((1, min(5, vocab)), (3, 0), (40, min(20, vocab)), (130, min(1, vocab)), (11, min(32, vocab))):
+        x, t = _logits(rows, vocab, dtype, rows)
+        t[0] = -100 if rows > 1 else t[0]
+        _check(scoring.token_scores(x.to(cuda), t.to(cuda), top=top), x, t, top)
+
+
+@GPU
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [33, 300, 2048, 3001, 33000, 70000])
+@pytest.mark.parametrize("rows", [16, 320])
+def test_kernel_on_hard_rows(rows, vocab, dtype):
+    for top in (0, 1, 32):
+        x, t = _hard(vocab, dtype, top)
+        x, t = x.repeat(rows // 16, 1), t.repeat(rows // 16)
+        _check(scoring.token_scores(x.to(cuda), t.to(cuda), top=top), x, t, top)
+
+
+@GPU
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [9, 300, 5000, 40000])
+def test_kernel_non_finite(vocab, dtype):
+    x, t = _logits(8, vocab, dtype, 3)
+    x[0, 0], x[1, vocab - 1], x[2, vocab // 2], x[3, 1], x[3, 5], x[4, 2], x[4, 3] = math.nan, math.nan, INF, INF, math.nan, INF, -INF
+    x[5] = math.nan
+    x[6] = INF
+    top = min(5, vocab)
+    _check(scoring.token_scores(x.to(cuda), t.to(cuda), top=top), x, t, top)
+
+
+@GPU
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab,pad,at", [(300, 7, 3), (300, 20, 4), (5001, 0, 0), (5001, 7, 1), (50001, 303, 0), (20011, 0, 0)])
+def test_kernel_views(vocab, pad, at, dtype):
+    x, t = _logits(5, vocab, dtype, 1)
+    wide = torch.full((5, vocab + pad), math.nan, dtype=dtype, device=cuda)
+    view = wide[:, at:at + vocab]
+    view.copy_(x)
+    _check(scoring.token_scores(view, t.to(cuda), top=7), x, t, 7)
+    y = scoring.token_scores(x.to(cuda).T.contiguous().T, t.to(cuda), top=7)
+    _check(y, x, t, 7)
+    _check(scoring.token_scores(x[:1].to(cuda).expand(5, vocab), t.to(cuda), top=7), x[:1].expand(5, vocab), t, 7)
+
+
+def _check_gradient(x, t, top, grads, layout=lambda x: x):
+    leaf = layout(x.to(cuda)).requires_grad_(True)
+    s = scoring.token_scores(leaf, t.to(cuda), top=top)
+    outs = [(o, g) for o, g in zip((s.logprob, s.entropy, s.top_logprobs), grads) if g is not None]
+    got = torch.autograd.grad([o for o, _ in outs], leaf, [g.to(cuda) for _, g in outs])[0]
+    assert got.dtype == x.dtype and got.shape == x.shape
+    gl, ge, gt = grads
+    want = scoring._gradient_reference(x.double(), t, s.top_ids.cpu(), gl, ge, gt)
+    vocab = x.shape[1]
+    logp, entropy = scoring._statement(x.double())
+    p = logp.exp()
+    given = (t >= 0) & (t < vocab)
+    own = torch.zeros_like(p)
+    if gl is not None:
+        own.scatter_add_(1, torch.where(given, t, 0)[:, None], torch.where(given, gl.abs(), 0.0)[:, None].double())
+    if gt is not None:
+        own.scatter_add_(1, s.top_ids.cpu(), gt.abs().double())
+    size = own.sum(1, keepdim=True) + (0 if ge is None else ge.abs()[:, None] * (logp.abs().nan_to_num(0, 0, 0) + entropy.abs()[:, None] + 1))
+    delta = 2.0 ** -21 + (vocab / 256 + 60) * 2.0 ** -24
+    off = 2 * (delta + 2.0 ** -23 * (logp.abs().nan_to_num(0, 0, 0) + 3 * (math.log(vocab) + 4))) + 34 * 2.0 ** -24
+    eps = torch.finfo(x.dtype).eps / 2
+    allowed = p * size * off * (2 * math.log(vocab) + 13) + own * 34 * 2.0 ** -24 + eps * (want.abs() + torch.finfo(x.dtype).smallest_normal)
+    d = (got.double().cpu() - want).abs()
+    assert (d <= allowed).all(), float((d / allowed).max())
+
+
+@GPU
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [1, 33, 300, 2048, 2049, 8192, 50001])
+def test_gradient_kernel(vocab, dtype):
+    for rows, top in ((1, min(5, vocab)), (19, 0), (150, min(32, vocab))):
+        x, t = _logits(rows, vocab, dtype, rows)
+        t[0] = -100 if rows > 1 else t[0]
+        g = torch.Generator().manual_seed(2)
+        gl, ge, gt = torch.randn(rows, generator=g), torch.randn(rows, generator=g), torch.randn(rows, top, generator=g)
+        for grads in ((gl, ge, gt if top else None), (gl, None, None), (None, ge, None)):
+            _check_gradient(x, t, top, grads)
+
+
+@GPU
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [33, 300, 3001, 33000])
+def test_gradient_kernel_on_hard_rows_and_views(vocab, dtype):
+    x, t = _hard(vocab, dtype, 5)
+    g = torch.Generator().manual_seed(2)
+    grads = (torch.randn(16, generator=g), torch.randn(16, generator=g), torch.randn(16, 5, generator=g))
+    _check_gradient(x, t, 5, grads)
+    for pad, at in ((7, 3), (8, 8), (vocab, 0)):
+        def layout(x):
+            wide = torch.zeros((16, vocab + pad), dtype=dtype, device=cuda)
+            wide[:, at:at + vocab] = x
+            return wide.detach()[:, at:at + vocab]
+        _check_gradient(x, t, 5, grads, layout)
+    _check_gradient(x, t, 5, (grads[0][:1].expand(16), None, grads[2][:, :1].expand(16, 5)))
+
+
+@GPU
+def test_gradient_accumulates_and_non_finite_rows():
+    x, t = _logits(6, 5000, torch.bfloat16)
+    x[2, 9] = math.nan
+    leaf = x.to(cuda).requires_grad_(True)
+    for _ in range(2):
+        scoring.token_scores(leaf, t.to(cuda)).logprob.sum().backward()
+    assert leaf.grad[2].isnan().all() and not leaf.grad[[0, 1, 3, 4, 5]].isnan().any()
+    one = torch.autograd.grad(scoring.token_scores(leaf, t.to(cuda)).logprob.sum(), leaf)[0]
+    assert torch.equal((one + one)[0], leaf.grad[0])
+
+
+@GPU
+def test_streams_and_graphs():
+    x, t = _logits(20, 9000, torch.bfloat16)
+    x, t = x.to(cuda), t.to(cuda)
+    want = scoring.token_scores(x, t, top=5)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = scoring.token_scores(x, t, top=5)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    leaf = x.clone().requires_grad_(True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s = scoring.token_scores(leaf, t, top=5)
+        d = torch.autograd.grad((s.logprob, s.entropy), leaf, (torch.ones(20, device=cuda), torch.ones(20, device=cuda)))[0]
+    with torch.no_grad():
+        leaf.mul_(0.5)
+    graph.replay()
+    want = scoring.token_scores(leaf.detach(), t, top=5)
+    assert all(torch.equal(a, b) for a, b in zip(s, want))
+    y = leaf.detach().clone().requires_grad_(True)
+    w = scoring.token_scores(y, t)
+    assert torch.equal(d, torch.autograd.grad((w.logprob, w.entropy), y, (torch.ones(20, device=cuda), torch.ones(20, device=cuda)))[0])
+
+
+@GPU
+def test_kernel_refusals():
+    x, t = _logits(3, 50, torch.float32)
+    for call in (lambda: scoring.token_scores(x.to(cuda), t), lambda: scoring.token_scores(x, t.to(cuda)), lambda: scoring.token_scores(x.to(cuda).double(), t.to(cuda))):
+        with pytest.raises(ValueError):
+            call()
