@@ -9,6 +9,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
+#include "../common/ptx.cuh"
 
 namespace st4 {
 
@@ -29,6 +30,10 @@ struct alignas(sizeof(T) * N) Vec {
 };
 
 __device__ __forceinline__ float bf16_bits(uint32_t low16) { return __uint_as_float(low16 << 16); }
+
+__device__ __forceinline__ float activate(float v, int act) {      // 0 none, 1 relu (NaN stays), 2 gelu
+  return act == 1 ? fmaxf(v, 0.0f) + (v != v ? v : 0.0f) : act == 2 ? st::gelu_tanh(v) : v;
+}
 
 // Nibbles e and e + 4 of a word as two numbers -8..7, exactly: the nibble is put into the low bits of 128 (bf16) or 1024 (fp16), where a unit is 1, and
 // 136 or 1032 is subtracted.

@@ -3,6 +3,7 @@
 #include "../common/ptx.cuh"
 #include "../common/chain.cuh"
 #include "int4.cuh"
+#include "int4_wide.h"
 
 namespace {
 using namespace st4;
@@ -30,8 +31,6 @@ template <> __device__ __forceinline__ void mma<__half>(float (&d)[4], const uin
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
-
-__device__ __forceinline__ float activate(float v, int act) { return act == 1 ? fmaxf(v, 0.0f) + (v != v ? v : 0.0f) : act == 2 ? st::gelu_tanh(v) : v; }
 
 // Elements k and k + 1 of a row of x as one word; what lies behind the row's end is zero.
 template <typename T, bool PAIRS>
@@ -142,13 +141,18 @@ int by_group(const LinearParams& p, cudaStream_t stream) {
 template <typename T>
 int dispatch(const LinearParams& p, cudaStream_t stream) {
   if (p.tokens <= 8) return by_group<T, 1, 1>(p, stream);
-  if (p.tokens <= 16) return by_group<T, 2, 1>(p, stream);
-  return by_group<T, 4, 2>(p, stream);
+  return by_group<T, 2, 1>(p, stream);
+}
+constexpr int kWideFrom = 17;
+
+int aligned(const void* x, long long row, int cols) {
+  if ((reinterpret_cast<uintptr_t>(x) & 15) == 0 && row % 8 == 0 && row >= cols) return ST_OK;
+  return st::fail(ST_ERR_INVALID, "int4: rows must lie on 16-byte boundaries");
 }
 }  // namespace
 
 // y [tokens, rows] = act(x [tokens, cols] W^T + bias) + residual.  Columns are contiguous, rows the given numbers of elements apart; bias and residual may be
-// null.  act: 0 none, 1 relu, 2 gelu (tanh form); type of x, bias, residual and y: 0 bf16, 1 fp16.
+// null.  From st_int4_wide_from() tokens on x lies on a 16-byte boundary, its rows a multiple of 8 elements apart.  act: 0 none, 1 relu, 2 gelu (tanh form); type of x, bias, residual and y: 0 bf16, 1 fp16.
 ST_API int st_int4_linear(const void* x, const void* codes, const void* scales, const void* bias, const void* residual, void* y, int tokens, int rows, int cols,
                           long long x_row, long long residual_row, long long y_row, int group, int act, int type, void* stream_v) {
   if (tokens < 0 || rows < 1 || cols < 1 || rows > 1 << 30 || cols > 1 << 30 || (group != 32 && group != 64 && group != 128) || act < 0 || act > 2)
@@ -158,7 +162,26 @@ ST_API int st_int4_linear(const void* x, const void* codes, const void* scales, 
   const LinearParams p{x, static_cast<const uint8_t*>(codes), static_cast<const __nv_bfloat16*>(scales), bias, residual, y, x_row, residual_row, y_row,
                        tokens, rows, cols, (cols + group - 1) / group, (cols + kTileCols - 1) / kTileCols, (rows + kTileRows - 1) / kTileRows, group, act};
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
+  if (type != 0 && type != 1) return st::fail(ST_ERR_INVALID, "int4: unknown type");
+  if (tokens >= kWideFrom) {
+    if (const int e = aligned(x, x_row, cols)) return e;
+    return wide(WideArgs{x, codes, scales, bias, residual, y, x_row, residual_row, y_row, tokens, rows, cols, group, act}, type, false, stream);
+  }
   if (type == 0) return dispatch<__nv_bfloat16>(p, stream);
-  if (type == 1) return dispatch<__half>(p, stream);
-  return st::fail(ST_ERR_INVALID, "int4: unknown type");
+  return dispatch<__half>(p, stream);
 }
+
+// dx [tokens, cols] = dy [tokens, rows] W.  dy lies on a 16-byte boundary, its rows a multiple of 8 elements apart.
+ST_API int st_int4_linear_grad(const void* dy, const void* codes, const void* scales, void* dx, int tokens, int rows, int cols, long long dy_row, long long dx_row,
+                               int group, int type, void* stream_v) {
+  if (tokens < 0 || rows < 1 || cols < 1 || rows > 1 << 30 || cols > 1 << 30 || (group != 32 && group != 64 && group != 128))
+    return st::fail(ST_ERR_INVALID, "int4: sizes out of range");
+  if ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15) return st::fail(ST_ERR_INVALID, "int4: codes and scales must lie on 16-byte boundaries");
+  if (type != 0 && type != 1) return st::fail(ST_ERR_INVALID, "int4: unknown type");
+  if (tokens == 0) return ST_OK;
+  if (const int e = aligned(dy, dy_row, rows)) return e;
+  return wide(WideArgs{dy, codes, scales, nullptr, nullptr, dx, dy_row, 0, dx_row, tokens, rows, cols, group, 0}, type, true, reinterpret_cast<cudaStream_t>(stream_v));
+}
+
+// From how many rows of x products go through tcgen05 (x then as dy above).
+ST_API int st_int4_wide_from() { return kWideFrom; }

@@ -14,6 +14,7 @@ CPU tensors use a plain PyTorch statement of the same (also the test oracle).  T
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -171,6 +172,20 @@ def dequantize(w: Weights, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
 
 
 # ---- products -------------------------------------------------------------------------------------------------------------------
+@functools.cache
+def _wide_from() -> int:
+    return native.lib().st_int4_wide_from()
+
+
+def _boundaries(x2: torch.Tensor) -> torch.Tensor:
+    """``x2``, or a copy of it, with every row on a 16-byte boundary, as tiled copies need them."""
+    rows, cols = x2.shape
+    stride, step = x2.stride()
+    if step == 1 and stride % 8 == 0 and stride >= cols and x2.data_ptr() % 16 == 0:
+        return x2
+    return x2.new_empty((rows, -(-cols // 8) * 8))[:, :cols].copy_(x2)
+
+
 def _product(x2, w, bias, act, residual2):
     """``[rows, in]`` to ``[rows, out]``."""
     global launch_count
@@ -184,6 +199,8 @@ def _product(x2, w, bias, act, residual2):
         bias = bias.contiguous()
     index = native.require_cuda("int4.linear", x2, w.codes, w.scales, bias, residual2)
     rows = x2.shape[0]
+    if rows >= _wide_from():
+        x2 = _boundaries(x2)
     y = x2.new_empty((rows, w.out_features))
     if rows == 0:
         return y
@@ -201,15 +218,19 @@ def _input_gradient(dy2, w):
     if not native.use_native(dy2):
         t = torch.float64 if dy2.dtype == torch.float64 else torch.float32
         return (dy2.to(t) @ dequantize_reference(w, t)).to(dy2.dtype)
-    from .gemm import gemm
-    dense = dequantize(w, torch.bfloat16)
-    if dy2.dtype == torch.bfloat16:
-        return gemm(dy2, dense, b_mn=True)
-    # an fp16 number is the sum of two bf16 numbers where the second is no smaller than they get
-    high = dy2.to(torch.bfloat16)
-    low = (dy2.float() - high.float()).to(torch.bfloat16)
-    out = gemm(high, dense, b_mn=True, out_dtype=torch.float32)
-    return gemm(low, dense, b_mn=True, out=out, accumulate=True).to(dy2.dtype)
+    global launch_count
+    dy2 = _boundaries(dy2)
+    index = native.require_cuda("int4.linear", dy2, w.codes, w.scales)
+    rows = dy2.shape[0]
+    dx = torch.empty((rows, w.in_features), dtype=dy2.dtype, device=dy2.device)
+    if rows == 0:
+        return dx
+    with native.on_device(index):
+        st = native.entry("st_int4_linear_grad", "ppppiiiqqiip")(dy2.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), dx.data_ptr(), rows, w.out_features,
+                                                               w.in_features, dy2.stride(0), w.in_features, w.group, _TYPES[dy2.dtype], native.raw_stream(index))
+    native.check(st, "st_int4_linear_grad")
+    launch_count += 1
+    return dx
 
 
 class _LinearFn(torch.autograd.Function):
@@ -224,7 +245,7 @@ class _LinearFn(torch.autograd.Function):
     def backward(ctx, dy):
         need_x, need_bias, need_residual, _ = ctx.needs_input_grad
         dy2 = dy.reshape(-1, ctx.w.out_features)
-        dx = _input_gradient(dy2.contiguous(), ctx.w).view(ctx.x_shape) if need_x else None
+        dx = _input_gradient(dy2, ctx.w).view(ctx.x_shape) if need_x else None
         db = dy2.sum(0, dtype=torch.float64 if dy.dtype == torch.float64 else torch.float32).to(dy.dtype) if need_bias else None
         return dx, db, dy if need_residual else None, None
 
