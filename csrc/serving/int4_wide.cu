@@ -16,10 +16,12 @@ using namespace st4;
 constexpr int kRing = 4;                     // weight operands in tensor memory, 32 columns each, behind two results
 constexpr int kMostTokens = 192;             // of a tile: 2 * 192 + 4 * 32 = 512 columns
 constexpr int kMostStages = 12;
-constexpr int kThreads = 512;                // warps: 0 copies, 1 products, 4-7 results, 8-15 weights
+constexpr int kTeams = 3;                    // of 4 warps, one for each 32 lanes of tensor memory, that take weights in turn
+constexpr int kThreads = 256 + kTeams * 128; // warps: 0 copies, 1 products, 4-7 results, from 8 on weights
 constexpr int kRoom = 200 * 1024;            // of shared memory for stages
 
-struct alignas(8) Shared {
+struct alignas(16) Shared {
+  unsigned char out[4][2048];      // 32 tokens by 32 rows of the result for each of its warps
   unsigned long long full[kMostStages], empty[kMostStages], ready[kRing], taken[kRing], done[2], drained[2];
   uint32_t tmem;
   int abort;
@@ -32,27 +34,55 @@ struct WideParams {
   long long residual_row, y_row;
   int tokens, outs, depth;      // outs: rows of the result's weights side; depth: chunks of 64 of the contraction
   int nt, stages, tiles_down, tiles, parts, act;
+  bool wide_rows;      // rows of y lie on 16-byte boundaries and are whole vectors
   unsigned* err;
 };
 
-template <typename T> __device__ __forceinline__ uint32_t times(uint32_t pair, uint32_t scale) {
-  if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
-    const __half2 d = __hmul2(*reinterpret_cast<const __half2*>(&pair), *reinterpret_cast<const __half2*>(&scale));
-    return *reinterpret_cast<const uint32_t*>(&d);
-  } else {
-    const __nv_bfloat162 d = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&pair), *reinterpret_cast<const __nv_bfloat162*>(&scale));
+// A whole warp's bounded wait, as st::mbar_wait_warp, but the clock is first read after 64 polls: every hop of this kernel's ring is short, and a read of the
+// global timer takes longer than it.
+__device__ __forceinline__ bool wait(const unsigned long long& barrier, uint32_t parity, volatile int* abort_flag) {
+  const uint32_t bar = st::smem_u32(&barrier);
+  bool ok = st::mbar_try_wait(bar, parity);
+  uint64_t t0 = 0;
+  for (uint32_t i = 1; !ok; ++i) {
+    ok = st::mbar_try_wait(bar, parity);
+    if (ok || (i & 63u)) continue;
+    if (*abort_flag) break;
+    const uint64_t now = st::globaltimer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > st::wait_limit_ns()) {
+      *abort_flag = 1;
+      break;
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
+// Codes times their scale, twice each, in the input's type.  bf16 in one step: 64 + code, whose unit is bit 1, times s less 72 s, both of which bf16 holds.  fp16 does not
+// hold 72 s of large scales: the code first.
+template <typename T> struct Scale;
+template <> struct Scale<__nv_bfloat16> {
+  __nv_bfloat162 s, less;
+  __device__ __forceinline__ void set(uint32_t low16) {
+    const uint32_t both = __byte_perm(low16, 0, 0x1010);
+    s = *reinterpret_cast<const __nv_bfloat162*>(&both);
+    less = __hmul2(s, __float2bfloat162_rn(-72.0f));
+  }
+  __device__ __forceinline__ uint32_t pair(uint32_t word, int e) const {
+    const uint32_t v = ((e == 0 ? word << 1 : word >> (4 * e - 1)) & 0x001E001Eu) | 0x42804280u;
+    const __nv_bfloat162 d = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&v), s, less);
     return *reinterpret_cast<const uint32_t*>(&d);
   }
-}
-// A bf16 scale, twice, in the input's type.
-template <typename T> __device__ __forceinline__ uint32_t splat(uint32_t low16) {
-  if constexpr (std::is_same<T, __half>::value) {
-    const __half2 h = __float2half2_rn(bf16_bits(low16 & 0xFFFFu));
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    return __byte_perm(low16, 0, 0x1010);
+};
+template <> struct Scale<__half> {
+  __half2 s;
+  __device__ __forceinline__ void set(uint32_t low16) { s = __float2half2_rn(bf16_bits(low16 & 0xFFFFu)); }
+  __device__ __forceinline__ uint32_t pair(uint32_t word, int e) const {
+    const uint32_t v = codes_to_pair<__half>(word, e);
+    const __half2 d = __hmul2(*reinterpret_cast<const __half2*>(&v), s);
+    return *reinterpret_cast<const uint32_t*>(&d);
   }
-}
+};
 __device__ __forceinline__ uint32_t turn_over(uint32_t block) {      // an 8 x 8 block of 16-bit numbers, a row per 4 lanes
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(block));
@@ -85,7 +115,7 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) st::mbar_init(st::smem_u32(&sh.full[i]), 1), st::mbar_init(st::smem_u32(&sh.empty[i]), 1);
-    for (int i = 0; i < kRing; ++i) st::mbar_init(st::smem_u32(&sh.ready[i]), 8), st::mbar_init(st::smem_u32(&sh.taken[i]), 1);
+    for (int i = 0; i < kRing; ++i) st::mbar_init(st::smem_u32(&sh.ready[i]), 4), st::mbar_init(st::smem_u32(&sh.taken[i]), 1);
     for (int i = 0; i < 2; ++i) st::mbar_init(st::smem_u32(&sh.done[i]), 1), st::mbar_init(st::smem_u32(&sh.drained[i]), 4);
     sh.abort = 0;
     st::fence_barrier_init();
@@ -112,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
     for (int t = first_tile; t < p.tiles && ok; t += tile_step) {
       const int down = t % p.tiles_down, m0 = t / p.tiles_down * p.nt;
       for (int c = c0; c < c1; ++c) {
-        if (!(ok = st::mbar_wait_warp(st::smem_u32(&sh.empty[stage]), phase ^ 1u, abort_flag))) break;
+        if (!(ok = wait(sh.empty[stage], phase ^ 1u, abort_flag))) break;
         if (leader) {
           const uint32_t bar = st::smem_u32(&sh.full[stage]);
           st::mbar_arrive_expect_tx(bar, x_bytes + kCodes + kScales);
@@ -136,11 +166,11 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
     uint32_t phase = 0, ring_phase = 0, buf_phase = 0;
     bool ok = true;
     for (int t = first_tile; t < p.tiles && ok; t += tile_step) {
-      if (!(ok = st::mbar_wait_warp(st::smem_u32(&sh.drained[buf]), buf_phase ^ 1u, abort_flag))) break;
+      if (!(ok = wait(sh.drained[buf], buf_phase ^ 1u, abort_flag))) break;
       st::tc_fence_after();
       for (int c = c0; c < c1; ++c) {
-        if (!(ok = st::mbar_wait_warp(st::smem_u32(&sh.full[stage]), phase, abort_flag))) break;
-        if (!(ok = st::mbar_wait_warp(st::smem_u32(&sh.ready[ring]), ring_phase, abort_flag))) break;
+        if (!(ok = wait(sh.full[stage], phase, abort_flag))) break;
+        if (!(ok = wait(sh.ready[ring], ring_phase, abort_flag))) break;
         st::tc_fence_after();
         if (leader) {
           const uint32_t low = st::smem_desc_lo(smem_x + stage * x_bytes, 16);
@@ -158,91 +188,117 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
       if (++buf == 2) buf = 0, buf_phase ^= 1u;
     }
   } else if (warp >= 8) {
-    const int quarter = warp & 3, half = warp >> 2 & 1;      // 16 of the quarter's 32 lanes of tensor memory
-    const uint32_t to = operands + (static_cast<uint32_t>(quarter * 32 + half * 16) << 16);
-    int stage = 0, ring = 0;
+    const int quarter = warp & 3, team = (warp >> 2) - 2;
+    const uint32_t to = operands + (static_cast<uint32_t>(quarter * 32) << 16);
+    int n = team;                                          // the block's chunks count on from tile to tile
+    int stage = team % p.stages, ring = team % kRing;
     uint32_t phase = 0, ring_phase = 0;
-    bool ok = true;
-    for (int t = first_tile; t < p.tiles && ok; t += tile_step) {
-      for (int c = c0; c < c1; ++c) {
-        if (!(ok = st::mbar_wait_warp(st::smem_u32(&sh.full[stage]), phase, abort_flag))) break;
-        const unsigned char* codes = raw + (smem_codes - smem_x) + stage * kCodes;
-        const unsigned char* scales = raw + (smem_scales - smem_x) + stage * kScales;
-        uint32_t word[4], low[4], high[4], r[16];
+    const int own = c1 - c0, all = own * ((p.tiles - first_tile + tile_step - 1) / tile_step);
+    for (; n < all; n += kTeams) {
+      if (!wait(sh.full[stage], phase, abort_flag)) break;
+      const unsigned char* codes = raw + (smem_codes - smem_x) + stage * kCodes;
+      const unsigned char* scales = raw + (smem_scales - smem_x) + stage * kScales;
+      uint32_t r[2][16];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {               // 16 lanes each
         if (TURN) {      // word `quarter % 2 * 2 + half` of column tile quarter / 2, from each of the 4 row tiles
           const int s = (quarter & 1) * 2 + half, group = ((quarter >> 1) * 64 + s * 16) / GROUP;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            word[i] = *reinterpret_cast<const uint32_t*>(codes + (i * 2 + (quarter >> 1)) * kTileBytes + lane * 16 + s * 4);
+            const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + (i * 2 + (quarter >> 1)) * kTileBytes + lane * 16 + s * 4);
             const uint32_t both = *reinterpret_cast<const uint32_t*>(scales + (i * kScaleGroups + group) * 32 + (lane >> 2) * 4);
-            low[i] = splat<T>(both), high[i] = splat<T>(both >> 16);
+            Scale<T> low, high;
+            low.set(both), high.set(both >> 16);
+            r[half][4 * i] = turn_over(low.pair(word, 0)), r[half][4 * i + 1] = turn_over(low.pair(word, 2));
+            r[half][4 * i + 2] = turn_over(high.pair(word, 1)), r[half][4 * i + 3] = turn_over(high.pair(word, 3));
           }
         } else {
           const int u = quarter * 2 + half;
           const uint4 four = *reinterpret_cast<const uint4*>(codes + u * kTileBytes + lane * 16);
-          word[0] = four.x, word[1] = four.y, word[2] = four.z, word[3] = four.w;
+          const uint32_t word[4] = {four.x, four.y, four.z, four.w};
+          Scale<T> low, high;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if (i % (4 / kScaleGroups) == 0) {
               const uint32_t both = *reinterpret_cast<const uint32_t*>(scales + (u * kScaleGroups + i / (4 / kScaleGroups)) * 32 + (lane >> 2) * 4);
-              low[i] = splat<T>(both), high[i] = splat<T>(both >> 16);
-            } else {
-              low[i] = low[i - 1], high[i] = high[i - 1];
+              low.set(both), high.set(both >> 16);
             }
+            r[half][4 * i] = low.pair(word[i], 0), r[half][4 * i + 1] = high.pair(word[i], 1);
+            r[half][4 * i + 2] = low.pair(word[i], 2), r[half][4 * i + 3] = high.pair(word[i], 3);
           }
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t a0 = times<T>(codes_to_pair<T>(word[i], 0), low[i]), a1 = times<T>(codes_to_pair<T>(word[i], 1), high[i]);
-          const uint32_t a2 = times<T>(codes_to_pair<T>(word[i], 2), low[i]), a3 = times<T>(codes_to_pair<T>(word[i], 3), high[i]);
-          if (TURN) {
-            r[4 * i] = turn_over(a0), r[4 * i + 1] = turn_over(a2), r[4 * i + 2] = turn_over(a1), r[4 * i + 3] = turn_over(a3);
-          } else {
-            r[4 * i] = a0, r[4 * i + 1] = a1, r[4 * i + 2] = a2, r[4 * i + 3] = a3;
-          }
-        }
-        if (!(ok = st::mbar_wait_warp(st::smem_u32(&sh.taken[ring]), ring_phase ^ 1u, abort_flag))) break;
-        st::tc_fence_after();
-        tmem_st_16x32(to + ring * 32, r);
-        st::tmem_st_wait();
-        st::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) st::mbar_arrive(st::smem_u32(&sh.ready[ring]));
-        if (++stage == p.stages) stage = 0, phase ^= 1u;
-        if (++ring == kRing) ring = 0, ring_phase ^= 1u;
       }
+      if (!wait(sh.taken[ring], ring_phase ^ 1u, abort_flag)) break;
+      st::tc_fence_after();
+      tmem_st_16x32(to + ring * 32, r[0]);
+      tmem_st_16x32(to + (16u << 16) + ring * 32, r[1]);
+      st::tmem_st_wait();
+      st::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) st::mbar_arrive(st::smem_u32(&sh.ready[ring]));
+      stage += kTeams;
+      while (stage >= p.stages) stage -= p.stages, phase ^= 1u;
+      ring += kTeams;
+      if (ring >= kRing) ring -= kRing, ring_phase ^= 1u;
     }
   } else if (warp >= 4) {
     const int quarter = warp & 3;
     const T* bias = static_cast<const T*>(p.bias);
     const T* residual = static_cast<const T*>(p.residual);
     T* y = static_cast<T*>(p.y);
+    unsigned char* out = sh.out[quarter];
     int buf = 0;
     uint32_t buf_phase = 0;
     for (int t = first_tile; t < p.tiles; t += tile_step) {
-      if (!st::mbar_wait_warp(st::smem_u32(&sh.done[buf]), buf_phase, abort_flag)) break;
+      if (!wait(sh.done[buf], buf_phase, abort_flag)) break;
       st::tc_fence_after();
-      const int r = t % p.tiles_down * 128 + quarter * 32 + lane, m0 = t / p.tiles_down * p.nt;
+      const int r0 = t % p.tiles_down * 128 + quarter * 32, r = r0 + lane, m0 = t / p.tiles_down * p.nt, end = min(p.nt, p.tokens - m0);
       const float b = bias != nullptr && p.parts == 1 && r < p.outs ? to_float(bias[r]) : 0.0f;
 #pragma unroll 1
-      for (int at = 0; at < p.nt; at += 16) {
-        uint32_t v[16];
-        st::tmem_ld_32x16(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kMostTokens + at, v);
+      for (int at = 0; at < end; at += 32) {
+        uint32_t v[32];
+        st::tmem_ld_32x32(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kMostTokens + at, v);
         st::tmem_ld_wait();
         if (p.parts > 1) {      // this block's share of the sums, for the cluster
-          float* sums = reinterpret_cast<float*>(raw);
+          float* sums = reinterpret_cast<float*>(raw) + quarter * 32 + lane;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sums[(at + i) * 128 + quarter * 32 + lane] = __uint_as_float(v[i]);
-        } else if (r < p.outs) {
+          for (int i = 0; i < 32; ++i)
+            if (at + i < end) sums[(at + i) * 128] = __uint_as_float(v[i]);
+          continue;
+        }
+        float f[32];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int m = m0 + at + i;
-            if (m < p.tokens) {
-              float f = activate(__uint_as_float(v[i]) + b, p.act);
-              if (residual) f += to_float(residual[m * p.residual_row + r]);
-              y[m * p.y_row + r] = from_float<T>(f);
-            }
+        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]) + b;
+        if (p.act == 1) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = activate(f[i], 1);
+        } else if (p.act == 2) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = st::gelu_tanh(f[i]);
+        }
+        if (residual && r < p.outs) {
+          const T* from = residual + (m0 + at) * p.residual_row + r;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (at + i < end) f[i] += to_float(*from);
+            from += p.residual_row;
           }
+        }
+        // to rows of 32: a token's 64 bytes, which 4 lanes take to memory
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) *reinterpret_cast<T*>(out + i * 64 + lane * 2) = from_float<T>(f[i]);
+        __syncwarp();
+        T* to = y + (m0 + at) * p.y_row + r0;
+        if (p.wide_rows) {
+          const int col = (lane & 3) * 8;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int m = i * 8 + (lane >> 2);
+            if (at + m < end && r0 + col < p.outs) *reinterpret_cast<uint4*>(to + m * p.y_row + col) = *reinterpret_cast<const uint4*>(out + m * 64 + col * 2);
+          }
+        } else if (r < p.outs) {
+          for (int i = 0; i < 32 && at + i < end; ++i) to[i * p.y_row + lane] = *reinterpret_cast<const T*>(out + i * 64 + lane * 2);
         }
       }
       st::tc_fence_before();
@@ -292,7 +348,8 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
 template <typename T, bool TURN, int GROUP>
 int launch(const st4::WideArgs& a, cudaStream_t stream) {
   const int sms = st::sm_count();
-  WideParams p{a.bias, a.residual, a.y, a.residual_row, a.y_row, a.tokens, TURN ? a.cols : a.rows, ((TURN ? a.rows : a.cols) + 63) / 64, 0, 0, 0, 0, 1, a.act, st::error_word()};
+  WideParams p{a.bias, a.residual, a.y, a.residual_row, a.y_row, a.tokens, TURN ? a.cols : a.rows, ((TURN ? a.rows : a.cols) + 63) / 64, 0, 0, 0, 0, 1, a.act, false, st::error_word()};
+  p.wide_rows = (reinterpret_cast<uintptr_t>(a.y) & 15) == 0 && a.y_row % 8 == 0 && p.outs % 8 == 0;
   p.tiles_down = (p.outs + 127) / 128;
   // tokens of a tile: the size whose rounds over the SMs take the fewest tokens' time; a tile of fewer than 64 takes as long as one of 64, its weights' conversion
   long long best = -1;
