@@ -13,16 +13,20 @@
 namespace {
 using namespace st4;
 
-constexpr int kRing = 4;                     // weight operands in tensor memory, 32 columns each, behind two results
-constexpr int kMostTokens = 192;             // of a tile: 2 * 192 + 4 * 32 = 512 columns
-constexpr int kMostStages = 12;
+constexpr int kMostRing = 6;                 // weight operands in tensor memory, 64 columns each, behind two results: as many as fit
+constexpr int kMostTokens = 192;             // of a tile: 2 * 192 + 2 * 64 = 512 columns
+constexpr int kMostStages = 8;
+constexpr int kMostParts = 8;                // blocks of a cluster
+constexpr int kCodes = 8192;                 // bytes of a stage: 128 rows by 128 columns of the weights, 8 by 2 tiles
 constexpr int kTeams = 3;                    // of 4 warps, one for each 32 lanes of tensor memory, that take weights in turn
 constexpr int kThreads = 256 + kTeams * 128; // warps: 0 copies, 1 products, 4-7 results, from 8 on weights
 constexpr int kRoom = 200 * 1024;            // of shared memory for stages
 
 struct alignas(16) Shared {
   unsigned char out[4][2048];      // 32 tokens by 32 rows of the result for each of its warps
-  unsigned long long full[kMostStages], empty[kMostStages], ready[kRing], taken[kRing], done[2], drained[2];
+  // Copies land in any order, and a team looks at every third stage only: with one barrier a stage it could come by before the turn ahead of its own had
+  // landed, which the parity of its own would take for done.  Two barriers a stage, in turns: the turn before on the same one is long used up.
+  unsigned long long full[2 * kMostStages], empty[kMostStages], ready[kMostRing], taken[kMostRing], done[2], drained[2];
   uint32_t tmem;
   int abort;
 };
@@ -32,8 +36,8 @@ struct WideParams {
   const void* residual;
   void* y;
   long long residual_row, y_row;
-  int tokens, outs, depth;      // outs: rows of the result's weights side; depth: chunks of 64 of the contraction
-  int nt, stages, tiles_down, tiles, parts, act;
+  int tokens, outs, depth;      // outs: columns of the result; depth: steps of 128 of the contraction
+  int nt, stages, ring, teams, tiles_down, tiles, parts, act;
   bool wide_rows;      // rows of y lie on 16-byte boundaries and are whole vectors
   unsigned* err;
 };
@@ -103,19 +107,18 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
   extern __shared__ __align__(1024) unsigned char unaligned[];
   __shared__ Shared sh;
   unsigned char* raw = unaligned + (-st::smem_u32(unaligned) & 1023u);      // the swizzle counts from 1024-byte boundaries
-  constexpr int kCodes = 4096;                                                     // bytes of a stage: 8 tiles of 512
-  constexpr int kScaleGroups = TURN ? 128 / GROUP : GROUP == 32 ? 2 : 1;            // of a stage and tile of 16 rows
-  constexpr int kScales = (TURN ? 4 : 8) * kScaleGroups * 32;
+  constexpr int kScaleGroups = 128 / GROUP, kScales = 8 * kScaleGroups * 32;      // of a stage: groups of a tile row, bytes
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   volatile int* abort_flag = &sh.abort;
   const int part = p.parts > 1 ? static_cast<int>(st::cluster_ctarank()) : 0;
   const int first_tile = blockIdx.x / p.parts, tile_step = gridDim.x / p.parts;
   const int c0 = p.depth * part / p.parts, c1 = p.depth * (part + 1) / p.parts;
-  const uint32_t x_bytes = p.nt * 128, smem_x = st::smem_u32(raw), smem_codes = smem_x + p.stages * x_bytes, smem_scales = smem_codes + p.stages * kCodes;
+  const uint32_t x_bytes = p.nt * 256, smem_x = st::smem_u32(raw), smem_codes = smem_x + p.stages * x_bytes, smem_scales = smem_codes + p.stages * kCodes;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < p.stages; ++i) st::mbar_init(st::smem_u32(&sh.full[i]), 1), st::mbar_init(st::smem_u32(&sh.empty[i]), 1);
-    for (int i = 0; i < kRing; ++i) st::mbar_init(st::smem_u32(&sh.ready[i]), 4), st::mbar_init(st::smem_u32(&sh.taken[i]), 1);
+    for (int i = 0; i < 2 * p.stages; ++i) st::mbar_init(st::smem_u32(&sh.full[i]), 1);
+    for (int i = 0; i < p.stages; ++i) st::mbar_init(st::smem_u32(&sh.empty[i]), 1);
+    for (int i = 0; i < p.ring; ++i) st::mbar_init(st::smem_u32(&sh.ready[i]), 4), st::mbar_init(st::smem_u32(&sh.taken[i]), 1);
     for (int i = 0; i < 2; ++i) st::mbar_init(st::smem_u32(&sh.done[i]), 1), st::mbar_init(st::smem_u32(&sh.drained[i]), 4);
     sh.abort = 0;
     st::fence_barrier_init();
@@ -131,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
   st::tc_fence_before();
   __syncthreads();
   st::tc_fence_after();
-  const uint32_t tmem = sh.tmem, operands = tmem + 2 * kMostTokens;
+  const uint32_t tmem = sh.tmem, operands = tmem + 512 - 64 * p.ring;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (warp == 0) {
@@ -144,16 +147,13 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
       for (int c = c0; c < c1; ++c) {
         if (!(ok = wait(sh.empty[stage], phase ^ 1u, abort_flag))) break;
         if (leader) {
-          const uint32_t bar = st::smem_u32(&sh.full[stage]);
+          const uint32_t bar = st::smem_u32(&sh.full[stage + phase * p.stages]);
           st::mbar_arrive_expect_tx(bar, x_bytes + kCodes + kScales);
-          if (TURN) {      // 64 weight rows (4 tiles) by 128 columns (2 tiles)
-            st::tma_load_2d(smem_codes + stage * kCodes, &map_codes, bar, down * 256, c * 4);
-            st::tma_load_2d(smem_scales + stage * kScales, &map_scales, bar, down * (128 / GROUP) * 16, c * 4);
-          } else {         // 128 weight rows by 64 columns
-            st::tma_load_2d(smem_codes + stage * kCodes, &map_codes, bar, c * 128, down * 8);
-            st::tma_load_2d(smem_scales + stage * kScales, &map_scales, bar, c * 64 / GROUP * 16, down * 8);
-          }
-          st::tma_load_2d(smem_x + stage * x_bytes, &map_x, bar, c * 64, m0);
+          const int row = TURN ? c : down, col = TURN ? down : c;      // of the 128 x 128 blocks of the weights
+          st::tma_load_2d(smem_codes + stage * kCodes, &map_codes, bar, col * 256, row * 8);
+          st::tma_load_2d(smem_scales + stage * kScales, &map_scales, bar, col * kScaleGroups * 16, row * 8);
+          st::tma_load_2d(smem_x + stage * x_bytes, &map_x, bar, c * 128, m0);
+          st::tma_load_2d(smem_x + stage * x_bytes + p.nt * 128, &map_x, bar, c * 128 + 64, m0);
         }
         if (++stage == p.stages) stage = 0, phase ^= 1u;
       }
@@ -163,83 +163,90 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
     const uint32_t idesc = st::make_idesc_bf16(128, p.nt, false, false) & ~(std::is_same<T, __half>::value ? (1u << 7 | 1u << 10) : 0u);
     const uint32_t high = st::smem_desc_hi(1024);
     int stage = 0, ring = 0, buf = 0;
-    uint32_t phase = 0, ring_phase = 0, buf_phase = 0;
+    uint32_t ring_phase = 0, buf_phase = 0;
     bool ok = true;
     for (int t = first_tile; t < p.tiles && ok; t += tile_step) {
       if (!(ok = wait(sh.drained[buf], buf_phase ^ 1u, abort_flag))) break;
       st::tc_fence_after();
       for (int c = c0; c < c1; ++c) {
-        if (!(ok = wait(sh.full[stage], phase, abort_flag))) break;
-        if (!(ok = wait(sh.ready[ring], ring_phase, abort_flag))) break;
+        if (!(ok = wait(sh.ready[ring], ring_phase, abort_flag))) break;      // its team has waited for the stage, x with it
         st::tc_fence_after();
         if (leader) {
           const uint32_t low = st::smem_desc_lo(smem_x + stage * x_bytes, 16);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            st::umma_bf16_ts_split(tmem + buf * kMostTokens, operands + ring * 32 + k * 8, low + 2 * k, high, idesc, c > c0 || k > 0);
+          for (int k = 0; k < 8; ++k)
+            st::umma_bf16_ts_split(tmem + buf * p.nt, operands + ring * 64 + k * 8, low + (k >> 2) * p.nt * 8 + 2 * (k & 3), high, idesc, c > c0 || k > 0);
           st::umma_commit(st::smem_u32(&sh.empty[stage]));
           st::umma_commit(st::smem_u32(&sh.taken[ring]));
           if (c == c1 - 1) st::umma_commit(st::smem_u32(&sh.done[buf]));
         }
         __syncwarp();
-        if (++stage == p.stages) stage = 0, phase ^= 1u;
-        if (++ring == kRing) ring = 0, ring_phase ^= 1u;
+        if (++stage == p.stages) stage = 0;
+        if (++ring == p.ring) ring = 0, ring_phase ^= 1u;
       }
       if (++buf == 2) buf = 0, buf_phase ^= 1u;
     }
   } else if (warp >= 8) {
     const int quarter = warp & 3, team = (warp >> 2) - 2;
     const uint32_t to = operands + (static_cast<uint32_t>(quarter * 32) << 16);
-    int n = team;                                          // the block's chunks count on from tile to tile
-    int stage = team % p.stages, ring = team % kRing;
-    uint32_t phase = 0, ring_phase = 0;
+    int n = team;                                          // the block's stages count on from tile to tile
+    int stage = team % p.stages, filled = team, ring = team % p.ring;
+    uint32_t fill_phase = 0, ring_phase = team / p.ring & 1;
     const int own = c1 - c0, all = own * ((p.tiles - first_tile + tile_step - 1) / tile_step);
-    for (; n < all; n += kTeams) {
-      if (!wait(sh.full[stage], phase, abort_flag)) break;
+    for (; n < all && team < p.teams; n += p.teams) {
+      if (!wait(sh.full[filled], fill_phase, abort_flag)) break;
       const unsigned char* codes = raw + (smem_codes - smem_x) + stage * kCodes;
       const unsigned char* scales = raw + (smem_scales - smem_x) + stage * kScales;
-      uint32_t r[2][16];
+      uint32_t all_r[2][2][16];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {               // 16 lanes each
-        if (TURN) {      // word `quarter % 2 * 2 + half` of column tile quarter / 2, from each of the 4 row tiles
-          const int s = (quarter & 1) * 2 + half, group = ((quarter >> 1) * 64 + s * 16) / GROUP;
+      for (int k = 0; k < 2; ++k) {                          // 64 of the 128 numbers of every lane
+        auto& r = all_r[k];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + (i * 2 + (quarter >> 1)) * kTileBytes + lane * 16 + s * 4);
-            const uint32_t both = *reinterpret_cast<const uint32_t*>(scales + (i * kScaleGroups + group) * 32 + (lane >> 2) * 4);
-            Scale<T> low, high;
-            low.set(both), high.set(both >> 16);
-            r[half][4 * i] = turn_over(low.pair(word, 0)), r[half][4 * i + 1] = turn_over(low.pair(word, 2));
-            r[half][4 * i + 2] = turn_over(high.pair(word, 1)), r[half][4 * i + 3] = turn_over(high.pair(word, 3));
-          }
-        } else {
-          const int u = quarter * 2 + half;
-          const uint4 four = *reinterpret_cast<const uint4*>(codes + u * kTileBytes + lane * 16);
-          const uint32_t word[4] = {four.x, four.y, four.z, four.w};
-          Scale<T> low, high;
+        for (int half = 0; half < 2; ++half) {               // 16 lanes each
+          if (TURN) {      // word `quarter % 2 * 2 + half` of column tile quarter / 2, from 4 of the row tiles
+            const int s = (quarter & 1) * 2 + half, group = ((quarter >> 1) * 64 + s * 16) / GROUP;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (i % (4 / kScaleGroups) == 0) {
-              const uint32_t both = *reinterpret_cast<const uint32_t*>(scales + (u * kScaleGroups + i / (4 / kScaleGroups)) * 32 + (lane >> 2) * 4);
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + ((4 * k + i) * 2 + (quarter >> 1)) * kTileBytes + lane * 16 + s * 4);
+              const uint32_t both = *reinterpret_cast<const uint32_t*>(scales + ((4 * k + i) * kScaleGroups + group) * 32 + (lane >> 2) * 4);
+              Scale<T> low, high;
               low.set(both), high.set(both >> 16);
+              r[half][4 * i] = turn_over(low.pair(word, 0)), r[half][4 * i + 1] = turn_over(low.pair(word, 2));
+              r[half][4 * i + 2] = turn_over(high.pair(word, 1)), r[half][4 * i + 3] = turn_over(high.pair(word, 3));
             }
-            r[half][4 * i] = low.pair(word[i], 0), r[half][4 * i + 1] = high.pair(word[i], 1);
-            r[half][4 * i + 2] = low.pair(word[i], 2), r[half][4 * i + 3] = high.pair(word[i], 3);
+          } else {
+            const int u = quarter * 2 + half;
+            const uint4 four = *reinterpret_cast<const uint4*>(codes + (u * 2 + k) * kTileBytes + lane * 16);
+            const uint32_t word[4] = {four.x, four.y, four.z, four.w};
+            Scale<T> low, high;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (i == 0 || (GROUP == 32 && i == 2)) {
+                const uint32_t both = *reinterpret_cast<const uint32_t*>(scales + (u * kScaleGroups + (k * 64 + i * 16) / GROUP) * 32 + (lane >> 2) * 4);
+                low.set(both), high.set(both >> 16);
+              }
+              r[half][4 * i] = low.pair(word[i], 0), r[half][4 * i + 1] = high.pair(word[i], 1);
+              r[half][4 * i + 2] = low.pair(word[i], 2), r[half][4 * i + 3] = high.pair(word[i], 3);
+            }
           }
         }
       }
       if (!wait(sh.taken[ring], ring_phase ^ 1u, abort_flag)) break;
       st::tc_fence_after();
-      tmem_st_16x32(to + ring * 32, r[0]);
-      tmem_st_16x32(to + (16u << 16) + ring * 32, r[1]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        tmem_st_16x32(to + ring * 64 + k * 32, all_r[k][0]);
+        tmem_st_16x32(to + (16u << 16) + ring * 64 + k * 32, all_r[k][1]);
+      }
       st::tmem_st_wait();
       st::tc_fence_before();
       __syncwarp();
       if (lane == 0) st::mbar_arrive(st::smem_u32(&sh.ready[ring]));
-      stage += kTeams;
-      while (stage >= p.stages) stage -= p.stages, phase ^= 1u;
-      ring += kTeams;
-      if (ring >= kRing) ring -= kRing, ring_phase ^= 1u;
+      stage = (stage + p.teams) % p.stages;
+      filled += p.teams;
+      if (filled >= 2 * p.stages) filled -= 2 * p.stages, fill_phase ^= 1u;
+      ring += p.teams;
+      while (ring >= p.ring) ring -= p.ring, ring_phase ^= 1u;
     }
   } else if (warp >= 4) {
     const int quarter = warp & 3;
@@ -257,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
 #pragma unroll 1
       for (int at = 0; at < end; at += 32) {
         uint32_t v[32];
-        st::tmem_ld_32x32(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kMostTokens + at, v);
+        st::tmem_ld_32x32(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * p.nt + at, v);
         st::tmem_ld_wait();
         if (p.parts > 1) {      // this block's share of the sums, for the cluster
           float* sums = reinterpret_cast<float*>(raw) + quarter * 32 + lane;
@@ -320,12 +327,13 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
     for (int at = part + p.parts * (threadIdx.x >> 7); at < p.nt; at += p.parts * (kThreads / 128)) {
       const int m = m0 + at;
       if (m >= p.tokens || r >= p.outs) break;
-      float f = 0.0f;
-      for (int q = 0; q < p.parts; ++q) {
-        float s;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(s) : "r"(st::cluster_map(smem_x + (at * 128 + (threadIdx.x & 127)) * 4, q)));
-        f += s;
-      }
+      float s[kMostParts], f = 0.0f;
+#pragma unroll
+      for (int q = 0; q < kMostParts; ++q)      // all on their way before the first is used
+        if (q < p.parts) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(s[q]) : "r"(st::cluster_map(smem_x + (at * 128 + (threadIdx.x & 127)) * 4, q)));
+#pragma unroll
+      for (int q = 0; q < kMostParts; ++q)
+        if (q < p.parts) f += s[q];
       if (bias) f += to_float(bias[r]);
       f = activate(f, p.act);
       if (residual) f += to_float(residual[m * p.residual_row + r]);
@@ -348,22 +356,45 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
 template <typename T, bool TURN, int GROUP>
 int launch(const st4::WideArgs& a, cudaStream_t stream) {
   const int sms = st::sm_count();
-  WideParams p{a.bias, a.residual, a.y, a.residual_row, a.y_row, a.tokens, TURN ? a.cols : a.rows, ((TURN ? a.rows : a.cols) + 63) / 64, 0, 0, 0, 0, 1, a.act, false, st::error_word()};
+  WideParams p{a.bias, a.residual, a.y, a.residual_row, a.y_row, a.tokens, TURN ? a.cols : a.rows, ((TURN ? a.rows : a.cols) + 127) / 128, 0, 0, 0, 0, 0, 0, 1, a.act, false, st::error_word()};
   p.wide_rows = (reinterpret_cast<uintptr_t>(a.y) & 15) == 0 && a.y_row % 8 == 0 && p.outs % 8 == 0;
   p.tiles_down = (p.outs + 127) / 128;
-  // tokens of a tile: the size whose rounds over the SMs take the fewest tokens' time; a tile of fewer than 64 takes as long as one of 64, its weights' conversion
+  constexpr int smem = kRoom + 1024;      // always: one block per SM
+  static int clusters[st::kMaxDevices][kMostParts + 1];      // that run at the same time, by their size
+  int (&at_once)[kMostParts + 1] = clusters[st::current_device()];
+  if (at_once[1] == 0) {
+    ST_CUDA_CHECK(cudaFuncSetAttribute(wide_kernel<T, TURN, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    for (int n = kMostParts; n > 0; --n) {
+      cudaLaunchAttribute attr{};
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = n, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(n * sms), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem, cfg.attrs = &attr, cfg.numAttrs = 1;
+      int found = 0;
+      ST_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&found, wide_kernel<T, TURN, GROUP>, &cfg));
+      at_once[n] = n > 1 ? found : sms;
+    }
+  }
+  // Tokens of a tile, and blocks that share one, by what steps of 128 in a row cost: its tokens' time and that of 100 more, with fewer than 3 weight operands (above
+  // 160 tokens) of 140 more; a cluster's start and join as much as 1150 (2.4 us).  4096 x 8192 x 2048 in tiles of 96 125 us, 128 112, 160 104, 176 111, 192 106;
+  // 64 x 2048 x 8192 with 1 block to a tile 24.4 us, 2 17.8, 4 12.3, 6 10.7.  Clusters that do not all run at once take twice as long: with 8 blocks 18.4.
   long long best = -1;
   for (int nt = kMostTokens; nt >= 16; nt -= 16) {
-    const long long across = (a.tokens + nt - 1) / nt, rounds = (across * p.tiles_down + sms - 1) / sms, cost = rounds * (nt > 64 ? nt : 64);
-    if (best < 0 || cost < best || (cost == best && across == (a.tokens + p.nt - 1) / p.nt)) best = cost, p.nt = nt;
+    const long long tiles = static_cast<long long>(p.tiles_down) * ((a.tokens + nt - 1) / nt);
+    for (int parts = 1; parts <= kMostParts && parts <= p.depth; ++parts) {
+      if (parts > 1 && tiles > at_once[parts]) continue;
+      const long long steps = parts > 1 ? (p.depth + parts - 1) / parts : (tiles + sms - 1) / sms * p.depth;
+      const long long cost = steps * (nt + (nt > 160 ? 140 : 100)) + (parts > 1 ? 1150 : 0);
+      if (best < 0 || cost < best) best = cost, p.nt = nt, p.parts = parts, p.tiles = static_cast<int>(min(tiles, 2147483647LL));
+    }
   }
-  const long long tiles = static_cast<long long>(p.tiles_down) * ((a.tokens + p.nt - 1) / p.nt);
-  if (tiles > 1 << 30) return st::fail(ST_ERR_TOO_LARGE, "int4: too many rows");
-  p.tiles = static_cast<int>(tiles);
-  while (p.parts < 8 && p.tiles * p.parts * 2 <= sms && p.depth >= 4 * p.parts) p.parts *= 2;
-  constexpr int kScales = (TURN ? 4 * (128 / GROUP) : 8 * (GROUP == 32 ? 2 : 1)) * 32;
-  const int stage = p.nt * 128 + 4096 + kScales;
+  if (p.tiles > 1 << 30) return st::fail(ST_ERR_TOO_LARGE, "int4: too many rows");
+  const int stage = p.nt * 256 + kCodes + 8 * (128 / GROUP) * 32;
   p.stages = min(kMostStages, kRoom / stage);
+  p.ring = min(kMostRing, (512 - 2 * p.nt) / 64);
+  p.teams = min(kTeams, min(p.ring, p.stages));      // no more: a barrier tells one turn of a ring from the next, not from the one after
+  // a stage two turns back is used up: the team's last operand waited for the product `ring` before it
+  if (2 * p.stages < p.teams + p.ring) return st::fail(ST_ERR_INVALID, "int4: too few stages");
   CUtensorMap mx, mc, ms;
   const uint64_t units = (a.rows + 15) / 16, chunks = (a.cols + 63) / 64, groups = (a.cols + GROUP - 1) / GROUP;
   {
@@ -375,20 +406,13 @@ int launch(const st4::WideArgs& a, cudaStream_t stream) {
   }
   {
     const uint64_t dims[2] = {chunks * 128, units}, strides[1] = {chunks * 512};
-    const uint32_t box[2] = {TURN ? 256u : 128u, TURN ? 4u : 8u};
+    const uint32_t box[2] = {256, 8};
     if (!st::encode_tmap(&mc, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, a.codes, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE)) return ST_ERR_CUDA;
   }
   {
     const uint64_t dims[2] = {groups * 16, units}, strides[1] = {groups * 32};
-    const uint32_t box[2] = {static_cast<uint32_t>(TURN ? 128 / GROUP * 16 : GROUP == 32 ? 32 : 16), TURN ? 4u : 8u};
+    const uint32_t box[2] = {128 / GROUP * 16, 8};
     if (!st::encode_tmap(&ms, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.scales, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE)) return ST_ERR_CUDA;
-  }
-  constexpr int smem = kRoom + 1024;      // always: one block per SM
-  static bool opted[st::kMaxDevices];
-  const int dev = st::current_device();
-  if (!opted[dev]) {
-    ST_CUDA_CHECK(cudaFuncSetAttribute(wide_kernel<T, TURN, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    opted[dev] = true;
   }
   const int blocks = p.parts > 1 ? p.tiles * p.parts : min(p.tiles, sms);
   const cudaError_t e = st::chained(wide_kernel<T, TURN, GROUP>, dim3(blocks), dim3(kThreads), smem, stream, p.parts)(mx, mc, ms, p);
