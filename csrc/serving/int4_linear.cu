@@ -18,6 +18,7 @@ struct LinearParams {
   void* y;
   long long x_row, residual_row, y_row;      // in elements
   int tokens, rows, cols, groups, chunks, units, group, act;
+  bool wide;      // rows of x lie on 16-byte boundaries
 };
 
 template <typename T> __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]);
@@ -32,117 +33,190 @@ template <> __device__ __forceinline__ void mma<__half>(float (&d)[4], const uin
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// Elements k and k + 1 of a row of x as one word; what lies behind the row's end is zero.
-template <typename T, bool PAIRS>
-__device__ __forceinline__ uint32_t load_pair(const T* row, int k, int cols) {
-  if (PAIRS) return k < cols ? *reinterpret_cast<const uint32_t*>(row + k) : 0u;
-  const uint16_t* h = reinterpret_cast<const uint16_t*>(row);
-  return (k < cols ? h[k] : 0u) | (k + 1 < cols ? static_cast<uint32_t>(h[k + 1]) << 16 : 0u);
+// x in shared memory: a token's 64 columns of a chunk are 128 bytes, in which the 16 bytes at 64 p + 16 t hold what lane t of a row's 4 takes to steps 2 p and 2 p + 1:
+// columns 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of each.  Tokens are 64 bytes more than a whole number of 128 apart, so that 8 lanes read from all banks.
+constexpr int kWarps = 8;
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ void stage_tokens(const T* x, long long x_row, uint32_t* to, int stride, int tokens, int room, int k0, int columns, int cols) {
+  // vectors of 8 columns: step s, half h of it; word t of them goes to 16 (s / 2) + 4 t + 2 (s % 2) + h
+  const int vectors = columns / 8;
+  for (int i = threadIdx.x; i < room * vectors; i += kWarps * 32) {
+    const int m = i / vectors, j = i - m * vectors, k = k0 + j * 8;
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (m < tokens) {
+      const T* from = x + m * x_row + k;
+      if (WIDE && k + 8 <= cols) {
+        const uint4 v = *reinterpret_cast<const uint4*>(from);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+      } else {
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(from);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (k + e < cols) w[e / 2] |= static_cast<uint32_t>(h[e]) << (16 * (e % 2));
+      }
+    }
+    uint32_t* at = to + m * stride + (j >> 3) * 32 + ((j >> 2) & 1) * 16 + ((j >> 1) & 1) * 2 + (j & 1);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) at[4 * t] = w[t];
+  }
 }
 
-// A warp multiplies U tiles of 16 weight rows, one under another, by NT tiles of 8 tokens: chunk by chunk of 64 columns, those of the
-// block's warps interleaved.  The weights are the matrix instruction's 16-row operand, the tokens its 8 columns.  The products of a group are
-// summed on their own and take its scale in fp32, so codes enter as the whole numbers that they are.
-template <typename T, int NT, int U, int GROUP, int WARPS, bool PAIRS>
-__global__ void __launch_bounds__(WARPS * 32) linear_kernel(const T* x, const uint8_t* codes, const __nv_bfloat16* scales, const T* bias, const T* residual, T* y,
-                                                            const LinearParams p) {
-  extern __shared__ float part[];      // [warp][token][row]
-  chain_begin(x, codes, scales, bias, residual, y);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int u0 = blockIdx.x * U, m0 = blockIdx.y * NT * 8;
-  constexpr int kGroups = GROUP >= 64 ? 1 : 2, kSteps = 4 / kGroups;      // groups of a chunk, steps of 16 columns in each
-  float acc[U][NT][4] = {};
-  for (int c = warp; c < p.chunks; c += WARPS) {
-    uint4 w[U];
-    uint32_t s[U][kGroups];
+// What a warp reads of a tile row: C chunks of codes side by side, 16 bytes a lane each, and their scales, 8 words (of 2 rows) to a group.
+template <int C, int GROUP>
+struct Slice {
+  static constexpr int kScales = C * 64 / GROUP > 0 ? C * 64 / GROUP : 1, kWords = (kScales * 8 + 31) / 32;
+  uint4 w[C];
+  uint32_t s[kWords];
+  __device__ __forceinline__ void load(const uint8_t* codes, const __nv_bfloat16* scales, long long u, int c0, int chunks, int groups, int lane) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const long long u = min(u0 + i, p.units - 1);
-      w[i] = *reinterpret_cast<const uint4*>(codes + (u * p.chunks + c) * kTileBytes + lane * 16);
+    for (int i = 0; i < C; ++i)
+      w[i] = c0 + i < chunks ? *reinterpret_cast<const uint4*>(codes + (u * chunks + c0 + i) * kTileBytes + lane * 16) : make_uint4(0, 0, 0, 0);
+    const int g0 = c0 * 64 / GROUP;
 #pragma unroll
-      for (int k = 0; k < kGroups; ++k) {
-        const int at = min(c * kTileCols / GROUP + k, p.groups - 1);
-        s[i][k] = *reinterpret_cast<const uint32_t*>(scales + (u * p.groups + at) * 16 + 2 * g);
-      }
-    }
-    uint32_t b[NT][8];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int m = m0 + n * 8 + g;
-      const T* row = x + static_cast<long long>(m) * p.x_row;
-#pragma unroll
-      for (int h = 0; h < 8; ++h) b[n][h] = m < p.tokens ? load_pair<T, PAIRS>(row, c * kTileCols + 8 * h + 2 * t, p.cols) : 0u;
-    }
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const uint32_t word[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-      for (int k = 0; k < kGroups; ++k) {
-        float sum[NT][4] = {};
-#pragma unroll
-        for (int j = k * kSteps; j < (k + 1) * kSteps; ++j) {
-          const uint32_t a[4] = {codes_to_pair<T>(word[j], 0), codes_to_pair<T>(word[j], 1), codes_to_pair<T>(word[j], 2), codes_to_pair<T>(word[j], 3)};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma<T>(sum[n], a, b[n][2 * j], b[n][2 * j + 1], sum[n]);
-        }
-        const float low = bf16_bits(s[i][k]), high = bf16_bits(s[i][k] >> 16);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          acc[i][n][0] = fmaf(low, sum[n][0], acc[i][n][0]);
-          acc[i][n][1] = fmaf(low, sum[n][1], acc[i][n][1]);
-          acc[i][n][2] = fmaf(high, sum[n][2], acc[i][n][2]);
-          acc[i][n][3] = fmaf(high, sum[n][3], acc[i][n][3]);
-        }
-      }
+    for (int i = 0; i < kWords; ++i) {
+      const int at = i * 32 + lane;
+      s[i] = at < kScales * 8 && g0 + at / 8 < groups ? *reinterpret_cast<const uint32_t*>(scales + (u * groups + g0) * 16 + at * 2) : 0u;
     }
   }
-  // the warps' sums, in the order of the warps
-  constexpr int kRows = U * kTileRows, kTokens = NT * 8;
+  // of chunk i, half k of it where groups are halves
+  __device__ __forceinline__ uint32_t scale(int i, int k, int lane) const {
+    const int at = ((i * 64 + k * 32) / GROUP) * 8;
+    return __shfl_sync(0xffffffffu, s[at / 32], at % 32 + (lane >> 2));
+  }
+};
+
+// Blocks take tile rows (16 weight rows) in turns; their 8 warps share the columns, C chunks of 64 each and that for `phases` stretches of 8 C.  The weights are the matrix
+// instruction's 16-row operand, NT times 8 tokens its columns.  The products of a group are summed on their own and take its scale in fp32, so codes enter as the
+// whole numbers that they are.  The next row's codes are on their way while one is multiplied.
+template <typename T, int NT, int C, int GROUP>
+__global__ void __launch_bounds__(kWarps * 32) linear_kernel(const T* x, const uint8_t* codes, const __nv_bfloat16* scales, const T* bias, const T* residual, T* y,
+                                                            const LinearParams p) {
+  extern __shared__ __align__(16) uint32_t room[];
+  chain_begin(x, codes, scales, bias, residual, y);
+  constexpr int kTokens = NT * 8, kOuts = kTokens * kTileRows, kColumns = kWarps * C * kTileCols;
+  constexpr int kStride = kColumns / 2 + 16;                   // words of a token
+  constexpr int kGroups = GROUP >= 64 ? 1 : 2, kSteps = 4 / kGroups;      // groups of a chunk, steps of 16 columns in each
+  uint32_t* tokens = room;
+  float* part = reinterpret_cast<float*>(room + kTokens * kStride);      // two of [warp][token][row]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int phases = (p.cols + kColumns - 1) / kColumns;
+  Slice<C, GROUP> now;
+  int u = blockIdx.x;
+  now.load(codes, scales, u, warp * C, p.chunks, p.groups, lane);
+  const auto stage = [&](int ph) {
+    const int columns = min(kColumns, (p.cols - ph * kColumns + 63) / 64 * 64);
+    if (p.wide) stage_tokens<T, true>(x, p.x_row, tokens, kStride, p.tokens, kTokens, ph * kColumns, columns, p.cols);
+    else stage_tokens<T, false>(x, p.x_row, tokens, kStride, p.tokens, kTokens, ph * kColumns, columns, p.cols);
+  };
+  if (phases == 1) {
+    stage(0);
+    __syncthreads();
+  }
+  for (int flip = 0; u < p.units; u += gridDim.x, flip ^= 1) {
+    // the element of the result that this thread will write (of the first 256; tokens beyond are few)
+    float add[(kOuts + kWarps * 32 - 1) / (kWarps * 32)], off[(kOuts + kWarps * 32 - 1) / (kWarps * 32)];
 #pragma unroll
-  for (int i = 0; i < U; ++i)
+    for (int j = 0; j * kWarps * 32 < kOuts; ++j) {
+      const int i = j * kWarps * 32 + threadIdx.x, m = i / kTileRows, r = u * kTileRows + i % kTileRows;
+      const bool in = i < kOuts && m < p.tokens && r < p.rows;
+      off[j] = bias && in ? to_float(bias[r]) : 0.0f;
+      add[j] = residual && in ? to_float(residual[m * p.residual_row + r]) : 0.0f;
+    }
+    float acc[NT][4] = {};
+    for (int ph = 0; ph < phases; ++ph) {
+      if (phases > 1) {
+        __syncthreads();      // the stretch before has been read
+        stage(ph);
+        __syncthreads();
+      }
+      const Slice<C, GROUP> own = now;
+      const int next_u = ph + 1 < phases ? u : u + gridDim.x, next_ph = ph + 1 < phases ? ph + 1 : 0;
+      if (next_u < p.units) now.load(codes, scales, next_u, (next_ph * kWarps + warp) * C, p.chunks, p.groups, lane);
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        if ((ph * kWarps + warp) * C + i >= p.chunks) break;
+        const uint32_t word[4] = {own.w[i].x, own.w[i].y, own.w[i].z, own.w[i].w};
+        uint4 b[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) b[n][h] = *reinterpret_cast<const uint4*>(tokens + (n * 8 + g) * kStride + (warp * C + i) * 32 + h * 16 + t * 4);
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) {
+          float sum[NT][4] = {};
+#pragma unroll
+          for (int j = k * kSteps; j < (k + 1) * kSteps; ++j) {
+            const uint32_t a[4] = {codes_to_pair<T>(word[j], 0), codes_to_pair<T>(word[j], 1), codes_to_pair<T>(word[j], 2), codes_to_pair<T>(word[j], 3)};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const uint4 v = b[n][j / 2];
+              mma<T>(sum[n], a, j % 2 ? v.z : v.x, j % 2 ? v.w : v.y, sum[n]);
+            }
+          }
+          const uint32_t both = own.scale(i, k, lane);
+          const float low = bf16_bits(both), high = __uint_as_float(both & 0xFFFF0000u);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            acc[n][0] = fmaf(low, sum[n][0], acc[n][0]);
+            acc[n][1] = fmaf(low, sum[n][1], acc[n][1]);
+            acc[n][2] = fmaf(high, sum[n][2], acc[n][2]);
+            acc[n][3] = fmaf(high, sum[n][3], acc[n][3]);
+          }
+        }
+      }
+    }
+    // the warps' sums, in the order of the warps
+    float* mine = part + flip * kWarps * kOuts;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) part[(warp * kTokens + n * 8 + 2 * t + (e & 1)) * kRows + i * kTileRows + g + 8 * (e >> 1)] = acc[i][n][e];
-  __syncthreads();
-  for (int i = threadIdx.x; i < kRows * kTokens; i += WARPS * 32) {
-    const int m = m0 + i / kRows;
-    const int r = u0 * kTileRows + i % kRows;
-    if (m >= p.tokens || r >= p.rows) continue;
-    float v = part[i];
-    for (int k = 1; k < WARPS; ++k) v += part[k * kRows * kTokens + i];
-    if (bias) v += to_float(bias[r]);
-    v = activate(v, p.act);
-    if (residual) v += to_float(residual[m * p.residual_row + r]);
-    y[m * p.y_row + r] = from_float<T>(v);
+      for (int e = 0; e < 4; ++e) mine[warp * kOuts + (n * 8 + 2 * t + (e & 1)) * kTileRows + g + 8 * (e >> 1)] = acc[n][e];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j * kWarps * 32 < kOuts; ++j) {
+      const int i = j * kWarps * 32 + threadIdx.x, m = i / kTileRows, r = u * kTileRows + i % kTileRows;
+      if (i >= kOuts || m >= p.tokens || r >= p.rows) continue;
+      float v = mine[i];
+#pragma unroll
+      for (int k = 1; k < kWarps; ++k) v += mine[k * kOuts + i];
+      y[m * p.y_row + r] = from_float<T>(activate(v + off[j], p.act) + add[j]);
+    }
   }
 }
 
-template <typename T, int NT, int U, int GROUP, bool PAIRS>
+template <typename T, int NT, int C, int GROUP>
 int launch(const LinearParams& p, cudaStream_t stream) {
-  constexpr int kWarps = 8;
-  constexpr size_t smem = sizeof(float) * kWarps * NT * 8 * U * kTileRows;
-  static_assert(smem <= 48 * 1024, "sums need no opting in");
-  const dim3 grid((p.units + U - 1) / U, (p.tokens + NT * 8 - 1) / (NT * 8));
-  if (grid.y > 65535) return st::fail(ST_ERR_TOO_LARGE, "int4: too many rows");
-  const cudaError_t e = st::chained(linear_kernel<T, NT, U, GROUP, kWarps, PAIRS>, grid, dim3(kWarps * 32), smem, stream)(
+  constexpr int smem = NT * 8 * (kWarps * C * kTileCols / 2 + 16) * 4 + 2 * kWarps * NT * 8 * kTileRows * 4;
+  static int resident[st::kMaxDevices];
+  int& blocks = resident[st::current_device()];
+  if (blocks == 0) {
+    if (smem > 48 * 1024) ST_CUDA_CHECK(cudaFuncSetAttribute(linear_kernel<T, NT, C, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    int n = 0;
+    ST_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, linear_kernel<T, NT, C, GROUP>, kWarps * 32, smem));
+    blocks = max(1, n) * st::sm_count();
+  }
+  // as many blocks as run at once, each the same number of rows or one more
+  const int turns = (p.units + blocks - 1) / blocks, grid = (p.units + turns - 1) / turns;
+  const cudaError_t e = st::chained(linear_kernel<T, NT, C, GROUP>, dim3(grid), dim3(kWarps * 32), smem, stream)(
       static_cast<const T*>(p.x), p.codes, p.scales, static_cast<const T*>(p.bias), static_cast<const T*>(p.residual), static_cast<T*>(p.y), p);
   return e == cudaSuccess ? ST_OK : st::fail_cuda(e, "int4 linear");
 }
 
-template <typename T, int NT, int U>
+template <typename T, int NT, int C>
 int by_group(const LinearParams& p, cudaStream_t stream) {
-  const bool pairs = (reinterpret_cast<uintptr_t>(p.x) & 3) == 0 && p.x_row % 2 == 0 && p.cols % 2 == 0;
-  if (p.group == 32) return pairs ? launch<T, NT, U, 32, true>(p, stream) : launch<T, NT, U, 32, false>(p, stream);
-  if (p.group == 64) return pairs ? launch<T, NT, U, 64, true>(p, stream) : launch<T, NT, U, 64, false>(p, stream);
-  return pairs ? launch<T, NT, U, 128, true>(p, stream) : launch<T, NT, U, 128, false>(p, stream);
+  if (p.group == 32) return launch<T, NT, C, 32>(p, stream);
+  if (p.group == 64) return launch<T, NT, C, 64>(p, stream);
+  return launch<T, NT, C, 128>(p, stream);
 }
 
 template <typename T>
 int dispatch(const LinearParams& p, cudaStream_t stream) {
-  if (p.tokens <= 8) return by_group<T, 1, 1>(p, stream);
-  return by_group<T, 2, 1>(p, stream);
+  // 2 chunks a warp where that is the whole depth, 4 otherwise
+  if (p.tokens <= 8) return p.chunks <= 2 * kWarps ? by_group<T, 1, 2>(p, stream) : by_group<T, 1, 4>(p, stream);
+  return p.chunks <= 2 * kWarps ? by_group<T, 2, 2>(p, stream) : by_group<T, 2, 4>(p, stream);
 }
+
 constexpr int kWideFrom = 17;
 
 int aligned(const void* x, long long row, int cols) {
@@ -151,24 +225,37 @@ int aligned(const void* x, long long row, int cols) {
 }
 }  // namespace
 
+struct StInt4LinearArgs {
+  const void* x;
+  const void* codes;
+  const void* scales;
+  const void* bias;
+  const void* residual;
+  void* y;
+  long long x_row, residual_row, y_row;
+  int tokens, rows, cols, group, act, type;
+};
+
 // y [tokens, rows] = act(x [tokens, cols] W^T + bias) + residual.  Columns are contiguous, rows the given numbers of elements apart; bias and residual may be
-// null.  From st_int4_wide_from() tokens on x lies on a 16-byte boundary, its rows a multiple of 8 elements apart.  act: 0 none, 1 relu, 2 gelu (tanh form); type of x, bias, residual and y: 0 bf16, 1 fp16.
-ST_API int st_int4_linear(const void* x, const void* codes, const void* scales, const void* bias, const void* residual, void* y, int tokens, int rows, int cols,
-                          long long x_row, long long residual_row, long long y_row, int group, int act, int type, void* stream_v) {
-  if (tokens < 0 || rows < 1 || cols < 1 || rows > 1 << 30 || cols > 1 << 30 || (group != 32 && group != 64 && group != 128) || act < 0 || act > 2)
+// null.  From st_int4_wide_from() tokens on x lies on a 16-byte boundary, its rows a multiple of 8 elements apart.  act: 0 none, 1 relu, 2 gelu (tanh form); type of x, bias,
+// residual and y: 0 bf16, 1 fp16.
+ST_API int st_int4_linear(const StInt4LinearArgs* a, void* stream_v) {
+  if (a->tokens < 0 || a->rows < 1 || a->cols < 1 || a->rows > 1 << 30 || a->cols > 1 << 30 || (a->group != 32 && a->group != 64 && a->group != 128) || a->act < 0 || a->act > 2)
     return st::fail(ST_ERR_INVALID, "int4: sizes out of range");
-  if ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15) return st::fail(ST_ERR_INVALID, "int4: codes and scales must lie on 16-byte boundaries");
-  if (tokens == 0) return ST_OK;
-  const LinearParams p{x, static_cast<const uint8_t*>(codes), static_cast<const __nv_bfloat16*>(scales), bias, residual, y, x_row, residual_row, y_row,
-                       tokens, rows, cols, (cols + group - 1) / group, (cols + kTileCols - 1) / kTileCols, (rows + kTileRows - 1) / kTileRows, group, act};
+  if (a->type != 0 && a->type != 1) return st::fail(ST_ERR_INVALID, "int4: unknown type");
+  if ((reinterpret_cast<uintptr_t>(a->codes) | reinterpret_cast<uintptr_t>(a->scales)) & 15) return st::fail(ST_ERR_INVALID, "int4: codes and scales must lie on 16-byte boundaries");
+  if (a->tokens == 0) return ST_OK;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
-  if (type != 0 && type != 1) return st::fail(ST_ERR_INVALID, "int4: unknown type");
-  if (tokens >= kWideFrom) {
-    if (const int e = aligned(x, x_row, cols)) return e;
-    return wide(WideArgs{x, codes, scales, bias, residual, y, x_row, residual_row, y_row, tokens, rows, cols, group, act}, type, false, stream);
+  if (a->tokens >= kWideFrom) {
+    if (const int e = aligned(a->x, a->x_row, a->cols)) return e;
+    return wide(WideArgs{a->x, a->codes, a->scales, a->bias, a->residual, a->y, a->x_row, a->residual_row, a->y_row, a->tokens, a->rows, a->cols, a->group, a->act}, a->type,
+                false, stream);
   }
-  if (type == 0) return dispatch<__nv_bfloat16>(p, stream);
-  return dispatch<__half>(p, stream);
+  const LinearParams p{a->x, static_cast<const uint8_t*>(a->codes), static_cast<const __nv_bfloat16*>(a->scales), a->bias, a->residual, a->y, a->x_row, a->residual_row,
+                       a->y_row, a->tokens, a->rows, a->cols, (a->cols + a->group - 1) / a->group, (a->cols + kTileCols - 1) / kTileCols,
+                       (a->rows + kTileRows - 1) / kTileRows, a->group, a->act,
+                       (reinterpret_cast<uintptr_t>(a->x) & 15) == 0 && a->x_row % 8 == 0};
+  return a->type == 0 ? dispatch<__nv_bfloat16>(p, stream) : dispatch<__half>(p, stream);
 }
 
 // dx [tokens, cols] = dy [tokens, rows] W.  dy lies on a 16-byte boundary, its rows a multiple of 8 elements apart.

@@ -203,6 +203,18 @@ typedef struct StInfoNceArgs {
   unsigned arrive_target;                           // cumulative arrivals expected per source rank
 } StInfoNceArgs;
 
+/* csrc/serving/int4_linear.cu */
+typedef struct StInt4LinearArgs {
+  const void* x;
+  const void* codes;
+  const void* scales;
+  const void* bias;
+  const void* residual;
+  void* y;
+  long long x_row, residual_row, y_row;
+  int tokens, rows, cols, group, act, type;
+} StInt4LinearArgs;
+
 /* csrc/vision/vision.cu */
 typedef struct StPreprocessArgs {
   int B, C, src_h, src_w, resize_h, resize_w, out_h, out_w, crop_y, crop_x, flip, do_jitter;
@@ -276,7 +288,7 @@ int st_im2col3x3_small(const void* x, void* col, int N, int H, int W, int C, int
 int st_info_nce_fwd(const StInfoNceArgs* a, void* stream_v);   /* csrc/comm/contrastive.cu */
 int st_info_nce_grad(const float* logits, const float* row_lse, const float* coef, void* dl, void* dl_t, int R, int C, int target_offset, void* stream_v);   /* csrc/comm/contrastive.cu */
 int st_int4_dequantize(const void* codes, const void* scales, void* w, int rows, int cols, long long stride, int group, int type, void* stream_v);   /* csrc/serving/int4_weights.cu */
-int st_int4_linear(const void* x, const void* codes, const void* scales, const void* bias, const void* residual, void* y, int tokens, int rows, int cols, long long x_row, long long residual_row, long long y_row, int group, int act, int type, void* stream_v);   /* csrc/serving/int4_linear.cu */
+int st_int4_linear(const StInt4LinearArgs* a, void* stream_v);   /* csrc/serving/int4_linear.cu */
 int st_int4_linear_grad(const void* dy, const void* codes, const void* scales, void* dx, int tokens, int rows, int cols, long long dy_row, long long dx_row, int group, int type, void* stream_v);   /* csrc/serving/int4_linear.cu */
 int st_int4_quantize(const void* w, void* codes, void* scales, int rows, int cols, long long stride, int group, int type, void* stream_v);   /* csrc/serving/int4_weights.cu */
 int st_int4_wide_from();   /* csrc/serving/int4_linear.cu */

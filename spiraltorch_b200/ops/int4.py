@@ -15,7 +15,8 @@ CPU tensors use a plain PyTorch statement of the same (also the test oracle).  T
 from __future__ import annotations
 
 import functools
-from typing import NamedTuple, Optional
+import struct
+from typing import Optional
 
 import torch
 
@@ -29,22 +30,36 @@ _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _ACTS = {None: 0, "relu": 1, "gelu": 2}
 
 
-class Weights(NamedTuple):
+# StInt4LinearArgs of csrc/serving/int4_linear.cu, in one call: a ctypes object for each of 16 arguments costs as much as the launch
+_pack_args = struct.Struct("@6P3q6i").pack
+
+
+class Weights:
     """``codes`` uint8 ``[tiles down, tiles across, 512]`` (16 rows by 64 columns each, in the order of the kernels), ``scales`` bf16 ``[tiles down, groups, 16]``;
     the matrix's ``out_features`` and ``in_features``, and the inputs to a scale."""
-    codes: torch.Tensor
-    scales: torch.Tensor
-    out_features: int
-    in_features: int
-    group: int
+    __slots__ = ("codes", "scales", "out_features", "in_features", "group")
 
-    @classmethod
-    def allocate(cls, out_features: int, in_features: int, group: int = 64, device="cuda") -> "Weights":
-        """Room for :func:`quantize` to write to."""
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, out_features: int, in_features: int, group: int):
         if group not in GROUPS:
             raise ValueError(f"int4: groups of {GROUPS} inputs, got {group}")
         if not (0 < out_features <= 1 << 30 and 0 < in_features <= 1 << 30):
             raise ValueError(f"int4: a matrix of {out_features} x {in_features} is not supported")
+        down = -(-out_features // 16)
+        if codes.dtype is not torch.uint8 or scales.dtype is not torch.bfloat16 or not codes.is_contiguous() or not scales.is_contiguous() \
+                or codes.shape != (down, -(-in_features // 64), 512) or scales.shape != (down, -(-in_features // group), 16) or codes.device != scales.device:
+            raise ValueError(f"int4: codes {codes.dtype} {tuple(codes.shape)} and scales {scales.dtype} {tuple(scales.shape)} are no weights of "
+                             f"{out_features} x {in_features} in groups of {group}")
+        for name, value in zip(self.__slots__, (codes, scales, out_features, in_features, group)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError("int4.Weights: sizes and memory stay as they were checked")
+
+    @classmethod
+    def allocate(cls, out_features: int, in_features: int, group: int = 64, device="cuda") -> "Weights":
+        """Room for :func:`quantize` to write to."""
+        if group not in GROUPS or not (0 < out_features <= 1 << 30 and 0 < in_features <= 1 << 30):
+            raise ValueError(f"int4: a matrix of {out_features} x {in_features} in groups of {group} is not supported")
         down = -(-out_features // 16)
         return cls(torch.empty((down, -(-in_features // 64), 512), dtype=torch.uint8, device=device),
                    torch.empty((down, -(-in_features // group), 16), dtype=torch.bfloat16, device=device), out_features, in_features, group)
@@ -54,14 +69,7 @@ class Weights(NamedTuple):
         return self.codes.nbytes + self.scales.nbytes
 
     def to(self, device) -> "Weights":
-        return self._replace(codes=self.codes.to(device), scales=self.scales.to(device))
-
-
-def _check(w: Weights, what: str) -> None:
-    codes, scales, n, k, group = w
-    if group not in GROUPS or codes.dtype is not torch.uint8 or scales.dtype is not torch.bfloat16 or not codes.is_contiguous() or not scales.is_contiguous() \
-            or codes.shape != (-(-n // 16), -(-k // 64), 512) or scales.shape != (-(-n // 16), -(-k // group), 16):
-        raise ValueError(f"{what}: codes {codes.dtype} {tuple(codes.shape)} and scales {scales.dtype} {tuple(scales.shape)} are no weights of {n} x {k} in groups of {group}")
+        return Weights(self.codes.to(device), self.scales.to(device), self.out_features, self.in_features, self.group)
 
 
 # ---- plain statement ------------------------------------------------------------------------------------------------------------
@@ -131,8 +139,7 @@ def quantize(weight: torch.Tensor, group: int = 64, *, out: Optional[Weights] = 
     if out is None:
         out = Weights.allocate(n, k, group, weight.device)
     else:
-        _check(out, "int4.quantize")
-        if out[2:] != (n, k, group):
+        if (out.out_features, out.in_features, out.group) != (n, k, group):
             raise ValueError(f"int4.quantize: a {n} x {k} matrix in groups of {group} into weights of {out.out_features} x {out.in_features} in groups of {out.group}")
         native.same_device("int4.quantize", weight, out.codes, out.scales)
     weight = weight.detach()
@@ -156,7 +163,6 @@ def quantize(weight: torch.Tensor, group: int = 64, *, out: Optional[Weights] = 
 def dequantize(w: Weights, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``[out, in]`` in bf16, fp16 or fp32: the same numbers in each."""
     global launch_count
-    _check(w, "int4.dequantize")
     if not native.use_native(w.codes):
         return dequantize_reference(w, dtype)
     if dtype not in _TYPES:
@@ -189,26 +195,31 @@ def _boundaries(x2: torch.Tensor) -> torch.Tensor:
 def _product(x2, w, bias, act, residual2):
     """``[rows, in]`` to ``[rows, out]``."""
     global launch_count
-    if not native.use_native(x2):
+    if not x2.is_cuda:
         return linear_reference(x2, dequantize_reference(w, x2.dtype if x2.dtype == torch.float64 else torch.float32), bias, act, residual2)
-    if x2.stride(1) != 1 and x2.shape[1] > 1:
-        x2 = x2.contiguous()
-    if residual2 is not None and residual2.stride(1) != 1 and residual2.shape[1] > 1:
-        residual2 = residual2.contiguous()
-    if bias is not None and bias.stride(0) != 1 and bias.shape[0] > 1:
-        bias = bias.contiguous()
     index = native.require_cuda("int4.linear", x2, w.codes, w.scales, bias, residual2)
-    rows = x2.shape[0]
-    if rows >= _wide_from():
-        x2 = _boundaries(x2)
-    y = x2.new_empty((rows, w.out_features))
+    (rows, cols), n = x2.shape, w.out_features
+    y = x2.new_empty((rows, n))
     if rows == 0:
         return y
+    if rows >= _wide_from():
+        x2 = _boundaries(x2)
+    x_row, step = x2.stride()
+    if step != 1 and cols > 1:
+        x2, x_row = x2.contiguous(), cols
+    residual_row = 0
+    if residual2 is not None:
+        residual_row, step = residual2.stride()
+        if step != 1 and n > 1:
+            residual2, residual_row = residual2.contiguous(), n
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    args = _pack_args(x2.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if residual2 is None else residual2.data_ptr(),
+                      y.data_ptr(), x_row, residual_row, n, rows, n, cols, w.group, _ACTS[act], _TYPES[x2.dtype])
     with native.on_device(index):
-        st = native.entry("st_int4_linear", "ppppppiiiqqqiiip")(
-            x2.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), native.address(bias), native.address(residual2), y.data_ptr(), rows, w.out_features,
-            w.in_features, x2.stride(0), 0 if residual2 is None else residual2.stride(0), w.out_features, w.group, _ACTS[act], _TYPES[x2.dtype], native.raw_stream(index))
-    native.check(st, "st_int4_linear")
+        st = native.entry("st_int4_linear", "sp")(args, native.raw_stream(index))
+    if st:
+        native.check(st, "st_int4_linear")
     launch_count += 1
     return y
 
@@ -256,23 +267,27 @@ def linear(x: torch.Tensor, w: Weights, bias: Optional[torch.Tensor] = None, *, 
     or ``"gelu"`` (tanh form).  Sums are in fp32; the result, in ``x``'s type, is rounded once.
 
     Differentiable in ``x``, ``bias`` and ``residual`` (the weights are constants) without ``act``: apply an activation to the result where gradients are needed."""
-    _check(w, "int4.linear")
     if act not in _ACTS:
         raise ValueError(f"int4.linear: act must be None, 'relu' or 'gelu', got {act!r}")
-    if x.dtype not in (torch.bfloat16, torch.float16) and (x.is_cuda or x.dtype not in (torch.float32, torch.float64)):
-        raise ValueError(f"int4.linear: bf16 and fp16 tensors, got {x.dtype}")
-    shape = (*x.shape[:-1], w.out_features)
-    if x.dim() == 0 or x.shape[-1] != w.in_features:
-        raise ValueError(f"int4.linear: x {tuple(x.shape)} does not end in the weights' {w.in_features} inputs")
-    for name, t, want in (("bias", bias, (w.out_features,)), ("residual", residual, shape)):
-        if t is not None and (t.shape != want or t.dtype != x.dtype):
-            raise ValueError(f"int4.linear: {name} must be {x.dtype} {tuple(want)}, got {t.dtype} {tuple(t.shape)}")
-    native.same_device("int4.linear", x, w.codes, w.scales, bias, residual)
+    dtype, shape = x.dtype, x.shape
+    if dtype is not torch.bfloat16 and dtype is not torch.float16 and (x.is_cuda or dtype not in (torch.float32, torch.float64)):
+        raise ValueError(f"int4.linear: bf16 and fp16 tensors, got {dtype}")
+    n = w.out_features
+    if len(shape) == 0 or shape[-1] != w.in_features:
+        raise ValueError(f"int4.linear: x {tuple(shape)} does not end in the weights' {w.in_features} inputs")
+    if bias is not None and (bias.shape != (n,) or bias.dtype is not dtype):
+        raise ValueError(f"int4.linear: bias must be {dtype} {(n,)}, got {bias.dtype} {tuple(bias.shape)}")
+    if residual is not None and (residual.shape != (*shape[:-1], n) or residual.dtype is not dtype):
+        raise ValueError(f"int4.linear: residual must be {dtype} {(*shape[:-1], n)}, got {residual.dtype} {tuple(residual.shape)}")
+    if not x.is_cuda:
+        native.same_device("int4.linear", x, w.codes, bias, residual)
     if native.has_tangent(x, bias, residual):
         raise ValueError("int4.linear: forward-mode differentiation is not supported")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, bias, residual)):
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad) or (residual is not None and residual.requires_grad)):
         if act is not None:
             raise ValueError("int4.linear: act with tensors that require gradients; apply it to the result")
         return _LinearFn.apply(x, bias, residual, w)
-    y = _product(x.reshape(-1, w.in_features), w, bias, act, None if residual is None else residual.reshape(-1, w.out_features))
-    return y.view(shape)
+    if len(shape) == 2:
+        return _product(x, w, bias, act, residual)
+    y = _product(x.reshape(-1, w.in_features), w, bias, act, None if residual is None else residual.reshape(-1, n))
+    return y.view(*shape[:-1], n)

@@ -171,12 +171,12 @@ def require_cuda(op: str, *tensors: Optional[torch.Tensor]) -> int:
     return index
 
 
-_CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "q": ctypes.c_longlong, "f": ctypes.c_float}
+_CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "q": ctypes.c_longlong, "f": ctypes.c_float, "s": ctypes.c_char_p}
 
 
 @functools.cache
 def entry(name: str, types: str):
-    """The launcher ``name`` with its argument types (p address, i int, q long long, f float) set: it then takes plain numbers.
+    """The launcher ``name`` with its argument types (p address, i int, q long long, f float, s bytes of a packed structure) set: it then takes plain numbers.
     A ctypes object built for each of a dozen arguments costs as much as the launch itself."""
     fn = getattr(lib(), name)
     fn.argtypes = [_CTYPES[t] for t in types]

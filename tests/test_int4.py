@@ -133,7 +133,7 @@ def test_refusals():
                  lambda: int4.quantize(w[:, :64], 32, out=held), lambda: int4.Weights.allocate(0, 4), lambda: int4.Weights.allocate(4, 4, 16),
                  lambda: int4.linear(x[:, :69], held), lambda: int4.linear(x, held, torch.zeros(21)), lambda: int4.linear(x, held, torch.zeros(20).half()),
                  lambda: int4.linear(x, held, residual=torch.zeros(2, 20)), lambda: int4.linear(x, held, act="tanh"), lambda: int4.linear(x.int(), held),
-                 lambda: int4.linear(x, held._replace(in_features=140)), lambda: int4.dequantize(held._replace(group=64)),
+                 lambda: int4.Weights(held.codes, held.scales, 20, 140, 32), lambda: int4.Weights(held.codes, held.scales, 20, 70, 64),
                  lambda: int4.linear(x.clone().requires_grad_(), held, act="gelu"), lambda: int4.linear(torch.tensor(1.0), held)):
         with pytest.raises(ValueError):
             call()
