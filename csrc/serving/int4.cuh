@@ -35,16 +35,23 @@ __device__ __forceinline__ float activate(float v, int act) {      // 0 none, 1 
   return act == 1 ? fmaxf(v, 0.0f) + (v != v ? v : 0.0f) : act == 2 ? st::gelu_tanh(v) : v;
 }
 
+// (word & mask) | bits in one instruction
+__device__ __forceinline__ uint32_t pick(uint32_t word, uint32_t mask, uint32_t bits) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(word), "r"(mask), "r"(bits));
+  return d;
+}
+
 // Nibbles e and e + 4 of a word as two numbers -8..7, exactly: the nibble is put into the low bits of 128 (bf16) or 1024 (fp16), where a unit is 1, and
 // 136 or 1032 is subtracted.
 template <typename T> __device__ __forceinline__ uint32_t codes_to_pair(uint32_t word, int e);
 template <> __device__ __forceinline__ uint32_t codes_to_pair<__nv_bfloat16>(uint32_t word, int e) {
-  const uint32_t v = ((word >> (4 * e)) & 0x000F000Fu) | 0x43004300u;
+  const uint32_t v = pick(word >> (4 * e), 0x000F000Fu, 0x43004300u);
   const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __nv_bfloat162(__float2bfloat16_rn(136.0f), __float2bfloat16_rn(136.0f)));
   return *reinterpret_cast<const uint32_t*>(&d);
 }
 template <> __device__ __forceinline__ uint32_t codes_to_pair<__half>(uint32_t word, int e) {
-  const uint32_t v = ((word >> (4 * e)) & 0x000F000Fu) | 0x64006400u;
+  const uint32_t v = pick(word >> (4 * e), 0x000F000Fu, 0x64006400u);
   const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v), __half2(__float2half_rn(1032.0f), __float2half_rn(1032.0f)));
   return *reinterpret_cast<const uint32_t*>(&d);
 }

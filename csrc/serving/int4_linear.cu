@@ -37,28 +37,39 @@ template <> __device__ __forceinline__ void mma<__half>(float (&d)[4], const uin
 // columns 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of each.  Tokens are 64 bytes more than a whole number of 128 apart, so that 8 lanes read from all banks.
 constexpr int kWarps = 8;
 
-template <typename T, bool WIDE>
-__device__ __forceinline__ void stage_tokens(const T* x, long long x_row, uint32_t* to, int stride, int tokens, int room, int k0, int columns, int cols) {
-  // vectors of 8 columns: step s, half h of it; word t of them goes to 16 (s / 2) + 4 t + 2 (s % 2) + h
-  const int vectors = columns / 8;
-  for (int i = threadIdx.x; i < room * vectors; i += kWarps * 32) {
-    const int m = i / vectors, j = i - m * vectors, k = k0 + j * 8;
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (m < tokens) {
+// A thread takes 8 columns (step s, half h; word t of them goes to 16 (s / 2) + 4 t + 2 (s % 2) + h) of every second or of all tokens, four at a time.  What stands in the
+// place of tokens that there are none of does not matter: they are columns of their own.
+template <typename T, int COLUMNS>
+__device__ __forceinline__ void stage_tokens(const T* x, long long x_row, uint32_t* to, int stride, int tokens, int k0, int cols, bool wide) {
+  constexpr int kVectors = COLUMNS / 8, kRows = kWarps * 32 / kVectors, kAhead = 4;
+  const int j = threadIdx.x % kVectors, k = k0 + j * 8;
+  if (k >= (cols + 63) / 64 * 64) return;
+  uint32_t* at = to + (j >> 3) * 32 + ((j >> 2) & 1) * 16 + ((j >> 1) & 1) * 2 + (j & 1);
+  for (int m0 = threadIdx.x / kVectors; m0 < tokens; m0 += kAhead * kRows) {
+    uint4 v[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int m = m0 + i * kRows;
       const T* from = x + m * x_row + k;
-      if (WIDE && k + 8 <= cols) {
-        const uint4 v = *reinterpret_cast<const uint4*>(from);
-        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+      v[i] = make_uint4(0, 0, 0, 0);
+      if (m >= tokens) continue;
+      if (wide && k + 8 <= cols) {
+        v[i] = *reinterpret_cast<const uint4*>(from);
       } else {
         const uint16_t* h = reinterpret_cast<const uint16_t*>(from);
+        uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (k + e < cols) w[e / 2] |= static_cast<uint32_t>(h[e]) << (16 * (e % 2));
+        v[i] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    uint32_t* at = to + m * stride + (j >> 3) * 32 + ((j >> 2) & 1) * 16 + ((j >> 1) & 1) * 2 + (j & 1);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) at[4 * t] = w[t];
+    for (int i = 0; i < kAhead; ++i) {
+      const int m = m0 + i * kRows;
+      if (m >= tokens) continue;
+      at[m * stride] = v[i].x, at[m * stride + 4] = v[i].y, at[m * stride + 8] = v[i].z, at[m * stride + 12] = v[i].w;
+    }
   }
 }
 
@@ -68,15 +79,24 @@ struct Slice {
   static constexpr int kScales = C * 64 / GROUP > 0 ? C * 64 / GROUP : 1, kWords = (kScales * 8 + 31) / 32;
   uint4 w[C];
   uint32_t s[kWords];
-  __device__ __forceinline__ void load(const uint8_t* codes, const __nv_bfloat16* scales, long long u, int c0, int chunks, int groups, int lane) {
-#pragma unroll
-    for (int i = 0; i < C; ++i)
-      w[i] = c0 + i < chunks ? *reinterpret_cast<const uint4*>(codes + (u * chunks + c0 + i) * kTileBytes + lane * 16) : make_uint4(0, 0, 0, 0);
+  // codes and scales: of the tile row
+  __device__ __forceinline__ void load(const uint8_t* codes, const __nv_bfloat16* scales, int c0, int chunks, int groups, int lane) {
+    const uint8_t* from = codes + static_cast<long long>(c0) * kTileBytes + lane * 16;
     const int g0 = c0 * 64 / GROUP;
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(scales) + g0 * 8 + lane;
+    if (c0 + C <= chunks) {
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) {
-      const int at = i * 32 + lane;
-      s[i] = at < kScales * 8 && g0 + at / 8 < groups ? *reinterpret_cast<const uint32_t*>(scales + (u * groups + g0) * 16 + at * 2) : 0u;
+      for (int i = 0; i < C; ++i) w[i] = *reinterpret_cast<const uint4*>(from + i * kTileBytes);
+#pragma unroll
+      for (int i = 0; i < kWords; ++i)
+        if (kScales * 8 % 32 == 0 || i * 32 + lane < kScales * 8) s[i] = words[i * 32];
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i)
+        if (c0 + i < chunks) w[i] = *reinterpret_cast<const uint4*>(from + i * kTileBytes);
+#pragma unroll
+      for (int i = 0; i < kWords; ++i)
+        if (i * 32 + lane < (groups - g0) * 8 && i * 32 + lane < kScales * 8) s[i] = words[i * 32];
     }
   }
   // of chunk i, half k of it where groups are halves
@@ -101,86 +121,111 @@ __global__ void __launch_bounds__(kWarps * 32) linear_kernel(const T* x, const u
   float* part = reinterpret_cast<float*>(room + kTokens * kStride);      // two of [warp][token][row]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int phases = (p.cols + kColumns - 1) / kColumns;
-  Slice<C, GROUP> now;
-  int u = blockIdx.x;
-  now.load(codes, scales, u, warp * C, p.chunks, p.groups, lane);
-  const auto stage = [&](int ph) {
-    const int columns = min(kColumns, (p.cols - ph * kColumns + 63) / 64 * 64);
-    if (p.wide) stage_tokens<T, true>(x, p.x_row, tokens, kStride, p.tokens, kTokens, ph * kColumns, columns, p.cols);
-    else stage_tokens<T, false>(x, p.x_row, tokens, kStride, p.tokens, kTokens, ph * kColumns, columns, p.cols);
-  };
-  if (phases == 1) {
-    stage(0);
-    __syncthreads();
-  }
-  for (int flip = 0; u < p.units; u += gridDim.x, flip ^= 1) {
-    // the element of the result that this thread will write (of the first 256; tokens beyond are few)
-    float add[(kOuts + kWarps * 32 - 1) / (kWarps * 32)], off[(kOuts + kWarps * 32 - 1) / (kWarps * 32)];
+  const auto stage = [&](int ph) { stage_tokens<T, kColumns>(x, p.x_row, tokens, kStride, p.tokens, ph * kColumns, p.cols, p.wide); };
+  const long long tile_row = static_cast<long long>(p.chunks) * kTileBytes, scale_row = static_cast<long long>(p.groups) * 16;
+  constexpr int kOwn = (kOuts + kWarps * 32 - 1) / (kWarps * 32);      // elements of the result that a thread writes
+  float acc[NT][4] = {}, off[kOwn], add[kOwn];
+  const auto fetch = [&](Slice<C, GROUP>& to, int u, int ph) { to.load(codes + u * tile_row, scales + u * scale_row, (ph * kWarps + warp) * C, p.chunks, p.groups, lane); };
+  const auto multiply = [&](const Slice<C, GROUP>& own, int ph) {
+    const int count = min(C, p.chunks - (ph * kWarps + warp) * C);
 #pragma unroll
-    for (int j = 0; j * kWarps * 32 < kOuts; ++j) {
+    for (int i = 0; i < C; ++i) {
+      if (i >= count) break;
+      const uint32_t word[4] = {own.w[i].x, own.w[i].y, own.w[i].z, own.w[i].w};
+      uint4 b[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) b[n][h] = *reinterpret_cast<const uint4*>(tokens + (n * 8 + g) * kStride + (warp * C + i) * 32 + h * 16 + t * 4);
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) {
+        float sum[NT][4] = {};
+#pragma unroll
+        for (int j = k * kSteps; j < (k + 1) * kSteps; ++j) {
+          const uint32_t a[4] = {codes_to_pair<T>(word[j], 0), codes_to_pair<T>(word[j], 1), codes_to_pair<T>(word[j], 2), codes_to_pair<T>(word[j], 3)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint4 v = b[n][j / 2];
+            mma<T>(sum[n], a, j % 2 ? v.z : v.x, j % 2 ? v.w : v.y, sum[n]);
+          }
+        }
+        const uint32_t both = own.scale(i, k, lane);
+        const float low = bf16_bits(both), high = __uint_as_float(both & 0xFFFF0000u);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          acc[n][0] = fmaf(low, sum[n][0], acc[n][0]);
+          acc[n][1] = fmaf(low, sum[n][1], acc[n][1]);
+          acc[n][2] = fmaf(high, sum[n][2], acc[n][2]);
+          acc[n][3] = fmaf(high, sum[n][3], acc[n][3]);
+        }
+      }
+    }
+  };
+  const auto addends = [&](int u) {      // on their way beside the codes
+    if (bias == nullptr && residual == nullptr) return;
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
       const int i = j * kWarps * 32 + threadIdx.x, m = i / kTileRows, r = u * kTileRows + i % kTileRows;
       const bool in = i < kOuts && m < p.tokens && r < p.rows;
       off[j] = bias && in ? to_float(bias[r]) : 0.0f;
       add[j] = residual && in ? to_float(residual[m * p.residual_row + r]) : 0.0f;
     }
-    float acc[NT][4] = {};
-    for (int ph = 0; ph < phases; ++ph) {
-      if (phases > 1) {
-        __syncthreads();      // the stretch before has been read
-        stage(ph);
-        __syncthreads();
-      }
-      const Slice<C, GROUP> own = now;
-      const int next_u = ph + 1 < phases ? u : u + gridDim.x, next_ph = ph + 1 < phases ? ph + 1 : 0;
-      if (next_u < p.units) now.load(codes, scales, next_u, (next_ph * kWarps + warp) * C, p.chunks, p.groups, lane);
-#pragma unroll
-      for (int i = 0; i < C; ++i) {
-        if ((ph * kWarps + warp) * C + i >= p.chunks) break;
-        const uint32_t word[4] = {own.w[i].x, own.w[i].y, own.w[i].z, own.w[i].w};
-        uint4 b[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) b[n][h] = *reinterpret_cast<const uint4*>(tokens + (n * 8 + g) * kStride + (warp * C + i) * 32 + h * 16 + t * 4);
-#pragma unroll
-        for (int k = 0; k < kGroups; ++k) {
-          float sum[NT][4] = {};
-#pragma unroll
-          for (int j = k * kSteps; j < (k + 1) * kSteps; ++j) {
-            const uint32_t a[4] = {codes_to_pair<T>(word[j], 0), codes_to_pair<T>(word[j], 1), codes_to_pair<T>(word[j], 2), codes_to_pair<T>(word[j], 3)};
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const uint4 v = b[n][j / 2];
-              mma<T>(sum[n], a, j % 2 ? v.z : v.x, j % 2 ? v.w : v.y, sum[n]);
-            }
-          }
-          const uint32_t both = own.scale(i, k, lane);
-          const float low = bf16_bits(both), high = __uint_as_float(both & 0xFFFF0000u);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            acc[n][0] = fmaf(low, sum[n][0], acc[n][0]);
-            acc[n][1] = fmaf(low, sum[n][1], acc[n][1]);
-            acc[n][2] = fmaf(high, sum[n][2], acc[n][2]);
-            acc[n][3] = fmaf(high, sum[n][3], acc[n][3]);
-          }
-        }
-      }
-    }
-    // the warps' sums, in the order of the warps
-    float* mine = part + flip * kWarps * kOuts;
+  };
+  const auto finish = [&](int u, float* mine) {      // the warps' sums, in the order of the warps
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mine[warp * kOuts + (n * 8 + 2 * t + (e & 1)) * kTileRows + g + 8 * (e >> 1)] = acc[n][e];
+      for (int e = 0; e < 4; ++e) {
+        mine[warp * kOuts + (n * 8 + 2 * t + (e & 1)) * kTileRows + g + 8 * (e >> 1)] = acc[n][e];
+        acc[n][e] = 0.0f;
+      }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j * kWarps * 32 < kOuts; ++j) {
+    for (int j = 0; j < kOwn; ++j) {
       const int i = j * kWarps * 32 + threadIdx.x, m = i / kTileRows, r = u * kTileRows + i % kTileRows;
       if (i >= kOuts || m >= p.tokens || r >= p.rows) continue;
       float v = mine[i];
 #pragma unroll
       for (int k = 1; k < kWarps; ++k) v += mine[k * kOuts + i];
       y[m * p.y_row + r] = from_float<T>(activate(v + off[j], p.act) + add[j]);
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < kOwn; ++j) off[j] = add[j] = 0.0f;
+  float* other = part + kWarps * kOuts;
+  Slice<C, GROUP> a, b;
+  int u = blockIdx.x;
+  const int step = gridDim.x;
+  fetch(a, u, 0);
+  if (phases == 1) {
+    addends(u);
+    stage(0);
+    __syncthreads();
+    for (;;) {      // two rows at a time: what is on its way needs no copy
+      if (u + step < p.units) fetch(b, u + step, 0);
+      multiply(a, 0);
+      finish(u, part);
+      if ((u += step) >= p.units) break;
+      addends(u);
+      if (u + step < p.units) fetch(a, u + step, 0);
+      multiply(b, 0);
+      finish(u, other);
+      if ((u += step) >= p.units) break;
+      addends(u);
+    }
+  } else {
+    for (; u < p.units; u += step) {
+      addends(u);
+      for (int ph = 0; ph < phases; ++ph) {
+        __syncthreads();      // the stretch before has been read
+        stage(ph);
+        __syncthreads();
+        b = a;
+        const bool more = ph + 1 < phases;
+        if (more || u + step < p.units) fetch(a, more ? u : u + step, more ? ph + 1 : 0);
+        multiply(b, ph);
+      }
+      finish(u, part);
     }
   }
 }
@@ -196,8 +241,7 @@ int launch(const LinearParams& p, cudaStream_t stream) {
     ST_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, linear_kernel<T, NT, C, GROUP>, kWarps * 32, smem));
     blocks = max(1, n) * st::sm_count();
   }
-  // as many blocks as run at once, each the same number of rows or one more
-  const int turns = (p.units + blocks - 1) / blocks, grid = (p.units + turns - 1) / turns;
+  const int grid = min(p.units, blocks);      // as many as run at once
   const cudaError_t e = st::chained(linear_kernel<T, NT, C, GROUP>, dim3(grid), dim3(kWarps * 32), smem, stream)(
       static_cast<const T*>(p.x), p.codes, p.scales, static_cast<const T*>(p.bias), static_cast<const T*>(p.residual), static_cast<T*>(p.y), p);
   return e == cudaSuccess ? ST_OK : st::fail_cuda(e, "int4 linear");

@@ -73,7 +73,7 @@ template <> struct Scale<__nv_bfloat16> {
     less = __hmul2(s, __float2bfloat162_rn(-72.0f));
   }
   __device__ __forceinline__ uint32_t pair(uint32_t word, int e) const {
-    const uint32_t v = ((e == 0 ? word << 1 : word >> (4 * e - 1)) & 0x001E001Eu) | 0x42804280u;
+    const uint32_t v = pick(e == 0 ? word << 1 : word >> (4 * e - 1), 0x001E001Eu, 0x42804280u);
     const __nv_bfloat162 d = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&v), s, less);
     return *reinterpret_cast<const uint32_t*>(&d);
   }
