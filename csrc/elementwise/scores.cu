@@ -1,24 +1,34 @@
 // Scores of given tokens: log probability, entropy of the distribution and the likeliest tokens, from logits in one pass, and the gradient.
 //
-//   m = max x,  S = sum e^(x - m),  T = sum e^(x - m) (x - m),  log p_j = x_j - m - log S,  entropy = log S - T / S
+//   m = max x,  y = (x - m) log2 e,  S = sum 2^y,  T = sum 2^y y,  log p_j = (y_j - log2 S) ln 2,  entropy = (log2 S - T / S) ln 2
 //   dx_j = sum_i g_i [j = id_i] - p_j (sum_i g_i + g_entropy (log p_j + entropy)),  i over the given token and the likeliest ones
 //
-// Bound by memory: a row is read once (forward; the gradient reads it again and writes as much).  Every thread keeps m, S and T of what it has seen and
-// joins them at the end.  The likeliest tokens come from the same pass: the largest elements of the threads' first vectors give a bound that `top` elements
-// reach, and only what reaches it (a hundredth of a row) is set aside in shared memory.
+// Bound by memory: a row is read once (forward; the gradient reads it again and writes as much).  Every thread keeps m, S and T of what it has seen, and where
+// its largest element stands; they are joined at the end.  Of the threads' largest elements the `top` best give a bound, which only elements of these threads can
+// reach: those are read again (25 vectors each of a row of 50304, out of L2) and what reaches the bound is ranked.
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "../common/chain.cuh"
 #include <cuda_fp16.h>
+#include <type_traits>
 
 namespace {
 using st::chain_begin;
 
 constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kMostTop = 32;
-constexpr float kLog2e = 1.4426950408889634f, kLowest = -3.402823466e38f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f, kLowest = -3.402823466e38f;
 constexpr float kMargin = 4.0f;       // how far an element may lie above a thread's m before that follows it: e^4 rows of S are far from overflow
-constexpr float kFar = -1.0e4f;       // of e^d d where d is -inf: the product is 0, not 0 times infinity
+// y is one multiplication and addition, x log2 e - (m log2 e), the second rounded once for all of a row; that rounding must stay below 1, so |m| below kUsual = 2^20.
+// Elements below the least usual one, -inf among them, count as that, which keeps 2^y y from being 0 times infinity.  Rows whose m is not usual are summed
+// again with care: y = (x - m) log2 e.
+constexpr float kUsual = 1048576.0f;
+constexpr float kFar = -1.0e4f;       // 2^kFar is 0
+template <typename T> constexpr float kLeast = -kUsual;
+template <> constexpr float kLeast<__half> = -65504.0f;
+template <typename T> __device__ __forceinline__ bool is_usual(float m) { return m > 0.9f * kLeast<T> && m < kUsual; }      // and what counts as the least is nothing beside it
+__device__ __forceinline__ float scaled(float m) { return __fmul_rn(m, kLog2e); }
+__device__ __forceinline__ float exponent(float x, float m, bool usual) { return usual ? fmaf(x, kLog2e, -scaled(m)) : (x - m) * kLog2e; }
 
 struct ScoreParams {
   long long row, rows;      // elements between rows
@@ -34,31 +44,94 @@ template <> __device__ __forceinline__ float from_float(float x) { return x; }
 template <> __device__ __forceinline__ __half from_float(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float(float x) { return __float2bfloat16_rn(x); }
 
+template <typename T> __device__ __forceinline__ float at_least(float x) { return x < kLeast<T> ? kLeast<T> : x; }      // NaN stays
+
 // 16 bytes of a row.
 template <typename T>
 struct alignas(16) Vec {
   static constexpr int N = 16 / sizeof(T);
   T v[N];
+  __device__ __forceinline__ void pairs(float2 (&f)[N / 2]) const {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) f[i] = make_float2(to_float(v[2 * i]), to_float(v[2 * i + 1]));
+  }
 };
+template <int N>
+__device__ __forceinline__ float largest_of(const float2 (&f)[N]) {
+  if constexpr (N == 4) return fmaxf(st::max3(f[0].x, f[0].y, f[1].x), fmaxf(st::max3(f[1].y, f[2].x, f[2].y), fmaxf(f[3].x, f[3].y)));
+  return fmaxf(fmaxf(f[0].x, f[0].y), fmaxf(f[1].x, f[1].y));
+}
+
+// The elements of a vector as pairs, none below the least usual one.
+template <typename T>
+__device__ __forceinline__ void usual_pairs(const Vec<T>& v, float2 (&f)[Vec<T>::N / 2]) {
+  if constexpr (sizeof(T) == 4) {
+    v.pairs(f);
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N / 2; ++i) f[i] = make_float2(at_least<T>(f[i].x), at_least<T>(f[i].y));
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {      // two at a time before they are fp32
+    const __nv_bfloat162 least = __float2bfloat162_rn(kLeast<T>);
+    const uint4 bits = *reinterpret_cast<const uint4*>(&v);
+    const uint32_t word[4] = {bits.x, bits.y, bits.z, bits.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 c = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&word[i]), least);
+      const uint32_t u = *reinterpret_cast<const uint32_t*>(&c);
+      f[i] = make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+    }
+  } else {
+    const __half2 least = __float2half2_rn(kLeast<T>);
+    const uint4 bits = *reinterpret_cast<const uint4*>(&v);
+    const uint32_t word[4] = {bits.x, bits.y, bits.z, bits.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __half22float2(__hmax2_nan(*reinterpret_cast<const __half2*>(&word[i]), least));
+  }
+}
+
+// Vectors v, v + step, ... below end, four of them on their way while others are worked on.
+template <typename T, typename F>
+__device__ __forceinline__ void stream(const Vec<T>* from, int v, int end, int step, F&& work) {
+  constexpr int kAhead = 4;
+  Vec<T> next[kAhead];
+  if (v + (kAhead - 1) * step < end) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) next[i] = from[v + i * step];
+    for (; v + (2 * kAhead - 1) * step < end; v += kAhead * step)
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const Vec<T> own = next[i];
+        next[i] = from[v + (i + kAhead) * step];
+        work(own, v + i * step);
+      }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) work(next[i], v + i * step);
+    v += kAhead * step;
+  }
+#pragma unroll
+  for (int i = 0; i < kAhead - 1; ++i)
+    if (v + i * step < end) next[i] = from[v + i * step];
+#pragma unroll
+  for (int i = 0; i < kAhead - 1; ++i)
+    if (v + i * step < end) work(next[i], v + i * step);
+}
 
 // ---- running sums -------------------------------------------------------------------------------------------------------------------
 struct Sums {
   float m = kLowest, S = 0.0f, T = 0.0f;
-  __device__ __forceinline__ void move(float to) {      // to a larger m
-    const float f = st::exp2_ftz((m - to) * kLog2e);
-    T = f > 0.0f ? f * fmaf(S, m - to, T) : f * S;      // f = 0: what was seen counts for nothing, and S (m - to) may be infinite
+  __device__ __forceinline__ void shift(float y) {      // by 2^y, to a larger m
+    const float f = st::exp2_ftz(y);
+    T = f > 0.0f ? f * fmaf(S, y, T) : f * S;           // f = 0: what was seen counts for nothing, and S y may be infinite
     S *= f;
+  }
+  __device__ __forceinline__ void move(float to) {
+    shift(to == m ? 0.0f : fabsf(m) < kUsual + 1.0f && fabsf(to) < kUsual + 1.0f ? scaled(m) - scaled(to) : (m - to) * kLog2e);
     m = to;
   }
-  template <int N>
-  __device__ __forceinline__ void add(const float (&x)[N], float largest) {
-    if (largest > m + kMargin) move(largest);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float d = x[i] - m, e = st::exp2_ftz(d * kLog2e);      // NaN, and infinity less infinity, make S NaN
-      S += e;
-      T = fmaf(e, fmaxf(d, kFar), T);
-    }
+  __device__ __forceinline__ void add(float x) {        // with care
+    if (x > m + kMargin) shift((m - x) * kLog2e), m = x;
+    const float y = (x - m) * kLog2e, e = st::exp2_ftz(y);      // NaN, and infinity less infinity, make S NaN
+    S += e;
+    T = fmaf(e, fmaxf(y, kFar), T);
   }
   __device__ __forceinline__ void join(float m2, float S2, float T2) {
     Sums o;
@@ -67,6 +140,29 @@ struct Sums {
     else o.move(m);
     S += o.S;
     T += o.T;
+  }
+};
+// Two elements at a time.
+template <typename E>
+struct PairSums {
+  float m = kLeast<E>;
+  float2 S = make_float2(0.0f, 0.0f), T = make_float2(0.0f, 0.0f);
+  template <int N>
+  __device__ __forceinline__ void add(const float2 (&x)[N], float largest) {
+    if (largest > m + kMargin) {
+      Sums a, b;
+      a.S = S.x, a.T = T.x, b.S = S.y, b.T = T.y;
+      const float y = scaled(m) - scaled(largest);
+      a.shift(y), b.shift(y);
+      m = largest, S = make_float2(a.S, b.S), T = make_float2(a.T, b.T);
+    }
+    const float2 less = st::splat2(-scaled(m));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float2 y = st::fma2(x[i], st::splat2(kLog2e), less), e = make_float2(st::exp2_ftz(y.x), st::exp2_ftz(y.y));
+      S = st::add2(S, e);
+      T = st::fma2(e, y, T);
+    }
   }
 };
 __device__ __forceinline__ void join_warp(Sums& s) {
@@ -100,9 +196,10 @@ struct Candidates {
   static constexpr int kRound = W * 32 * 8, kRoom = 2 * kRound;
   unsigned long long key[kRoom];
   unsigned long long best[kMostTop];
-  unsigned long long bound[W];
+  unsigned long long bound[W], reach;      // reach: what the `top` best threads' largest elements reach
   float sums[W][3];
   int count;
+  uint16_t who[W * 32], owner[kMostTop];      // threads of the first keys; the `top` best threads
 };
 
 template <int W> __device__ __forceinline__ void sync() {
@@ -185,13 +282,27 @@ __device__ __noinline__ void select_carefully(Candidates<W>& c, const T* x, int 
   }
 }
 
+template <int W>
+__device__ __forceinline__ void join_group(Candidates<W>& c, Sums& s, int warp, int lane) {
+  join_warp(s);
+  if (W == 1) {      // lanes joined in orders of their own
+    s.m = __shfl_sync(0xffffffffu, s.m, 0), s.S = __shfl_sync(0xffffffffu, s.S, 0), s.T = __shfl_sync(0xffffffffu, s.T, 0);
+    return;
+  }
+  if (lane == 0) c.sums[warp][0] = s.m, c.sums[warp][1] = s.S, c.sums[warp][2] = s.T;
+  sync<W>();
+  s = Sums();
+#pragma unroll
+  for (int i = 0; i < W; ++i) s.join(c.sums[i][0], c.sums[i][1], c.sums[i][2]);
+}
+
 // One row (or, in a cluster, one part of it) per W warps.
 template <typename T, int W, bool TOP>
 __global__ void __launch_bounds__(kThreads) scores_kernel(const T* logits, const long long* targets, float* logprob, float* entropy, float2* stats, long long* top_ids,
                                                           float* top_logprobs, const ScoreParams p) {
   extern __shared__ __align__(16) uint8_t room[];
   chain_begin(logits, targets, logprob, entropy, stats, top_ids, top_logprobs);
-  constexpr int N = Vec<T>::N, kGroup = W * 32, kSample = 2;
+  constexpr int N = Vec<T>::N, kGroup = W * 32;
   Candidates<W>& c = reinterpret_cast<Candidates<W>*>(room)[W == 1 ? threadIdx.x >> 5 : 0];
   const int tid = threadIdx.x % kGroup, warp = tid >> 5, lane = tid & 31;
   const int part = W == 1 ? 0 : blockIdx.x % p.parts;
@@ -203,105 +314,95 @@ __global__ void __launch_bounds__(kThreads) scores_kernel(const T* logits, const
   const int vectors = (p.vocab - head) / N, rest = head + vectors * N, singles = head + p.vocab - rest;
   const int share = (vectors + p.parts - 1) / p.parts, v0 = part * share, v1 = min(vectors, v0 + share);
   const Vec<T>* xv = reinterpret_cast<const Vec<T>*>(x + head);
-  Sums s;
   if (TOP && tid == 0) c.count = 0;
+  PairSums<T> pairs;
+  Sums s;
+  float best = __uint_as_float(0x7FC00000u);      // the thread's largest element, in vector best_at
+  int best_at = -1;
+  const int one = tid < head ? tid : rest + tid - head;
+  const bool has_single = part == 0 && tid < singles;
+  const float single = has_single ? to_float(x[one]) : 0.0f;
 
-  unsigned long long bound = 0;
-  float limit = kLowest;      // value of the bound
-  const auto keep = [&](float v, int index) {
-    const unsigned long long key = key_of(v, index);
-    if (key >= bound) {
-      const int at = atomicAdd(&c.count, 1);
-      if (at < Candidates<W>::kRoom) c.key[at] = key;
-    }
-  };
-  const auto unpack = [](const Vec<T>& v, float (&f)[N], float& largest) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = to_float(v.v[i]);
-    largest = f[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) largest = fmaxf(largest, f[i]);
-  };
-
-  int v = v0 + tid;
-  {
-    Vec<T> first[kSample];
-    float single = 0.0f, f[N], largest;
-    const int one = tid < head ? tid : rest + tid - head;
-    const bool has_single = part == 0 && tid < singles;
-#pragma unroll
-    for (int i = 0; i < kSample; ++i)
-      if (v + i * kGroup < v1) first[i] = xv[v + i * kGroup];
-    if (has_single) single = to_float(x[one]);
-    unsigned long long best = 0;
-    if (has_single) {
-      const float own[1] = {single};
-      s.add(own, single);
-      if (TOP) best = key_of(single, one);
-    }
-#pragma unroll
-    for (int i = 0; i < kSample; ++i)
-      if (v + i * kGroup < v1) {
-        unpack(first[i], f, largest);
-        s.add(f, largest);
-        if (TOP) {
-          int at = 0;
-#pragma unroll
-          for (int k = N - 1; k >= 0; --k) at = f[k] == largest ? k : at;
-          best = max(best, key_of(largest, head + (v + i * kGroup) * N + at));
-        }
-      }
-    if (TOP) {
-      sync<W>();      // the count
-      bound = max(bound_of(c, best, p.top, warp, lane), 1ull);
-      limit = bound > 1 ? value_of(bound) : -INFINITY;
-      if (has_single) keep(single, one);
-#pragma unroll
-      for (int i = 0; i < kSample; ++i)
-        if (v + i * kGroup < v1) {
-          unpack(first[i], f, largest);
-          if (largest >= limit)
-#pragma unroll
-            for (int k = 0; k < N; ++k)
-              if (f[k] >= limit) keep(f[k], head + (v + i * kGroup) * N + k);
-        }
-    }
-    v += kSample * kGroup;
+  stream(xv, v0 + tid, v1, kGroup, [&](const Vec<T>& vec, int v) {
+    float2 f[N / 2];
+    usual_pairs(vec, f);
+    const float largest = largest_of(f);
+    if (TOP && !(largest <= best)) best = largest, best_at = v;
+    pairs.add(f, largest);
+  });
+  s.m = pairs.m, s.S = pairs.S.x + pairs.S.y, s.T = pairs.T.x + pairs.T.y;
+  if (has_single) {
+    const float x1 = at_least<T>(single);
+    if (x1 > s.m + kMargin) s.shift(scaled(s.m) - scaled(x1)), s.m = x1;
+    const float y = fmaf(x1, kLog2e, -scaled(s.m)), e = st::exp2_ftz(y);
+    s.S += e, s.T = fmaf(e, y, s.T);
   }
-  constexpr int kAhead = 4;
-  for (; v < v1; v += kAhead * kGroup) {
-    Vec<T> next[kAhead];
+
+  if (TOP) {
+    unsigned long long key = has_single ? key_of(single, one) : 0;
+    if (best_at >= 0) {
+      const Vec<T> again = xv[best_at];
+      int at = 0;
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-      if (v + i * kGroup < v1) next[i] = xv[v + i * kGroup];
+      for (int k = N - 1; k >= 0; --k) at = at_least<T>(to_float(again.v[k])) == best ? k : at;
+      float value = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-      if (v + i * kGroup < v1) {
-        float f[N], largest;
-        unpack(next[i], f, largest);
-        s.add(f, largest);
-        if (TOP && largest >= limit)
+      for (int k = 0; k < N; ++k) value = k == at ? to_float(again.v[k]) : value;
+      key = max(key, key_of(value, head + best_at * N + at));
+    }
+    const unsigned long long loose = max(bound_of(c, key, p.top, warp, lane), 1ull);      // and the count is 0 for all
+    sync<W>();
+    if (key >= loose) {
+      const int at = atomicAdd(&c.count, 1);
+      c.key[at] = key, c.who[at] = static_cast<uint16_t>(tid);
+    }
+    sync<W>();
+    const int n = c.count;
+    if (tid == 0 && n < p.top) c.reach = 1;
+    if (tid < n) {
+      const unsigned long long own = c.key[tid];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += c.key[j] > own;
+      if (rank < p.top) c.owner[rank] = c.who[tid];
+      if (rank == p.top - 1) c.reach = own;
+    }
+    sync<W>();
+    const unsigned long long reach = c.reach;
+    if (tid == 0) c.count = 0;
+    sync<W>();
+    const float limit = reach > 1 ? value_of(reach) : -INFINITY;
+    const auto keep = [&](float value, int index) {
+      const unsigned long long k = key_of(value, index);
+      if (value >= limit && k >= reach) {
+        const int at = atomicAdd(&c.count, 1);
+        if (at < Candidates<W>::kRoom) c.key[at] = k;
+      }
+    };
+    if (has_single) keep(single, one);
+    for (int o = warp; o < min(n, p.top); o += W)
+      for (int at = v0 + c.owner[o] + lane * kGroup; at < v1; at += 32 * kGroup) {
+        const Vec<T> again = xv[at];
 #pragma unroll
-          for (int k = 0; k < N; ++k)
-            if (f[k] >= limit) keep(f[k], head + (v + i * kGroup) * N + k);
+        for (int k = 0; k < N; ++k) keep(to_float(again.v[k]), head + at * N + k);
       }
   }
 
   // sums of the row (part): in every thread
-  join_warp(s);
-  if (W == 1) {      // lanes joined in orders of their own
-    s.m = __shfl_sync(0xffffffffu, s.m, 0), s.S = __shfl_sync(0xffffffffu, s.S, 0), s.T = __shfl_sync(0xffffffffu, s.T, 0);
-  } else {
-    if (lane == 0) c.sums[warp][0] = s.m, c.sums[warp][1] = s.S, c.sums[warp][2] = s.T;
-    sync<W>();
+  join_group(c, s, warp, lane);
+  if (!is_usual<T>(s.m) && s.S == s.S) {
     s = Sums();
-#pragma unroll
-    for (int i = 0; i < W; ++i) s.join(c.sums[i][0], c.sums[i][1], c.sums[i][2]);
+    for (int v = v0 + tid; v < v1; v += kGroup)
+      for (int k = 0; k < N; ++k) s.add(to_float(x[head + v * N + k]));
+    if (has_single) s.add(single);
+    sync<W>();
+    join_group(c, s, warp, lane);
   }
   if (TOP) {
     sync<W>();
-    // a NaN hides from comparisons (and an infinity makes S one); keys that found no room are lost
-    if (c.count > Candidates<W>::kRoom || s.S != s.S) {
+    // With care: a NaN hides from comparisons (and an infinity makes S one); keys that found no room are lost; of elements that count as the least usual one, a
+    // thread has not kept the largest.
+    const unsigned long long reach = c.reach;
+    if (c.count > Candidates<W>::kRoom || s.S != s.S || (reach > 1 && !(value_of(reach) > kLeast<T>))) {
       if (part == 0) {      // its single elements too: with one part these are the row
         if (p.parts == 1) {
           select_carefully<T, W>(c, x, 0, p.vocab, p.top, tid);
@@ -352,18 +453,22 @@ __global__ void __launch_bounds__(kThreads) scores_kernel(const T* logits, const
   }
 
   // an empty row, all -inf: no probability anywhere
-  const bool empty = s.S == 0.0f;
-  const float log_S = empty ? INFINITY : logf(s.S), m = empty ? 0.0f : s.m;
+  const bool empty = s.S == 0.0f, usual = is_usual<T>(s.m);
+  const float log_S = empty ? INFINITY : log2f(s.S), m = empty ? 0.0f : s.m;
+  const auto log_p = [&](float v) {
+    const float y = exponent(v, m, usual);
+    return y == -INFINITY ? v - m - log_S * kLn2 : (y - log_S) * kLn2;      // v log2 e may be infinite where v is not
+  };
   if (tid == 0) {
     const long long t = targets[row];
-    logprob[row] = t >= 0 && t < p.vocab ? to_float(x[t]) - m - log_S : 0.0f;
-    entropy[row] = empty ? 0.0f : log_S - s.T / s.S;
+    logprob[row] = t >= 0 && t < p.vocab ? log_p(to_float(x[t])) : 0.0f;
+    entropy[row] = empty ? 0.0f : (log_S - s.T / s.S) * kLn2;
     if (stats) stats[row] = make_float2(m, log_S);
   }
   if (TOP && tid < p.top) {
     const unsigned long long key = c.best[tid];
     top_ids[row * p.top + tid] = static_cast<long long>(~static_cast<uint32_t>(key));
-    top_logprobs[row * p.top + tid] = value_of(key) - m - log_S;
+    top_logprobs[row * p.top + tid] = log_p(value_of(key));
   }
 }
 
@@ -402,9 +507,16 @@ __global__ void __launch_bounds__(kThreads) scores_grad_kernel(const T* logits, 
   sync<W>();
   float all = 0.0f;
   for (int i = 0; i < n; ++i) all += weight[slot][i];
-  const auto shared = [&](float v) {      // what the distribution contributes
-    const float lp = v - m - log_S, e = st::exp2_ftz(lp * kLog2e);
-    return -e * fmaf(gH, fmaxf(lp, kFar) + H, all);
+  // what the distribution contributes: p (factor log2 p + rest)
+  const bool usual = is_usual<T>(m);
+  const float factor = -gH * kLn2, rest_of = -fmaf(gH, H, all);
+  const auto shared = [&](float v) {
+    const float y = exponent(v, m, usual) - log_S;
+    return st::exp2_ftz(y) * fmaf(factor, fmaxf(y, kFar), rest_of);
+  };
+  const auto shared_pair = [&](float2 v) {
+    const float2 y = st::add2(st::fma2(v, st::splat2(kLog2e), st::splat2(-scaled(m))), st::splat2(-log_S));
+    return st::mul2(make_float2(st::exp2_ftz(y.x), st::exp2_ftz(y.y)), st::fma2(st::splat2(factor), y, st::splat2(rest_of)));
   };
   if (WIDE) {
     const int head = min(p.vocab, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)));
@@ -416,19 +528,21 @@ __global__ void __launch_bounds__(kThreads) scores_grad_kernel(const T* logits, 
       const int at = tid < head ? tid : rest + tid - head;
       y[at] = from_float<T>(empty ? 0.0f : shared(to_float(x[at])));
     }
-    constexpr int kAhead = 4;
-    for (int v = v0 + tid; v < v1; v += kAhead * kGroup) {
-      Vec<T> next[kAhead];
+    if (empty || !usual) {
+      for (int v = v0 + tid; v < v1; v += kGroup)
+        for (int k = 0; k < N; ++k) y[head + v * N + k] = from_float<T>(empty ? 0.0f : shared(to_float(x[head + v * N + k])));
+    } else {
+      stream(xv, v0 + tid, v1, kGroup, [&](const Vec<T>& vec, int v) {
+        float2 f[N / 2];
+        usual_pairs(vec, f);
+        Vec<T> g;
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i)
-        if (v + i * kGroup < v1) next[i] = xv[v + i * kGroup];
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i)
-        if (v + i * kGroup < v1) {
-#pragma unroll
-          for (int k = 0; k < N; ++k) next[i].v[k] = from_float<T>(empty ? 0.0f : shared(to_float(next[i].v[k])));
-          yv[v + i * kGroup] = next[i];
+        for (int k = 0; k < N / 2; ++k) {
+          const float2 d = shared_pair(f[k]);
+          g.v[2 * k] = from_float<T>(d.x), g.v[2 * k + 1] = from_float<T>(d.y);
         }
+        yv[v] = g;
+      });
     }
   } else {
     const int share_e = (p.vocab + p.parts - 1) / p.parts;
