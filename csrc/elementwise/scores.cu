@@ -165,11 +165,14 @@ struct PairSums {
     }
   }
 };
-__device__ __forceinline__ void join_warp(Sums& s) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m = __shfl_xor_sync(0xffffffffu, s.m, o), S = __shfl_xor_sync(0xffffffffu, s.S, o), T = __shfl_xor_sync(0xffffffffu, s.T, o);
-    s.join(m, S, T);
+// Sums of a warp's lanes, or of the first `lanes` (a power of two) of them, in the same for all of these: the largest m first, then one shift each.
+__device__ __forceinline__ void join_lanes(Sums& s, int lanes) {
+  float m = s.m;
+  for (int o = lanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  s.move(m);
+  for (int o = lanes / 2; o > 0; o >>= 1) {
+    s.S += __shfl_xor_sync(0xffffffffu, s.S, o);
+    s.T += __shfl_xor_sync(0xffffffffu, s.T, o);
   }
 }
 
@@ -197,7 +200,7 @@ struct Candidates {
   unsigned long long key[kRoom];
   unsigned long long best[kMostTop];
   unsigned long long bound[W], reach;      // reach: what the `top` best threads' largest elements reach
-  float sums[W][3];
+  float sums[W][3], total[3];
   int count;
   uint16_t who[W * 32], owner[kMostTop];      // threads of the first keys; the `top` best threads
 };
@@ -282,18 +285,21 @@ __device__ __noinline__ void select_carefully(Candidates<W>& c, const T* x, int 
   }
 }
 
+// The sums of all of a row's threads, in all of them.
 template <int W>
 __device__ __forceinline__ void join_group(Candidates<W>& c, Sums& s, int warp, int lane) {
-  join_warp(s);
-  if (W == 1) {      // lanes joined in orders of their own
-    s.m = __shfl_sync(0xffffffffu, s.m, 0), s.S = __shfl_sync(0xffffffffu, s.S, 0), s.T = __shfl_sync(0xffffffffu, s.T, 0);
-    return;
-  }
+  join_lanes(s, 32);
+  if (W == 1) return;
   if (lane == 0) c.sums[warp][0] = s.m, c.sums[warp][1] = s.S, c.sums[warp][2] = s.T;
   sync<W>();
-  s = Sums();
-#pragma unroll
-  for (int i = 0; i < W; ++i) s.join(c.sums[i][0], c.sums[i][1], c.sums[i][2]);
+  if (warp == 0) {
+    const int i = lane & (W - 1);
+    s.m = c.sums[i][0], s.S = c.sums[i][1], s.T = c.sums[i][2];
+    join_lanes(s, W);
+    if (lane == 0) c.total[0] = s.m, c.total[1] = s.S, c.total[2] = s.T;
+  }
+  sync<W>();
+  s.m = c.total[0], s.S = c.total[1], s.T = c.total[2];
 }
 
 // One row (or, in a cluster, one part of it) per W warps.
@@ -372,8 +378,9 @@ __global__ void __launch_bounds__(kThreads) scores_kernel(const T* logits, const
     sync<W>();
     const float limit = reach > 1 ? value_of(reach) : -INFINITY;
     const auto keep = [&](float value, int index) {
+      if (!(value >= limit)) return;
       const unsigned long long k = key_of(value, index);
-      if (value >= limit && k >= reach) {
+      if (k >= reach) {
         const int at = atomicAdd(&c.count, 1);
         if (at < Candidates<W>::kRoom) c.key[at] = k;
       }
@@ -382,8 +389,11 @@ __global__ void __launch_bounds__(kThreads) scores_kernel(const T* logits, const
     for (int o = warp; o < min(n, p.top); o += W)
       for (int at = v0 + c.owner[o] + lane * kGroup; at < v1; at += 32 * kGroup) {
         const Vec<T> again = xv[at];
+        float2 f[N / 2];
+        again.pairs(f);
+        if (!(largest_of(f) >= limit)) continue;
 #pragma unroll
-        for (int k = 0; k < N; ++k) keep(to_float(again.v[k]), head + at * N + k);
+        for (int k = 0; k < N; ++k) keep(k % 2 ? f[k / 2].y : f[k / 2].x, head + at * N + k);
       }
   }
 
