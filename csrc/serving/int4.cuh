@@ -56,4 +56,29 @@ template <> __device__ __forceinline__ uint32_t codes_to_pair<__half>(uint32_t w
   return *reinterpret_cast<const uint32_t*>(&d);
 }
 
+// Two codes times their scale in a type, exactly.  bf16 in one step: 64 + code, whose unit is bit 1, times s less 72 s, both of which bf16 holds.  fp16 does not
+// hold 72 s of large scales: the code first.
+template <typename T> struct Scale;
+template <> struct Scale<__nv_bfloat16> {
+  __nv_bfloat162 s, less;
+  __device__ __forceinline__ void set(uint32_t low16) {
+    const uint32_t both = __byte_perm(low16, 0, 0x1010);
+    s = *reinterpret_cast<const __nv_bfloat162*>(&both);
+    less = __hmul2(s, __float2bfloat162_rn(-72.0f));
+  }
+  __device__ __forceinline__ uint32_t pair(uint32_t word, int e) const {
+    const uint32_t v = pick(e == 0 ? word << 1 : word >> (4 * e - 1), 0x001E001Eu, 0x42804280u);
+    const __nv_bfloat162 d = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&v), s, less);
+    return *reinterpret_cast<const uint32_t*>(&d);
+  }
+};
+template <> struct Scale<__half> {
+  __half2 s;
+  __device__ __forceinline__ void set(uint32_t low16) { s = __float2half2_rn(bf16_bits(low16 & 0xFFFFu)); }
+  __device__ __forceinline__ uint32_t pair(uint32_t word, int e) const {
+    const uint32_t v = codes_to_pair<__half>(word, e);
+    const __half2 d = __hmul2(*reinterpret_cast<const __half2*>(&v), s);
+    return *reinterpret_cast<const uint32_t*>(&d);
+  }
+};
 }  // namespace st4

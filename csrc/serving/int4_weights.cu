@@ -13,6 +13,7 @@
 #include "../common/host.h"
 #include "../common/chain.cuh"
 #include "int4.cuh"
+#include <type_traits>
 
 namespace {
 using namespace st4;
@@ -27,27 +28,80 @@ struct WeightsParams {
   int rows, cols, groups, chunks, blocks;      // groups of a row; tiles and 128-column blocks beside one another
 };
 
-// The scale from the group's least and largest element.
-__device__ __forceinline__ float scale_of(float low, float high, bool finite) {
+// The scale from the group's least and largest element, either of which is NaN where one of the group is.
+__device__ __forceinline__ float scale_of(float low, float high) {
   const bool pos = high > -low;      // the extremum is positive: the scale negative
   uint32_t u = __float_as_uint(fmaxf(high, -low) * 0.125f);
   u = (u + 0x7FFFFu + ((u >> 20) & 1u)) & ~0xFFFFFu;      // 3 of 23 bits behind the leading one
   const float s = fminf(fmaxf(__uint_as_float(u), kLeast), kLargest);
-  return !finite ? __uint_as_float(0x7FC00000u) : pos ? -s : s;
+  return !(isfinite(low) && isfinite(high)) ? __uint_as_float(0x7FC00000u) : pos ? -s : s;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
 }
 
-// w / s to the nearest, ties to even.  w * (1 / s) may fall on the wrong side of a border; the remainder, which fmaf gives exactly, says so.
-__device__ __forceinline__ int code_of(float w, float s, float inv, float half) {
-  float q = rintf(w * inv);
-  const float r = fmaf(-q, s, w);
-  const float a = fabsf(r);
-  if (a > half || (a == half && (static_cast<int>(q) & 1))) q += (r < 0.0f) == (s < 0.0f) ? 1.0f : -1.0f;
-  return static_cast<int>(fminf(fmaxf(q, -8.0f), 7.0f));      // NaN: -8, which the scale covers
+// 16 bytes or, of fp32, 32: 8 elements of a row.
+template <typename T> __device__ __forceinline__ void extremes(const Vec<T, 8>& v, float& low, float& high);
+template <> __device__ __forceinline__ void extremes(const Vec<float, 8>& v, float& low, float& high) {
+  low = high = v.v[0];
+#pragma unroll
+  for (int e = 1; e < 8; ++e) low = min_nan(low, v.v[e]), high = max_nan(high, v.v[e]);
+}
+template <> __device__ __forceinline__ void extremes(const Vec<__nv_bfloat16, 8>& v, float& low, float& high) {
+  const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&v);
+  const __nv_bfloat162 a = __hmin2_nan(__hmin2_nan(p[0], p[1]), __hmin2_nan(p[2], p[3])), b = __hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3]));
+  low = min_nan(__low2float(a), __high2float(a)), high = max_nan(__low2float(b), __high2float(b));
+}
+template <> __device__ __forceinline__ void extremes(const Vec<__half, 8>& v, float& low, float& high) {
+  const __half2* p = reinterpret_cast<const __half2*>(&v);
+  const __half2 a = __hmin2_nan(__hmin2_nan(p[0], p[1]), __hmin2_nan(p[2], p[3])), b = __hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3]));
+  low = min_nan(__low2float(a), __high2float(a)), high = max_nan(__low2float(b), __high2float(b));
+}
+
+// 8 codes plus 8, four bits each: w / s to the nearest, ties to even, within -8..7.
+// w * (1 / s) may lie up to 2^-20 beside the quotient.  A quotient of a 16-bit w that is no tie is at least 2^-16 from one (w is at most 11 bits, s 4): rounded to multiples of
+// 2^-18 first, ties are ties again and nothing else changes sides.  For fp32 the remainder, which fmaf gives exactly, says on which side of the border w is.
+template <typename T>
+__device__ __forceinline__ uint32_t codes_of(const Vec<T, 8>& v, float s) {
+  const float inv = 1.0f / s;
+  uint32_t packed = 0;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      float2 t = st::mul2(make_float2(to_float(v.v[e]), to_float(v.v[e + 1])), st::splat2(inv));
+      t = make_float2(fminf(fmaxf(t.x, -8.0f), 7.0f), fminf(fmaxf(t.y, -8.0f), 7.0f));      // NaN: -8, which the scale covers
+      t = st::add2(st::add2(t, st::splat2(48.0f)), st::splat2(-48.0f));
+      t = st::add2(t, st::splat2(12582912.0f + 8.0f));                                    // 1.5 2^23: whole numbers in the low bits
+      packed += (__float_as_uint(t.x) << (4 * e)) + (__float_as_uint(t.y) << (4 * e + 4));
+    }
+    uint32_t more = 0;      // 0x4B400000 of each
+#pragma unroll
+    for (int e = 0; e < 8; ++e) more += 0x4B400000u << (4 * e);
+    return packed - more;
+  } else {
+    const float half = 0.5f * fabsf(s);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float w = v.v[e];
+      float q = rintf(w * inv);
+      const float r = fmaf(-q, s, w), a = fabsf(r);
+      if (a > half || (a == half && (static_cast<int>(q) & 1))) q += (r < 0.0f) == (s < 0.0f) ? 1.0f : -1.0f;
+      packed |= static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(q, -8.0f), 7.0f)) + 8) << (4 * e);
+    }
+    return packed;
+  }
 }
 
 // Lane l of a warp holds columns 8 (l % 16) to 8 (l % 16) + 7 of rows 2 i + l / 16.
-template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const T* w, uint8_t* codes, __nv_bfloat16* scales, const WeightsParams p, const int group) {
+template <typename T, int GROUP, bool WIDE>
+__global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const T* w, uint8_t* codes, __nv_bfloat16* scales, const WeightsParams p) {
   __shared__ uint32_t word[kWarps][16][17];      // 8 codes of a row; 17: rows on banks of their own
   chain_begin(w, codes, scales);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -56,47 +110,32 @@ __global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const T* w, uint8
   if (u * kTileRows >= p.rows) return;
   const int c0 = j * kCols + (lane & 15) * 8, r0 = u * kTileRows + (lane >> 4);
   Vec<T, 8> v[8];
+  const T* at = w + r0 * p.stride + c0;
+  if (WIDE && (u + 1) * kTileRows <= p.rows && (j + 1) * kCols <= p.cols) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = r0 + 2 * i;
-    const T* at = w + r * p.stride + c0;
-    if (WIDE && r < p.rows && c0 + 8 <= p.cols) {
-      if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<uint4*>(&v[i]) = *reinterpret_cast<const uint4*>(at);
-      } else {
-        reinterpret_cast<uint4*>(&v[i])[0] = reinterpret_cast<const uint4*>(at)[0];
-        reinterpret_cast<uint4*>(&v[i])[1] = reinterpret_cast<const uint4*>(at)[1];
-      }
-    } else {
+    for (int i = 0; i < 8; ++i, at += 2 * p.stride)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[i].v[e] = r < p.rows && c0 + e < p.cols ? at[e] : from_float<T>(0.0f);
-    }
+      for (int h = 0; h < static_cast<int>(sizeof(T)) / 2; ++h) reinterpret_cast<uint4*>(&v[i])[h] = reinterpret_cast<const uint4*>(at)[h];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i, at += 2 * p.stride)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i].v[e] = r0 + 2 * i < p.rows && c0 + e < p.cols ? at[e] : from_float<T>(0.0f);
   }
+  __nv_bfloat16* to = scales + (static_cast<long long>(u) * p.groups + c0 / GROUP) * 16 + (lane >> 4) * 2;
+  const bool first = c0 % GROUP == 0 && c0 / GROUP < p.groups;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float low = to_float(v[i].v[0]), high = low;
-    bool finite = true;
+    float low, high;
+    extremes(v[i], low, high);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = to_float(v[i].v[e]);
-      low = fminf(low, x);
-      high = fmaxf(high, x);
-      finite = finite && isfinite(x);
+    for (int o = 1; o < GROUP / 8; o <<= 1) {
+      low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
+      high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
     }
-    for (int o = 1; o < group / 8; o <<= 1) {
-      low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-      high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
-      finite = __shfl_xor_sync(0xffffffffu, finite, o) && finite;
-    }
-    const float s = scale_of(low, high, finite), inv = 1.0f / s, half = 0.5f * fabsf(s);
-    uint32_t packed = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) packed |= static_cast<uint32_t>(code_of(to_float(v[i].v[e]), s, inv, half) + 8) << (4 * e);
-    const int row = 2 * i + (lane >> 4);
-    word[warp][row][lane & 15] = packed;
-    const int at = c0 / group;
-    if (c0 % group == 0 && at < p.groups)
-      scales[(static_cast<long long>(u) * p.groups + at) * 16 + 2 * (row & 7) + (row >> 3)] = __float2bfloat16_rn(s);
+    const float s = scale_of(low, high);
+    word[warp][2 * i + (lane >> 4)][lane & 15] = codes_of(v[i], s);
+    if (first) to[(i & 3) * 4 + (i >> 2)] = __float2bfloat16_rn(s);      // row 2 i + l / 16: place 2 (row % 8) + row / 8
   }
   __syncwarp();
   const int g = lane >> 2, t = lane & 3;
@@ -105,33 +144,49 @@ __global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const T* w, uint8
     if (2 * j + c >= p.chunks) break;
     uint32_t out[4];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      out[s] = 0;
+    for (int s = 0; s < 4; ++s) {      // byte t of 8 codes: columns 2 t and 2 t + 1 of them; of the 4 bytes the low nibbles, then the high ones
+      uint32_t four = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {      // byte t of 8 codes: columns 2 t and 2 t + 1 of them
-        const uint32_t pair = word[warp][g + 8 * (e & 1)][8 * c + 2 * s + (e >> 1)] >> (8 * t);
-        out[s] |= (pair & 15u) << (4 * e) | ((pair >> 4) & 15u) << (4 * e + 16);
-      }
+      for (int e = 0; e < 4; ++e) four |= (word[warp][g + 8 * (e & 1)][8 * c + 2 * s + (e >> 1)] >> (8 * t) & 0xFFu) << (8 * e);
+      const uint32_t low = four & 0x0F0F0F0Fu, high = four >> 4 & 0x0F0F0F0Fu;
+      out[s] = __byte_perm(low | low >> 4, high | high >> 4, 0x6420);
     }
     *reinterpret_cast<uint4*>(codes + (static_cast<long long>(u) * p.chunks + 2 * j + c) * kTileBytes + lane * 16) = make_uint4(out[0], out[1], out[2], out[3]);
   }
 }
 
-template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* codes, const __nv_bfloat16* scales, T* w, const WeightsParams p, const int group) {
-  __shared__ uint4 word[kWarps][2][4][8];      // [tile][word][g]: those of lanes 4 g to 4 g + 3 together
+// The pairs of numbers that a lane's words hold go to shared memory as rows, from where they leave 16 bytes a lane.
+template <typename T, int GROUP, bool WIDE>
+__global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* codes, const __nv_bfloat16* scales, T* w, const WeightsParams p) {
+  using E = typename std::conditional<std::is_same<T, __half>::value, __half, __nv_bfloat16>::type;      // fp32 from bf16, which holds them all
+  __shared__ __align__(16) uint32_t pair[kWarps][16][68];      // 64 pairs of a row; 68: rows on banks of their own
   chain_begin(codes, scales, w);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const long long b = static_cast<long long>(blockIdx.x) * kWarps + warp;
   const int u = static_cast<int>(b / p.blocks), j = static_cast<int>(b - static_cast<long long>(u) * p.blocks);
   if (u * kTileRows >= p.rows) return;
+  uint4 in[2];
+  uint32_t both[128 / GROUP];      // scales of rows g and g + 8
+  const uint32_t* from = reinterpret_cast<const uint32_t*>(scales + (static_cast<long long>(u) * p.groups + j * (128 / GROUP)) * 16) + g;
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+    if (2 * j + c < p.chunks) in[c] = *reinterpret_cast<const uint4*>(codes + (static_cast<long long>(u) * p.chunks + 2 * j + c) * kTileBytes + lane * 16);
+#pragma unroll
+  for (int i = 0; i < 128 / GROUP; ++i)
+    if (j * (128 / GROUP) + i < p.groups) both[i] = from[i * 8];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     if (2 * j + c >= p.chunks) break;
-    const uint4 in = *reinterpret_cast<const uint4*>(codes + (static_cast<long long>(u) * p.chunks + 2 * j + c) * kTileBytes + lane * 16);
-    const uint32_t part[4] = {in.x, in.y, in.z, in.w};
+    const uint32_t word[4] = {in[c].x, in[c].y, in[c].z, in[c].w};
+    Scale<E> low, high;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) reinterpret_cast<uint32_t*>(word[warp][c][s])[lane] = part[s];
+    for (int s = 0; s < 4; ++s) {
+      constexpr int kSteps = GROUP >= 64 ? 4 : 2;      // of 16 columns in a group
+      if (s % kSteps == 0) low.set(both[(c * 64 + s * 16) / GROUP]), high.set(both[(c * 64 + s * 16) / GROUP] >> 16);
+      uint32_t* to = &pair[warp][g][c * 32 + s * 8 + t];
+      to[0] = low.pair(word[s], 0), to[4] = low.pair(word[s], 2);
+      to[8 * 68] = high.pair(word[s], 1), to[8 * 68 + 4] = high.pair(word[s], 3);
+    }
   }
   __syncwarp();
   const int c0 = j * kCols + (lane & 15) * 8;
@@ -140,29 +195,26 @@ __global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* 
   for (int i = 0; i < 8; ++i) {
     const int row = 2 * i + (lane >> 4), r = u * kTileRows + row;
     if (r >= p.rows) break;
-    const uint4 in = word[warp][(lane >> 3) & 1][(lane & 7) >> 1][row & 7];
-    const uint32_t part[4] = {in.x, in.y, in.z, in.w};
-    const float s = __bfloat162float(scales[(static_cast<long long>(u) * p.groups + c0 / group) * 16 + 2 * (row & 7) + (row >> 3)]);
-    const int e = 2 * (lane & 1) + (row >> 3);
-    Vec<T, 8> v;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      v.v[2 * t] = from_float<T>(static_cast<float>(static_cast<int>((part[t] >> (4 * e)) & 15u) - 8) * s);
-      v.v[2 * t + 1] = from_float<T>(static_cast<float>(static_cast<int>((part[t] >> (4 * e + 16)) & 15u) - 8) * s);
-    }
+    const uint4 eight = *reinterpret_cast<const uint4*>(&pair[warp][row][(lane & 15) * 4]);
     T* at = w + r * p.stride + c0;
-    if (WIDE && c0 + 8 <= p.cols) {
-      if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(&v);
-      } else {
-        reinterpret_cast<uint4*>(at)[0] = reinterpret_cast<const uint4*>(&v)[0];
-        reinterpret_cast<uint4*>(at)[1] = reinterpret_cast<const uint4*>(&v)[1];
+    if constexpr (sizeof(T) == 2) {
+      if (WIDE && c0 + 8 <= p.cols) {
+        *reinterpret_cast<uint4*>(at) = eight;
+        continue;
       }
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (c0 + k < p.cols) at[k] = v.v[k];
     }
+    const Vec<E, 8> v = *reinterpret_cast<const Vec<E, 8>*>(&eight);
+    if constexpr (sizeof(T) == 4) {
+      if (WIDE && c0 + 8 <= p.cols) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          reinterpret_cast<float4*>(at)[h] = make_float4(to_float(v.v[4 * h]), to_float(v.v[4 * h + 1]), to_float(v.v[4 * h + 2]), to_float(v.v[4 * h + 3]));
+        continue;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c0 + k < p.cols) at[k] = from_float<T>(to_float(v.v[k]));
   }
 }
 
@@ -178,20 +230,32 @@ int plan(WeightsParams& p, unsigned& grid, int group, const void* codes, const v
   return ST_OK;
 }
 
-template <typename T>
-int quantize(const void* w, uint8_t* codes, __nv_bfloat16* scales, const WeightsParams& p, unsigned grid, int group, cudaStream_t stream) {
+template <typename T, int GROUP>
+int quantize(const void* w, uint8_t* codes, __nv_bfloat16* scales, const WeightsParams& p, unsigned grid, cudaStream_t stream) {
   const bool wide = (reinterpret_cast<uintptr_t>(w) & 15) == 0 && p.stride * sizeof(T) % 16 == 0;
-  const cudaError_t e = st::chained(wide ? quantize_kernel<T, true> : quantize_kernel<T, false>, dim3(grid), dim3(kWarps * 32), 0, stream)(
-      static_cast<const T*>(w), codes, scales, p, group);
+  const cudaError_t e = st::chained(wide ? quantize_kernel<T, GROUP, true> : quantize_kernel<T, GROUP, false>, dim3(grid), dim3(kWarps * 32), 0, stream)(
+      static_cast<const T*>(w), codes, scales, p);
   return e == cudaSuccess ? ST_OK : st::fail_cuda(e, "int4 quantize");
 }
+template <typename T>
+int quantize(const void* w, uint8_t* codes, __nv_bfloat16* scales, const WeightsParams& p, unsigned grid, int group, cudaStream_t stream) {
+  if (group == 32) return quantize<T, 32>(w, codes, scales, p, grid, stream);
+  if (group == 64) return quantize<T, 64>(w, codes, scales, p, grid, stream);
+  return quantize<T, 128>(w, codes, scales, p, grid, stream);
+}
 
+template <typename T, int GROUP>
+int dequantize(const uint8_t* codes, const __nv_bfloat16* scales, void* w, const WeightsParams& p, unsigned grid, cudaStream_t stream) {
+  const bool wide = (reinterpret_cast<uintptr_t>(w) & 15) == 0 && p.stride * sizeof(T) % 16 == 0;
+  const cudaError_t e = st::chained(wide ? dequantize_kernel<T, GROUP, true> : dequantize_kernel<T, GROUP, false>, dim3(grid), dim3(kWarps * 32), 0, stream)(
+      codes, scales, static_cast<T*>(w), p);
+  return e == cudaSuccess ? ST_OK : st::fail_cuda(e, "int4 dequantize");
+}
 template <typename T>
 int dequantize(const uint8_t* codes, const __nv_bfloat16* scales, void* w, const WeightsParams& p, unsigned grid, int group, cudaStream_t stream) {
-  const bool wide = (reinterpret_cast<uintptr_t>(w) & 15) == 0 && p.stride * sizeof(T) % 16 == 0;
-  const cudaError_t e = st::chained(wide ? dequantize_kernel<T, true> : dequantize_kernel<T, false>, dim3(grid), dim3(kWarps * 32), 0, stream)(
-      codes, scales, static_cast<T*>(w), p, group);
-  return e == cudaSuccess ? ST_OK : st::fail_cuda(e, "int4 dequantize");
+  if (group == 32) return dequantize<T, 32>(codes, scales, w, p, grid, stream);
+  if (group == 64) return dequantize<T, 64>(codes, scales, w, p, grid, stream);
+  return dequantize<T, 128>(codes, scales, w, p, grid, stream);
 }
 }  // namespace
 

@@ -49,8 +49,12 @@ class Weights:
                 or codes.shape != (down, -(-in_features // 64), 512) or scales.shape != (down, -(-in_features // group), 16) or codes.device != scales.device:
             raise ValueError(f"int4: codes {codes.dtype} {tuple(codes.shape)} and scales {scales.dtype} {tuple(scales.shape)} are no weights of "
                              f"{out_features} x {in_features} in groups of {group}")
-        for name, value in zip(self.__slots__, (codes, scales, out_features, in_features, group)):
+        self._set(codes, scales, out_features, in_features, group)
+
+    def _set(self, *values):
+        for name, value in zip(self.__slots__, values):
             object.__setattr__(self, name, value)
+        return self
 
     def __setattr__(self, name, value):
         raise AttributeError("int4.Weights: sizes and memory stay as they were checked")
@@ -61,8 +65,8 @@ class Weights:
         if group not in GROUPS or not (0 < out_features <= 1 << 30 and 0 < in_features <= 1 << 30):
             raise ValueError(f"int4: a matrix of {out_features} x {in_features} in groups of {group} is not supported")
         down = -(-out_features // 16)
-        return cls(torch.empty((down, -(-in_features // 64), 512), dtype=torch.uint8, device=device),
-                   torch.empty((down, -(-in_features // group), 16), dtype=torch.bfloat16, device=device), out_features, in_features, group)
+        codes = torch.empty((down, -(-in_features // 64), 512), dtype=torch.uint8, device=device)
+        return cls.__new__(cls)._set(codes, codes.new_empty((down, -(-in_features // group), 16), dtype=torch.bfloat16), out_features, in_features, group)
 
     @property
     def nbytes(self) -> int:
@@ -141,10 +145,9 @@ def quantize(weight: torch.Tensor, group: int = 64, *, out: Optional[Weights] = 
     else:
         if (out.out_features, out.in_features, out.group) != (n, k, group):
             raise ValueError(f"int4.quantize: a {n} x {k} matrix in groups of {group} into weights of {out.out_features} x {out.in_features} in groups of {out.group}")
-        native.same_device("int4.quantize", weight, out.codes, out.scales)
-    weight = weight.detach()
-    if not native.use_native(weight):
-        q, s = quantize_reference(weight, group)
+        native.same_device("int4.quantize", weight, out.codes)
+    if not weight.is_cuda:
+        q, s = quantize_reference(weight.detach(), group)
         out.codes.copy_(_tiles(q))
         s = torch.nn.functional.pad(s, (0, 0, 0, -n % 16), value=LEAST_SCALE)
         out.scales.copy_(s.view(-1, 2, 8, s.shape[1]).permute(0, 3, 2, 1).flatten(-2))
@@ -155,7 +158,8 @@ def quantize(weight: torch.Tensor, group: int = 64, *, out: Optional[Weights] = 
     with native.on_device(index):
         st = native.entry("st_int4_quantize", "pppiiqiip")(weight.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), n, k, weight.stride(0), group,
                                                          _TYPES[weight.dtype], native.raw_stream(index))
-    native.check(st, "st_int4_quantize")
+    if st:
+        native.check(st, "st_int4_quantize")
     launch_count += 1
     return out
 

@@ -6,6 +6,7 @@ likeliest tokens beside them, in one pass over the logits; differentiable.
 Reference parity: none (its losses take probabilities and give one number)."""
 from __future__ import annotations
 
+import struct
 from typing import NamedTuple
 
 import torch
@@ -15,6 +16,8 @@ from . import native
 launch_count = 0
 MOST_TOP = 32
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+# StTokenScoresArgs of csrc/elementwise/scores.cu, in one call: a ctypes object for each of a dozen arguments costs as much as the launch
+_pack_args = struct.Struct("@7P2q3i").pack
 
 
 class TokenScores(NamedTuple):
@@ -75,21 +78,24 @@ def _gradient_reference(logits, targets, ids, g_logprob, g_entropy, g_top):
 def _forward(logits, targets, top, keep):
     """Scores of ``[rows, vocab]`` and, where ``keep``, what the gradient needs."""
     global launch_count
-    if not native.use_native(logits):
+    if not logits.is_cuda:
         return token_scores_reference(logits, targets, top), None
     rows, vocab = logits.shape
     index = native.require_cuda("token_scores", logits, targets)
-    # one allocation for the 32-bit results: several take longer than the launch
-    stats, logprob, entropy, top_logprobs = torch.empty((4 + top) * rows, dtype=torch.float32, device=logits.device).split_with_sizes(
-        (2 * rows, rows, rows, rows * top))      # pairs first: they lie on 8-byte boundaries
-    ids = torch.empty((rows, top), dtype=torch.int64, device=logits.device)
+    ids = targets.new_empty((rows, top))
+    logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    entropy, top_logprobs = logprob.new_empty(rows), logprob.new_empty((rows, top))
+    stats = logprob.new_empty((rows, 2)) if keep else None
+    if rows == 0:
+        return TokenScores(logprob, entropy, ids, top_logprobs), stats
+    args = _pack_args(logits.data_ptr(), targets.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), native.address(stats), ids.data_ptr(), top_logprobs.data_ptr(), rows,
+                      logits.stride(0), vocab, top, _TYPES[logits.dtype])
     with native.on_device(index):
-        st = native.entry("st_token_scores", "pppppppqqiiip")(
-            logits.data_ptr(), targets.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr() if keep else 0, ids.data_ptr(), top_logprobs.data_ptr(),
-            rows, logits.stride(0), vocab, top, _TYPES[logits.dtype], native.raw_stream(index))
-    native.check(st, "st_token_scores")
+        st = native.entry("st_token_scores", "sp")(args, native.raw_stream(index))
+    if st:
+        native.check(st, "st_token_scores")
     launch_count += 1
-    return TokenScores(logprob, entropy, ids, top_logprobs.view(rows, top)), stats
+    return TokenScores(logprob, entropy, ids, top_logprobs), stats
 
 
 class _TokenScoresFn(torch.autograd.Function):
@@ -134,26 +140,32 @@ def token_scores(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0) -
     nothing else has entropy 0, log probabilities of -inf and no gradient.  A row with a NaN or ``+inf`` has NaN for all of its scores.
 
     Differentiable in ``logits`` through ``logprob``, ``entropy`` and ``top_logprobs``; the logits must not change before that."""
-    if logits.dtype not in _TYPES and not (logits.dtype == torch.float64 and not logits.is_cuda):
+    on_cuda, shape = logits.is_cuda, targets.shape
+    if logits.dtype not in _TYPES and not (logits.dtype == torch.float64 and not on_cuda):
         raise ValueError(f"token_scores: bf16, fp16 or fp32 logits, got {logits.dtype}")
-    if logits.dim() < 1 or targets.shape != logits.shape[:-1] or targets.dtype != torch.int64:
-        raise ValueError(f"token_scores: targets must be int64 {tuple(logits.shape[:-1])}, got {targets.dtype} {tuple(targets.shape)}")
+    if logits.dim() < 1 or shape != logits.shape[:-1] or targets.dtype is not torch.int64:
+        raise ValueError(f"token_scores: targets must be int64 {tuple(logits.shape[:-1])}, got {targets.dtype} {tuple(shape)}")
     vocab = logits.shape[-1]
     if not 1 <= vocab <= 1 << 30:
         raise ValueError(f"token_scores: a vocabulary of {vocab}")
     if not 0 <= top <= min(MOST_TOP, vocab):
         raise ValueError(f"token_scores: top must be 0 to {min(MOST_TOP, vocab)}, got {top}")
-    native.same_device("token_scores", logits, targets)
+    if not on_cuda:
+        native.same_device("token_scores", logits, targets)
     if native.has_tangent(logits):
         raise ValueError("token_scores: forward-mode differentiation is not supported")
-    shape = targets.shape
-    rows, flat = logits.reshape(-1, vocab), targets.reshape(-1).contiguous()
-    if rows.stride(1) != 1 and vocab > 1:
+    flat = len(shape) == 1
+    rows = logits if flat else logits.reshape(-1, vocab)
+    if not flat:
+        targets = targets.reshape(-1)
+    if not targets.is_contiguous():
+        targets = targets.contiguous()
+    if vocab > 1 and rows.stride(1) != 1:
         rows = rows.contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
-        scores = _TokenScoresFn.apply(rows, flat, top)
+        scores = _TokenScoresFn.apply(rows, targets, top)
     else:
-        scores = _forward(rows, flat, top, False)[0]
-    if len(shape) == 1:
-        return TokenScores(*scores)
+        scores = _forward(rows, targets, top, False)[0]
+    if flat:
+        return scores if type(scores) is TokenScores else TokenScores(*scores)
     return TokenScores(scores[0].view(shape), scores[1].view(shape), scores[2].view(*shape, top), scores[3].view(*shape, top))
