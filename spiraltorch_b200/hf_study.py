@@ -36,6 +36,8 @@ from typing import Callable, Dict, Iterable, Iterator, List, Mapping, Optional, 
 
 import torch
 
+from .ops import int4
+
 PLAN_SCHEMA = "spiraltorch_b200.hf_study_plan.v1"
 EVENT_SCHEMA = "spiraltorch_b200.hf_study_event.v1"
 SUMMARY_SCHEMA = "spiraltorch_b200.hf_study_summary.v1"
@@ -317,17 +319,40 @@ def run_study(plan: Mapping[str, object], runner: Optional[Callable[[Mapping[str
 
 # ---------------------------------------------------------------------------------------------------------------
 # LoRA on torch modules
-class LoraWrapped(torch.nn.Module):
-    """``y = base(x) + (alpha / r) · x A B`` over a frozen ``nn.Linear`` or GPT-2 ``Conv1D``; B starts at zero."""
+class FrozenLinear4(torch.nn.Module):
+    """A frozen ``nn.Linear`` or GPT-2 ``Conv1D`` with its weight in four bits (:mod:`spiraltorch_b200.ops.int4`): a quarter of the memory of 16 bits, and
+    a gradient for its input.  On a GPU for bf16 and fp16 activations."""
 
-    def __init__(self, base: torch.nn.Module, rank: int, alpha: float, generator: Optional[torch.Generator] = None):
+    def __init__(self, base: torch.nn.Module, group: int = 64):
+        super().__init__()
+        w = base.weight.detach()
+        held = int4.quantize(w.t() if type(base).__name__ == "Conv1D" else w, group)
+        self.out_features, self.in_features, self.group = held.out_features, held.in_features, group
+        self.register_buffer("codes", held.codes)
+        self.register_buffer("scales", held.scales.view(torch.int16))      # as bits: a cast of the module's floats must not round them
+        self.bias = None if base.bias is None else torch.nn.Parameter(base.bias.detach(), requires_grad=False)
+
+    def held(self) -> int4.Weights:
+        return int4.Weights(self.codes, self.scales.view(torch.bfloat16), self.out_features, self.in_features, self.group)
+
+    def forward(self, x):
+        return int4.linear(x, self.held(), self.bias)
+
+
+class LoraWrapped(torch.nn.Module):
+    """``y = base(x) + (alpha / r) · x A B`` over a frozen ``nn.Linear`` or GPT-2 ``Conv1D``; B starts at zero.  ``base_bits`` 4: the
+    frozen weight in four bits (:class:`FrozenLinear4`)."""
+
+    def __init__(self, base: torch.nn.Module, rank: int, alpha: float, generator: Optional[torch.Generator] = None, base_bits: int = 16, group: int = 64):
         super().__init__()
         w = base.weight
         conv1d = type(base).__name__ == "Conv1D"               # transformers' GPT-2 layer stores (in, out)
         fan_in, fan_out = (w.shape[0], w.shape[1]) if conv1d else (w.shape[1], w.shape[0])
         if not 1 <= rank <= min(fan_in, fan_out):
             raise StudyError(f"rank {rank} outside [1, {min(fan_in, fan_out)}]")
-        self.base, self.scale = base, alpha / rank
+        if base_bits not in (4, 16):
+            raise StudyError(f"base weights of 4 or 16 bits, got {base_bits}")
+        self.base, self.scale = FrozenLinear4(base, group) if base_bits == 4 else base, alpha / rank
         for p in base.parameters():
             p.requires_grad_(False)
         a = torch.empty(fan_in, rank, dtype=w.dtype, device=w.device)
@@ -341,8 +366,9 @@ class LoraWrapped(torch.nn.Module):
         return self.scale * (self.lora_a @ self.lora_b)
 
 
-def inject_lora(model: torch.nn.Module, targets: Sequence[str], rank: int, alpha: float = 16.0, seed: int = 0) -> List[str]:
-    """Freeze ``model`` and wrap every ``nn.Linear`` / ``Conv1D`` whose qualified name ends with one of ``targets``."""
+def inject_lora(model: torch.nn.Module, targets: Sequence[str], rank: int, alpha: float = 16.0, seed: int = 0, base_bits: int = 16, group: int = 64) -> List[str]:
+    """Freeze ``model`` and wrap every ``nn.Linear`` / ``Conv1D`` whose qualified name ends with one of ``targets``; ``base_bits`` 4 holds their frozen
+    weights in four bits with a scale for every ``group`` inputs."""
     for p in model.parameters():
         p.requires_grad_(False)
     gen = torch.Generator().manual_seed(seed)
@@ -353,7 +379,7 @@ def inject_lora(model: torch.nn.Module, targets: Sequence[str], rank: int, alpha
         if not (isinstance(module, torch.nn.Linear) or type(module).__name__ == "Conv1D"):
             continue
         parent = model.get_submodule(name.rpartition(".")[0]) if "." in name else model
-        setattr(parent, name.rpartition(".")[2], LoraWrapped(module, rank, alpha, gen))
+        setattr(parent, name.rpartition(".")[2], LoraWrapped(module, rank, alpha, gen, base_bits, group))
         wrapped.append(name)
     if not wrapped:
         raise StudyError(f"no layer matches the LoRA targets {list(targets)}")
@@ -489,10 +515,10 @@ def _lm_loss(model, batch):
 
 def lora_finetune_run(config: Mapping[str, object], output_dir: Path, *, model_factory: Optional[Callable[[], torch.nn.Module]] = None) -> dict:
     """One run of a study.  ``config`` keys (all optional): steps, batch_size, seq_len, lr, weight_decay, lora_rank,
-    lora_alpha, lora_targets, eval_batches, corpus (path of a text file; a synthetic corpus otherwise), corpus_seed,
+    lora_alpha, lora_targets, base_bits (4: the frozen layers in four bits), eval_batches, corpus (path of a text file; a synthetic corpus otherwise), corpus_seed,
     model (kwargs of ``ByteCausalLM``), pretrain_steps (dense steps on the first half of the corpus before adapters go
     in, standing in for a pretrained checkpoint), feedback (``LossFeedbackGate`` fields), device."""
-    c = {"steps": 60, "batch_size": 16, "seq_len": 64, "lr": 3e-3, "weight_decay": 0.0, "lora_rank": 4, "lora_alpha": 8.0,
+    c = {"steps": 60, "batch_size": 16, "seq_len": 64, "lr": 3e-3, "weight_decay": 0.0, "lora_rank": 4, "lora_alpha": 8.0, "base_bits": 16,
          "lora_targets": ["attn.qkv", "attn.proj", "mlp.fc", "mlp.out"], "eval_batches": 4, "corpus": None, "corpus_seed": 1234, "model": {},
          "pretrain_steps": 0, "feedback": {}, "device": "cpu", "arm": "observe", "seed": 0, **dict(config)}
     device, seed = torch.device(c["device"]), int(c["seed"])
@@ -517,7 +543,7 @@ def lora_finetune_run(config: Mapping[str, object], output_dir: Path, *, model_f
             opt0.zero_grad(set_to_none=True)
             _lm_loss(model, windows(train[: train.numel() // 2], int(c["batch_size"]), gp)).backward()
             opt0.step()
-    wrapped = inject_lora(model, list(c["lora_targets"]), int(c["lora_rank"]), float(c["lora_alpha"]), seed)
+    wrapped = inject_lora(model, list(c["lora_targets"]), int(c["lora_rank"]), float(c["lora_alpha"]), seed, int(c["base_bits"]))
     params = [p for p in model.parameters() if p.requires_grad]
     opt = torch.optim.AdamW(params, lr=float(c["lr"]), weight_decay=float(c["weight_decay"]))
     gate = gate_for_arm(str(c["arm"]), c["feedback"])

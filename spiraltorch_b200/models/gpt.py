@@ -39,6 +39,7 @@ from ..ops import loss as loss_ops
 from ..ops import native
 from ..ops import norm as norm_ops
 from ..ops import rotary as rotary_ops
+from ..ops import scoring
 from ..parallel.tp import TPContext
 
 
@@ -394,17 +395,33 @@ class GPTModel(nn.Module):
         return _GPTLossFn.apply(self, tokens, targets, loss_scale, self.p["norm_f.gamma"])
 
     # ------------------------------------------------------------------------------------------
-    def decoder(self, sequences: int, max_length: int, *, pages: Optional[int] = None, page_size: int = 64):
+    def decoder(self, sequences: int, max_length: int, *, pages: Optional[int] = None, page_size: int = 64, weight_bits: int = 16, head_bits: int = 16,
+                group: int = 64):
         """A :class:`~spiraltorch_b200.models.gpt_decoder.GPTDecoder` of this model: an 8-bit paged cache for ``sequences``
-        sequences of up to ``max_length`` tokens."""
+        sequences of up to ``max_length`` tokens, and weights of 16 bits or 4 (with a scale for every ``group`` inputs)."""
         from .gpt_decoder import GPTDecoder
-        return GPTDecoder(self, sequences, max_length, pages=pages, page_size=page_size)
+        return GPTDecoder(self, sequences, max_length, pages=pages, page_size=page_size, weight_bits=weight_bits, head_bits=head_bits, group=group)
 
-    def generate(self, prompts, max_new_tokens: int, *, stop: Optional[int] = None, page_size: int = 64) -> list:
+    def generate(self, prompts, max_new_tokens: int, *, stop: Optional[int] = None, page_size: int = 64, scores: Optional[int] = None, weight_bits: int = 16,
+                 head_bits: int = 16) -> list:
         """The likeliest continuation of each prompt (a list of token ids), token by token, up to ``max_new_tokens`` or the token ``stop``.
-        Returns the new tokens of each."""
+        Returns the new tokens of each; with ``scores`` (0 to 32 alternatives) their scores too, as ``GPTDecoder.generate`` does."""
         longest = max((len(p) for p in prompts), default=0) + max(max_new_tokens - 1, 0)      # the last new token is not appended
-        return self.decoder(len(prompts), longest, page_size=page_size).generate(prompts, max_new_tokens, stop=stop)
+        decoder = self.decoder(len(prompts), longest, page_size=page_size, weight_bits=weight_bits, head_bits=head_bits)
+        return decoder.generate(prompts, max_new_tokens, stop=stop, scores=scores)
+
+    @torch.no_grad()
+    def score(self, tokens: torch.Tensor, *, top: int = 0) -> scoring.TokenScores:
+        """Scores of the tokens of ``[B, S]`` (int64) behind each other: ``[B, S - 1]``, those of token ``i + 1`` at ``i``; ``top`` of the likeliest alternatives of each.
+        A token below 0 is padding: it has log probability 0 and the model reads token 0 in its place."""
+        if self.tp.world != 1:
+            raise ValueError("GPTModel.score: tensor-parallel models are not supported")
+        if tokens.dim() != 2 or tokens.shape[1] < 2 or tokens.dtype != torch.int64:
+            raise ValueError(f"GPTModel.score: int64 tokens [B, S] with two positions at least, got {tokens.dtype} {tuple(tokens.shape)}")
+        logits, _ = self._forward(tokens.clamp(min=0), None, 1.0, keep=False)
+        # the last position of a sequence has no token behind it
+        targets = torch.cat([tokens[:, 1:], tokens.new_full((tokens.shape[0], 1), loss_ops.IGNORE_INDEX)], 1)
+        return scoring.TokenScores(*(t[:, :-1] for t in scoring.token_scores(logits.view(*tokens.shape, -1), targets, top=top)))
 
     # ------------------------------------------------------------------------------------------
     def sync_replicated_grads(self) -> None:

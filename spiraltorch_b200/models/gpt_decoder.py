@@ -9,23 +9,36 @@ values that later tokens do, by weights that are rounded to bf16 there and to fp
 A part of a prompt beside single tokens of other sequences slows these: attention takes its tile from the longest part (``max_queries``).  63 single tokens at
 4096 with 16 heads take 170 us, with a part of 256 tokens in the same call 497, where the part alone takes 39.
 
+A step of few sequences is little but reading weights: ``weight_bits=4`` (and ``head_bits=4`` for the logits' product) keeps a copy of the matrices in four bits
+(:mod:`ops.int4`), which :meth:`GPTDecoder.refresh` makes anew after an update of the model.
+
 The reference has no counterpart (its language models do not decode with a cache)."""
 from __future__ import annotations
 
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 
 from ..ops import attention as attn_ops
 from ..ops import elementwise as ew
 from ..ops import gemm as gemm_ops
+from ..ops import int4
 from ..ops import native
 from ..ops import paged
 from ..ops import rotary as rotary_ops
+from ..ops import scoring
 
 # Tokens of a whole prompt.  16 heads of 128, us over the cache and read back, one prompt: 512 tokens 22 and 66, 1024 28 and 50, 1536 45 and 51, 2048 71 and 51,
 # 4096 167 and 88.  Reading back takes two launches for each prompt, the cache's kernel one for all: four prompts of 2048 188 and 211, of 4096 521 and 353.
 DENSE_FROM = 2048
+
+
+class GeneratedScores(NamedTuple):
+    """For every new token of a sequence: its log probability, the entropy of the distribution behind it, the likeliest tokens and theirs."""
+    logprob: list
+    entropy: list
+    top_ids: list
+    top_logprobs: list
 
 
 class GPTDecoder:
@@ -35,9 +48,12 @@ class GPTDecoder:
     :meth:`step` do not pass through them: once a step has been captured, every other call first takes them from the device (:meth:`sync`).
 
     A kernel that gives up (a page that is none, a wait that runs out) leaves an error record; :meth:`extend` and :meth:`step` raise what calls and replays before
-    them left, :meth:`generate` what its own passes leave."""
+    them left, :meth:`generate` what its own passes leave.
 
-    def __init__(self, model, sequences: int, max_length: int, *, pages: Optional[int] = None, page_size: int = 64):
+    ``weight_bits`` 4: the layers' matrices in four bits, with a scale for every ``group`` inputs; ``head_bits`` 4: those of the logits too."""
+
+    def __init__(self, model, sequences: int, max_length: int, *, pages: Optional[int] = None, page_size: int = 64, weight_bits: int = 16, head_bits: int = 16,
+                 group: int = 64):
         cfg = model.cfg
         if model.tp.world != 1:
             raise ValueError("GPTDecoder: tensor-parallel models are not supported")
@@ -45,6 +61,8 @@ class GPTDecoder:
             raise ValueError(f"GPTDecoder: {sequences} sequences of up to {max_length} tokens")
         if cfg.positional == "learned" and max_length > cfg.seq_len:
             raise ValueError(f"GPTDecoder: learned positions end at {cfg.seq_len}, not at {max_length}")
+        if weight_bits not in (4, 16) or head_bits not in (4, 16):
+            raise ValueError(f"GPTDecoder: weights of 4 or 16 bits, got {weight_bits} and {head_bits} for the logits")
         self.model, self.sequences, self.max_length, self.page_size = model, sequences, max_length, page_size
         dev = model.flat_w.device
         width = -(-max_length // page_size)
@@ -63,6 +81,17 @@ class GPTDecoder:
         self._taking = torch.ones(sequences, **i32)
         self._place_of_row, self._row_of_place = torch.arange(sequences, device=dev), torch.arange(sequences, device=dev)
         self._captured = False
+        names = [f"h{l}.{n}.weight" for l in range(cfg.n_layers) for n in ("qkv", "proj", "fc1", "fc2")] if weight_bits == 4 else []
+        self.weights = {n: int4.quantize(model.p[n], group) for n in names + (["embed.weight"] if head_bits == 4 else [])}
+
+    def refresh(self) -> None:
+        """The weights in four bits from what the model's are now, in the memory that captured steps read."""
+        for n, held in self.weights.items():
+            int4.quantize(self.model.p[n], held.group, out=held)
+
+    def _product(self, x: torch.Tensor, name: str, act: Optional[str] = None) -> torch.Tensor:
+        held = self.weights.get(name)
+        return gemm_ops.gemm(x, self.model.p[name], act=act) if held is None else int4.linear(x, held, act=act)
 
     # ---- host side ------------------------------------------------------------------------------------------------------------
     def _blocks(self, tokens: int) -> int:
@@ -130,22 +159,22 @@ class GPTDecoder:
             y, h, _, _ = m._norm_fwd(resid if x is None else x, f"h{l}.norm1", residual=None if x is None else resid)
             if x is not None:
                 resid = h
-            qkv = gemm_ops.gemm(y, m.p[f"h{l}.qkv.weight"]).view(rows, 3, H, D)
+            qkv = self._product(y, f"h{l}.qkv.weight").view(rows, 3, H, D)
             q, k, v = qkv[:, 0], qkv[:, 1], qkv[:, 2]
             if m.rope_freq is not None:
                 rotary_ops.rotary_(q, k, step.positions, m.rope_freq, interleaved=cfg.rope_interleaved)
             paged.store(k, v, self.cache[l], step.slots)
             o = self._dense(q, l, counts, step.lengths) if dense else paged.attention(q, self.cache[l], self.table, step.starts, step.lengths, max_queries=most)
-            a = gemm_ops.gemm(o.view(rows, H * D), m.p[f"h{l}.proj.weight"])
+            a = self._product(o.view(rows, H * D), f"h{l}.proj.weight")
             y, resid, _, _ = m._norm_fwd(a, f"h{l}.norm2", residual=resid)
-            u = gemm_ops.gemm(y, m.p[f"h{l}.fc1.weight"], act="gelu")
-            x = gemm_ops.gemm(u, m.p[f"h{l}.fc2.weight"])
+            u = self._product(y, f"h{l}.fc1.weight", "gelu")
+            x = self._product(u, f"h{l}.fc2.weight")
         if last is not None:
             x, resid = x.index_select(0, last), resid.index_select(0, last)
         y, _, _, _ = m._norm_fwd(x, "norm_f", residual=resid)
         if by_place:
             y = ew.embedding_forward(self._row_of_place, y)
-        logits = gemm_ops.gemm(y, m.p["embed.weight"])
+        logits = self._product(y, "embed.weight")
         # only now does the step take effect: a call that failed before appended nothing, and what it wrote to the table and the pages is written anew
         self.lengths.copy_(step.lengths)
         self.free_count.copy_(step.free_count)
@@ -226,30 +255,38 @@ class GPTDecoder:
         self._lost = [x and not d for x, d in zip(self._lost, done)]
         self._wait([w or d for w, d in zip(self._waiting, done)])
 
-    def generate(self, prompts: Sequence, max_new_tokens: int, *, stop: Optional[int] = None) -> list:
+    def generate(self, prompts: Sequence, max_new_tokens: int, *, stop: Optional[int] = None, scores: Optional[int] = None):
         """The likeliest continuation of a prompt in every place, up to ``max_new_tokens`` or the token ``stop`` (which is not returned).
-        A place that met ``stop`` waits.  Starts from empty places."""
+        A place that met ``stop`` waits.  Starts from empty places.
+
+        ``scores``: returns ``(tokens, scores)``, with a :class:`GeneratedScores` of each sequence's tokens and as many of their likeliest alternatives (0 to 32)."""
         self._settle()
         if any(self.held):
             raise ValueError("GPTDecoder: generate starts from empty places; release them first")
         if max_new_tokens < 0 or any(len(p) == 0 for p in prompts):
             raise ValueError("GPTDecoder: prompts need a token at least")
-        out = [[] for _ in prompts]
+        if scores is not None and not 0 <= scores <= min(scoring.MOST_TOP, self.model.cfg.vocab_size):
+            raise ValueError(f"GPTDecoder: scores with 0 to {min(scoring.MOST_TOP, self.model.cfg.vocab_size)} alternatives, got {scores}")
+        out, judged = [[] for _ in prompts], [GeneratedScores([], [], [], []) for _ in prompts]
         if max_new_tokens == 0:
-            return out
+            return out if scores is None else (out, judged)
         active = list(range(self.sequences))
         logits = self.extend(prompts)
         while True:
             best = logits.argmax(-1)
+            given = None if scores is None else [t.tolist() for t in scoring.token_scores(logits, best, top=scores)]
             going, feed, chosen = [], [[] for _ in prompts], best.tolist()
             native.poll()      # the pass is done
-            for b, t in zip(active, chosen):
+            for i, (b, t) in enumerate(zip(active, chosen)):
                 if t != stop:
                     out[b].append(t)
+                    if given is not None:
+                        for to, values in zip(judged[b], given):
+                            to.append(values[i])
                     if len(out[b]) < max_new_tokens:
                         going.append(b)
                         feed[b] = [t]
             if not going:
-                return out
+                return out if scores is None else (out, judged)
             active = going
             logits = self.step(best) if len(going) == self.sequences else self.extend(feed)

@@ -301,3 +301,130 @@ def test_kernel_refusals():
                  lambda: int4.dequantize(held, torch.float64), lambda: int4.quantize(torch.randn(20, 70), 32, out=held), lambda: int4.linear(x.bfloat16(), held.to("cpu"))):
         with pytest.raises(ValueError):
             call()
+
+
+# ---- where the framework uses them ------------------------------------------------------------------------------------------------
+def _small_model(device="cpu", dtype=torch.float32):
+    from spiraltorch_b200.models.gpt import GPTConfig, GPTModel
+    return GPTModel(GPTConfig(vocab_size=96, d_model=128, n_layers=2, n_heads=2, ffn=256, seq_len=256, init_std=0.08), device=device, dtype=dtype)
+
+
+def _with_quantised(model, head):
+    """The same model, its matrices replaced by what four bits stand for."""
+    for name, p in model.p.items():
+        if p.dim() == 2 and (head or name != "embed.weight"):
+            p.data.copy_(int4.dequantize(int4.quantize(p, 64), p.dtype))
+    return model
+
+
+@pytest.mark.parametrize("head", [False, True])
+def test_decoder_with_four_bit_weights(head):
+    """Equal, but for the order of sums, to a decoder of the model whose weights are what the four bits stand for (with a head of 16 bits the embedding stays)."""
+    prompts = [[1, 2, 3], [7], list(range(30))]
+    d = _small_model().decoder(3, 64, weight_bits=4, head_bits=4 if head else 16)
+    assert len(d.weights) == 8 + head
+    plain = _with_quantised(_small_model(), False)
+    e = plain.decoder(3, 64)
+    got, want = d.extend(prompts), e.extend(prompts)
+    if head:      # the embedding of the tokens stays in 16 bits, the product with it does not
+        assert not torch.allclose(got, want, atol=1e-4) and torch.nn.functional.cosine_similarity(got, want).min() > 0.97
+    else:
+        assert torch.allclose(got, want, atol=1e-4)
+    for p, q in zip(d.model.p.values(), plain.p.values()):      # an update of the model, and the four bits made anew
+        p.data.mul_(0.5)
+        q.data.mul_(0.5)
+    d.refresh()
+    one = torch.tensor([4, 5, 6])
+    if not head:
+        assert torch.allclose(d.step(one), e.step(one), atol=1e-4)
+    with pytest.raises(ValueError, match="4 or 16"):
+        _small_model().decoder(1, 8, weight_bits=8)
+
+
+def test_generate_with_four_bit_weights():
+    model = _small_model()
+    assert model.generate([[1, 2, 3], [9]], 5, weight_bits=4) == _with_quantised(_small_model(), False).generate([[1, 2, 3], [9]], 5)
+
+
+def test_frozen_layers_in_four_bits_train_their_adapters():
+    from spiraltorch_b200 import hf_study as H
+    torch.manual_seed(0)
+    model = H.ByteCausalLM(d_model=32, n_layer=1, n_head=2, max_len=16)
+    dense = model.blocks[0].attn.qkv.weight.detach().clone()
+    H.inject_lora(model, ["attn.qkv", "mlp.out"], rank=2, base_bits=4, group=32)
+    layer = model.blocks[0].attn.qkv
+    with torch.no_grad():
+        layer.lora_b.normal_()
+    w = int4.dequantize(int4.quantize(dense, 32), torch.float32)
+    x = torch.randn(3, 32, requires_grad=True)
+    y = layer(x)
+    want = x @ (w.t() + layer.merged_delta()) + layer.base.bias
+    assert torch.allclose(y, want, atol=1e-5)
+    dy = torch.randn_like(y)
+    got = torch.autograd.grad(y, (x, layer.lora_a, layer.lora_b), dy, retain_graph=True)
+    ref = torch.autograd.grad(want, (x, layer.lora_a, layer.lora_b), dy)
+    assert all(torch.allclose(a, b, atol=1e-5) for a, b in zip(got, ref))
+    assert [n for n, p in model.named_parameters() if p.requires_grad] == [f"blocks.0.{m}.lora_{s}" for m in ("attn.qkv", "mlp.out") for s in "ab"]
+    state = model.state_dict()
+    other = H.ByteCausalLM(d_model=32, n_layer=1, n_head=2, max_len=16)
+    H.inject_lora(other, ["attn.qkv", "mlp.out"], rank=2, base_bits=4, group=32)
+    other.load_state_dict(state)
+    ids = torch.randint(0, 256, (2, 16))
+    assert torch.equal(other(ids), model(ids))
+    assert torch.equal(layer.base.double().held().scales, layer.base.held().scales)      # a cast leaves the scales' bits
+    with pytest.raises(H.StudyError, match="4 or 16"):
+        H.inject_lora(H.ByteCausalLM(d_model=32, n_layer=1, n_head=2), ["attn.qkv"], rank=2, base_bits=8)
+
+
+def test_a_study_run_with_frozen_layers_in_four_bits(tmp_path):
+    from spiraltorch_b200 import hf_study as H
+    out = H.lora_finetune_run({"steps": 2, "batch_size": 2, "seq_len": 16, "model": {"d_model": 32, "n_layer": 1, "n_head": 2}, "eval_batches": 1, "base_bits": 4}, tmp_path)
+    assert out["steps"] == 2 and math.isfinite(out["eval_loss_after"])
+
+
+@GPU
+def test_decoder_with_four_bit_weights_on_the_gpu():
+    """A whole run: prompts, steps, a captured step, an update and its replay, against the model whose weights are what the four bits stand for.  Both round the same
+    products to bf16 and sum them in other orders, so a layer's input may differ by a bf16 step here and there; the logits' directions agree."""
+    model = _small_model("cuda", torch.bfloat16)
+    plain = _with_quantised(_small_model("cuda", torch.bfloat16), False)
+    d, e = model.decoder(3, 128, weight_bits=4), plain.decoder(3, 128)
+    prompts = [[1, 2, 3], [7], list(range(60))]
+
+    def close(a, b):
+        assert torch.nn.functional.cosine_similarity(a.float(), b.float()).min() > 0.999
+
+    close(d.extend(prompts), e.extend(prompts))
+    tokens = torch.tensor([4, 5, 6], device="cuda")
+    close(d.step(tokens), e.step(tokens))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        logits = d.step(tokens)
+    for p, q in zip(model.p.values(), plain.p.values()):
+        p.data.mul_(0.5)
+        q.data.mul_(0.5)
+    d.refresh()
+    graph.replay()
+    close(logits, e.step(tokens))
+    big = _small_model("cuda", torch.bfloat16)
+    tokens, scores = big.generate(prompts, 4, weight_bits=4, head_bits=4, scores=3)
+    assert [len(t) for t in tokens] == [4, 4, 4]
+    for t, s in zip(tokens, scores):
+        assert [row[0] for row in s.top_ids] == t and s.logprob == [row[0] for row in s.top_logprobs] and all(x >= 0 for x in s.entropy)
+
+
+@GPU
+def test_frozen_layers_in_four_bits_on_the_gpu():
+    from spiraltorch_b200 import hf_study as H
+    torch.manual_seed(0)
+    layer = torch.nn.Linear(200, 136).to(cuda, torch.bfloat16)
+    w = int4.dequantize(int4.quantize(layer.weight.detach(), 64), torch.float32).double()
+    wrapped = H.LoraWrapped(layer, 4, 8.0, base_bits=4)
+    x = torch.randn(2, 30, 200, device=cuda, dtype=torch.bfloat16, requires_grad=True)
+    y = wrapped.base(x)
+    dy = torch.randn_like(y)
+    dx = torch.autograd.grad(y, x, dy)[0]
+    want = dy.double() @ w
+    assert ((dx.double() - want).abs().view(60, 200) <= _allowed(dy.double().view(60, 136), w.T, want.view(60, 200), torch.bfloat16)).all()
+    wrapped(x).sum().backward()
+    assert wrapped.lora_b.grad.isfinite().all() and x.grad.isfinite().all()

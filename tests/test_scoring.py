@@ -287,3 +287,64 @@ def test_kernel_refusals():
     for call in (lambda: scoring.token_scores(x.to(cuda), t), lambda: scoring.token_scores(x, t.to(cuda)), lambda: scoring.token_scores(x.to(cuda).double(), t.to(cuda))):
         with pytest.raises(ValueError):
             call()
+
+
+# ---- where the framework uses them ------------------------------------------------------------------------------------------------
+def _model(device="cpu", dtype=torch.float32):
+    from spiraltorch_b200.models.gpt import GPTConfig, GPTModel
+    return GPTModel(GPTConfig(vocab_size=96, d_model=128, n_layers=2, n_heads=2, ffn=256, seq_len=256, init_std=0.08), device=device, dtype=dtype)
+
+
+def _check_model_scores(model):
+    g = torch.Generator().manual_seed(4)
+    tokens = torch.randint(0, 96, (3, 17), generator=g).to(model.flat_w.device)
+    tokens[1, 9:] = -1
+    got = model.score(tokens, top=4)
+    logits = model(tokens.clamp(min=0)).view(3, 17, 96).float()
+    lp = torch.log_softmax(logits.double(), -1)
+    assert got.logprob.shape == got.entropy.shape == (3, 16) and got.top_ids.shape == got.top_logprobs.shape == (3, 16, 4)
+    want = lp[:, :-1].gather(2, tokens[:, 1:].clamp(min=0)[..., None])[..., 0]
+    want = torch.where(tokens[:, 1:] >= 0, want, 0.0)
+    assert torch.allclose(got.logprob.double(), want, atol=2e-5) and (got.logprob[1, 8:] == 0).all()
+    assert torch.allclose(got.entropy.double(), -(lp.exp() * lp).sum(-1)[:, :-1], atol=2e-5)
+    assert torch.allclose(got.top_logprobs.double(), lp[:, :-1].topk(4).values, atol=2e-5)
+    # minus the mean of the log probabilities is the loss
+    whole = tokens.clamp(min=0)
+    s = model.score(whole)
+    targets = torch.cat([whole[:, 1:], whole.new_full((3, 1), -100)], 1)
+    with torch.no_grad():
+        assert torch.allclose(-s.logprob.mean(), model(whole, targets), atol=2e-5)
+
+
+def test_scores_of_a_model():
+    model = _model()
+    _check_model_scores(model)
+    with pytest.raises(ValueError):
+        model.score(torch.zeros(3, 1, dtype=torch.int64))
+    with pytest.raises(ValueError):
+        model.score(torch.zeros(5, dtype=torch.int64))
+
+
+def test_generated_tokens_with_scores():
+    model = _model()
+    prompts = [[1, 2, 3], [7], list(range(30))]
+    plain = model.generate(prompts, 6)
+    tokens, scores = model.generate(prompts, 6, scores=5)
+    assert tokens == plain
+    for p, t, s in zip(prompts, tokens, scores):
+        assert len(s.logprob) == len(s.entropy) == len(s.top_ids) == len(s.top_logprobs) == 6
+        assert [row[0] for row in s.top_ids] == t and [row[0] for row in s.top_logprobs] == s.logprob
+        # the first of them is what the model says of the prompt
+        got = model.score(torch.tensor([p + t[:1]]), top=5)
+        assert abs(float(got.logprob[0, -1]) - s.logprob[0]) < 0.1 and abs(float(got.entropy[0, -1]) - s.entropy[0]) < 0.1      # the cache holds 8 bits
+    stop = tokens[0][2]
+    cut, judged = model.generate(prompts, 6, stop=stop, scores=0)
+    assert [len(t) for t in cut] == [len(s.logprob) for s in judged] and all(row == [] for s in judged for row in s.top_ids)
+    assert model.generate(prompts, 0, scores=2) == ([[], [], []], [([], [], [], [])] * 3)
+    with pytest.raises(ValueError, match="alternatives"):
+        model.generate(prompts, 1, scores=33)
+
+
+@GPU
+def test_scores_of_a_model_on_the_gpu():
+    _check_model_scores(_model("cuda", torch.bfloat16))
