@@ -19,6 +19,7 @@ struct LinearParams {
   long long x_row, residual_row, y_row;      // in elements
   int tokens, rows, cols, groups, chunks, units, group, act;
   bool wide;      // rows of x lie on 16-byte boundaries
+  int parts;      // blocks of a cluster
 };
 
 template <typename T> __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]);
@@ -35,7 +36,7 @@ template <> __device__ __forceinline__ void mma<__half>(float (&d)[4], const uin
 
 // x in shared memory: a token's 64 columns of a chunk are 128 bytes, in which the 16 bytes at 64 p + 16 t hold what lane t of a row's 4 takes to steps 2 p and 2 p + 1:
 // columns 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of each.  Tokens are 64 bytes more than a whole number of 128 apart, so that 8 lanes read from all banks.
-constexpr int kWarps = 8;
+constexpr int kWarps = 8, kMostParts = 8;
 
 // A thread takes 8 columns (step s, half h; word t of them goes to 16 (s / 2) + 4 t + 2 (s % 2) + h) of every second or of all tokens, four at a time.  What stands in the
 // place of tokens that there are none of does not matter: they are columns of their own.
@@ -96,7 +97,7 @@ struct Slice {
         if (c0 + i < chunks) w[i] = *reinterpret_cast<const uint4*>(from + i * kTileBytes);
 #pragma unroll
       for (int i = 0; i < kWords; ++i)
-        if (i * 32 + lane < (groups - g0) * 8 && i * 32 + lane < kScales * 8) s[i] = words[i * 32];
+        s[i] = i * 32 + lane < min(kScales, groups - g0) * 8 ? words[i * 32] : 0u;      // half a chunk may be behind the last group
     }
   }
   // of chunk i, half k of it where groups are halves
@@ -106,11 +107,12 @@ struct Slice {
   }
 };
 
-// Blocks take tile rows (16 weight rows) in turns; their 8 warps share the columns, C chunks of 64 each and that for `phases` stretches of 8 C.  The weights are the matrix
-// instruction's 16-row operand, NT times 8 tokens its columns.  The products of a group are summed on their own and take its scale in fp32, so codes enter as the
-// whole numbers that they are.  The next row's codes are on their way while one is multiplied.
+// Blocks take tile rows (16 weight rows) in turns; their 8 warps share the columns, C chunks of 64 each: a stretch of 8 C.  Where there are more columns, a cluster's
+// blocks take a stretch each (every eighth, beyond 8) and join their sums.  The weights are the matrix instruction's 16-row operand, NT times 8 tokens its
+// columns.  The products of a group are summed on their own and take its scale in fp32, so codes enter as the whole numbers that they are.
+// The next row's codes are on their way while one is multiplied.
 template <typename T, int NT, int C, int GROUP>
-__global__ void __launch_bounds__(kWarps * 32) linear_kernel(const T* x, const uint8_t* codes, const __nv_bfloat16* scales, const T* bias, const T* residual, T* y,
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) linear_kernel(const T* x, const uint8_t* codes, const __nv_bfloat16* scales, const T* bias, const T* residual, T* y,
                                                             const LinearParams p) {
   extern __shared__ __align__(16) uint32_t room[];
   chain_begin(x, codes, scales, bias, residual, y);
@@ -118,9 +120,10 @@ __global__ void __launch_bounds__(kWarps * 32) linear_kernel(const T* x, const u
   constexpr int kStride = kColumns / 2 + 16;                   // words of a token
   constexpr int kGroups = GROUP >= 64 ? 1 : 2, kSteps = 4 / kGroups;      // groups of a chunk, steps of 16 columns in each
   uint32_t* tokens = room;
-  float* part = reinterpret_cast<float*>(room + kTokens * kStride);      // two of [warp][token][row]
+  float* part = reinterpret_cast<float*>(room + kTokens * kStride);       // two of [warp][token][row]
+  float* total = part + 2 * kWarps * kOuts;                               // two of [token][row], in a cluster
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int phases = (p.cols + kColumns - 1) / kColumns;
+  const int rank = p.parts > 1 ? static_cast<int>(st::cluster_ctarank()) : 0, stretches = (p.cols + kColumns - 1) / kColumns;
   const auto stage = [&](int ph) { stage_tokens<T, kColumns>(x, p.x_row, tokens, kStride, p.tokens, ph * kColumns, p.cols, p.wide); };
   const long long tile_row = static_cast<long long>(p.chunks) * kTileBytes, scale_row = static_cast<long long>(p.groups) * 16;
   constexpr int kOwn = (kOuts + kWarps * 32 - 1) / (kWarps * 32);      // elements of the result that a thread writes
@@ -171,7 +174,8 @@ __global__ void __launch_bounds__(kWarps * 32) linear_kernel(const T* x, const u
       add[j] = residual && in ? to_float(residual[m * p.residual_row + r]) : 0.0f;
     }
   };
-  const auto finish = [&](int u, float* mine) {      // the warps' sums, in the order of the warps
+  const auto finish = [&](int u, int flip) {      // the warps' sums, in the order of the warps; in a cluster then the blocks', in theirs
+    float* mine = part + flip * kWarps * kOuts;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -180,69 +184,102 @@ __global__ void __launch_bounds__(kWarps * 32) linear_kernel(const T* x, const u
         acc[n][e] = 0.0f;
       }
     __syncthreads();
+    if (p.parts > 1) {
+#pragma unroll
+      for (int j = 0; j < kOwn; ++j) {
+        const int i = j * kWarps * 32 + threadIdx.x;
+        if (i >= min(kOuts, p.tokens * kTileRows)) continue;
+        float v = mine[i];
+#pragma unroll
+        for (int k = 1; k < kWarps; ++k) v += mine[k * kOuts + i];
+        total[flip * kOuts + i] = v;
+      }
+      st::cluster_sync();
+    }
 #pragma unroll
     for (int j = 0; j < kOwn; ++j) {
       const int i = j * kWarps * 32 + threadIdx.x, m = i / kTileRows, r = u * kTileRows + i % kTileRows;
       if (i >= kOuts || m >= p.tokens || r >= p.rows) continue;
-      float v = mine[i];
+      float v;
+      if (p.parts > 1) {
+        if (m % p.parts != rank) continue;      // a token's 16 rows by one of the blocks
+        float f[kMostParts];
+        const uint32_t at = st::smem_u32(total + flip * kOuts + i);
 #pragma unroll
-      for (int k = 1; k < kWarps; ++k) v += mine[k * kOuts + i];
+        for (int q = 0; q < kMostParts; ++q)
+          if (q < p.parts) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f[q]) : "r"(st::cluster_map(at, q)));
+        v = f[0];
+#pragma unroll
+        for (int q = 1; q < kMostParts; ++q)
+          if (q < p.parts) v += f[q];
+      } else {
+        v = mine[i];
+#pragma unroll
+        for (int k = 1; k < kWarps; ++k) v += mine[k * kOuts + i];
+      }
       y[m * p.y_row + r] = from_float<T>(activate(v + off[j], p.act) + add[j]);
     }
   };
 #pragma unroll
   for (int j = 0; j < kOwn; ++j) off[j] = add[j] = 0.0f;
-  float* other = part + kWarps * kOuts;
   Slice<C, GROUP> a, b;
-  int u = blockIdx.x;
-  const int step = gridDim.x;
-  fetch(a, u, 0);
-  if (phases == 1) {
+  int u = blockIdx.x / p.parts;
+  const int step = gridDim.x / p.parts;
+  fetch(a, u, rank);
+  if (rank + p.parts >= stretches) {      // this block's only stretch: its x stays
     addends(u);
-    stage(0);
+    stage(rank);
     __syncthreads();
     for (;;) {      // two rows at a time: what is on its way needs no copy
-      if (u + step < p.units) fetch(b, u + step, 0);
-      multiply(a, 0);
-      finish(u, part);
+      if (u + step < p.units) fetch(b, u + step, rank);
+      multiply(a, rank);
+      finish(u, 0);
       if ((u += step) >= p.units) break;
       addends(u);
-      if (u + step < p.units) fetch(a, u + step, 0);
-      multiply(b, 0);
-      finish(u, other);
+      if (u + step < p.units) fetch(a, u + step, rank);
+      multiply(b, rank);
+      finish(u, 1);
       if ((u += step) >= p.units) break;
       addends(u);
     }
   } else {
-    for (; u < p.units; u += step) {
+    for (int flip = 0; u < p.units; u += step, flip ^= 1) {
       addends(u);
-      for (int ph = 0; ph < phases; ++ph) {
+      for (int s = rank; s < stretches; s += p.parts) {
         __syncthreads();      // the stretch before has been read
-        stage(ph);
+        stage(s);
         __syncthreads();
         b = a;
-        const bool more = ph + 1 < phases;
-        if (more || u + step < p.units) fetch(a, more ? u : u + step, more ? ph + 1 : 0);
-        multiply(b, ph);
+        const bool more = s + p.parts < stretches;
+        if (more || u + step < p.units) fetch(a, more ? u : u + step, more ? s + p.parts : rank);
+        multiply(b, s);
       }
-      finish(u, part);
+      finish(u, flip);
     }
   }
+  if (p.parts > 1) st::cluster_sync();      // until then its sums are read
 }
 
 template <typename T, int NT, int C, int GROUP>
-int launch(const LinearParams& p, cudaStream_t stream) {
-  constexpr int smem = NT * 8 * (kWarps * C * kTileCols / 2 + 16) * 4 + 2 * kWarps * NT * 8 * kTileRows * 4;
-  static int resident[st::kMaxDevices];
-  int& blocks = resident[st::current_device()];
-  if (blocks == 0) {
+int launch(LinearParams p, cudaStream_t stream) {
+  constexpr int kOuts = NT * 8 * kTileRows, kColumns = kWarps * C * kTileCols;
+  constexpr int smem = NT * 8 * (kColumns / 2 + 16) * 4 + 2 * (kWarps + 1) * kOuts * 4;
+  p.parts = min(kMostParts, (p.cols + kColumns - 1) / kColumns);
+  static int resident[st::kMaxDevices][kMostParts + 1];      // clusters that run at once, by their size
+  int& clusters = resident[st::current_device()][p.parts];
+  if (clusters == 0) {
     if (smem > 48 * 1024) ST_CUDA_CHECK(cudaFuncSetAttribute(linear_kernel<T, NT, C, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = p.parts, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(p.parts * st::sm_count()), cfg.blockDim = dim3(kWarps * 32), cfg.dynamicSmemBytes = smem, cfg.attrs = &attr, cfg.numAttrs = 1;
     int n = 0;
-    ST_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, linear_kernel<T, NT, C, GROUP>, kWarps * 32, smem));
-    blocks = max(1, n) * st::sm_count();
+    ST_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, linear_kernel<T, NT, C, GROUP>, &cfg));
+    clusters = max(1, n);
   }
-  const int grid = min(p.units, blocks);      // as many as run at once
-  const cudaError_t e = st::chained(linear_kernel<T, NT, C, GROUP>, dim3(grid), dim3(kWarps * 32), smem, stream)(
+  const int grid = min(p.units, clusters) * p.parts;
+  const cudaError_t e = st::chained(linear_kernel<T, NT, C, GROUP>, dim3(grid), dim3(kWarps * 32), smem, stream, p.parts)(
       static_cast<const T*>(p.x), p.codes, p.scales, static_cast<const T*>(p.bias), static_cast<const T*>(p.residual), static_cast<T*>(p.y), p);
   return e == cudaSuccess ? ST_OK : st::fail_cuda(e, "int4 linear");
 }
@@ -261,7 +298,9 @@ int dispatch(const LinearParams& p, cudaStream_t stream) {
   return p.chunks <= 2 * kWarps ? by_group<T, 2, 2>(p, stream) : by_group<T, 2, 4>(p, stream);
 }
 
-constexpr int kWideFrom = 17;
+// Whether products go through tcgen05 (int4_wide.cu): from 17 tokens on, and from 9 where the weights are more than 2^24.  us of this kernel and that one, 16 tokens: 2048 x 2048
+// 4.9 and 6.1, 8192 x 2048 8.8 and 9.1, 50304 x 2048 25.8 and 19.8; 8 tokens 3.6 and 5.9, 6.2 and 9.0, 19.8 and 19.7.
+bool is_wide(int tokens, int rows, int cols) { return tokens > 16 || (tokens > 8 && static_cast<long long>(rows) * cols > 1 << 24); }
 
 int aligned(const void* x, long long row, int cols) {
   if ((reinterpret_cast<uintptr_t>(x) & 15) == 0 && row % 8 == 0 && row >= cols) return ST_OK;
@@ -281,7 +320,7 @@ struct StInt4LinearArgs {
 };
 
 // y [tokens, rows] = act(x [tokens, cols] W^T + bias) + residual.  Columns are contiguous, rows the given numbers of elements apart; bias and residual may be
-// null.  From st_int4_wide_from() tokens on x lies on a 16-byte boundary, its rows a multiple of 8 elements apart.  act: 0 none, 1 relu, 2 gelu (tanh form); type of x, bias,
+// null.  Where st_int4_is_wide() x lies on a 16-byte boundary, its rows a multiple of 8 elements apart.  act: 0 none, 1 relu, 2 gelu (tanh form); type of x, bias,
 // residual and y: 0 bf16, 1 fp16.
 ST_API int st_int4_linear(const StInt4LinearArgs* a, void* stream_v) {
   if (a->tokens < 0 || a->rows < 1 || a->cols < 1 || a->rows > 1 << 30 || a->cols > 1 << 30 || (a->group != 32 && a->group != 64 && a->group != 128) || a->act < 0 || a->act > 2)
@@ -290,7 +329,7 @@ ST_API int st_int4_linear(const StInt4LinearArgs* a, void* stream_v) {
   if ((reinterpret_cast<uintptr_t>(a->codes) | reinterpret_cast<uintptr_t>(a->scales)) & 15) return st::fail(ST_ERR_INVALID, "int4: codes and scales must lie on 16-byte boundaries");
   if (a->tokens == 0) return ST_OK;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
-  if (a->tokens >= kWideFrom) {
+  if (is_wide(a->tokens, a->rows, a->cols)) {
     if (const int e = aligned(a->x, a->x_row, a->cols)) return e;
     return wide(WideArgs{a->x, a->codes, a->scales, a->bias, a->residual, a->y, a->x_row, a->residual_row, a->y_row, a->tokens, a->rows, a->cols, a->group, a->act}, a->type,
                 false, stream);
@@ -298,7 +337,7 @@ ST_API int st_int4_linear(const StInt4LinearArgs* a, void* stream_v) {
   const LinearParams p{a->x, static_cast<const uint8_t*>(a->codes), static_cast<const __nv_bfloat16*>(a->scales), a->bias, a->residual, a->y, a->x_row, a->residual_row,
                        a->y_row, a->tokens, a->rows, a->cols, (a->cols + a->group - 1) / a->group, (a->cols + kTileCols - 1) / kTileCols,
                        (a->rows + kTileRows - 1) / kTileRows, a->group, a->act,
-                       (reinterpret_cast<uintptr_t>(a->x) & 15) == 0 && a->x_row % 8 == 0};
+                       (reinterpret_cast<uintptr_t>(a->x) & 15) == 0 && a->x_row % 8 == 0, 1};
   return a->type == 0 ? dispatch<__nv_bfloat16>(p, stream) : dispatch<__half>(p, stream);
 }
 
@@ -314,5 +353,5 @@ ST_API int st_int4_linear_grad(const void* dy, const void* codes, const void* sc
   return wide(WideArgs{dy, codes, scales, nullptr, nullptr, dx, dy_row, 0, dx_row, tokens, rows, cols, group, 0}, type, true, reinterpret_cast<cudaStream_t>(stream_v));
 }
 
-// From how many rows of x products go through tcgen05 (x then as dy above).
-ST_API int st_int4_wide_from() { return kWideFrom; }
+// Whether a product of these sizes goes through tcgen05 (x then as dy above).
+ST_API int st_int4_is_wide(int tokens, int rows, int cols) { return is_wide(tokens, rows, cols); }

@@ -14,7 +14,6 @@ CPU tensors use a plain PyTorch statement of the same (also the test oracle).  T
 """
 from __future__ import annotations
 
-import functools
 import struct
 from typing import Optional
 
@@ -182,11 +181,6 @@ def dequantize(w: Weights, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
 
 
 # ---- products -------------------------------------------------------------------------------------------------------------------
-@functools.cache
-def _wide_from() -> int:
-    return native.lib().st_int4_wide_from()
-
-
 def _boundaries(x2: torch.Tensor) -> torch.Tensor:
     """``x2``, or a copy of it, with every row on a 16-byte boundary, as tiled copies need them."""
     rows, cols = x2.shape
@@ -206,7 +200,7 @@ def _product(x2, w, bias, act, residual2):
     y = x2.new_empty((rows, n))
     if rows == 0:
         return y
-    if rows >= _wide_from():
+    if rows > 16 or rows > 8 and native.entry("st_int4_is_wide", "iii")(rows, n, cols):
         x2 = _boundaries(x2)
     x_row, step = x2.stride()
     if step != 1 and cols > 1:
