@@ -661,20 +661,32 @@ ST_API int st_token_scores(const StTokenScoresArgs* a, void* stream_v) {
   return st::fail(ST_ERR_INVALID, "scores: unknown type");
 }
 
+struct StTokenScoresGradArgs {
+  const void* logits;
+  const long long* targets;
+  const void* stats;
+  const float* entropy;
+  const long long* top_ids;
+  const float* g_logprob;
+  const float* g_entropy;
+  const float* g_top;
+  void* out;
+  long long rows, row, out_row;
+  int vocab, top, type;
+};
+
 // Gradient of the logits from those of log probability, entropy and the likeliest tokens' log probabilities (each may be null: 0).
-ST_API int st_token_scores_grad(const void* logits, const long long* targets, const void* stats, const float* entropy, const long long* top_ids, const float* g_logprob,
-                                const float* g_entropy, const float* g_top, void* out, long long rows, long long row, long long out_row, int vocab, int top, int type,
-                                void* stream_v) {
-  if (rows < 0 || vocab < 1 || vocab > 1 << 30 || top < 0 || top > kMostTop || top > vocab) return st::fail(ST_ERR_INVALID, "scores: sizes out of range");
-  if (reinterpret_cast<uintptr_t>(stats) & 7) return st::fail(ST_ERR_INVALID, "scores: stats must lie on an 8-byte boundary");
-  if (rows == 0) return ST_OK;
-  const GradParams p{row, out_row, rows, vocab, top, 1};
+ST_API int st_token_scores_grad(const StTokenScoresGradArgs* a, void* stream_v) {
+  if (a->rows < 0 || a->vocab < 1 || a->vocab > 1 << 30 || a->top < 0 || a->top > kMostTop || a->top > a->vocab) return st::fail(ST_ERR_INVALID, "scores: sizes out of range");
+  if (reinterpret_cast<uintptr_t>(a->stats) & 7) return st::fail(ST_ERR_INVALID, "scores: stats must lie on an 8-byte boundary");
+  if (a->rows == 0) return ST_OK;
+  const GradParams p{a->row, a->out_row, a->rows, a->vocab, a->top, 1};
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
-  const float2* ms = static_cast<const float2*>(stats);
-  switch (type) {
-    case 0: return backward<__nv_bfloat16>(logits, targets, ms, entropy, top_ids, g_logprob, g_entropy, g_top, out, p, stream);
-    case 1: return backward<__half>(logits, targets, ms, entropy, top_ids, g_logprob, g_entropy, g_top, out, p, stream);
-    case 2: return backward<float>(logits, targets, ms, entropy, top_ids, g_logprob, g_entropy, g_top, out, p, stream);
+  const float2* ms = static_cast<const float2*>(a->stats);
+  switch (a->type) {
+    case 0: return backward<__nv_bfloat16>(a->logits, a->targets, ms, a->entropy, a->top_ids, a->g_logprob, a->g_entropy, a->g_top, a->out, p, stream);
+    case 1: return backward<__half>(a->logits, a->targets, ms, a->entropy, a->top_ids, a->g_logprob, a->g_entropy, a->g_top, a->out, p, stream);
+    case 2: return backward<float>(a->logits, a->targets, ms, a->entropy, a->top_ids, a->g_logprob, a->g_entropy, a->g_top, a->out, p, stream);
   }
   return st::fail(ST_ERR_INVALID, "scores: unknown type");
 }

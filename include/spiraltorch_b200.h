@@ -249,6 +249,21 @@ typedef struct StTokenScoresArgs {
   int vocab, top, type;
 } StTokenScoresArgs;
 
+/* csrc/elementwise/scores.cu */
+typedef struct StTokenScoresGradArgs {
+  const void* logits;
+  const long long* targets;
+  const void* stats;
+  const float* entropy;
+  const long long* top_ids;
+  const float* g_logprob;
+  const float* g_entropy;
+  const float* g_top;
+  void* out;
+  long long rows, row, out_row;
+  int vocab, top, type;
+} StTokenScoresGradArgs;
+
 /* ---- libst_b200.so ---------------------------------------------------------------- */
 int st_abi_version();   /* csrc/runtime/runtime.cu */
 int st_act_bwd(const void* x, const void* dy, void* dx, long long n, int relu, void* stream_v);   /* csrc/elementwise/elementwise.cu */
@@ -369,7 +384,7 @@ int st_specmul(const float* x_reim, float* y_reim, long long rows, int cols, flo
 int st_sumsq(const void* x, int is_bf16, long long n, float* out, void* stream_v);   /* csrc/optim/optim.cu */
 int st_temporal_render(const float* voxels, const float* harmonics, const float* decay, float* out, long long n_voxels, int channels, int frames, float sample_rate_hz, void* stream_v);   /* csrc/spectral/spectral.cu */
 int st_token_scores(const StTokenScoresArgs* a, void* stream_v);   /* csrc/elementwise/scores.cu */
-int st_token_scores_grad(const void* logits, const long long* targets, const void* stats, const float* entropy, const long long* top_ids, const float* g_logprob, const float* g_entropy, const float* g_top, void* out, long long rows, long long row, long long out_row, int vocab, int top, int type, void* stream_v);   /* csrc/elementwise/scores.cu */
+int st_token_scores_grad(const StTokenScoresGradArgs* a, void* stream_v);   /* csrc/elementwise/scores.cu */
 int st_wave_gate_bwd(const float* z, const float* dy, float* dz, int B, int H, void* stream);   /* csrc/recurrent/recurrent.cu */
 int st_wave_gate_fwd(const float* z, float* y, int B, int H, void* stream);   /* csrc/recurrent/recurrent.cu */
 

@@ -224,38 +224,58 @@ def _product(x2, w, bias, act, residual2):
 
 def _input_gradient(dy2, w):
     """``[rows, out]`` to ``[rows, in]``: ``dy W``."""
-    if not native.use_native(dy2):
+    global launch_count
+    if not dy2.is_cuda:
         t = torch.float64 if dy2.dtype == torch.float64 else torch.float32
         return (dy2.to(t) @ dequantize_reference(w, t)).to(dy2.dtype)
-    global launch_count
     dy2 = _boundaries(dy2)
     index = native.require_cuda("int4.linear", dy2, w.codes, w.scales)
-    rows = dy2.shape[0]
-    dx = torch.empty((rows, w.in_features), dtype=dy2.dtype, device=dy2.device)
+    rows, k = dy2.shape[0], w.in_features
+    dx = dy2.new_empty((rows, k))
     if rows == 0:
         return dx
     with native.on_device(index):
-        st = native.entry("st_int4_linear_grad", "ppppiiiqqiip")(dy2.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), dx.data_ptr(), rows, w.out_features,
-                                                               w.in_features, dy2.stride(0), w.in_features, w.group, _TYPES[dy2.dtype], native.raw_stream(index))
-    native.check(st, "st_int4_linear_grad")
+        st = native.entry("st_int4_linear_grad", "ppppiiiqqiip")(dy2.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), dx.data_ptr(), rows, w.out_features, k,
+                                                               dy2.stride(0), k, w.group, _TYPES[dy2.dtype], native.raw_stream(index))
+    if st:
+        native.check(st, "st_int4_linear_grad")
     launch_count += 1
     return dx
+
+
+class _InputGradientFn(torch.autograd.Function):
+    """``dy W`` where a graph of the gradient is asked for: linear in ``dy`` as the product is in ``x``."""
+
+    @staticmethod
+    def forward(ctx, dy2, w):
+        ctx.w = w
+        return _input_gradient(dy2, w)
+
+    @staticmethod
+    def backward(ctx, d):
+        return linear(d, ctx.w), None
 
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, bias, residual, w):
-        ctx.w, ctx.x_shape = w, x.shape
+        ctx.w = w
+        if x.dim() == 2:
+            return _product(x, w, bias, None, residual)
         y = _product(x.reshape(-1, x.shape[-1]), w, bias, None, None if residual is None else residual.reshape(-1, w.out_features))
         return y.view(*x.shape[:-1], w.out_features)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         need_x, need_bias, need_residual, _ = ctx.needs_input_grad
-        dy2 = dy.reshape(-1, ctx.w.out_features)
-        dx = _input_gradient(dy2, ctx.w).view(ctx.x_shape) if need_x else None
-        db = dy2.sum(0, dtype=torch.float64 if dy.dtype == torch.float64 else torch.float32).to(dy.dtype) if need_bias else None
+        w, dx, db = ctx.w, None, None
+        dy2 = dy if dy.dim() == 2 else dy.reshape(-1, w.out_features)
+        if need_x:
+            dx = _InputGradientFn.apply(dy2, w) if torch.is_grad_enabled() and dy.requires_grad else _input_gradient(dy2, w)
+            if dy.dim() != 2:
+                dx = dx.view(*dy.shape[:-1], w.in_features)
+        if need_bias:
+            db = dy2.sum(0, dtype=torch.float64 if dy.dtype == torch.float64 else torch.float32).to(dy.dtype)
         return dx, db, dy if need_residual else None, None
 
 

@@ -18,6 +18,7 @@ MOST_TOP = 32
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 # StTokenScoresArgs of csrc/elementwise/scores.cu, in one call: a ctypes object for each of a dozen arguments costs as much as the launch
 _pack_args = struct.Struct("@7P2q3i").pack
+_pack_grad = struct.Struct("@9P3q3i").pack      # StTokenScoresGradArgs
 
 
 class TokenScores(NamedTuple):
@@ -98,38 +99,58 @@ def _forward(logits, targets, top, keep):
     return TokenScores(logprob, entropy, ids, top_logprobs), stats
 
 
+def _gradient(logits, targets, stats, entropy, ids, g_logprob, g_entropy, g_top):
+    global launch_count
+    if not logits.is_cuda:
+        return _gradient_reference(logits, targets, ids, g_logprob, g_entropy, g_top)
+    rows, vocab = logits.shape
+    gl, ge, gt = (g if g is None or (g.dtype is torch.float32 and g.is_contiguous()) else g.to(torch.float32).contiguous() for g in (g_logprob, g_entropy, g_top))
+    # rows as far apart as the logits' where that is not much more than they hold: both are then at the same place between 16-byte boundaries
+    stride = logits.stride(0)
+    room = stride if vocab <= stride <= vocab + vocab // 8 else vocab
+    out = logits.new_empty((rows, room))
+    if room != vocab:
+        out = out[:, :vocab]
+    if rows == 0:
+        return out
+    index = native.require_cuda("token_scores", logits, targets, gl, ge, gt)
+    args = _pack_grad(logits.data_ptr(), targets.data_ptr(), stats.data_ptr(), entropy.data_ptr(), ids.data_ptr(), native.address(gl), native.address(ge),
+                      native.address(gt), out.data_ptr(), rows, stride, room, vocab, 0 if gt is None else ids.shape[1], _TYPES[logits.dtype])
+    with native.on_device(index):
+        st = native.entry("st_token_scores_grad", "sp")(args, native.raw_stream(index))
+    if st:
+        native.check(st, "st_token_scores_grad")
+    launch_count += 1
+    return out
+
+
+class _GradientFn(torch.autograd.Function):
+    """The gradient where a graph of it is asked for: there is none."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _gradient(*args)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("token_scores: not differentiable twice")
+
+
 class _TokenScoresFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top):
         scores, stats = _forward(logits, targets, top, True)
-        ctx.save_for_backward(logits, targets, stats, scores.entropy.detach(), scores.top_ids)
+        ctx.save_for_backward(logits, targets, stats, scores.entropy, scores.top_ids)
         ctx.mark_non_differentiable(scores.top_ids)
         ctx.set_materialize_grads(False)
-        return tuple(scores)
+        return scores.logprob, scores.entropy, scores.top_ids, scores.top_logprobs
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_logprob, g_entropy, _, g_top):
-        global launch_count
-        logits, targets, stats, entropy, ids = ctx.saved_tensors
         if g_logprob is None and g_entropy is None and g_top is None:
             return None, None, None
-        if not native.use_native(logits):
-            return _gradient_reference(logits, targets, ids, g_logprob, g_entropy, g_top), None, None
-        rows, vocab = logits.shape
-        gl, ge, gt = (None if g is None else g.to(torch.float32).contiguous() for g in (g_logprob, g_entropy, g_top))
-        # rows as far apart as the logits' where that is not much more than they hold: both are then at the same place between 16-byte boundaries
-        stride = logits.stride(0)
-        room = stride if vocab <= stride <= vocab + vocab // 8 else vocab
-        out = torch.empty((rows, room), dtype=logits.dtype, device=logits.device)[:, :vocab]
-        index = native.require_cuda("token_scores", logits, targets, gl, ge, gt)
-        with native.on_device(index):
-            st = native.entry("st_token_scores_grad", "pppppppppqqqiiip")(
-                logits.data_ptr(), targets.data_ptr(), stats.data_ptr(), entropy.data_ptr(), ids.data_ptr(), native.address(gl), native.address(ge), native.address(gt),
-                out.data_ptr(), rows, logits.stride(0), room, vocab, 0 if gt is None else ids.shape[1], _TYPES[logits.dtype], native.raw_stream(index))
-        native.check(st, "st_token_scores_grad")
-        launch_count += 1
-        return out, None, None
+        f = _GradientFn.apply if torch.is_grad_enabled() else _gradient
+        return f(*ctx.saved_tensors, g_logprob, g_entropy, g_top), None, None
 
 
 def token_scores(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0) -> TokenScores:

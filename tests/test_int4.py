@@ -119,6 +119,7 @@ def test_linear_statement_and_gradients():
     dx, db, dr = torch.autograd.grad(y, (x, b, r), dy)
     assert torch.allclose(dx, dy @ w, atol=1e-12) and torch.allclose(db, dy.sum((0, 1)), atol=1e-12) and torch.equal(dr, dy)
     assert torch.autograd.gradcheck(lambda x, b, r: int4.linear(x, held, b, residual=r), (x, b, r))
+    assert torch.autograd.gradgradcheck(lambda x: int4.linear(x, held) ** 2, (x,))
     with torch.no_grad():
         assert torch.equal(int4.linear(x, held, act="relu"), torch.relu(x @ w.T))
         assert torch.allclose(int4.linear(x, held, b, act="gelu", residual=r), torch.nn.functional.gelu(x @ w.T + b, approximate="tanh") + r, atol=1e-12)

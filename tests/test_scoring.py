@@ -348,3 +348,12 @@ def test_generated_tokens_with_scores():
 @GPU
 def test_scores_of_a_model_on_the_gpu():
     _check_model_scores(_model("cuda", torch.bfloat16))
+
+
+def test_gradients_are_not_differentiated_twice():
+    x, t = _logits(3, 11, torch.float32)
+    x.requires_grad_(True)
+    g = torch.autograd.grad(scoring.token_scores(x, t).logprob.sum(), x, create_graph=True)[0]
+    assert torch.equal(g, torch.autograd.grad(scoring.token_scores(x, t).logprob.sum(), x)[0])
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(g.pow(2).sum(), x)
