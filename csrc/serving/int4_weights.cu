@@ -19,7 +19,7 @@ namespace {
 using namespace st4;
 using st::chain_begin;
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 2;      // few: small matrices on as many SMs as they fill
 constexpr int kCols = 128;      // of a warp's block
 constexpr float kLeast = 9.5367431640625e-07f, kLargest = 7680.0f;      // 2^-20, 1.875 * 2^12
 
@@ -66,18 +66,21 @@ template <> __device__ __forceinline__ void extremes(const Vec<__half, 8>& v, fl
 }
 
 // 8 codes plus 8, four bits each: w / s to the nearest, ties to even, within -8..7.
-// w * (1 / s) may lie up to 2^-20 beside the quotient.  A quotient of a 16-bit w that is no tie is at least 2^-16 from one (w is at most 11 bits, s 4): rounded to multiples of
-// 2^-18 first, ties are ties again and nothing else changes sides.  For fp32 the remainder, which fmaf gives exactly, says on which side of the border w is.
+// w * (1 / s), of an approximate reciprocal, may lie up to 2^-19 beside the quotient.  A quotient of a 16-bit w that is no tie is at least 2^-16 from one (w is at most 11 bits, s 4):
+// rounded to multiples of 2^-17 first, ties are ties again and nothing else changes sides.  For fp32 the remainder, which fmaf gives exactly, says on which side of
+// the border w is.
 template <typename T>
 __device__ __forceinline__ uint32_t codes_of(const Vec<T, 8>& v, float s) {
-  const float inv = 1.0f / s;
+  const float inv = st::rcp_approx(s);
   uint32_t packed = 0;
   if constexpr (sizeof(T) == 2) {
+    const bool within = fabsf(s) < kLargest;      // nothing lies below -8.5 steps, which is -8, unless the scale was bounded
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       float2 t = st::mul2(make_float2(to_float(v.v[e]), to_float(v.v[e + 1])), st::splat2(inv));
-      t = make_float2(fminf(fmaxf(t.x, -8.0f), 7.0f), fminf(fmaxf(t.y, -8.0f), 7.0f));      // NaN: -8, which the scale covers
-      t = st::add2(st::add2(t, st::splat2(48.0f)), st::splat2(-48.0f));
+      if (!within) t = make_float2(fmaxf(t.x, -8.0f), fmaxf(t.y, -8.0f));                 // and NaN: -8, which the scale covers
+      t = make_float2(fminf(t.x, 7.0f), fminf(t.y, 7.0f));
+      t = st::add2(st::add2(t, st::splat2(96.0f)), st::splat2(-96.0f));
       t = st::add2(t, st::splat2(12582912.0f + 8.0f));                                    // 1.5 2^23: whole numbers in the low bits
       packed += (__float_as_uint(t.x) << (4 * e)) + (__float_as_uint(t.y) << (4 * e + 4));
     }
@@ -145,9 +148,8 @@ __global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const T* w, uint8
     uint32_t out[4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {      // byte t of 8 codes: columns 2 t and 2 t + 1 of them; of the 4 bytes the low nibbles, then the high ones
-      uint32_t four = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) four |= (word[warp][g + 8 * (e & 1)][8 * c + 2 * s + (e >> 1)] >> (8 * t) & 0xFFu) << (8 * e);
+      const uint8_t* from = reinterpret_cast<const uint8_t*>(&word[warp][g][8 * c + 2 * s]) + t;
+      const uint32_t four = __byte_perm(__byte_perm(from[0], from[8 * 17 * 4], 0x0040), __byte_perm(from[4], from[8 * 17 * 4 + 4], 0x0040), 0x5410);
       const uint32_t low = four & 0x0F0F0F0Fu, high = four >> 4 & 0x0F0F0F0Fu;
       out[s] = __byte_perm(low | low >> 4, high | high >> 4, 0x6420);
     }
@@ -259,34 +261,42 @@ int dequantize(const uint8_t* codes, const __nv_bfloat16* scales, void* w, const
 }
 }  // namespace
 
+struct StInt4WeightsArgs {
+  void* w;
+  void* codes;
+  void* scales;
+  long long stride;
+  int rows, cols, group, type;
+};
+
 // w [rows, cols] (type 0 bf16, 1 fp16, 2 fp32; rows `stride` elements apart, columns contiguous) to codes and scales in the layout of int4.cuh; group: 32, 64 or 128.
-ST_API int st_int4_quantize(const void* w, void* codes, void* scales, int rows, int cols, long long stride, int group, int type, void* stream_v) {
-  WeightsParams p{stride, rows, cols, 0, 0, 0};
+ST_API int st_int4_quantize(const StInt4WeightsArgs* a, void* stream_v) {
+  WeightsParams p{a->stride, a->rows, a->cols, 0, 0, 0};
   unsigned grid;
-  if (const int e = plan(p, grid, group, codes, scales)) return e;
-  uint8_t* c = static_cast<uint8_t*>(codes);
-  __nv_bfloat16* s = static_cast<__nv_bfloat16*>(scales);
+  if (const int e = plan(p, grid, a->group, a->codes, a->scales)) return e;
+  uint8_t* c = static_cast<uint8_t*>(a->codes);
+  __nv_bfloat16* s = static_cast<__nv_bfloat16*>(a->scales);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
-  switch (type) {
-    case 0: return quantize<__nv_bfloat16>(w, c, s, p, grid, group, stream);
-    case 1: return quantize<__half>(w, c, s, p, grid, group, stream);
-    case 2: return quantize<float>(w, c, s, p, grid, group, stream);
+  switch (a->type) {
+    case 0: return quantize<__nv_bfloat16>(a->w, c, s, p, grid, a->group, stream);
+    case 1: return quantize<__half>(a->w, c, s, p, grid, a->group, stream);
+    case 2: return quantize<float>(a->w, c, s, p, grid, a->group, stream);
   }
   return st::fail(ST_ERR_INVALID, "int4: unknown type");
 }
 
 // The weights that codes and scales stand for, into w.
-ST_API int st_int4_dequantize(const void* codes, const void* scales, void* w, int rows, int cols, long long stride, int group, int type, void* stream_v) {
-  WeightsParams p{stride, rows, cols, 0, 0, 0};
+ST_API int st_int4_dequantize(const StInt4WeightsArgs* a, void* stream_v) {
+  WeightsParams p{a->stride, a->rows, a->cols, 0, 0, 0};
   unsigned grid;
-  if (const int e = plan(p, grid, group, codes, scales)) return e;
-  const uint8_t* c = static_cast<const uint8_t*>(codes);
-  const __nv_bfloat16* s = static_cast<const __nv_bfloat16*>(scales);
+  if (const int e = plan(p, grid, a->group, a->codes, a->scales)) return e;
+  const uint8_t* c = static_cast<const uint8_t*>(a->codes);
+  const __nv_bfloat16* s = static_cast<const __nv_bfloat16*>(a->scales);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
-  switch (type) {
-    case 0: return dequantize<__nv_bfloat16>(c, s, w, p, grid, group, stream);
-    case 1: return dequantize<__half>(c, s, w, p, grid, group, stream);
-    case 2: return dequantize<float>(c, s, w, p, grid, group, stream);
+  switch (a->type) {
+    case 0: return dequantize<__nv_bfloat16>(c, s, a->w, p, grid, a->group, stream);
+    case 1: return dequantize<__half>(c, s, a->w, p, grid, a->group, stream);
+    case 2: return dequantize<float>(c, s, a->w, p, grid, a->group, stream);
   }
   return st::fail(ST_ERR_INVALID, "int4: unknown type");
 }

@@ -215,6 +215,15 @@ typedef struct StInt4LinearArgs {
   int tokens, rows, cols, group, act, type;
 } StInt4LinearArgs;
 
+/* csrc/serving/int4_weights.cu */
+typedef struct StInt4WeightsArgs {
+  void* w;
+  void* codes;
+  void* scales;
+  long long stride;
+  int rows, cols, group, type;
+} StInt4WeightsArgs;
+
 /* csrc/vision/vision.cu */
 typedef struct StPreprocessArgs {
   int B, C, src_h, src_w, resize_h, resize_w, out_h, out_w, crop_y, crop_x, flip, do_jitter;
@@ -315,11 +324,11 @@ int st_im2col3x3_planes(const void* x, void* col, const void* weights, void* pad
 int st_im2col3x3_small(const void* x, void* col, int N, int H, int W, int C, int Kpad, void* stream_v);   /* csrc/conv/conv.cu */
 int st_info_nce_fwd(const StInfoNceArgs* a, void* stream_v);   /* csrc/comm/contrastive.cu */
 int st_info_nce_grad(const float* logits, const float* row_lse, const float* coef, void* dl, void* dl_t, int R, int C, int target_offset, void* stream_v);   /* csrc/comm/contrastive.cu */
-int st_int4_dequantize(const void* codes, const void* scales, void* w, int rows, int cols, long long stride, int group, int type, void* stream_v);   /* csrc/serving/int4_weights.cu */
+int st_int4_dequantize(const StInt4WeightsArgs* a, void* stream_v);   /* csrc/serving/int4_weights.cu */
 int st_int4_is_wide(int tokens, int rows, int cols);   /* csrc/serving/int4_linear.cu */
 int st_int4_linear(const StInt4LinearArgs* a, void* stream_v);   /* csrc/serving/int4_linear.cu */
 int st_int4_linear_grad(const void* dy, const void* codes, const void* scales, void* dx, int tokens, int rows, int cols, long long dy_row, long long dx_row, int group, int type, void* stream_v);   /* csrc/serving/int4_linear.cu */
-int st_int4_quantize(const void* w, void* codes, void* scales, int rows, int cols, long long stride, int group, int type, void* stream_v);   /* csrc/serving/int4_weights.cu */
+int st_int4_quantize(const StInt4WeightsArgs* a, void* stream_v);   /* csrc/serving/int4_weights.cu */
 const char* st_last_error();   /* csrc/runtime/runtime.cu */
 int st_lstm_gate_bwd(const float* act, const float* c_prev, const float* c, const float* dh, const float* dc_next, float* dz, float* dc_prev, int B, int H, void* stream);   /* csrc/recurrent/recurrent.cu */
 int st_lstm_gate_fwd(const float* z, const float* c_prev, float* c_out, float* h_out, float* act, int B, int H, void* stream);   /* csrc/recurrent/recurrent.cu */

@@ -31,6 +31,7 @@ _ACTS = {None: 0, "relu": 1, "gelu": 2}
 
 # StInt4LinearArgs of csrc/serving/int4_linear.cu, in one call: a ctypes object for each of 16 arguments costs as much as the launch
 _pack_args = struct.Struct("@6P3q6i").pack
+_pack_weights = struct.Struct("@3Pq4i").pack      # StInt4WeightsArgs of int4_weights.cu
 
 
 class Weights:
@@ -133,51 +134,51 @@ def linear_reference(x, weight, bias=None, act=None, residual=None):
 def quantize(weight: torch.Tensor, group: int = 64, *, out: Optional[Weights] = None) -> Weights:
     """``weight`` ``[out, in]`` in bf16, fp16 or fp32 (rows may be strided) in four bits; ``out``: written to instead of new memory, as after
     an update of weights that a captured step holds."""
-    global launch_count
-    if weight.dim() != 2 or weight.dtype not in _TYPES and not (weight.dtype == torch.float64 and not weight.is_cuda):
+    on_cuda = weight.is_cuda
+    if weight.dim() != 2 or weight.dtype not in _TYPES and not (weight.dtype == torch.float64 and not on_cuda):
         raise ValueError(f"int4.quantize: a bf16, fp16 or fp32 matrix, got {weight.dtype} {tuple(weight.shape)}")
     if group not in GROUPS:
         raise ValueError(f"int4.quantize: groups of {GROUPS} inputs, got {group}")
     n, k = weight.shape
     if out is None:
         out = Weights.allocate(n, k, group, weight.device)
+    elif (out.out_features, out.in_features, out.group) != (n, k, group):
+        raise ValueError(f"int4.quantize: a {n} x {k} matrix in groups of {group} into weights of {out.out_features} x {out.in_features} in groups of {out.group}")
     else:
-        if (out.out_features, out.in_features, out.group) != (n, k, group):
-            raise ValueError(f"int4.quantize: a {n} x {k} matrix in groups of {group} into weights of {out.out_features} x {out.in_features} in groups of {out.group}")
         native.same_device("int4.quantize", weight, out.codes)
-    if not weight.is_cuda:
+    if not on_cuda:
         q, s = quantize_reference(weight.detach(), group)
         out.codes.copy_(_tiles(q))
         s = torch.nn.functional.pad(s, (0, 0, 0, -n % 16), value=LEAST_SCALE)
         out.scales.copy_(s.view(-1, 2, 8, s.shape[1]).permute(0, 3, 2, 1).flatten(-2))
         return out
-    if weight.stride(1) != 1 and k > 1:
-        weight = weight.contiguous()
-    index = native.require_cuda("int4.quantize", weight, out.codes, out.scales)
-    with native.on_device(index):
-        st = native.entry("st_int4_quantize", "pppiiqiip")(weight.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), n, k, weight.stride(0), group,
-                                                         _TYPES[weight.dtype], native.raw_stream(index))
-    if st:
-        native.check(st, "st_int4_quantize")
-    launch_count += 1
+    stride, step = weight.stride()
+    if step != 1 and k > 1:
+        weight, stride = weight.contiguous(), k
+    _weights_call("st_int4_quantize", weight, stride, out)
     return out
 
 
 def dequantize(w: Weights, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``[out, in]`` in bf16, fp16 or fp32: the same numbers in each."""
-    global launch_count
-    if not native.use_native(w.codes):
+    if not w.codes.is_cuda:
         return dequantize_reference(w, dtype)
     if dtype not in _TYPES:
         raise ValueError(f"int4.dequantize: bf16, fp16 or fp32, got {dtype}")
-    index = native.require_cuda("int4.dequantize", w.codes, w.scales)
-    y = torch.empty((w.out_features, w.in_features), dtype=dtype, device=w.codes.device)
-    with native.on_device(index):
-        st = native.entry("st_int4_dequantize", "pppiiqiip")(w.codes.data_ptr(), w.scales.data_ptr(), y.data_ptr(), w.out_features, w.in_features, w.in_features,
-                                                           w.group, _TYPES[dtype], native.raw_stream(index))
-    native.check(st, "st_int4_dequantize")
-    launch_count += 1
+    y = w.codes.new_empty((w.out_features, w.in_features), dtype=dtype)
+    _weights_call("st_int4_dequantize", y, w.in_features, w)
     return y
+
+
+def _weights_call(name: str, matrix: torch.Tensor, stride: int, w: Weights) -> None:
+    global launch_count
+    index = matrix.get_device()
+    args = _pack_weights(matrix.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), stride, w.out_features, w.in_features, w.group, _TYPES[matrix.dtype])
+    with native.on_device(index):
+        st = native.entry(name, "sp")(args, native.raw_stream(index))
+    if st:
+        native.check(st, name)
+    launch_count += 1
 
 
 # ---- products -------------------------------------------------------------------------------------------------------------------
