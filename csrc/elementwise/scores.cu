@@ -19,16 +19,16 @@ constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kMostTop = 32;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f, kLowest = -3.402823466e38f;
 constexpr float kMargin = 4.0f;       // how far an element may lie above a thread's m before that follows it: e^4 rows of S are far from overflow
-// y is one multiplication and addition, x log2 e - (m log2 e), the second rounded once for all of a row; that rounding must stay below 1, so |m| below kUsual = 2^20.
-// Elements below the least usual one, -inf among them, count as that, which keeps 2^y y from being 0 times infinity.  Rows whose m is not usual are summed
-// again with care: y = (x - m) log2 e.
+// y is one multiplication and addition, x log2 e - (m log2 e), the second rounded once for all of a block; that rounding must stay below 1, so |m| below kUsual = 2^20, and
+// it is known, so that it is taken out of the block's sums.  Elements below the least usual one, -inf among them, count as that, which keeps 2^y y from being 0
+// times infinity.  Where m is not usual the sums are formed again with care: y = (x - m) log2 e.
 constexpr float kUsual = 1048576.0f;
 constexpr float kFar = -1.0e4f;       // 2^kFar is 0
 template <typename T> constexpr float kLeast = -kUsual;
 template <> constexpr float kLeast<__half> = -65504.0f;
 template <typename T> __device__ __forceinline__ bool is_usual(float m) { return m > 0.9f * kLeast<T> && m < kUsual; }      // and what counts as the least is nothing beside it
 __device__ __forceinline__ float scaled(float m) { return __fmul_rn(m, kLog2e); }
-__device__ __forceinline__ float exponent(float x, float m, bool usual) { return usual ? fmaf(x, kLog2e, -scaled(m)) : (x - m) * kLog2e; }
+__device__ __forceinline__ float off_by(float m) { return -fmaf(m, kLog2e, -scaled(m)); }      // what is added to x log2 e - scaled(m) for (x - m) log2 e
 
 struct ScoreParams {
   long long row, rows;      // elements between rows
@@ -123,8 +123,8 @@ struct Sums {
     T = f > 0.0f ? f * fmaf(S, y, T) : f * S;           // f = 0: what was seen counts for nothing, and S y may be infinite
     S *= f;
   }
-  __device__ __forceinline__ void move(float to) {
-    shift(to == m ? 0.0f : fabsf(m) < kUsual + 1.0f && fabsf(to) < kUsual + 1.0f ? scaled(m) - scaled(to) : (m - to) * kLog2e);
+  __device__ __forceinline__ void move(float to, bool usual) {
+    shift(to == m ? 0.0f : usual ? scaled(m) - scaled(to) : (m - to) * kLog2e);
     m = to;
   }
   __device__ __forceinline__ void add(float x) {        // with care
@@ -133,11 +133,11 @@ struct Sums {
     S += e;
     T = fmaf(e, fmaxf(y, kFar), T);
   }
-  __device__ __forceinline__ void join(float m2, float S2, float T2) {
+  __device__ __forceinline__ void join(float m2, float S2, float T2) {      // with care
     Sums o;
     o.m = m2, o.S = S2, o.T = T2;
-    if (m2 > m) move(m2);
-    else o.move(m);
+    if (m2 > m) move(m2, false);
+    else o.move(m, false);
     S += o.S;
     T += o.T;
   }
@@ -166,10 +166,10 @@ struct PairSums {
   }
 };
 // Sums of a warp's lanes, or of the first `lanes` (a power of two) of them, in the same for all of these: the largest m first, then one shift each.
-__device__ __forceinline__ void join_lanes(Sums& s, int lanes) {
+__device__ __forceinline__ void join_lanes(Sums& s, int lanes, bool usual) {
   float m = s.m;
   for (int o = lanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  s.move(m);
+  s.move(m, usual);
   for (int o = lanes / 2; o > 0; o >>= 1) {
     s.S += __shfl_xor_sync(0xffffffffu, s.S, o);
     s.T += __shfl_xor_sync(0xffffffffu, s.T, o);
@@ -287,15 +287,15 @@ __device__ __noinline__ void select_carefully(Candidates<W>& c, const T* x, int 
 
 // The sums of all of a row's threads, in all of them.
 template <int W>
-__device__ __forceinline__ void join_group(Candidates<W>& c, Sums& s, int warp, int lane) {
-  join_lanes(s, 32);
+__device__ __forceinline__ void join_group(Candidates<W>& c, Sums& s, int warp, int lane, bool usual) {
+  join_lanes(s, 32, usual);
   if (W == 1) return;
   if (lane == 0) c.sums[warp][0] = s.m, c.sums[warp][1] = s.S, c.sums[warp][2] = s.T;
   sync<W>();
   if (warp == 0) {
     const int i = lane & (W - 1);
     s.m = c.sums[i][0], s.S = c.sums[i][1], s.T = c.sums[i][2];
-    join_lanes(s, W);
+    join_lanes(s, W, usual);
     if (lane == 0) c.total[0] = s.m, c.total[1] = s.S, c.total[2] = s.T;
   }
   sync<W>();
@@ -400,14 +400,16 @@ __global__ void __launch_bounds__(kThreads) scores_kernel(const T* logits, const
   }
 
   // sums of the row (part): in every thread
-  join_group(c, s, warp, lane);
-  if (!is_usual<T>(s.m) && s.S == s.S) {
+  join_group(c, s, warp, lane, true);
+  if (is_usual<T>(s.m)) {
+    s.shift(off_by(s.m));
+  } else if (s.S == s.S) {
     s = Sums();
     for (int v = v0 + tid; v < v1; v += kGroup)
       for (int k = 0; k < N; ++k) s.add(to_float(x[head + v * N + k]));
     if (has_single) s.add(single);
     sync<W>();
-    join_group(c, s, warp, lane);
+    join_group(c, s, warp, lane, false);
   }
   if (TOP) {
     sync<W>();
@@ -465,11 +467,11 @@ __global__ void __launch_bounds__(kThreads) scores_kernel(const T* logits, const
   }
 
   // an empty row, all -inf: no probability anywhere
-  const bool empty = s.S == 0.0f, usual = is_usual<T>(s.m);
+  const bool empty = s.S == 0.0f;
   const float log_S = empty ? INFINITY : log2f(s.S), m = empty ? 0.0f : s.m;
   const auto log_p = [&](float v) {
-    const float y = exponent(v, m, usual);
-    return y == -INFINITY ? v - m - log_S * kLn2 : (y - log_S) * kLn2;      // v log2 e may be infinite where v is not
+    const float d = v - m;      // d log2 e may be infinite where d is not
+    return fabsf(d) < kUsual ? (d * kLog2e - log_S) * kLn2 : d - log_S * kLn2;
   };
   if (tid == 0) {
     logprob[row] = target >= 0 && target < p.vocab ? log_p(given) : 0.0f;
@@ -520,13 +522,13 @@ __global__ void __launch_bounds__(kThreads) scores_grad_kernel(const T* logits, 
   for (int i = 0; i < n; ++i) all += weight[slot][i];
   // what the distribution contributes: p (factor log2 p + rest)
   const bool usual = is_usual<T>(m);
-  const float factor = -gH * kLn2, rest_of = -fmaf(gH, H, all);
+  const float factor = -gH * kLn2, rest_of = -fmaf(gH, H, all), less = off_by(m) - log_S;
   const auto shared = [&](float v) {
-    const float y = exponent(v, m, usual) - log_S;
+    const float y = (v - m) * kLog2e - log_S;
     return st::exp2_ftz(y) * fmaf(factor, fmaxf(y, kFar), rest_of);
   };
   const auto shared_pair = [&](float2 v) {
-    const float2 y = st::add2(st::fma2(v, st::splat2(kLog2e), st::splat2(-scaled(m))), st::splat2(-log_S));
+    const float2 y = st::add2(st::fma2(v, st::splat2(kLog2e), st::splat2(-scaled(m))), st::splat2(less));
     return st::mul2(make_float2(st::exp2_ftz(y.x), st::exp2_ftz(y.y)), st::fma2(st::splat2(factor), y, st::splat2(rest_of)));
   };
   if (WIDE) {

@@ -42,26 +42,9 @@ struct WideParams {
   unsigned* err;
 };
 
-// A whole warp's bounded wait, as st::mbar_wait_warp, but the clock is first read after 64 polls: every hop of this kernel's ring is short, and a read of the
-// global timer takes longer than it.
-__device__ __forceinline__ bool wait(const unsigned long long& barrier, uint32_t parity, volatile int* abort_flag) {
-  const uint32_t bar = st::smem_u32(&barrier);
-  bool ok = st::mbar_try_wait(bar, parity);
-  uint64_t t0 = 0;
-  for (uint32_t i = 1; !ok; ++i) {
-    ok = st::mbar_try_wait(bar, parity);
-    if (ok || (i & 63u)) continue;
-    if (*abort_flag) break;
-    const uint64_t now = st::globaltimer_ns();
-    if (t0 == 0) t0 = now;
-    if (now - t0 > st::wait_limit_ns()) {
-      *abort_flag = 1;
-      break;
-    }
-  }
-  return __all_sync(0xffffffffu, ok);
+__device__ __forceinline__ bool wait(const unsigned long long& barrier, uint32_t parity, volatile int* abort_flag) {      // the whole warp
+  return st::mbar_wait_warp(st::smem_u32(&barrier), parity, abort_flag);
 }
-
 __device__ __forceinline__ uint32_t turn_over(uint32_t block) {      // an 8 x 8 block of 16-bit numbers, a row per 4 lanes
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(block));

@@ -63,6 +63,8 @@ class GPTDecoder:
             raise ValueError(f"GPTDecoder: learned positions end at {cfg.seq_len}, not at {max_length}")
         if weight_bits not in (4, 16) or head_bits not in (4, 16):
             raise ValueError(f"GPTDecoder: weights of 4 or 16 bits, got {weight_bits} and {head_bits} for the logits")
+        if (weight_bits == 4 or head_bits == 4) and model.flat_w.is_cuda and model.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"GPTDecoder: weights of 4 bits are multiplied by bf16 and fp16 activations, not by {model.dtype}")
         self.model, self.sequences, self.max_length, self.page_size = model, sequences, max_length, page_size
         dev = model.flat_w.device
         width = -(-max_length // page_size)

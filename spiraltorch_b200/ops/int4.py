@@ -68,6 +68,9 @@ class Weights:
         codes = torch.empty((down, -(-in_features // 64), 512), dtype=torch.uint8, device=device)
         return cls.__new__(cls)._set(codes, codes.new_empty((down, -(-in_features // group), 16), dtype=torch.bfloat16), out_features, in_features, group)
 
+    def __reduce__(self):
+        return Weights, tuple(getattr(self, name) for name in self.__slots__)
+
     @property
     def nbytes(self) -> int:
         return self.codes.nbytes + self.scales.nbytes
@@ -146,6 +149,7 @@ def quantize(weight: torch.Tensor, group: int = 64, *, out: Optional[Weights] = 
         raise ValueError(f"int4.quantize: a {n} x {k} matrix in groups of {group} into weights of {out.out_features} x {out.in_features} in groups of {out.group}")
     else:
         native.same_device("int4.quantize", weight, out.codes)
+        torch.autograd.graph.increment_version((out.codes, out.scales))      # gradients of products with what they held are refused
     if not on_cuda:
         q, s = quantize_reference(weight.detach(), group)
         out.codes.copy_(_tiles(q))
@@ -261,6 +265,7 @@ class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, bias, residual, w):
         ctx.w = w
+        ctx.save_for_backward(w.codes, w.scales)
         if x.dim() == 2:
             return _product(x, w, bias, None, residual)
         y = _product(x.reshape(-1, x.shape[-1]), w, bias, None, None if residual is None else residual.reshape(-1, w.out_features))
@@ -269,6 +274,7 @@ class _LinearFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         need_x, need_bias, need_residual, _ = ctx.needs_input_grad
+        _ = ctx.saved_tensors      # refuses weights that were quantised anew since
         w, dx, db = ctx.w, None, None
         dy2 = dy if dy.dim() == 2 else dy.reshape(-1, w.out_features)
         if need_x:

@@ -143,6 +143,25 @@ def test_refusals():
             int4.linear(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)), held)
 
 
+def test_weights_quantised_anew_are_no_gradient_of_the_old():
+    held = int4.quantize(_matrix(7, 45, torch.float32), 32)
+    x = torch.randn(3, 45, requires_grad=True)
+    y = int4.linear(x, held)
+    int4.quantize(_matrix(7, 45, torch.float32, 1), 32, out=held)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_weights_are_copied_saved_and_not_changed(tmp_path):
+    import copy
+    held = int4.quantize(_matrix(20, 70, torch.float32), 32)
+    torch.save(held, tmp_path / "w")
+    for other in (copy.deepcopy(held), torch.load(tmp_path / "w", weights_only=False), held.to("cpu")):
+        assert torch.equal(int4.dequantize(other), int4.dequantize(held)) and other.nbytes == held.nbytes
+    with pytest.raises(AttributeError):
+        held.in_features = 69
+
+
 # ---- kernels --------------------------------------------------------------------------------------------------------------------
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 
@@ -219,6 +238,36 @@ def test_linear_kernel(rows, n, k, group):
 
 
 @GPU
+@pytest.mark.parametrize("rows,n,k,group,act", [(1000, 4003, 300, 32, "gelu"), (190, 18900, 256, 64, None), (1, 9000, 2100, 64, "relu"), (7, 300, 17000, 128, "gelu"),
+                                                (16, 20000, 1000, 128, None), (12, 48, 9000, 32, "relu"), (600, 16, 20000, 64, None)])
+def test_linear_sizes_that_share_and_repeat_tiles(rows, n, k, group, act):
+    """More tiles than SMs, tiles of 192 tokens, more rows of weights than blocks, clusters and stretches beyond their 8 blocks."""
+    held, x, b, r, w, y = _product_case(rows, n, k, group, torch.bfloat16, True, act, True)
+    got = int4.linear(x, held, b, act=act, residual=r)
+    assert ((got.double() - y).abs() <= _allowed(x.double(), w, y, torch.bfloat16)).all()
+    x.requires_grad_(True)
+    dy = torch.randn(rows, n, generator=torch.Generator().manual_seed(6)).to(x.dtype).to(cuda)
+    want = dy.double() @ w
+    got = torch.autograd.grad(int4.linear(x, held), x, dy)[0]
+    assert ((got.double() - want).abs() <= _allowed(dy.double(), w.T, want, x.dtype)).all()
+
+
+@GPU
+@pytest.mark.parametrize("rows", [3, 20])
+def test_linear_offsets_beyond_32_bits(rows):
+    """Rows of x and of the residual 2^30 and 2^28 elements apart: their last ones lie behind 2^32 bytes."""
+    held, x, b, r, w, y = _product_case(rows, 136, 200, 64, torch.bfloat16, True, None, True)
+    step = 1 << (30 if rows == 3 else 28)
+    memory = torch.empty((rows - 1) * step + 256, dtype=torch.bfloat16, device=cuda)
+    far = memory.as_strided((rows, 200), (step, 1))
+    far.copy_(x)
+    assert torch.equal(int4.linear(far, held, b, residual=r), int4.linear(x, held, b, residual=r))
+    far = memory.as_strided((rows, 136), (step, 1))
+    far.copy_(r)
+    assert torch.equal(int4.linear(x, held, b, residual=far), int4.linear(x, held, b, residual=r))
+
+
+@GPU
 @pytest.mark.parametrize("rows", [1, 5, 16, 40, 200])
 def test_linear_views_and_places(rows):
     held, x, b, r, w, _ = _product_case(rows, 150, 328, 64, torch.bfloat16, True, None, True)
@@ -287,11 +336,19 @@ def test_linear_streams_graphs_and_updates():
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         y = int4.linear(x, held, b, act="gelu", residual=r)
+    with torch.cuda.graph(other := torch.cuda.CUDAGraph()):      # two captured calls, in turns and at once
+        z = int4.linear(torch.cat([x, x, x]), held, b)
     new = _matrix(130, 512, torch.bfloat16, 8, cuda)
     int4.quantize(new, 64, out=held)      # the replay multiplies by what the weights are now
     x.copy_(torch.randn_like(x))
     graph.replay()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other.replay()
+    graph.replay()
+    torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(y, int4.linear(x, held, b, act="gelu", residual=r))
+    assert torch.equal(z, int4.linear(torch.cat([x, x, x]), held, b))
 
 
 @GPU

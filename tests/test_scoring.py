@@ -38,7 +38,9 @@ def _hard(vocab, dtype, top):
     lows = base.clone()
     lows[::2] = low
     rows = [base, torch.full((vocab,), -INF), torch.zeros(vocab), torch.full((vocab,), low), ramp, ramp.flip(0), one, some, holes, lows, base + 1000.0, base - 1000.0,
-            torch.where(torch.arange(vocab) % 2 == 0, 0.0, -0.0), torch.full((vocab,), big), base.round(), torch.where(torch.arange(vocab) == vocab - 1, 50.0, low)]
+            torch.where(torch.arange(vocab) % 2 == 0, 0.0, -0.0), torch.full((vocab,), big), base.round(), torch.where(torch.arange(vocab) == vocab - 1, 50.0, low),
+            base * 1e3 + (3e4 if dtype == torch.float16 else 3e6), base - (60000 if dtype == torch.float16 else 1048570), torch.where(base > 0, -INF, low),
+            torch.where(torch.arange(vocab) < vocab // 2, -INF, base)]
     x = torch.stack(rows).to(dtype)
     t = torch.randint(0, vocab, (len(rows),), generator=torch.Generator().manual_seed(9))
     t[6], t[0] = vocab // 2, -100
@@ -152,18 +154,18 @@ def test_kernel(vocab, dtype):
 
 @GPU
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("vocab", [33, 300, 2048, 3001, 33000, 70000])
-@pytest.mark.parametrize("rows", [16, 320])
+@pytest.mark.parametrize("vocab", [33, 300, 2048, 3001, 33000, 140001])
+@pytest.mark.parametrize("rows", [20, 320])
 def test_kernel_on_hard_rows(rows, vocab, dtype):
     for top in (0, 1, 32):
         x, t = _hard(vocab, dtype, top)
-        x, t = x.repeat(rows // 16, 1), t.repeat(rows // 16)
+        x, t = x.repeat(rows // 20, 1), t.repeat(rows // 20)
         _check(scoring.token_scores(x.to(cuda), t.to(cuda), top=top), x, t, top)
 
 
 @GPU
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("vocab", [9, 300, 5000, 40000])
+@pytest.mark.parametrize("vocab", [9, 300, 5000, 40000, 70001, 263000])
 def test_kernel_non_finite(vocab, dtype):
     x, t = _logits(8, vocab, dtype, 3)
     x[0, 0], x[1, vocab - 1], x[2, vocab // 2], x[3, 1], x[3, 5], x[4, 2], x[4, 3] = math.nan, math.nan, INF, INF, math.nan, INF, -INF
@@ -228,19 +230,32 @@ def test_gradient_kernel(vocab, dtype):
 
 @GPU
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("vocab", [33, 300, 3001, 33000])
+@pytest.mark.parametrize("vocab", [33, 300, 3001, 70000])
 def test_gradient_kernel_on_hard_rows_and_views(vocab, dtype):
     x, t = _hard(vocab, dtype, 5)
     g = torch.Generator().manual_seed(2)
-    grads = (torch.randn(16, generator=g), torch.randn(16, generator=g), torch.randn(16, 5, generator=g))
+    grads = (torch.randn(20, generator=g), torch.randn(20, generator=g), torch.randn(20, 5, generator=g))
     _check_gradient(x, t, 5, grads)
     for pad, at in ((7, 3), (8, 8), (vocab, 0)):
         def layout(x):
-            wide = torch.zeros((16, vocab + pad), dtype=dtype, device=cuda)
+            wide = torch.zeros((20, vocab + pad), dtype=dtype, device=cuda)
             wide[:, at:at + vocab] = x
             return wide.detach()[:, at:at + vocab]
         _check_gradient(x, t, 5, grads, layout)
-    _check_gradient(x, t, 5, (grads[0][:1].expand(16), None, grads[2][:, :1].expand(16, 5)))
+    _check_gradient(x, t, 5, (grads[0][:1].expand(20), None, grads[2][:, :1].expand(20, 5)))
+
+
+@GPU
+def test_offsets_beyond_32_bits():
+    x, t = _logits(3, 3001, torch.bfloat16)
+    far = torch.empty((2 << 30) + 3008, dtype=torch.bfloat16, device=cuda).as_strided((3, 3001), (1 << 30, 1))
+    far.copy_(x)
+    far.requires_grad_(True)
+    s = scoring.token_scores(far, t.to(cuda), top=3)
+    _check(scoring.TokenScores(*(v.detach() for v in s)), x, t, 3)
+    near = x.to(cuda).requires_grad_(True)
+    want = torch.autograd.grad(scoring.token_scores(near, t.to(cuda)).logprob.sum(), near)[0]
+    assert torch.equal(torch.autograd.grad(s.logprob.sum(), far)[0], want)
 
 
 @GPU
