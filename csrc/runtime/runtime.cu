@@ -48,6 +48,15 @@ st::WaitLimitSetter g_setters[kMaxSetters];
 int g_n_setters = 0;
 }  // namespace
 
+namespace {
+// For what is set up at its first use, which may be inside a stream capture: calls that a capture refuses although they touch no stream.
+struct DuringCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  DuringCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~DuringCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+}  // namespace
+
 namespace st {
 
 void register_wait_limit_setter(WaitLimitSetter fn) {
@@ -72,6 +81,7 @@ unsigned* error_word() {
   if (g_err_dev[dev]) return g_err_dev[dev];
   std::lock_guard<std::mutex> lk(g_mu);
   if (g_err_dev[dev]) return g_err_dev[dev];
+  const DuringCapture relaxed;
   unsigned* h = nullptr;
   if (cudaHostAlloc(reinterpret_cast<void**>(&h), 4 * sizeof(unsigned), cudaHostAllocMapped) !=
       cudaSuccess)
@@ -112,6 +122,7 @@ bool encode_tmap(CUtensorMap* out, CUtensorMapDataType dtype, int rank, const vo
   // a no-op runtime call binds the primary context of the current device.
   static thread_local bool ctx_bound = false;
   if (!ctx_bound) {
+    const DuringCapture relaxed;
     cudaFree(nullptr);
     ctx_bound = true;
   }

@@ -352,6 +352,26 @@ def test_linear_streams_graphs_and_updates():
 
 
 @GPU
+@pytest.mark.parametrize("rows", [3, 27])
+def test_the_first_call_of_a_process_may_be_captured(rows):
+    """What the launchers set up at their first use does not end a capture."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = f"""
+import torch
+from spiraltorch_b200.ops import int4
+held = int4.quantize(torch.randn(256, 512, device="cuda", dtype=torch.bfloat16))
+x = torch.randn({rows}, 512, device="cuda", dtype=torch.bfloat16)
+with torch.cuda.graph(g := torch.cuda.CUDAGraph()):
+    y = int4.linear(x, held)
+g.replay()
+assert torch.equal(y, int4.linear(x, held))
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=Path(__file__).resolve().parents[1], timeout=300)
+
+
+@GPU
 def test_kernel_refusals():
     held = int4.quantize(torch.randn(20, 70, device=cuda), 32)
     x = torch.randn(3, 70, device=cuda)
