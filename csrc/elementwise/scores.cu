@@ -195,14 +195,18 @@ __device__ __forceinline__ unsigned long long warp_largest(unsigned long long ke
 
 // W warps on one row; kRoom keys, of which a round of the careful pass fills half.
 template <int W>
-struct Candidates {
-  static constexpr int kRound = W * 32 * 8, kRoom = 2 * kRound;
+struct Joined {
+  float sums[W][3], total[3];
+};
+template <int W>
+struct Candidates : Joined<W> {      // without alternatives only what is joined has room
+  static constexpr int kEach = 4, kRound = W * 32 * kEach, kRoom = 2 * kRound;      // elements of a thread, and of all, in a round
   unsigned long long key[kRoom];
   unsigned long long best[kMostTop];
-  unsigned long long bound[W], reach;      // reach: what the `top` best threads' largest elements reach
-  float sums[W][3], total[3];
-  int count;
-  uint16_t who[W * 32], owner[kMostTop];      // threads of the first keys; the `top` best threads
+  unsigned long long bound[W], thread[W * 32];      // thread: largest elements of those that may be among the best
+  uint32_t reach;                                   // in the order of the keys: what the `top` best threads' largest elements reach; 0: fewer threads have any
+  int threads, owners, count, kept;
+  uint16_t owner[W * 32];                           // threads whose largest element reaches that
 };
 
 template <int W> __device__ __forceinline__ void sync() {
@@ -267,7 +271,7 @@ __device__ __noinline__ void select_carefully(Candidates<W>& c, const T* x, int 
   if (tid == 0) c.count = 0;
   sync<W>();
   for (int at = from; at < to; at += Candidates<W>::kRound) {
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < Candidates<W>::kEach; ++i) {
       const int j = at + i * W * 32 + tid;
       if (j < to) {
         const unsigned long long key = key_of(to_float(x[j]), j);
@@ -302,9 +306,65 @@ __device__ __forceinline__ void join_group(Candidates<W>& c, Sums& s, int warp, 
   s.m = c.total[0], s.S = c.total[1], s.T = c.total[2];
 }
 
+// The elements, of vectors v0 to v1, that may be among the `top` largest, to c.key; best: the thread's largest element, none below the least usual one.
+template <typename T, int W>
+__device__ __noinline__ void gather_likeliest(Candidates<W>& c, const T* x, float best, int head, int v0, int v1, int top, int single, int tid) {
+  constexpr int N = Vec<T>::N, kGroup = W * 32;
+  const Vec<T>* xv = reinterpret_cast<const Vec<T>*>(x + head);
+  const int warp = tid >> 5, lane = tid & 31;
+  const unsigned long long key = v0 + tid < v1 || single >= 0 ? key_of(best, tid) : 0;
+  const uint32_t loose = static_cast<uint32_t>(bound_of(c, key, top, warp, lane) >> 32);      // and the counts are 0 for all
+  sync<W>();
+  if (key != 0 && static_cast<uint32_t>(key >> 32) >= loose) c.thread[atomicAdd(&c.threads, 1)] = key;
+  sync<W>();
+  const int n = c.threads;
+  if (tid == 0 && n < top) c.reach = 0;
+  if (tid < n) {
+    const unsigned long long own = c.thread[tid];
+    int rank = 0, above = 0;      // among the threads, and of larger values: equal ones may hold a lower index
+    for (int j = 0; j < n; ++j) {
+      const unsigned long long other = c.thread[j];
+      rank += other > own;
+      above += static_cast<uint32_t>(other >> 32) > static_cast<uint32_t>(own >> 32);
+    }
+    if (rank == top - 1) c.reach = static_cast<uint32_t>(own >> 32);
+    if (above < top) c.owner[atomicAdd(&c.owners, 1)] = static_cast<uint16_t>(~static_cast<uint32_t>(own));
+  }
+  sync<W>();
+  const uint32_t reach = c.reach;
+  const float limit = reach ? value_of(static_cast<unsigned long long>(reach) << 32) : -INFINITY;
+  const auto keep = [&](float value, int index) {
+    if (!(value >= limit)) return;
+    const int at = atomicAdd(&c.count, 1);
+    if (at < Candidates<W>::kRoom) c.key[at] = key_of(value, index);
+  };
+  if (single >= 0) keep(to_float(x[single]), single);
+  // the owners' vectors, two to a thread at a time
+  const int each = (v1 - v0 + kGroup - 1) / kGroup, all = c.owners * each;
+  for (int i = tid; i < all; i += 2 * kGroup) {
+    Vec<T> again[2];
+    int at[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int item = i + h * kGroup, o = item / each;
+      at[h] = item < all ? v0 + c.owner[o] + (item - o * each) * kGroup : v1;
+      if (at[h] < v1) again[h] = xv[at[h]];
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (at[h] >= v1) continue;
+      float2 f[N / 2];
+      again[h].pairs(f);
+      if (!(largest_of(f) >= limit)) continue;
+#pragma unroll
+      for (int k = 0; k < N; ++k) keep(k % 2 ? f[k / 2].y : f[k / 2].x, head + at[h] * N + k);
+    }
+  }
+}
+
 // One row (or, in a cluster, one part of it) per W warps.
 template <typename T, int W, bool TOP>
-__global__ void __launch_bounds__(kThreads) scores_kernel(const T* logits, const long long* targets, float* logprob, float* entropy, float2* stats, long long* top_ids,
+__global__ void __launch_bounds__(W == 1 ? kThreads : W * 32, W == 1 ? 1 : 32 / W) scores_kernel(const T* logits, const long long* targets, float* logprob, float* entropy, float2* stats, long long* top_ids,
                                                           float* top_logprobs, const ScoreParams p) {
   extern __shared__ __align__(16) uint8_t room[];
   chain_begin(logits, targets, logprob, entropy, stats, top_ids, top_logprobs);
@@ -320,22 +380,21 @@ __global__ void __launch_bounds__(kThreads) scores_kernel(const T* logits, const
   const int vectors = (p.vocab - head) / N, rest = head + vectors * N, singles = head + p.vocab - rest;
   const int share = (vectors + p.parts - 1) / p.parts, v0 = part * share, v1 = min(vectors, v0 + share);
   const Vec<T>* xv = reinterpret_cast<const Vec<T>*>(x + head);
-  if (TOP && tid == 0) c.count = 0;
+  if (TOP && tid == 0) c.threads = c.owners = c.count = 0;
   PairSums<T> pairs;
   Sums s;
-  float best = __uint_as_float(0x7FC00000u);      // the thread's largest element, in vector best_at
-  int best_at = -1;
+  float best = -INFINITY;      // the thread's largest element
   const int one = tid < head ? tid : rest + tid - head;
   const bool has_single = part == 0 && tid < singles;
   const float single = has_single ? to_float(x[one]) : 0.0f;
   const long long target = tid == 0 && part == 0 ? targets[row] : -1;
   const float given = target >= 0 && target < p.vocab ? to_float(x[target]) : 0.0f;
 
-  stream(xv, v0 + tid, v1, kGroup, [&](const Vec<T>& vec, int v) {
+  stream(xv, v0 + tid, v1, kGroup, [&](const Vec<T>& vec, int) {
     float2 f[N / 2];
     usual_pairs(vec, f);
     const float largest = largest_of(f);
-    if (TOP && !(largest <= best)) best = largest, best_at = v;
+    if (TOP) best = fmaxf(best, largest);
     pairs.add(f, largest);
   });
   s.m = pairs.m, s.S = pairs.S.x + pairs.S.y, s.T = pairs.T.x + pairs.T.y;
@@ -346,58 +405,7 @@ __global__ void __launch_bounds__(kThreads) scores_kernel(const T* logits, const
     s.S += e, s.T = fmaf(e, y, s.T);
   }
 
-  if (TOP) {
-    unsigned long long key = has_single ? key_of(single, one) : 0;
-    if (best_at >= 0) {
-      const Vec<T> again = xv[best_at];
-      int at = 0;
-#pragma unroll
-      for (int k = N - 1; k >= 0; --k) at = at_least<T>(to_float(again.v[k])) == best ? k : at;
-      float value = 0.0f;
-#pragma unroll
-      for (int k = 0; k < N; ++k) value = k == at ? to_float(again.v[k]) : value;
-      key = max(key, key_of(value, head + best_at * N + at));
-    }
-    const unsigned long long loose = max(bound_of(c, key, p.top, warp, lane), 1ull);      // and the count is 0 for all
-    sync<W>();
-    if (key >= loose) {
-      const int at = atomicAdd(&c.count, 1);
-      c.key[at] = key, c.who[at] = static_cast<uint16_t>(tid);
-    }
-    sync<W>();
-    const int n = c.count;
-    if (tid == 0 && n < p.top) c.reach = 1;
-    if (tid < n) {
-      const unsigned long long own = c.key[tid];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += c.key[j] > own;
-      if (rank < p.top) c.owner[rank] = c.who[tid];
-      if (rank == p.top - 1) c.reach = own;
-    }
-    sync<W>();
-    const unsigned long long reach = c.reach;
-    if (tid == 0) c.count = 0;
-    sync<W>();
-    const float limit = reach > 1 ? value_of(reach) : -INFINITY;
-    const auto keep = [&](float value, int index) {
-      if (!(value >= limit)) return;
-      const unsigned long long k = key_of(value, index);
-      if (k >= reach) {
-        const int at = atomicAdd(&c.count, 1);
-        if (at < Candidates<W>::kRoom) c.key[at] = k;
-      }
-    };
-    if (has_single) keep(single, one);
-    for (int o = warp; o < min(n, p.top); o += W)
-      for (int at = v0 + c.owner[o] + lane * kGroup; at < v1; at += 32 * kGroup) {
-        const Vec<T> again = xv[at];
-        float2 f[N / 2];
-        again.pairs(f);
-        if (!(largest_of(f) >= limit)) continue;
-#pragma unroll
-        for (int k = 0; k < N; ++k) keep(k % 2 ? f[k / 2].y : f[k / 2].x, head + at * N + k);
-      }
-  }
+  if (TOP) gather_likeliest<T, W>(c, x, has_single ? fmaxf(best, at_least<T>(single)) : best, head, v0, v1, p.top, has_single ? one : -1, tid);
 
   // sums of the row (part): in every thread
   join_group(c, s, warp, lane, true);
@@ -415,8 +423,8 @@ __global__ void __launch_bounds__(kThreads) scores_kernel(const T* logits, const
     sync<W>();
     // With care: a NaN hides from comparisons (and an infinity makes S one); keys that found no room are lost; of elements that count as the least usual one, a
     // thread has not kept the largest.
-    const unsigned long long reach = c.reach;
-    if (c.count > Candidates<W>::kRoom || s.S != s.S || (reach > 1 && !(value_of(reach) > kLeast<T>))) {
+    const uint32_t reach = c.reach;
+    if (c.count > Candidates<W>::kRoom || s.S != s.S || (reach && !(value_of(static_cast<unsigned long long>(reach) << 32) > kLeast<T>))) {
       if (part == 0) {      // its single elements too: with one part these are the row
         if (p.parts == 1) {
           select_carefully<T, W>(c, x, 0, p.vocab, p.top, tid);
@@ -432,9 +440,12 @@ __global__ void __launch_bounds__(kThreads) scores_kernel(const T* logits, const
     select(c, p.top, tid);
   }
   if (W > 1 && p.parts > 1) {      // the parts of a row: blocks of a cluster, read by the first
-    const int n = c.count < p.top ? c.count : p.top;
+    const int n = TOP ? min(c.count, p.top) : 0;
     sync<W>();
-    if (tid == 0) c.sums[0][0] = s.m, c.sums[0][1] = s.S, c.sums[0][2] = s.T, c.count = n;
+    if (tid == 0) {
+      c.sums[0][0] = s.m, c.sums[0][1] = s.S, c.sums[0][2] = s.T;
+      if (TOP) c.kept = n;
+    }
     st::cluster_sync();
     if (part == 0) {
       s = Sums();
@@ -446,18 +457,16 @@ __global__ void __launch_bounds__(kThreads) scores_kernel(const T* logits, const
         s.join(f[0], f[1], f[2]);
       }
       if (TOP) {
-        // up to 8 parts of up to 32 keys: one for every thread
-        const int r = tid >> 5, i = tid & 31;
-        unsigned long long key = 0;
-        if (r < p.parts) {
-          int have;
-          asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(have) : "r"(st::cluster_map(st::smem_u32(&c.count), r)));
-          if (i < have) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key) : "r"(st::cluster_map(st::smem_u32(&c.best[i]), r)));
-        }
         sync<W>();
         if (tid == 0) c.count = 0;
         sync<W>();
-        if (key) c.key[atomicAdd(&c.count, 1)] = key;
+        for (int r = warp; r < p.parts; r += W) {      // up to 32 keys of each
+          unsigned long long key = 0;
+          int have;
+          asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(have) : "r"(st::cluster_map(st::smem_u32(&c.kept), r)));
+          if (lane < have) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key) : "r"(st::cluster_map(st::smem_u32(&c.best[lane]), r)));
+          if (key) c.key[atomicAdd(&c.count, 1)] = key;
+        }
         sync<W>();
         select(c, p.top, tid);
       }
@@ -595,9 +604,9 @@ int forward(const void* logits, const long long* targets, float* logprob, float*
   p.parts = W == 1 ? 1 : parts_of(p.rows, p.vocab);
   const long long blocks = W == 1 ? (p.rows + kWarps - 1) / kWarps : p.rows * p.parts;
   if (blocks > 2147483647LL) return st::fail(ST_ERR_TOO_LARGE, "scores: too many rows");
-  const size_t smem = sizeof(Candidates<W>) * (W == 1 ? kWarps : 1);
+  const size_t smem = (TOP ? sizeof(Candidates<W>) : sizeof(Joined<W>)) * (W == 1 ? kWarps : 1);
   static_assert(sizeof(Candidates<W>) * (W == 1 ? kWarps : 1) <= 48 * 1024, "candidates need no opting in");
-  const cudaError_t e = st::chained(scores_kernel<T, W, TOP>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), smem, stream, p.parts)(
+  const cudaError_t e = st::chained(scores_kernel<T, W, TOP>, dim3(static_cast<unsigned>(blocks)), dim3(W == 1 ? kThreads : W * 32), smem, stream, p.parts)(
       static_cast<const T*>(logits), targets, logprob, entropy, stats, top_ids, top_logprobs, p);
   return e == cudaSuccess ? ST_OK : st::fail_cuda(e, "token scores");
 }
@@ -608,8 +617,10 @@ int forward(const void* logits, const long long* targets, float* logprob, float*
   if (p.vocab <= kWarpRow)
     return p.top ? forward<T, 1, true>(logits, targets, logprob, entropy, stats, top_ids, top_logprobs, p, stream)
                  : forward<T, 1, false>(logits, targets, logprob, entropy, stats, top_ids, top_logprobs, p, stream);
-  return p.top ? forward<T, kWarps, true>(logits, targets, logprob, entropy, stats, top_ids, top_logprobs, p, stream)
-               : forward<T, kWarps, false>(logits, targets, logprob, entropy, stats, top_ids, top_logprobs, p, stream);
+  if (p.top) return forward<T, kWarps, true>(logits, targets, logprob, entropy, stats, top_ids, top_logprobs, p, stream);
+  // 4 warps to a row where there are rows for many turns of the SMs: 8192 x 50304 141 us, 149 with 8 (with alternatives 211 and 200); 300 x 50304 13.1 and 11.4, 1 row 6.0 and 5.1
+  return p.rows >= 16 * st::sm_count() ? forward<T, 4, false>(logits, targets, logprob, entropy, stats, top_ids, top_logprobs, p, stream)
+                                      : forward<T, kWarps, false>(logits, targets, logprob, entropy, stats, top_ids, top_logprobs, p, stream);
 }
 
 template <typename T, int W, bool WIDE>

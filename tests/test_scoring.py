@@ -165,6 +165,16 @@ def test_kernel_on_hard_rows(rows, vocab, dtype):
 
 @GPU
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [2100, 5001])
+def test_kernel_on_many_rows(vocab, dtype):
+    for top in (0, 20):
+        x, t = _hard(vocab, dtype, top)
+        x, t = x.repeat(125, 1), t.repeat(125)
+        _check(scoring.token_scores(x.to(cuda), t.to(cuda), top=top), x, t, top)
+
+
+@GPU
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("vocab", [9, 300, 5000, 40000, 70001, 263000])
 def test_kernel_non_finite(vocab, dtype):
     x, t = _logits(8, vocab, dtype, 3)
