@@ -155,24 +155,28 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
       if (!wait(sh.full[filled], fill_phase, abort_flag)) break;
       const unsigned char* codes = raw + (smem_codes - smem_x) + stage * kCodes;
       const unsigned char* scales = raw + (smem_scales - smem_x) + stage * kScales;
-      uint32_t all_r[2][2][16];
+      uint32_t r[2][2][16];      // [64 of the 128 numbers of every lane][16 lanes]
+      if (TURN) {      // words `quarter % 2 * 2` and the next of column tile quarter / 2, 16 columns each, from the 8 row tiles; both lie in one group
+        const int s = (quarter & 1) * 2, group = ((quarter >> 1) * 64 + s * 16) / GROUP;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {                          // 64 of the 128 numbers of every lane
-        auto& r = all_r[k];
+        for (int i = 0; i < 8; ++i) {
+          const uint2 words = *reinterpret_cast<const uint2*>(codes + (i * 2 + (quarter >> 1)) * kTileBytes + lane * 16 + s * 4);
+          const uint32_t both = *reinterpret_cast<const uint32_t*>(scales + (i * kScaleGroups + group) * 32 + (lane >> 2) * 4);
+          Scale<T> low, high;
+          low.set(both), high.set(both >> 16);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {               // 16 lanes each
-          if (TURN) {      // word `quarter % 2 * 2 + half` of column tile quarter / 2, from 4 of the row tiles
-            const int s = (quarter & 1) * 2 + half, group = ((quarter >> 1) * 64 + s * 16) / GROUP;
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t word = half ? words.y : words.x;
+            uint32_t* to = r[i >> 2][half] + 4 * (i & 3);
+            to[0] = turn_over(low.pair(word, 0)), to[1] = turn_over(low.pair(word, 2));
+            to[2] = turn_over(high.pair(word, 1)), to[3] = turn_over(high.pair(word, 3));
+          }
+        }
+      } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + ((4 * k + i) * 2 + (quarter >> 1)) * kTileBytes + lane * 16 + s * 4);
-              const uint32_t both = *reinterpret_cast<const uint32_t*>(scales + ((4 * k + i) * kScaleGroups + group) * 32 + (lane >> 2) * 4);
-              Scale<T> low, high;
-              low.set(both), high.set(both >> 16);
-              r[half][4 * i] = turn_over(low.pair(word, 0)), r[half][4 * i + 1] = turn_over(low.pair(word, 2));
-              r[half][4 * i + 2] = turn_over(high.pair(word, 1)), r[half][4 * i + 3] = turn_over(high.pair(word, 3));
-            }
-          } else {
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
             const int u = quarter * 2 + half;
             const uint4 four = *reinterpret_cast<const uint4*>(codes + (u * 2 + k) * kTileBytes + lane * 16);
             const uint32_t word[4] = {four.x, four.y, four.z, four.w};
@@ -183,18 +187,17 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
                 const uint32_t both = *reinterpret_cast<const uint32_t*>(scales + (u * kScaleGroups + (k * 64 + i * 16) / GROUP) * 32 + (lane >> 2) * 4);
                 low.set(both), high.set(both >> 16);
               }
-              r[half][4 * i] = low.pair(word[i], 0), r[half][4 * i + 1] = high.pair(word[i], 1);
-              r[half][4 * i + 2] = low.pair(word[i], 2), r[half][4 * i + 3] = high.pair(word[i], 3);
+              r[k][half][4 * i] = low.pair(word[i], 0), r[k][half][4 * i + 1] = high.pair(word[i], 1);
+              r[k][half][4 * i + 2] = low.pair(word[i], 2), r[k][half][4 * i + 3] = high.pair(word[i], 3);
             }
           }
-        }
       }
       if (!wait(sh.taken[ring], ring_phase ^ 1u, abort_flag)) break;
       st::tc_fence_after();
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        tmem_st_16x32(to + ring * 64 + k * 32, all_r[k][0]);
-        tmem_st_16x32(to + (16u << 16) + ring * 64 + k * 32, all_r[k][1]);
+        tmem_st_16x32(to + ring * 64 + k * 32, r[k][0]);
+        tmem_st_16x32(to + (16u << 16) + ring * 64 + k * 32, r[k][1]);
       }
       st::tmem_st_wait();
       st::tc_fence_before();

@@ -149,7 +149,7 @@ def quantize(weight: torch.Tensor, group: int = 64, *, out: Optional[Weights] = 
         raise ValueError(f"int4.quantize: a {n} x {k} matrix in groups of {group} into weights of {out.out_features} x {out.in_features} in groups of {out.group}")
     else:
         native.same_device("int4.quantize", weight, out.codes)
-        torch.autograd.graph.increment_version((out.codes, out.scales))      # gradients of products with what they held are refused
+        torch.autograd.graph.increment_version(out.codes)      # gradients of products with what they held are refused
     if not on_cuda:
         q, s = quantize_reference(weight.detach(), group)
         out.codes.copy_(_tiles(q))
@@ -264,8 +264,7 @@ class _InputGradientFn(torch.autograd.Function):
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, bias, residual, w):
-        ctx.w = w
-        ctx.save_for_backward(w.codes, w.scales)
+        ctx.w, ctx.version = w, w.codes._version
         if x.dim() == 2:
             return _product(x, w, bias, None, residual)
         y = _product(x.reshape(-1, x.shape[-1]), w, bias, None, None if residual is None else residual.reshape(-1, w.out_features))
@@ -274,8 +273,9 @@ class _LinearFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         need_x, need_bias, need_residual, _ = ctx.needs_input_grad
-        _ = ctx.saved_tensors      # refuses weights that were quantised anew since
         w, dx, db = ctx.w, None, None
+        if w.codes._version != ctx.version:
+            raise RuntimeError("int4.linear: weights needed for a gradient have been modified by an inplace operation: they were quantised anew")
         dy2 = dy if dy.dim() == 2 else dy.reshape(-1, w.out_features)
         if need_x:
             dx = _InputGradientFn.apply(dy2, w) if torch.is_grad_enabled() and dy.requires_grad else _input_gradient(dy2, w)

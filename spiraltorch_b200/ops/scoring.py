@@ -84,8 +84,8 @@ def _forward(logits, targets, top, keep):
     rows, vocab = logits.shape
     index = native.require_cuda("token_scores", logits, targets)
     ids = targets.new_empty((rows, top))
-    logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    entropy, top_logprobs = logprob.new_empty(rows), logprob.new_empty((rows, top))
+    logprob = torch.empty_like(targets, dtype=torch.float32)
+    entropy, top_logprobs = torch.empty_like(logprob), logprob.new_empty((rows, top))
     stats = logprob.new_empty((rows, 2)) if keep else None
     if rows == 0:
         return TokenScores(logprob, entropy, ids, top_logprobs), stats
