@@ -8,8 +8,9 @@
 // costs 0.4% of the error that scales of full precision leave (0.0953 and 0.0949 of the weights' size).  The sign of s puts the extremum on -8, which symmetric codes of
 // -7..7 leave unused (0.108).  A group with a NaN or an infinity has a scale that is NaN.
 //
-// Bound by memory.  A warp takes 16 rows by 128 columns, which holds whole groups of every size: its loads are all in flight together, extrema are joined by
+// A warp takes 16 rows by 128 columns, which holds whole groups of every size: its loads are all in flight together, extrema are joined by
 // shuffles, and 1 KB of shared memory turns the codes from rows to the order of int4.cuh.
+// Measured: 8192 x 8192 in bf16 44 us quantised, 3.9 TB/s of the 6.6 that a copy reaches: instructions bound it (the ALU pipe busy 76%); 31 us read back, 5.5 TB/s.
 #include "../common/host.h"
 #include "../common/chain.cuh"
 #include "int4.cuh"

@@ -288,7 +288,7 @@ class _LinearFn(torch.autograd.Function):
 
 def linear(x: torch.Tensor, w: Weights, bias: Optional[torch.Tensor] = None, *, act: Optional[str] = None,
            residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``act(x W^T + bias) + residual``: ``x`` ``[..., in]`` in bf16 or fp16, ``bias`` ``[out]`` and ``residual`` ``[..., out]`` of the same type, ``act`` None, ``"relu"``
+    """``act(x W^T + bias) + residual``: ``x`` ``[..., in]`` in bf16 or fp16 (2^30 rows at most), ``bias`` ``[out]`` and ``residual`` ``[..., out]`` of the same type, ``act`` None, ``"relu"``
     or ``"gelu"`` (tanh form).  Sums are in fp32; the result, in ``x``'s type, is rounded once.
 
     Differentiable in ``x``, ``bias`` and ``residual`` (the weights are constants) without ``act``: apply an activation to the result where gradients are needed."""
@@ -300,6 +300,8 @@ def linear(x: torch.Tensor, w: Weights, bias: Optional[torch.Tensor] = None, *, 
     n = w.out_features
     if len(shape) == 0 or shape[-1] != w.in_features:
         raise ValueError(f"int4.linear: x {tuple(shape)} does not end in the weights' {w.in_features} inputs")
+    if x.numel() > w.in_features << 30:
+        raise ValueError(f"int4.linear: at most 2^30 rows, got x {tuple(shape)}")
     if bias is not None and (bias.shape != (n,) or bias.dtype is not dtype):
         raise ValueError(f"int4.linear: bias must be {dtype} {(n,)}, got {bias.dtype} {tuple(bias.shape)}")
     if residual is not None and (residual.shape != (*shape[:-1], n) or residual.dtype is not dtype):

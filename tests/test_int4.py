@@ -135,7 +135,8 @@ def test_refusals():
                  lambda: int4.linear(x[:, :69], held), lambda: int4.linear(x, held, torch.zeros(21)), lambda: int4.linear(x, held, torch.zeros(20).half()),
                  lambda: int4.linear(x, held, residual=torch.zeros(2, 20)), lambda: int4.linear(x, held, act="tanh"), lambda: int4.linear(x.int(), held),
                  lambda: int4.Weights(held.codes, held.scales, 20, 140, 32), lambda: int4.Weights(held.codes, held.scales, 20, 70, 64),
-                 lambda: int4.linear(x.clone().requires_grad_(), held, act="gelu"), lambda: int4.linear(torch.tensor(1.0), held)):
+                 lambda: int4.linear(x.clone().requires_grad_(), held, act="gelu"), lambda: int4.linear(torch.tensor(1.0), held),
+                 lambda: int4.linear(x[:1].expand((1 << 30) + 1, 70), held)):
         with pytest.raises(ValueError):
             call()
     with torch.autograd.forward_ad.dual_level():
