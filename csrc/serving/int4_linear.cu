@@ -93,16 +93,19 @@ struct Slice {
     if (c0 + C <= chunks) {
 #pragma unroll
       for (int i = 0; i < C; ++i) w[i] = *reinterpret_cast<const uint4*>(from + i * kTileBytes);
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i)
+        if (c0 + i < chunks) w[i] = *reinterpret_cast<const uint4*>(from + i * kTileBytes);
+    }
+    // apart from the codes: of groups of 32 the last chunk may have one, and what follows in memory are the next tile row's
+    if (g0 + kScales <= groups) {
 #pragma unroll
       for (int i = 0; i < kWords; ++i)
         if (kScales * 8 % 32 == 0 || i * 32 + lane < kScales * 8) s[i] = words[i * 32];
     } else {
 #pragma unroll
-      for (int i = 0; i < C; ++i)
-        if (c0 + i < chunks) w[i] = *reinterpret_cast<const uint4*>(from + i * kTileBytes);
-#pragma unroll
-      for (int i = 0; i < kWords; ++i)
-        s[i] = i * 32 + lane < min(kScales, groups - g0) * 8 ? words[i * 32] : 0u;      // half a chunk may be behind the last group
+      for (int i = 0; i < kWords; ++i) s[i] = i * 32 + lane < min(kScales, groups - g0) * 8 ? words[i * 32] : 0u;
     }
   }
   // of chunk i, half k of it where groups are halves

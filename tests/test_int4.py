@@ -305,6 +305,26 @@ def test_linear_non_finite_values_stay_in_their_rows(rows):
 
 @GPU
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("k", [20, 84, 200, 1000, 1230, 4050])      # half of the last 64 columns have no group of 32, where a warp's columns end with the row's or before
+@pytest.mark.parametrize("rows", [1, 9, 16])
+def test_linear_reads_the_scales_of_its_own_rows(rows, k, dtype):
+    _, x, _, _, w, _ = _product_case(rows, 37, k, 32, dtype, False, None, False)
+    held = int4.quantize(w.float(), 32)
+    base = int4.linear(x, held)
+    # an infinity at the beginning of a row is in no other row's scales
+    v = w.float().clone()
+    v[20, 0] = math.inf
+    got = int4.linear(x, int4.quantize(v, 32))
+    assert got[:, 20].isnan().all() and torch.equal(got[:, :20], base[:, :20]) and torch.equal(got[:, 21:], base[:, 21:])
+    # what lies behind the last scales is not read
+    memory = torch.full((held.scales.numel() + 512,), 0xFF, dtype=torch.uint8, device=cuda).repeat(2).view(torch.bfloat16)
+    scales = memory[:held.scales.numel()].view(held.scales.shape)
+    scales.copy_(held.scales)
+    assert torch.equal(int4.linear(x, int4.Weights(held.codes, scales, 37, k, 32)), base)
+
+
+@GPU
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("rows,n,k,group", [(1, 16, 64, 64), (5, 37, 100, 32), (33, 300, 129, 128), (200, 130, 777, 64), (300, 520, 264, 32)])
 def test_linear_gradients(rows, n, k, group, dtype):
     held, x, b, r, w, _ = _product_case(rows, n, k, group, dtype, True, None, True)
