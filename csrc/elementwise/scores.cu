@@ -271,6 +271,7 @@ __device__ void select(Candidates<W>& c, int top, int tid) {
 template <typename T, int W>
 __device__ __noinline__ void select_carefully(Candidates<W>& c, const T* x, int from, int to, int top, int tid) {
   unsigned long long bound = 0;
+  sync<W>();      // the count may be what brought the row here: all have read it
   if (tid == 0) c.count = 0;
   sync<W>();
   for (int at = from; at < to; at += Candidates<W>::kRound) {

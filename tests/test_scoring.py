@@ -174,6 +174,26 @@ def test_kernel_on_many_rows(vocab, dtype):
 
 
 @GPU
+@pytest.mark.parametrize("vocab,rows", [(1500, 3000), (2100, 3000), (5001, 3000), (5001, 5), (20011, 1000), (140001, 40), (263000, 3)])
+@pytest.mark.parametrize("top", [1, 20, 32])
+def test_kernel_on_coarse_values_row_after_row(vocab, rows, top):
+    """More elements than there is room for reach the bound in every second row, whose warps must agree that it is looked through with care."""
+    g = torch.Generator().manual_seed(8)
+    x = torch.where(torch.rand(rows, vocab, generator=g) < 0.999 - 0.9 * torch.rand(rows, 1, generator=g), 2.0, 1.0)
+    x[1::2] = torch.randn(x[1::2].shape, generator=g)
+    t = torch.randint(0, vocab, (rows,), generator=g)
+    at = torch.arange(vocab)
+    want = torch.where(x[0::2] == 2.0, at, at + vocab).topk(top, dim=1, largest=False).values % vocab
+    x, t = x.bfloat16().to(cuda), t.to(cuda)
+    _check(scoring.token_scores(x[:6], t[:6], top=top), x[:6].cpu(), t[:6].cpu(), top)
+    first = scoring.token_scores(x, t, top=top)
+    assert torch.equal(first.top_ids[0::2].cpu(), want)
+    for _ in range(5):
+        again = scoring.token_scores(x, t, top=top)
+        assert all(torch.equal(a, b) for a, b in zip(again, first))
+
+
+@GPU
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("vocab", [9, 300, 5000, 40000, 70001, 263000])
 def test_kernel_non_finite(vocab, dtype):
