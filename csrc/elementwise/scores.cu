@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(W == 1 ? kThreads : W * 32, W == 1 ? 1 : 32 / 
   join_group(c, s, warp, lane, true);
   if (is_usual<T>(s.m)) {
     s.shift(off_by(s.m));
-  } else if (s.S == s.S) {
+  } else {      // whatever the sums are: beyond 2.3e38 a finite m's y is infinite, and differences of two such are NaN
     s = Sums();
     for (int v = v0 + tid; v < v1; v += kGroup)
       for (int k = 0; k < N; ++k) s.add(to_float(x[head + v * N + k]));

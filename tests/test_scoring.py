@@ -193,6 +193,37 @@ def test_kernel_on_coarse_values_row_after_row(vocab, rows, top):
         assert all(torch.equal(a, b) for a, b in zip(again, first))
 
 
+def _huge(vocab, dtype):
+    """Different finite logits whose multiple log2 e is infinite (from 2.36e38 on): in one vector, in one thread's, in those of other lanes, warps and blocks."""
+    base, t = _logits(11, vocab, torch.float32, 6)
+    at = torch.arange(vocab)
+    base[0, 1], base[0, 2] = 2.5e38, 3.3e38
+    base[1, 1], base[1, 2] = 3.3e38, 2.5e38
+    base[2], base[3] = torch.linspace(2.4e38, 3.38e38, vocab), torch.linspace(3.38e38, 2.4e38, vocab)
+    base[4, 0], base[4, -1] = 2.5e38, 3.3e38
+    base[5, ::8] = 2.3e38 + 1e38 * torch.rand(base[5, ::8].shape, generator=torch.Generator().manual_seed(7))
+    base[6] = torch.where(at % 3 == 0, 3.3e38, 2.5e38)
+    base[7] = torch.where(at % 2 == 0, -INF, torch.where(at % 5 == 0, 3e38, 2.4e38))
+    base[8, -3:] = torch.tensor([2.35e38, 2.36e38, 2.37e38])
+    base[9, vocab // 2], base[9, vocab // 2 + 1] = torch.finfo(dtype).max, 2.5e38
+    base[10, :3] = torch.tensor([3.3e38, 2.5e38, math.nan])
+    return base.to(dtype), t
+
+
+@GPU
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [9, 300, 2048, 5001, 50304, 140001, 263000])
+def test_kernel_and_gradient_on_huge_rows(vocab, dtype):
+    x, t = _huge(vocab, dtype)
+    top = min(5, vocab)
+    for k in (0, top):
+        got = scoring.token_scores(x.to(cuda), t.to(cuda), top=k)
+        _check(got, x, t, k)
+        assert got.logprob[:10].isfinite().sum() >= 9 and got.entropy[:10].isfinite().all() and got.entropy[10].isnan()
+    g = torch.Generator().manual_seed(2)
+    _check_gradient(x[:10], t[:10], top, (torch.randn(10, generator=g), torch.randn(10, generator=g), torch.randn(10, top, generator=g)))
+
+
 @GPU
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("vocab", [9, 300, 5000, 40000, 70001, 263000])
