@@ -42,12 +42,15 @@ __device__ __forceinline__ uint32_t pick(uint32_t word, uint32_t mask, uint32_t 
   return d;
 }
 
-// Nibbles e and e + 4 of a word as two numbers -8..7, exactly: the nibble is put into the low bits of 128 (bf16) or 1024 (fp16), where a unit is 1, and
-// 136 or 1032 is subtracted.
+// Nibbles e and e + 4 of a word as two numbers of -8 to 7 units, exactly: the nibble is put into the low bits of 128 (bf16) or 1024 (fp16) units, where a unit is 1, and
+// 136 or 1032 of them are subtracted.  A unit is 1 in fp16 and 2^-10 in bf16: the products with a group of 128 inputs then sum up to no more than the largest of them, so that no
+// finite bf16 overflows before the scale is known.  They stay whole multiples of 2^-143, which fp32 holds.
+template <typename T> constexpr float kUnits = 1.0f;      // in 1
+template <> constexpr float kUnits<__nv_bfloat16> = 1024.0f;
 template <typename T> __device__ __forceinline__ uint32_t codes_to_pair(uint32_t word, int e);
 template <> __device__ __forceinline__ uint32_t codes_to_pair<__nv_bfloat16>(uint32_t word, int e) {
-  const uint32_t v = pick(word >> (4 * e), 0x000F000Fu, 0x43004300u);
-  const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __nv_bfloat162(__float2bfloat16_rn(136.0f), __float2bfloat16_rn(136.0f)));
+  const uint32_t v = pick(word >> (4 * e), 0x000F000Fu, 0x3E003E00u);
+  const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __float2bfloat162_rn(136.0f / kUnits<__nv_bfloat16>));
   return *reinterpret_cast<const uint32_t*>(&d);
 }
 template <> __device__ __forceinline__ uint32_t codes_to_pair<__half>(uint32_t word, int e) {

@@ -117,7 +117,7 @@ struct Slice {
 
 // Blocks take tile rows (16 weight rows) in turns; their 8 warps share the columns, C chunks of 64 each: a stretch of 8 C.  Where there are more columns, a cluster's
 // blocks take a stretch each (every eighth, beyond 8) and join their sums.  The weights are the matrix instruction's 16-row operand, NT times 8 tokens its
-// columns.  The products of a group are summed on their own and take its scale in fp32, so codes enter as the whole numbers that they are.
+// columns.  The products of a group are summed on their own and take its scale in fp32, so codes enter as whole numbers of units.
 // The next row's codes are on their way while one is multiplied.
 template <typename T, int NT, int C, int GROUP>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) linear_kernel(const T* x, const uint8_t* codes, const __nv_bfloat16* scales, const T* bias, const T* residual, T* y,
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) linear_kernel(co
           }
         }
         const uint32_t both = own.scale(i, k, lane);
-        const float low = bf16_bits(both), high = __uint_as_float(both & 0xFFFF0000u);
+        const float low = bf16_bits(both) * kUnits<T>, high = __uint_as_float(both & 0xFFFF0000u) * kUnits<T>;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           acc[n][0] = fmaf(low, sum[n][0], acc[n][0]);

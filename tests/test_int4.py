@@ -324,6 +324,36 @@ def test_linear_reads_the_scales_of_its_own_rows(rows, k, dtype):
 
 
 @GPU
+@pytest.mark.parametrize("group", int4.GROUPS)
+@pytest.mark.parametrize("k", [64, 200, 4050])
+@pytest.mark.parametrize("rows", [1, 8, 9, 16, 17])
+def test_linear_of_inputs_near_the_ends_of_the_type(rows, k, group):
+    """Inputs up to the largest bf16 by weights that leave the product finite, however the codes are summed before they meet their scale; and products of
+    few binary digits, which every order of sums gives exactly, down to 2^-126."""
+    held, _, _, _, w, _ = _product_case(rows, 50, k, group, torch.bfloat16, False, None, False)
+    held = int4.quantize((w * 1e-4).float(), group)
+    w = int4.dequantize(held, torch.float32).double()
+    x = torch.full((rows, k), torch.finfo(torch.bfloat16).max, dtype=torch.bfloat16, device=cuda)
+    x[:, ::3] *= -1
+    x[rows // 2:] = 3e37
+    got = int4.linear(x, held)
+    want = x.double() @ w.T
+    a = x.double().abs() @ w.abs().T
+    assert got.isfinite().all()
+    assert ((got.double() - want).abs() <= torch.finfo(torch.bfloat16).eps / 2 * want.abs() + (k / 16 + 40) * 2.0 ** -22 * a).all()
+    g = torch.Generator().manual_seed(3)
+    codes = torch.randint(-8, 8, (50, k), generator=g).float()
+    codes[:, ::32] = -8
+    held = int4.quantize(codes.to(cuda), group)      # scales of 1
+    x = torch.randint(-1, 2, (rows, k), generator=g).to(torch.bfloat16).to(cuda)
+    x[:, 16:] = 0
+    base = int4.linear(x, held)
+    assert torch.equal(base.double(), x.double() @ codes.double().to(cuda).T)
+    for e in (-100, -120, -126):
+        assert torch.equal(int4.linear(x * 2.0 ** e, held), base * 2.0 ** e)
+
+
+@GPU
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("rows,n,k,group", [(1, 16, 64, 64), (5, 37, 100, 32), (33, 300, 129, 128), (200, 130, 777, 64), (300, 520, 264, 32)])
 def test_linear_gradients(rows, n, k, group, dtype):
