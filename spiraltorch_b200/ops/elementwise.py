@@ -144,6 +144,8 @@ def embedding_forward(idx: torch.Tensor, weight: torch.Tensor, pos: Optional[tor
     global launch_count
     flat = idx.reshape(-1)
     T, d = flat.numel(), weight.shape[1]
+    if pos is not None and T and not 1 <= min(seq_len, T) <= pos.shape[0]:      # the kernel would read behind the table
+        raise ValueError(f"embedding_forward: sequences of {seq_len} tokens, learned positions for {pos.shape[0]}")
     if not native.use_native(weight):
         local = flat - vocab_start
         ok = (local >= 0) & (local < weight.shape[0])

@@ -433,3 +433,22 @@ def test_gradients_are_not_differentiated_twice():
     assert torch.equal(g, torch.autograd.grad(scoring.token_scores(x, t).logprob.sum(), x)[0])
     with pytest.raises(RuntimeError, match="twice"):
         torch.autograd.grad(g.pow(2).sum(), x)
+
+
+def _check_longer_than_learned_positions(device, dtype):
+    from spiraltorch_b200.models.gpt import GPTConfig, GPTModel
+    model = GPTModel(GPTConfig(vocab_size=96, d_model=128, n_layers=1, n_heads=2, ffn=256, seq_len=16, norm="layer", positional="learned"), device=device, dtype=dtype)
+    tokens = torch.zeros(2, 17, dtype=torch.int64, device=device)
+    for call in (lambda: model.score(tokens), lambda: model(tokens), lambda: model(tokens, tokens), lambda: model.forward_backward(tokens, tokens)):
+        with pytest.raises(ValueError, match="learned positions for 16"):
+            call()
+    assert model.score(tokens[:, :16]).logprob.isfinite().all()
+
+
+def test_sequences_longer_than_the_learned_positions():
+    _check_longer_than_learned_positions("cpu", torch.float32)
+
+
+@GPU
+def test_sequences_longer_than_the_learned_positions_on_the_gpu():
+    _check_longer_than_learned_positions("cuda", torch.bfloat16)
