@@ -248,23 +248,33 @@ def _input_gradient(dy2, w):
     return dx
 
 
+def _version(w: Weights) -> tuple:
+    return w.codes._version, w.scales._version
+
+
+def _check_version(w: Weights, version: tuple) -> None:
+    if _version(w) != version:
+        raise RuntimeError("int4.linear: weights needed for a gradient have been modified by an inplace operation: they were quantised anew")
+
+
 class _InputGradientFn(torch.autograd.Function):
     """``dy W`` where a graph of the gradient is asked for: linear in ``dy`` as the product is in ``x``."""
 
     @staticmethod
     def forward(ctx, dy2, w):
-        ctx.w = w
+        ctx.w, ctx.version = w, _version(w)
         return _input_gradient(dy2, w)
 
     @staticmethod
     def backward(ctx, d):
+        _check_version(ctx.w, ctx.version)
         return linear(d, ctx.w), None
 
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, bias, residual, w):
-        ctx.w, ctx.version = w, w.codes._version
+        ctx.w, ctx.version = w, _version(w)
         if x.dim() == 2:
             return _product(x, w, bias, None, residual)
         y = _product(x.reshape(-1, x.shape[-1]), w, bias, None, None if residual is None else residual.reshape(-1, w.out_features))
@@ -274,8 +284,7 @@ class _LinearFn(torch.autograd.Function):
     def backward(ctx, dy):
         need_x, need_bias, need_residual, _ = ctx.needs_input_grad
         w, dx, db = ctx.w, None, None
-        if w.codes._version != ctx.version:
-            raise RuntimeError("int4.linear: weights needed for a gradient have been modified by an inplace operation: they were quantised anew")
+        _check_version(w, ctx.version)
         dy2 = dy if dy.dim() == 2 else dy.reshape(-1, w.out_features)
         if need_x:
             dx = _InputGradientFn.apply(dy2, w) if torch.is_grad_enabled() and dy.requires_grad else _input_gradient(dy2, w)

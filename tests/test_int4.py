@@ -153,6 +153,23 @@ def test_weights_quantised_anew_are_no_gradient_of_the_old():
         y.sum().backward()
 
 
+def test_weights_quantised_anew_are_no_second_derivative_of_the_old():
+    held = int4.quantize(_matrix(7, 45, torch.float32), 32)
+    w = int4.dequantize(held, torch.float32)
+    x, dy = torch.randn(3, 45, requires_grad=True), torch.randn(3, 7, requires_grad=True)
+    dx = torch.autograd.grad(int4.linear(x, held), x, dy, create_graph=True)[0]
+    again = torch.autograd.grad(dx.sum(), dy, retain_graph=True)[0]
+    assert torch.allclose(again, torch.ones(3, 45) @ w.T, atol=1e-5)
+    int4.quantize(_matrix(7, 45, torch.float32, 1), 32, out=held)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(dx.sum(), dy)
+    # other scales alone are other weights too
+    y = int4.linear(x, held)
+    held.scales.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 def test_weights_are_copied_saved_and_not_changed(tmp_path):
     import copy
     held = int4.quantize(_matrix(20, 70, torch.float32), 32)
