@@ -15,6 +15,7 @@ CPU tensors use a plain PyTorch statement of the same (also the test oracle).  T
 from __future__ import annotations
 
 import struct
+from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -65,8 +66,11 @@ class Weights:
         if group not in GROUPS or not (0 < out_features <= 1 << 30 and 0 < in_features <= 1 << 30):
             raise ValueError(f"int4: a matrix of {out_features} x {in_features} in groups of {group} is not supported")
         down = -(-out_features // 16)
-        codes = torch.empty((down, -(-in_features // 64), 512), dtype=torch.uint8, device=device)
-        return cls.__new__(cls)._set(codes, codes.new_empty((down, -(-in_features // group), 16), dtype=torch.bfloat16), out_features, in_features, group)
+        # tensors of inference mode could not be written to outside it, nor be looked at for updates by a gradient
+        with torch.inference_mode(False) if torch.is_inference_mode_enabled() else nullcontext():
+            codes = torch.empty((down, -(-in_features // 64), 512), dtype=torch.uint8, device=device)
+            scales = codes.new_empty((down, -(-in_features // group), 16), dtype=torch.bfloat16)
+        return cls.__new__(cls)._set(codes, scales, out_features, in_features, group)
 
     def __reduce__(self):
         return Weights, tuple(getattr(self, name) for name in self.__slots__)
@@ -76,7 +80,8 @@ class Weights:
         return self.codes.nbytes + self.scales.nbytes
 
     def to(self, device) -> "Weights":
-        return Weights(self.codes.to(device), self.scales.to(device), self.out_features, self.in_features, self.group)
+        with torch.inference_mode(False) if torch.is_inference_mode_enabled() else nullcontext():
+            return Weights(self.codes.to(device), self.scales.to(device), self.out_features, self.in_features, self.group)
 
 
 # ---- plain statement ------------------------------------------------------------------------------------------------------------
@@ -322,6 +327,8 @@ def linear(x: torch.Tensor, w: Weights, bias: Optional[torch.Tensor] = None, *, 
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad) or (residual is not None and residual.requires_grad)):
         if act is not None:
             raise ValueError("int4.linear: act with tensors that require gradients; apply it to the result")
+        if w.codes.is_inference() or w.scales.is_inference():
+            raise ValueError("int4.linear: tensors that require gradients by weights whose memory was made in inference mode")
         return _LinearFn.apply(x, bias, residual, w)
     if len(shape) == 2:
         return _product(x, w, bias, act, residual)

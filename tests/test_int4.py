@@ -170,6 +170,42 @@ def test_weights_quantised_anew_are_no_second_derivative_of_the_old():
         y.sum().backward()
 
 
+def _check_weights_of_inference_mode(device, dtype):
+    w, x = _matrix(7, 45, dtype, device=device), _matrix(3, 45, dtype, 1, device).requires_grad_(True)
+    want = int4.linear(x, int4.quantize(w, 32))
+    with torch.inference_mode():
+        held = int4.quantize(w, 32)
+        moved = held.to(device)
+        assert torch.equal(int4.linear(x, held), want)
+    for h in (held, moved):
+        y = int4.linear(x, h)
+        assert torch.equal(y, want)
+        assert torch.equal(torch.autograd.grad(y.sum(), x)[0], torch.autograd.grad(int4.linear(x, int4.quantize(w, 32)).sum(), x)[0])
+    y = int4.linear(x, held)
+    int4.quantize(w * 2, 32, out=held)
+    assert torch.equal(int4.dequantize(held, dtype), 2 * int4.dequantize(int4.quantize(w, 32), dtype))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    y = int4.linear(x, held)
+    with torch.inference_mode():
+        int4.quantize(w, 32, out=held)
+        parts = int4.Weights(held.codes.clone(), held.scales.clone(), 7, 45, 32)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    assert torch.equal(int4.linear(x.detach(), parts), want)
+    with pytest.raises(ValueError, match="inference mode"):
+        int4.linear(x, parts)
+
+
+def test_weights_of_inference_mode():
+    _check_weights_of_inference_mode("cpu", torch.float32)
+
+
+@GPU
+def test_weights_of_inference_mode_on_the_gpu():
+    _check_weights_of_inference_mode("cuda", torch.bfloat16)
+
+
 def test_weights_are_copied_saved_and_not_changed(tmp_path):
     import copy
     held = int4.quantize(_matrix(20, 70, torch.float32), 32)
