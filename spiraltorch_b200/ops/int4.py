@@ -128,10 +128,16 @@ def dequantize_reference(w: Weights, dtype: torch.dtype = torch.float32) -> torc
     return (_untile(w.codes, w.out_features, w.in_features).to(s.dtype) * s).to(dtype)
 
 
+def _matmul(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
+    """In their type, under autocast too."""
+    with torch.autocast(a.device.type, enabled=False):
+        return a @ b
+
+
 def linear_reference(x, weight, bias=None, act=None, residual=None):
     """``weight`` ``[out, in]``: sums in fp32 (fp64 for fp64 ``x``), rounded once."""
     t = torch.float64 if x.dtype == torch.float64 else torch.float32
-    y = x.to(t) @ weight.to(t).T
+    y = _matmul(x.to(t), weight.to(t).T)
     if bias is not None:
         y = y + bias.to(t)
     y = torch.relu(y) if act == "relu" else gelu_tanh(y) if act == "gelu" else y
@@ -237,7 +243,7 @@ def _input_gradient(dy2, w):
     global launch_count
     if not dy2.is_cuda:
         t = torch.float64 if dy2.dtype == torch.float64 else torch.float32
-        return (dy2.to(t) @ dequantize_reference(w, t)).to(dy2.dtype)
+        return _matmul(dy2.to(t), dequantize_reference(w, t)).to(dy2.dtype)
     dy2 = _boundaries(dy2)
     index = native.require_cuda("int4.linear", dy2, w.codes, w.scales)
     rows, k = dy2.shape[0], w.in_features

@@ -126,6 +126,21 @@ def test_linear_statement_and_gradients():
         assert int4.linear(x[0, 0], held).shape == (7,) and int4.linear(x[:0], held).shape == (0, 3, 7)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_linear_statement_under_autocast(dtype):
+    """Sums stay in fp32, as the kernels' do."""
+    held = int4.quantize(_matrix(7, 45, torch.float32), 32)
+    x, b, dy = _matrix(3, 45, dtype, 1).requires_grad_(True), _matrix(1, 7, dtype, 2)[0], _matrix(3, 7, dtype, 3)
+    want = int4.linear(x, held, b)
+    dx = torch.autograd.grad(want, x, dy)[0]
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        y = int4.linear(x, held, b)
+        assert torch.equal(y, want) and y.dtype == dtype
+        assert torch.equal(torch.autograd.grad(y, x, dy)[0], dx)
+        with torch.no_grad():
+            assert torch.equal(int4.linear(x, held, b), want)
+
+
 def test_refusals():
     w = _matrix(20, 70, torch.float32)
     held = int4.quantize(w, 32)
