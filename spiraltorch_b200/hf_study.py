@@ -321,7 +321,8 @@ def run_study(plan: Mapping[str, object], runner: Optional[Callable[[Mapping[str
 # LoRA on torch modules
 class FrozenLinear4(torch.nn.Module):
     """A frozen ``nn.Linear`` or GPT-2 ``Conv1D`` with its weight in four bits (:mod:`spiraltorch_b200.ops.int4`): a quarter of the memory of 16 bits, and
-    a gradient for its input.  On a GPU for bf16 and fp16 activations."""
+    a gradient for its input.  On a GPU fp32 activations (and the bias beside them) are rounded to bf16 for the product, which keeps their range; its result is fp32 again.
+    Under autocast the layer computes and answers in autocast's type, as ``nn.Linear`` does."""
 
     def __init__(self, base: torch.nn.Module, group: int = 64):
         super().__init__()
@@ -336,7 +337,11 @@ class FrozenLinear4(torch.nn.Module):
         return int4.Weights(self.codes, self.scales.view(torch.bfloat16), self.out_features, self.in_features, self.group)
 
     def forward(self, x):
-        return int4.linear(x, self.held(), self.bias)
+        kind, out = x.device.type, x.dtype
+        if out != torch.float64 and torch.is_autocast_enabled(kind):
+            out = torch.get_autocast_dtype(kind)
+        t = torch.bfloat16 if x.is_cuda and out == torch.float32 else out
+        return int4.linear(x.to(t), self.held(), None if self.bias is None else self.bias.to(t)).to(out)
 
 
 class LoraWrapped(torch.nn.Module):

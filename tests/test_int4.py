@@ -625,3 +625,55 @@ def test_frozen_layers_in_four_bits_on_the_gpu():
     assert ((dx.double() - want).abs().view(60, 200) <= _allowed(dy.double().view(60, 136), w.T, want.view(60, 200), torch.bfloat16)).all()
     wrapped(x).sum().backward()
     assert wrapped.lora_b.grad.isfinite().all() and x.grad.isfinite().all()
+
+
+def _check_frozen_layer_under_autocast(device, dtype):
+    from spiraltorch_b200 import hf_study as H
+    torch.manual_seed(0)
+    layer = torch.nn.Linear(45, 24).to(device)
+    frozen = H.FrozenLinear4(layer, 32)
+    for x in (torch.randn(3, 45, device=device), torch.randn(3, 45, device=device, dtype=dtype)):
+        with torch.autocast(device, dtype=dtype):
+            y = frozen(x.requires_grad_())
+            assert y.dtype == layer(x).dtype == dtype
+        assert torch.equal(y, int4.linear(x.to(dtype), frozen.held(), layer.bias.to(dtype)))
+        assert torch.autograd.grad(y.sum(), x)[0].dtype == x.dtype
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_frozen_layers_in_four_bits_under_autocast(dtype):
+    _check_frozen_layer_under_autocast("cpu", dtype)
+
+
+@GPU
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_frozen_layers_in_four_bits_under_autocast_on_the_gpu(dtype):
+    _check_frozen_layer_under_autocast("cuda", dtype)
+
+
+@GPU
+@pytest.mark.parametrize("rows", [5, 40])
+def test_frozen_layers_in_four_bits_of_fp32_models_on_the_gpu(rows):
+    """The product of the rounded activations, within its tolerance; their gradient, that of the rounded output's."""
+    from spiraltorch_b200 import hf_study as H
+    torch.manual_seed(0)
+    layer = torch.nn.Linear(200, 136).to(cuda)
+    frozen = H.FrozenLinear4(layer)
+    w = int4.dequantize(frozen.held(), torch.float32).double()
+    x = torch.randn(rows, 200, device=cuda, requires_grad=True)
+    y = frozen(x)
+    xb = x.detach().bfloat16().double()
+    want = xb @ w.T + layer.bias.detach().bfloat16().double()
+    assert y.dtype == torch.float32 and ((y.double() - want).abs() <= _allowed(xb, w, want, torch.bfloat16)).all()
+    dy = torch.randn_like(y)
+    dx = torch.autograd.grad(y, x, dy)[0]
+    db = dy.bfloat16().double()
+    assert dx.dtype == torch.float32 and ((dx.double() - db @ w).abs() <= _allowed(db, w.T, db @ w, torch.bfloat16)).all()
+
+
+@GPU
+def test_a_study_run_with_frozen_layers_in_four_bits_on_the_gpu(tmp_path):
+    from spiraltorch_b200 import hf_study as H
+    out = H.lora_finetune_run({"steps": 2, "batch_size": 2, "seq_len": 16, "model": {"d_model": 32, "n_layer": 1, "n_head": 2}, "eval_batches": 1, "pretrain_steps": 1,
+                               "base_bits": 4, "device": "cuda"}, tmp_path)
+    assert out["steps"] == 2 and math.isfinite(out["eval_loss_after"])
