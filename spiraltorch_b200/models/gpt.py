@@ -403,11 +403,11 @@ class GPTModel(nn.Module):
         return GPTDecoder(self, sequences, max_length, pages=pages, page_size=page_size, weight_bits=weight_bits, head_bits=head_bits, group=group)
 
     def generate(self, prompts, max_new_tokens: int, *, stop: Optional[int] = None, page_size: int = 64, scores: Optional[int] = None, weight_bits: int = 16,
-                 head_bits: int = 16) -> list:
+                 head_bits: int = 16, group: int = 64) -> list:
         """The likeliest continuation of each prompt (a list of token ids), token by token, up to ``max_new_tokens`` or the token ``stop``.
-        Returns the new tokens of each; with ``scores`` (0 to 32 alternatives) their scores too, as ``GPTDecoder.generate`` does."""
+        Returns the new tokens of each; with ``scores`` (0 to 32 alternatives) their scores too, as ``GPTDecoder.generate`` does.  Weights as for :meth:`decoder`."""
         longest = max((len(p) for p in prompts), default=0) + max(max_new_tokens - 1, 0)      # the last new token is not appended
-        decoder = self.decoder(len(prompts), longest, page_size=page_size, weight_bits=weight_bits, head_bits=head_bits)
+        decoder = self.decoder(len(prompts), longest, page_size=page_size, weight_bits=weight_bits, head_bits=head_bits, group=group)
         return decoder.generate(prompts, max_new_tokens, stop=stop, scores=scores)
 
     @torch.no_grad()

@@ -543,6 +543,18 @@ def test_generate_with_four_bit_weights():
     assert model.generate([[1, 2, 3], [9]], 5, weight_bits=4) == _with_quantised(_small_model(), False).generate([[1, 2, 3], [9]], 5)
 
 
+def test_generate_with_groups_of_another_size():
+    model, prompts = _small_model(), [[1, 2, 3], [9]]
+    for group in (32, 128):
+        d = model.decoder(2, 16, weight_bits=4, head_bits=4, group=group)
+        assert all(w.group == group for w in d.weights.values())
+        tokens, scores = model.generate(prompts, 5, weight_bits=4, head_bits=4, group=group, scores=0)
+        want, judged = d.generate(prompts, 5, scores=0)
+        assert tokens == want and [s.logprob for s in scores] == [s.logprob for s in judged]
+    with pytest.raises(ValueError, match="groups"):
+        model.generate(prompts, 2, weight_bits=4, group=48)
+
+
 def test_frozen_layers_in_four_bits_train_their_adapters():
     from spiraltorch_b200 import hf_study as H
     torch.manual_seed(0)
