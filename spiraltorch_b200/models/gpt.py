@@ -416,8 +416,10 @@ class GPTModel(nn.Module):
         A token below 0 is padding: it has log probability 0 and the model reads token 0 in its place."""
         if self.tp.world != 1:
             raise ValueError("GPTModel.score: tensor-parallel models are not supported")
-        if tokens.dim() != 2 or tokens.shape[1] < 2 or tokens.dtype != torch.int64:
-            raise ValueError(f"GPTModel.score: int64 tokens [B, S] with two positions at least, got {tokens.dtype} {tuple(tokens.shape)}")
+        if tokens.dim() != 2 or tokens.shape[0] < 1 or tokens.shape[1] < 2 or tokens.dtype != torch.int64:
+            raise ValueError(f"GPTModel.score: int64 tokens [B, S] with a sequence and two positions at least, got {tokens.dtype} {tuple(tokens.shape)}")
+        if not 0 <= top <= min(scoring.MOST_TOP, self.cfg.vocab_size):      # before the model runs
+            raise ValueError(f"GPTModel.score: top must be 0 to {min(scoring.MOST_TOP, self.cfg.vocab_size)}, got {top}")
         logits, _ = self._forward(tokens.clamp(min=0), None, 1.0, keep=False)
         # the last position of a sequence has no token behind it
         targets = torch.cat([tokens[:, 1:], tokens.new_full((tokens.shape[0], 1), loss_ops.IGNORE_INDEX)], 1)

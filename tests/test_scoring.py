@@ -401,6 +401,13 @@ def test_scores_of_a_model():
         model.score(torch.zeros(5, dtype=torch.int64))
 
 
+def test_scores_of_no_sequence_are_refused():
+    with pytest.raises(ValueError, match="with a sequence"):
+        _model().score(torch.zeros(0, 5, dtype=torch.int64))
+    with pytest.raises(ValueError, match="top must be 0 to 32"):
+        _model().score(torch.zeros(1, 5, dtype=torch.int64), top=33)
+
+
 def test_generated_tokens_with_scores():
     model = _model()
     prompts = [[1, 2, 3], [7], list(range(30))]
