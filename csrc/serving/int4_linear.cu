@@ -90,20 +90,17 @@ struct Slice {
     const uint8_t* from = codes + static_cast<long long>(c0) * kTileBytes + lane * 16;
     const int g0 = c0 * 64 / GROUP;
     const uint32_t* words = reinterpret_cast<const uint32_t*>(scales) + g0 * 8 + lane;
-    if (c0 + C <= chunks) {
+    // groups of 32: the last chunk may have one, and what follows in memory are the next tile row's
+    if (c0 + C <= chunks && (GROUP > 32 || g0 + kScales <= groups)) {
 #pragma unroll
       for (int i = 0; i < C; ++i) w[i] = *reinterpret_cast<const uint4*>(from + i * kTileBytes);
-    } else {
-#pragma unroll
-      for (int i = 0; i < C; ++i)
-        if (c0 + i < chunks) w[i] = *reinterpret_cast<const uint4*>(from + i * kTileBytes);
-    }
-    // apart from the codes: of groups of 32 the last chunk may have one, and what follows in memory are the next tile row's
-    if (g0 + kScales <= groups) {
 #pragma unroll
       for (int i = 0; i < kWords; ++i)
         if (kScales * 8 % 32 == 0 || i * 32 + lane < kScales * 8) s[i] = words[i * 32];
     } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i)
+        if (c0 + i < chunks) w[i] = *reinterpret_cast<const uint4*>(from + i * kTileBytes);
 #pragma unroll
       for (int i = 0; i < kWords; ++i) s[i] = i * 32 + lane < min(kScales, groups - g0) * 8 ? words[i * 32] : 0u;
     }
