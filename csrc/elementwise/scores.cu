@@ -1,6 +1,6 @@
 // Scores of given tokens: log probability, entropy of the distribution and the likeliest tokens, from logits in one pass, and the gradient.
 //
-//   m = max x,  y = (x - m) log2 e,  S = sum 2^y,  T = sum 2^y y,  log p_j = (y_j - log2 S) ln 2,  entropy = (log2 S - T / S) ln 2
+//   m = max x,  y = (x - m) log2 e,  S = sum 2^y,  T = sum 2^y y,  log p_j = x_j - m - ln S,  entropy = (log2 S - T / S) ln 2
 //   dx_j = sum_i g_i [j = id_i] - p_j (sum_i g_i + g_entropy (log p_j + entropy)),  i over the given token and the likeliest ones
 //
 // Bound by memory: a row is read once (forward; the gradient reads it again and writes as much).  Every thread keeps m, S and T of what it has seen, and what
@@ -482,10 +482,7 @@ __global__ void __launch_bounds__(W == 1 ? kThreads : W * 32, W == 1 ? 1 : 32 / 
   // an empty row, all -inf: no probability anywhere
   const bool empty = s.S == 0.0f;
   const float log_S = empty ? INFINITY : log2f(s.S), m = empty ? 0.0f : s.m;
-  const auto log_p = [&](float v) {
-    const float d = v - m;      // d log2 e may be infinite where d is not
-    return fabsf(d) < kUsual ? (d * kLog2e - log_S) * kLn2 : d - log_S * kLn2;
-  };
+  const auto log_p = [&](float v) { return fmaf(-log_S, kLn2, v - m); };
   if (tid == 0) {
     logprob[row] = target >= 0 && target < p.vocab ? log_p(given) : 0.0f;
     entropy[row] = empty ? 0.0f : (log_S - s.T / s.S) * kLn2;

@@ -226,6 +226,19 @@ def test_kernel_and_gradient_on_huge_rows(vocab, dtype):
 
 @GPU
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [7, 300, 5001, 50304])
+@pytest.mark.parametrize("scale", [30.0, 1000.0, 1e5])
+def test_kernel_on_logits_far_apart(scale, vocab, dtype):
+    """Log probabilities of thousands: as near as their difference from the largest logit allows."""
+    if dtype == torch.float16 and scale > 1000:
+        scale = 1e4
+    x, t = _logits(400 if vocab < 50304 else 40, vocab, dtype, 3, scale)
+    top = min(32, vocab)
+    _check(scoring.token_scores(x.to(cuda), t.to(cuda), top=top), x, t, top)
+
+
+@GPU
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("vocab", [9, 300, 5000, 40000, 70001, 263000])
 def test_kernel_non_finite(vocab, dtype):
     x, t = _logits(8, vocab, dtype, 3)
