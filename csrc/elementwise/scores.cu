@@ -6,7 +6,8 @@
 // Bound by memory: a row is read once (forward; the gradient reads it again and writes as much).  Every thread keeps m, S and T of what it has seen, and what
 // its largest element is; they are joined at the end.  Of the threads' largest elements the `top` best give a bound, which only elements of these threads can
 // reach: those are read again (25 vectors each of a row of 50304, out of L2) and what reaches the bound is ranked.
-// Measured: 8192 x 50304 in bf16 139 to 141 us, 5.9 TB/s of the 6.6 that a copy reaches; with 20 alternatives 198 to 201, 4.2; forward and gradient 395, the gradient 256 of it (6.4).
+// Measured: 8192 x 50304 in bf16 139 to 141 us, 5.9 TB/s of the 6.6 that a copy reaches; with 20 alternatives 198 to 201, 4.2; forward and gradient 395, the gradient 256 of it (6.4).  In fp16
+// 139, 195 and 394; in fp32 242 (6.8 TB/s), 315 and 744.
 // At 2048 x 50304 the XU pipe, whose exponentials come next, is busy 70%, and the alternatives are 30% of the instructions.
 #include "../common/host.h"
 #include "../common/ptx.cuh"
@@ -501,6 +502,7 @@ struct GradParams {
   int vocab, top, parts;
 };
 
+// Probabilities below 2^-126 count as 0, as their exponentials are: what that leaves out of an element is below 10^-35 of the row's gradients.
 // Blocks share a row in `parts` pieces of whole vectors; WIDE: rows of logits and gradient are at the same place between 16-byte boundaries.
 template <typename T, int W, bool WIDE>
 __global__ void __launch_bounds__(kThreads) scores_grad_kernel(const T* logits, const long long* targets, const float2* stats, const float* entropy,
@@ -597,7 +599,10 @@ int parts_of(long long rows, int vocab) {
   return parts;
 }
 
-constexpr int kWarpRow = 2048;      // rows of up to as many elements go to a warp each
+// Rows of up to as many elements go to a warp each, longer ones to 8 (or 4, below).  us by 8 warps and by one, with 5 alternatives: 1 x 1024 6.2 and 5.5, 1 x 2048 5.5 and 6.3, 1 x 4096 5.7
+// and 7.9; 8192 x 2048 70 and 28, 8192 x 4096 75 and 38, 8192 x 8192 83 and 57; without, 8192 x 2048 21 and 17, 8192 x 3000 23 and 24; the gradient of 1 x 1024 4.0 and 3.8, of 1 x 2048 4.0
+// and 4.5, of 8192 x 2048 45 and 16, of 8192 x 8192 66 and 50.  One row has its border between 1024 and 2048, many have theirs beyond 8192, where the one would lose half its time again.
+constexpr int kWarpRow = 2048;
 
 template <typename T, int W, bool TOP>
 int forward(const void* logits, const long long* targets, float* logprob, float* entropy, float2* stats, long long* top_ids, float* top_logprobs, ScoreParams p,
@@ -619,7 +624,8 @@ int forward(const void* logits, const long long* targets, float* logprob, float*
     return p.top ? forward<T, 1, true>(logits, targets, logprob, entropy, stats, top_ids, top_logprobs, p, stream)
                  : forward<T, 1, false>(logits, targets, logprob, entropy, stats, top_ids, top_logprobs, p, stream);
   if (p.top) return forward<T, kWarps, true>(logits, targets, logprob, entropy, stats, top_ids, top_logprobs, p, stream);
-  // 4 warps to a row where there are rows for many turns of the SMs: 8192 x 50304 141 us, 149 with 8 (with alternatives 211 and 200); 300 x 50304 13.1 and 11.4, 1 row 6.0 and 5.1
+  // 4 warps to a row from 16 rows an SM (2368) on, where the SMs have many turns.  us with 8 and with 4: 4096 elements, 300 rows 4.4 and 4.4, 1200 9.0 and 7.1, 8192 41 and 26; 16384, 300 6.1 and 7.0,
+  // 1200 14.6 and 14.1, 8192 68 and 57; 50304, 300 11.9 and 14.1, 1776 42 and 46, 2368 52 and 51, 8192 147 and 140; 131072, 1776 87 and 99, 3000 135 and 139.  With alternatives 8192 x 50304 200 and 211.
   return p.rows >= 16 * st::sm_count() ? forward<T, 4, false>(logits, targets, logprob, entropy, stats, top_ids, top_logprobs, p, stream)
                                       : forward<T, kWarps, false>(logits, targets, logprob, entropy, stats, top_ids, top_logprobs, p, stream);
 }

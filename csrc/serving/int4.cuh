@@ -42,7 +42,7 @@ __device__ __forceinline__ uint32_t pick(uint32_t word, uint32_t mask, uint32_t 
   return d;
 }
 
-// Nibbles e and e + 4 of a word as two numbers of -8 to 7 units, exactly: the nibble is put into the low bits of 128 (bf16) or 1024 (fp16) units, where a unit is 1, and
+// Nibbles e and e + 4 of a word as two numbers of -8 to 7 units, exactly (the published method of mixed-precision kernels): the nibble is put into the low bits of 128 (bf16) or 1024 (fp16) units, where a unit is 1, and
 // 136 or 1032 of them are subtracted.  A unit is 1 in fp16 and 2^-10 in bf16: the products with a group of 128 inputs then sum up to no more than the largest of them, so that no
 // finite bf16 overflows before the scale is known.  They stay whole multiples of 2^-143, which fp32 holds.
 template <typename T> constexpr float kUnits = 1.0f;      // in 1

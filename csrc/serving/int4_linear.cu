@@ -1,9 +1,10 @@
 // Products with weights of four bits:  y = act(x W^T + bias) + residual,  W = q s  (int4.cuh): few rows here, by matrix instructions on codes converted in registers.
 //
-// Bound by the codes' bytes where there are enough of them, and by instructions before that: a shift, a selection and a subtraction turn two codes into numbers, two thirds of what
-// a warp does.  tcgen05 needs the same and a way through tensor memory (int4_wide.cu); is_wide says where it pays.
-// Measured, one row in bf16: 2048 inputs to 50304 outputs in groups of 128 17.1 to 17.4 us, 3.1 TB/s, 59% of the issue slots; in groups of 64 2048 to 2048 3.5, 2048 to 8192 5.7,
-// 8192 to 2048 7.3.
+// At a floor of the codes' bytes no single thing bounds it: one row, 2048 inputs to 50304 outputs in groups of 128, takes 17.1 to 17.7 us in bf16, 3.1 TB/s.  60% of the issue slots are
+// taken, and of what keeps a warp from issuing, waiting for memory is the most (1.9 warps an issue; instructions before 1.6, the ALU pipe 1.1, barriers 0.7).  A
+// slice of 16 rows by 256 columns takes 378 instructions of a warp, half of which turn codes into numbers (a shift, a selection and a subtraction for two).  444 blocks take 3144 tile rows in 8
+// turns where 7.08 would do, and a store of partial sums meets three bank conflicts.  In groups of 64 2048 to 2048 takes 3.5 us, 2048 to 8192 5.6 to 6.0, 8192 to 2048 7.3.
+// tcgen05 needs the same instructions and a way through tensor memory (int4_wide.cu); is_wide says where it pays.
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "../common/chain.cuh"
@@ -303,8 +304,11 @@ int dispatch(const LinearParams& p, cudaStream_t stream) {
   return p.chunks <= 2 * kWarps ? by_group<T, 2, 2>(p, stream) : by_group<T, 2, 4>(p, stream);
 }
 
-// Whether products go through tcgen05 (int4_wide.cu): from 17 tokens on, and from 9 where the weights are more than 2^24.  us of this kernel and that one, 16 tokens: 2048 x 2048
-// 4.9 and 6.1, 8192 x 2048 8.8 and 9.1, 50304 x 2048 25.8 and 19.8; 8 tokens 3.6 and 5.9, 6.2 and 9.0, 19.8 and 19.7.
+// Whether products go through tcgen05 (int4_wide.cu): from 17 tokens on, and from 9 where the weights are more than 2^24.  us of this kernel and that one (outputs x inputs), 9 and 16 tokens:
+//   2048 x 2048 5.3 / 7.0, 6.4 / 7.3     8192 x 2048 8.1 / 9.5, 9.4 / 9.5     2048 x 8192 9.4 / 9.2, 10.9 / 9.6     4096 x 4096 9.5 / 8.7, 11.2 / 9.0
+//   12288 x 2048 10.1 / 9.7, 11.4 / 9.8  6144 x 4096 12.0 / 10.6, 14.0 / 11.0  8192 x 8192 23.0 / 15.7, 25.5 / 16.2  50304 x 2048 23.6 / 19.8, 25.6 / 20.1
+// 2^24 weights (second to fourth) are even, all larger ones gain.  At 8 tokens tcgen05 is even from there to 2^25 (8192 x 2048 7.7 / 9.5, 4096 x 4096 9.1 / 8.7, 50304 x 2048 20.1 / 19.8) and gains
+// by deep matrices beyond (8192 x 8192 18.7 / 15.5, 18944 x 4096 20.0 / 15.1): those are left here.
 bool is_wide(int tokens, int rows, int cols) { return tokens > 16 || (tokens > 8 && static_cast<long long>(rows) * cols > 1 << 24); }
 
 int aligned(const void* x, long long row, int cols) {

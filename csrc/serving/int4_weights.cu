@@ -10,7 +10,8 @@
 //
 // A warp takes 16 rows by 128 columns, which holds whole groups of every size: its loads are all in flight together, extrema are joined by
 // shuffles, and 1 KB of shared memory turns the codes from rows to the order of int4.cuh.
-// Measured: 8192 x 8192 in bf16 44 us quantised, 3.9 TB/s of the 6.6 that a copy reaches: instructions bound it (the ALU pipe busy 76%); 31 us read back, 5.5 TB/s.
+// Measured: 8192 x 8192 in bf16 43 to 44 us quantised, 3.9 TB/s of the 6.6 that a copy reaches: instructions bound it (the ALU pipe busy 76%); 30 to 31 us read back, 5.6 TB/s.  In fp16 41
+// and 30, in fp32 83 and 52 us (3.7 and 5.8 TB/s).
 #include "../common/host.h"
 #include "../common/chain.cuh"
 #include "int4.cuh"

@@ -7,7 +7,8 @@
 //
 // Bound by the products where rows are many: 4096 rows, 2048 inputs to 8192 outputs, 98 to 103 us in two runs, 1337 to 1398 TFLOP/s of the 1678 that a library's product reaches in
 // bursts, the tensor pipe busy 78%; the gradient 106 to 112, 72%.  777 rows, 2048 to 6144, 21 us: two rounds of tiles.  64 rows, 8192 to 2048, 11 to 12.  Few rows are bound by
-// conversion: at 32 rows, 8192 to 18944, a team converts a step in 1250 cycles and stores it in 250, three teams at a time, and a product is issued every 600.
+// conversion: 32 rows, 8192 to 18944, take 26 us (the codes' bytes alone 13), which leaves some 720 cycles for each of a block's 64 steps; a team converts a step in 1250 cycles and stores it
+// in 250, three teams at a time.  50304 x 2048 by 16, 32 and 64 rows 19.8, 20.5 and 22.5 us.  The gradient of one row to 64: 7.0 to 8.7 us at 2048 x 2048, 9.8 to 11.5 with four times the weights.
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "../common/chain.cuh"
